@@ -6,11 +6,14 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <climits>
 #include <string>
 #include <vector>
 
 #include "comm.h"
 #include "gemm.h"
+#include "kv_fp8.h"
 #include "layers.h"
 #include "moe.h"
 
@@ -214,6 +217,163 @@ int64_t decode_attention_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t max_ct
 
 int64_t decode_workspace_floats(int64_t B, int64_t Hq, int64_t max_ctx) {
   return B * Hq * cx::decode_attention_splits((int)max_ctx) * 130;
+}
+
+// ---- 8-bit paged KV cache ----------------------------------------------------
+int sms_of(const at::Tensor& t) { return at::cuda::getDeviceProperties(t.get_device())->multiProcessorCount; }
+
+void check_same_device(const at::Tensor& a, std::initializer_list<const at::Tensor*> others, const char* what) {
+  for (const auto* t : others)
+    TORCH_CHECK(t->device() == a.device(), what, ": every tensor must be on ", a.device());
+}
+
+// rows of 16-byte vectors: [rows, cols] bf16 with contiguous rows
+int row_ld16(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && t.scalar_type() == at::kBFloat16, what,
+              " must be bf16 [rows, columns] with contiguous rows");
+  const int64_t ld = t.size(0) > 1 ? t.stride(0) : t.size(1);
+  TORCH_CHECK(ld >= t.size(1) && ld % 8 == 0 && ld <= INT_MAX && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
+              what, ": rows must start on 16-byte boundaries and not overlap");
+  return (int)ld;
+}
+
+cx::KvFp8 fp8_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs,
+                    const char* what) {
+  check_same_device(k, {&v, &ks, &vs}, what);
+  TORCH_CHECK(k.dim() == 4 && k.size(2) == 16 && k.size(3) == 128 && k.size(1) > 0 && k.is_contiguous() &&
+                  v.is_contiguous() && v.sizes() == k.sizes() && k.scalar_type() == at::kFloat8_e4m3fn &&
+                  v.scalar_type() == at::kFloat8_e4m3fn,
+              what, ": caches must be contiguous float8_e4m3fn [blocks, Hkv, 16, 128]");
+  for (const auto* t : {&ks, &vs})
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 2 && t->size(0) == k.size(0) &&
+                    t->size(1) == k.size(1),
+                what, ": scales must be contiguous fp32 [blocks, Hkv]");
+  TORCH_CHECK(k.size(0) <= INT_MAX && ((reinterpret_cast<uintptr_t>(k.data_ptr()) |
+                                        reinterpret_cast<uintptr_t>(v.data_ptr())) & 15) == 0,
+              what, ": caches must start on a 16-byte boundary");
+  return cx::KvFp8{static_cast<uint8_t*>(k.data_ptr()), static_cast<uint8_t*>(v.data_ptr()), ks.data_ptr<float>(),
+                   vs.data_ptr<float>(), (int)k.size(0), (int)k.size(1)};
+}
+
+void rope_cache_fp8(const at::Tensor& qkv, const at::Tensor& pos, const at::Tensor& cos_sin, const at::Tensor& slots,
+                    const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
+                    at::Tensor& out, int64_t Hq, int64_t Hkv, const c10::optional<at::Tensor>& status,
+                    const c10::optional<at::Tensor>& q_norm, const c10::optional<at::Tensor>& k_norm, double eps) {
+  check_same_device(qkv, {&pos, &cos_sin, &slots, &kc, &out}, "rope_cache_fp8");
+  const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "rope_cache_fp8");
+  const int ldq = row_ld16(qkv, "rope_cache_fp8: qkv"), ldo = row_ld16(out, "rope_cache_fp8: out");
+  const int64_t T = qkv.size(0);
+  TORCH_CHECK(Hq > 0 && Hkv == kc.size(1) && qkv.size(1) == (Hq + 2 * Hkv) * 128,
+              "rope_cache_fp8: qkv must hold exactly (Hq + 2 Hkv) heads of 128, Hkv as in the cache");
+  TORCH_CHECK(out.size(0) == T && out.size(1) == Hq * 128, "rope_cache_fp8: out must be [T, Hq * 128]");
+  TORCH_CHECK(T <= INT_MAX, "rope_cache_fp8: too many rows");
+  TORCH_CHECK(pos.scalar_type() == at::kInt && pos.is_contiguous() && pos.numel() == T,
+              "rope_cache_fp8: positions must be contiguous int32 [T]");
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.numel() == T,
+              "rope_cache_fp8: slot_mapping must be contiguous int64 [T]");
+  TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.dim() == 2 && cos_sin.size(1) == 128 &&
+                  cos_sin.is_contiguous() && (reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) & 15) == 0,
+              "rope_cache_fp8: cos_sin must be contiguous fp32 [positions, 128]");
+  const void *qn = nullptr, *kn = nullptr;
+  for (const auto* w : {&q_norm, &k_norm})
+    if (w->has_value())
+      TORCH_CHECK((*w)->device() == qkv.device() && (*w)->scalar_type() == at::kBFloat16 && (*w)->numel() == 128 &&
+                      (*w)->is_contiguous() && (reinterpret_cast<uintptr_t>((*w)->data_ptr()) & 15) == 0,
+                  "rope_cache_fp8: q/k norm weights must be contiguous bf16 CUDA [128]");
+  if (q_norm.has_value()) qn = q_norm->data_ptr();
+  if (k_norm.has_value()) kn = k_norm->data_ptr();
+  // q is rotated by the block that reads it: out may be qkv's own q columns, but no other part of it
+  if (T > 0) {
+    const char* a = static_cast<const char*>(qkv.data_ptr());
+    const char* b = static_cast<const char*>(out.data_ptr());
+    const char* a1 = a + ((T - 1) * (int64_t)ldq + qkv.size(1)) * 2;
+    const char* b1 = b + ((T - 1) * (int64_t)ldo + out.size(1)) * 2;
+    TORCH_CHECK(b1 <= a || a1 <= b || (a == b && (ldq == ldo || T == 1)),
+                "rope_cache_fp8: out overlaps qkv other than as its q columns");
+  }
+  CHECK_CUDA(qkv);
+  const c10::cuda::CUDAGuard g(qkv.device());
+  cx::rope_cache_fp8(qkv.data_ptr(), ldq, pos.data_ptr<int>(), cos_sin.data_ptr<float>(), slots.data_ptr<int64_t>(), c,
+                     out.data_ptr(), ldo, (int)T, (int)Hq, (int)std::min<int64_t>(cos_sin.size(0), INT_MAX),
+                     status_ptr(status), cur_stream(qkv), qn, kn, (float)eps);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+int64_t decode_fp8_rows(int64_t device, int64_t B, int64_t Hkv, int64_t G) {
+  TORCH_CHECK(B >= 0 && Hkv > 0 && G > 0, "decode_workspace_fp8: bad sizes");
+  return cx::decode_fp8_rows(at::cuda::getDeviceProperties(device)->multiProcessorCount, (int)B, (int)Hkv, (int)G);
+}
+
+void decode_attention_fp8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
+                          const at::Tensor& vs, const at::Tensor& block_tables, const at::Tensor& ctx_lens,
+                          at::Tensor& out, int64_t Hq, double scale, at::Tensor& ws,
+                          const c10::optional<at::Tensor>& status) {
+  check_same_device(q, {&kc, &block_tables, &ctx_lens, &out, &ws}, "decode_attention_fp8");
+  const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "decode_attention_fp8");
+  const int ldq = row_ld16(q, "decode_attention_fp8: q"), ldo = row_ld16(out, "decode_attention_fp8: out");
+  const int64_t B = q.size(0);
+  TORCH_CHECK(Hq > 0 && Hq % c.Hkv == 0 && Hq / c.Hkv <= 16,
+              "decode_attention_fp8: the query heads must be a multiple of the KV heads, 16 of them per KV head at most");
+  TORCH_CHECK(q.size(1) >= Hq * 128 && out.size(0) == B && out.size(1) == Hq * 128,
+              "decode_attention_fp8: q must hold Hq heads of 128 per row and out be [B, Hq * 128]");
+  TORCH_CHECK(B <= cx::DEC8_MAX_BATCH, "decode_attention_fp8: at most ", cx::DEC8_MAX_BATCH, " sequences per call");
+  TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
+                  block_tables.size(0) == B,
+              "decode_attention_fp8: block_tables must be contiguous int32 [B, max_blocks]");
+  TORCH_CHECK(ctx_lens.scalar_type() == at::kInt && ctx_lens.is_contiguous() && ctx_lens.numel() == B,
+              "decode_attention_fp8: ctx_lens must be contiguous int32 [B]");
+  TORCH_CHECK(B * c.Hkv * block_tables.size(1) < (int64_t)1 << 30 && block_tables.size(1) < (int64_t)1 << 26,
+              "decode_attention_fp8: block tables too large");
+  const int64_t G = Hq / c.Hkv;
+  CHECK_CUDA(q);
+  TORCH_CHECK(ws.scalar_type() == at::kFloat && ws.is_contiguous() && ws.dim() == 2 && ws.size(1) == G * cx::DEC8_ROW &&
+                  ws.size(0) >= cx::decode_fp8_rows(sms_of(q), (int)B, c.Hkv, (int)G),
+              "decode_attention_fp8: the workspace must come from decode_workspace_fp8 for these heads and at least ", B,
+              " sequences");
+  const c10::cuda::CUDAGuard g(q.device());
+  cx::decode_attention_fp8(q.data_ptr(), ldq, c, block_tables.data_ptr<int>(), (int)block_tables.size(1),
+                           ctx_lens.data_ptr<int>(), out.data_ptr(), ldo, (int)B, (int)Hq, (float)scale,
+                           ws.data_ptr<float>(), ws.size(0), sms_of(q), status_ptr(status), cur_stream(q));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+void kv_copy_blocks(at::Tensor& kv, const at::Tensor& pairs, const c10::optional<at::Tensor>& scales,
+                    const c10::optional<at::Tensor>& status) {
+  TORCH_CHECK(kv.dim() == 6 && kv.size(1) == 2 && kv.is_contiguous(),
+              "kv_copy_blocks: kv must be contiguous [layers, 2, blocks, Hkv, tokens, head_dim]");
+  check_same_device(kv, {&pairs}, "kv_copy_blocks");
+  TORCH_CHECK(pairs.scalar_type() == at::kInt && pairs.dim() == 2 && pairs.size(1) == 2 && pairs.is_contiguous(),
+              "kv_copy_blocks: pairs must be contiguous int32 [n, 2] (source, destination)");
+  const int64_t n = pairs.size(0), block = kv.size(3) * kv.size(4) * kv.size(5) * kv.element_size();
+  TORCH_CHECK(block % 16 == 0 && (reinterpret_cast<uintptr_t>(kv.data_ptr()) & 15) == 0,
+              "kv_copy_blocks: blocks must be multiples of 16 bytes on 16-byte boundaries");
+  TORCH_CHECK(n <= INT_MAX && kv.size(0) * 2 <= 65535 && kv.size(2) <= INT_MAX, "kv_copy_blocks: too many blocks");
+  float* sp = nullptr;
+  if (scales.has_value()) {
+    check_same_device(kv, {&*scales}, "kv_copy_blocks");
+    TORCH_CHECK(scales->scalar_type() == at::kFloat && scales->is_contiguous() && scales->dim() == 4 &&
+                    scales->size(0) == kv.size(0) && scales->size(1) == 2 && scales->size(2) == kv.size(2) &&
+                    scales->size(3) == kv.size(3),
+                "kv_copy_blocks: scales must be contiguous fp32 [layers, 2, blocks, Hkv]");
+    sp = scales->data_ptr<float>();
+  } else {
+    TORCH_CHECK(kv.scalar_type() != at::kFloat8_e4m3fn, "kv_copy_blocks: an 8-bit cache is copied with its scales");
+  }
+  CHECK_CUDA(kv);
+  const c10::cuda::CUDAGuard g(kv.device());
+  cx::kv_copy_blocks(kv.data_ptr(), sp, pairs.data_ptr<int>(), (int)n, (int)kv.size(0) * 2, (int)kv.size(2), block,
+                     (int)kv.size(3), sms_of(kv), status_ptr(status), cur_stream(kv));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+void kv_dequant_blocks(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
+                       const at::Tensor& table, at::Tensor& kout, at::Tensor& vout,
+                       const c10::optional<at::Tensor>& status) {
+  const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "kv_dequant_blocks");
+  const c10::cuda::CUDAGuard g(kc.device());
+  cx::kv_dequant_blocks(c, table.data_ptr<int>(), (int)table.numel(), kout.data_ptr(), vout.data_ptr(),
+                        status_ptr(status), cur_stream(kc));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 // ---- peer-memory movement (addresses may be local or peer-mapped) ----------
@@ -458,6 +618,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attention", &decode_attention);
   m.def("decode_attention_plan", &decode_attention_plan);
   m.def("decode_workspace_floats", &decode_workspace_floats);
+  m.def("rope_cache_fp8", &rope_cache_fp8);
+  m.def("decode_fp8_rows", &decode_fp8_rows);
+  m.attr("DECODE_FP8_ROW") = cx::DEC8_ROW;
+  m.def("decode_attention_fp8", &decode_attention_fp8);
+  m.def("kv_copy_blocks", &kv_copy_blocks);
+  m.def("kv_dequant_blocks", &kv_dequant_blocks);
   m.def("kv_push_layer", &kv_push_layer);
   m.def("gemm_splits", &gemm_splits);
   m.def("gemm_raster_group", &cx::gemm_raster_group);

@@ -1,0 +1,760 @@
+// The 8-bit paged KV cache: quantising write, decode attention over it, block
+// copies.
+//
+// Values are e4m3 with one power-of-two scale per (block of 16 tokens, KV
+// head).  e4m3 is a floating format, so the scale's mantissa would buy no
+// accuracy; as a power of two, raising a block's scale for a later, larger
+// token moves exponents only (exact except for values that fall under the
+// smallest e4m3 step), and every cached value is an exact bf16 number.
+#include <algorithm>
+#include <stdexcept>
+
+#include "common.cuh"
+#include "kv_fp8.h"
+
+namespace cx {
+
+namespace kvq {
+constexpr int D = 128, BS = 16;
+constexpr int MIN_EXP = -100, MAX_EXP = 120;   // 448 * 2^120 covers every finite bf16
+constexpr int THREADS = 256;
+}  // namespace kvq
+
+// 2^e for e of [-126, 127]
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// The smallest e >= MIN_EXP with a <= 448 * 2^e = 1.75 * 2^(e + 8), for finite a >= 0.
+__device__ __forceinline__ int fp8_exp_for(float a) {
+  const uint32_t u = __float_as_uint(a);
+  const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return max(e, kvq::MIN_EXP);
+}
+__device__ __forceinline__ int fp8_exp_of(float scale) {
+  return min(max((int)((__float_as_uint(scale) >> 23) & 255u) - 127, kvq::MIN_EXP), kvq::MAX_EXP);
+}
+// two fp32 -> two e4m3 bytes (lo in the low byte), nearest even, NaN kept
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// two e4m3 bytes -> f16x2, exact
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return r;
+}
+__device__ __forceinline__ float f16_lo(uint32_t v) {
+  float f;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.f32.f16 %0, l;\n\t}" : "=f"(f) : "r"(v));
+  return f;
+}
+__device__ __forceinline__ float f16_hi(uint32_t v) {
+  float f;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.f32.f16 %0, h;\n\t}" : "=f"(f) : "r"(v));
+  return f;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float finite_or_zero(float a) {   // |a| of a finite value, 0 of Inf and NaN
+  const uint32_t u = __float_as_uint(a) & 0x7fffffffu;
+  return u < 0x7f800000u ? __uint_as_float(u) : 0.f;
+}
+// x * mul as e4m3 would hold it: e4m3 has no infinities, so Inf becomes NaN
+__device__ __forceinline__ float scaled_or_nan(float x, float mul) {
+  return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fffffffu) : x * mul;
+}
+
+// ------------------------------------------------- RoPE + quantising write
+// One CTA per token.  All 256 threads rotate the token's q heads (16 lanes of
+// 16 bytes per head).  The CTA of the first token that falls into a block
+// also writes the block: its scale depends on every row that this call puts
+// there, so one CTA collects them -- a scan of the call's slots, which keeps
+// the result independent of the rows' order (of two rows for one slot the
+// later wins) -- and each warp takes one KV head of K or V: rotated rows in
+// registers, their largest magnitude, the scale, the block's older rows
+// requantised if the scale grew, the new rows.  A block whose row 0 is
+// written starts anew; otherwise its scale never shrinks.
+__global__ void __launch_bounds__(kvq::THREADS)
+    rope_cache_fp8_kernel(const __nv_bfloat16* qkv, int ldq, const int* __restrict__ pos,
+                          const float* __restrict__ cos_sin, const int64_t* __restrict__ slots, KvFp8 c,
+                          __nv_bfloat16* out, int ldo, int T, int Hq, int max_pos, int* status,
+                          const __nv_bfloat16* __restrict__ qn, const __nv_bfloat16* __restrict__ kn, float eps) {
+  using namespace kvq;
+  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int p = pos[t];
+  const bool pos_ok = p >= 0 && p < max_pos;
+  const int64_t slot = slots[t];
+  const int64_t blk = slot >> 4;
+  if (tid == 0 && (!pos_ok || (slot >= 0 && blk >= c.num_blocks))) record_status(status, CX_ERR_BOUNDS);
+
+  // ---- this token's block, if it is the first of its rows
+  __shared__ int row_of[BS];      // the token of each row of the block (-1: not written by this call)
+  __shared__ int first;
+  bool lead = pos_ok && slot >= 0 && blk < c.num_blocks;
+  if (lead && t > 0) {            // most tokens of a prompt follow one of the same block
+    const int64_t s1 = slots[t - 1];
+    const int p1 = pos[t - 1];
+    lead = !(s1 >= 0 && (s1 >> 4) == blk && p1 >= 0 && p1 < max_pos);
+  }
+  if (lead) {                     // uniform over the CTA
+    if (tid < BS) row_of[tid] = -1;
+    if (tid == 0) first = 0x7fffffff;
+    __syncthreads();
+    for (int i = tid; i < T; i += THREADS) {
+      const int64_t si = slots[i];
+      if (si >= 0 && (si >> 4) == blk) {
+        const int pi = pos[i];
+        if (pi >= 0 && pi < max_pos) {
+          atomicMax(&row_of[(int)(si & 15)], i);
+          atomicMin(&first, i);
+        }
+      }
+    }
+    __syncthreads();
+    lead = first == t;
+  }
+  if (lead) {
+    const int half = lane >> 4, i4 = 4 * (lane & 15);   // this lane: dims [4 lane, 4 lane + 4)
+    for (int item = warp; item < 2 * c.Hkv; item += THREADS / 32) {
+      const bool is_v = item >= c.Hkv;
+      const int h = is_v ? item - c.Hkv : item;
+      const __nv_bfloat16* src = qkv + (size_t)(Hq + item) * D + 4 * lane;
+      uint32_t x[BS][2];          // bf16 pairs of the new rows
+      float amax = 0.f;
+#pragma unroll
+      for (int r = 0; r < BS; ++r) {
+        const int tok = row_of[r];
+        if (tok < 0) continue;    // uniform over the warp
+        const uint2 raw = *reinterpret_cast<const uint2*>(src + (size_t)tok * ldq);
+        x[r][0] = raw.x;
+        x[r][1] = raw.y;
+        if (!is_v) {
+          float a[4] = {bf16_lo(raw.x), bf16_hi(raw.x), bf16_lo(raw.y), bf16_hi(raw.y)};
+          if (kn != nullptr) {
+            const float ss = warp_sum(a[0] * a[0] + a[1] * a[1] + a[2] * a[2] + a[3] * a[3]);
+            const float n = rsqrtf(ss * (1.0f / D) + eps);
+            const uint2 w = *reinterpret_cast<const uint2*>(kn + 4 * lane);
+            // bf16 between the norm and the rotation, like a norm layer of its own
+            const uint32_t y0 = pack_bf16x2(a[0] * n * bf16_lo(w.x), a[1] * n * bf16_hi(w.x));
+            const uint32_t y1 = pack_bf16x2(a[2] * n * bf16_lo(w.y), a[3] * n * bf16_hi(w.y));
+            a[0] = bf16_lo(y0); a[1] = bf16_hi(y0); a[2] = bf16_lo(y1); a[3] = bf16_hi(y1);
+          }
+          const float* cs = cos_sin + (size_t)pos[tok] * D + i4;
+          const float4 co = *reinterpret_cast<const float4*>(cs), si = *reinterpret_cast<const float4*>(cs + D / 2);
+          float b[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) b[e] = __shfl_xor_sync(0xffffffffu, a[e], 16);
+          const float sg = half ? 1.f : -1.f;   // first half: a cos - b sin; second: a cos + b sin
+          // rounded to bf16 before e4m3: what a bf16 cache would hold is what is quantised
+          x[r][0] = pack_bf16x2(a[0] * co.x + sg * b[0] * si.x, a[1] * co.y + sg * b[1] * si.y);
+          x[r][1] = pack_bf16x2(a[2] * co.z + sg * b[2] * si.z, a[3] * co.w + sg * b[3] * si.w);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          amax = fmaxf(amax, fmaxf(finite_or_zero(bf16_lo(x[r][e])), finite_or_zero(bf16_hi(x[r][e]))));
+      }
+      amax = warp_max(amax);
+      float* scale = (is_v ? c.vs : c.ks) + (size_t)blk * c.Hkv + h;
+      uint8_t* dst = (is_v ? c.v : c.k) + ((size_t)blk * c.Hkv + h) * (BS * D) + 4 * lane;
+      int e = fp8_exp_for(amax);
+      if (row_of[0] < 0) {        // the block's rows so far stay
+        const int old = fp8_exp_of(*scale);
+        if (e <= old) {
+          e = old;
+        } else {
+          const float f = exp2_int(max(old - e, -126));
+#pragma unroll 4
+          for (int r = 0; r < BS; ++r) {
+            if (row_of[r] >= 0) continue;
+            uint32_t* q = reinterpret_cast<uint32_t*>(dst + r * D);
+            const uint32_t w = *q;
+            const uint32_t a = e4m3x2_to_f16x2((uint16_t)w), b = e4m3x2_to_f16x2((uint16_t)(w >> 16));
+            *q = to_e4m3x2(f16_lo(a) * f, f16_hi(a) * f) | to_e4m3x2(f16_lo(b) * f, f16_hi(b) * f) << 16;
+          }
+        }
+      }
+      __syncwarp();               // every lane has read the old scale
+      if (lane == 0) *scale = exp2_int(e);
+      const float mul = exp2_int(-e);
+#pragma unroll
+      for (int r = 0; r < BS; ++r) {
+        if (row_of[r] < 0) continue;
+        const uint32_t lo = to_e4m3x2(scaled_or_nan(bf16_lo(x[r][0]), mul), scaled_or_nan(bf16_hi(x[r][0]), mul));
+        const uint32_t hi = to_e4m3x2(scaled_or_nan(bf16_lo(x[r][1]), mul), scaled_or_nan(bf16_hi(x[r][1]), mul));
+        *reinterpret_cast<uint32_t*>(dst + r * D) = lo | hi << 16;
+      }
+    }
+  }
+
+  // ---- q: 16 lanes per head, dims [8 j, 8 j + 8)
+  const int j = tid & 15;
+  const float sg = j < 8 ? -1.f : 1.f;
+  float co[8], si[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) co[e] = si[e] = 0.f;   // a position out of range: a row of zeros
+  if (pos_ok) {
+    const float* cs = cos_sin + (size_t)p * D + 8 * (j & 7);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float4 a = *reinterpret_cast<const float4*>(cs + 4 * e);
+      const float4 b = *reinterpret_cast<const float4*>(cs + D / 2 + 4 * e);
+      co[4 * e] = a.x; co[4 * e + 1] = a.y; co[4 * e + 2] = a.z; co[4 * e + 3] = a.w;
+      si[4 * e] = b.x; si[4 * e + 1] = b.y; si[4 * e + 2] = b.z; si[4 * e + 3] = b.w;
+    }
+  }
+  for (int h0 = 0; h0 < Hq; h0 += THREADS / 16) {    // whole warps stay in the loop: two heads per warp
+    const int h = h0 + (tid >> 4);
+    const bool on = h < Hq;
+    u128 raw = on ? ld_v4(qkv + (size_t)t * ldq + (size_t)h * D + 8 * j) : u128{0, 0, 0, 0};
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
+    float a[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a[2 * e] = bf16_lo(w[e]);
+      a[2 * e + 1] = bf16_hi(w[e]);
+    }
+    if (qn != nullptr) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += a[e] * a[e];
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float n = rsqrtf(ss * (1.0f / D) + eps);
+      const u128 nw = ld_v4(qn + 8 * j);
+      const uint32_t* pw = reinterpret_cast<const uint32_t*>(&nw);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t y = pack_bf16x2(a[2 * e] * n * bf16_lo(pw[e]), a[2 * e + 1] * n * bf16_hi(pw[e]));
+        a[2 * e] = bf16_lo(y);
+        a[2 * e + 1] = bf16_hi(y);
+      }
+    }
+    float o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float b = __shfl_xor_sync(0xffffffffu, a[e], 8);
+      o[e] = pos_ok ? a[e] * co[e] + sg * b * si[e] : 0.f;
+    }
+    if (on) {
+      u128 r;
+      uint32_t* pr = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pr[e] = pack_bf16x2(o[2 * e], o[2 * e + 1]);
+      st_v4(out + (size_t)t * ldo + (size_t)h * D + 8 * j, r);
+    }
+  }
+}
+
+void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_sin, const int64_t* slots,
+                    const KvFp8& c, void* out, int ldo, int T, int Hq, int max_pos, int* status, cudaStream_t s,
+                    const void* q_norm, const void* k_norm, float eps) {
+  // Each block's first row scans the call's slots, so rows are taken
+  // KVQ_MAX_ROWS at a time to keep the scan linear in T.
+  for (int t0 = 0; t0 < T; t0 += KVQ_MAX_ROWS) {
+    const int n = std::min(KVQ_MAX_ROWS, T - t0);
+    rope_cache_fp8_kernel<<<n, kvq::THREADS, 0, s>>>(
+        reinterpret_cast<const __nv_bfloat16*>(qkv) + (size_t)t0 * ldq, ldq, pos + t0, cos_sin, slots + t0, c,
+        reinterpret_cast<__nv_bfloat16*>(out) + (size_t)t0 * ldo, ldo, n, Hq, max_pos, status,
+        reinterpret_cast<const __nv_bfloat16*>(q_norm), reinterpret_cast<const __nv_bfloat16*>(k_norm), eps);
+  }
+}
+
+// ------------------------------------------------------- decode attention
+// S = q.K^T and O^T = V^T.W^T on mma.sync m16n8k16 (f16 in, fp32 out) from
+// registers alone: the cached bytes are loaded straight into the layout the
+// fragments need and converted e4m3 -> f16 (exact) in place.
+//   K: lane (g = lane / 4, c = lane % 4) loads bytes [16 c, 16 c + 16) of both
+//      64-byte halves of tokens g and g + 8.  The contraction may take the
+//      dims in any order as long as q uses the same one, so bytes 4j..4j+3 of
+//      a load are the four k-values a lane holds of MMA step j.
+//   V: the lane loads bytes [16 g, 16 g + 16) of tokens 2c, 2c + 1, 2c + 8,
+//      2c + 9 -- the tokens of its column pairs -- and interleaves the bytes
+//      of two tokens, which makes byte pair (2j, 2j + 1) the rows of MMA tile j.
+// S comes out with the heads on the rows and each lane holding tokens 2c,
+// 2c + 1 (+ 8), which is the second product's B fragment as it stands.
+// The block scales stay out of the operands: K's multiplies the logits, V's
+// is folded into the weights exp2(s_j + log2 v_j - mv) with a running maximum
+// mv of their own (f16 weights then keep their precision whatever the ratio
+// of the scales), next to the usual maximum m of the softmax sum.
+// q is scaled by a power of two per head into f16's range: exact but for
+// elements 2^29 times smaller than the head's largest.
+//
+// Work split: the blocks of all (sequence, KV head) pairs, laid end to end,
+// are cut into equal runs, one per CTA, from the lengths themselves -- the
+// same launch (a graph replay) is balanced for any lengths.  A pair that
+// spans several CTAs leaves partial results in the workspace, and the CTA
+// that arrives last merges them (a counter that wraps to zero by itself).
+namespace dec8 {
+constexpr int D = kvq::D, BS = kvq::BS, WARPS = 4, THREADS = 32 * WARPS, CTAS_PER_SM = 4;
+constexpr int MIN_BLOCKS = 2 * WARPS;   // a CTA takes at least this many blocks
+constexpr float RESCALE = 8.f;          // O is rescaled once mv grows by this much (weights stay under 2^9)
+}  // namespace dec8
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// NT: tiles of 8 query heads per KV head (1: groups up to 8, 2: up to 16).
+template <int NT>
+__global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
+    decode_attn_fp8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, KvFp8 c, const int* __restrict__ tables,
+                           int max_blocks, const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, int ldo,
+                           int B, int Hq, float scale_log2, float* __restrict__ part, uint32_t* __restrict__ counters,
+                           int* status) {
+  using namespace dec8;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* so = reinterpret_cast<float*>(smem);                 // [WARPS][8 NT][D]
+  float* sm = so + WARPS * 8 * NT * D;                        // [WARPS][8 NT][m, l, mv]
+  int* pre = reinterpret_cast<int*>(sm + WARPS * 8 * NT * 4); // [B + 1] blocks of the pairs before sequence b
+  __shared__ int wsum[WARPS];
+  __shared__ uint32_t ticket;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int gq = lane >> 2, qd = lane & 3;
+  const int Hkv = c.Hkv, G = Hq / Hkv;
+
+  auto len_of = [&](int b) { return min(max(ctx_lens[b], 0), max_blocks * BS); };
+  // ---- prefix sums of the pairs' blocks
+  if (tid == 0) pre[0] = 0;
+  int run = 0;
+  for (int b0 = 0; b0 < B; b0 += THREADS) {
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < B) {
+      const int len = ctx_lens[b];
+      if (len > max_blocks * BS && blockIdx.x == 0) record_status(status, CX_ERR_BOUNDS);
+      n = (len_of(b) + BS - 1) / BS * Hkv;
+    }
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) wsum[warp] = x;
+    __syncthreads();
+    int add = run;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) add += wsum[w];
+      run += wsum[w];
+    }
+    if (b < B) pre[b + 1] = add + x;
+    __syncthreads();
+  }
+  const int total = run;
+  // rows without tokens: zeros
+  for (int b = blockIdx.x; b < B; b += gridDim.x)
+    if (pre[b + 1] == pre[b])
+      for (int i = tid; i < Hq * D / 8; i += THREADS) st_v4(out + (size_t)b * ldo + 8 * i, u128{0, 0, 0, 0});
+  const int n_cta = max(1, min((int)gridDim.x, (total + MIN_BLOCKS - 1) / MIN_BLOCKS));
+  const int per = (total + n_cta - 1) / n_cta;
+  const int u0 = min(total, (int)blockIdx.x * per), u1 = min(total, u0 + per);
+
+  int b = 0;
+  {  // the sequence that holds u0: the last b with pre[b] <= u0
+    int lo = 0, hi = B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= u0) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+  }
+  for (int u = u0; u < u1;) {
+    while (pre[b + 1] <= u) ++b;
+    const int nblk = (pre[b + 1] - pre[b]) / Hkv;
+    const int h = (u - pre[b]) / nblk;                         // KV head
+    const int pair0 = pre[b] + h * nblk;                       // first block of the pair
+    const int j0 = u - pair0, j1 = min(nblk, u1 - pair0);      // its blocks in this CTA
+    const int len = len_of(b);
+    const int* bt = tables + (size_t)b * max_blocks;
+
+    // ---- q fragments, scaled by a power of two per head
+    uint32_t qa[8][2 * NT];
+    float qf[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int hh = gq + 8 * nt;
+      u128 raw[4];
+      float am = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {                            // dims (i / 2) * 64 + qd * 16 + (i % 2) * 8 ..
+        raw[i] = hh < G ? ld_v4(q + (size_t)b * ldq + (size_t)(h * G + hh) * D + (i >> 1) * 64 + qd * 16 + (i & 1) * 8)
+                        : u128{0, 0, 0, 0};
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) am = fmaxf(am, fmaxf(finite_or_zero(bf16_lo(w[e])), finite_or_zero(bf16_hi(w[e]))));
+      }
+      am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+      am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
+      // am * 2^-eq in [2^14, 2^15)
+      const int eq = am > 0.f ? max((int)(__float_as_uint(am) >> 23) - 127 - 14, -126) : 0;
+      const float down = exp2_int(-eq);
+      qf[nt] = exp2_int(eq) * scale_log2;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)                            // step 2i + e / 2; dims 0,1 then 2,3 of the four
+          qa[2 * i + (e >> 1)][2 * nt + (e & 1)] = pack_f16x2(bf16_lo(w[e]) * down, bf16_hi(w[e]) * down);
+      }
+    }
+
+    float o[NT][8][4];
+    float m[NT], l[NT], mv[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt] = mv[nt] = -INFINITY;
+      l[nt] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][mt][e] = 0.f;
+    }
+    u128 kr[4], vr[4];
+    float ks = 1.f, vs = 1.f;
+    int id = -1;
+    // block ids of the warp's next 32 blocks, one per lane
+    int ids = 0, ids_at = j0 + warp;
+    auto id_of = [&](int j) -> int {                           // j advances by WARPS; uniform over the warp
+      if (((j - ids_at) / WARPS) >= 32) ids_at = j;
+      if (j == ids_at) {
+        const int jj = j + WARPS * lane;
+        ids = jj < j1 ? bt[jj] : -1;
+      }
+      int r = __shfl_sync(0xffffffffu, ids, ((j - ids_at) / WARPS) & 31);
+      if (j < j1 && (r < 0 || r >= c.num_blocks)) {
+        if (lane == 0) record_status(status, CX_ERR_BOUNDS);
+        r = -1;
+      }
+      return j < j1 ? r : -1;
+    };
+    auto load_k = [&](int i) {
+      if (i < 0) return;
+      const uint8_t* p = c.k + ((size_t)i * Hkv + h) * (BS * D) + gq * D + qd * 16;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) kr[e] = ld_nc_v4(p + (e >> 1) * 8 * D + (e & 1) * 64);
+      ks = c.ks[(size_t)i * Hkv + h];
+    };
+    auto load_v = [&](int i) {
+      if (i < 0) return;
+      const uint8_t* p = c.v + ((size_t)i * Hkv + h) * (BS * D) + 2 * qd * D + gq * 16;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vr[e] = ld_nc_v4(p + ((e >> 1) * 8 + (e & 1)) * D);
+      vs = c.vs[(size_t)i * Hkv + h];
+    };
+    int j = j0 + warp;
+    if (j < j1) {
+      id = id_of(j);
+      load_k(id);
+      load_v(id);
+    }
+    for (; j < j1; j += WARPS) {
+      const int cur = id;
+      const int next = j + WARPS < j1 ? id_of(j + WARPS) : -1;
+      id = next;
+      float s[2][4];                                           // tokens 0-7, 8-15 of the block
+      if (cur >= 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.f;
+#pragma unroll
+        for (int st = 0; st < 8; ++st) {                       // 16 dims each
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(&kr[2 * tt + (st >> 2)])[st & 3];
+            const uint32_t b0 = e4m3x2_to_f16x2((uint16_t)w), b1 = e4m3x2_to_f16x2((uint16_t)(w >> 16));
+            mma_f16(s[tt], qa[st][0], NT == 2 ? qa[st][2 * NT - 2] : 0u, qa[st][1], NT == 2 ? qa[st][2 * NT - 1] : 0u,
+                    b0, b1);
+          }
+        }
+      }
+      const float kscale = ks, vscale = vs;
+      load_k(next);
+      if (cur < 0) {
+        load_v(next);
+        continue;
+      }
+      const int tok0 = j * BS;
+      const bool tail = tok0 + BS > len;
+      const float ev = (float)((int)(__float_as_uint(vscale) >> 23) - 127);
+      uint32_t wb[NT][2];                                      // weights as the B fragment of the second product
+      float alpha[NT];
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float x[4] = {s[0][2 * nt], s[0][2 * nt + 1], s[1][2 * nt], s[1][2 * nt + 1]};
+        const float f = qf[nt] * kscale;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] *= f;
+          if (tail && tok0 + 2 * qd + (e & 1) + (e >> 1) * 8 >= len) x[e] = -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(m[nt], mx), base = m_new == -INFINITY ? 0.f : m_new;
+        l[nt] = l[nt] * ex2(m[nt] - base) + ((ex2(x[0] - base) + ex2(x[1] - base)) + (ex2(x[2] - base) + ex2(x[3] - base)));
+        m[nt] = m_new;
+        alpha[nt] = 1.f;
+        if (mx + ev > mv[nt] + RESCALE || mv[nt] == -INFINITY) {
+          const float mv_new = fmaxf(mv[nt], mx + ev);
+          alpha[nt] = mv_new == -INFINITY ? 1.f : ex2(mv[nt] - mv_new);
+          mv[nt] = mv_new;
+          grow = true;
+        }
+        const float vb = ev - (mv[nt] == -INFINITY ? 0.f : mv[nt]);
+        wb[nt][0] = pack_f16x2(ex2(x[0] + vb), ex2(x[1] + vb));
+        wb[nt][1] = pack_f16x2(ex2(x[2] + vb), ex2(x[3] + vb));
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {                      // O^T's columns are heads 2 qd, 2 qd + 1
+          const float a0 = __shfl_sync(0xffffffffu, alpha[nt], 8 * qd), a1 = __shfl_sync(0xffffffffu, alpha[nt], 8 * qd + 4);
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) {
+            o[nt][mt][0] *= a0;
+            o[nt][mt][1] *= a1;
+            o[nt][mt][2] *= a0;
+            o[nt][mt][3] *= a1;
+          }
+        }
+      }
+      if (tail) {   // rows past the end were never written: 0 x NaN would poison O
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (tok0 + 2 * qd + (e & 1) + (e >> 1) * 8 >= len) vr[e] = u128{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {                            // 4 bytes of each token: MMA tiles 2w, 2w + 1
+        uint32_t t4[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t4[e] = reinterpret_cast<const uint32_t*>(&vr[e])[w];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const uint32_t x = __byte_perm(t4[0], t4[1], hf ? 0x7362 : 0x5140);
+          const uint32_t y = __byte_perm(t4[2], t4[3], hf ? 0x7362 : 0x5140);
+          const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)x), a1 = e4m3x2_to_f16x2((uint16_t)(x >> 16));
+          const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)y), a3 = e4m3x2_to_f16x2((uint16_t)(y >> 16));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + hf], a0, a1, a2, a3, wb[nt][0], wb[nt][1]);
+        }
+      }
+      load_v(next);
+    }
+
+    // ---- the warps' results of this pair
+    __syncthreads();                                           // the previous pair's reads of so / sm are done
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float ls = l[nt];
+      ls += __shfl_xor_sync(0xffffffffu, ls, 1);
+      ls += __shfl_xor_sync(0xffffffffu, ls, 2);
+      if (qd == 0) {
+        float* p = sm + (warp * 8 * NT + nt * 8 + gq) * 4;
+        p[0] = m[nt];
+        p[1] = ls;
+        p[2] = mv[nt];
+      }
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          so[(warp * 8 * NT + nt * 8 + 2 * qd + (e & 1)) * D + gq * 16 + 2 * mt + (e >> 1)] = o[nt][mt][e];
+    }
+    __syncthreads();
+    const int c0 = pair0 / per, c1 = (pair0 + nblk - 1) / per;  // the CTAs that share the pair
+    // thread: dim tid of every head
+    for (int hh = 0; hh < G; ++hh) {
+      float M = -INFINITY, MV = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float* p = sm + (w * 8 * NT + hh) * 4;
+        M = fmaxf(M, p[0]);
+        MV = fmaxf(MV, p[2]);
+      }
+      const float mb = M == -INFINITY ? 0.f : M, vb = MV == -INFINITY ? 0.f : MV;
+      float num = 0.f, den = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float* p = sm + (w * 8 * NT + hh) * 4;
+        num += so[(w * 8 * NT + hh) * D + tid] * ex2(p[2] - vb);
+        den += p[1] * ex2(p[0] - mb);
+      }
+      if (c0 == c1) {
+        out[(size_t)b * ldo + (size_t)(h * G + hh) * D + tid] = __float2bfloat16(den == 0.f ? 0.f : num / den * ex2(vb - mb));
+      } else {   // a CTA's first pair goes to its slot 0, its last to slot 1
+        float* p = part + ((size_t)(blockIdx.x * 2 + (u == u0 ? 0 : 1)) * G + hh) * DEC8_ROW;
+        p[tid] = num;
+        if (tid == 0) {
+          p[D] = M;
+          p[D + 1] = den;
+          p[D + 2] = MV;
+        }
+      }
+    }
+    if (c0 != c1) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) ticket = atomicInc(&counters[b * Hkv + h], (uint32_t)(c1 - c0));   // wraps to 0 at the last
+      __syncthreads();
+      if (ticket == (uint32_t)(c1 - c0)) {
+        __threadfence();
+        for (int hh = 0; hh < G; ++hh) {
+          auto slot = [&](int cc) {   // the pair is the first of every CTA but perhaps c0
+            return part + ((size_t)(cc * 2 + (cc == c0 && pair0 != c0 * per ? 1 : 0)) * G + hh) * DEC8_ROW;
+          };
+          float M = -INFINITY, MV = -INFINITY;
+          for (int cc = c0; cc <= c1; ++cc) {
+            M = fmaxf(M, __ldcg(slot(cc) + D));
+            MV = fmaxf(MV, __ldcg(slot(cc) + D + 2));
+          }
+          const float mb = M == -INFINITY ? 0.f : M, vb = MV == -INFINITY ? 0.f : MV;
+          float num = 0.f, den = 0.f;
+          for (int cc = c0; cc <= c1; ++cc) {
+            const float* p = slot(cc);
+            num += __ldcg(p + tid) * ex2(__ldcg(p + D + 2) - vb);
+            den += __ldcg(p + D + 1) * ex2(__ldcg(p + D) - mb);
+          }
+          out[(size_t)b * ldo + (size_t)(h * G + hh) * D + tid] = __float2bfloat16(den == 0.f ? 0.f : num / den * ex2(vb - mb));
+        }
+      }
+    }
+    u = pair0 + j1;
+  }
+}
+
+int decode_fp8_ctas(int sms) { return sms * dec8::CTAS_PER_SM; }
+long decode_fp8_rows(int sms, int B, int Hkv, int G) {
+  const long row = (long)G * DEC8_ROW;
+  return 2L * decode_fp8_ctas(sms) + ((long)B * Hkv + row - 1) / row;
+}
+
+void decode_attention_fp8(const void* q, int ldq, const KvFp8& c, const int* block_tables, int max_blocks,
+                          const int* ctx_lens, void* out, int ldo, int B, int Hq, float scale, float* ws, long ws_rows,
+                          int sms, int* status, cudaStream_t s) {
+  if (B == 0) return;
+  const int G = Hq / c.Hkv;
+  const int ctas = decode_fp8_ctas(sms);
+  // the partial results sit at the front, the counters behind them: neither moves with the batch
+  uint32_t* counters = reinterpret_cast<uint32_t*>(ws + 2L * ctas * G * DEC8_ROW);
+  const int nt = G > 8 ? 2 : 1;
+  const long most = ((long)B * c.Hkv * max_blocks + dec8::MIN_BLOCKS - 1) / dec8::MIN_BLOCKS;
+  const int grid = (int)std::max(1L, std::min((long)ctas, most));
+  const int smem = (dec8::WARPS * 8 * nt * (dec8::D + 4)) * 4 + (B + 1) * 4;
+  auto kern = nt == 2 ? decode_attn_fp8_kernel<2> : decode_attn_fp8_kernel<1>;
+  static bool attr[64][2] = {};
+  int dev;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63][nt - 1]) {
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         (dec8::WARPS * 8 * nt * (dec8::D + 4)) * 4 + (DEC8_MAX_BATCH + 1) * 4);
+    attr[dev & 63][nt - 1] = true;
+  }
+  kern<<<grid, dec8::THREADS, smem, s>>>(reinterpret_cast<const __nv_bfloat16*>(q), ldq, c, block_tables, max_blocks,
+                                         ctx_lens, reinterpret_cast<__nv_bfloat16*>(out), ldo, B, Hq,
+                                         scale * 1.4426950408889634f, ws, counters, status);
+}
+
+// ------------------------------------------------------------ block copies
+// A CTA moves one pair's block in a run of planes.  A pair whose destination
+// is another pair's source, or the destination of another source, has no
+// defined result: it is left out and recorded.  The check is a scan of the
+// pairs while the first plane's bytes are in flight.
+namespace kvc {
+constexpr int THREADS = 256;
+}
+__global__ void __launch_bounds__(kvc::THREADS)
+    kv_copy_blocks_kernel(uint8_t* kv, float* scales, const int* __restrict__ pairs, int n, int planes, int per,
+                          int num_blocks, int64_t block_bytes, int Hkv, int* status) {
+  const int i = blockIdx.x, tid = threadIdx.x;
+  const int src = pairs[2 * i], dst = pairs[2 * i + 1];
+  const int p0 = blockIdx.y * per, p1 = min(planes, p0 + per);
+  if (src < 0 || src >= num_blocks || dst < 0 || dst >= num_blocks) {
+    if (tid == 0) record_status(status, CX_ERR_BOUNDS);
+    return;
+  }
+  if (src == dst) return;
+  bool bad = false;
+  for (int k = tid; k < n; k += kvc::THREADS) {
+    const int s = pairs[2 * k], d = pairs[2 * k + 1];
+    bad |= (s == dst && d != dst) || (d == dst && s != src);
+  }
+  if (__syncthreads_or(bad)) {
+    if (tid == 0) record_status(status, CX_ERR_BOUNDS);
+    return;
+  }
+  const int64_t nv = block_bytes >> 4;
+  for (int p = p0; p < p1; ++p) {
+    const uint8_t* a = kv + ((int64_t)p * num_blocks + src) * block_bytes;
+    uint8_t* b = kv + ((int64_t)p * num_blocks + dst) * block_bytes;
+    for (int64_t v = tid; v < nv; v += 8 * kvc::THREADS) {
+      u128 r[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v + e * kvc::THREADS < nv) r[e] = ld_nc_v4(a + (v + e * kvc::THREADS) * 16);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v + e * kvc::THREADS < nv) st_cs_v4(b + (v + e * kvc::THREADS) * 16, r[e]);
+    }
+    if (scales != nullptr)
+      for (int h = tid; h < Hkv; h += kvc::THREADS)
+        scales[((int64_t)p * num_blocks + dst) * Hkv + h] = scales[((int64_t)p * num_blocks + src) * Hkv + h];
+  }
+}
+
+void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes, int num_blocks, int64_t block_bytes,
+                    int Hkv, int sms, int* status, cudaStream_t s) {
+  if (n == 0 || planes == 0) return;
+  const long want = 8L * sms;
+  const int per = (int)std::max(1L, std::min((long)planes, (long)n * planes / want));
+  kv_copy_blocks_kernel<<<dim3(n, (planes + per - 1) / per), kvc::THREADS, 0, s>>>(
+      reinterpret_cast<uint8_t*>(kv), scales, pairs, n, planes, per, num_blocks, block_bytes, Hkv, status);
+}
+
+// --------------------------------------------------------- dequantised blocks
+__global__ void __launch_bounds__(256)
+    kv_dequant_kernel(KvFp8 c, const int* __restrict__ table, __nv_bfloat16* ko, __nv_bfloat16* vo, int* status) {
+  using namespace kvq;
+  const int i = blockIdx.x, h = blockIdx.y, id = table[i];
+  if (id < 0 || id >= c.num_blocks) {
+    if (threadIdx.x == 0) record_status(status, CX_ERR_BOUNDS);
+    return;
+  }
+  const size_t at = ((size_t)id * c.Hkv + h) * (BS * D), to = ((size_t)i * c.Hkv + h) * (BS * D);
+  const int half = threadIdx.x >> 7, e = (threadIdx.x & 127) * 16;
+  const u128 raw = ld_nc_v4((half ? c.v : c.k) + at + e);
+  const float f = (half ? c.vs : c.ks)[(size_t)id * c.Hkv + h];
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
+  u128 o[2];
+  uint32_t* po = reinterpret_cast<uint32_t*>(o);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t a = e4m3x2_to_f16x2((uint16_t)w[k]), b = e4m3x2_to_f16x2((uint16_t)(w[k] >> 16));
+    po[2 * k] = pack_bf16x2(f16_lo(a) * f, f16_hi(a) * f);
+    po[2 * k + 1] = pack_bf16x2(f16_lo(b) * f, f16_hi(b) * f);
+  }
+  __nv_bfloat16* d = (half ? vo : ko) + to + e;
+  st_v4(d, o[0]);
+  st_v4(d + 8, o[1]);
+}
+
+void kv_dequant_blocks(const KvFp8& c, const int* table, int n, void* kout, void* vout, int* status, cudaStream_t s) {
+  if (n == 0) return;
+  kv_dequant_kernel<<<dim3(n, c.Hkv), 256, 0, s>>>(c, table, reinterpret_cast<__nv_bfloat16*>(kout),
+                                                   reinterpret_cast<__nv_bfloat16*>(vout), status);
+}
+
+}  // namespace cx

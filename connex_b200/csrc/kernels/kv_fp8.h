@@ -1,0 +1,49 @@
+// Host entry points of the 8-bit paged KV cache kernels (kv_fp8.cu).
+//
+// A cache holds e4m3 values [blocks, Hkv, 16, 128] and one fp32 scale per
+// (block, KV head) [blocks, Hkv], a power of two, for K and for V each: a
+// cached element stands for value * scale.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace cx {
+
+struct KvFp8 {
+  uint8_t* k;
+  uint8_t* v;
+  float* ks;
+  float* vs;
+  int num_blocks, Hkv;
+};
+
+// Rows of the fused QKV buffer [T, (Hq + 2 Hkv) * 128] (ld ldq): q rotated
+// into out [T, Hq * 128] (ld ldo; may be the q columns of qkv), k rotated and
+// v quantised into the slots' blocks (slot < 0: not cached).
+void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_sin, const int64_t* slots,
+                    const KvFp8& c, void* out, int ldo, int T, int Hq, int max_pos, int* status, cudaStream_t s,
+                    const void* q_norm, const void* k_norm, float eps);
+
+// Rows of one call that are handled together; longer calls run as successive launches.
+constexpr int KVQ_MAX_ROWS = 8192;
+
+// One query row per sequence over its cached tokens.  ws: fp32
+// [decode_fp8_rows(sms, B, Hkv, G), G * DEC8_ROW], zero before its first use
+// (each call leaves its counters zero).
+constexpr int DEC8_ROW = 132;        // floats of one head's partial result
+constexpr int DEC8_MAX_BATCH = 4096;
+int decode_fp8_ctas(int sms);
+long decode_fp8_rows(int sms, int B, int Hkv, int G);
+void decode_attention_fp8(const void* q, int ldq, const KvFp8& c, const int* block_tables, int max_blocks,
+                          const int* ctx_lens, void* out, int ldo, int B, int Hq, float scale, float* ws, long ws_rows,
+                          int sms, int* status, cudaStream_t s);
+
+// Blocks pairs[i] = (source, destination) of every plane [planes, num_blocks,
+// block_bytes] and, where given, of the scales [planes, num_blocks, Hkv].
+void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes, int num_blocks, int64_t block_bytes,
+                    int Hkv, int sms, int* status, cudaStream_t s);
+
+// e4m3 blocks table[i] -> bf16 blocks i of kout / vout [n, Hkv, 16, 128].
+void kv_dequant_blocks(const KvFp8& c, const int* table, int n, void* kout, void* vout, int* status, cudaStream_t s);
+
+}  // namespace cx

@@ -272,6 +272,100 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return out
 
 
+# ------------------------------------------------------ 8-bit KV cache
+def rope_cache_fp8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, n_q_heads: int,
+                   n_kv_heads: int, slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   k_scale: torch.Tensor, v_scale: torch.Tensor, out: Optional[torch.Tensor] = None,
+                   status: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
+                   k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+    """Rotate q and k of the fused QKV rows and quantise k and v into an 8-bit
+    paged cache; returns the rotated q [T, Hq * 128] (``out``; may be
+    ``qkv[:, :Hq * 128]``).  ``qkv``'s k and v columns stay as they are.
+
+    ``k_cache`` / ``v_cache``: float8_e4m3fn [blocks, Hkv, 16, 128];
+    ``k_scale`` / ``v_scale``: fp32 [blocks, Hkv], powers of two: a cached
+    element stands for value * scale.  A block's scale is the smallest that
+    holds its largest finite element within +-448.  When a call writes row 0
+    of a block the block starts anew; otherwise its scale may only grow, and
+    the rows it holds are then requantised.  Infinities and NaN are stored as
+    NaN.  A row with slot < 0 is not cached; one with a position or slot out
+    of range is not cached either and recorded in ``status`` (a position out
+    of range also gives a q of zeros).  Of two rows for the same slot the
+    later wins.  More than 8192 rows run as successive calls of 8192.
+    ``q_norm`` / ``k_norm`` as in :func:`rope_cache`."""
+    if out is None:
+        out = torch.empty(qkv.shape[0], n_q_heads * 128, dtype=qkv.dtype, device=qkv.device)
+    _C.rope_cache_fp8(qkv, positions, cos_sin, slot_mapping, k_cache, v_cache, k_scale, v_scale, out, n_q_heads,
+                      n_kv_heads, status, q_norm, k_norm, eps)
+    _n(-(-qkv.shape[0] // 8192))
+    return out
+
+
+def decode_workspace_fp8(batch: int, n_q_heads: int, n_kv_heads: int, device) -> torch.Tensor:
+    """Workspace of :func:`decode_attention_fp8` for up to ``batch`` sequences:
+    zero before its first use, and left ready for the next call.  Calls that
+    may run at the same time (on different streams, or graphs replayed side
+    by side) each need their own."""
+    device = torch.device(device)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    if n_kv_heads <= 0 or n_q_heads <= 0 or n_q_heads % n_kv_heads:
+        raise ValueError("decode_workspace_fp8: the query heads must be a multiple of the KV heads")
+    g = n_q_heads // n_kv_heads
+    return torch.zeros(_C.decode_fp8_rows(index, batch, n_kv_heads, g), g * _C.DECODE_FP8_ROW, dtype=torch.float32,
+                       device=device)
+
+
+def decode_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                         v_scale: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor, n_q_heads: int,
+                         workspace: torch.Tensor, out: Optional[torch.Tensor] = None,
+                         scale: Optional[float] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One query row per sequence over its 8-bit paged cache (see
+    :func:`rope_cache_fp8`; scales must be powers of two), up to 16 query
+    heads per KV head.  ``q`` [B, >= Hq * 128] (q heads first), ``ctx_lens``
+    [B] tokens to attend to (0: a row of zeros), ``block_tables``
+    [B, max_blocks].  The work is divided on the device from ``ctx_lens``, so
+    a captured call stays balanced for any lengths.  A block id out of range
+    is left out, and a length beyond the table cut, both recorded in
+    ``status``."""
+    if out is None:
+        out = torch.empty(q.shape[0], n_q_heads * 128, dtype=q.dtype, device=q.device)
+    _C.decode_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, out, n_q_heads,
+                            scale if scale is not None else 1.0 / math.sqrt(128), workspace, status)
+    _n()
+    return out
+
+
+def prefill_attention_paged_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
+                                tile_info: torch.Tensor, n_q_heads: int, n_kv_heads: int,
+                                out: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                                status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`prefill_attention_paged` over an 8-bit cache: causal attention of
+    prompt chunks, ``q`` [T, Hq * 128] rotated, keys and values of the whole
+    context -- this chunk's included -- from the cache."""
+    width = block_tables.shape[1]
+    n = block_tables.numel()
+    k = torch.empty(n, n_kv_heads, 16, 128, dtype=q.dtype, device=q.device)
+    v = torch.empty_like(k)
+    _C.kv_dequant_blocks(k_cache, v_cache, k_scale, v_scale, block_tables, k, v, status)
+    table = torch.arange(n, dtype=torch.int32, device=q.device).view(-1, width)
+    pad = torch.nn.functional.pad(q, (0, 2 * n_kv_heads * 128))
+    _n()
+    return prefill_attention_paged(pad, k, v, table, tile_info, n_q_heads, n_kv_heads, out, scale, status)
+
+
+def kv_copy_blocks(kv: torch.Tensor, pairs: torch.Tensor, scales: Optional[torch.Tensor] = None,
+                   status: Optional[torch.Tensor] = None) -> None:
+    """Copy blocks inside a paged cache, all layers in one launch:
+    ``kv[:, :, dst] = kv[:, :, src]`` for the rows (src, dst) of ``pairs``
+    (int32 [n, 2]), and the same for ``scales`` [layers, 2, blocks, Hkv] of an
+    8-bit cache.  The copies are one step, so a destination may be neither
+    another pair's source nor the destination of another source: such pairs,
+    and ids out of range, are left out and recorded in ``status``."""
+    _C.kv_copy_blocks(kv, pairs, scales, status)
+    _n()
+
+
 # ------------------------------------------------------- peer memory
 def kv_push_layer(src_k: int, src_v: int, dst_k: int, dst_v: int, pairs: torch.Tensor, *,
                   src_heads: int, dst_heads: int, src_h0: int = 0, dst_h0: int = 0,

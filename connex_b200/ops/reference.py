@@ -108,6 +108,76 @@ def paged_prefill_attention(q, k_cache, v_cache, block_tables, ctx, n_new, scale
     return out
 
 
+# ---- 8-bit KV cache (64-bit arithmetic)
+def fp8_values(cache, scale):
+    """What an 8-bit cache [blocks, Hkv, BS, D] with scales [blocks, Hkv] stands for."""
+    return cache.double() * scale.double()[..., None, None]
+
+
+def fp8_scale(amax):
+    """The smallest power of two s >= 2^-100 with amax <= 448 s."""
+    m, p = torch.frexp(amax.double())
+    e = (p - 9 + (m > 0.875).to(p.dtype)).clamp(min=-100)
+    return torch.ldexp(torch.ones_like(m), torch.where(amax > 0, e, torch.full_like(e, -100)))
+
+
+def fp8_append(cache, scale, rows, slots):
+    """In place: ``rows`` [T, Hkv, D] (bf16) into their slots; a block whose row
+    0 is written starts anew, any other keeps at least its scale and its
+    other rows; the later of two rows for a slot wins, slots < 0 are skipped."""
+    BS = cache.shape[2]
+    by = {}
+    for t, s in enumerate(slots.tolist()):
+        if s >= 0:
+            by.setdefault(s // BS, {})[s % BS] = t
+    for b, at in by.items():
+        off, tok = torch.tensor(list(at), device=rows.device), torch.tensor(list(at.values()), device=rows.device)
+        x = rows[tok].double()                                          # [n, Hkv, D]
+        amax = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x)).amax((0, 2))
+        new = fp8_scale(amax)
+        if 0 not in at:
+            old = scale[b].double()
+            new = torch.maximum(new, old)
+            cache[b] = (cache[b].double() * (old / new)[:, None, None]).float().to(cache.dtype)
+        x = torch.where(torch.isfinite(x), x, torch.full_like(x, math.nan)) / new[None, :, None]
+        cache[b].view(torch.uint8)[:, off] = x.float().to(cache.dtype).view(torch.uint8).transpose(0, 1)
+        scale[b] = new.float()
+
+
+def paged_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx, n_new, scale=None):
+    """Causal attention of ``n_new[i]`` query rows of each sequence behind
+    ``ctx[i]`` cached tokens: q [T, Hq, D] -> [T, Hq, D] fp64, and the same
+    sums over |v| (the size that rounding errors of the weights act on)."""
+    T, Hq, D = q.shape
+    Hkv, BS = k_cache.shape[1], k_cache.shape[2]
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    out = torch.zeros(T, Hq, D, dtype=torch.float64, device=q.device)
+    mag = torch.zeros_like(out)
+    s = 0
+    for b, (c, n) in enumerate(zip(ctx, n_new)):
+        tot = c + n
+        if tot > 0 and n > 0:
+            ids = block_tables[b, :(tot + BS - 1) // BS].long()
+            k, v = (fp8_values(x.view(torch.uint8)[ids].view(x.dtype), z[ids]).transpose(0, 1).reshape(Hkv, -1, D)[:, :tot]
+                    .repeat_interleave(Hq // Hkv, 0) for x, z in ((k_cache, k_scale), (v_cache, v_scale)))
+            a = (q[s:s + n].double().transpose(0, 1) @ k.transpose(1, 2)) * scale
+            late = torch.arange(tot, device=q.device) > (c + torch.arange(n, device=q.device))[:, None]
+            p = a.masked_fill(late, float("-inf")).softmax(-1)
+            out[s:s + n] = (p @ v).transpose(0, 1)
+            mag[s:s + n] = (p @ v.abs()).transpose(0, 1)
+        s += n
+    return out, mag
+
+
+def kv_copy_blocks(kv, pairs, scales=None):
+    """In-place reference of kv_copy_blocks on plain tensors."""
+    src, dst = pairs[:, 0].long(), pairs[:, 1].long()
+    raw = kv.view(torch.uint8) if kv.element_size() == 1 else kv
+    raw[:, :, dst] = raw[:, :, src]
+    if scales is not None:
+        scales[:, :, dst] = scales[:, :, src]
+
+
 def kv_push(src_k, src_v, dst_k, dst_v, pairs, src_h0=0, dst_h0=0, n_heads=None):
     """In-place reference of kv_push_layer on plain tensors."""
     nh = n_heads if n_heads is not None else src_k.shape[1]

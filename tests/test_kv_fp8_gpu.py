@@ -1,0 +1,484 @@
+"""The 8-bit paged KV cache on the GPU: the quantising write, decode and
+chunked prefill attention over it and block copies, each against a plain
+64-bit statement.
+
+Tolerances.  One rounding to a type t is off by at most eps(t) / 2 of the
+value: bf16 2^-8, f16 2^-11, fp32 2^-24, e4m3 2^-4 (and half of its smallest
+step, 2^-10 of the scale, below the normal range)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+D, BS = 128, 16
+U_BF16, U_F16, U_F32, U_E4M3 = 2.0 ** -8, 2.0 ** -11, 2.0 ** -24, 2.0 ** -4
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return torch.device("cuda", 0)
+
+
+def _g(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+def _cache(nb, hkv, dev, seed, lo=-8, hi=-4):
+    g = _g(dev, seed)
+    x = (torch.randn(nb, hkv, BS, D, generator=g, device=dev) * 60).clamp(-448, 448).to(torch.float8_e4m3fn)
+    e = torch.randint(lo, hi, (nb, hkv), generator=g, device=dev)
+    return x, torch.ldexp(torch.ones(nb, hkv, device=dev), e).float()
+
+
+def _nan_rows(cache, table, lens):
+    """Cache rows behind each sequence's last token hold NaN bytes."""
+    raw = cache.view(torch.uint8)
+    for b, n in enumerate(lens):
+        if n % BS:
+            raw[int(table[b, n // BS]), :, n % BS:] = 0x7F
+        elif n == 0:
+            raw[int(table[b, 0])] = 0xFF
+
+
+def _table(lens, dev, seed, width=None):
+    need = [max(1, -(-n // BS)) for n in lens]
+    perm = torch.randperm(sum(need) + 3, generator=_g(dev, seed), device=dev).to(torch.int32)
+    w = width or max(need)
+    t = torch.full((len(lens), w), -1, dtype=torch.int32, device=dev)   # ids behind the end are never read
+    at = 0
+    for b, n in enumerate(need):
+        t[b, :n] = perm[at:at + n]
+        at += n
+    return t, sum(need) + 3
+
+
+def _attention_tolerance(ref, mag, q, k_cache, k_scale, table, ctx, n_new, u_weight, vmax):
+    """|out - ref| <= bf16 of the result + the weights' rounding (u_weight, and
+    f16's smallest half step for each) + the logits' fp32 sums (128 products:
+    128 * 2^-24 of sum |q_i k_i| each, twice: the weight and the sum)."""
+    from connex_b200.ops import reference as R
+    big, s = [], 0
+    hkv = k_cache.shape[1]
+    for b, (c, n) in enumerate(zip(ctx, n_new)):
+        if c + n == 0 or n == 0:
+            s += n
+            continue
+        ids = table[b, :-(-(c + n) // BS)].long()
+        k = R.fp8_values(k_cache.view(torch.uint8)[ids].view(k_cache.dtype), k_scale[ids]).nan_to_num(0.0)
+        k = k.transpose(0, 1).reshape(hkv, -1, D)[:, :c + n].abs().repeat_interleave(q.shape[1] // hkv, 0)
+        qs = q[s:s + n].double().abs().transpose(0, 1)
+        big.append((qs @ k.transpose(1, 2)).max().item() / math.sqrt(D))
+        s += n
+    logit = (max(big) if big else 0.0) * D * U_F32
+    n = max([c + m for c, m in zip(ctx, n_new)] + [1])
+    return U_BF16 * ref.abs() + mag * (2 * u_weight + 4 * logit + n * U_F32 + 2.0 ** -20) + n * 2.0 ** -25 * vmax
+
+
+DECODE_LENS = [[1], [0, 5, 0], [16], [17, 1, 15, 16, 31, 33], [500], [4096, 3, 0, 1000], [129] * 70, [20000, 1]]
+
+
+@pytest.mark.parametrize("heads", [(32, 8), (8, 8), (6, 2), (7, 1), (16, 1), (20, 2), (32, 4)])
+@pytest.mark.parametrize("lens", DECODE_LENS, ids=lambda v: f"{len(v)}x{max(v)}")
+def test_decode_attention(dev, heads, lens):
+    from connex_b200 import ops
+    from connex_b200.ops import reference as R
+    hq, hkv = heads
+    table, nb = _table(lens, dev, 1)
+    k, ks = _cache(nb, hkv, dev, 2)
+    v, vs = _cache(nb, hkv, dev, 3, -12, 3)
+    _nan_rows(k, table, lens)
+    _nan_rows(v, table, lens)
+    B = len(lens)
+    # q as a slice of wider rows, as the fused projection leaves it
+    wide = (torch.randn(B, (hq + 2) * D, generator=_g(dev, 4), device=dev) * 1.5).to(torch.bfloat16)
+    q = wide[:, :hq * D]
+    st = ops.new_status(dev)
+    ws = ops.decode_workspace_fp8(B, hq, hkv, dev)
+    lt = torch.tensor(lens, dtype=torch.int32, device=dev)
+    out = ops.decode_attention_fp8(wide, k, v, ks, vs, table, lt, hq, ws, status=st)
+    torch.cuda.synchronize()
+    ops.check_status(st, "decode_attention_fp8")
+    ctx = [max(0, n - 1) for n in lens]
+    live = torch.tensor([n > 0 for n in lens], device=dev)
+    got = out.view(B, hq, D).double()
+    assert torch.equal(got[~live], torch.zeros_like(got[~live]))
+    rows = q.reshape(B, hq, D)[live]
+    tl = table[live]
+    ref, mag = R.paged_attention_fp8(rows, k, v, ks, vs, tl, [c for c, n in zip(ctx, lens) if n], [1] * int(live.sum()))
+    tol = _attention_tolerance(ref, mag, rows, k, ks, tl, [c for c, n in zip(ctx, lens) if n], [1] * int(live.sum()),
+                               U_F16, float(vs.max()) * 448)
+    assert ((got[live] - ref).abs() <= tol).all(), float(((got[live] - ref).abs() / tol).max())
+    # the workspace is left ready: the same call again, the same bits
+    again = ops.decode_attention_fp8(wide, k, v, ks, vs, table, lt, hq, ws)
+    assert torch.equal(again.view(torch.int16), out.view(torch.int16))
+
+
+PREFILL_ROWS = [[(0, 100)], [(64, 128)], [(1000, 300), (17, 5)], [(2000, 1), (130, 513)], [(5, 64), (0, 200), (3999, 129)],
+                [(2048, 600)], [(7, 9), (0, 1), (15, 1), (16, 1)], [(300, 0), (41, 30)]]
+
+
+@pytest.mark.parametrize("heads", [(8, 2), (3, 3), (7, 1), (16, 1)])
+@pytest.mark.parametrize("rows", PREFILL_ROWS, ids=lambda v: "_".join(f"{c}+{n}" for c, n in v))
+def test_prefill_attention(dev, heads, rows):
+    from connex_b200 import ops
+    from connex_b200.ops import reference as R
+    hq, hkv = heads
+    ctx, new = [c for c, _ in rows], [n for _, n in rows]
+    lens = [c + n for c, n in rows]
+    table, nb = _table(lens, dev, 5)
+    table.clamp_(min=0)
+    k, ks = _cache(nb, hkv, dev, 6)
+    v, vs = _cache(nb, hkv, dev, 7, -10, -2)
+    _nan_rows(k, table, lens)
+    _nan_rows(v, table, lens)
+    T = sum(new)
+    q = (torch.randn(T, hq * D, generator=_g(dev, 8), device=dev) * 1.5).to(torch.bfloat16)
+    st = ops.new_status(dev)
+    ti = ops.prefill_tile_info(new, dev, ctx=ctx)
+    out = ops.prefill_attention_paged_fp8(q, k, v, ks, vs, table, ti, hq, hkv, status=st)
+    torch.cuda.synchronize()
+    ops.check_status(st, "prefill_attention_paged_fp8")
+    ref, mag = R.paged_attention_fp8(q.view(T, hq, D), k, v, ks, vs, table, ctx, new)
+    tol = _attention_tolerance(ref, mag, q.view(T, hq, D), k, ks, table, ctx, new, U_BF16, float(vs.max()) * 448)
+    err = (out.view(T, hq, D).double() - ref).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+def _write_case(dev, rows, hq, hkv, seed, norm=False, spread=3.0):
+    """A cache that holds each sequence's first ctx tokens, and n new rows."""
+    from connex_b200 import ops
+    lens = [c + n for c, n in rows]
+    table, nb = _table(lens, dev, seed)
+    k, ks = _cache(nb, hkv, dev, seed + 1, -9, -4)
+    v, vs = _cache(nb, hkv, dev, seed + 2, -9, -4)
+    pos = [p for c, n in rows for p in range(c, c + n)]
+    slots = [int(table[b, p // BS]) * BS + p % BS for b, (c, n) in enumerate(rows) for p in range(c, c + n)]
+    g = _g(dev, seed + 3)
+    mag = torch.exp2(torch.rand(hq + 2 * hkv, 1, generator=g, device=dev) * 2 * spread - spread)
+    qkv = (torch.randn(len(pos), hq + 2 * hkv, D, generator=g, device=dev) * mag).to(torch.bfloat16).view(len(pos), -1)
+    cs = ops.rope_cos_sin(max(lens), D, 5e5, dev)
+    w = [(torch.rand(D, generator=g, device=dev) + 0.5).to(torch.bfloat16) for _ in range(2)] if norm else [None, None]
+    return dict(k=k, ks=ks, v=v, vs=vs, pos=torch.tensor(pos, dtype=torch.int32, device=dev),
+                slots=torch.tensor(slots, dtype=torch.int64, device=dev), qkv=qkv, cs=cs, qn=w[0], kn=w[1], nb=nb)
+
+
+def _turned(x, pos, cs, w):
+    """Rotated rows in 64 bits, and a bound on what a flip of the norm's bf16 rounding moves them."""
+    x = x.double()
+    slack = torch.zeros_like(x)
+    if w is not None:
+        x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6) * w.double()
+        x = x.to(torch.bfloat16).double()
+        pair = x.abs() + x.abs().roll(D // 2, -1)
+        slack = 2 * U_BF16 * pair
+    t = cs.double()[pos.long()][:, None]
+    c, s = t[..., :D // 2], t[..., D // 2:]
+    a, b = x[..., :D // 2], x[..., D // 2:]
+    # two products and a sum in fp32
+    slack = slack + 4 * U_F32 * (x.abs() + x.abs().roll(D // 2, -1))
+    return torch.cat([a * c - b * s, b * c + a * s], -1), slack
+
+
+WRITE_ROWS = [[(0, 1)], [(0, 16)], [(15, 1)], [(16, 1)], [(37, 1), (100, 1), (0, 1), (15, 1)], [(0, 33), (7, 9), (5, 70)],
+              [(1000, 129)], [(3, 2), (20, 40), (0, 300)], [(i, 1) for i in range(70)]]
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("heads", [(8, 2), (3, 3), (7, 1), (32, 8), (20, 5)])
+@pytest.mark.parametrize("rows", WRITE_ROWS, ids=lambda v: f"{len(v)}x{v[0][0]}+{v[0][1]}")
+def test_write(dev, rows, heads, norm):
+    from connex_b200 import ops
+    from connex_b200.ops import reference as R
+    hq, hkv = heads
+    s = _write_case(dev, rows, hq, hkv, 11, norm)
+    T = s["qkv"].shape[0]
+    x = s["qkv"].view(T, hq + 2 * hkv, D)
+    before = {n: s[n].clone() for n in ("k", "ks", "v", "vs", "qkv")}
+    st = ops.new_status(dev)
+    q = ops.rope_cache_fp8(s["qkv"], s["pos"], s["cs"], hq, hkv, s["slots"], s["k"], s["v"], s["ks"], s["vs"], status=st,
+                           q_norm=s["qn"], k_norm=s["kn"])
+    torch.cuda.synchronize()
+    ops.check_status(st, "rope_cache_fp8")
+    assert torch.equal(s["qkv"], before["qkv"])
+    ref, slack = _turned(x[:, :hq], s["pos"], s["cs"], s["qn"])
+    err = (q.view(T, hq, D).double() - ref).abs()
+    assert (err <= U_BF16 * ref.abs() + 2 * slack).all()
+    # v is quantised as it stands: the very bytes and scales
+    v, vs = before["v"].clone(), before["vs"].clone()
+    R.fp8_append(v, vs, x[:, hq + hkv:], s["slots"])
+    assert torch.equal(vs, s["vs"])
+    touched = torch.zeros(s["nb"], dtype=torch.bool, device=dev)
+    touched[s["slots"] // BS] = True
+    assert torch.equal(v.float(), s["v"].float())
+    assert torch.equal(before["v"][~touched].view(torch.uint8), s["v"][~touched].view(torch.uint8))
+    assert torch.equal(before["k"][~touched].view(torch.uint8), s["k"][~touched].view(torch.uint8))
+    assert torch.equal(before["ks"][~touched], s["ks"][~touched])
+    # k: each row within half an e4m3 step of its rotated value, held by its scale
+    kr, ks_ = _turned(x[:, hq:hq + hkv], s["pos"], s["cs"], s["kn"])
+    val = R.fp8_values(s["k"], s["ks"])
+    blk, off = s["slots"] // BS, s["slots"] % BS
+    got, sc = val[blk, :, off], s["ks"].double()[blk][..., None]
+    tol = (1 + 2 * U_BF16) * (U_E4M3 * kr.abs()).maximum(2.0 ** -10 * sc) + U_BF16 * kr.abs() + 2 * ks_
+    assert ((got - kr).abs() <= tol).all()
+    # the scale is the smallest that holds the rows (or the old one, where the block goes on)
+    low = torch.zeros(s["nb"], hkv, dtype=torch.float64, device=dev).index_reduce_(0, blk, (kr.abs() * (1 - 2 * U_BF16) - 2 * ks_).amax(-1), "amax")
+    top = torch.zeros(s["nb"], hkv, dtype=torch.float64, device=dev).index_reduce_(0, blk, (kr.abs() * (1 + 2 * U_BF16) + 2 * ks_).amax(-1), "amax")
+    fresh = torch.zeros(s["nb"], dtype=torch.bool, device=dev)
+    fresh[blk[off == 0]] = True
+    old = torch.where(fresh[:, None], torch.zeros_like(low), before["ks"].double())
+    assert (s["ks"].double() >= torch.maximum(R.fp8_scale(low), old))[touched].all()
+    assert (s["ks"].double() <= torch.maximum(R.fp8_scale(top), old))[touched].all()
+    # rows that the call did not write keep their values, to half the smallest step of a raised scale
+    kept = torch.ones(s["nb"], BS, dtype=torch.bool, device=dev)
+    kept[blk, off] = False
+    kept &= touched[:, None] & ~fresh[:, None]
+    was = R.fp8_values(before["k"], before["ks"])
+    d = (val - was).abs().transpose(1, 2)[kept]
+    room = (2.0 ** -10 * s["ks"].double() * (s["ks"] != before["ks"]))[:, None, :, None].expand(-1, BS, -1, D)[kept]
+    assert (d <= room).all()
+
+
+def test_write_order_repeats_and_skips(dev):
+    """Rows of one block apart from each other, a slot written twice, slots below zero."""
+    from connex_b200 import ops
+    from connex_b200.ops import reference as R
+    hq, hkv, nb = 4, 2, 40
+    k, ks = _cache(nb, hkv, dev, 21)
+    v, vs = _cache(nb, hkv, dev, 22)
+    slots = [5 * BS + 3, 7 * BS, 5 * BS + 4, 7 * BS + 1, -1, 5 * BS + 3, 9 * BS + 15, 7 * BS, -7, 5 * BS + 2]
+    T = len(slots)
+    qkv = torch.randn(T, (hq + 2 * hkv) * D, generator=_g(dev, 23), device=dev).to(torch.bfloat16) * 4
+    pos = torch.arange(T, dtype=torch.int32, device=dev)
+    cs = ops.rope_cos_sin(64, D, 1e4, dev)
+    st = ops.new_status(dev)
+    rv, rvs = v.clone(), vs.clone()
+    sl = torch.tensor(slots, dtype=torch.int64, device=dev)
+    ops.rope_cache_fp8(qkv, pos, cs, hq, hkv, sl, k, v, ks, vs, status=st)
+    ops.check_status(st)
+    R.fp8_append(rv, rvs, qkv.view(T, -1, D)[:, hq + hkv:], sl)
+    assert torch.equal(vs, rvs) and torch.equal(v.float(), rv.float())
+
+
+def test_write_out_of_range(dev):
+    """Bad slots and positions are recorded, cached nowhere, and change nothing else."""
+    from connex_b200 import ops
+    hq, hkv, nb = 4, 2, 6
+    for slots, pos in (([nb * BS, 0], [0, 1]), ([0, 16], [64, 1]), ([0, 1], [3, -1]), ([1 << 40, 5], [0, 0])):
+        k, ks = _cache(nb, hkv, dev, 31)
+        v, vs = _cache(nb, hkv, dev, 32)
+        good = [0 <= s < nb * BS and 0 <= p < 64 for s, p in zip(slots, pos)]
+        qkv = torch.randn(2, (hq + 2 * hkv) * D, generator=_g(dev, 33), device=dev).to(torch.bfloat16)
+        st = ops.new_status(dev)
+        k0, v0 = k.clone(), v.clone()
+        cs = ops.rope_cos_sin(64, D, 1e4, dev)
+        q = ops.rope_cache_fp8(qkv, torch.tensor(pos, dtype=torch.int32, device=dev), cs, hq, hkv,
+                               torch.tensor(slots, dtype=torch.int64, device=dev), k, v, ks, vs, status=st)
+        with pytest.raises(RuntimeError, match="bounds"):
+            ops.check_status(st)
+        assert torch.isfinite(q.float()).all()
+        hit = {s // BS for s, g in zip(slots, good) if g}
+        for b in range(nb):
+            if b not in hit:
+                assert torch.equal(k[b].view(torch.uint8), k0[b].view(torch.uint8))
+                assert torch.equal(v[b].view(torch.uint8), v0[b].view(torch.uint8))
+        for i, p in enumerate(pos):
+            if not 0 <= p < 64:
+                assert not q[i].any()
+
+
+def test_write_special_values(dev):
+    """NaN and infinities are stored as NaN and leave the scale alone; zeros take the smallest scale."""
+    from connex_b200 import ops
+    hq, hkv, nb = 2, 1, 4
+    k, ks = _cache(nb, hkv, dev, 41)
+    v, vs = _cache(nb, hkv, dev, 42)
+    qkv = torch.zeros(3, (hq + 2 * hkv) * D, device=dev, dtype=torch.bfloat16)
+    qkv[0, -D:] = 3.0
+    qkv[0, -D] = float("inf")
+    qkv[0, -D + 1] = float("nan")
+    qkv[0, -D + 2] = float("-inf")
+    qkv[2, -D:] = torch.finfo(torch.bfloat16).max
+    cs = ops.rope_cos_sin(64, D, 1e4, dev)
+    i32 = torch.tensor([0, 1, 2], dtype=torch.int32, device=dev)
+    ops.rope_cache_fp8(qkv, i32, cs, hq, hkv, torch.tensor([0, 16, 32], dtype=torch.int64, device=dev), k, v, ks, vs)
+    row = v[0, 0, 0].float()
+    assert torch.isnan(row[:3]).all() and torch.equal(row[3:] * vs[0, 0], torch.full((D - 3,), 3.0, device=dev))
+    assert float(vs[1, 0]) == 2.0 ** -100 and not v[1, 0, 0].float().any()
+    # the largest bf16 is 1.992 * 2^127: in steps of 2^124 the nearest e4m3 value is 2^128, so the scale is 2^120
+    assert float(vs[2, 0]) == 2.0 ** 120 and torch.equal(v[2, 0, 0].float(), torch.full((D,), 256.0, device=dev))
+
+
+def test_write_long_call(dev):
+    """Past 8192 rows a call runs as successive ones; a block at the seam holds both parts."""
+    from connex_b200 import ops
+    from connex_b200.ops import reference as R
+    hq, hkv, T = 1, 1, 8192 + 40
+    nb = T // BS + 4
+    k, ks = _cache(nb, hkv, dev, 51)
+    v, vs = _cache(nb, hkv, dev, 52)
+    qkv = torch.randn(T, 3 * D, generator=_g(dev, 53), device=dev).to(torch.bfloat16)
+    slots = torch.arange(5, T + 5, device=dev)
+    pos = torch.arange(T, dtype=torch.int32, device=dev)
+    rv, rvs = v.clone(), vs.clone()
+    ops.rope_cache_fp8(qkv, pos, ops.rope_cos_sin(T, D, 1e4, dev), hq, hkv, slots, k, v, ks, vs)
+    rows = qkv.view(T, 3, D)[:, 2:]
+    R.fp8_append(rv, rvs, rows[:8192], slots[:8192])
+    R.fp8_append(rv, rvs, rows[8192:], slots[8192:])
+    assert torch.equal(vs, rvs) and torch.equal(v.float(), rv.float())
+
+
+def test_write_in_place(dev):
+    """out as qkv's own q columns gives the same q."""
+    from connex_b200 import ops
+    s = _write_case(dev, [(0, 40), (9, 3)], 6, 2, 61)
+    a = ops.rope_cache_fp8(s["qkv"], s["pos"], s["cs"], 6, 2, s["slots"], s["k"], s["v"], s["ks"], s["vs"])
+    ops.rope_cache_fp8(s["qkv"], s["pos"], s["cs"], 6, 2, s["slots"], s["k"], s["v"], s["ks"], s["vs"],
+                       out=s["qkv"][:, :6 * D])
+    assert torch.equal(s["qkv"][:, :6 * D], a)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("layers,nb,hkv,n", [(1, 4, 1, 1), (3, 50, 2, 17), (32, 40, 8, 20), (2, 9000, 1, 4000)])
+def test_copy_blocks(dev, dtype, layers, nb, hkv, n):
+    from connex_b200 import ops
+    from connex_b200.ops import reference as R
+    g = _g(dev, 71)
+    kv = torch.randint(0, 256, (layers, 2, nb, hkv, BS, D * dtype.itemsize), generator=g, device=dev,
+                       dtype=torch.uint8).view(dtype)
+    scales = torch.rand(layers, 2, nb, hkv, generator=g, device=dev) if dtype == torch.float8_e4m3fn else None
+    perm = torch.randperm(nb, generator=g, device=dev).to(torch.int32)
+    pairs = torch.stack([perm[:n], perm[n:2 * n]], 1).contiguous()
+    if n > 3:                                # one source for two destinations; a repeated pair; a block onto itself
+        pairs[1, 0] = pairs[0, 0]
+        pairs[2] = pairs[0]
+        pairs[3, 1] = pairs[3, 0]
+    ref, rs = kv.clone(), None if scales is None else scales.clone()
+    R.kv_copy_blocks(ref, pairs, rs)
+    st = ops.new_status(dev)
+    ops.kv_copy_blocks(kv, pairs, scales, status=st)
+    ops.check_status(st, "kv_copy_blocks")
+    assert torch.equal(kv.view(torch.uint8), ref.view(torch.uint8))
+    assert scales is None or torch.equal(scales, rs)
+
+
+def test_copy_blocks_conflicts(dev):
+    """Pairs without a defined result are left out and recorded; the others run."""
+    from connex_b200 import ops
+    g = _g(dev, 81)
+    base = torch.randn(2, 2, 12, 1, BS, D, generator=g, device=dev).to(torch.bfloat16)
+    for pairs, done in (([(0, 1), (1, 2)], [(1, 2)]), ([(0, 5), (3, 5)], []), ([(0, 12), (3, 4)], [(3, 4)]),
+                        ([(-1, 2), (3, 4)], [(3, 4)]), ([(6, 7), (7, 6)], []), ([(2, 2), (3, 2)], [])):
+        kv, ref = base.clone(), base.clone()
+        for a, b in done:
+            ref[:, :, b] = base[:, :, a]
+        st = ops.new_status(dev)
+        ops.kv_copy_blocks(kv, torch.tensor(pairs, dtype=torch.int32, device=dev), status=st)
+        with pytest.raises(RuntimeError, match="bounds"):
+            ops.check_status(st)
+        assert torch.equal(kv, ref), pairs
+
+
+def test_decode_bad_pages_and_lengths(dev):
+    """A block id out of range is left out, a length beyond the table cut; both recorded."""
+    from connex_b200 import ops
+    from connex_b200.ops import reference as R
+    hq, hkv = 8, 2
+    k, ks = _cache(20, hkv, dev, 91)
+    v, vs = _cache(20, hkv, dev, 92)
+    q = torch.randn(2, hq * D, generator=_g(dev, 93), device=dev).to(torch.bfloat16)
+    ws = ops.decode_workspace_fp8(2, hq, hkv, dev)
+    for table, lens, like in (([[3, 20, 5], [1, 2, 4]], [48, 48], ([[3, 5, 5], [1, 2, 4]], [32, 48])),
+                              ([[3, -5, 5], [1, 2, 4]], [48, 20], ([[3, 5, 5], [1, 2, 4]], [32, 20])),
+                              ([[3, 4, 5], [1, 2, 6]], [49, -3], ([[3, 4, 5], [1, 2, 6]], [48, 0]))):
+        st = ops.new_status(dev)
+        i = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+        out = ops.decode_attention_fp8(q, k, v, ks, vs, i(table), i(lens), hq, ws, status=st)
+        with pytest.raises(RuntimeError, match="bounds"):
+            ops.check_status(st)
+        t, n = like
+        ref, mag = R.paged_attention_fp8(q.view(2, hq, D), k, v, ks, vs, i(t), [x - 1 if x else 0 for x in n], [1, 1])
+        for b in range(2):
+            if n[b] == 0:
+                assert not out[b].any()
+            else:
+                err = (out[b].view(hq, D).double() - ref[b]).abs()
+                assert (err <= U_BF16 * ref[b].abs() + mag[b] * 2.0 ** -8 + 1e-6).all()
+
+
+def test_decode_nan_and_extreme_logits(dev):
+    """A NaN key poisons its own head only; logits far apart and q's of any size stay exact enough."""
+    from connex_b200 import ops
+    from connex_b200.ops import reference as R
+    hq, hkv = 4, 2
+    table, nb = _table([100, 60], dev, 101)
+    k, ks = _cache(nb, hkv, dev, 102)
+    v, vs = _cache(nb, hkv, dev, 103)
+    ws = ops.decode_workspace_fp8(2, hq, hkv, dev)
+    lens = torch.tensor([100, 60], dtype=torch.int32, device=dev)
+    for size in (1e-30, 1e-3, 300.0, 1e30):
+        q = (torch.randn(2, hq * D, generator=_g(dev, 104), device=dev) * size).to(torch.bfloat16)
+        out = ops.decode_attention_fp8(q, k, v, ks, vs, table, lens, hq, ws).view(2, hq, D).double()
+        ref, mag = R.paged_attention_fp8(q.view(2, hq, D), k, v, ks, vs, table, [99, 59], [1, 1])
+        tol = _attention_tolerance(ref, mag, q.view(2, hq, D), k, ks, table, [99, 59], [1, 1], U_F16, float(vs.max()) * 448)
+        assert ((out - ref).abs() <= tol).all(), size
+    k.view(torch.uint8)[table[0, 2].long(), 1, 5, 7] = 0x7F
+    q = torch.randn(2, hq * D, generator=_g(dev, 105), device=dev).to(torch.bfloat16)
+    out = ops.decode_attention_fp8(q, k, v, ks, vs, table, lens, hq, ws).view(2, hq, D)
+    assert torch.isnan(out[0, 2:].float()).all()
+    assert torch.isfinite(out[0, :2].float()).all() and torch.isfinite(out[1].float()).all()
+
+
+def test_step_in_a_graph(dev):
+    """Write and decode captured together and replayed while the lengths grow, next
+    to the same steps run eagerly; a second graph with its own workspace on another stream."""
+    from connex_b200 import ops
+    hq, hkv, B, width = 8, 2, 5, 8
+    nb = B * width + 1
+    table = torch.arange(1, nb, dtype=torch.int32, device=dev).view(B, width)
+    cs = ops.rope_cos_sin(256, D, 1e4, dev)
+
+    def make():
+        c = [torch.zeros(nb, hkv, BS, D, device=dev).to(torch.float8_e4m3fn) for _ in range(2)]
+        c += [torch.ones(nb, hkv, device=dev) for _ in range(2)]
+        io = dict(qkv=torch.zeros(B, (hq + 2 * hkv) * D, dtype=torch.bfloat16, device=dev),
+                  pos=torch.zeros(B, dtype=torch.int32, device=dev), slots=torch.full((B,), -1, dtype=torch.int64, device=dev),
+                  lens=torch.ones(B, dtype=torch.int32, device=dev), ws=ops.decode_workspace_fp8(B, hq, hkv, dev),
+                  st=ops.new_status(dev))
+        return c, io
+
+    def step(c, io):
+        q = ops.rope_cache_fp8(io["qkv"], io["pos"], cs, hq, hkv, io["slots"], *c, status=io["st"])
+        return ops.decode_attention_fp8(q, *c, table, io["lens"], hq, io["ws"], status=io["st"])
+    sides = [make() for _ in range(3)]
+    graphs = []
+    for c, io in sides[:2]:
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            step(c, io)
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(c, io)
+        graphs.append((g, out, s))
+    for t in range(40):
+        x = (torch.randn(B, (hq + 2 * hkv) * D, generator=_g(dev, 200 + t), device=dev) * (1 + t % 7)).to(torch.bfloat16)
+        pos = torch.tensor([(t + 3 * b) % 100 if t >= 0 else 0 for b in range(B)], dtype=torch.int32, device=dev)
+        for c, io in sides:
+            io["qkv"].copy_(x)
+            io["pos"].copy_(pos)
+            io["slots"].copy_(table.gather(1, (pos.long() // BS)[:, None])[:, 0].long() * BS + pos.long() % BS)
+            io["lens"].copy_(pos + 1)
+        torch.cuda.synchronize()
+        for g, _, s in graphs:
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = step(*sides[2])
+        torch.cuda.synchronize()
+        for (g, out, _), (c, io) in zip(graphs, sides):
+            assert torch.equal(out.view(torch.int16), eager.view(torch.int16)), t
+            for a, b in zip(c, sides[2][0]):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    for _, io in sides:
+        ops.check_status(io["st"])

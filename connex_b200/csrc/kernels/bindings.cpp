@@ -322,7 +322,7 @@ void decode_attention_fp8(const at::Tensor& q, const at::Tensor& kc, const at::T
               "decode_attention_fp8: block_tables must be contiguous int32 [B, max_blocks]");
   TORCH_CHECK(ctx_lens.scalar_type() == at::kInt && ctx_lens.is_contiguous() && ctx_lens.numel() == B,
               "decode_attention_fp8: ctx_lens must be contiguous int32 [B]");
-  TORCH_CHECK(B * c.Hkv * block_tables.size(1) < (int64_t)1 << 30 && block_tables.size(1) < (int64_t)1 << 26,
+  TORCH_CHECK(B * c.Hkv * (block_tables.size(1) + 16) < (int64_t)1 << 30 && block_tables.size(1) < (int64_t)1 << 26,
               "decode_attention_fp8: block tables too large");
   const int64_t G = Hq / c.Hkv;
   CHECK_CUDA(q);

@@ -263,49 +263,106 @@ void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_s
 }
 
 // ------------------------------------------------------- decode attention
-// S = q.K^T and O^T = V^T.W^T on mma.sync m16n8k16 (f16 in, fp32 out) from
-// registers alone: the cached bytes are loaded straight into the layout the
-// fragments need and converted e4m3 -> f16 (exact) in place.
-//   K: lane (g = lane / 4, c = lane % 4) loads bytes [16 c, 16 c + 16) of both
+// S = q.K^T and O^T = V^T.W^T on mma.sync m16n8k32 with e4m3 operands: the
+// cached bytes go into the tensor cores as they are (measured: 4.3 cycles per
+// instruction and SM quarter against 8 for the f16 m16n8k16 of half the
+// depth, sums exact to 2^-25; a version that converted K and V to f16 spent
+// twice the instructions and stayed at 0.60 of the HBM rate where this one
+// reaches RATE).  q and the softmax weights enter as the sum of two
+// e4m3 numbers each:
+//   q     scaled by a power of two per head to at most 448; bf16's 8-bit
+//         significand is two 4-bit ones, so only elements 2^11 times smaller
+//         than the head's largest lose bits (at most 2^-18 of the largest).
+//         With up to 8 heads the two parts are rows 0-7 and 8-15 of one A.
+//   w     exp2(z - max z of the 32 tokens + 8): two parts leave 2^-8 of the
+//         value, as bf16 would, and 2^-18 of the largest weight.  The 32
+//         tokens' product is its own sum, added to O in fp32 with the factor
+//         that relates the two maxima.
+// Fragments come straight from the cache's layout:
+//   K: lane (g = lane / 4, c = lane % 4) takes bytes [16 c, 16 c + 16) of both
 //      64-byte halves of tokens g and g + 8.  The contraction may take the
-//      dims in any order as long as q uses the same one, so bytes 4j..4j+3 of
-//      a load are the four k-values a lane holds of MMA step j.
-//   V: the lane loads bytes [16 g, 16 g + 16) of tokens 2c, 2c + 1, 2c + 8,
-//      2c + 9 -- the tokens of its column pairs -- and interleaves the bytes
-//      of two tokens, which makes byte pair (2j, 2j + 1) the rows of MMA tile j.
-// S comes out with the heads on the rows and each lane holding tokens 2c,
-// 2c + 1 (+ 8), which is the second product's B fragment as it stands.
+//      dims in any order as long as q uses the same one, so words 2i, 2i + 1
+//      of a piece are the eight k-values a lane holds of an MMA step.
+//   V: the lane takes bytes [16 g, 16 g + 16) of tokens 2c, 2c + 1, 2c + 8,
+//      2c + 9 of each block -- the tokens whose weights S leaves in this lane, four k-values
+//      of the second product -- and transposes 4 x 4 bytes.
 // The block scales stay out of the operands: K's multiplies the logits, V's
-// is folded into the weights exp2(s_j + log2 v_j - mv) with a running maximum
-// mv of their own (f16 weights then keep their precision whatever the ratio
-// of the scales), next to the usual maximum m of the softmax sum.
-// q is scaled by a power of two per head into f16's range: exact but for
-// elements 2^29 times smaller than the head's largest.
+// is part of z = s + log2 v, which has maxima of its own next to the one of
+// the softmax sum.
 //
-// Work split: the blocks of all (sequence, KV head) pairs, laid end to end,
-// are cut into equal runs, one per CTA, from the lengths themselves -- the
-// same launch (a graph replay) is balanced for any lengths.  A pair that
-// spans several CTAs leaves partial results in the workspace, and the CTA
-// that arrives last merges them (a counter that wraps to zero by itself).
+// Loads: cp.async into two blocks' worth of shared memory per warp, K and V in
+// turn: as soon as a warp has K of its blocks in registers the next K is under
+// way, and the same for V, without barriers between warps.  Block ids and
+// scales come 32 blocks at a time, one per lane.
+//
+// Work split: the blocks of all (sequence, KV head) pairs, laid end to end
+// with PAIR_COST blocks' worth for the fixed cost of a pair, are cut into
+// equal runs, one per CTA, from the lengths themselves -- the same launch (a
+// graph replay) is balanced for any lengths.  A pair that spans several CTAs
+// leaves partial results in the workspace, and the CTA that arrives last
+// merges them (a counter that wraps to zero by itself).
 namespace dec8 {
 constexpr int D = kvq::D, BS = kvq::BS, WARPS = 4, THREADS = 32 * WARPS, CTAS_PER_SM = 4;
-constexpr int MIN_BLOCKS = 2 * WARPS;   // a CTA takes at least this many blocks
-constexpr float RESCALE = 8.f;          // O is rescaled once mv grows by this much (weights stay under 2^9)
+constexpr int MIN_UNITS = 4 * WARPS;    // a CTA takes at least this many blocks' worth
+constexpr int PAIR_COST = 2 * WARPS;
+constexpr float WEIGHT_BITS = 8.f;      // the largest weight of 32 tokens is 2^8
+constexpr float RESCALE = 8.f;          // O is rescaled once the maximum has grown by this much
+constexpr int SLOT = 2 * BS * D;        // K (or V) of two blocks
+constexpr int RING = WARPS * 2 * SLOT;
+template <int NT>
+struct Smem {                           // ring, then the warps' O in its place | (m, l, mv) | scales | prefix sums
+  static constexpr int O = WARPS * 8 * NT * D * 4;
+  static constexpr int HEAD = RING > O ? RING : O;
+  static constexpr int SCALES = HEAD + WARPS * 8 * NT * 16;
+  static constexpr int PRE = SCALES + WARPS * 2 * 16;
+  static constexpr int bytes(int B) { return PRE + (B + 1) * 4; }
+};
 }  // namespace dec8
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ u128 lds16(uint32_t a) {
+  u128 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t word(const u128& v, int i) { return reinterpret_cast<const uint32_t*>(&v)[i]; }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// two fp32 of at most 448 as the sums of two e4m3 each: pairs of bytes hi and lo
+__device__ __forceinline__ void split_e4m3x2(float a, float b, uint16_t& hi, uint16_t& lo) {
+  asm("{\n\t.reg .b32 w, r;\n\t"
+      "cvt.rn.f16x2.f32 w, %3, %2;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 %0, w;\n\t"
+      "cvt.rn.f16x2.e4m3x2 r, %0;\n\t"
+      "sub.rn.f16x2 r, w, r;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 %1, r;\n\t}"
+      : "=&h"(hi), "=h"(lo)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ uint32_t pair16(uint16_t lo, uint16_t hi) { return (uint32_t)lo | (uint32_t)hi << 16; }
 
 // NT: tiles of 8 query heads per KV head (1: groups up to 8, 2: up to 16).
 template <int NT>
@@ -316,9 +373,10 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
                            int* status) {
   using namespace dec8;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* so = reinterpret_cast<float*>(smem);                 // [WARPS][8 NT][D]
-  float* sm = so + WARPS * 8 * NT * D;                        // [WARPS][8 NT][m, l, mv]
-  int* pre = reinterpret_cast<int*>(sm + WARPS * 8 * NT * 4); // [B + 1] blocks of the pairs before sequence b
+  float* so = reinterpret_cast<float*>(smem);                           // [WARPS][8 NT][D], once the ring is drained
+  float* sm = reinterpret_cast<float*>(smem + Smem<NT>::HEAD);          // [WARPS][8 NT][m, l, mv]
+  float4* sc = reinterpret_cast<float4*>(smem + Smem<NT>::SCALES);      // [WARPS][2] (K, V) scales of two blocks
+  int* pre = reinterpret_cast<int*>(smem + Smem<NT>::PRE);              // [B + 1] units of the pairs before sequence b
   __shared__ int wsum[WARPS];
   __shared__ uint32_t ticket;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -326,16 +384,16 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
   const int Hkv = c.Hkv, G = Hq / Hkv;
 
   auto len_of = [&](int b) { return min(max(ctx_lens[b], 0), max_blocks * BS); };
-  // ---- prefix sums of the pairs' blocks
+  // ---- prefix sums of the pairs' units
   if (tid == 0) pre[0] = 0;
   int run = 0;
   for (int b0 = 0; b0 < B; b0 += THREADS) {
     const int b = b0 + tid;
     int n = 0;
     if (b < B) {
-      const int len = ctx_lens[b];
-      if (len > max_blocks * BS && blockIdx.x == 0) record_status(status, CX_ERR_BOUNDS);
-      n = (len_of(b) + BS - 1) / BS * Hkv;
+      if (ctx_lens[b] > max_blocks * BS && blockIdx.x == 0) record_status(status, CX_ERR_BOUNDS);
+      const int len = len_of(b);
+      n = len > 0 ? ((len + BS - 1) / BS + PAIR_COST) * Hkv : 0;
     }
     int x = n;
 #pragma unroll
@@ -359,7 +417,7 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
   for (int b = blockIdx.x; b < B; b += gridDim.x)
     if (pre[b + 1] == pre[b])
       for (int i = tid; i < Hq * D / 8; i += THREADS) st_v4(out + (size_t)b * ldo + 8 * i, u128{0, 0, 0, 0});
-  const int n_cta = max(1, min((int)gridDim.x, (total + MIN_BLOCKS - 1) / MIN_BLOCKS));
+  const int n_cta = max(1, min((int)gridDim.x, (total + MIN_UNITS - 1) / MIN_UNITS));
   const int per = (total + n_cta - 1) / n_cta;
   const int u0 = min(total, (int)blockIdx.x * per), u1 = min(total, u0 + per);
 
@@ -375,15 +433,82 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
   }
   for (int u = u0; u < u1;) {
     while (pre[b + 1] <= u) ++b;
-    const int nblk = (pre[b + 1] - pre[b]) / Hkv;
-    const int h = (u - pre[b]) / nblk;                         // KV head
-    const int pair0 = pre[b] + h * nblk;                       // first block of the pair
-    const int j0 = u - pair0, j1 = min(nblk, u1 - pair0);      // its blocks in this CTA
+    const int units = (pre[b + 1] - pre[b]) / Hkv;
+    const int h = (u - pre[b]) / units;                        // KV head
+    const int pair0 = pre[b] + h * units;                      // first unit of the pair
+    const int j0 = max(0, u - pair0 - PAIR_COST), j1 = min(units, u1 - pair0) - PAIR_COST;   // its blocks in this CTA
+    const int next_u = min(pair0 + units, u1);
+    if (j1 <= 0) {                                             // this CTA has none but the pair's fixed cost
+      u = next_u;
+      continue;
+    }
     const int len = len_of(b);
-    const int* bt = tables + (size_t)b * max_blocks;
 
-    // ---- q fragments, scaled by a power of two per head
-    uint32_t qa[8][2 * NT];
+    // ---- the warp's loads: block pair it = blocks j0 + 2 (warp + WARPS it) + {0, 1}
+    int ids = -1, id0 = -1, id1 = -1;
+    float lks = 0.f, lvs = 0.f;
+    // Both land row by row, 512 contiguous bytes per instruction (measured: with
+    // every lane fetching the pieces it reads back, K in 64-byte halves and V
+    // in every other row, the loads alone took 122 us of 64 x 4096 where these
+    // take 96).  16-byte pieces are permuted inside a row so that the fragment
+    // reads meet no bank twice: K by the row's lowest bit (two rows at a time
+    // are read), V by the two above it (rows 2c, c = 0 .. 3).
+    const uint32_t kslot = smem_u32(smem) + warp * (2 * SLOT), vslot = kslot + SLOT;
+    const uint32_t kput = kslot + (lane >> 3) * D + (((lane & 7) ^ (lane >> 3 & 1) * 4) << 4);
+    const uint32_t kget = kslot + gq * D + ((qd ^ (gq & 1) * 4) << 4);
+    const int khalf = gq & 1 ? -64 : 64;
+    const uint32_t vput = (lane >> 3) * D + (((lane & 7) ^ (lane >> 4) * 2) << 4);   // rows 0-3; ^ 64 in rows 4-7
+    const uint32_t vget = vslot + 2 * qd * D + ((gq ^ qd * 2) << 4);
+    const int vhalf = gq >> 1 & 1;       // 8-byte half of the piece that comes first (bank conflicts again)
+    float2* const scw = reinterpret_cast<float2*>(sc + warp * 2);
+    auto fetch_k = [&](int it) {
+      const int j = j0 + 2 * (warp + it * WARPS);
+      id0 = id1 = -1;
+      if (j < j1) {
+        if ((it & 15) == 0) {
+          const int mine = j + (lane >> 1) * (2 * WARPS) + (lane & 1);
+          ids = -1;
+          if (mine < j1) {
+            ids = tables[(size_t)b * max_blocks + mine];
+            if (ids < 0 || ids >= c.num_blocks) {
+              record_status(status, CX_ERR_BOUNDS);
+              ids = -1;
+            }
+          }
+          lks = ids >= 0 ? c.ks[(size_t)ids * Hkv + h] : -1.f;   // below 0: no block
+          lvs = ids >= 0 ? c.vs[(size_t)ids * Hkv + h] : 0.f;
+        }
+        const int l0 = 2 * (it & 15);
+        id0 = __shfl_sync(0xffffffffu, ids, l0);
+        id1 = __shfl_sync(0xffffffffu, ids, l0 + 1);
+        if ((lane >> 1) == (it & 15)) scw[2 * (it & 1) + (lane & 1)] = make_float2(lks, lvs);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int id = i ? id1 : id0;
+          if (id < 0) continue;
+          const uint8_t* p = c.k + ((size_t)id * Hkv + h) * (BS * D) + lane * 16;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) cp_async16(kput + (4 * i + e) * 512, p + e * 512);
+        }
+      }
+      cp_async_commit();
+    };
+    auto fetch_v = [&]() {                                     // of the pair whose K was fetched last
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int id = i ? id1 : id0;
+        if (id < 0) continue;
+        const uint8_t* p = c.v + ((size_t)id * Hkv + h) * (BS * D) + lane * 16;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) cp_async16(vslot + (4 * i + e) * 512 + (vput ^ (e & 1) * 64), p + e * 512);
+      }
+      cp_async_commit();
+    };
+    fetch_k(0);
+    fetch_v();
+
+    // ---- q fragments: step i covers words 2 (i % 2), 2 (i % 2) + 1 of the pieces i / 2
+    uint32_t qa[NT][4][4];
     float qf[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -391,25 +516,32 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
       u128 raw[4];
       float am = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {                            // dims (i / 2) * 64 + qd * 16 + (i % 2) * 8 ..
+      for (int i = 0; i < 4; ++i) {                            // 8 dims at (i / 2) * 64 + qd * 16 + (i % 2) * 8
         raw[i] = hh < G ? ld_v4(q + (size_t)b * ldq + (size_t)(h * G + hh) * D + (i >> 1) * 64 + qd * 16 + (i & 1) * 8)
                         : u128{0, 0, 0, 0};
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) am = fmaxf(am, fmaxf(finite_or_zero(bf16_lo(w[e])), finite_or_zero(bf16_hi(w[e]))));
+        for (int e = 0; e < 4; ++e)
+          am = fmaxf(am, fmaxf(finite_or_zero(bf16_lo(word(raw[i], e))), finite_or_zero(bf16_hi(word(raw[i], e)))));
       }
       am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
       am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
-      // am * 2^-eq in [2^14, 2^15)
-      const int eq = am > 0.f ? max((int)(__float_as_uint(am) >> 23) - 127 - 14, -126) : 0;
+      const int eq = min(max((int)(__float_as_uint(am) >> 23) - 127 - 8 + ((__float_as_uint(am) & 0x7fffffu) > 0x600000u), -126), 126);
       const float down = exp2_int(-eq);
       qf[nt] = exp2_int(eq) * scale_log2;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)                            // step 2i + e / 2; dims 0,1 then 2,3 of the four
-          qa[2 * i + (e >> 1)][2 * nt + (e & 1)] = pack_f16x2(bf16_lo(w[e]) * down, bf16_hi(w[e]) * down);
+        for (int e = 0; e < 2; ++e) {                          // four dims: words 2e, 2e + 1 of the bf16 piece
+          float f[4] = {bf16_lo(word(raw[i], 2 * e)), bf16_hi(word(raw[i], 2 * e)), bf16_lo(word(raw[i], 2 * e + 1)),
+                        bf16_hi(word(raw[i], 2 * e + 1))};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) f[k] = scaled_or_nan(f[k], down);
+          uint16_t h0, h1, l0, l1;
+          split_e4m3x2(f[0], f[1], h0, l0);
+          split_e4m3x2(f[2], f[3], h1, l1);
+          qa[nt][i][2 * e] = pair16(h0, h1);
+          qa[nt][i][2 * e + 1] = pair16(l0, l1);
+        }
       }
     }
 
@@ -424,100 +556,96 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][mt][e] = 0.f;
     }
-    u128 kr[4], vr[4];
-    float ks = 1.f, vs = 1.f;
-    int id = -1;
-    // block ids of the warp's next 32 blocks, one per lane
-    int ids = 0, ids_at = j0 + warp;
-    auto id_of = [&](int j) -> int {                           // j advances by WARPS; uniform over the warp
-      if (((j - ids_at) / WARPS) >= 32) ids_at = j;
-      if (j == ids_at) {
-        const int jj = j + WARPS * lane;
-        ids = jj < j1 ? bt[jj] : -1;
-      }
-      int r = __shfl_sync(0xffffffffu, ids, ((j - ids_at) / WARPS) & 31);
-      if (j < j1 && (r < 0 || r >= c.num_blocks)) {
-        if (lane == 0) record_status(status, CX_ERR_BOUNDS);
-        r = -1;
-      }
-      return j < j1 ? r : -1;
-    };
-    auto load_k = [&](int i) {
-      if (i < 0) return;
-      const uint8_t* p = c.k + ((size_t)i * Hkv + h) * (BS * D) + gq * D + qd * 16;
+    for (int it = 0, j = j0 + 2 * warp; j < j1; ++it, j += 2 * WARPS) {
+      cp_async_wait<1>();                                      // K of this pair
+      __syncwarp();                                            // of every lane, and its scales
+      const float4 scale = sc[warp * 2 + (it & 1)];            // K, V of the first block, K, V of the second
+      float x[NT][8];                                          // logits: 4 of each block
 #pragma unroll
-      for (int e = 0; e < 4; ++e) kr[e] = ld_nc_v4(p + (e >> 1) * 8 * D + (e & 1) * 64);
-      ks = c.ks[(size_t)i * Hkv + h];
-    };
-    auto load_v = [&](int i) {
-      if (i < 0) return;
-      const uint8_t* p = c.v + ((size_t)i * Hkv + h) * (BS * D) + 2 * qd * D + gq * 16;
+      for (int i = 0; i < 2; ++i) {
+        const float ks = i ? scale.z : scale.x;
+        if (ks < 0.f) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) vr[e] = ld_nc_v4(p + ((e >> 1) * 8 + (e & 1)) * D);
-      vs = c.vs[(size_t)i * Hkv + h];
-    };
-    int j = j0 + warp;
-    if (j < j1) {
-      id = id_of(j);
-      load_k(id);
-      load_v(id);
-    }
-    for (; j < j1; j += WARPS) {
-      const int cur = id;
-      const int next = j + WARPS < j1 ? id_of(j + WARPS) : -1;
-      id = next;
-      float s[2][4];                                           // tokens 0-7, 8-15 of the block
-      if (cur >= 0) {
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[nt][4 * i + e] = -INFINITY;
+          continue;
+        }
+        u128 kr[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kr[e] = lds16(kget + (e & 1) * khalf + i * (BS * D) + (e >> 1) * 8 * D);
+        float s[2][4];                                         // tokens 0-7, 8-15 of the block
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.f;
 #pragma unroll
-        for (int st = 0; st < 8; ++st) {                       // 16 dims each
+        for (int st = 0; st < 4; ++st)
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt) {
-            const uint32_t w = reinterpret_cast<const uint32_t*>(&kr[2 * tt + (st >> 2)])[st & 3];
-            const uint32_t b0 = e4m3x2_to_f16x2((uint16_t)w), b1 = e4m3x2_to_f16x2((uint16_t)(w >> 16));
-            mma_f16(s[tt], qa[st][0], NT == 2 ? qa[st][2 * NT - 2] : 0u, qa[st][1], NT == 2 ? qa[st][2 * NT - 1] : 0u,
-                    b0, b1);
+            const uint32_t b0 = word(kr[2 * tt + (st >> 1)], 2 * (st & 1)), b1 = word(kr[2 * tt + (st >> 1)], 2 * (st & 1) + 1);
+            if (NT == 1) {                                     // rows 0-7 the larger parts, rows 8-15 the rest
+              mma_e4m3(s[tt], qa[0][st][0], qa[0][st][1], qa[0][st][2], qa[0][st][3], b0, b1);
+            } else {                                           // rows: 16 heads; the parts one after the other
+              mma_e4m3(s[tt], qa[0][st][0], qa[NT - 1][st][0], qa[0][st][2], qa[NT - 1][st][2], b0, b1);
+              mma_e4m3(s[tt], qa[0][st][1], qa[NT - 1][st][1], qa[0][st][3], qa[NT - 1][st][3], b0, b1);
+            }
           }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float f = qf[nt] * ks;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[nt][4 * i + e] = (NT == 1 ? s[e >> 1][e & 1] + s[e >> 1][2 + (e & 1)] : s[e >> 1][2 * nt + (e & 1)]) * f;
         }
       }
-      const float kscale = ks, vscale = vs;
-      load_k(next);
-      if (cur < 0) {
-        load_v(next);
-        continue;
+      __syncwarp();                                            // K has been read by all
+      fetch_k(it + 1);
+      const int tok0 = j * BS + 2 * qd;                        // this lane's tokens: + {0, 1, 8, 9} of each block
+      const bool tail = (j + 2) * BS > len;
+      if (tail) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (tok0 + (e & 1) + ((e >> 1) & 1) * 8 + (e >> 2) * BS >= len)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) x[nt][e] = -INFINITY;
       }
-      const int tok0 = j * BS;
-      const bool tail = tok0 + BS > len;
-      const float ev = (float)((int)(__float_as_uint(vscale) >> 23) - 127);
-      uint32_t wb[NT][2];                                      // weights as the B fragment of the second product
-      float alpha[NT];
+      const float e0 = (float)((int)(__float_as_uint(scale.y) >> 23) - 127);
+      const float e1 = (float)((int)(__float_as_uint(scale.w) >> 23) - 127);
+      uint32_t wh[NT][2], wl[NT][2];                           // weights' two parts: B fragments of the second product
+      float alpha[NT], beta[NT];
       bool grow = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float x[4] = {s[0][2 * nt], s[0][2 * nt + 1], s[1][2 * nt], s[1][2 * nt + 1]};
-        const float f = qf[nt] * kscale;
+        float a0 = fmaxf(fmaxf(x[nt][0], x[nt][1]), fmaxf(x[nt][2], x[nt][3]));
+        float a1 = fmaxf(fmaxf(x[nt][4], x[nt][5]), fmaxf(x[nt][6], x[nt][7]));
+        a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, 1));
+        a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, 1));
+        a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, 2));
+        a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, 2));
+        const float m_new = fmaxf(m[nt], fmaxf(a0, a1)), base = m_new == -INFINITY ? 0.f : m_new;
+        float ls = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] *= f;
-          if (tail && tok0 + 2 * qd + (e & 1) + (e >> 1) * 8 >= len) x[e] = -INFINITY;
-        }
-        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m[nt], mx), base = m_new == -INFINITY ? 0.f : m_new;
-        l[nt] = l[nt] * ex2(m[nt] - base) + ((ex2(x[0] - base) + ex2(x[1] - base)) + (ex2(x[2] - base) + ex2(x[3] - base)));
+        for (int e = 0; e < 8; ++e) ls += ex2(x[nt][e] - base);
+        l[nt] = l[nt] * ex2(m[nt] - base) + ls;
         m[nt] = m_new;
+        const float mt = fmaxf(a0 + e0, a1 + e1);              // of z = x + log2 of V's scale
         alpha[nt] = 1.f;
-        if (mx + ev > mv[nt] + RESCALE || mv[nt] == -INFINITY) {
-          const float mv_new = fmaxf(mv[nt], mx + ev);
-          alpha[nt] = mv_new == -INFINITY ? 1.f : ex2(mv[nt] - mv_new);
-          mv[nt] = mv_new;
+        if (mt > mv[nt] + RESCALE || mv[nt] == -INFINITY) {
+          alpha[nt] = mt == -INFINITY ? 1.f : ex2(mv[nt] - mt);
+          mv[nt] = mt;
           grow = true;
         }
-        const float vb = ev - (mv[nt] == -INFINITY ? 0.f : mv[nt]);
-        wb[nt][0] = pack_f16x2(ex2(x[0] + vb), ex2(x[1] + vb));
-        wb[nt][1] = pack_f16x2(ex2(x[2] + vb), ex2(x[3] + vb));
+        const float tb = mt == -INFINITY ? 0.f : mt;
+        beta[nt] = mt == -INFINITY ? 0.f : ex2(mt - WEIGHT_BITS - mv[nt]);
+        const float z0 = e0 - tb + WEIGHT_BITS, z1 = e1 - tb + WEIGHT_BITS;
+        uint16_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          split_e4m3x2(ex2(x[nt][2 * e] + (e < 2 ? z0 : z1)), ex2(x[nt][2 * e + 1] + (e < 2 ? z0 : z1)), hi[e], lo[e]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          wh[nt][i] = pair16(hi[2 * i], hi[2 * i + 1]);
+          wl[nt][i] = pair16(lo[2 * i], lo[2 * i + 1]);
+        }
       }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -532,31 +660,61 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
           }
         }
       }
-      if (tail) {   // rows past the end were never written: 0 x NaN would poison O
+      float bc[NT][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (tok0 + 2 * qd + (e & 1) + (e >> 1) * 8 >= len) vr[e] = u128{0, 0, 0, 0};
+      for (int nt = 0; nt < NT; ++nt) {
+        bc[nt][0] = __shfl_sync(0xffffffffu, beta[nt], 8 * qd);
+        bc[nt][1] = __shfl_sync(0xffffffffu, beta[nt], 8 * qd + 4);
       }
+      cp_async_wait<1>();                                      // V of this pair
+      __syncwarp();
+      const bool gaps = tail || scale.x < 0.f || scale.z < 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {                            // 4 bytes of each token: MMA tiles 2w, 2w + 1
-        uint32_t t4[4];
+      for (int w2 = 0; w2 < 2; ++w2) {                         // 8 dims of each token: MMA tiles 4 w2 ..
+        uint2 vr[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t4[e] = reinterpret_cast<const uint32_t*>(&vr[e])[w];
+        for (int e = 0; e < 8; ++e) vr[e] = lds8(vget + (e >> 2) * (BS * D) + ((e >> 1 & 1) * 8 + (e & 1)) * D + 8 * (w2 ^ vhalf));
+        if (gaps) {                                            // rows never written: 0 x NaN would poison O
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const uint32_t x = __byte_perm(t4[0], t4[1], hf ? 0x7362 : 0x5140);
-          const uint32_t y = __byte_perm(t4[2], t4[3], hf ? 0x7362 : 0x5140);
-          const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)x), a1 = e4m3x2_to_f16x2((uint16_t)(x >> 16));
-          const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)y), a3 = e4m3x2_to_f16x2((uint16_t)(y >> 16));
+          for (int e = 0; e < 8; ++e)
+            if (tok0 + (e & 1) + ((e >> 1) & 1) * 8 + (e >> 2) * BS >= len || (e < 4 ? scale.x : scale.z) < 0.f)
+              vr[e] = make_uint2(0, 0);
+        }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + hf], a0, a1, a2, a3, wb[nt][0], wb[nt][1]);
+        for (int w = 0; w < 2; ++w) {                          // 4 dims: two tiles
+          uint32_t r[2][4];                                    // [block][dim]: four tokens' bytes
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t t0 = w ? vr[4 * i].y : vr[4 * i].x, t1 = w ? vr[4 * i + 1].y : vr[4 * i + 1].x,
+                           t2 = w ? vr[4 * i + 2].y : vr[4 * i + 2].x, t3 = w ? vr[4 * i + 3].y : vr[4 * i + 3].x;
+            const uint32_t p0 = __byte_perm(t0, t1, 0x5140), p1 = __byte_perm(t2, t3, 0x5140);
+            const uint32_t p2 = __byte_perm(t0, t1, 0x7362), p3 = __byte_perm(t2, t3, 0x7362);
+            r[i][0] = __byte_perm(p0, p1, 0x5410);
+            r[i][1] = __byte_perm(p0, p1, 0x7632);
+            r[i][2] = __byte_perm(p2, p3, 0x5410);
+            r[i][3] = __byte_perm(p2, p3, 0x7632);
+          }
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float t[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_e4m3(t, r[0][2 * hf], r[0][2 * hf + 1], r[1][2 * hf], r[1][2 * hf + 1], wh[nt][0], wh[nt][1]);
+              mma_e4m3(t, r[0][2 * hf], r[0][2 * hf + 1], r[1][2 * hf], r[1][2 * hf + 1], wl[nt][0], wl[nt][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nt][4 * w2 + 2 * w + hf][e] += t[e] * bc[nt][e & 1];
+            }
+          if (w2 == 1 && w == 0) {                             // every lane has read all of its V by now
+            __syncwarp();
+            fetch_v();
+          }
         }
       }
-      load_v(next);
     }
+    cp_async_wait<0>();
 
     // ---- the warps' results of this pair
-    __syncthreads();                                           // the previous pair's reads of so / sm are done
+    __syncthreads();                                           // every warp has drained its ring
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float ls = l[nt];
@@ -572,10 +730,11 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
       for (int mt = 0; mt < 8; ++mt)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          so[(warp * 8 * NT + nt * 8 + 2 * qd + (e & 1)) * D + gq * 16 + 2 * mt + (e >> 1)] = o[nt][mt][e];
+          so[(warp * 8 * NT + nt * 8 + 2 * qd + (e & 1)) * D + gq * 16 + 2 * (mt ^ 4 * vhalf) + (e >> 1)] = o[nt][mt][e];
     }
     __syncthreads();
-    const int c0 = pair0 / per, c1 = (pair0 + nblk - 1) / per;  // the CTAs that share the pair
+    // the CTAs that share the pair; the first may start inside the pair's fixed cost
+    const int c0 = (pair0 + PAIR_COST) / per, c1 = (pair0 + units - 1) / per;
     // thread: dim tid of every head
     for (int hh = 0; hh < G; ++hh) {
       float M = -INFINITY, MV = -INFINITY;
@@ -594,9 +753,10 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
         den += p[1] * ex2(p[0] - mb);
       }
       if (c0 == c1) {
-        out[(size_t)b * ldo + (size_t)(h * G + hh) * D + tid] = __float2bfloat16(den == 0.f ? 0.f : num / den * ex2(vb - mb));
+        out[(size_t)b * ldo + (size_t)(h * G + hh) * D + tid] =
+            __float2bfloat16(den == 0.f ? 0.f : num / den * ex2(vb - mb));
       } else {   // a CTA's first pair goes to its slot 0, its last to slot 1
-        float* p = part + ((size_t)(blockIdx.x * 2 + (u == u0 ? 0 : 1)) * G + hh) * DEC8_ROW;
+        float* p = part + ((size_t)(blockIdx.x * 2 + (pair0 <= u0 ? 0 : 1)) * G + hh) * DEC8_ROW;
         p[tid] = num;
         if (tid == 0) {
           p[D] = M;
@@ -612,27 +772,57 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
       __syncthreads();
       if (ticket == (uint32_t)(c1 - c0)) {
         __threadfence();
-        for (int hh = 0; hh < G; ++hh) {
-          auto slot = [&](int cc) {   // the pair is the first of every CTA but perhaps c0
-            return part + ((size_t)(cc * 2 + (cc == c0 && pair0 != c0 * per ? 1 : 0)) * G + hh) * DEC8_ROW;
+        // a warp per head: lanes over the CTAs for the statistics, over the dims for the sums
+        for (int hh = warp; hh < G; hh += WARPS) {
+          auto slot = [&](int cc) {
+            return part + ((size_t)(cc * 2 + (pair0 <= cc * per ? 0 : 1)) * G + hh) * DEC8_ROW;
           };
           float M = -INFINITY, MV = -INFINITY;
-          for (int cc = c0; cc <= c1; ++cc) {
+          for (int cc = c0 + lane; cc <= c1; cc += 32) {
             M = fmaxf(M, __ldcg(slot(cc) + D));
             MV = fmaxf(MV, __ldcg(slot(cc) + D + 2));
           }
+          M = warp_max(M);
+          MV = warp_max(MV);
           const float mb = M == -INFINITY ? 0.f : M, vb = MV == -INFINITY ? 0.f : MV;
-          float num = 0.f, den = 0.f;
-          for (int cc = c0; cc <= c1; ++cc) {
-            const float* p = slot(cc);
-            num += __ldcg(p + tid) * ex2(__ldcg(p + D + 2) - vb);
-            den += __ldcg(p + D + 1) * ex2(__ldcg(p + D) - mb);
+          float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+          float den = 0.f;
+          for (int cb = c0; cb <= c1; cb += 32) {
+            const int mine = cb + lane, n = min(32, c1 - cb + 1);
+            float f = 0.f;
+            if (mine <= c1) {
+              den += __ldcg(slot(mine) + D + 1) * ex2(__ldcg(slot(mine) + D) - mb);
+              f = ex2(__ldcg(slot(mine) + D + 2) - vb);
+            }
+            for (int i = 0; i < n; i += 8) {
+              float4 x[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                x[k] = i + k < n ? __ldcg(reinterpret_cast<const float4*>(slot(cb + i + k)) + lane)
+                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float g = __shfl_sync(0xffffffffu, f, (i + k) & 31);
+                if (i + k < n) {
+                  num.x += x[k].x * g;
+                  num.y += x[k].y * g;
+                  num.z += x[k].z * g;
+                  num.w += x[k].w * g;
+                }
+              }
+            }
           }
-          out[(size_t)b * ldo + (size_t)(h * G + hh) * D + tid] = __float2bfloat16(den == 0.f ? 0.f : num / den * ex2(vb - mb));
+          den = warp_sum(den);
+          const float inv = den == 0.f ? 0.f : ex2(vb - mb) / den;
+          uint2 w;
+          w.x = pack_bf16x2(num.x * inv, num.y * inv);
+          w.y = pack_bf16x2(num.z * inv, num.w * inv);
+          *reinterpret_cast<uint2*>(out + (size_t)b * ldo + (size_t)(h * G + hh) * D + 4 * lane) = w;
         }
       }
     }
-    u = pair0 + j1;
+    u = next_u;
+    __syncthreads();                                           // so is read before the ring fills again
   }
 }
 
@@ -651,16 +841,17 @@ void decode_attention_fp8(const void* q, int ldq, const KvFp8& c, const int* blo
   // the partial results sit at the front, the counters behind them: neither moves with the batch
   uint32_t* counters = reinterpret_cast<uint32_t*>(ws + 2L * ctas * G * DEC8_ROW);
   const int nt = G > 8 ? 2 : 1;
-  const long most = ((long)B * c.Hkv * max_blocks + dec8::MIN_BLOCKS - 1) / dec8::MIN_BLOCKS;
+  const long most = ((long)B * c.Hkv * (max_blocks + dec8::PAIR_COST) + dec8::MIN_UNITS - 1) / dec8::MIN_UNITS;
   const int grid = (int)std::max(1L, std::min((long)ctas, most));
-  const int smem = (dec8::WARPS * 8 * nt * (dec8::D + 4)) * 4 + (B + 1) * 4;
+  const int smem = nt == 2 ? dec8::Smem<2>::bytes(B) : dec8::Smem<1>::bytes(B);
   auto kern = nt == 2 ? decode_attn_fp8_kernel<2> : decode_attn_fp8_kernel<1>;
   static bool attr[64][2] = {};
   int dev;
   cudaGetDevice(&dev);
   if (!attr[dev & 63][nt - 1]) {
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         (dec8::WARPS * 8 * nt * (dec8::D + 4)) * 4 + (DEC8_MAX_BATCH + 1) * 4);
+                         nt == 2 ? dec8::Smem<2>::bytes(DEC8_MAX_BATCH) : dec8::Smem<1>::bytes(DEC8_MAX_BATCH));
+    cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
     attr[dev & 63][nt - 1] = true;
   }
   kern<<<grid, dec8::THREADS, smem, s>>>(reinterpret_cast<const __nv_bfloat16*>(q), ldq, c, block_tables, max_blocks,

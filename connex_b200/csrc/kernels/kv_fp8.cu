@@ -297,24 +297,26 @@ void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_s
 //
 // Work split: the blocks of all (sequence, KV head) pairs, laid end to end
 // with PAIR_COST blocks' worth for the fixed cost of a pair, are cut into
-// equal runs, one per CTA, from the lengths themselves -- the same launch (a
+// equal shares, one per CTA, from the lengths themselves -- the same launch (a
 // graph replay) is balanced for any lengths.  A pair that spans several CTAs
 // leaves partial results in the workspace, and the CTA that arrives last
 // merges them (a counter that wraps to zero by itself).
 namespace dec8 {
 constexpr int D = kvq::D, BS = kvq::BS, WARPS = 4, THREADS = 32 * WARPS, CTAS_PER_SM = 4;
 constexpr int MIN_UNITS = 4 * WARPS;    // a CTA takes at least this many blocks' worth
-constexpr int PAIR_COST = 2 * WARPS;
+constexpr int PAIR_COST = 4 * WARPS;    // measured on ragged lengths: 49 us with 8, 43 with 16 and with 24
 constexpr float WEIGHT_BITS = 8.f;      // the largest weight of 32 tokens is 2^8
 constexpr float RESCALE = 8.f;          // O is rescaled once the maximum has grown by this much
 constexpr int SLOT = 2 * BS * D;        // K (or V) of two blocks
-constexpr int RING = WARPS * 2 * SLOT;
+constexpr int SLOTS = 3;                // per warp: one in use, two on their way
+constexpr int RING = WARPS * SLOTS * SLOT;
+constexpr int O_ROW = D + 4;            // floats of a head's row of O: eight lanes' stores fall on eight banks
 template <int NT>
-struct Smem {                           // ring, then the warps' O in its place | (m, l, mv) | scales | prefix sums
-  static constexpr int O = WARPS * 8 * NT * D * 4;
-  static constexpr int HEAD = RING > O ? RING : O;
-  static constexpr int SCALES = HEAD + WARPS * 8 * NT * 16;
-  static constexpr int PRE = SCALES + WARPS * 2 * 16;
+struct Smem {                           // rings, later the warps' O | their (m, l, mv) | q fragments | prefix sums
+  static constexpr int STATS = RING;
+  static_assert(WARPS * 8 * NT * O_ROW * 4 <= RING, "O fits in the drained rings");
+  static constexpr int Q = STATS + WARPS * 8 * NT * 16;
+  static constexpr int PRE = Q + NT * 4 * 32 * 16;
   static constexpr int bytes(int B) { return PRE + (B + 1) * 4; }
 };
 }  // namespace dec8
@@ -373,9 +375,9 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
                            int* status) {
   using namespace dec8;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* so = reinterpret_cast<float*>(smem);                           // [WARPS][8 NT][D], once the ring is drained
-  float* sm = reinterpret_cast<float*>(smem + Smem<NT>::HEAD);          // [WARPS][8 NT][m, l, mv]
-  float4* sc = reinterpret_cast<float4*>(smem + Smem<NT>::SCALES);      // [WARPS][2] (K, V) scales of two blocks
+  float* so = reinterpret_cast<float*>(smem);                           // [WARPS][8 NT][O_ROW], once the rings are drained
+  float* sm = reinterpret_cast<float*>(smem + Smem<NT>::STATS);         // [WARPS][8 NT][m, l, mv]
+  uint4* sq = reinterpret_cast<uint4*>(smem + Smem<NT>::Q);             // [NT][4 steps][32 lanes]
   int* pre = reinterpret_cast<int*>(smem + Smem<NT>::PRE);              // [B + 1] units of the pairs before sequence b
   __shared__ int wsum[WARPS];
   __shared__ uint32_t ticket;
@@ -420,7 +422,6 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
   const int n_cta = max(1, min((int)gridDim.x, (total + MIN_UNITS - 1) / MIN_UNITS));
   const int per = (total + n_cta - 1) / n_cta;
   const int u0 = min(total, (int)blockIdx.x * per), u1 = min(total, u0 + per);
-
   int b = 0;
   {  // the sequence that holds u0: the last b with pre[b] <= u0
     int lo = 0, hi = B;
@@ -431,42 +432,39 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
     }
     b = lo;
   }
-  for (int u = u0; u < u1;) {
-    while (pre[b + 1] <= u) ++b;
-    const int units = (pre[b + 1] - pre[b]) / Hkv;
-    const int h = (u - pre[b]) / units;                        // KV head
-    const int pair0 = pre[b] + h * units;                      // first unit of the pair
-    const int j0 = max(0, u - pair0 - PAIR_COST), j1 = min(units, u1 - pair0) - PAIR_COST;   // its blocks in this CTA
-    const int next_u = min(pair0 + units, u1);
-    if (j1 <= 0) {                                             // this CTA has none but the pair's fixed cost
-      u = next_u;
-      continue;
-    }
-    const int len = len_of(b);
-
-    // ---- the warp's loads: block pair it = blocks j0 + 2 (warp + WARPS it) + {0, 1}
-    int ids = -1, id0 = -1, id1 = -1;
-    float lks = 0.f, lvs = 0.f;
     // Both land row by row, 512 contiguous bytes per instruction (measured: with
     // every lane fetching the pieces it reads back, K in 64-byte halves and V
     // in every other row, the loads alone took 122 us of 64 x 4096 where these
     // take 96).  16-byte pieces are permuted inside a row so that the fragment
     // reads meet no bank twice: K by the row's lowest bit (two rows at a time
     // are read), V by the two above it (rows 2c, c = 0 .. 3).
-    const uint32_t kslot = smem_u32(smem) + warp * (2 * SLOT), vslot = kslot + SLOT;
-    const uint32_t kput = kslot + (lane >> 3) * D + (((lane & 7) ^ (lane >> 3 & 1) * 4) << 4);
-    const uint32_t kget = kslot + gq * D + ((qd ^ (gq & 1) * 4) << 4);
+    const uint32_t ring = smem_u32(smem) + warp * (SLOTS * SLOT);
+    const uint32_t kput = (lane >> 3) * D + (((lane & 7) ^ (lane >> 3 & 1) * 4) << 4);
+    const uint32_t kget = gq * D + ((qd ^ (gq & 1) * 4) << 4);
     const int khalf = gq & 1 ? -64 : 64;
     const uint32_t vput = (lane >> 3) * D + (((lane & 7) ^ (lane >> 4) * 2) << 4);   // rows 0-3; ^ 64 in rows 4-7
-    const uint32_t vget = vslot + 2 * qd * D + ((gq ^ qd * 2) << 4);
+    const uint32_t vget = 2 * qd * D + ((gq ^ qd * 2) << 4);
     const int vhalf = gq >> 1 & 1;       // 8-byte half of the piece that comes first (bank conflicts again)
-    float2* const scw = reinterpret_cast<float2*>(sc + warp * 2);
-    auto fetch_k = [&](int it) {
-      const int j = j0 + 2 * (warp + it * WARPS);
+
+  for (int u = u0; u < u1;) {
+    // ---- the blocks [j0, j1) of KV head h of sequence b
+    while (pre[b + 1] <= u) ++b;
+    const int units = (pre[b + 1] - pre[b]) / Hkv;
+    const int h = (u - pre[b]) / units;
+    const int pair0 = pre[b] + h * units;                      // first unit of the pair
+    const int j0 = max(0, u - pair0 - PAIR_COST), j1 = min(units, u1 - pair0) - PAIR_COST;
+    u = min(pair0 + units, u1);
+    if (j1 <= 0) continue;                                     // none but the pair's fixed cost
+    const int len = len_of(b);
+
+    // ---- the warp's loads, two blocks at a time: K and V of it, K and V of the next, ...
+    int fj = j0 + 2 * warp, fcount = 0, ids = -1, id0 = -1, id1 = -1;
+    float lks = 0.f, lvs = 0.f;
+    auto fetch_k = [&](uint32_t slot) {
       id0 = id1 = -1;
-      if (j < j1) {
-        if ((it & 15) == 0) {
-          const int mine = j + (lane >> 1) * (2 * WARPS) + (lane & 1);
+      if (fj < j1) {
+        if ((fcount & 15) == 0) {                              // ids of the next 32 blocks, one per lane
+          const int mine = fj + (lane >> 1) * (2 * WARPS) + (lane & 1);
           ids = -1;
           if (mine < j1) {
             ids = tables[(size_t)b * max_blocks + mine];
@@ -475,75 +473,91 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
               ids = -1;
             }
           }
-          lks = ids >= 0 ? c.ks[(size_t)ids * Hkv + h] : -1.f;   // below 0: no block
-          lvs = ids >= 0 ? c.vs[(size_t)ids * Hkv + h] : 0.f;
         }
-        const int l0 = 2 * (it & 15);
-        id0 = __shfl_sync(0xffffffffu, ids, l0);
-        id1 = __shfl_sync(0xffffffffu, ids, l0 + 1);
-        if ((lane >> 1) == (it & 15)) scw[2 * (it & 1) + (lane & 1)] = make_float2(lks, lvs);
+        id0 = __shfl_sync(0xffffffffu, ids, 2 * (fcount & 15));
+        id1 = __shfl_sync(0xffffffffu, ids, 2 * (fcount & 15) + 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int id = i ? id1 : id0;
           if (id < 0) continue;
           const uint8_t* p = c.k + ((size_t)id * Hkv + h) * (BS * D) + lane * 16;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) cp_async16(kput + (4 * i + e) * 512, p + e * 512);
+          for (int e = 0; e < 4; ++e) cp_async16(slot + kput + (4 * i + e) * 512, p + e * 512);
         }
+        if ((fcount & 15) == 0) {                              // their scales: needed when the blocks are used
+          lks = ids >= 0 ? c.ks[(size_t)ids * Hkv + h] : -1.f; // below 0: no block
+          lvs = ids >= 0 ? c.vs[(size_t)ids * Hkv + h] : 0.f;
+        }
+        fj += 2 * WARPS;
+        ++fcount;
       }
       cp_async_commit();
     };
-    auto fetch_v = [&]() {                                     // of the pair whose K was fetched last
+    auto fetch_v = [&](uint32_t slot) {                        // of the blocks whose K was fetched last
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int id = i ? id1 : id0;
         if (id < 0) continue;
         const uint8_t* p = c.v + ((size_t)id * Hkv + h) * (BS * D) + lane * 16;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) cp_async16(vslot + (4 * i + e) * 512 + (vput ^ (e & 1) * 64), p + e * 512);
+        for (int e = 0; e < 4; ++e) cp_async16(slot + (4 * i + e) * 512 + (vput ^ (e & 1) * 64), p + e * 512);
       }
       cp_async_commit();
     };
-    fetch_k(0);
-    fetch_v();
-
-    // ---- q fragments: step i covers words 2 (i % 2), 2 (i % 2) + 1 of the pieces i / 2
-    uint32_t qa[NT][4][4];
+    float ks0, ks1, vs0, vs1;                                  // scales of the two blocks in use
+    auto scales = [&](int n) {                                 // of the warp's n-th two blocks
+      const int at = 2 * (n & 15);
+      ks0 = __shfl_sync(0xffffffffu, lks, at);
+      ks1 = __shfl_sync(0xffffffffu, lks, at + 1);
+      vs0 = __shfl_sync(0xffffffffu, lvs, at);
+      vs1 = __shfl_sync(0xffffffffu, lvs, at + 1);
+    };
+    // ---- q fragments: step i covers words 2 (i % 2), 2 (i % 2) + 1 of the pieces i / 2; warp i makes it
     float qf[NT];
+    u128 raw[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)                              // 8 dims at (i / 2) * 64 + qd * 16 + (i % 2) * 8
+        raw[nt][i] = gq + 8 * nt < G ? ld_v4(q + (size_t)b * ldq + (size_t)(h * G + gq + 8 * nt) * D + (i >> 1) * 64 +
+                                             qd * 16 + (i & 1) * 8)
+                                     : u128{0, 0, 0, 0};
+    uint32_t s0 = ring, s1 = ring + SLOT, s2 = ring + 2 * SLOT;   // K in use, V in use, the next K
+    fetch_k(s0);
+    fetch_v(s1);
+    fetch_k(s2);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int hh = gq + 8 * nt;
-      u128 raw[4];
       float am = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {                            // 8 dims at (i / 2) * 64 + qd * 16 + (i % 2) * 8
-        raw[i] = hh < G ? ld_v4(q + (size_t)b * ldq + (size_t)(h * G + hh) * D + (i >> 1) * 64 + qd * 16 + (i & 1) * 8)
-                        : u128{0, 0, 0, 0};
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          am = fmaxf(am, fmaxf(finite_or_zero(bf16_lo(word(raw[i], e))), finite_or_zero(bf16_hi(word(raw[i], e)))));
-      }
+          am = fmaxf(am, fmaxf(finite_or_zero(bf16_lo(word(raw[nt][i], e))), finite_or_zero(bf16_hi(word(raw[nt][i], e)))));
       am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
       am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
       const int eq = min(max((int)(__float_as_uint(am) >> 23) - 127 - 8 + ((__float_as_uint(am) & 0x7fffffu) > 0x600000u), -126), 126);
       const float down = exp2_int(-eq);
       qf[nt] = exp2_int(eq) * scale_log2;
+      static_assert(WARPS == 4, "a warp per step");
+      const u128 mine = warp == 0 ? raw[nt][0] : warp == 1 ? raw[nt][1] : warp == 2 ? raw[nt][2] : raw[nt][3];
+      uint32_t part4[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int e = 0; e < 2; ++e) {                            // four dims: words 2e, 2e + 1 of the bf16 piece
+        float f[4] = {bf16_lo(word(mine, 2 * e)), bf16_hi(word(mine, 2 * e)), bf16_lo(word(mine, 2 * e + 1)),
+                      bf16_hi(word(mine, 2 * e + 1))};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {                          // four dims: words 2e, 2e + 1 of the bf16 piece
-          float f[4] = {bf16_lo(word(raw[i], 2 * e)), bf16_hi(word(raw[i], 2 * e)), bf16_lo(word(raw[i], 2 * e + 1)),
-                        bf16_hi(word(raw[i], 2 * e + 1))};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) f[k] = scaled_or_nan(f[k], down);
-          uint16_t h0, h1, l0, l1;
-          split_e4m3x2(f[0], f[1], h0, l0);
-          split_e4m3x2(f[2], f[3], h1, l1);
-          qa[nt][i][2 * e] = pair16(h0, h1);
-          qa[nt][i][2 * e + 1] = pair16(l0, l1);
-        }
+        for (int k = 0; k < 4; ++k) f[k] = scaled_or_nan(f[k], down);
+        uint16_t h0, h1, l0, l1;
+        split_e4m3x2(f[0], f[1], h0, l0);
+        split_e4m3x2(f[2], f[3], h1, l1);
+        part4[2 * e] = pair16(h0, h1);
+        part4[2 * e + 1] = pair16(l0, l1);
       }
+      // (larger, rest) of words 2e and 2e + 1
+      sq[(nt * 4 + warp) * 32 + lane] = make_uint4(part4[0], part4[1], part4[2], part4[3]);
     }
+    __syncthreads();
 
     float o[NT][8][4];
     float m[NT], l[NT], mv[NT];
@@ -556,14 +570,14 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][mt][e] = 0.f;
     }
-    for (int it = 0, j = j0 + 2 * warp; j < j1; ++it, j += 2 * WARPS) {
-      cp_async_wait<1>();                                      // K of this pair
-      __syncwarp();                                            // of every lane, and its scales
-      const float4 scale = sc[warp * 2 + (it & 1)];            // K, V of the first block, K, V of the second
+    scales(0);
+    for (int j = j0 + 2 * warp; j < j1; j += 2 * WARPS) {
+      cp_async_wait<2>();                                      // K of these blocks
+      __syncwarp();                                            // of every lane
       float x[NT][8];                                          // logits: 4 of each block
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float ks = i ? scale.z : scale.x;
+        const float ks = i ? ks1 : ks0;
         if (ks < 0.f) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -573,22 +587,26 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
         }
         u128 kr[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) kr[e] = lds16(kget + (e & 1) * khalf + i * (BS * D) + (e >> 1) * 8 * D);
+        for (int e = 0; e < 4; ++e) kr[e] = lds16(s0 + kget + (e & 1) * khalf + i * (BS * D) + (e >> 1) * 8 * D);
         float s[2][4];                                         // tokens 0-7, 8-15 of the block
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.f;
 #pragma unroll
-        for (int st = 0; st < 4; ++st)
+        for (int st = 0; st < 4; ++st) {
+          uint4 qa[NT];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) qa[nt] = sq[(nt * 4 + st) * 32 + lane];
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt) {
             const uint32_t b0 = word(kr[2 * tt + (st >> 1)], 2 * (st & 1)), b1 = word(kr[2 * tt + (st >> 1)], 2 * (st & 1) + 1);
             if (NT == 1) {                                     // rows 0-7 the larger parts, rows 8-15 the rest
-              mma_e4m3(s[tt], qa[0][st][0], qa[0][st][1], qa[0][st][2], qa[0][st][3], b0, b1);
+              mma_e4m3(s[tt], qa[0].x, qa[0].y, qa[0].z, qa[0].w, b0, b1);
             } else {                                           // rows: 16 heads; the parts one after the other
-              mma_e4m3(s[tt], qa[0][st][0], qa[NT - 1][st][0], qa[0][st][2], qa[NT - 1][st][2], b0, b1);
-              mma_e4m3(s[tt], qa[0][st][1], qa[NT - 1][st][1], qa[0][st][3], qa[NT - 1][st][3], b0, b1);
+              mma_e4m3(s[tt], qa[0].x, qa[NT - 1].x, qa[0].z, qa[NT - 1].z, b0, b1);
+              mma_e4m3(s[tt], qa[0].y, qa[NT - 1].y, qa[0].w, qa[NT - 1].w, b0, b1);
             }
           }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float f = qf[nt] * ks;
@@ -598,7 +616,7 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
         }
       }
       __syncwarp();                                            // K has been read by all
-      fetch_k(it + 1);
+      fetch_v(s0);                                             // of the next blocks
       const int tok0 = j * BS + 2 * qd;                        // this lane's tokens: + {0, 1, 8, 9} of each block
       const bool tail = (j + 2) * BS > len;
       if (tail) {
@@ -608,8 +626,8 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) x[nt][e] = -INFINITY;
       }
-      const float e0 = (float)((int)(__float_as_uint(scale.y) >> 23) - 127);
-      const float e1 = (float)((int)(__float_as_uint(scale.w) >> 23) - 127);
+      const float e0 = (float)((int)(__float_as_uint(vs0) >> 23) - 127);
+      const float e1 = (float)((int)(__float_as_uint(vs1) >> 23) - 127);
       uint32_t wh[NT][2], wl[NT][2];                           // weights' two parts: B fragments of the second product
       float alpha[NT], beta[NT];
       bool grow = false;
@@ -666,18 +684,18 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
         bc[nt][0] = __shfl_sync(0xffffffffu, beta[nt], 8 * qd);
         bc[nt][1] = __shfl_sync(0xffffffffu, beta[nt], 8 * qd + 4);
       }
-      cp_async_wait<1>();                                      // V of this pair
+      cp_async_wait<2>();                                      // V of these blocks
       __syncwarp();
-      const bool gaps = tail || scale.x < 0.f || scale.z < 0.f;
+      const bool gaps = tail || ks0 < 0.f || ks1 < 0.f;
 #pragma unroll
       for (int w2 = 0; w2 < 2; ++w2) {                         // 8 dims of each token: MMA tiles 4 w2 ..
         uint2 vr[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) vr[e] = lds8(vget + (e >> 2) * (BS * D) + ((e >> 1 & 1) * 8 + (e & 1)) * D + 8 * (w2 ^ vhalf));
+        for (int e = 0; e < 8; ++e) vr[e] = lds8(s1 + vget + (e >> 2) * (BS * D) + ((e >> 1 & 1) * 8 + (e & 1)) * D + 8 * (w2 ^ vhalf));
         if (gaps) {                                            // rows never written: 0 x NaN would poison O
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (tok0 + (e & 1) + ((e >> 1) & 1) * 8 + (e >> 2) * BS >= len || (e < 4 ? scale.x : scale.z) < 0.f)
+            if (tok0 + (e & 1) + ((e >> 1) & 1) * 8 + (e >> 2) * BS >= len || (e < 4 ? ks0 : ks1) < 0.f)
               vr[e] = make_uint2(0, 0);
         }
 #pragma unroll
@@ -704,71 +722,74 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
 #pragma unroll
               for (int e = 0; e < 4; ++e) o[nt][4 * w2 + 2 * w + hf][e] += t[e] * bc[nt][e & 1];
             }
-          if (w2 == 1 && w == 0) {                             // every lane has read all of its V by now
-            __syncwarp();
-            fetch_v();
-          }
         }
       }
+      __syncwarp();                                            // V has been read by all
+      scales(fcount - 1);                                      // before the fetch may replace them
+      fetch_k(s1);
+      const uint32_t t = s0;                                   // next: K in s2, V in s0, the K after it in s1
+      s0 = s2;
+      s2 = s1;
+      s1 = t;
     }
     cp_async_wait<0>();
-
-    // ---- the warps' results of this pair
     __syncthreads();                                           // every warp has drained its ring
+
+    // ---- the warps' results of this run
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float ls = l[nt];
       ls += __shfl_xor_sync(0xffffffffu, ls, 1);
       ls += __shfl_xor_sync(0xffffffffu, ls, 2);
-      if (qd == 0) {
-        float* p = sm + (warp * 8 * NT + nt * 8 + gq) * 4;
-        p[0] = m[nt];
-        p[1] = ls;
-        p[2] = mv[nt];
-      }
+      if (qd == 0) *reinterpret_cast<float4*>(sm + (warp * 8 * NT + nt * 8 + gq) * 4) = make_float4(m[nt], ls, mv[nt], 0.f);
+      // dim gq * 16 + k of a head in column k * 8 + gq
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          so[(warp * 8 * NT + nt * 8 + 2 * qd + (e & 1)) * D + gq * 16 + 2 * (mt ^ 4 * vhalf) + (e >> 1)] = o[nt][mt][e];
+          so[(warp * 8 * NT + nt * 8 + 2 * qd + (e & 1)) * O_ROW + (2 * (mt ^ 4 * vhalf) + (e >> 1)) * 8 + gq] = o[nt][mt][e];
     }
     __syncthreads();
     // the CTAs that share the pair; the first may start inside the pair's fixed cost
     const int c0 = (pair0 + PAIR_COST) / per, c1 = (pair0 + units - 1) / per;
-    // thread: dim tid of every head
-    for (int hh = 0; hh < G; ++hh) {
+    // two heads at a time, a thread for two dims of one
+    for (int hh = tid >> 6; hh < G; hh += 2) {
+      const int d16 = tid & 7, d2 = tid >> 3 & 7, dim = d16 * 16 + 2 * d2;
+      float4 st[WARPS];
       float M = -INFINITY, MV = -INFINITY;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float* p = sm + (w * 8 * NT + hh) * 4;
-        M = fmaxf(M, p[0]);
-        MV = fmaxf(MV, p[2]);
+        st[w] = *reinterpret_cast<const float4*>(sm + (w * 8 * NT + hh) * 4);
+        M = fmaxf(M, st[w].x);
+        MV = fmaxf(MV, st[w].z);
       }
       const float mb = M == -INFINITY ? 0.f : M, vb = MV == -INFINITY ? 0.f : MV;
-      float num = 0.f, den = 0.f;
+      float2 num = make_float2(0.f, 0.f);
+      float den = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float* p = sm + (w * 8 * NT + hh) * 4;
-        num += so[(w * 8 * NT + hh) * D + tid] * ex2(p[2] - vb);
-        den += p[1] * ex2(p[0] - mb);
+        const float* p = so + (w * 8 * NT + hh) * O_ROW + 16 * d2 + d16;
+        const float f = ex2(st[w].z - vb);
+        num.x += p[0] * f;
+        num.y += p[8] * f;
+        den += st[w].y * ex2(st[w].x - mb);
       }
       if (c0 == c1) {
-        out[(size_t)b * ldo + (size_t)(h * G + hh) * D + tid] =
-            __float2bfloat16(den == 0.f ? 0.f : num / den * ex2(vb - mb));
+        const float inv = den == 0.f ? 0.f : ex2(vb - mb) / den;
+        *reinterpret_cast<uint32_t*>(out + (size_t)b * ldo + (size_t)(h * G + hh) * D + dim) =
+            pack_bf16x2(num.x * inv, num.y * inv);
       } else {   // a CTA's first pair goes to its slot 0, its last to slot 1
         float* p = part + ((size_t)(blockIdx.x * 2 + (pair0 <= u0 ? 0 : 1)) * G + hh) * DEC8_ROW;
-        p[tid] = num;
-        if (tid == 0) {
-          p[D] = M;
-          p[D + 1] = den;
-          p[D + 2] = MV;
+        *reinterpret_cast<float2*>(p + dim) = num;
+        if ((tid & 63) == 0) {
+          *reinterpret_cast<float4*>(p + D) = make_float4(M, den, MV, 0.f);
         }
       }
     }
     if (c0 != c1) {
       __threadfence();
       __syncthreads();
-      if (tid == 0) ticket = atomicInc(&counters[b * Hkv + h], (uint32_t)(c1 - c0));   // wraps to 0 at the last
+      if (tid == 0) ticket = atomicInc(&counters[b * Hkv + h], (uint32_t)(c1 - c0));
       __syncthreads();
       if (ticket == (uint32_t)(c1 - c0)) {
         __threadfence();
@@ -777,41 +798,49 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
           auto slot = [&](int cc) {
             return part + ((size_t)(cc * 2 + (pair0 <= cc * per ? 0 : 1)) * G + hh) * DEC8_ROW;
           };
-          float M = -INFINITY, MV = -INFINITY;
-          for (int cc = c0 + lane; cc <= c1; cc += 32) {
-            M = fmaxf(M, __ldcg(slot(cc) + D));
-            MV = fmaxf(MV, __ldcg(slot(cc) + D + 2));
-          }
-          M = warp_max(M);
-          MV = warp_max(MV);
-          const float mb = M == -INFINITY ? 0.f : M, vb = MV == -INFINITY ? 0.f : MV;
+          float m_all = -INFINITY, mv_all = -INFINITY, den = 0.f;
           float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-          float den = 0.f;
-          for (int cb = c0; cb <= c1; cb += 32) {
-            const int mine = cb + lane, n = min(32, c1 - cb + 1);
-            float f = 0.f;
-            if (mine <= c1) {
-              den += __ldcg(slot(mine) + D + 1) * ex2(__ldcg(slot(mine) + D) - mb);
-              f = ex2(__ldcg(slot(mine) + D + 2) - vb);
-            }
-            for (int i = 0; i < n; i += 8) {
-              float4 x[8];
+          for (int cb = c0; cb <= c1; cb += 32) {              // 32 CTAs at a time, rescaled as the maxima grow
+            const int n = min(32, c1 - cb + 1);
+            const float4 st = lane < n ? __ldcg(reinterpret_cast<const float4*>(slot(cb + lane) + D))
+                                       : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+            float4 x[8];
+            auto rows = [&](int i) {
 #pragma unroll
               for (int k = 0; k < 8; ++k)
                 x[k] = i + k < n ? __ldcg(reinterpret_cast<const float4*>(slot(cb + i + k)) + lane)
                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+            };
+            rows(0);                                           // on their way while the maxima are found
+            const float m_new = fmaxf(m_all, warp_max(st.x)), mv_new = fmaxf(mv_all, warp_max(st.z));
+            const float mb = m_new == -INFINITY ? 0.f : m_new, vb = mv_new == -INFINITY ? 0.f : mv_new;
+            const float fv = ex2(mv_all - vb);
+            den = den * ex2(m_all - mb) + st.y * ex2(st.x - mb);
+            num.x *= fv;
+            num.y *= fv;
+            num.z *= fv;
+            num.w *= fv;
+            m_all = m_new;
+            mv_all = mv_new;
+            const float f = ex2(st.z - vb);
+            for (int i = 0; i < n; i += 8) {
+              float4 y[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) y[k] = x[k];
+              if (i + 8 < n) rows(i + 8);
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
                 const float g = __shfl_sync(0xffffffffu, f, (i + k) & 31);
                 if (i + k < n) {
-                  num.x += x[k].x * g;
-                  num.y += x[k].y * g;
-                  num.z += x[k].z * g;
-                  num.w += x[k].w * g;
+                  num.x += y[k].x * g;
+                  num.y += y[k].y * g;
+                  num.z += y[k].z * g;
+                  num.w += y[k].w * g;
                 }
               }
             }
           }
+          const float mb = m_all == -INFINITY ? 0.f : m_all, vb = mv_all == -INFINITY ? 0.f : mv_all;
           den = warp_sum(den);
           const float inv = den == 0.f ? 0.f : ex2(vb - mb) / den;
           uint2 w;
@@ -821,8 +850,7 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
         }
       }
     }
-    u = next_u;
-    __syncthreads();                                           // so is read before the ring fills again
+    __syncthreads();                                           // O and the statistics have been read
   }
 }
 

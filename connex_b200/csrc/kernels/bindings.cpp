@@ -294,7 +294,7 @@ void rope_cache_fp8(const at::Tensor& qkv, const at::Tensor& pos, const at::Tens
   CHECK_CUDA(qkv);
   const c10::cuda::CUDAGuard g(qkv.device());
   cx::rope_cache_fp8(qkv.data_ptr(), ldq, pos.data_ptr<int>(), cos_sin.data_ptr<float>(), slots.data_ptr<int64_t>(), c,
-                     out.data_ptr(), ldo, (int)T, (int)Hq, (int)std::min<int64_t>(cos_sin.size(0), INT_MAX),
+                     out.data_ptr(), ldo, (int)T, (int)Hq, (int)std::min<int64_t>(cos_sin.size(0), INT_MAX), sms_of(qkv),
                      status_ptr(status), cur_stream(qkv), qn, kn, (float)eps);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
@@ -347,7 +347,8 @@ void kv_copy_blocks(at::Tensor& kv, const at::Tensor& pairs, const c10::optional
   const int64_t n = pairs.size(0), block = kv.size(3) * kv.size(4) * kv.size(5) * kv.element_size();
   TORCH_CHECK(block % 16 == 0 && (reinterpret_cast<uintptr_t>(kv.data_ptr()) & 15) == 0,
               "kv_copy_blocks: blocks must be multiples of 16 bytes on 16-byte boundaries");
-  TORCH_CHECK(n <= INT_MAX && kv.size(0) * 2 <= 65535 && kv.size(2) <= INT_MAX, "kv_copy_blocks: too many blocks");
+  TORCH_CHECK(n <= INT_MAX && kv.size(0) * 2 <= 65535 && kv.size(2) <= INT_MAX && kv.size(0) * 2 * (block / 16) <= INT_MAX / 2,
+              "kv_copy_blocks: too many blocks, or blocks too large");
   float* sp = nullptr;
   if (scales.has_value()) {
     check_same_device(kv, {&*scales}, "kv_copy_blocks");

@@ -8,6 +8,7 @@
 // smallest e4m3 step), and every cached value is an exact bf16 number.
 #include <algorithm>
 #include <stdexcept>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kv_fp8.h"
@@ -17,7 +18,8 @@ namespace cx {
 namespace kvq {
 constexpr int D = 128, BS = 16;
 constexpr int MIN_EXP = -100, MAX_EXP = 120;   // 448 * 2^120 covers every finite bf16
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int SMEM = BS * D * 4 + WARPS * BS * D * 2;   // cos / sin rows, each warp's rows
 }  // namespace kvq
 
 // 2^e for e of [-126, 127]
@@ -67,198 +69,349 @@ __device__ __forceinline__ float scaled_or_nan(float x, float mul) {
   return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fffffffu) : x * mul;
 }
 
-// ------------------------------------------------- RoPE + quantising write
-// One CTA per token.  All 256 threads rotate the token's q heads (16 lanes of
-// 16 bytes per head).  The CTA of the first token that falls into a block
-// also writes the block: its scale depends on every row that this call puts
-// there, so one CTA collects them -- a scan of the call's slots, which keeps
-// the result independent of the rows' order (of two rows for one slot the
-// later wins) -- and each warp takes one KV head of K or V: rotated rows in
-// registers, their largest magnitude, the scale, the block's older rows
-// requantised if the scale grew, the new rows.  A block whose row 0 is
-// written starts anew; otherwise its scale never shrinks.
-__global__ void __launch_bounds__(kvq::THREADS)
-    rope_cache_fp8_kernel(const __nv_bfloat16* qkv, int ldq, const int* __restrict__ pos,
-                          const float* __restrict__ cos_sin, const int64_t* __restrict__ slots, KvFp8 c,
-                          __nv_bfloat16* out, int ldo, int T, int Hq, int max_pos, int* status,
-                          const __nv_bfloat16* __restrict__ qn, const __nv_bfloat16* __restrict__ kn, float eps) {
-  using namespace kvq;
-  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int p = pos[t];
-  const bool pos_ok = p >= 0 && p < max_pos;
-  const int64_t slot = slots[t];
-  const int64_t blk = slot >> 4;
-  if (tid == 0 && (!pos_ok || (slot >= 0 && blk >= c.num_blocks))) record_status(status, CX_ERR_BOUNDS);
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ u128 lds16(uint32_t a) {
+  u128 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ void sts16(uint32_t a, const u128& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint64_t unpack_bf16x2(uint32_t w) { return f32x2(bf16_lo(w), bf16_hi(w)); }
+// larger magnitudes of two bf16 pairs, signs undefined; NaN only where both are
+__device__ __forceinline__ uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// a cos + b sin of a pair of dims, rounded to bf16
+__device__ __forceinline__ uint32_t turn_bf16x2(uint32_t a, uint32_t b, uint64_t co, uint64_t si) {
+  const uint64_t r = fma_f32x2(unpack_bf16x2(b), si, mul_f32x2(unpack_bf16x2(a), co));
+  return pack_bf16x2(lo_f32(r), hi_f32(r));
+}
+struct alignas(16) f32x4 {        // two pairs of fp32
+  uint64_t a, b;
+};
 
-  // ---- this token's block, if it is the first of its rows
+// ------------------------------------------------- RoPE + quantising write
+// CTAs of two kinds.  Block CTAs write the cache.  A block's scale depends on
+// every row that the call puts there, so one CTA collects them: the one whose
+// token is the first to fall into the block scans the call's slots, which
+// keeps the result independent of the rows' order (of two rows for one slot
+// the later wins).  Each of its warps takes K or V of one KV head on its own:
+// all rows' loads in flight together, K rotated, the largest magnitude, the
+// scale, the block's older rows requantised if the scale grew, the new rows.  A block whose row 0 is written
+// starts anew; otherwise its scale never shrinks.  Tokens are dealt to these
+// CTAs with an odd stride: the first rows of blocks, every 16th token of a
+// prompt, then spread over all of them, and so do the rows of decode steps.
+// Rotation CTAs take the q heads, eight of a token per warp at a time.
+__device__ __forceinline__ void write_block(const __nv_bfloat16* qkv, int ldq, const int* pos, const float* cos_sin,
+                                            const int64_t* slots, const KvFp8& c, int t, int blk, int group, int T,
+                                            int Hq, int max_pos, const __nv_bfloat16* kn, float eps) {
+  using namespace kvq;
   __shared__ int row_of[BS];      // the token of each row of the block (-1: not written by this call)
   __shared__ int first;
-  bool lead = pos_ok && slot >= 0 && blk < c.num_blocks;
-  if (lead && t > 0) {            // most tokens of a prompt follow one of the same block
-    const int64_t s1 = slots[t - 1];
-    const int p1 = pos[t - 1];
-    lead = !(s1 >= 0 && (s1 >> 4) == blk && p1 >= 0 && p1 < max_pos);
-  }
-  if (lead) {                     // uniform over the CTA
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // which rows the call writes, and whether t is the first of their tokens
+  auto scan = [&](bool check) {
+    __syncthreads();
     if (tid < BS) row_of[tid] = -1;
     if (tid == 0) first = 0x7fffffff;
     __syncthreads();
-    for (int i = tid; i < T; i += THREADS) {
-      const int64_t si = slots[i];
-      if (si >= 0 && (si >> 4) == blk) {
-        const int pi = pos[i];
-        if (pi >= 0 && pi < max_pos) {
-          atomicMax(&row_of[(int)(si & 15)], i);
-          atomicMin(&first, i);
-        }
+    auto take = [&](int i, int64_t si) {
+      if ((si >> 4) != blk) return;                     // below 0: not cached
+      atomicMin(&first, i);
+      if (!check || (pos[i] >= 0 && pos[i] < max_pos)) atomicMax(&row_of[(int)(si & 15)], i);
+    };
+    if ((reinterpret_cast<uintptr_t>(slots) & 15) == 0) {
+#pragma unroll 8
+      for (int i = 2 * tid; i < (T & ~1); i += 2 * THREADS) {
+        const longlong2 s2 = *reinterpret_cast<const longlong2*>(slots + i);
+        take(i, s2.x);
+        take(i + 1, s2.y);
       }
+      if ((T & 1) && tid == 0) take(T - 1, slots[T - 1]);
+    } else {
+      for (int i = tid; i < T; i += THREADS) take(i, slots[i]);
     }
     __syncthreads();
-    lead = first == t;
+  };
+  scan(false);
+  if (first != t) return;         // uniform over the CTA
+  int tok = row_of[lane & 15], ptok = tok >= 0 ? pos[tok] : 0;     // lane r (and r + 16): row r
+  if (__any_sync(0xffffffffu, ptok < 0 || ptok >= max_pos)) {      // positions out of range: those rows do not count
+    scan(true);
+    tok = row_of[lane & 15];
+    ptok = tok >= 0 ? pos[tok] : 0;
   }
-  if (lead) {
-    const int half = lane >> 4, i4 = 4 * (lane & 15);   // this lane: dims [4 lane, 4 lane + 4)
-    for (int item = warp; item < 2 * c.Hkv; item += THREADS / 32) {
-      const bool is_v = item >= c.Hkv;
-      const int h = is_v ? item - c.Hkv : item;
-      const __nv_bfloat16* src = qkv + (size_t)(Hq + item) * D + 4 * lane;
-      uint32_t x[BS][2];          // bf16 pairs of the new rows
-      float amax = 0.f;
-#pragma unroll
-      for (int r = 0; r < BS; ++r) {
-        const int tok = row_of[r];
-        if (tok < 0) continue;    // uniform over the warp
-        const uint2 raw = *reinterpret_cast<const uint2*>(src + (size_t)tok * ldq);
-        x[r][0] = raw.x;
-        x[r][1] = raw.y;
-        if (!is_v) {
-          float a[4] = {bf16_lo(raw.x), bf16_hi(raw.x), bf16_lo(raw.y), bf16_hi(raw.y)};
-          if (kn != nullptr) {
-            const float ss = warp_sum(a[0] * a[0] + a[1] * a[1] + a[2] * a[2] + a[3] * a[3]);
-            const float n = rsqrtf(ss * (1.0f / D) + eps);
-            const uint2 w = *reinterpret_cast<const uint2*>(kn + 4 * lane);
-            // bf16 between the norm and the rotation, like a norm layer of its own
-            const uint32_t y0 = pack_bf16x2(a[0] * n * bf16_lo(w.x), a[1] * n * bf16_hi(w.x));
-            const uint32_t y1 = pack_bf16x2(a[2] * n * bf16_lo(w.y), a[3] * n * bf16_hi(w.y));
-            a[0] = bf16_lo(y0); a[1] = bf16_hi(y0); a[2] = bf16_lo(y1); a[3] = bf16_hi(y1);
-          }
-          const float* cs = cos_sin + (size_t)pos[tok] * D + i4;
-          const float4 co = *reinterpret_cast<const float4*>(cs), si = *reinterpret_cast<const float4*>(cs + D / 2);
-          float b[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) b[e] = __shfl_xor_sync(0xffffffffu, a[e], 16);
-          const float sg = half ? 1.f : -1.f;   // first half: a cos - b sin; second: a cos + b sin
-          // rounded to bf16 before e4m3: what a bf16 cache would hold is what is quantised
-          x[r][0] = pack_bf16x2(a[0] * co.x + sg * b[0] * si.x, a[1] * co.y + sg * b[1] * si.y);
-          x[r][1] = pack_bf16x2(a[2] * co.z + sg * b[2] * si.z, a[3] * co.w + sg * b[3] * si.w);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          amax = fmaxf(amax, fmaxf(finite_or_zero(bf16_lo(x[r][e])), finite_or_zero(bf16_hi(x[r][e]))));
-      }
-      amax = warp_max(amax);
-      float* scale = (is_v ? c.vs : c.ks) + (size_t)blk * c.Hkv + h;
-      uint8_t* dst = (is_v ? c.v : c.k) + ((size_t)blk * c.Hkv + h) * (BS * D) + 4 * lane;
-      int e = fp8_exp_for(amax);
-      if (row_of[0] < 0) {        // the block's rows so far stay
-        const int old = fp8_exp_of(*scale);
-        if (e <= old) {
-          e = old;
-        } else {
-          const float f = exp2_int(max(old - e, -126));
+  const uint32_t rows = __ballot_sync(0xffffffffu, tok >= 0) & 0xffffu;
+  if (rows == 0) return;
+  // A warp: K or V of one head; step i: rows 2i and 2i + 1, 16 lanes of 8 dims
+  // each.  The rows pass through shared memory: asynchronous copies, all in
+  // flight at once.  (Kept in registers instead, with the loops unrolled, the
+  // same rows took 47 us of 8192 where this takes 43, and 5.3 us of 64 decode
+  // rows where this takes 4.1: the code is long for what each CTA runs once.)
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int half = lane >> 4, j = lane & 15;
+  const uint32_t table = smem_u32(smem), mine = table + BS * D * 4 + warp * (BS * D * 2) + half * (D * 2) + j * 16;
+  __syncthreads();                // the previous block is done with the table
+  for (int r = warp; r < BS; r += WARPS) {              // cos / sin: a row per warp at a time
+    const int pr = __shfl_sync(0xffffffffu, ptok, r);
+    if (rows >> r & 1) cp_async16(table + r * (D * 4) + lane * 16, cos_sin + (size_t)pr * D + lane * 4);
+  }
+  const int h = (group * WARPS + warp) >> 1;            // K in the even warps, V in the odd ones
+  const bool on = h < c.Hkv, is_v = warp & 1;
+  float* scale = (is_v ? c.vs : c.ks) + (size_t)blk * c.Hkv + h;
+  float old = 1.f;
+  if (on) {
+    old = *scale;
+    const __nv_bfloat16* src = qkv + (size_t)(Hq + (is_v ? c.Hkv : 0) + h) * D + 8 * j;
 #pragma unroll 4
-          for (int r = 0; r < BS; ++r) {
-            if (row_of[r] >= 0) continue;
-            uint32_t* q = reinterpret_cast<uint32_t*>(dst + r * D);
-            const uint32_t w = *q;
-            const uint32_t a = e4m3x2_to_f16x2((uint16_t)w), b = e4m3x2_to_f16x2((uint16_t)(w >> 16));
-            *q = to_e4m3x2(f16_lo(a) * f, f16_hi(a) * f) | to_e4m3x2(f16_lo(b) * f, f16_hi(b) * f) << 16;
-          }
+    for (int i = 0; i < 8; ++i) {
+      const int tr = __shfl_sync(0xffffffffu, tok, 2 * i + half);
+      if (tr >= 0) cp_async16(mine + i * (D * 4), src + (size_t)tr * ldq);
+    }
+  }
+  cp_async_commit();
+  cp_async_wait<0>();
+  __syncthreads();                                    // the table
+  if (!on) return;
+  uint32_t top = 0;
+#pragma unroll 2
+  for (int i = 0; i < 8; ++i) {
+    if (!(rows >> 2 * i & 3)) continue;               // uniform over the warp
+    const bool here = rows >> (2 * i + half) & 1;
+    u128 x = here ? lds16(mine + i * (D * 4)) : u128{0, 0, 0, 0};
+    uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+    if (!is_v) {
+      u128 y = here ? lds16(mine + (j < 8 ? D : -D) + i * (D * 4)) : u128{0, 0, 0, 0};   // the partner dims, 64 away
+      uint32_t* z = reinterpret_cast<uint32_t*>(&y);
+      __syncwarp();                                   // both halves of a row are read before one is written
+      if (kn != nullptr) {
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ss += bf16_lo(w[e]) * bf16_lo(w[e]) + bf16_hi(w[e]) * bf16_hi(w[e]);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float n = rsqrtf(ss * (1.0f / D) + eps);
+        const u128 nw = ld_v4(kn + 8 * j), nz = ld_v4(kn + 8 * (j ^ 8));
+        const uint32_t *pw = reinterpret_cast<const uint32_t*>(&nw), *pz = reinterpret_cast<const uint32_t*>(&nz);
+        // bf16 between the norm and the rotation, like a norm layer of its own
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = pack_bf16x2(bf16_lo(w[e]) * n * bf16_lo(pw[e]), bf16_hi(w[e]) * n * bf16_hi(pw[e]));
+          z[e] = pack_bf16x2(bf16_lo(z[e]) * n * bf16_lo(pz[e]), bf16_hi(z[e]) * n * bf16_hi(pz[e]));
         }
       }
-      __syncwarp();               // every lane has read the old scale
-      if (lane == 0) *scale = exp2_int(e);
-      const float mul = exp2_int(-e);
+      const uint32_t flip = j < 8 ? 0x80008000u : 0u; // first half: a cos - b sin; second: a cos + b sin
+      const uint32_t cs = table + (2 * i + half) * (D * 4) + (j & 7) * 32;
 #pragma unroll
-      for (int r = 0; r < BS; ++r) {
-        if (row_of[r] < 0) continue;
-        const uint32_t lo = to_e4m3x2(scaled_or_nan(bf16_lo(x[r][0]), mul), scaled_or_nan(bf16_hi(x[r][0]), mul));
-        const uint32_t hi = to_e4m3x2(scaled_or_nan(bf16_lo(x[r][1]), mul), scaled_or_nan(bf16_hi(x[r][1]), mul));
-        *reinterpret_cast<uint32_t*>(dst + r * D) = lo | hi << 16;
+      for (int e = 0; e < 2; ++e) {
+        const u128 co = lds16(cs + 16 * e), si = lds16(cs + 2 * D + 16 * e);
+        const f32x4 &c4 = reinterpret_cast<const f32x4&>(co), &s4 = reinterpret_cast<const f32x4&>(si);
+        // rounded to bf16 before e4m3: what a bf16 cache would hold is what is quantised
+        w[2 * e] = turn_bf16x2(w[2 * e], z[2 * e] ^ flip, c4.a, s4.a);
+        w[2 * e + 1] = turn_bf16x2(w[2 * e + 1], z[2 * e + 1] ^ flip, c4.b, s4.b);
+      }
+      if (here) sts16(mine + i * (D * 4), x);
+      else x = u128{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max_abs_bf16x2(top, w[e]);
+  }
+  top &= 0x7fff7fffu;
+  float amax = fmaxf(bf16_lo(top), bf16_hi(top));
+  // Inf or NaN among the new rows: they have no part in the scale
+  const bool special = __any_sync(0xffffffffu, (top & 0xffffu) >= 0x7f80u || top >= 0x7f800000u);
+  if (special) {
+    amax = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const u128 x = rows >> (2 * i + half) & 1 ? lds16(mine + i * (D * 4)) : u128{0, 0, 0, 0};
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fmaxf(finite_or_zero(bf16_lo(w[e])), finite_or_zero(bf16_hi(w[e]))));
+    }
+  }
+  amax = warp_max(amax);
+  uint8_t* dst = (is_v ? c.v : c.k) + ((size_t)blk * c.Hkv + h) * (BS * D) + half * D + 8 * j;
+  int e = fp8_exp_for(amax);
+  if (!(rows & 1)) {            // the block's rows so far stay
+    const int was = fp8_exp_of(old);
+    if (e <= was) {
+      e = was;
+    } else {
+      const float f = exp2_int(max(was - e, -126));
+      uint2 w[8];                                     // all loads before the first store
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const uint2*>(dst + 2 * i * D);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (rows >> (2 * i + half) & 1) continue;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t& v = k ? w[i].y : w[i].x;
+          const uint32_t a = e4m3x2_to_f16x2((uint16_t)v), b = e4m3x2_to_f16x2((uint16_t)(v >> 16));
+          v = to_e4m3x2(f16_lo(a) * f, f16_hi(a) * f) | to_e4m3x2(f16_lo(b) * f, f16_hi(b) * f) << 16;
+        }
+        *reinterpret_cast<uint2*>(dst + 2 * i * D) = w[i];
       }
     }
   }
-
-  // ---- q: 16 lanes per head, dims [8 j, 8 j + 8)
-  const int j = tid & 15;
-  const float sg = j < 8 ? -1.f : 1.f;
-  float co[8], si[8];
+  __syncwarp();                 // every lane has read the old scale
+  if (lane == 0) *scale = exp2_int(e);
+  const float mul = exp2_int(-e);
+  const uint64_t mul2 = f32x2(mul, mul);
+  auto store = [&](auto inf) {
+#pragma unroll 2
+    for (int i = 0; i < 8; ++i) {
+      if (!(rows >> (2 * i + half) & 1)) continue;
+      const u128 x = lds16(mine + i * (D * 4));
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+      uint32_t q[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) co[e] = si[e] = 0.f;   // a position out of range: a row of zeros
+      for (int k = 0; k < 4; ++k) {
+        const uint64_t r = mul_f32x2(unpack_bf16x2(w[k]), mul2);
+        q[k] = inf ? to_e4m3x2(scaled_or_nan(bf16_lo(w[k]), mul), scaled_or_nan(bf16_hi(w[k]), mul))
+                   : to_e4m3x2(lo_f32(r), hi_f32(r));
+      }
+      *reinterpret_cast<uint2*>(dst + 2 * i * D) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+    }
+  };
+  if (special) store(std::true_type{});
+  else store(std::false_type{});
+}
+
+// Heads [8 hu, 8 hu + 8) of token t's q: a lane holds dims [8 j, 8 j + 8) of four of them.
+__device__ __forceinline__ void rotate_q(const __nv_bfloat16* qkv, int ldq, const int* pos, const float* cos_sin,
+                                         __nv_bfloat16* out, int ldo, int t, int hu, int Hq, int max_pos,
+                                         const __nv_bfloat16* qn, float eps) {
+  using namespace kvq;
+  const int lane = threadIdx.x & 31, j = lane & 15, h0 = 8 * hu + (lane >> 4);
+  u128 raw[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    raw[k] = h0 + 2 * k < Hq ? ld_v4(qkv + (size_t)t * ldq + (size_t)(h0 + 2 * k) * D + 8 * j) : u128{0, 0, 0, 0};
+  const int p = pos[t];
+  const bool pos_ok = p >= 0 && p < max_pos;
+  f32x4 co[2], si[2];                                   // sin negated in the first half: a cos - b sin
+  co[0] = co[1] = si[0] = si[1] = f32x4{0ull, 0ull};
   if (pos_ok) {
-    const float* cs = cos_sin + (size_t)p * D + 8 * (j & 7);
+    const f32x4* cs = reinterpret_cast<const f32x4*>(cos_sin + (size_t)p * D + 8 * (j & 7));
+    const uint64_t flip = j < 8 ? 0x8000000080000000ull : 0ull;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float4 a = *reinterpret_cast<const float4*>(cs + 4 * e);
-      const float4 b = *reinterpret_cast<const float4*>(cs + D / 2 + 4 * e);
-      co[4 * e] = a.x; co[4 * e + 1] = a.y; co[4 * e + 2] = a.z; co[4 * e + 3] = a.w;
-      si[4 * e] = b.x; si[4 * e + 1] = b.y; si[4 * e + 2] = b.z; si[4 * e + 3] = b.w;
+      co[e] = cs[e];
+      si[e] = cs[D / 8 + e];
+      si[e].a ^= flip;
+      si[e].b ^= flip;
     }
   }
-  for (int h0 = 0; h0 < Hq; h0 += THREADS / 16) {    // whole warps stay in the loop: two heads per warp
-    const int h = h0 + (tid >> 4);
-    const bool on = h < Hq;
-    u128 raw = on ? ld_v4(qkv + (size_t)t * ldq + (size_t)h * D + 8 * j) : u128{0, 0, 0, 0};
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
-    float a[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      a[2 * e] = bf16_lo(w[e]);
-      a[2 * e + 1] = bf16_hi(w[e]);
-    }
+  for (int k = 0; k < 4; ++k) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&raw[k]);
     if (qn != nullptr) {
       float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss += a[e] * a[e];
+      for (int e = 0; e < 4; ++e) ss += bf16_lo(w[e]) * bf16_lo(w[e]) + bf16_hi(w[e]) * bf16_hi(w[e]);
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       const float n = rsqrtf(ss * (1.0f / D) + eps);
       const u128 nw = ld_v4(qn + 8 * j);
       const uint32_t* pw = reinterpret_cast<const uint32_t*>(&nw);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t y = pack_bf16x2(a[2 * e] * n * bf16_lo(pw[e]), a[2 * e + 1] * n * bf16_hi(pw[e]));
-        a[2 * e] = bf16_lo(y);
-        a[2 * e + 1] = bf16_hi(y);
-      }
+      for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(bf16_lo(w[e]) * n * bf16_lo(pw[e]), bf16_hi(w[e]) * n * bf16_hi(pw[e]));
     }
-    float o[8];
+    u128 r;
+    uint32_t* pr = reinterpret_cast<uint32_t*>(&r);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float b = __shfl_xor_sync(0xffffffffu, a[e], 8);
-      o[e] = pos_ok ? a[e] * co[e] + sg * b * si[e] : 0.f;
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t b0 = __shfl_xor_sync(0xffffffffu, w[2 * e], 8), b1 = __shfl_xor_sync(0xffffffffu, w[2 * e + 1], 8);
+      pr[2 * e] = turn_bf16x2(w[2 * e], b0, co[e].a, si[e].a);
+      pr[2 * e + 1] = turn_bf16x2(w[2 * e + 1], b1, co[e].b, si[e].b);
     }
-    if (on) {
-      u128 r;
-      uint32_t* pr = reinterpret_cast<uint32_t*>(&r);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pr[e] = pack_bf16x2(o[2 * e], o[2 * e + 1]);
-      st_v4(out + (size_t)t * ldo + (size_t)h * D + 8 * j, r);
+    if (!pos_ok) r = u128{0, 0, 0, 0};                  // a position out of range: zeros
+    if (h0 + 2 * k < Hq) st_v4(out + (size_t)t * ldo + (size_t)(h0 + 2 * k) * D + 8 * j, r);
+  }
+}
+
+// CTAs 0, 2, 4, .. write blocks (n_block for each group of WARPS of a block's
+// K and V heads), the others rotate q; once one kind is used up the rest is
+// the other.
+__global__ void __launch_bounds__(kvq::THREADS, 4)
+    rope_cache_fp8_kernel(const __nv_bfloat16* qkv, int ldq, const int* __restrict__ pos,
+                          const float* __restrict__ cos_sin, const int64_t* __restrict__ slots, KvFp8 c,
+                          __nv_bfloat16* out, int ldo, int T, int Hq, int max_pos, int* status,
+                          const __nv_bfloat16* __restrict__ qn, const __nv_bfloat16* __restrict__ kn, float eps,
+                          int n_block, int groups, int n_rot) {
+  using namespace kvq;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n_b = n_block * groups, both = 2 * min(n_b, n_rot), i = blockIdx.x;
+  const bool block_cta = i < both ? (i & 1) == 0 : n_b > n_rot;
+  int k = i < both ? i >> 1 : i - both / 2;             // its number among its kind
+  if (!block_cta) {
+    const uint32_t hus = (Hq + 7) / 8;
+    const uint32_t units = (uint32_t)T * hus;           // T <= KVQ_MAX_ROWS
+    for (uint32_t u = k * WARPS + warp; u < units; u += n_rot * WARPS) {
+      const uint32_t t = u / hus;
+      rotate_q(qkv, ldq, pos, cos_sin, out, ldo, t, u - t * hus, Hq, max_pos, qn, eps);
+    }
+    return;
+  }
+  const int group = k / n_block;
+  k -= group * n_block;
+  for (int base = k; base < T; base += 32 * n_block) {  // 32 of the CTA's tokens at a time, one per lane
+    const int64_t tl = base + (int64_t)lane * n_block;
+    bool cand = false;
+    int block = -1;
+    if (tl < T) {
+      const int64_t slot = slots[tl], before = tl > 0 ? slots[tl - 1] : -1;
+      const int p = pos[tl];
+      const bool in = slot >= 0 && (slot >> 4) < c.num_blocks;
+      if (warp == 0 && group == 0 && ((slot >= 0 && !in) || p < 0 || p >= max_pos)) record_status(status, CX_ERR_BOUNDS);
+      cand = in && (before < 0 || (before >> 4) != (slot >> 4));   // most tokens of a prompt follow one of the same block
+      block = (int)(slot >> 4);
+    }
+    for (uint32_t m = __ballot_sync(0xffffffffu, cand); m != 0; m &= m - 1) { // the same in every warp
+      const int blk = __shfl_sync(0xffffffffu, block, __ffs(m) - 1);
+      write_block(qkv, ldq, pos, cos_sin, slots, c, base + (__ffs(m) - 1) * n_block, blk, group, T, Hq, max_pos, kn, eps);
     }
   }
 }
 
 void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_sin, const int64_t* slots,
-                    const KvFp8& c, void* out, int ldo, int T, int Hq, int max_pos, int* status, cudaStream_t s,
-                    const void* q_norm, const void* k_norm, float eps) {
+                    const KvFp8& c, void* out, int ldo, int T, int Hq, int max_pos, int sms, int* status,
+                    cudaStream_t s, const void* q_norm, const void* k_norm, float eps) {
+  static bool attr[64] = {};
+  int dev;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63]) {
+    cudaFuncSetAttribute(rope_cache_fp8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kvq::SMEM);
+    attr[dev & 63] = true;
+  }
   // Each block's first row scans the call's slots, so rows are taken
   // KVQ_MAX_ROWS at a time to keep the scan linear in T.
   for (int t0 = 0; t0 < T; t0 += KVQ_MAX_ROWS) {
     const int n = std::min(KVQ_MAX_ROWS, T - t0);
-    rope_cache_fp8_kernel<<<n, kvq::THREADS, 0, s>>>(
+    // tokens per CTA: few enough that two first rows rarely meet in one (8192 rows:
+    // 43 us with n / 14 and with n / 8; five 613-row prompts: 22 and 17 us)
+    const int n_block = std::min(n, std::max(n / 8, 2 * sms) | 1);
+    const int64_t units = (int64_t)n * ((Hq + 7) / 8);
+    const int groups = (2 * c.Hkv + kvq::WARPS - 1) / kvq::WARPS;
+    const int n_rot = (int)std::min<int64_t>((units + kvq::WARPS - 1) / kvq::WARPS, 6 * sms);
+    rope_cache_fp8_kernel<<<n_block * groups + n_rot, kvq::THREADS, kvq::SMEM, s>>>(
         reinterpret_cast<const __nv_bfloat16*>(qkv) + (size_t)t0 * ldq, ldq, pos + t0, cos_sin, slots + t0, c,
         reinterpret_cast<__nv_bfloat16*>(out) + (size_t)t0 * ldo, ldo, n, Hq, max_pos, status,
-        reinterpret_cast<const __nv_bfloat16*>(q_norm), reinterpret_cast<const __nv_bfloat16*>(k_norm), eps);
+        reinterpret_cast<const __nv_bfloat16*>(q_norm), reinterpret_cast<const __nv_bfloat16*>(k_norm), eps, n_block,
+        groups, n_rot);
   }
 }
 
@@ -266,9 +419,7 @@ void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_s
 // S = q.K^T and O^T = V^T.W^T on mma.sync m16n8k32 with e4m3 operands: the
 // cached bytes go into the tensor cores as they are (measured: 4.3 cycles per
 // instruction and SM quarter against 8 for the f16 m16n8k16 of half the
-// depth, sums exact to 2^-25; a version that converted K and V to f16 spent
-// twice the instructions and stayed at 0.60 of the HBM rate where this one
-// reaches RATE).  q and the softmax weights enter as the sum of two
+// depth, sums exact to 2^-25).  q and the softmax weights enter as the sum of two
 // e4m3 numbers each:
 //   q     scaled by a power of two per head to at most 448; bf16's 8-bit
 //         significand is two 4-bit ones, so only elements 2^11 times smaller
@@ -328,19 +479,6 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ u128 lds16(uint32_t a) {
-  u128 r;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
-  return r;
 }
 __device__ __forceinline__ uint2 lds8(uint32_t a) {
   uint2 r;
@@ -432,19 +570,19 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
     }
     b = lo;
   }
-    // Both land row by row, 512 contiguous bytes per instruction (measured: with
-    // every lane fetching the pieces it reads back, K in 64-byte halves and V
-    // in every other row, the loads alone took 122 us of 64 x 4096 where these
-    // take 96).  16-byte pieces are permuted inside a row so that the fragment
-    // reads meet no bank twice: K by the row's lowest bit (two rows at a time
-    // are read), V by the two above it (rows 2c, c = 0 .. 3).
-    const uint32_t ring = smem_u32(smem) + warp * (SLOTS * SLOT);
-    const uint32_t kput = (lane >> 3) * D + (((lane & 7) ^ (lane >> 3 & 1) * 4) << 4);
-    const uint32_t kget = gq * D + ((qd ^ (gq & 1) * 4) << 4);
-    const int khalf = gq & 1 ? -64 : 64;
-    const uint32_t vput = (lane >> 3) * D + (((lane & 7) ^ (lane >> 4) * 2) << 4);   // rows 0-3; ^ 64 in rows 4-7
-    const uint32_t vget = 2 * qd * D + ((gq ^ qd * 2) << 4);
-    const int vhalf = gq >> 1 & 1;       // 8-byte half of the piece that comes first (bank conflicts again)
+  // Both land row by row, 512 contiguous bytes per instruction (measured: with
+  // every lane fetching the pieces it reads back, K in 64-byte halves and V
+  // in every other row, the loads alone took 122 us of 64 x 4096 where these
+  // take 96).  16-byte pieces are permuted inside a row so that the fragment
+  // reads meet no bank twice: K by the row's lowest bit (two rows at a time
+  // are read), V by the two above it (rows 2c, c = 0 .. 3).
+  const uint32_t ring = smem_u32(smem) + warp * (SLOTS * SLOT);
+  const uint32_t kput = (lane >> 3) * D + (((lane & 7) ^ (lane >> 3 & 1) * 4) << 4);
+  const uint32_t kget = gq * D + ((qd ^ (gq & 1) * 4) << 4);
+  const int khalf = gq & 1 ? -64 : 64;
+  const uint32_t vput = (lane >> 3) * D + (((lane & 7) ^ (lane >> 4) * 2) << 4);   // rows 0-3; ^ 64 in rows 4-7
+  const uint32_t vget = 2 * qd * D + ((gq ^ qd * 2) << 4);
+  const int vhalf = gq >> 1 & 1;       // 8-byte half of the piece that comes first (bank conflicts again)
 
   for (int u = u0; u < u1;) {
     // ---- the blocks [j0, j1) of KV head h of sequence b
@@ -915,23 +1053,36 @@ __global__ void __launch_bounds__(kvc::THREADS)
     if (tid == 0) record_status(status, CX_ERR_BOUNDS);
     return;
   }
-  const int64_t nv = block_bytes >> 4;
-  for (int p = p0; p < p1; ++p) {
-    const uint8_t* a = kv + ((int64_t)p * num_blocks + src) * block_bytes;
-    uint8_t* b = kv + ((int64_t)p * num_blocks + dst) * block_bytes;
-    for (int64_t v = tid; v < nv; v += 8 * kvc::THREADS) {
-      u128 r[8];
+  // the planes' vectors end to end, eight of a thread in flight
+  const int nv = (int)(block_bytes >> 4);
+  const int64_t plane = (int64_t)num_blocks * block_bytes;
+  const uint8_t* a = kv + p0 * plane + src * block_bytes;
+  uint8_t* b = kv + p0 * plane + dst * block_bytes;
+  const int total = (p1 - p0) * nv;
+  int v = tid;                    // the thread's next vector of plane `at`
+  int64_t at = 0;
+  for (int i = tid; i < total; i += 8 * kvc::THREADS) {
+    u128 r[8];
+    int64_t off[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (v + e * kvc::THREADS < nv) r[e] = ld_nc_v4(a + (v + e * kvc::THREADS) * 16);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (v + e * kvc::THREADS < nv) st_cs_v4(b + (v + e * kvc::THREADS) * 16, r[e]);
+    for (int e = 0; e < 8; ++e) {
+      while (v >= nv) {
+        v -= nv;
+        at += plane;
+      }
+      off[e] = at + (int64_t)v * 16;
+      if (i + e * kvc::THREADS < total) r[e] = ld_nc_v4(a + off[e]);
+      v += kvc::THREADS;
     }
-    if (scales != nullptr)
-      for (int h = tid; h < Hkv; h += kvc::THREADS)
-        scales[((int64_t)p * num_blocks + dst) * Hkv + h] = scales[((int64_t)p * num_blocks + src) * Hkv + h];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e * kvc::THREADS < total) st_cs_v4(b + off[e], r[e]);
   }
+  if (scales != nullptr)
+    for (int i = tid; i < (p1 - p0) * Hkv; i += kvc::THREADS) {
+      const int64_t row = (int64_t)(p0 + i / Hkv) * num_blocks;
+      scales[(row + dst) * Hkv + i % Hkv] = scales[(row + src) * Hkv + i % Hkv];
+    }
 }
 
 void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes, int num_blocks, int64_t block_bytes,

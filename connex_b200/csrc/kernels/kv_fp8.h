@@ -21,7 +21,7 @@ struct KvFp8 {
 // into out [T, Hq * 128] (ld ldo; may be the q columns of qkv), k rotated and
 // v quantised into the slots' blocks (slot < 0: not cached).
 void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_sin, const int64_t* slots,
-                    const KvFp8& c, void* out, int ldo, int T, int Hq, int max_pos, int* status, cudaStream_t s,
+                    const KvFp8& c, void* out, int ldo, int T, int Hq, int max_pos, int sms, int* status, cudaStream_t s,
                     const void* q_norm, const void* k_norm, float eps);
 
 // Rows of one call that are handled together; longer calls run as successive launches.

@@ -367,13 +367,36 @@ void kv_copy_blocks(at::Tensor& kv, const at::Tensor& pairs, const c10::optional
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-void kv_dequant_blocks(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
-                       const at::Tensor& table, at::Tensor& kout, at::Tensor& vout,
-                       const c10::optional<at::Tensor>& status) {
-  const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "kv_dequant_blocks");
-  const c10::cuda::CUDAGuard g(kc.device());
-  cx::kv_dequant_blocks(c, table.data_ptr<int>(), (int)table.numel(), kout.data_ptr(), vout.data_ptr(),
-                        status_ptr(status), cur_stream(kc));
+// Two launches: the tables' blocks as bf16 into workspaces of the caller, the
+// paged prefill attention over them.
+void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
+                                 const at::Tensor& vs, const at::Tensor& block_tables, at::Tensor& out,
+                                 const at::Tensor& tile_info, int64_t Hq, int64_t Hkv, double scale, at::Tensor& kw,
+                                 at::Tensor& vw, at::Tensor& table, const c10::optional<at::Tensor>& status) {
+  check_same_device(q, {&kc, &block_tables, &out, &tile_info, &kw, &vw, &table}, "prefill_attention_paged_fp8");
+  const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "prefill_attention_paged_fp8");
+  const int ldq = row_ld16(q, "prefill_attention_paged_fp8: q"), ldo = row_ld16(out, "prefill_attention_paged_fp8: out");
+  const int64_t T = q.size(0);
+  TORCH_CHECK(Hkv == c.Hkv && Hq > 0 && Hq % Hkv == 0,
+              "prefill_attention_paged_fp8: Hkv as in the cache, the query heads a multiple of it");
+  TORCH_CHECK(q.size(1) >= Hq * 128 && out.size(0) == T && out.size(1) == Hq * 128,
+              "prefill_attention_paged_fp8: q must hold Hq heads of 128 per row and out be [T, Hq * 128]");
+  TORCH_CHECK(tile_info.scalar_type() == at::kInt && tile_info.dim() == 2 && tile_info.size(1) == 5 &&
+                  tile_info.is_contiguous(),
+              "prefill_attention_paged_fp8: tile_info must be contiguous int32 [n, 5]");
+  TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
+                  block_tables.numel() * Hkv * 16 <= INT_MAX,
+              "prefill_attention_paged_fp8: block_tables must be contiguous int32 [B, max_blocks]");
+  CHECK_CUDA(q);
+  const c10::cuda::CUDAGuard g(q.device());
+  if (T == 0 || tile_info.size(0) == 0) return;
+  cx::kv_dequant_blocks(c, block_tables.data_ptr<int>(), (int)block_tables.numel(), kw.data_ptr(), vw.data_ptr(),
+                        table.data_ptr<int>(), status_ptr(status), cur_stream(q));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  cx::prefill_attention_paged_tc(q.data_ptr(), ldq, (int)(Hq * 128), (int)T, kw.data_ptr(), vw.data_ptr(),
+                                 block_tables.numel() * Hkv * 16, table.data_ptr<int>(), (int)block_tables.size(1),
+                                 out.data_ptr(), ldo, tile_info.data_ptr<int>(), (int)tile_info.size(0), (int)Hq,
+                                 (int)Hkv, (float)scale, status_ptr(status), cur_stream(q), 256);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -624,7 +647,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("DECODE_FP8_ROW") = cx::DEC8_ROW;
   m.def("decode_attention_fp8", &decode_attention_fp8);
   m.def("kv_copy_blocks", &kv_copy_blocks);
-  m.def("kv_dequant_blocks", &kv_dequant_blocks);
+  m.def("prefill_attention_paged_fp8", &prefill_attention_paged_fp8);
   m.def("kv_push_layer", &kv_push_layer);
   m.def("gemm_splits", &gemm_splits);
   m.def("gemm_raster_group", &cx::gemm_raster_group);

@@ -1095,18 +1095,24 @@ void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes
 }
 
 // --------------------------------------------------------- dequantised blocks
+// Blocks of the tables' entries as bf16 (exact: the scales are powers of two),
+// one after the other, and the table that finds them there.
 __global__ void __launch_bounds__(256)
-    kv_dequant_kernel(KvFp8 c, const int* __restrict__ table, __nv_bfloat16* ko, __nv_bfloat16* vo, int* status) {
+    kv_dequant_kernel(KvFp8 c, const int* __restrict__ table, __nv_bfloat16* ko, __nv_bfloat16* vo, int* table_out,
+                      int* status) {
   using namespace kvq;
   const int i = blockIdx.x, h = blockIdx.y, id = table[i];
-  if (id < 0 || id >= c.num_blocks) {
-    if (threadIdx.x == 0) record_status(status, CX_ERR_BOUNDS);
-    return;
-  }
-  const size_t at = ((size_t)id * c.Hkv + h) * (BS * D), to = ((size_t)i * c.Hkv + h) * (BS * D);
+  if (h == 0 && threadIdx.x == 0) table_out[i] = i;
+  const bool in = id >= 0 && id < c.num_blocks;
+  if (!in && h == 0 && threadIdx.x == 0) record_status(status, CX_ERR_BOUNDS);
+  const size_t to = ((size_t)i * c.Hkv + h) * (BS * D);
   const int half = threadIdx.x >> 7, e = (threadIdx.x & 127) * 16;
-  const u128 raw = ld_nc_v4((half ? c.v : c.k) + at + e);
-  const float f = (half ? c.vs : c.ks)[(size_t)id * c.Hkv + h];
+  u128 raw{0, 0, 0, 0};           // an id out of range reads as zeros
+  float f = 0.f;
+  if (in) {
+    raw = ld_nc_v4((half ? c.v : c.k) + ((size_t)id * c.Hkv + h) * (BS * D) + e);
+    f = (half ? c.vs : c.ks)[(size_t)id * c.Hkv + h];
+  }
   const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
   u128 o[2];
   uint32_t* po = reinterpret_cast<uint32_t*>(o);
@@ -1121,10 +1127,11 @@ __global__ void __launch_bounds__(256)
   st_v4(d + 8, o[1]);
 }
 
-void kv_dequant_blocks(const KvFp8& c, const int* table, int n, void* kout, void* vout, int* status, cudaStream_t s) {
+void kv_dequant_blocks(const KvFp8& c, const int* table, int n, void* kout, void* vout, int* table_out, int* status,
+                       cudaStream_t s) {
   if (n == 0) return;
   kv_dequant_kernel<<<dim3(n, c.Hkv), 256, 0, s>>>(c, table, reinterpret_cast<__nv_bfloat16*>(kout),
-                                                   reinterpret_cast<__nv_bfloat16*>(vout), status);
+                                                   reinterpret_cast<__nv_bfloat16*>(vout), table_out, status);
 }
 
 }  // namespace cx

@@ -43,7 +43,8 @@ void decode_attention_fp8(const void* q, int ldq, const KvFp8& c, const int* blo
 void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes, int num_blocks, int64_t block_bytes,
                     int Hkv, int sms, int* status, cudaStream_t s);
 
-// e4m3 blocks table[i] -> bf16 blocks i of kout / vout [n, Hkv, 16, 128].
-void kv_dequant_blocks(const KvFp8& c, const int* table, int n, void* kout, void* vout, int* status, cudaStream_t s);
+// e4m3 blocks table[i] -> bf16 blocks i of kout / vout [n, Hkv, 16, 128]; table_out[i] = i.
+void kv_dequant_blocks(const KvFp8& c, const int* table, int n, void* kout, void* vout, int* table_out, int* status,
+                       cudaStream_t s);
 
 }  // namespace cx

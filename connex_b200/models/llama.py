@@ -11,7 +11,10 @@ Storage layout, chosen for the kernels rather than for checkpoint parity:
                                         GEMM epilogue emits SiLU(gate) * up directly
 * ``wo``, ``w2``                     -- consumed with the residual-add epilogue
 * paged KV cache [L, 2, blocks, Hkv, 16, 128]: one head of one block is a
-  contiguous 4 KB slice, the unit the PD push kernel moves.
+  contiguous 4 KB slice, the unit the PD push kernel moves.  With
+  ``dtype=torch.float8_e4m3fn`` it holds 8-bit values and one power-of-two
+  scale per (block, KV head); attention then reads K and V from the cache in
+  prefill steps too, so a prompt gives the same rows however it is chunked.
 
 The forward passes launch only this package's kernels (tcgen05 GEMM,
 RMSNorm, RoPE + cache write, attention, argmax); a per-layer hook lets the
@@ -199,7 +202,16 @@ def random_trainer_weights(cfg: LlamaConfig, device, dtype=torch.float32, seed: 
 
 
 class PagedKVCache:
-    """Paged KV cache [L, 2, blocks, Hkv, BS, D] with a free-block allocator."""
+    """Paged KV cache [L, 2, blocks, Hkv, BS, D] with a free-block allocator.
+
+    ``dtype=torch.float8_e4m3fn``: an 8-bit cache; ``scales`` [L, 2, blocks,
+    Hkv] fp32 then belong to it (see :func:`connex_b200.ops.rope_cache_fp8`),
+    otherwise ``scales`` is None.
+
+    Blocks can be shared: :meth:`fork` gives sequences that continue another
+    one tables on its full blocks, and :meth:`free` returns a block to the
+    pool with its last owner.  Shared blocks are only read (a sequence appends
+    behind its last full block)."""
 
     def __init__(self, cfg: LlamaConfig, num_blocks: int, device, dtype=torch.bfloat16,
                  storage: Optional[torch.Tensor] = None):
@@ -207,13 +219,23 @@ class PagedKVCache:
         self.num_blocks = num_blocks
         shape = (cfg.layers, 2, num_blocks, cfg.kv_heads, cfg.block_size, cfg.head_dim)
         self.kv = storage.view(shape) if storage is not None else torch.empty(shape, dtype=dtype, device=device)
+        self.scales = None
+        if self.kv.dtype == torch.float8_e4m3fn:
+            self.scales = torch.ones(shape[:4], dtype=torch.float32, device=self.kv.device)
         self._free = list(range(num_blocks - 1, -1, -1))
+        self._shared = {}              # block -> owners beyond the first
 
     def k(self, layer: int) -> torch.Tensor:
         return self.kv[layer, 0]
 
     def v(self, layer: int) -> torch.Tensor:
         return self.kv[layer, 1]
+
+    def k_scale(self, layer: int) -> torch.Tensor:
+        return self.scales[layer, 0]
+
+    def v_scale(self, layer: int) -> torch.Tensor:
+        return self.scales[layer, 1]
 
     @property
     def head_slice_bytes(self) -> int:
@@ -236,7 +258,75 @@ class PagedKVCache:
         return [self._free.pop() for _ in range(n_blocks)]
 
     def free(self, blocks: Sequence[int]) -> None:
-        self._free.extend(reversed(list(blocks)))
+        """One owner gives the blocks up; shared ones stay with the others."""
+        if not self._shared:
+            self._free.extend(reversed(list(blocks)))
+            return
+        for b in reversed(list(blocks)):
+            left = self._shared.get(b, 0)
+            if left == 0:
+                self._free.append(b)
+            elif left == 1:
+                del self._shared[b]
+            else:
+                self._shared[b] = left - 1
+
+    def copy_blocks(self, pairs: Sequence[Sequence[int]]) -> None:
+        """Copy whole blocks (source, destination) in every layer, scales
+        included, in order with the current stream."""
+        pairs = [(int(s), int(d)) for s, d in pairs]
+        dst = {d for _, d in pairs}
+        if len(dst) != len(pairs) or any(s in dst for s, _ in pairs):
+            raise ValueError("copy_blocks: a destination may be neither a source nor another pair's destination")
+        if any(not 0 <= b < self.num_blocks for p in pairs for b in p):
+            raise ValueError(f"copy_blocks: block ids must lie in [0, {self.num_blocks})")
+        if not pairs:
+            return
+        t = torch.tensor(pairs, dtype=torch.int32)
+        if self.kv.is_cuda:
+            ops.kv_copy_blocks(self.kv, t.pin_memory().to(self.kv.device, non_blocking=True), self.scales)
+            return
+        from connex_b200.ops import reference as R
+        R.kv_copy_blocks(self.kv, t, self.scales)
+
+    def fork(self, blocks: Sequence[int], n_tokens: int, n: int = 1) -> List[List[int]]:
+        """Block tables of ``n`` sequences that go on from the first
+        ``n_tokens`` of the one with table ``blocks``: its full blocks are
+        shared, a partly filled last one is copied (one launch for all)."""
+        bs = self.cfg.block_size
+        full, rest = divmod(n_tokens, bs)
+        if n_tokens < 0 or self.blocks_needed(n_tokens) > len(blocks):
+            raise ValueError(f"fork: {n_tokens} tokens do not lie in {len(blocks)} blocks")
+        if n < 0:
+            raise ValueError("fork: n must not be negative")
+        tails = self.allocate(n) if rest else []
+        self.copy_blocks([(blocks[full], t) for t in tails])
+        if n:
+            for b in blocks[:full]:
+                self._shared[b] = self._shared.get(b, 0) + n
+        return [list(blocks[:full]) + tails[i:i + 1] for i in range(n)]
+
+    def compact(self, tables) -> int:
+        """Move the blocks of ``tables`` (the block lists of the live
+        sequences, changed in place) down so that the pool's used blocks are
+        its lowest ones; blocks in none of them stay where they are.  Returns
+        the number of blocks moved."""
+        tables = list(tables)
+        used = self.num_blocks - len(self._free)
+        holes = sorted(b for b in self._free if b < used)
+        high = sorted({b for t in tables for b in t if b >= used}, reverse=True)
+        moves = dict(zip(high, holes))
+        if not moves:
+            return 0
+        self.copy_blocks(list(moves.items()))
+        for t in tables:
+            t[:] = [moves.get(b, b) for b in t]
+        for s, d in moves.items():
+            if s in self._shared:
+                self._shared[d] = self._shared.pop(s)
+        taken = set(moves.values())
+        self._free = sorted([b for b in self._free if b not in taken] + list(moves), reverse=True)
+        return len(moves)
 
     @property
     def free_blocks(self) -> int:
@@ -291,6 +381,45 @@ class LlamaModel:
         ops.gemm(a, w, x, residual=x if tp.rank == 0 else None, status=self.status)
         tp.all_reduce(x)
 
+    def _rotate_and_cache(self, i: int, qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
+                          **norms) -> torch.Tensor:
+        """Rotate q (in place) and write the rows' K and V to layer ``i`` of the
+        cache; returns what the attention reads its queries from."""
+        cfg, c = self.cfg, self.cache
+        if c.scales is None:
+            ops.rope_cache(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots, c.k(i), c.v(i),
+                           status=self.status, **norms)
+            return qkv
+        return ops.rope_cache_fp8(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots, c.k(i), c.v(i),
+                                  c.k_scale(i), c.v_scale(i), out=qkv[:, :cfg.heads * cfg.head_dim],
+                                  status=self.status, **norms)
+
+    def _decode_attention(self, i: int, q: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
+                          max_ctx: int, workspace: torch.Tensor, out: torch.Tensor) -> None:
+        cfg, c = self.cfg, self.cache
+        if c.scales is None:
+            ops.decode_attention(q, c.k(i), c.v(i), block_tables, ctx_lens, cfg.heads, max_ctx, workspace, out=out)
+        else:
+            ops.decode_attention_fp8(q, c.k(i), c.v(i), c.k_scale(i), c.v_scale(i), block_tables, ctx_lens, cfg.heads,
+                                     workspace, out=out, status=self.status)
+
+    def _chunk_attention(self, i: int, q: torch.Tensor, block_tables: torch.Tensor, tile_info: torch.Tensor,
+                         out: torch.Tensor) -> None:
+        cfg, c = self.cfg, self.cache
+        if c.scales is None:
+            ops.prefill_attention_paged(q, c.k(i), c.v(i), block_tables, tile_info, cfg.heads, cfg.kv_heads, out=out,
+                                        status=self.status)
+        else:
+            ops.prefill_attention_paged_fp8(q, c.k(i), c.v(i), c.k_scale(i), c.v_scale(i), block_tables, tile_info,
+                                            cfg.heads, cfg.kv_heads, out=out, status=self.status)
+
+    def decode_workspace(self, max_batch: int, max_ctx: int) -> torch.Tensor:
+        """The decode attention's workspace for this model's cache."""
+        cfg = self.cfg
+        if self.cache.scales is None:
+            return ops.decode_workspace(max_batch, cfg.heads, max_ctx, self.device)
+        return ops.decode_workspace_fp8(max_batch, cfg.heads, cfg.kv_heads, self.device)
+
     def _layer_tail(self, l: int, T: int):
         cfg, lw = self.cfg, self.w.layers[l]
         x, h = self.x[:T], self.h[:T]
@@ -310,8 +439,13 @@ class LlamaModel:
 
     def prefill(self, ids: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                 seq_lens: Sequence[int], last_rows: torch.Tensor, tile_info: torch.Tensor,
-                layer_hook: Optional[LayerHook] = None, hook_after_attention: bool = False) -> torch.Tensor:
+                layer_hook: Optional[LayerHook] = None, hook_after_attention: bool = False,
+                block_tables: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Prefill a packed batch; returns the greedy next token of each sequence.
+
+        With an 8-bit cache the attention reads it: ``block_tables`` [B,
+        max_blocks] is then needed, and ``tile_info`` from
+        ``prefill_tile_info(seq_lens, device, ctx)``.
 
         ``layer_hook(l)`` runs (on the host, in stream order) right after layer
         l's K/V are in the paged cache: the PD path launches its push there.
@@ -320,6 +454,8 @@ class LlamaModel:
         than its attention kernel)."""
         cfg, T = self.cfg, ids.numel()
         assert T <= self.max_tokens
+        if self.cache.scales is not None and block_tables is None:
+            raise ValueError("prefill over an 8-bit cache needs block_tables")
         nvtx.push(f"prefill T={T}")
         ops.embedding(ids, self.w.embed, self.x[:T], status=self.status)
         ops.rmsnorm(self.x[:T], self.w.layers[0].attn_norm, cfg.eps, out=self.h[:T])
@@ -327,11 +463,13 @@ class LlamaModel:
             nvtx.push(f"layer {l}")
             qkv = self.qkv[:T]
             ops.gemm(self.h[:T], lw.wqkv, qkv, status=self.status)
-            ops.rope_cache(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots,
-                           self.cache.k(l), self.cache.v(l), status=self.status)
+            q = self._rotate_and_cache(l, qkv, positions, slots)
             if layer_hook is not None and not hook_after_attention:
                 layer_hook(l)
-            ops.prefill_attention(qkv, tile_info, cfg.heads, cfg.kv_heads, out=self.attn[:T])
+            if self.cache.scales is None:
+                ops.prefill_attention(qkv, tile_info, cfg.heads, cfg.kv_heads, out=self.attn[:T])
+            else:
+                self._chunk_attention(l, q, block_tables, tile_info, self.attn[:T])
             if layer_hook is not None and hook_after_attention:
                 layer_hook(l)
             self._layer_tail(l, T)
@@ -343,7 +481,8 @@ class LlamaModel:
     def decode(self, ids: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                block_tables: torch.Tensor, ctx_lens: torch.Tensor, max_ctx: int,
                workspace: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
-        """One decode step for B sequences (ctx_lens include the new token)."""
+        """One decode step for B sequences (ctx_lens include the new token);
+        ``workspace`` from :meth:`decode_workspace`."""
         cfg, B = self.cfg, ids.numel()
         nvtx.push(f"decode B={B}")
         ops.embedding(ids, self.w.embed, self.x[:B], status=self.status)
@@ -351,10 +490,8 @@ class LlamaModel:
         for l, lw in enumerate(self.w.layers):
             qkv = self.qkv[:B]
             ops.gemm(self.h[:B], lw.wqkv, qkv, status=self.status)
-            ops.rope_cache(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots,
-                           self.cache.k(l), self.cache.v(l), status=self.status)
-            ops.decode_attention(qkv, self.cache.k(l), self.cache.v(l), block_tables, ctx_lens,
-                                 cfg.heads, max_ctx, workspace, out=self.attn[:B])
+            q = self._rotate_and_cache(l, qkv, positions, slots)
+            self._decode_attention(l, q, block_tables, ctx_lens, max_ctx, workspace, self.attn[:B])
             self._layer_tail(l, B)
         out = self._head(rows, B)
         nvtx.pop()

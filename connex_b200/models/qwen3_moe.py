@@ -99,7 +99,7 @@ class Qwen3MoeRank:
     """One EP rank: replicated attention weights, its expert slots, its KV cache."""
 
     def __init__(self, cfg: Qwen3MoeConfig, rank: int, slots_per_rank: int, placement: List[List[int]], device,
-                 num_blocks: int, max_tokens: int, seed: int = 0):
+                 num_blocks: int, max_tokens: int, seed: int = 0, kv_dtype: torch.dtype = torch.bfloat16):
         """``placement[l][p]``: logical expert in physical slot ``p`` of layer
         ``l`` (-1 = empty); this rank holds slots ``[rank*S, (rank+1)*S)``."""
         self.cfg, self.rank, self.S, self.device = cfg, rank, slots_per_rank, torch.device(device)
@@ -131,7 +131,7 @@ class Qwen3MoeRank:
         from connex_b200.models.llama import LlamaConfig, PagedKVCache
         kv_cfg = LlamaConfig(vocab_size=cfg.vocab_size, hidden=cfg.hidden, layers=cfg.layers, heads=cfg.heads,
                              kv_heads=cfg.kv_heads, head_dim=cfg.head_dim, block_size=cfg.block_size)
-        self.cache = PagedKVCache(kv_cfg, num_blocks, dev)
+        self.cache = PagedKVCache(kv_cfg, num_blocks, dev, kv_dtype)
         self.cos_sin = ops.rope_cos_sin(cfg.max_pos, cfg.head_dim, cfg.rope_theta, dev)
         self.status = ops.new_status(dev)
         bf = dict(dtype=torch.bfloat16, device=dev)
@@ -149,7 +149,8 @@ class Qwen3MoeRank:
         return self.w13[layer, local_slot], self.w2[layer, local_slot]
 
     def decode(self, ids, positions, slots, block_tables, ctx_lens, max_ctx, workspace, routing, l2p, l2p_cnt):
-        """One decode step of this rank's batch; ``routing[l] = (topk_idx, topk_w)``."""
+        """One decode step of this rank's batch; ``routing[l] = (topk_idx, topk_w)``;
+        ``workspace`` from ``ops.decode_workspace`` (8-bit cache: ``ops.decode_workspace_fp8``)."""
         cfg, T = self.cfg, ids.numel()
         x, h = self.x[:T], self.h[:T]
         ops.embedding(ids, self.embed, x, status=self.status)
@@ -157,10 +158,18 @@ class Qwen3MoeRank:
         for l, a in enumerate(self.attn):
             qkv = self.qkv[:T]
             ops.gemm(h, a.wqkv, qkv, status=self.status)
-            ops.rope_cache(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots, self.cache.k(l),
-                           self.cache.v(l), status=self.status, q_norm=a.q_norm, k_norm=a.k_norm, eps=cfg.eps)
-            ops.decode_attention(qkv, self.cache.k(l), self.cache.v(l), block_tables, ctx_lens, cfg.heads, max_ctx,
-                                 workspace, out=self.att[:T])
+            c = self.cache
+            if c.scales is None:
+                ops.rope_cache(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots, c.k(l), c.v(l),
+                               status=self.status, q_norm=a.q_norm, k_norm=a.k_norm, eps=cfg.eps)
+                ops.decode_attention(qkv, c.k(l), c.v(l), block_tables, ctx_lens, cfg.heads, max_ctx, workspace,
+                                     out=self.att[:T])
+            else:
+                q = ops.rope_cache_fp8(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots, c.k(l), c.v(l),
+                                       c.k_scale(l), c.v_scale(l), out=qkv[:, :cfg.heads * cfg.head_dim],
+                                       status=self.status, q_norm=a.q_norm, k_norm=a.k_norm, eps=cfg.eps)
+                ops.decode_attention_fp8(q, c.k(l), c.v(l), c.k_scale(l), c.v_scale(l), block_tables, ctx_lens,
+                                         cfg.heads, workspace, out=self.att[:T], status=self.status)
             ops.gemm(self.att[:T], a.wo, x, residual=x, status=self.status)
             ops.rmsnorm(x, a.mlp_norm, cfg.eps, out=h)
             self.moe.w13 = self.w13[l].reshape(-1, cfg.hidden)

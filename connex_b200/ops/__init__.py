@@ -343,15 +343,14 @@ def prefill_attention_paged_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache:
     """:func:`prefill_attention_paged` over an 8-bit cache: causal attention of
     prompt chunks, ``q`` [T, Hq * 128] rotated, keys and values of the whole
     context -- this chunk's included -- from the cache."""
-    width = block_tables.shape[1]
-    n = block_tables.numel()
-    k = torch.empty(n, n_kv_heads, 16, 128, dtype=q.dtype, device=q.device)
-    v = torch.empty_like(k)
-    _C.kv_dequant_blocks(k_cache, v_cache, k_scale, v_scale, block_tables, k, v, status)
-    table = torch.arange(n, dtype=torch.int32, device=q.device).view(-1, width)
-    pad = torch.nn.functional.pad(q, (0, 2 * n_kv_heads * 128))
-    _n()
-    return prefill_attention_paged(pad, k, v, table, tile_info, n_q_heads, n_kv_heads, out, scale, status)
+    if out is None:
+        out = torch.empty(q.shape[0], n_q_heads * 128, dtype=q.dtype, device=q.device)
+    k = torch.empty(block_tables.numel(), n_kv_heads, 16, 128, dtype=torch.bfloat16, device=q.device)
+    _C.prefill_attention_paged_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tables, out, tile_info, n_q_heads,
+                                   n_kv_heads, scale if scale is not None else 1.0 / math.sqrt(128), k,
+                                   torch.empty_like(k), torch.empty_like(block_tables), status)
+    _n(2)
+    return out
 
 
 def kv_copy_blocks(kv: torch.Tensor, pairs: torch.Tensor, scales: Optional[torch.Tensor] = None,

@@ -40,6 +40,13 @@ from connex_b200.utils.nvtx import nvtx_range
 from connex_b200.models.llama import LlamaModel, PagedKVCache, slot_mapping
 
 
+def _bf16_only(cache: PagedKVCache) -> None:
+    """The layerwise transfer moves a cache's values alone: an 8-bit cache's
+    scales would be left behind."""
+    if getattr(cache, "scales", None) is not None:
+        raise ValueError("the layerwise KV transfer moves bf16 caches; an 8-bit cache's scales do not travel with it")
+
+
 @dataclass
 class KVDestination:
     """Where a prefill instance writes KV: a decode cache (local or peer-mapped)."""
@@ -55,6 +62,7 @@ class KVDestination:
     @classmethod
     def of_cache(cls, cache: PagedKVCache, ready: torch.Tensor, base: Optional[int] = None,
                  ready_addr: Optional[int] = None) -> "KVDestination":
+        _bf16_only(cache)
         return cls(base=base if base is not None else cache.kv.data_ptr(),
                    layer_stride=cache.layer_stride_bytes, kv_stride=cache.kv_stride_bytes,
                    heads=cache.cfg.kv_heads, num_blocks=cache.num_blocks,
@@ -72,6 +80,7 @@ class LayerwiseKVPusher:
     the prefill's per-layer hook; counts the CTAs the decode side must see."""
 
     def __init__(self, src: PagedKVCache, max_ctas: int = 0, priority: int = -1, threads: int = 128):
+        _bf16_only(src)
         self.src = src
         # High priority: push CTAs take SM slots ahead of the queued prefill
         # CTAs.  The prefill's GEMM and attention kernels are persistent (one
@@ -183,6 +192,7 @@ class LayerwiseKVPuller:
     publishes each layer."""
 
     def __init__(self, dst: PagedKVCache, max_ctas: int = 0, timeout_s: float = 30.0):
+        _bf16_only(dst)
         self.dst = dst
         self.max_ctas = max_ctas
         self.timeout_s = timeout_s

@@ -110,21 +110,17 @@ class StageModel(LlamaModel):
         for i, lw in enumerate(self.w.layers):
             qkv = self.qkv[:T]
             ops.gemm(self.h[:T], lw.wqkv, qkv, status=self.status)
-            ops.rope_cache(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots, self.cache.k(i),
-                           self.cache.v(i), status=self.status)
+            q = self._rotate_and_cache(i, qkv, positions, slots)
             if n_dec is not None:
                 if n_dec:
-                    ops.decode_attention(qkv[:n_dec], self.cache.k(i), self.cache.v(i), block_tables[:n_dec],
-                                         ctx_lens, cfg.heads, max_ctx, workspace, out=self.attn[:n_dec])
+                    self._decode_attention(i, q[:n_dec], block_tables[:n_dec], ctx_lens, max_ctx, workspace,
+                                           self.attn[:n_dec])
                 if T > n_dec:
-                    ops.prefill_attention_paged(qkv[n_dec:], self.cache.k(i), self.cache.v(i), block_tables[n_dec:],
-                                                tile_info, cfg.heads, cfg.kv_heads, out=self.attn[n_dec:T],
-                                                status=self.status)
+                    self._chunk_attention(i, q[n_dec:], block_tables[n_dec:], tile_info, self.attn[n_dec:T])
             elif prefill:
                 ops.prefill_attention(qkv, tile_info, cfg.heads, cfg.kv_heads, out=self.attn[:T])
             else:
-                ops.decode_attention(qkv, self.cache.k(i), self.cache.v(i), block_tables, ctx_lens, cfg.heads,
-                                     max_ctx, workspace, out=self.attn[:T])
+                self._decode_attention(i, q, block_tables, ctx_lens, max_ctx, workspace, self.attn[:T])
             self._tail(i, T)
         if self.is_last:
             return self._head(rows, B)
@@ -136,23 +132,24 @@ class StageRuntime:
 
     def __init__(self, cfg: LlamaConfig, l0: int, l1: int, device, num_blocks: int, max_tokens: int,
                  max_batch: int = 256, max_ctx: int = 8192, seed: int = 0, weights: Optional[LlamaWeights] = None,
-                 tp=None):
+                 tp=None, kv_dtype: torch.dtype = torch.bfloat16):
         """``weights``: layers ``[l0, l1)`` already on ``device`` (e.g. from
-        :func:`connex_b200.models.hf.load_llama`); random from ``seed`` if absent."""
+        :func:`connex_b200.models.hf.load_llama`); random from ``seed`` if absent.
+        ``kv_dtype``: ``torch.float8_e4m3fn`` for an 8-bit KV cache."""
         self.cfg = cfg
         self.device = torch.device(device)
         if weights is not None and len(weights.layers) != l1 - l0:
             raise ValueError(f"weights hold {len(weights.layers)} layers, the stage owns {l1 - l0}")
         self.weights = weights if weights is not None else stage_weights(cfg, l0, l1, self.device, seed)
         stage_cfg = LlamaConfig(**{**cfg.__dict__, "layers": l1 - l0})
-        self.cache = PagedKVCache(stage_cfg, num_blocks, self.device)
+        self.cache = PagedKVCache(stage_cfg, num_blocks, self.device, kv_dtype)
         self.model = StageModel(self.weights, l0, l1, self.cache, max_tokens, max_batch, self.device, tp=tp)
         self.model.cfg = cfg
         self.bs = cfg.block_size
         self.max_ctx = max_ctx
         self.tables: Dict[object, List[int]] = {}
         self.held: Dict[object, int] = {}
-        self.ws = ops.decode_workspace(max_batch, cfg.heads, max_ctx, self.device)
+        self.ws = self.model.decode_workspace(max_batch, max_ctx)
         self.steps = 0
         self.act: Optional[torch.Tensor] = None      # activation log (non-last stages)
         self.act_slot: Dict[object, int] = {}
@@ -296,6 +293,30 @@ class StageRuntime:
     def abort(self, rids) -> None:
         self.release(rids)
 
+    def fork(self, rid, new_rids: Sequence) -> None:
+        """Requests ``new_rids`` go on from where ``rid`` stands: they share its
+        full KV blocks and get copies of its partly filled last one."""
+        new_rids = list(new_rids)
+        if rid not in self.held:
+            raise KeyError(f"fork: no KV of {rid!r} here")
+        if len(set(new_rids)) != len(new_rids) or any(r in self.tables for r in new_rids):
+            raise ValueError("fork: the new requests must be new and distinct")
+        n = self.held[rid]
+        slots = []
+        if self.act is not None:
+            if len(self.act_slot) + len(new_rids) > self.act.shape[0]:
+                raise MemoryError("activation log full")
+            slots = range(len(self.act_slot), len(self.act_slot) + len(new_rids))
+        for r, t in zip(new_rids, self.cache.fork(self.tables[rid], n, len(new_rids))):
+            self.tables[r], self.held[r] = t, n
+        for r, sl in zip(new_rids, slots):
+            self.act_slot[r] = sl
+            self.act[sl, :n] = self.act[self.act_slot[rid], :n]
+
+    def compact(self) -> int:
+        """Move the live requests' KV blocks to the low end of the pool; returns the number moved."""
+        return self.cache.compact(self.tables.values())
+
     def _blocks_for(self, rid, upto: int) -> List[int]:
         t = self.tables.setdefault(rid, [])
         need = -(-upto // self.bs)
@@ -310,7 +331,8 @@ class StageRuntime:
         ctx = list(td[CX_CTX])
         n_new = list(td["n_new"])
         kind = td["kind"]
-        if kind == "prefill" and any(ctx):      # chunks that continue cached sequences
+        # chunks that continue cached sequences; an 8-bit cache is read for whole prompts, too
+        if kind == "prefill" and (any(ctx) or self.cache.scales is not None):
             kind = "mixed"
         n_dec = int(td.get("n_dec", 0)) if kind == "mixed" else None
         prefill = kind == "prefill"

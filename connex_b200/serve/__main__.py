@@ -38,6 +38,8 @@ def model_args(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--device", default="cuda:0")
     ap.add_argument("--num-blocks", type=int, default=0, help="KV blocks (0: from --kv-fraction of free memory)")
     ap.add_argument("--kv-fraction", type=float, default=0.8)
+    ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "fp8"],
+                    help="KV cache: bf16, or fp8 (e4m3 with a scale per block and head: twice the blocks)")
     ap.add_argument("--max-batch", type=int, default=64)
     ap.add_argument("--max-ctx", type=int, default=4096)
     ap.add_argument("--max-step-tokens", type=int, default=8192)
@@ -84,7 +86,8 @@ def kv_blocks(a, cfg, l0: int, l1: int) -> int:
     n_layers = l1 - l0
     per_layer = cfg.qkv_dim * cfg.hidden + cfg.hidden * cfg.heads * cfg.head_dim + 3 * cfg.ffn * cfg.hidden
     weights = 2 * (n_layers * per_layer + 2 * cfg.vocab_size * cfg.hidden)
-    block = 2 * n_layers * cfg.kv_heads * cfg.block_size * cfg.head_dim * 2
+    head = cfg.block_size * cfg.head_dim + 4 if getattr(a, "kv_dtype", "bf16") == "fp8" else cfg.block_size * cfg.head_dim * 2
+    block = 2 * n_layers * cfg.kv_heads * head
     scratch = 2 << 30                       # activations, workspaces, allocator slack
     return max(64, int((free - weights - scratch) * a.kv_fraction) // block)
 
@@ -104,7 +107,7 @@ def build_stepper(a):
     if a.num_stages == 1:
         n = kv_blocks(a, cfg, 0, cfg.layers)
         return ModelStepper(cfg, dev, n, a.max_batch, a.max_ctx, a.max_step_tokens, a.checkpoint, a.seed,
-                            graphs=not a.no_graphs), None
+                            graphs=not a.no_graphs, kv_dtype=a.kv_dtype), None
     from connex_b200.serve import pipeline
     ranges = pipeline.split_layers(cfg.layers, a.num_stages, a.stage_starts)
     if not a.directory:
@@ -113,7 +116,7 @@ def build_stepper(a):
     ep, client = pipeline.join(a.model_name or "connex-b200", 0, a.num_stages, a.replica, dev, a.directory, a.data,
                                a.store, a.store_master, a.advertise_host, a.recv_timeout_s)
     st = PipelineStepper(cfg, ranges[0][1], dev, ep, n, a.max_batch, a.max_ctx, a.max_step_tokens, a.checkpoint,
-                         a.seed, a.recv_timeout_s, graphs=not a.no_graphs)
+                         a.seed, a.recv_timeout_s, graphs=not a.no_graphs, kv_dtype=a.kv_dtype)
     ep.warm_stage(1)
     ep.auto_warm = True
     ep.watchdog = pipeline.watchdog(ep, st.link, client, step_timeout=a.step_timeout_s)
@@ -165,7 +168,7 @@ def _tp_stepper(a, cfg):
     t = torch.tensor([blocks], device=dev)
     dist.all_reduce(t, op=dist.ReduceOp.MIN)              # every rank sizes its KV cache alike
     inner = ModelStepper(cfg, dev, int(t.item()), a.max_batch, a.max_ctx, a.max_step_tokens, a.checkpoint,
-                         a.seed, graphs=False, tp=TPGroup(rank, world))
+                         a.seed, graphs=False, tp=TPGroup(rank, world), kv_dtype=a.kv_dtype)
     if rank == 0:
         return TPStepper(inner, cpu), ("tp", cpu)
     log.info("TP rank %d of %d following rank 0", rank, world)

@@ -247,12 +247,13 @@ class _RuntimeSteps(Stepper):
         self.rt.release(list(rids))
 
 
-def _make_runtime(cfg, l0, l1, device, num_blocks, max_batch, max_ctx, max_step_tokens, checkpoint, seed, tp=None):
+def _make_runtime(cfg, l0, l1, device, num_blocks, max_batch, max_ctx, max_step_tokens, checkpoint, seed, tp=None,
+                  kv_dtype="bf16"):
     """A StageRuntime for layers [l0, l1); with ``tp`` (a TPGroup) this rank's
     shard of them (checkpoint shards are cut on the host; random weights are
     drawn whole and cut, so every TP degree serves the same model)."""
     from connex_b200.runtime.pp import StageRuntime, stage_weights
-    weights, rcfg = None, cfg
+    weights, rcfg, kv = None, cfg, torch_kv_dtype(kv_dtype)
     if checkpoint:
         from connex_b200.models.hf import load_llama
         weights = load_llama(checkpoint, device, layers=(l0, l1), cfg=cfg,
@@ -265,7 +266,16 @@ def _make_runtime(cfg, l0, l1, device, num_blocks, max_batch, max_ctx, max_step_
         full.cfg = rcfg = tp_config(cfg, tp.world)
         weights = full
     return StageRuntime(rcfg, l0, l1, device, num_blocks=num_blocks, max_tokens=max_step_tokens, max_batch=max_batch,
-                        max_ctx=max_ctx, seed=seed, weights=weights, tp=tp)
+                        max_ctx=max_ctx, seed=seed, weights=weights, tp=tp, kv_dtype=kv)
+
+
+def torch_kv_dtype(name: str):
+    """``bf16`` or ``fp8`` (e4m3 with a scale per block and head) -> torch dtype of the KV cache."""
+    import torch
+    try:
+        return {"bf16": torch.bfloat16, "fp8": torch.float8_e4m3fn}[name]
+    except KeyError:
+        raise ValueError(f"KV cache type {name!r}: bf16 or fp8") from None
 
 
 class ModelStepper(_RuntimeSteps):
@@ -273,12 +283,12 @@ class ModelStepper(_RuntimeSteps):
 
     def __init__(self, cfg, device, num_blocks: int, max_batch: int = 64, max_ctx: int = 4096,
                  max_step_tokens: int = 8192, checkpoint: Optional[str] = None, seed: int = 0, graphs: bool = True,
-                 tp=None):
+                 tp=None, kv_dtype: str = "bf16"):
         self.cfg = cfg
         self.max_batch, self.max_ctx, self.max_step_tokens = max_batch, max_ctx, max_step_tokens
         self.block_size, self.vocab_size = cfg.block_size, cfg.vocab_size
         self.rt = _make_runtime(cfg, 0, cfg.layers, device, num_blocks, max_batch, max_ctx, max_step_tokens,
-                                checkpoint, seed, tp)
+                                checkpoint, seed, tp, kv_dtype)
         if graphs:
             self.rt.enable_decode_graphs()
         self.num_blocks = self.rt.cache.free_blocks          # less the graphs' trash block
@@ -439,7 +449,7 @@ class PipelineStepper(_RuntimeSteps):
 
     def __init__(self, cfg, l1: int, device, endpoint, num_blocks: int, max_batch: int = 64, max_ctx: int = 4096,
                  max_step_tokens: int = 8192, checkpoint: Optional[str] = None, seed: int = 0,
-                 recv_timeout_s: float = 30.0, graphs: bool = True, rt=None):
+                 recv_timeout_s: float = 30.0, graphs: bool = True, rt=None, kv_dtype: str = "bf16"):
         """``rt``: stage 0's compute when not the Llama runtime (the CPU
         stand-in :class:`RuleStageRuntime`)."""
         from connex.pp.link import Stage0Link
@@ -447,7 +457,7 @@ class PipelineStepper(_RuntimeSteps):
         self.max_batch, self.max_ctx, self.max_step_tokens = max_batch, max_ctx, max_step_tokens
         self.block_size, self.vocab_size = cfg.block_size, cfg.vocab_size
         self.rt = rt if rt is not None else _make_runtime(cfg, 0, l1, device, num_blocks, max_batch, max_ctx,
-                                                          max_step_tokens, checkpoint, seed)
+                                                          max_step_tokens, checkpoint, seed, kv_dtype=kv_dtype)
         if graphs and rt is None:
             self.rt.enable_decode_graphs()
         # downstream stages keep a trash block too when they run graphs

@@ -34,13 +34,15 @@ def run_stage(a, stop: threading.Event) -> dict:
     from connex_b200.models.hf import load_llama
     from connex_b200.runtime.pp import StageRuntime
     from connex_b200.serve import pipeline
+    from connex_b200.serve.engine import torch_kv_dtype
     cfg = llama_config(a)
     dev = torch.device(a.device)
     torch.cuda.set_device(dev)
     l0, l1 = pipeline.split_layers(cfg.layers, a.num_stages, a.stage_starts)[a.stage]
     weights = load_llama(a.checkpoint, dev, layers=(l0, l1), cfg=cfg) if a.checkpoint else None
     rt = StageRuntime(cfg, l0, l1, dev, num_blocks=kv_blocks(a, cfg, l0, l1), max_tokens=a.max_step_tokens,
-                      max_batch=a.max_batch, max_ctx=a.max_ctx, seed=a.seed, weights=weights)
+                      max_batch=a.max_batch, max_ctx=a.max_ctx, seed=a.seed, weights=weights,
+                      kv_dtype=torch_kv_dtype(a.kv_dtype))
     if not a.no_graphs:
         rt.enable_decode_graphs()
     ep, client = pipeline.join(a.model_name or "connex-b200", a.stage, a.num_stages, a.replica, dev, a.directory,

@@ -1,0 +1,280 @@
+"""The 8-bit KV cache and the block operations on the CPU: the quantising
+append's plain statement against its definition, shared blocks (fork, free,
+compaction) of both cache types, and the refusals of the operators' entry
+points -- argument checks come before the device check, so they run here."""
+import argparse
+import random
+
+import pytest
+import torch
+
+from connex_b200 import ops
+from connex_b200.models.llama import LlamaConfig, PagedKVCache
+from connex_b200.ops import reference as R
+
+BS, D = 16, 128
+
+
+def _cache(dtype, blocks=24, layers=2):
+    cfg = LlamaConfig.tiny(layers=layers)
+    c = PagedKVCache(cfg, blocks, "cpu", dtype)
+    g = torch.Generator().manual_seed(1)
+    raw = torch.randint(0, 120, c.kv.shape, generator=g, dtype=torch.uint8)
+    if dtype == torch.float8_e4m3fn:
+        c.kv.copy_(raw.view(torch.float8_e4m3fn))
+        c.scales.copy_(torch.rand(c.scales.shape, generator=g))
+    else:
+        c.kv.copy_(raw.float())
+    return c
+
+
+def _rows(c, table, n):
+    """What a sequence reads: values (and scales) of its first n tokens, layer by layer."""
+    bs = c.cfg.block_size
+    out = []
+    for i in range(n):
+        b, o = table[i // bs], i % bs
+        v = c.kv[:, :, b, :, o].float()
+        out.append(v if c.scales is None else v * c.scales[:, :, b][..., None])
+    return torch.stack(out) if out else torch.zeros(0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("n", [0, 1, 15, 16, 17, 48, 50])
+def test_fork_shares_full_blocks_and_copies_the_tail(dtype, n):
+    c = _cache(dtype)
+    t = c.allocate(4)
+    before = _rows(c, t, n)
+    free = c.free_blocks
+    a, b = c.fork(t, n, 2)
+    full = n // BS
+    assert a[:full] == b[:full] == t[:full]
+    assert len(a) == len(b) == c.blocks_needed(n)
+    assert free - c.free_blocks == (2 if n % BS else 0)
+    if n % BS:
+        assert len({t[full], a[-1], b[-1]}) == 3
+    assert torch.equal(_rows(c, a, n), before) and torch.equal(_rows(c, b, n), before)
+    # the child writes on in its own block only
+    if n % BS:
+        c.kv.view(torch.uint8 if dtype == torch.float8_e4m3fn else torch.bfloat16)[:, :, a[-1], :, n % BS:] = 0
+        assert torch.equal(_rows(c, t, n), before) and torch.equal(_rows(c, b, n), before)
+    for x in (a, t, b):
+        c.free(x)
+    assert c.free_blocks == 24 and sorted(c._free) == list(range(24)) and not c._shared
+
+
+def test_free_without_sharing_keeps_its_order():
+    c = _cache(torch.bfloat16)
+    a, b = c.allocate(3), c.allocate(2)
+    c.free(a)
+    assert c.allocate(3) == a
+    c.free(b)
+    assert c.allocate(1) == b[:1]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_compact_keeps_what_sequences_read(dtype):
+    rng = random.Random(3)
+    for _ in range(20):
+        c = _cache(dtype)
+        tables, lens = [], []
+        pin = c.allocate(1)                          # in no table: stays where it is
+        for _ in range(6):
+            n = rng.randint(1, 45)
+            if c.blocks_needed(n) > c.free_blocks:
+                break
+            tables.append(c.allocate(c.blocks_needed(n)))
+            lens.append(n)
+        k = rng.randrange(len(tables))
+        need = 1 if lens[k] % BS else 0
+        if c.free_blocks >= need:
+            tables += c.fork(tables[k], lens[k])
+            lens.append(lens[k])
+        for _ in range(rng.randint(0, 2)):
+            i = rng.randrange(len(tables))
+            c.free(tables.pop(i))
+            lens.pop(i)
+        before = [_rows(c, t, n) for t, n in zip(tables, lens)]
+        pinned = c.kv[:, :, pin[0]].clone()
+        free = c.free_blocks
+        moved = c.compact(tables)
+        assert c.free_blocks == free
+        used = {b for t in tables for b in t} | set(pin)
+        assert used == set(range(len(used))) and sorted(c._free) == list(range(len(used), 24))
+        for t, n, x in zip(tables, lens, before):
+            assert torch.equal(_rows(c, t, n), x)
+        assert torch.equal(c.kv[:, :, pin[0]].view(torch.uint8), pinned.view(torch.uint8))
+        assert c.compact(tables) == 0 or moved == 0
+        for t in tables:
+            c.free(t)
+        c.free(pin)
+        assert sorted(c._free) == list(range(24)) and not c._shared
+
+
+def test_cache_refusals():
+    c = _cache(torch.bfloat16)
+    t = c.allocate(2)
+    for n in (-1, 33):
+        with pytest.raises(ValueError, match="fork"):
+            c.fork(t, n)
+    with pytest.raises(ValueError, match="fork"):
+        c.fork(t, 5, -1)
+    c.allocate(21)
+    shared = dict(c._shared)
+    with pytest.raises(MemoryError):
+        c.fork(t, 20, 2)
+    assert c._shared == shared and c.free_blocks == 1       # a failed fork leaves nothing behind
+    for pairs in ([(0, 1), (1, 2)], [(0, 3), (1, 3)], [(2, 2)], [(0, 24)], [(-1, 2)]):
+        with pytest.raises(ValueError, match="copy_blocks"):
+            c.copy_blocks(pairs)
+    c.copy_blocks([])
+
+
+def test_append_statement_follows_the_definition():
+    """Scale: smallest power of two with amax <= 448 s; rows within half a step; old rows keep their values."""
+    g = torch.Generator().manual_seed(5)
+    for trial in range(40):
+        cache = (torch.randn(3, 2, BS, D, generator=g) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+        scale = torch.exp2(torch.randint(-6, 0, (3, 2), generator=g).float())
+        was, old = R.fp8_values(cache, scale), scale.clone()
+        n = int(torch.randint(1, 20, (1,), generator=g))
+        slots = torch.randint(-1, 3 * BS, (n,), generator=g)
+        rows = (torch.randn(n, 2, D, generator=g) * 10.0 ** float(torch.randint(-3, 4, (1,), generator=g))).to(torch.bfloat16)
+        R.fp8_append(cache, scale, rows, slots)
+        now = R.fp8_values(cache, scale)
+        last = {int(s): t for t, s in enumerate(slots.tolist()) if s >= 0}
+        for b in range(3):
+            mine = {s % BS: t for s, t in last.items() if s // BS == b}
+            top = torch.stack([rows[t].double().abs().amax(-1) for t in mine.values()]).amax(0) if mine else None
+            for h in range(2):
+                s = float(scale[b, h])
+                if not mine:
+                    assert s == float(old[b, h]) and torch.equal(now[b, h], was[b, h])
+                    continue
+                floor = 0.0 if 0 in mine else float(old[b, h])
+                assert float(top[h]) <= 448 * s and s >= floor
+                assert s == floor or float(top[h]) > 224 * s
+                for r in range(BS):
+                    if r in mine:
+                        x = rows[mine[r], h].double()
+                        assert ((now[b, h, r] - x).abs() <= (x.abs() * 2.0 ** -4).clamp(min=2.0 ** -10 * s)).all()
+                    elif 0 not in mine:
+                        assert ((now[b, h, r] - was[b, h, r]).abs() <= 2.0 ** -10 * s).all()
+
+
+def _args(hq=4, hkv=2, T=3, nb=5, B=2):
+    f8 = torch.float8_e4m3fn
+    return dict(qkv=torch.zeros(T, (hq + 2 * hkv) * D, dtype=torch.bfloat16), pos=torch.zeros(T, dtype=torch.int32),
+                cs=torch.zeros(64, D), slots=torch.zeros(T, dtype=torch.int64),
+                k=torch.zeros(nb, hkv, BS, D).to(f8), v=torch.zeros(nb, hkv, BS, D).to(f8), ks=torch.ones(nb, hkv),
+                vs=torch.ones(nb, hkv), q=torch.zeros(B, hq * D, dtype=torch.bfloat16),
+                bt=torch.zeros(B, 4, dtype=torch.int32), lens=torch.ones(B, dtype=torch.int32),
+                ws=torch.zeros(10, 2 * 132), ti=torch.zeros(1, 5, dtype=torch.int32))
+
+
+def _write(a, hq=4, hkv=2, **kw):
+    return ops.rope_cache_fp8(a["qkv"], a["pos"], a["cs"], hq, hkv, a["slots"], a["k"], a["v"], a["ks"], a["vs"], **kw)
+
+
+def _decode(a, hq=4, **kw):
+    return ops.decode_attention_fp8(a["q"], a["k"], a["v"], a["ks"], a["vs"], a["bt"], a["lens"], hq, a["ws"], **kw)
+
+
+def _prefill(a, hq=4, hkv=2, **kw):
+    return ops.prefill_attention_paged_fp8(a["q"], a["k"], a["v"], a["ks"], a["vs"], a["bt"], a["ti"], hq, hkv, **kw)
+
+
+@pytest.mark.parametrize("call,change,match", [
+    (_write, {"qkv": lambda t: t.float()}, "bf16"),
+    (_write, {"qkv": lambda t: t[:, 8:]}, "heads of 128"),
+    (_write, {"qkv": lambda t: torch.zeros(3, 8 * D + 4, dtype=torch.bfloat16)[:, 4:]}, "16-byte"),
+    (_write, {"qkv": lambda t: t[:, :1].expand(3, 8 * D)}, "contiguous rows|16-byte"),
+    (_write, {"pos": lambda t: t.long()}, "positions"),
+    (_write, {"pos": lambda t: t[:2]}, "positions"),
+    (_write, {"slots": lambda t: t.int()}, "slot_mapping"),
+    (_write, {"slots": lambda t: torch.zeros(4, dtype=torch.int64)}, "slot_mapping"),
+    (_write, {"cs": lambda t: t.double()}, "cos_sin"),
+    (_write, {"cs": lambda t: t[:, :64]}, "cos_sin"),
+    (_write, {"k": lambda t: t.view(torch.uint8)}, "float8_e4m3fn"),
+    (_write, {"v": lambda t: t[:4]}, "float8_e4m3fn"),
+    (_write, {"k": lambda t: t[:, :1], "v": lambda t: t[:, :1]}, "float8_e4m3fn"),
+    (_write, {"ks": lambda t: t.double()}, "scales"),
+    (_write, {"vs": lambda t: t[:4]}, "scales"),
+    (_write, {}, "must be a CUDA tensor"),
+    (_decode, {"q": lambda t: t.half()}, "bf16"),
+    (_decode, {"q": lambda t: t[:, :256]}, "Hq heads"),
+    (_decode, {"bt": lambda t: t.long()}, "block_tables"),
+    (_decode, {"bt": lambda t: t[:1]}, "block_tables"),
+    (_decode, {"bt": lambda t: torch.zeros(2, 8, dtype=torch.int32)[:, ::2]}, "block_tables"),
+    (_decode, {"lens": lambda t: t.long()}, "ctx_lens"),
+    (_decode, {"lens": lambda t: t[:1]}, "ctx_lens"),
+    (_decode, {"vs": lambda t: t.t().contiguous()}, "scales"),
+    (_decode, {}, "must be a CUDA tensor"),
+    (_prefill, {"q": lambda t: t.float()}, "bf16"),
+    (_prefill, {"q": lambda t: t[:, :256]}, "Hq heads"),
+    (_prefill, {"ti": lambda t: t[:, :3]}, "tile_info"),
+    (_prefill, {"ti": lambda t: t.long()}, "tile_info"),
+    (_prefill, {"bt": lambda t: t.long()}, "block_tables"),
+    (_prefill, {"k": lambda t: t.view(torch.uint8)}, "float8_e4m3fn"),
+    (_prefill, {"ks": lambda t: t.double()}, "scales"),
+    (_prefill, {}, "must be a CUDA tensor"),
+])
+def test_refusals(call, change, match):
+    a = _args()
+    a.update({n: f(a[n]) for n, f in change.items()})
+    with pytest.raises(RuntimeError, match=match):
+        call(a)
+
+
+def test_more_refusals():
+    a = _args()
+    with pytest.raises(RuntimeError, match="q/k norm"):
+        _write(a, q_norm=torch.ones(64, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError, match="overlaps"):
+        _write(a, out=a["qkv"][:, D:5 * D])
+    with pytest.raises(RuntimeError, match="out must be"):
+        _write(a, out=a["qkv"][:, :3 * D])
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        _write(a, out=a["qkv"][:, :4 * D])                          # in place is allowed
+    with pytest.raises(RuntimeError, match="multiple of the KV heads"):
+        _decode(a, hq=3)
+    with pytest.raises(RuntimeError, match="16 of them"):
+        _decode({**_args(hq=34), "q": torch.zeros(2, 34 * D, dtype=torch.bfloat16)}, hq=34)
+    with pytest.raises(ValueError, match="multiple of the KV heads"):
+        ops.decode_workspace_fp8(4, 10, 4, "cuda:0")
+    kv = torch.zeros(2, 2, 5, 2, BS, D, dtype=torch.bfloat16)
+    pairs = torch.zeros(1, 2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ops.kv_copy_blocks(kv[:, :, ::2], pairs)
+    with pytest.raises(RuntimeError, match="pairs"):
+        ops.kv_copy_blocks(kv, pairs.long())
+    with pytest.raises(RuntimeError, match="with its scales"):
+        ops.kv_copy_blocks(kv.to(torch.float8_e4m3fn), pairs)
+    with pytest.raises(RuntimeError, match="scales"):
+        ops.kv_copy_blocks(kv.to(torch.float8_e4m3fn), pairs, torch.ones(2, 2, 5, 3))
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        ops.kv_copy_blocks(kv, pairs)
+
+
+def test_layerwise_transfer_refuses_an_8_bit_cache():
+    from connex_b200.runtime.pd import KVDestination
+    c = _cache(torch.float8_e4m3fn)
+    with pytest.raises(ValueError, match="scales do not travel"):
+        KVDestination.of_cache(c, torch.zeros(1, dtype=torch.int32))
+    KVDestination.of_cache(_cache(torch.bfloat16), torch.zeros(1, dtype=torch.int32))
+
+
+def test_cli_kv_dtype(monkeypatch):
+    from connex_b200.serve.__main__ import kv_blocks, model_args
+    from connex_b200.serve.engine import torch_kv_dtype
+    ap = argparse.ArgumentParser()
+    model_args(ap)
+    cfg = LlamaConfig.tiny()
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a: (60 << 30, 0))
+    n16, n8 = (kv_blocks(ap.parse_args(["--kv-dtype", d]), cfg, 0, 2) for d in ("bf16", "fp8"))
+    assert 1.99 < n8 / n16 <= 2.0
+    assert torch_kv_dtype("fp8") == torch.float8_e4m3fn and torch_kv_dtype("bf16") == torch.bfloat16
+    with pytest.raises(ValueError, match="bf16 or fp8"):
+        torch_kv_dtype("int8")
+    with pytest.raises(SystemExit):
+        ap.parse_args(["--kv-dtype", "int8"])

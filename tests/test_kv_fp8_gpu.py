@@ -482,3 +482,112 @@ def test_step_in_a_graph(dev):
                 assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
     for _, io in sides:
         ops.check_status(io["st"])
+
+
+def _runtime(dev, dtype, seed=0, layers=2, max_batch=8):
+    from connex_b200.models.llama import LlamaConfig
+    from connex_b200.runtime.pp import StageRuntime
+    cfg = LlamaConfig.tiny(layers=2)
+    return cfg, StageRuntime(cfg, 0, layers, dev, num_blocks=128, max_tokens=512, max_batch=max_batch, max_ctx=512,
+                             seed=seed, kv_dtype=dtype)
+
+
+def _compute(rt, kind, rids, ctx, n_new, ids, n_dec=None):
+    from connex.pp.handover import CX_CTX, REQUEST_IDS
+    td = {"kind": kind, REQUEST_IDS: rids, CX_CTX: ctx, "n_new": n_new,
+          "ids": torch.tensor(ids, dtype=torch.int32, device=rt.device)}
+    if n_dec is not None:
+        td["n_dec"] = n_dec
+    out = rt.compute(td, [])
+    return out["x"].float() if "x" in out else out["next"]
+
+
+def test_stage_runtime_8_bit(dev):
+    """A stage of the model over an 8-bit cache: residual rows near those of the
+    bf16 cache, whole or chunked prompt, decode rows in the same steps."""
+    g = torch.Generator().manual_seed(3)
+    prompt = torch.randint(3, 1000, (200,), generator=g).tolist()
+    got = {}
+    for dtype in (torch.bfloat16, torch.float8_e4m3fn):
+        _, rt = _runtime(dev, dtype, layers=1)
+        whole = _compute(rt, "prefill", ["w"], [0], [200], prompt)
+        parts, done = [], 0
+        for n in (16, 1, 50, 133):
+            parts.append(_compute(rt, "mixed", ["c"], [done], [n], prompt[done:done + n], n_dec=1 if n == 1 else 0))
+            done += n
+        dec = _compute(rt, "decode", ["w", "c"], [200, 200], [1, 1], [5, 5])
+        mix = _compute(rt, "mixed", ["w", "d"], [201, 0], [1, 40], [7] + prompt[:40], n_dec=1)
+        torch.cuda.synchronize()
+        assert int(rt.model.status) == 0
+        got[dtype] = (whole, torch.cat(parts), dec, mix)
+    a, b = got[torch.bfloat16], got[torch.float8_e4m3fn]
+    # the attention's share of the residual changes by at most e4m3's 2^-4 of it (K and V); the random
+    # weights' attention output is a small part of the rows
+    for x, y in zip(a, b):
+        assert (x - y).norm() <= 2.0 ** -4 * x.norm()
+    w, c, dec, _ = b
+    assert (w - c).norm() <= 2.0 ** -6 * w.norm()          # only rows of shared blocks were scaled twice
+    assert (dec[0] - dec[1]).norm() <= 2.0 ** -6 * dec[0].norm()
+
+
+def test_decode_graphs_and_fork_8_bit(dev):
+    """Decode graphs (padding rows on one trash slot) give the eager rows; forked
+    requests continue like their parent, before and after a compaction."""
+    g = torch.Generator().manual_seed(4)
+    prompts = [torch.randint(3, 1000, (n,), generator=g).tolist() for n in (37, 16, 90)]
+    outs = []
+    for graphs in (False, True):
+        cfg, rt = _runtime(dev, torch.float8_e4m3fn)
+        if graphs:
+            rt.enable_decode_graphs((4, 8))
+        _compute(rt, "prefill", ["a", "b", "c"], [0] * 3, [len(p) for p in prompts], sum(prompts, []))
+        lens, steps = [len(p) for p in prompts], []
+        for t in range(20):
+            steps.append(_compute(rt, "decode", ["a", "b", "c"], lens, [1] * 3, [7 + t, 9 + t, 11 + t]).tolist())
+            lens = [n + 1 for n in lens]
+        rt.fork("a", ["x", "y"])
+        assert rt.held["x"] == lens[0] and rt.tables["x"][0] == rt.tables["a"][0]
+        rt.release(["b"])
+        assert rt.compact() > 0 or graphs
+        for t in range(18):
+            s = _compute(rt, "decode", ["a", "x", "y", "c"], [lens[0]] * 3 + [lens[2]], [1] * 4, [30 + t] * 3 + [t + 3]).tolist()
+            assert s[0] == s[1] == s[2]
+            steps.append(s)
+            lens = [n + 1 for n in lens]
+        rt.release(["a", "x", "y", "c"])
+        assert rt.cache.free_blocks == 128 - (1 if graphs else 0) and not rt.cache._shared
+        assert int(rt.model.status) == 0
+        outs.append(steps)
+    assert outs[0] == outs[1]
+
+
+def test_model_stepper_8_bit(dev):
+    """The serving engine's stepper over an 8-bit cache: prefill, chunked prefill and decode agree."""
+    from connex_b200.models.llama import LlamaConfig
+    from connex_b200.serve.engine import ModelStepper
+    st = ModelStepper(LlamaConfig.tiny(), dev, 96, max_batch=4, max_ctx=256, max_step_tokens=256, kv_dtype="fp8")
+    seq = list(range(3, 80))
+    a = st.prefill(["p"], [seq])
+    b = st.mixed(["q"], [seq], [0], [64])
+    b = st.mixed(["q"], [seq], [64], [13])
+    assert a == b
+    d1 = st.decode(["p", "q"], [seq + a, seq + a])
+    assert d1[0] == d1[1]
+    st.release(["p", "q"])
+
+
+def test_push_moves_an_8_bit_cache_in_two_calls(dev):
+    """kv_push_layer takes the values by head slices of 2 KB and the scales as one 16-byte unit per block."""
+    from connex_b200 import ops
+    nb, hkv = 12, 4
+    k, ks = _cache(nb, hkv, dev, 111)
+    v, vs = _cache(nb, hkv, dev, 112)
+    dst = [torch.zeros_like(t) for t in (k, v, ks, vs)]
+    pairs = torch.tensor([[3, 7], [5, 1]], dtype=torch.int32, device=dev)
+    ops.kv_push_layer(k.data_ptr(), v.data_ptr(), dst[0].data_ptr(), dst[1].data_ptr(), pairs, src_heads=hkv,
+                      dst_heads=hkv, chunk_bytes=BS * D, src_blocks=nb, dst_blocks=nb)
+    ops.kv_push_layer(ks.data_ptr(), vs.data_ptr(), dst[2].data_ptr(), dst[3].data_ptr(), pairs, src_heads=1,
+                      dst_heads=1, chunk_bytes=4 * hkv, src_blocks=nb, dst_blocks=nb)
+    for s, d in ((3, 7), (5, 1)):
+        for a, b in zip((k, v, ks, vs), dst):
+            assert torch.equal(a[s].view(torch.uint8), b[d].view(torch.uint8))

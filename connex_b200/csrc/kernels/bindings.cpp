@@ -372,8 +372,9 @@ void kv_copy_blocks(at::Tensor& kv, const at::Tensor& pairs, const c10::optional
 void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
                                  const at::Tensor& vs, const at::Tensor& block_tables, at::Tensor& out,
                                  const at::Tensor& tile_info, int64_t Hq, int64_t Hkv, double scale, at::Tensor& kw,
-                                 at::Tensor& vw, at::Tensor& table, const c10::optional<at::Tensor>& status) {
-  check_same_device(q, {&kc, &block_tables, &out, &tile_info, &kw, &vw, &table}, "prefill_attention_paged_fp8");
+                                 at::Tensor& vw, at::Tensor& table, at::Tensor& tiles,
+                                 const c10::optional<at::Tensor>& status) {
+  check_same_device(q, {&kc, &block_tables, &out, &tile_info, &kw, &vw, &table, &tiles}, "prefill_attention_paged_fp8");
   const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "prefill_attention_paged_fp8");
   const int ldq = row_ld16(q, "prefill_attention_paged_fp8: q"), ldo = row_ld16(out, "prefill_attention_paged_fp8: out");
   const int64_t T = q.size(0);
@@ -385,18 +386,26 @@ void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, cons
                   tile_info.is_contiguous(),
               "prefill_attention_paged_fp8: tile_info must be contiguous int32 [n, 5]");
   TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
-                  block_tables.numel() * Hkv * 16 <= INT_MAX,
+                  block_tables.numel() * Hkv * 16 <= INT_MAX && block_tables.size(0) <= 65535,
               "prefill_attention_paged_fp8: block_tables must be contiguous int32 [B, max_blocks]");
+  TORCH_CHECK(kw.numel() == block_tables.numel() * Hkv * 16 * 128 && vw.sizes() == kw.sizes() && kw.is_contiguous() &&
+                  vw.is_contiguous() && kw.scalar_type() == at::kBFloat16 && vw.scalar_type() == at::kBFloat16 &&
+                  table.scalar_type() == at::kInt && table.sizes() == block_tables.sizes() && table.is_contiguous() &&
+                  tiles.scalar_type() == at::kInt && tiles.sizes() == tile_info.sizes() && tiles.is_contiguous(),
+              "prefill_attention_paged_fp8: workspaces must be bf16 [B * max_blocks, Hkv, 16, 128] and int32 like the tables and tiles");
   CHECK_CUDA(q);
   const c10::cuda::CUDAGuard g(q.device());
+  TORCH_CHECK(T == 0 || tile_info.size(0) == 0 || block_tables.numel() > 0,
+              "prefill_attention_paged_fp8: no block table for the tiles");
   if (T == 0 || tile_info.size(0) == 0) return;
-  cx::kv_dequant_blocks(c, block_tables.data_ptr<int>(), (int)block_tables.numel(), kw.data_ptr(), vw.data_ptr(),
-                        table.data_ptr<int>(), status_ptr(status), cur_stream(q));
+  cx::kv_dequant_blocks(c, block_tables.data_ptr<int>(), (int)block_tables.size(0), (int)block_tables.size(1),
+                        tile_info.data_ptr<int>(), (int)tile_info.size(0), (int)T, kw.data_ptr(), vw.data_ptr(),
+                        table.data_ptr<int>(), tiles.data_ptr<int>(), status_ptr(status), cur_stream(q));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   cx::prefill_attention_paged_tc(q.data_ptr(), ldq, (int)(Hq * 128), (int)T, kw.data_ptr(), vw.data_ptr(),
                                  block_tables.numel() * Hkv * 16, table.data_ptr<int>(), (int)block_tables.size(1),
-                                 out.data_ptr(), ldo, tile_info.data_ptr<int>(), (int)tile_info.size(0), (int)Hq,
-                                 (int)Hkv, (float)scale, status_ptr(status), cur_stream(q), 256);
+                                 out.data_ptr(), ldo, tiles.data_ptr<int>(), (int)tiles.size(0), (int)Hq, (int)Hkv,
+                                 (float)scale, status_ptr(status), cur_stream(q), 256);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 

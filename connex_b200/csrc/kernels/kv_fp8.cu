@@ -1095,43 +1095,94 @@ void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes
 }
 
 // --------------------------------------------------------- dequantised blocks
-// Blocks of the tables' entries as bf16 (exact: the scales are powers of two),
-// one after the other, and the table that finds them there.
-__global__ void __launch_bounds__(256)
-    kv_dequant_kernel(KvFp8 c, const int* __restrict__ table, __nv_bfloat16* ko, __nv_bfloat16* vo, int* table_out,
-                      int* status) {
+// The blocks that the tiles of a chunked prefill read, as bf16 (exact: the
+// scales are powers of two), entry i of the tables in block i, and the tables
+// that find them there.  Bound by memory and short next to the attention that
+// follows: 10 of 226 us for 2048 rows at 6144.  (Converting inside the
+// attention kernel, by four more warps between the copies and the MMAs, took
+// 302 us: the thread that issues the MMAs is busy 83 % of its time, and a
+// converter on its SM quarter slows it.)
+// One CTA per entry: all heads of K, then of V, 16 bytes of a lane each.  The
+// first CTA also hands the tiles on, checked: the attention kernel takes them
+// as they are, so one that does not fit the rows or the tables is recorded and
+// replaced by a valid one (whose rows are then written twice, alike).
+namespace kvd {
+constexpr int THREADS = 256;
+}
+__device__ __forceinline__ bool tile_fits(const int* ti, int T, int B, int width) {
+  const int start = ti[0], n = ti[1], q0 = ti[2], ctx = ti[3], seq = ti[4];
+  return seq >= 0 && seq < B && n > 0 && q0 >= 0 && q0 < n && ctx >= 0 && start >= 0 && (int64_t)start + n <= T &&
+         (int64_t)ctx + n <= (int64_t)width * kvq::BS;
+}
+__global__ void __launch_bounds__(kvd::THREADS)
+    kv_dequant_kernel(KvFp8 c, const int* __restrict__ tables, int width, const int* __restrict__ tile_info, int n_tiles,
+                      int T, __nv_bfloat16* ko, __nv_bfloat16* vo, int* tables_out, int* tiles_out, int* status) {
   using namespace kvq;
-  const int i = blockIdx.x, h = blockIdx.y, id = table[i];
-  if (h == 0 && threadIdx.x == 0) table_out[i] = i;
+  const int seq = blockIdx.y, tid = threadIdx.x, B = gridDim.y;
+  const int64_t i = (int64_t)seq * width + blockIdx.x;
+  // tokens of the sequence: any of its tiles tells
+  int total = 0;
+  for (int t = tid; t < n_tiles; t += kvd::THREADS)
+    if (tile_info[5 * t + 4] == seq && tile_fits(tile_info + 5 * t, T, B, width))
+      total = max(total, tile_info[5 * t + 1] + tile_info[5 * t + 3]);
+  __shared__ int most, valid;
+  if (tid == 0) {
+    most = 0;
+    valid = 0x7fffffff;
+  }
+  __syncthreads();
+  if (total > 0) atomicMax(&most, total);
+  if (blockIdx.x == 0 && seq == 0) {
+    for (int t = tid; t < n_tiles; t += kvd::THREADS)
+      if (tile_fits(tile_info + 5 * t, T, B, width)) atomicMin(&valid, t);
+    __syncthreads();
+    for (int t = tid; t < n_tiles; t += kvd::THREADS) {
+      const bool fits = tile_fits(tile_info + 5 * t, T, B, width);
+      if (!fits) record_status(status, CX_ERR_BOUNDS);
+      const int from = fits ? t : valid;
+      for (int e = 0; e < 5; ++e)
+        tiles_out[5 * t + e] = from < n_tiles ? tile_info[5 * from + e] : e == 1;   // none fits: one row, one key
+    }
+  }
+  __syncthreads();
+  if (tid == 0) tables_out[i] = (int)i;
+  if (blockIdx.x >= (most + BS - 1) / BS) return;       // behind the end: never read
+  const int id = tables[i];
   const bool in = id >= 0 && id < c.num_blocks;
-  if (!in && h == 0 && threadIdx.x == 0) record_status(status, CX_ERR_BOUNDS);
-  const size_t to = ((size_t)i * c.Hkv + h) * (BS * D);
-  const int half = threadIdx.x >> 7, e = (threadIdx.x & 127) * 16;
-  u128 raw{0, 0, 0, 0};           // an id out of range reads as zeros
-  float f = 0.f;
-  if (in) {
-    raw = ld_nc_v4((half ? c.v : c.k) + ((size_t)id * c.Hkv + h) * (BS * D) + e);
-    f = (half ? c.vs : c.ks)[(size_t)id * c.Hkv + h];
-  }
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
-  u128 o[2];
-  uint32_t* po = reinterpret_cast<uint32_t*>(o);
+  if (!in && tid == 0) record_status(status, CX_ERR_BOUNDS);
+  const int per = c.Hkv * (BS * D / 16);                // 16-byte pieces of K, and of V
+#pragma unroll 4
+  for (int v = tid; v < 2 * per; v += kvd::THREADS) {
+    const bool is_v = v >= per;
+    const int e = (is_v ? v - per : v) * 16, h = e / (BS * D);
+    u128 raw{0, 0, 0, 0};                               // an id out of range reads as zeros
+    float f = 0.f;
+    if (in) {
+      raw = ld_nc_v4((is_v ? c.v : c.k) + (size_t)id * c.Hkv * (BS * D) + e);
+      f = (is_v ? c.vs : c.ks)[(size_t)id * c.Hkv + h];
+    }
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
+    u128 o[2];
+    uint32_t* po = reinterpret_cast<uint32_t*>(o);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint32_t a = e4m3x2_to_f16x2((uint16_t)w[k]), b = e4m3x2_to_f16x2((uint16_t)(w[k] >> 16));
-    po[2 * k] = pack_bf16x2(f16_lo(a) * f, f16_hi(a) * f);
-    po[2 * k + 1] = pack_bf16x2(f16_lo(b) * f, f16_hi(b) * f);
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t a = e4m3x2_to_f16x2((uint16_t)w[k]), b = e4m3x2_to_f16x2((uint16_t)(w[k] >> 16));
+      po[2 * k] = pack_bf16x2(f16_lo(a) * f, f16_hi(a) * f);
+      po[2 * k + 1] = pack_bf16x2(f16_lo(b) * f, f16_hi(b) * f);
+    }
+    __nv_bfloat16* d = (is_v ? vo : ko) + (size_t)i * c.Hkv * (BS * D) + e;
+    st_v4(d, o[0]);
+    st_v4(d + 8, o[1]);
   }
-  __nv_bfloat16* d = (half ? vo : ko) + to + e;
-  st_v4(d, o[0]);
-  st_v4(d + 8, o[1]);
 }
 
-void kv_dequant_blocks(const KvFp8& c, const int* table, int n, void* kout, void* vout, int* table_out, int* status,
-                       cudaStream_t s) {
-  if (n == 0) return;
-  kv_dequant_kernel<<<dim3(n, c.Hkv), 256, 0, s>>>(c, table, reinterpret_cast<__nv_bfloat16*>(kout),
-                                                   reinterpret_cast<__nv_bfloat16*>(vout), table_out, status);
+void kv_dequant_blocks(const KvFp8& c, const int* tables, int B, int width, const int* tile_info, int n_tiles, int T,
+                       void* kout, void* vout, int* tables_out, int* tiles_out, int* status, cudaStream_t s) {
+  if (B == 0 || width == 0) return;
+  kv_dequant_kernel<<<dim3(width, B), kvd::THREADS, 0, s>>>(c, tables, width, tile_info, n_tiles, T,
+                                                            reinterpret_cast<__nv_bfloat16*>(kout),
+                                                            reinterpret_cast<__nv_bfloat16*>(vout), tables_out,
+                                                            tiles_out, status);
 }
 
 }  // namespace cx

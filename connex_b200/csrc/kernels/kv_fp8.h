@@ -43,8 +43,11 @@ void decode_attention_fp8(const void* q, int ldq, const KvFp8& c, const int* blo
 void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes, int num_blocks, int64_t block_bytes,
                     int Hkv, int sms, int* status, cudaStream_t s);
 
-// e4m3 blocks table[i] -> bf16 blocks i of kout / vout [n, Hkv, 16, 128]; table_out[i] = i.
-void kv_dequant_blocks(const KvFp8& c, const int* table, int n, void* kout, void* vout, int* table_out, int* status,
-                       cudaStream_t s);
+// The e4m3 blocks that the tiles (tile_info [n_tiles, 5] of the paged prefill)
+// read through tables [B, width], as bf16 blocks of kout / vout [B * width,
+// Hkv, 16, 128]: entry i in block i; tables_out[i] = i.  tiles_out: the tiles,
+// those that do not fit T rows and the tables replaced.
+void kv_dequant_blocks(const KvFp8& c, const int* tables, int B, int width, const int* tile_info, int n_tiles, int T,
+                       void* kout, void* vout, int* tables_out, int* tiles_out, int* status, cudaStream_t s);
 
 }  // namespace cx

@@ -341,14 +341,22 @@ def prefill_attention_paged_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache:
                                 out: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                                 status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`prefill_attention_paged` over an 8-bit cache: causal attention of
-    prompt chunks, ``q`` [T, Hq * 128] rotated, keys and values of the whole
-    context -- this chunk's included -- from the cache."""
+    prompt chunks, ``q`` [T, >= Hq * 128] rotated (q heads first), keys and
+    values of the whole context -- this chunk's included -- from the cache.
+    ``tile_info`` from ``prefill_tile_info(n_new, device, ctx)``.  The blocks
+    that the chunks read are turned into bf16 first (exact: the scales are
+    powers of two), in a workspace of the tables' size, so the tables should
+    be no wider than the longest sequence.  Entries behind a sequence's end
+    are not read.  A block id out of range reads as zeros, and a tile that
+    does not fit ``q``'s rows or the tables is left out; both are recorded in
+    ``status``."""
     if out is None:
         out = torch.empty(q.shape[0], n_q_heads * 128, dtype=q.dtype, device=q.device)
     k = torch.empty(block_tables.numel(), n_kv_heads, 16, 128, dtype=torch.bfloat16, device=q.device)
     _C.prefill_attention_paged_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tables, out, tile_info, n_q_heads,
                                    n_kv_heads, scale if scale is not None else 1.0 / math.sqrt(128), k,
-                                   torch.empty_like(k), torch.empty_like(block_tables), status)
+                                   torch.empty_like(k), torch.empty_like(block_tables), torch.empty_like(tile_info),
+                                   status)
     _n(2)
     return out
 

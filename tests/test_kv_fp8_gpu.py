@@ -128,7 +128,6 @@ def test_prefill_attention(dev, heads, rows):
     ctx, new = [c for c, _ in rows], [n for _, n in rows]
     lens = [c + n for c, n in rows]
     table, nb = _table(lens, dev, 5)
-    table.clamp_(min=0)
     k, ks = _cache(nb, hkv, dev, 6)
     v, vs = _cache(nb, hkv, dev, 7, -10, -2)
     _nan_rows(k, table, lens)
@@ -405,6 +404,44 @@ def test_decode_bad_pages_and_lengths(dev):
             else:
                 err = (out[b].view(hq, D).double() - ref[b]).abs()
                 assert (err <= U_BF16 * ref[b].abs() + mag[b] * 2.0 ** -8 + 1e-6).all()
+
+
+def test_prefill_bad_pages_and_tiles(dev):
+    """A block id out of range reads as zeros; a tile that fits neither the rows nor the tables is left out."""
+    from connex_b200 import ops
+    from connex_b200.ops import reference as R
+    hq, hkv, nb = 4, 2, 12
+    k, ks = _cache(nb, hkv, dev, 121)
+    v, vs = _cache(nb, hkv, dev, 122)
+    q = torch.randn(40, hq * D, generator=_g(dev, 123), device=dev).to(torch.bfloat16)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    table = i32([[3, 4, 1], [5, 6, 2]])
+    good = [(0, 20, 0, 28, 0), (20, 20, 0, 10, 1)]
+    st = ops.new_status(dev)
+    ref = ops.prefill_attention_paged_fp8(q, k, v, ks, vs, table, i32(good), hq, hkv, status=st)
+    ops.check_status(st)
+    for bad in ((20, 20, 0, 29, 1), (21, 20, 0, 10, 1), (-1, 5, 0, 0, 1), (20, 20, 0, 10, 2), (20, 20, 20, 10, 1),
+                (20, 0, 0, 10, 1), (20, 20, 0, -1, 1), (20, 20, -1, 10, 1), (20, 20, 0, 2**31 - 1, 1)):
+        st = ops.new_status(dev)
+        out = torch.full_like(ref, 7.0)
+        ops.prefill_attention_paged_fp8(q, k, v, ks, vs, table, i32([good[0], bad]), hq, hkv, out=out, status=st)
+        with pytest.raises(RuntimeError, match="bounds"):
+            ops.check_status(st)
+        assert torch.equal(out[:20], ref[:20]) and (out[20:] == 7.0).all()
+    for bad in (nb, -1, 2**31 - 1):
+        st = ops.new_status(dev)
+        t = table.clone()
+        t[1, 1] = bad
+        out = ops.prefill_attention_paged_fp8(q, k, v, ks, vs, t, i32(good), hq, hkv, status=st)
+        with pytest.raises(RuntimeError, match="bounds"):
+            ops.check_status(st)
+        assert torch.equal(out[:20], ref[:20])
+        k0, v0 = k.clone(), v.clone()
+        k0.view(torch.uint8)[6] = 0
+        v0.view(torch.uint8)[6] = 0
+        want, mag = R.paged_attention_fp8(q.view(40, hq, D)[20:], k0, v0, ks, vs, table[1:], [10], [20])
+        err = (out[20:].view(20, hq, D).double() - want).abs()
+        assert (err <= U_BF16 * want.abs() + mag * 2.0 ** -6 + 1e-6).all()
 
 
 def test_decode_nan_and_extreme_logits(dev):

@@ -416,35 +416,30 @@ void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_s
 }
 
 // ------------------------------------------------------- decode attention
-// S = q.K^T and O^T = V^T.W^T on mma.sync m16n8k32 with e4m3 operands: the
-// cached bytes go into the tensor cores as they are (measured: 4.3 cycles per
-// instruction and SM quarter against 8 for the f16 m16n8k16 of half the
-// depth, sums exact to 2^-25).  q and the softmax weights enter as the sum of two
-// e4m3 numbers each:
-//   q     scaled by a power of two per head to at most 448; bf16's 8-bit
-//         significand is two 4-bit ones, so only elements 2^11 times smaller
-//         than the head's largest lose bits (at most 2^-18 of the largest).
-//         With up to 8 heads the two parts are rows 0-7 and 8-15 of one A.
-//   w     exp2(z - max z of the 32 tokens + 8): two parts leave 2^-8 of the
-//         value, as bf16 would, and 2^-18 of the largest weight.  The 32
-//         tokens' product is its own sum, added to O in fp32 with the factor
-//         that relates the two maxima.
-// Fragments come straight from the cache's layout:
+// S = q.K^T and O^T = V^T.W^T on mma.sync m16n8k16 (f16 in, fp32 out).  The
+// cached bytes are turned into f16 (exact) in registers, in the fragments'
+// layout as they come from the cache; the block scales stay out of the
+// operands.  (mma.sync takes e4m3 operands too, but on this GPU it converts
+// both of them at every instruction: 17 instructions and 30 cycles of an SM
+// quarter for one m16n8k32, where two f16 ones take 16 cycles and q needs no
+// conversion at all; 64 x 4096 took 103 us with them, 101 with f16, ragged
+// lengths 38 and 34.)
 //   K: lane (g = lane / 4, c = lane % 4) takes bytes [16 c, 16 c + 16) of both
 //      64-byte halves of tokens g and g + 8.  The contraction may take the
-//      dims in any order as long as q uses the same one, so words 2i, 2i + 1
-//      of a piece are the eight k-values a lane holds of an MMA step.
+//      dims in any order as long as q uses the same one, so each word of a
+//      piece is the four k-values a lane holds of an MMA step.
 //   V: the lane takes bytes [16 g, 16 g + 16) of tokens 2c, 2c + 1, 2c + 8,
-//      2c + 9 of each block -- the tokens whose weights S leaves in this lane, four k-values
-//      of the second product -- and transposes 4 x 4 bytes.
-// The block scales stay out of the operands: K's multiplies the logits, V's
-// is part of z = s + log2 v, which has maxima of its own next to the one of
-// the softmax sum.
+//      2c + 9 of each block -- the tokens whose weights S leaves in this lane --
+//      and interleaves the bytes of two tokens.
+// q is scaled by a power of two per head into f16's range: exact but for
+// elements 2^29 times smaller than the head's largest.  K's scale multiplies
+// the logits.  V's is part of the weights 2^(x - mv) v, which have a running
+// maximum mv of their own next to the one of the softmax sum, so that f16
+// holds them (2^-11 of each) whatever the ratio of the blocks' scales.
 //
-// Loads: cp.async into two blocks' worth of shared memory per warp, K and V in
-// turn: as soon as a warp has K of its blocks in registers the next K is under
-// way, and the same for V, without barriers between warps.  Block ids and
-// scales come 32 blocks at a time, one per lane.
+// Loads: cp.async into three slots per warp, each K or V of two blocks, in the
+// order of their use: one is read while two are under way, without barriers
+// between warps.  Block ids and scales come 32 blocks at a time, one per lane.
 //
 // Work split: the blocks of all (sequence, KV head) pairs, laid end to end
 // with PAIR_COST blocks' worth for the fixed cost of a pair, are cut into
@@ -456,8 +451,7 @@ namespace dec8 {
 constexpr int D = kvq::D, BS = kvq::BS, WARPS = 4, THREADS = 32 * WARPS, CTAS_PER_SM = 4;
 constexpr int MIN_UNITS = 4 * WARPS;    // a CTA takes at least this many blocks' worth
 constexpr int PAIR_COST = 4 * WARPS;    // measured on ragged lengths: 49 us with 8, 43 with 16 and with 24
-constexpr float WEIGHT_BITS = 8.f;      // the largest weight of 32 tokens is 2^8
-constexpr float RESCALE = 8.f;          // O is rescaled once the maximum has grown by this much
+constexpr float RESCALE = 8.f;          // O is rescaled once mv has grown by this much: weights stay under 2^9
 constexpr int SLOT = 2 * BS * D;        // K (or V) of two blocks
 constexpr int SLOTS = 3;                // per warp: one in use, two on their way
 constexpr int RING = WARPS * SLOTS * SLOT;
@@ -472,10 +466,10 @@ struct Smem {                           // rings, later the warps' O | their (m,
 };
 }  // namespace dec8
 
-__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -491,19 +485,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// two fp32 of at most 448 as the sums of two e4m3 each: pairs of bytes hi and lo
-__device__ __forceinline__ void split_e4m3x2(float a, float b, uint16_t& hi, uint16_t& lo) {
-  asm("{\n\t.reg .b32 w, r;\n\t"
-      "cvt.rn.f16x2.f32 w, %3, %2;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f16x2 %0, w;\n\t"
-      "cvt.rn.f16x2.e4m3x2 r, %0;\n\t"
-      "sub.rn.f16x2 r, w, r;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f16x2 %1, r;\n\t}"
-      : "=&h"(hi), "=h"(lo)
-      : "f"(a), "f"(b));
-}
-__device__ __forceinline__ uint32_t pair16(uint16_t lo, uint16_t hi) { return (uint32_t)lo | (uint32_t)hi << 16; }
-
 // NT: tiles of 8 query heads per KV head (1: groups up to 8, 2: up to 16).
 template <int NT>
 __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
@@ -650,7 +631,7 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
       vs0 = __shfl_sync(0xffffffffu, lvs, at);
       vs1 = __shfl_sync(0xffffffffu, lvs, at + 1);
     };
-    // ---- q fragments: step i covers words 2 (i % 2), 2 (i % 2) + 1 of the pieces i / 2; warp i makes it
+    // ---- q fragments: two words' dims of the pieces at a time; warp i makes [.][i]
     float qf[NT];
     u128 raw[NT][4];
 #pragma unroll
@@ -674,26 +655,16 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
           am = fmaxf(am, fmaxf(finite_or_zero(bf16_lo(word(raw[nt][i], e))), finite_or_zero(bf16_hi(word(raw[nt][i], e)))));
       am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
       am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
-      const int eq = min(max((int)(__float_as_uint(am) >> 23) - 127 - 8 + ((__float_as_uint(am) & 0x7fffffu) > 0x600000u), -126), 126);
+      // am * 2^-eq in [2^14, 2^15)
+      const int eq = am > 0.f ? max((int)(__float_as_uint(am) >> 23) - 127 - 14, -126) : 0;
       const float down = exp2_int(-eq);
       qf[nt] = exp2_int(eq) * scale_log2;
-      static_assert(WARPS == 4, "a warp per step");
+      static_assert(WARPS == 4, "a warp per two words");
       const u128 mine = warp == 0 ? raw[nt][0] : warp == 1 ? raw[nt][1] : warp == 2 ? raw[nt][2] : raw[nt][3];
-      uint32_t part4[4];
+      uint32_t f[4];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {                            // four dims: words 2e, 2e + 1 of the bf16 piece
-        float f[4] = {bf16_lo(word(mine, 2 * e)), bf16_hi(word(mine, 2 * e)), bf16_lo(word(mine, 2 * e + 1)),
-                      bf16_hi(word(mine, 2 * e + 1))};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) f[k] = scaled_or_nan(f[k], down);
-        uint16_t h0, h1, l0, l1;
-        split_e4m3x2(f[0], f[1], h0, l0);
-        split_e4m3x2(f[2], f[3], h1, l1);
-        part4[2 * e] = pair16(h0, h1);
-        part4[2 * e + 1] = pair16(l0, l1);
-      }
-      // (larger, rest) of words 2e and 2e + 1
-      sq[(nt * 4 + warp) * 32 + lane] = make_uint4(part4[0], part4[1], part4[2], part4[3]);
+      for (int e = 0; e < 4; ++e) f[e] = pack_f16x2(bf16_lo(word(mine, e)) * down, bf16_hi(word(mine, e)) * down);
+      sq[(nt * 4 + warp) * 32 + lane] = make_uint4(f[0], f[1], f[2], f[3]);
     }
     __syncthreads();
 
@@ -712,49 +683,47 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
     for (int j = j0 + 2 * warp; j < j1; j += 2 * WARPS) {
       cp_async_wait<2>();                                      // K of these blocks
       __syncwarp();                                            // of every lane
-      float x[NT][8];                                          // logits: 4 of each block
+      float s[2][2][4];                                        // [block][tokens 0-7, 8-15]
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float ks = i ? ks1 : ks0;
-        if (ks < 0.f) {
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+        for (int e = 0; e < 4; ++e) s[i][0][e] = s[i][1][e] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[nt][4 * i + e] = -INFINITY;
-          continue;
-        }
-        u128 kr[4];
+      for (int p = 0; p < 2; ++p) {                            // pieces: 64 dims each
+        u128 kr[2][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) kr[e] = lds16(s0 + kget + (e & 1) * khalf + i * (BS * D) + (e >> 1) * 8 * D);
-        float s[2][4];                                         // tokens 0-7, 8-15 of the block
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.f;
+          for (int tt = 0; tt < 2; ++tt) kr[i][tt] = lds16(s0 + kget + p * khalf + i * (BS * D) + tt * 8 * D);
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
+        for (int w2 = 0; w2 < 2; ++w2) {                       // two words
           uint4 qa[NT];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) qa[nt] = sq[(nt * 4 + st) * 32 + lane];
+          for (int nt = 0; nt < NT; ++nt) qa[nt] = sq[(nt * 4 + 2 * p + w2) * 32 + lane];
 #pragma unroll
-          for (int tt = 0; tt < 2; ++tt) {
-            const uint32_t b0 = word(kr[2 * tt + (st >> 1)], 2 * (st & 1)), b1 = word(kr[2 * tt + (st >> 1)], 2 * (st & 1) + 1);
-            if (NT == 1) {                                     // rows 0-7 the larger parts, rows 8-15 the rest
-              mma_e4m3(s[tt], qa[0].x, qa[0].y, qa[0].z, qa[0].w, b0, b1);
-            } else {                                           // rows: 16 heads; the parts one after the other
-              mma_e4m3(s[tt], qa[0].x, qa[NT - 1].x, qa[0].z, qa[NT - 1].z, b0, b1);
-              mma_e4m3(s[tt], qa[0].y, qa[NT - 1].y, qa[0].w, qa[NT - 1].w, b0, b1);
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+              const uint32_t wa = word(kr[i][tt], 2 * w2), wb = word(kr[i][tt], 2 * w2 + 1);
+              mma_f16(s[i][tt], qa[0].x, NT == 2 ? qa[NT - 1].x : 0u, qa[0].y, NT == 2 ? qa[NT - 1].y : 0u,
+                      e4m3x2_to_f16x2((uint16_t)wa), e4m3x2_to_f16x2((uint16_t)(wa >> 16)));
+              mma_f16(s[i][tt], qa[0].z, NT == 2 ? qa[NT - 1].z : 0u, qa[0].w, NT == 2 ? qa[NT - 1].w : 0u,
+                      e4m3x2_to_f16x2((uint16_t)wb), e4m3x2_to_f16x2((uint16_t)(wb >> 16)));
             }
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float f = qf[nt] * ks;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[nt][4 * i + e] = (NT == 1 ? s[e >> 1][e & 1] + s[e >> 1][2 + (e & 1)] : s[e >> 1][2 * nt + (e & 1)]) * f;
         }
       }
       __syncwarp();                                            // K has been read by all
       fetch_v(s0);                                             // of the next blocks
+      float x[NT][8];                                          // logits: 4 of each block
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float f0 = qf[nt] * ks0, f1 = qf[nt] * ks1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[nt][e] = ks0 < 0.f ? -INFINITY : s[0][e >> 1][2 * nt + (e & 1)] * f0;   // below 0: no block
+          x[nt][4 + e] = ks1 < 0.f ? -INFINITY : s[1][e >> 1][2 * nt + (e & 1)] * f1;
+        }
+      }
       const int tok0 = j * BS + 2 * qd;                        // this lane's tokens: + {0, 1, 8, 9} of each block
       const bool tail = (j + 2) * BS > len;
       if (tail) {
@@ -766,8 +735,8 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
       }
       const float e0 = (float)((int)(__float_as_uint(vs0) >> 23) - 127);
       const float e1 = (float)((int)(__float_as_uint(vs1) >> 23) - 127);
-      uint32_t wh[NT][2], wl[NT][2];                           // weights' two parts: B fragments of the second product
-      float alpha[NT], beta[NT];
+      uint32_t wb[NT][4];                                      // weights: B fragments of the second product
+      float alpha[NT];
       bool grow = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -778,30 +747,23 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
         a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, 2));
         a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, 2));
         const float m_new = fmaxf(m[nt], fmaxf(a0, a1)), base = m_new == -INFINITY ? 0.f : m_new;
-        float ls = 0.f;
+        float p[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ls += ex2(x[nt][e] - base);
-        l[nt] = l[nt] * ex2(m[nt] - base) + ls;
+        for (int e = 0; e < 8; ++e) p[e] = ex2(x[nt][e] - base);
+        l[nt] = l[nt] * ex2(m[nt] - base) + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
         m[nt] = m_new;
-        const float mt = fmaxf(a0 + e0, a1 + e1);              // of z = x + log2 of V's scale
+        const float mt = fmaxf(a0 + e0, a1 + e1);              // of x + log2 of V's scale
         alpha[nt] = 1.f;
         if (mt > mv[nt] + RESCALE || mv[nt] == -INFINITY) {
           alpha[nt] = mt == -INFINITY ? 1.f : ex2(mv[nt] - mt);
           mv[nt] = mt;
           grow = true;
         }
-        const float tb = mt == -INFINITY ? 0.f : mt;
-        beta[nt] = mt == -INFINITY ? 0.f : ex2(mt - WEIGHT_BITS - mv[nt]);
-        const float z0 = e0 - tb + WEIGHT_BITS, z1 = e1 - tb + WEIGHT_BITS;
-        uint16_t hi[4], lo[4];
+        // p 2^(e + m - mv); the bound keeps blocks whose scales are 2^126 apart finite
+        const float vb = base - (mv[nt] == -INFINITY ? 0.f : mv[nt]);
+        const float c0 = ex2(fminf(e0 + vb, 126.f)), c1 = ex2(fminf(e1 + vb, 126.f));
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          split_e4m3x2(ex2(x[nt][2 * e] + (e < 2 ? z0 : z1)), ex2(x[nt][2 * e + 1] + (e < 2 ? z0 : z1)), hi[e], lo[e]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          wh[nt][i] = pair16(hi[2 * i], hi[2 * i + 1]);
-          wl[nt][i] = pair16(lo[2 * i], lo[2 * i + 1]);
-        }
+        for (int i = 0; i < 4; ++i) wb[nt][i] = pack_f16x2(p[2 * i] * (i < 2 ? c0 : c1), p[2 * i + 1] * (i < 2 ? c0 : c1));
       }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -815,12 +777,6 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
             o[nt][mt][3] *= a1;
           }
         }
-      }
-      float bc[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        bc[nt][0] = __shfl_sync(0xffffffffu, beta[nt], 8 * qd);
-        bc[nt][1] = __shfl_sync(0xffffffffu, beta[nt], 8 * qd + 4);
       }
       cp_async_wait<2>();                                      // V of these blocks
       __syncwarp();
@@ -838,28 +794,20 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
         }
 #pragma unroll
         for (int w = 0; w < 2; ++w) {                          // 4 dims: two tiles
-          uint32_t r[2][4];                                    // [block][dim]: four tokens' bytes
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint32_t t0 = w ? vr[4 * i].y : vr[4 * i].x, t1 = w ? vr[4 * i + 1].y : vr[4 * i + 1].x,
                            t2 = w ? vr[4 * i + 2].y : vr[4 * i + 2].x, t3 = w ? vr[4 * i + 3].y : vr[4 * i + 3].x;
-            const uint32_t p0 = __byte_perm(t0, t1, 0x5140), p1 = __byte_perm(t2, t3, 0x5140);
-            const uint32_t p2 = __byte_perm(t0, t1, 0x7362), p3 = __byte_perm(t2, t3, 0x7362);
-            r[i][0] = __byte_perm(p0, p1, 0x5410);
-            r[i][1] = __byte_perm(p0, p1, 0x7632);
-            r[i][2] = __byte_perm(p2, p3, 0x5410);
-            r[i][3] = __byte_perm(p2, p3, 0x7632);
-          }
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf)
+            for (int hf = 0; hf < 2; ++hf) {                   // bytes of two tokens side by side: dims 2 hf, 2 hf + 1
+              const uint32_t y = __byte_perm(t0, t1, hf ? 0x7362 : 0x5140), z = __byte_perm(t2, t3, hf ? 0x7362 : 0x5140);
+              const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)y), a1 = e4m3x2_to_f16x2((uint16_t)(y >> 16));
+              const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)z), a3 = e4m3x2_to_f16x2((uint16_t)(z >> 16));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float t[4] = {0.f, 0.f, 0.f, 0.f};
-              mma_e4m3(t, r[0][2 * hf], r[0][2 * hf + 1], r[1][2 * hf], r[1][2 * hf + 1], wh[nt][0], wh[nt][1]);
-              mma_e4m3(t, r[0][2 * hf], r[0][2 * hf + 1], r[1][2 * hf], r[1][2 * hf + 1], wl[nt][0], wl[nt][1]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[nt][4 * w2 + 2 * w + hf][e] += t[e] * bc[nt][e & 1];
+              for (int nt = 0; nt < NT; ++nt)
+                mma_f16(o[nt][4 * w2 + 2 * w + hf], a0, a1, a2, a3, wb[nt][2 * i], wb[nt][2 * i + 1]);
             }
+          }
         }
       }
       __syncwarp();                                            // V has been read by all

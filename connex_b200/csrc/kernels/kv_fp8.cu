@@ -449,8 +449,8 @@ void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_s
 // merges them (a counter that wraps to zero by itself).
 namespace dec8 {
 constexpr int D = kvq::D, BS = kvq::BS, WARPS = 4, THREADS = 32 * WARPS, CTAS_PER_SM = 4;
-constexpr int MIN_UNITS = 4 * WARPS;    // a CTA takes at least this many blocks' worth
-constexpr int PAIR_COST = 4 * WARPS;    // measured on ragged lengths: 49 us with 8, 43 with 16 and with 24
+constexpr int MIN_UNITS = 2 * WARPS;    // a CTA takes at least this many blocks' worth (500 tokens alone: 6.6 us; 7.5 with twice as many)
+constexpr int PAIR_COST = 4 * WARPS;    // measured on ragged lengths: 41 us with 8, 34 with 16 and with 32
 constexpr float RESCALE = 8.f;          // O is rescaled once mv has grown by this much: weights stay under 2^9
 constexpr int SLOT = 2 * BS * D;        // K (or V) of two blocks
 constexpr int SLOTS = 3;                // per warp: one in use, two on their way

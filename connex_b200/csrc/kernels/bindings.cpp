@@ -227,6 +227,10 @@ void check_same_device(const at::Tensor& a, std::initializer_list<const at::Tens
     TORCH_CHECK(t->device() == a.device(), what, ": every tensor must be on ", a.device());
 }
 
+void check_status_device(const at::Tensor& a, const c10::optional<at::Tensor>& status, const char* what) {
+  if (status.has_value()) check_same_device(a, {&*status}, what);
+}
+
 // rows of 16-byte vectors: [rows, cols] bf16 with contiguous rows
 int row_ld16(const at::Tensor& t, const char* what) {
   TORCH_CHECK(t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && t.scalar_type() == at::kBFloat16, what,
@@ -260,6 +264,7 @@ void rope_cache_fp8(const at::Tensor& qkv, const at::Tensor& pos, const at::Tens
                     at::Tensor& out, int64_t Hq, int64_t Hkv, const c10::optional<at::Tensor>& status,
                     const c10::optional<at::Tensor>& q_norm, const c10::optional<at::Tensor>& k_norm, double eps) {
   check_same_device(qkv, {&pos, &cos_sin, &slots, &kc, &out}, "rope_cache_fp8");
+  check_status_device(qkv, status, "rope_cache_fp8");
   const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "rope_cache_fp8");
   const int ldq = row_ld16(qkv, "rope_cache_fp8: qkv"), ldo = row_ld16(out, "rope_cache_fp8: out");
   const int64_t T = qkv.size(0);
@@ -309,6 +314,7 @@ void decode_attention_fp8(const at::Tensor& q, const at::Tensor& kc, const at::T
                           at::Tensor& out, int64_t Hq, double scale, at::Tensor& ws,
                           const c10::optional<at::Tensor>& status) {
   check_same_device(q, {&kc, &block_tables, &ctx_lens, &out, &ws}, "decode_attention_fp8");
+  check_status_device(q, status, "decode_attention_fp8");
   const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "decode_attention_fp8");
   const int ldq = row_ld16(q, "decode_attention_fp8: q"), ldo = row_ld16(out, "decode_attention_fp8: out");
   const int64_t B = q.size(0);
@@ -342,6 +348,7 @@ void kv_copy_blocks(at::Tensor& kv, const at::Tensor& pairs, const c10::optional
   TORCH_CHECK(kv.dim() == 6 && kv.size(1) == 2 && kv.is_contiguous(),
               "kv_copy_blocks: kv must be contiguous [layers, 2, blocks, Hkv, tokens, head_dim]");
   check_same_device(kv, {&pairs}, "kv_copy_blocks");
+  check_status_device(kv, status, "kv_copy_blocks");
   TORCH_CHECK(pairs.scalar_type() == at::kInt && pairs.dim() == 2 && pairs.size(1) == 2 && pairs.is_contiguous(),
               "kv_copy_blocks: pairs must be contiguous int32 [n, 2] (source, destination)");
   const int64_t n = pairs.size(0), block = kv.size(3) * kv.size(4) * kv.size(5) * kv.element_size();
@@ -375,6 +382,7 @@ void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, cons
                                  at::Tensor& vw, at::Tensor& table, at::Tensor& tiles,
                                  const c10::optional<at::Tensor>& status) {
   check_same_device(q, {&kc, &block_tables, &out, &tile_info, &kw, &vw, &table, &tiles}, "prefill_attention_paged_fp8");
+  check_status_device(q, status, "prefill_attention_paged_fp8");
   const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "prefill_attention_paged_fp8");
   const int ldq = row_ld16(q, "prefill_attention_paged_fp8: q"), ldo = row_ld16(out, "prefill_attention_paged_fp8: out");
   const int64_t T = q.size(0);

@@ -14,7 +14,8 @@ Storage layout, chosen for the kernels rather than for checkpoint parity:
   contiguous 4 KB slice, the unit the PD push kernel moves.  With
   ``dtype=torch.float8_e4m3fn`` it holds 8-bit values and one power-of-two
   scale per (block, KV head); attention then reads K and V from the cache in
-  prefill steps too, so a prompt gives the same rows however it is chunked.
+  prefill steps too, so a prompt split at block boundaries attends to the same
+  keys and values as a whole one.
 
 The forward passes launch only this package's kernels (tcgen05 GEMM,
 RMSNorm, RoPE + cache write, attention, argmax); a per-layer hook lets the
@@ -299,6 +300,8 @@ class PagedKVCache:
             raise ValueError(f"fork: {n_tokens} tokens do not lie in {len(blocks)} blocks")
         if n < 0:
             raise ValueError("fork: n must not be negative")
+        if any(not 0 <= b < self.num_blocks for b in blocks[:self.blocks_needed(n_tokens)]):
+            raise ValueError(f"fork: block ids must lie in [0, {self.num_blocks})")
         tails = self.allocate(n) if rest else []
         self.copy_blocks([(blocks[full], t) for t in tails])
         if n:

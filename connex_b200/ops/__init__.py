@@ -306,11 +306,13 @@ def decode_workspace_fp8(batch: int, n_q_heads: int, n_kv_heads: int, device) ->
     zero before its first use, and left ready for the next call.  Calls that
     may run at the same time (on different streams, or graphs replayed side
     by side) each need their own."""
-    device = torch.device(device)
-    index = device.index if device.index is not None else torch.cuda.current_device()
     if n_kv_heads <= 0 or n_q_heads <= 0 or n_q_heads % n_kv_heads:
         raise ValueError("decode_workspace_fp8: the query heads must be a multiple of the KV heads")
     g = n_q_heads // n_kv_heads
+    if g > 16:
+        raise ValueError("decode_workspace_fp8: at most 16 query heads per KV head")
+    device = torch.device(device)
+    index = device.index if device.index is not None else torch.cuda.current_device()
     return torch.zeros(_C.decode_fp8_rows(index, batch, n_kv_heads, g), g * _C.DECODE_FP8_ROW, dtype=torch.float32,
                        device=device)
 

@@ -120,6 +120,12 @@ def test_cache_refusals():
     with pytest.raises(ValueError, match="fork"):
         c.fork(t, 5, -1)
     c.allocate(21)
+    free = c.free_blocks
+    with pytest.raises(ValueError, match="block ids"):
+        c.fork([t[0], 24], 20, 1)
+    with pytest.raises(ValueError, match="block ids"):
+        c.fork([-1, t[0]], 20, 1)
+    assert c.free_blocks == free
     shared = dict(c._shared)
     with pytest.raises(MemoryError):
         c.fork(t, 20, 2)
@@ -242,6 +248,8 @@ def test_more_refusals():
         _decode({**_args(hq=34), "q": torch.zeros(2, 34 * D, dtype=torch.bfloat16)}, hq=34)
     with pytest.raises(ValueError, match="multiple of the KV heads"):
         ops.decode_workspace_fp8(4, 10, 4, "cuda:0")
+    with pytest.raises(ValueError, match="16 query heads"):
+        ops.decode_workspace_fp8(4, 34, 2, "cuda:0")
     kv = torch.zeros(2, 2, 5, 2, BS, D, dtype=torch.bfloat16)
     pairs = torch.zeros(1, 2, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="contiguous"):
@@ -254,6 +262,13 @@ def test_more_refusals():
         ops.kv_copy_blocks(kv.to(torch.float8_e4m3fn), pairs, torch.ones(2, 2, 5, 3))
     with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
         ops.kv_copy_blocks(kv, pairs)
+    # a status word of another device would be a bad address for the kernel
+    elsewhere = torch.zeros(1, dtype=torch.int32, device="meta")
+    for call in (_write, _decode, _prefill):
+        with pytest.raises(RuntimeError, match="every tensor must be on"):
+            call(a, status=elsewhere)
+    with pytest.raises(RuntimeError, match="every tensor must be on"):
+        ops.kv_copy_blocks(kv, pairs, status=elsewhere)
 
 
 def test_layerwise_transfer_refuses_an_8_bit_cache():

@@ -446,11 +446,16 @@ void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_s
 // equal shares, one per CTA, from the lengths themselves -- the same launch (a
 // graph replay) is balanced for any lengths.  A pair that spans several CTAs
 // leaves partial results in the workspace, and the CTA that arrives last
-// merges them (a counter that wraps to zero by itself).
+// merges them (a counter that wraps to zero by itself).  Where no pair is
+// longer than two shares, cuts move by up to SLACK blocks' worth to the pair's
+// start or end: a part more costs a CTA more than that (64 x 128 tokens 7.7 us,
+// 14.3 with the cuts where they fall; 64 x 500 15.2 and 19.5; with twice the
+// slack 100 x 2048 takes 84, not 80; ragged lengths gain nothing).
 namespace dec8 {
 constexpr int D = kvq::D, BS = kvq::BS, WARPS = 4, THREADS = 32 * WARPS, CTAS_PER_SM = 4;
 constexpr int MIN_UNITS = 2 * WARPS;    // a CTA takes at least this many blocks' worth (500 tokens alone: 6.6 us; 7.5 with twice as many)
 constexpr int PAIR_COST = 4 * WARPS;    // measured on ragged lengths: 41 us with 8, 34 with 16 and with 32
+constexpr int SLACK = 2 * PAIR_COST;    // see the work split above
 constexpr float RESCALE = 8.f;          // O is rescaled once mv has grown by this much: weights stay under 2^9
 constexpr int SLOT = 2 * BS * D;        // K (or V) of two blocks
 constexpr int SLOTS = 3;                // per warp: one in use, two on their way
@@ -498,7 +503,8 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
   float* sm = reinterpret_cast<float*>(smem + Smem<NT>::STATS);         // [WARPS][8 NT][m, l, mv]
   uint4* sq = reinterpret_cast<uint4*>(smem + Smem<NT>::Q);             // [NT][4 steps][32 lanes]
   int* pre = reinterpret_cast<int*>(smem + Smem<NT>::PRE);              // [B + 1] units of the pairs before sequence b
-  __shared__ int wsum[WARPS];
+  __shared__ int wsum[WARPS], wtop[WARPS];
+  __shared__ int2 share[2];
   __shared__ uint32_t ticket;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gq = lane >> 2, qd = lane & 3;
@@ -507,7 +513,7 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
   auto len_of = [&](int b) { return min(max(ctx_lens[b], 0), max_blocks * BS); };
   // ---- prefix sums of the pairs' units
   if (tid == 0) pre[0] = 0;
-  int run = 0;
+  int run = 0, top = 0;                                         // all units; the longest sequence's
   for (int b0 = 0; b0 < B; b0 += THREADS) {
     const int b = b0 + tid;
     int n = 0;
@@ -522,13 +528,18 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    if (lane == 31) wsum[warp] = x;
+    const int longest = __reduce_max_sync(0xffffffffu, n);
+    if (lane == 31) {
+      wsum[warp] = x;
+      wtop[warp] = longest;
+    }
     __syncthreads();
     int add = run;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       if (w < warp) add += wsum[w];
       run += wsum[w];
+      top = max(top, wtop[w]);
     }
     if (b < B) pre[b + 1] = add + x;
     __syncthreads();
@@ -540,17 +551,27 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
       for (int i = tid; i < Hq * D / 8; i += THREADS) st_v4(out + (size_t)b * ldo + 8 * i, u128{0, 0, 0, 0});
   const int n_cta = max(1, min((int)gridDim.x, (total + MIN_UNITS - 1) / MIN_UNITS));
   const int per = (total + n_cta - 1) / n_cta;
-  const int u0 = min(total, (int)blockIdx.x * per), u1 = min(total, u0 + per);
-  int b = 0;
-  {  // the sequence that holds u0: the last b with pre[b] <= u0
-    int lo = 0, hi = B;
+  // blocks' worth by which a cut moves to the start or the end of the pair it falls into
+  const int most = top <= 2 * per * Hkv ? SLACK : 0;
+  auto slack_of = [&](int units) { return min((units - PAIR_COST) / 2, most); };
+  const int x = (blockIdx.x + (tid & 1)) * per;          // thread 0 finds the share's start, thread 1 its end
+  int lo = 0, end = total;
+  if (x < total) {
+    int hi = B;                                         // the sequence that holds x: the last b with pre[b] <= x
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (pre[mid] <= u0) lo = mid;
+      if (pre[mid] <= x) lo = mid;
       else hi = mid;
     }
-    b = lo;
+    const int units = (pre[lo + 1] - pre[lo]) / Hkv, into = (x - pre[lo]) % units, slack = slack_of(units);
+    end = into <= PAIR_COST + slack ? x - into : units - into <= slack ? x - into + units : x;
   }
+  // (through shared memory, not shuffles: the compiler then knows that they are the same in all
+  // lanes; 64 x 4096 took 115 us otherwise)
+  if (tid < 2) share[tid] = make_int2(end, lo);
+  __syncthreads();
+  const int u0 = share[0].x, u1 = share[1].x;
+  int b = share[0].y;
   // Both land row by row, 512 contiguous bytes per instruction (measured: with
   // every lane fetching the pieces it reads back, K in 64-byte halves and V
   // in every other row, the loads alone took 122 us of 64 x 4096 where these
@@ -836,8 +857,8 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
           so[(warp * 8 * NT + nt * 8 + 2 * qd + (e & 1)) * O_ROW + (2 * (mt ^ 4 * vhalf) + (e >> 1)) * 8 + gq] = o[nt][mt][e];
     }
     __syncthreads();
-    // the CTAs that share the pair; the first may start inside the pair's fixed cost
-    const int c0 = (pair0 + PAIR_COST) / per, c1 = (pair0 + units - 1) / per;
+    // the CTAs that share the pair: those of the cuts left inside it, and the one before
+    const int slack = slack_of(units), c0 = (pair0 + PAIR_COST + slack) / per, c1 = (pair0 + units - slack - 1) / per;
     // two heads at a time, a thread for two dims of one
     for (int hh = tid >> 6; hh < G; hh += 2) {
       const int d16 = tid & 7, d2 = tid >> 3 & 7, dim = d16 * 16 + 2 * d2;
@@ -860,19 +881,19 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
         num.y += p[8] * f;
         den += st[w].y * ex2(st[w].x - mb);
       }
-      if (c0 == c1) {
+      if (c0 >= c1) {
         const float inv = den == 0.f ? 0.f : ex2(vb - mb) / den;
         *reinterpret_cast<uint32_t*>(out + (size_t)b * ldo + (size_t)(h * G + hh) * D + dim) =
             pack_bf16x2(num.x * inv, num.y * inv);
-      } else {   // a CTA's first pair goes to its slot 0, its last to slot 1
-        float* p = part + ((size_t)(blockIdx.x * 2 + (pair0 <= u0 ? 0 : 1)) * G + hh) * DEC8_ROW;
+      } else {   // slot 1 for the pair that goes on in the next CTA, 0 for one that began before
+        float* p = part + ((size_t)(blockIdx.x * 2 + ((int)blockIdx.x == c0)) * G + hh) * DEC8_ROW;
         *reinterpret_cast<float2*>(p + dim) = num;
         if ((tid & 63) == 0) {
           *reinterpret_cast<float4*>(p + D) = make_float4(M, den, MV, 0.f);
         }
       }
     }
-    if (c0 != c1) {
+    if (c0 < c1) {
       __threadfence();
       __syncthreads();
       if (tid == 0) ticket = atomicInc(&counters[b * Hkv + h], (uint32_t)(c1 - c0));
@@ -882,7 +903,7 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
         // a warp per head: lanes over the CTAs for the statistics, over the dims for the sums
         for (int hh = warp; hh < G; hh += WARPS) {
           auto slot = [&](int cc) {
-            return part + ((size_t)(cc * 2 + (pair0 <= cc * per ? 0 : 1)) * G + hh) * DEC8_ROW;
+            return part + ((size_t)(cc * 2 + (cc == c0)) * G + hh) * DEC8_ROW;
           };
           float m_all = -INFINITY, mv_all = -INFINITY, den = 0.f;
           float4 num = make_float4(0.f, 0.f, 0.f, 0.f);

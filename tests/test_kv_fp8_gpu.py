@@ -76,7 +76,8 @@ def _attention_tolerance(ref, mag, q, k_cache, k_scale, table, ctx, n_new, u_wei
     return U_BF16 * ref.abs() + mag * (2 * u_weight + 4 * logit + n * U_F32 + 2.0 ** -20) + n * 2.0 ** -25 * vmax
 
 
-DECODE_LENS = [[1], [0, 5, 0], [16], [17, 1, 15, 16, 31, 33], [500], [4096, 3, 0, 1000], [129] * 70, [20000, 1]]
+DECODE_LENS = [[1], [0, 5, 0], [16], [17, 1, 15, 16, 31, 33], [500], [4096, 3, 0, 1000], [129] * 70, [20000, 1],
+               [128] * 64, [1500] * 40 + [0, 1480]]
 
 
 @pytest.mark.parametrize("heads", [(32, 8), (8, 8), (6, 2), (7, 1), (16, 1), (20, 2), (32, 4)])

@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(fatc::THREADS, 2)
                            const __grid_constant__ CUtensorMap tmv, __nv_bfloat16* __restrict__ out, int ldo,
                            const int* __restrict__ tile_info, int n_tiles, int Hq, int Hkv, float scale_log2,
                            const int* __restrict__ block_tables, int bt_stride, int* status,
-                           unsigned long long* /*prof: two-tile kernel only*/) {
+                           unsigned long long* /*prof: two-tile kernel only*/, AttnPlan /*the same*/) {
   using namespace fatc;
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {  // swizzled operands need a 1 KB-aligned base
@@ -454,6 +454,11 @@ __global__ void __launch_bounds__(fatc::THREADS, 2)
 // done, its first scores are computed while the softmax warps still store
 // the previous item's O, and the next P.V (which overwrites O_X) waits for
 // P_X(0) -- which that warpgroup writes only after its epilogue read O_X.
+// SPLIT: the CTAs' work comes from a plan (AttnPlan): equal shares of the
+// items' key tiles laid end to end, so an item may be cut into pieces of
+// consecutive CTAs.  A piece leaves its unnormalised O, running maxima and
+// sums in the workspace; the warpgroup that arrives last for a tile adds them
+// up in the pieces' order.
 // Warps: 0 TMA producer, 1 MMA issuer (2, 3 idle: warpgroup granularity of
 // the register split), 4-7 softmax of tile 0, 8-11 of tile 1 (warp w reaches
 // tensor-memory lanes 32 (w % 4) .. + 31).
@@ -491,6 +496,8 @@ static_assert(SMEM <= 227 * 1024, "shared memory");
 struct Item {
   int seq_start, seq_len, q0, ctx, total, h, g, nkv;
   int nt[2];          // key tiles that Q tile X takes part in (0: the tile lies past the sequence end)
+  int j0;             // first key tile (SPLIT: of the piece, and nkv, nt count from it)
+  int all[2];         // SPLIT: nt of the whole item
   const int* bt;      // paged: the sequence's block table
 };
 template <bool PAGED>
@@ -513,6 +520,7 @@ __device__ __forceinline__ Item item_of(int w, const int* __restrict__ tile_info
     it.nt[x] = r0 < it.seq_len ? (min(it.total, it.ctx + r0 + BM) + BN - 1) / BN : 0;
   }
   it.nkv = max(it.nt[0], it.nt[1]);
+  it.j0 = 0;
   return it;
 }
 // Item of round k for CTA b of G: rounds alternate direction (0..G-1, then
@@ -521,13 +529,13 @@ __device__ __forceinline__ Item item_of(int w, const int* __restrict__ tile_info
 __device__ __forceinline__ int item_at(int k, int b, int G) { return k * G + ((k & 1) ? G - 1 - b : b); }
 }  // namespace fap
 
-template <bool PAGED, int EMU, bool PROF>
+template <bool PAGED, int EMU, bool PROF, bool SPLIT>
 __global__ void __maxnreg__(fap::LAUNCH_REGS)
     prefill_attn_pair_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                              const __grid_constant__ CUtensorMap tmv, __nv_bfloat16* __restrict__ out, int ldo,
                              const int* __restrict__ tile_info, int n_tiles, int Hq, int Hkv, float scale_log2,
                              const int* __restrict__ block_tables, int bt_stride, int* status,
-                             unsigned long long* prof) {
+                             unsigned long long* prof, AttnPlan plan) {
   using namespace fap;
   if constexpr (!PROF) prof = nullptr;   // counters compiled out
   using fatc::RESCALE_THRESHOLD;
@@ -548,8 +556,6 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
   uint64_t* o_full = bars + 16;   // [tile]  O_X of the item final
   uint64_t* drain = bars + 18;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
-  const int n_items = n_tiles * Hq;
-
   const int warp = warp_id(), lane = lane_id();
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < 2; ++s) {
@@ -579,6 +585,37 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const int n_items = SPLIT ? n_tiles * (Hq / plan.team) : n_tiles * Hq;
+  // the CTA's k-th item (n_items: no more)
+  int2 cut0 = make_int2(0, 0), cut1 = cut0;
+  int team = 0, member = 0;
+  if constexpr (SPLIT) {
+    team = blockIdx.x / plan.team;
+    member = blockIdx.x - team * plan.team;
+    cut0 = plan.cuts[team];
+    cut1 = plan.cuts[team + 1];
+  }
+  auto item_no = [&](int k) -> int {
+    if constexpr (SPLIT) {
+      const int w = cut0.x + k;
+      return w < cut1.x || (w == cut1.x && cut1.y > (k == 0 ? cut0.y : 0)) ? w : n_items;
+    } else {
+      return item_at(k, blockIdx.x, gridDim.x);
+    }
+  };
+  auto item = [&](int w, int k) -> Item {
+    Item it = item_of<PAGED>(SPLIT ? w * plan.team + member : w, tile_info, n_tiles, Hq, Hkv, block_tables, bt_stride);
+    if constexpr (SPLIT) {
+      it.j0 = k == 0 ? cut0.y : 0;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        it.all[x] = it.nt[x];
+        it.nt[x] = max(0, (w == cut1.x ? min(it.nt[x], cut1.y) : it.nt[x]) - it.j0);
+      }
+      it.nkv = max(it.nt[0], it.nt[1]);
+    }
+    return it;
+  };
 
   if (warp < 4) {
     // producer and MMA warps need few registers: hand them to the softmax
@@ -596,9 +633,8 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
         };
         uint32_t kv = 0;   // key tiles loaded so far: ring position of the item's tile 0
         uint32_t nq[2] = {0u, 0u}, nk[2] = {0u, 0u}, nv[2] = {0u, 0u};   // loads issued per barrier
-        for (int n_it = 0, w = item_at(0, blockIdx.x, gridDim.x); w < n_items && good;
-             ++n_it, w = item_at(n_it, blockIdx.x, gridDim.x)) {
-          const Item it = item_of<PAGED>(w, tile_info, n_tiles, Hq, Hkv, block_tables, bt_stride);
+        for (int n_it = 0, w = item_no(0); w < n_items && good; ++n_it, w = item_no(n_it)) {
+          const Item it = item(w, n_it);
           const int qcol = it.h * D, kcol = (Hq + it.g) * D, vcol = (Hq + Hkv + it.g) * D;
   #pragma unroll
           for (int x = 0; x < 2; ++x) {   // rows past the tensor end are zero-filled, past the sequence unused
@@ -616,7 +652,7 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
           auto rows_of = [&](int j, int (&r)[BPT]) {
   #pragma unroll
             for (int i = 0; i < BPT; ++i) {
-              const int b = j * BPT + i;
+              const int b = (it.j0 + j) * BPT + i;
               r[i] = (it.bt[b < nblk ? b : 0] * Hkv + it.g) * 16;  // past the end: any valid block (masked)
             }
           };
@@ -709,9 +745,8 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
                          fatc::umma_desc_sw128_mn(sV + kk * 2048, HALF_KV), IDESC_PV, (!first || kk > 0) ? 1u : 0u);
           }
         };
-        for (int n_it = 0, w = item_at(0, blockIdx.x, gridDim.x); w < n_items && ok;
-             ++n_it, w = item_at(n_it, blockIdx.x, gridDim.x)) {
-          const Item it = item_of<PAGED>(w, tile_info, n_tiles, Hq, Hkv, block_tables, bt_stride);
+        for (int n_it = 0, w = item_no(0); w < n_items && ok; ++n_it, w = item_no(n_it)) {
+          const Item it = item(w, n_it);
           for (int x = 0; x < 2 && ok; ++x) ok = mwait(0, &q_full[x], n_it & 1);
           if (!ok) break;
           if (!mwait(1, &k_full[kv & 1], (kv >> 1) & 1)) { ok = false; break; }
@@ -774,9 +809,8 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
     bool ok = true;
     const bool rec = prof != nullptr && q == 0 && lane == 0;   // profiling: waits / softmax / epilogue cycles
     long long t_s = 0, t_c = 0, t_e = 0, t_o = 0, t_mark = 0;
-    for (int k = 0, w = item_at(0, blockIdx.x, gridDim.x); w < n_items && ok;
-         ++k, w = item_at(k, blockIdx.x, gridDim.x)) {
-      const Item it = item_of<PAGED>(w, tile_info, n_tiles, Hq, Hkv, block_tables, bt_stride);
+    for (int k = 0, w = item_no(0); w < n_items && ok; ++k, w = item_no(k)) {
+      const Item it = item(w, k);
       const int r0 = it.q0 + x * BM;      // first query of the tile
       const int qpos = it.ctx + r0 + row; // position in the sequence
       const int n = it.nt[x];
@@ -796,7 +830,7 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
         tmem_ld_wait();
-        const int key0 = j * BN;
+        const int key0 = (it.j0 + j) * BN;
         // only tiles that cross the diagonal or the sequence end pay for the
         // mask (one compare per score against the row's last valid key)
         const bool mask = (key0 + BN - 1 > it.ctx + r0) || (key0 + BN > it.total);
@@ -896,6 +930,104 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
         const float inv = l > 0.f ? 1.f / l : 0.f;
         const bool valid = r0 + row < it.seq_len;
         __nv_bfloat16* orow = out + (size_t)(it.seq_start + r0 + row) * ldo + (size_t)it.h * D;
+        if constexpr (SPLIT) {
+          // the teams whose CTAs have a piece of this tile
+          int c0 = team, c1 = team;
+          if (k == 0)
+            for (int2 c = cut0; c.x == w && c.y > 0; c = plan.cuts[c0]) --c0;
+          if (w == cut1.x)
+            for (int2 c = cut1; c.x == w && c.y > 0 && c.y < it.all[x]; c = plan.cuts[c1 + 1]) ++c1;
+          if (c0 != c1) {
+            auto tile_sync = [&] {                   // of the tile's warpgroup
+              if (x == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+              else asm volatile("bar.sync 2, 128;" ::: "memory");
+            };
+            // slot 1 for the item that goes on in the next CTA, 0 for one that began before
+            auto slot = [&](int c) {
+              return plan.part + (size_t)(2 * (c * plan.team + member) + (c == c0)) * AttnPlan::SLOT +
+                     x * (AttnPlan::SLOT / 2);
+            };
+            // whoever finds the others there adds up; the rest leave theirs: [32 quads of dims][128 rows][4],
+            // then the rows' maxima and sums
+            int* ticket = reinterpret_cast<int*>(bars + 20) + x;
+            int* arrived = &plan.arrived[2 * (c0 * plan.team + member) + x];
+            if (row == 0) *ticket = (int)ld_acquire_gpu_u32(reinterpret_cast<const uint32_t*>(arrived));
+            tile_sync();
+            bool last = *ticket == c1 - c0;
+            if (!last) {
+              float* mine = slot(team);
+#pragma unroll 1
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(tO + c * 32, o);
+                tmem_ld_wait();
+                if (valid)
+#pragma unroll
+                  for (int e = 0; e < 8; ++e)
+                    st_v4(mine + ((c * 8 + e) * BM + row) * 4, u128{o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]});
+              }
+              if (valid) {
+                mine[D * BM + row] = m;
+                mine[(D + 1) * BM + row] = l;
+              }
+              __threadfence();
+              tile_sync();
+              if (row == 0) *ticket = atomicAdd(arrived, 1);
+              tile_sync();
+              last = *ticket == c1 - c0;
+            }
+            if (last) {
+              __threadfence();
+              float M = m;
+#pragma unroll 4
+              for (int c = c0; c <= c1; ++c)
+                if (c != team) M = fmaxf(M, __ldcg(slot(c) + D * BM + row));
+              const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll 1
+              for (int half = 0; half < 2; ++half) {         // 64 dims at a time, in the pieces' order
+                float acc[64], L = 0.f;
+#pragma unroll
+                for (int e = 0; e < 64; ++e) acc[e] = 0.f;
+#pragma unroll 1
+                for (int c = c0; c <= c1; ++c) {
+                  uint32_t o[64];
+                  float mc = m, lc = l;
+                  if (c == team) {
+                    tmem_ld32(tO + half * 64, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+                    tmem_ld32(tO + half * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
+                    tmem_ld_wait();
+                  } else {
+                    const float* p = slot(c);
+                    mc = __ldcg(p + D * BM + row);
+                    lc = __ldcg(p + (D + 1) * BM + row);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                      *reinterpret_cast<uint4*>(&o[4 * e]) =
+                          __ldcg(reinterpret_cast<const uint4*>(p) + (half * 16 + e) * BM + row);
+                  }
+                  const float f = fatc::fast_exp2(mc - base);
+                  L += f * lc;
+#pragma unroll
+                  for (int e = 0; e < 64; ++e) acc[e] += f * __uint_as_float(o[e]);
+                }
+                const float norm = L > 0.f ? 1.f / L : 0.f;
+                if (valid)
+#pragma unroll
+                  for (int v = 0; v < 8; ++v) {
+                    u128 wv;
+                    wv.x = pack_bf16x2(acc[8 * v + 0] * norm, acc[8 * v + 1] * norm);
+                    wv.y = pack_bf16x2(acc[8 * v + 2] * norm, acc[8 * v + 3] * norm);
+                    wv.z = pack_bf16x2(acc[8 * v + 4] * norm, acc[8 * v + 5] * norm);
+                    wv.w = pack_bf16x2(acc[8 * v + 6] * norm, acc[8 * v + 7] * norm);
+                    st_v4(orow + half * 64 + v * 8, wv);
+                  }
+              }
+            }
+            tc_fence_before();                       // as below
+            kv += it.nkv;
+            continue;
+          }
+        }
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -952,17 +1084,18 @@ struct AttnArgs {
   const int* bt;
   int bt_stride;
   int* status;
+  AttnPlan plan{};
 };
 
 // PAIR: the two-tile kernel (256 query rows per CTA, one CTA per SM);
 // otherwise the one-tile kernel (128 rows, two CTAs per SM).  PROF: the
 // two-tile kernel with its cycle counters.
-template <bool PAIR, bool PAGED, int EMU, bool PROF = false>
+template <bool PAIR, bool PAGED, int EMU, bool PROF = false, bool SPLIT = false>
 static void launch_attn(const AttnArgs& a, cudaStream_t s) {
   static bool attr[64] = {false};
   int dev;
   cudaGetDevice(&dev);
-  auto* kern = PAIR ? prefill_attn_pair_kernel<PAGED, EMU, PROF> : prefill_attn_tc_kernel<PAGED, EMU>;
+  auto* kern = PAIR ? prefill_attn_pair_kernel<PAGED, EMU, PROF, SPLIT> : prefill_attn_tc_kernel<PAGED, EMU>;
   const int smem = PAIR ? fap::SMEM : fatc::SMEM;
   if (!attr[dev & 63]) {
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -972,11 +1105,11 @@ static void launch_attn(const AttnArgs& a, cudaStream_t s) {
   if (PAIR) {   // persistent: one CTA per SM over all (tile, head) items
     static int sms[64] = {0};
     if (sms[dev & 63] == 0) cudaDeviceGetAttribute(&sms[dev & 63], cudaDevAttrMultiProcessorCount, dev);
-    grid = dim3(min(a.n_tiles * a.Hq, sms[dev & 63]), 1);
+    grid = dim3(SPLIT ? a.plan.n_cta : min(a.n_tiles * a.Hq, sms[dev & 63]), 1);
   }
   kern<<<grid, PAIR ? fap::THREADS : fatc::THREADS, smem, s>>>(
       a.tq, a.tk, a.tv, reinterpret_cast<__nv_bfloat16*>(a.out), a.ldo, a.tile_info, a.n_tiles, a.Hq, a.Hkv,
-      a.scale_log2, a.bt, a.bt_stride, a.status, PAIR ? g_attn_prof : nullptr);
+      a.scale_log2, a.bt, a.bt_stride, a.status, PAIR ? g_attn_prof : nullptr, a.plan);
 }
 
 template <bool PAIR, bool PAGED>
@@ -1019,7 +1152,7 @@ void prefill_attention_tc(const void* qkv, int ldq, int qkv_cols, int T, void* o
 void prefill_attention_paged_tc(const void* qkv, int ldq, int qkv_cols, int T, const void* kc, const void* vc,
                                 int64_t cache_rows, const int* block_tables, int bt_stride, void* out, int ldo,
                                 const int* tile_info, int n_tiles, int Hq, int Hkv, float scale, int* status,
-                                cudaStream_t s, int tile_rows) {
+                                cudaStream_t s, int tile_rows, const AttnPlan* plan) {
   if (n_tiles == 0) return;
   AttnArgs a;
   a.tq = make_tmap_bf16_2d(qkv, (uint64_t)qkv_cols, (uint64_t)T, (uint64_t)ldq * 2, 64, 128, true);
@@ -1036,7 +1169,10 @@ void prefill_attention_paged_tc(const void* qkv, int ldq, int qkv_cols, int T, c
   a.bt = block_tables;
   a.bt_stride = bt_stride;
   a.status = status;
-  if (tile_rows == fap::ROWS)
+  if (plan != nullptr) {
+    a.plan = *plan;
+    launch_attn<true, true, 0, false, true>(a, s);
+  } else if (tile_rows == fap::ROWS)
     launch_attn_split<true, true>(a, s);
   else
     launch_attn_split<false, true>(a, s);

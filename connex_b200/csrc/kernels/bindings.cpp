@@ -374,14 +374,20 @@ void kv_copy_blocks(at::Tensor& kv, const at::Tensor& pairs, const c10::optional
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
+// Workspace of prefill_attention_paged_fp8 besides the blocks: int32 words and fp32 words.
+std::tuple<int64_t, int64_t> prefill_fp8_words(int64_t device, int64_t entries, int64_t n_tiles) {
+  const int64_t ctas = at::cuda::getDeviceProperties(device)->multiProcessorCount;
+  return {2 * (n_tiles + 1) + 2 * (ctas + 1) + 2 * ctas + entries + 5 * n_tiles, 2 * ctas * cx::AttnPlan::SLOT};
+}
+
 // Two launches: the tables' blocks as bf16 into workspaces of the caller, the
 // paged prefill attention over them.
 void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
                                  const at::Tensor& vs, const at::Tensor& block_tables, at::Tensor& out,
-                                 const at::Tensor& tile_info, int64_t Hq, int64_t Hkv, double scale, at::Tensor& kw,
-                                 at::Tensor& vw, at::Tensor& table, at::Tensor& tiles,
+                                 const at::Tensor& tile_info, int64_t Hq, int64_t Hkv, double scale, at::Tensor& kv,
+                                 const c10::optional<at::Tensor>& ints, const c10::optional<at::Tensor>& part,
                                  const c10::optional<at::Tensor>& status) {
-  check_same_device(q, {&kc, &block_tables, &out, &tile_info, &kw, &vw, &table, &tiles}, "prefill_attention_paged_fp8");
+  check_same_device(q, {&kc, &block_tables, &out, &tile_info, &kv}, "prefill_attention_paged_fp8");
   check_status_device(q, status, "prefill_attention_paged_fp8");
   const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "prefill_attention_paged_fp8");
   const int ldq = row_ld16(q, "prefill_attention_paged_fp8: q"), ldo = row_ld16(out, "prefill_attention_paged_fp8: out");
@@ -391,29 +397,45 @@ void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, cons
   TORCH_CHECK(q.size(1) >= Hq * 128 && out.size(0) == T && out.size(1) == Hq * 128,
               "prefill_attention_paged_fp8: q must hold Hq heads of 128 per row and out be [T, Hq * 128]");
   TORCH_CHECK(tile_info.scalar_type() == at::kInt && tile_info.dim() == 2 && tile_info.size(1) == 5 &&
-                  tile_info.is_contiguous(),
+                  tile_info.is_contiguous() && (tile_info.size(0) + 1) * Hq <= INT_MAX,
               "prefill_attention_paged_fp8: tile_info must be contiguous int32 [n, 5]");
   TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
                   block_tables.numel() * Hkv * 16 <= INT_MAX && block_tables.size(0) <= 65535,
               "prefill_attention_paged_fp8: block_tables must be contiguous int32 [B, max_blocks]");
-  TORCH_CHECK(kw.numel() == block_tables.numel() * Hkv * 16 * 128 && vw.sizes() == kw.sizes() && kw.is_contiguous() &&
-                  vw.is_contiguous() && kw.scalar_type() == at::kBFloat16 && vw.scalar_type() == at::kBFloat16 &&
-                  table.scalar_type() == at::kInt && table.sizes() == block_tables.sizes() && table.is_contiguous() &&
-                  tiles.scalar_type() == at::kInt && tiles.sizes() == tile_info.sizes() && tiles.is_contiguous(),
-              "prefill_attention_paged_fp8: workspaces must be bf16 [B * max_blocks, Hkv, 16, 128] and int32 like the tables and tiles");
   CHECK_CUDA(q);
+  const int64_t entries = block_tables.numel(), n_tiles = tile_info.size(0);
+  const auto [n_ints, n_part] = prefill_fp8_words(q.device().index(), entries, n_tiles);
+  TORCH_CHECK(kv.numel() == 2 * entries * Hkv * 16 * 128 && kv.is_contiguous() && kv.scalar_type() == at::kBFloat16 &&
+                  ints.has_value() && ints->scalar_type() == at::kInt && ints->numel() == n_ints && ints->is_contiguous() &&
+                  part.has_value() && part->scalar_type() == at::kFloat && part->numel() == n_part && part->is_contiguous(),
+              "prefill_attention_paged_fp8: workspaces of other sizes");
+  check_same_device(q, {&*ints, &*part}, "prefill_attention_paged_fp8");
   const c10::cuda::CUDAGuard g(q.device());
-  TORCH_CHECK(T == 0 || tile_info.size(0) == 0 || block_tables.numel() > 0,
-              "prefill_attention_paged_fp8: no block table for the tiles");
-  if (T == 0 || tile_info.size(0) == 0) return;
+  TORCH_CHECK(T == 0 || n_tiles == 0 || entries > 0, "prefill_attention_paged_fp8: no block table for the tiles");
+  if (T == 0 || n_tiles == 0) return;
+  cx::KvChunks o;
+  o.k = kv.data_ptr();
+  o.v = static_cast<char*>(kv.data_ptr()) + kv.nbytes() / 2;
+  // query heads of a KV head run side by side, so that its keys come from L2 for all but one
+  // (2 x 256 rows at 32256: 263 us, 272 one by one); four at most, or the last team leaves
+  // SMs without work (8 query heads of one KV head, 2048 rows at 6144: 71 us, 79 with eight)
+  o.team = 1;
+  for (int t = 2; t <= 4; ++t)
+    if (Hq / Hkv % t == 0) o.team = t;
+  const int sms = sms_of(q);
+  o.n_cta = std::max(1, sms / o.team) * o.team;
+  o.before = reinterpret_cast<int64_t*>(ints->data_ptr<int>());      // the 8-byte words first
+  o.cuts = reinterpret_cast<int2*>(o.before + n_tiles + 1);
+  o.arrived = reinterpret_cast<int*>(o.cuts + sms + 1);
+  o.tables = o.arrived + 2 * sms;
+  o.tiles = o.tables + entries;
   cx::kv_dequant_blocks(c, block_tables.data_ptr<int>(), (int)block_tables.size(0), (int)block_tables.size(1),
-                        tile_info.data_ptr<int>(), (int)tile_info.size(0), (int)T, kw.data_ptr(), vw.data_ptr(),
-                        table.data_ptr<int>(), tiles.data_ptr<int>(), status_ptr(status), cur_stream(q));
+                        tile_info.data_ptr<int>(), (int)n_tiles, (int)T, (int)Hq, o, status_ptr(status), cur_stream(q));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  cx::prefill_attention_paged_tc(q.data_ptr(), ldq, (int)(Hq * 128), (int)T, kw.data_ptr(), vw.data_ptr(),
-                                 block_tables.numel() * Hkv * 16, table.data_ptr<int>(), (int)block_tables.size(1),
-                                 out.data_ptr(), ldo, tiles.data_ptr<int>(), (int)tiles.size(0), (int)Hq, (int)Hkv,
-                                 (float)scale, status_ptr(status), cur_stream(q), 256);
+  const cx::AttnPlan plan{o.cuts, part->data_ptr<float>(), o.arrived, o.n_cta, o.team};
+  cx::prefill_attention_paged_tc(q.data_ptr(), ldq, (int)(Hq * 128), (int)T, o.k, o.v, entries * Hkv * 16, o.tables,
+                                 (int)block_tables.size(1), out.data_ptr(), ldo, o.tiles, (int)n_tiles, (int)Hq,
+                                 (int)Hkv, (float)scale, status_ptr(status), cur_stream(q), 256, &plan);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -664,6 +686,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("DECODE_FP8_ROW") = cx::DEC8_ROW;
   m.def("decode_attention_fp8", &decode_attention_fp8);
   m.def("kv_copy_blocks", &kv_copy_blocks);
+  m.def("prefill_fp8_words", &prefill_fp8_words);
   m.def("prefill_attention_paged_fp8", &prefill_attention_paged_fp8);
   m.def("kv_push_layer", &kv_push_layer);
   m.def("gemm_splits", &gemm_splits);

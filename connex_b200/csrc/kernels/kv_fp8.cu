@@ -1067,54 +1067,122 @@ void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes
 // The blocks that the tiles of a chunked prefill read, as bf16 (exact: the
 // scales are powers of two), entry i of the tables in block i, and the tables
 // that find them there.  Bound by memory and short next to the attention that
-// follows: 10 of 226 us for 2048 rows at 6144.  (Converting inside the
+// follows: 12 of 211 us for 2048 rows at 6144.  (Converting inside the
 // attention kernel, by four more warps between the copies and the MMAs, took
-// 302 us: the thread that issues the MMAs is busy 83 % of its time, and a
-// converter on its SM quarter slows it.)
+// 302 us where two launches took 225: the thread that issues the MMAs is busy
+// 83 % of its time, and a converter on its SM quarter slows it.)
 // One CTA per entry: all heads of K, then of V, 16 bytes of a lane each.  The
-// first CTA also hands the tiles on, checked: the attention kernel takes them
-// as they are, so one that does not fit the rows or the tables is recorded and
-// replaced by a valid one (whose rows are then written twice, alike).
+// first CTA also hands on the tiles that fit the rows and the tables -- the
+// attention kernel takes them as they are -- and divides their work.
+//
+// The work: an item is a tile and a team's query heads, its length its key
+// tiles and ITEM_COST for its fixed cost.  The items, laid end to end, are cut
+// into equal shares, one per team; a cut within CUT_SLACK of an item's start
+// or end moves there.  Against one item per CTA at a time: 16 rows at 131056
+// 540 us, 1810 without; 256 rows at 7936 60 us, 131; 2048 rows at 6144 211 us,
+// 225; eight prompts of 2048, whose items balance by themselves, 304 and 292.
 namespace kvd {
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int ROWS = 256, KEYS = 128;                   // of a tile of the attention
+constexpr int ITEM_COST = 2;                            // 4 x 512 rows at 8192: 302 us, 311 with 1, 320 with 4
+constexpr int CUT_SLACK = 1;                            // 2048 rows at 6144: 210 us, 215 with 3
+constexpr int MIN_SHARE = 3;                            // less is all fixed cost: 131 rows at 2000 31 us, 34 with 4
 }
 __device__ __forceinline__ bool tile_fits(const int* ti, int T, int B, int width) {
   const int start = ti[0], n = ti[1], q0 = ti[2], ctx = ti[3], seq = ti[4];
   return seq >= 0 && seq < B && n > 0 && q0 >= 0 && q0 < n && ctx >= 0 && start >= 0 && (int64_t)start + n <= T &&
          (int64_t)ctx + n <= (int64_t)width * kvq::BS;
 }
+// key tiles of a tile that fits
+__device__ __forceinline__ int tile_keys(const int* ti) {
+  return (min(ti[3] + ti[1], ti[3] + ti[2] + kvd::ROWS) + kvd::KEYS - 1) / kvd::KEYS;
+}
+__device__ __forceinline__ void kv_prefill_plan(const int* __restrict__ tile_info, int n_tiles, int T, int B, int width,
+                                                int Hq, const KvChunks& o, int* status) {
+  using namespace kvd;
+  __shared__ int64_t wlen[WARPS];
+  __shared__ int wfit[WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t len = 0;                                      // of the tiles so far, for one head
+  int kept = 0;
+  for (int t0 = 0; t0 < n_tiles; t0 += THREADS) {
+    const int t = t0 + tid;
+    const int* ti = tile_info + 5 * (int64_t)t;
+    const bool fits = t < n_tiles && tile_fits(ti, T, B, width);
+    if (t < n_tiles && !fits) record_status(status, CX_ERR_BOUNDS);
+    const int64_t n = fits ? tile_keys(ti) + ITEM_COST : 0;
+    int64_t x = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    const uint32_t fit = __ballot_sync(0xffffffffu, fits);
+    if (lane == 31) {
+      wlen[warp] = x;
+      wfit[warp] = __popc(fit);
+    }
+    __syncthreads();
+    int64_t at = len + x - n;
+    int to = kept + __popc(fit & ((1u << lane) - 1));
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) {
+        at += wlen[w];
+        to += wfit[w];
+      }
+      len += wlen[w];
+      kept += wfit[w];
+    }
+    if (fits) {
+      for (int e = 0; e < 5; ++e) o.tiles[5 * (int64_t)to + e] = ti[e];
+      o.before[to] = at;
+    }
+    __syncthreads();
+  }
+  for (int i = tid; i < 2 * o.n_cta; i += THREADS) o.arrived[i] = 0;
+  const int teams = o.n_cta / o.team, each = Hq / o.team;    // items of a tile
+  const int64_t total = len * each, per = max((int64_t)MIN_SHARE, (total + teams - 1) / teams);
+  for (int i = tid; i <= teams; i += THREADS) {
+    const int64_t x = i * per;
+    int2 cut = make_int2(kept * each, 0);
+    if (x < total) {
+      int lo = 0, hi = kept;                            // the tile that holds x
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (o.before[mid] * each <= x) lo = mid;
+        else hi = mid;
+      }
+      const int n = tile_keys(o.tiles + 5 * (int64_t)lo) + ITEM_COST;
+      const int64_t in = x - o.before[lo] * each;
+      const int h = (int)(in / n), p = (int)(in - (int64_t)h * n);
+      const int slack = min((n - ITEM_COST) / 2, CUT_SLACK);
+      cut = p <= ITEM_COST + slack ? make_int2(lo * each + h, 0)
+            : n - p <= slack       ? make_int2(lo * each + h + 1, 0)
+                                   : make_int2(lo * each + h, p - ITEM_COST);
+    }
+    o.cuts[i] = cut;
+  }
+}
 __global__ void __launch_bounds__(kvd::THREADS)
     kv_dequant_kernel(KvFp8 c, const int* __restrict__ tables, int width, const int* __restrict__ tile_info, int n_tiles,
-                      int T, __nv_bfloat16* ko, __nv_bfloat16* vo, int* tables_out, int* tiles_out, int* status) {
+                      int T, int Hq, KvChunks out, int* status) {
   using namespace kvq;
   const int seq = blockIdx.y, tid = threadIdx.x, B = gridDim.y;
   const int64_t i = (int64_t)seq * width + blockIdx.x;
+  __nv_bfloat16 *ko = reinterpret_cast<__nv_bfloat16*>(out.k), *vo = reinterpret_cast<__nv_bfloat16*>(out.v);
   // tokens of the sequence: any of its tiles tells
   int total = 0;
   for (int t = tid; t < n_tiles; t += kvd::THREADS)
     if (tile_info[5 * t + 4] == seq && tile_fits(tile_info + 5 * t, T, B, width))
       total = max(total, tile_info[5 * t + 1] + tile_info[5 * t + 3]);
-  __shared__ int most, valid;
-  if (tid == 0) {
-    most = 0;
-    valid = 0x7fffffff;
-  }
+  __shared__ int most;
+  if (tid == 0) most = 0;
   __syncthreads();
   if (total > 0) atomicMax(&most, total);
-  if (blockIdx.x == 0 && seq == 0) {
-    for (int t = tid; t < n_tiles; t += kvd::THREADS)
-      if (tile_fits(tile_info + 5 * t, T, B, width)) atomicMin(&valid, t);
-    __syncthreads();
-    for (int t = tid; t < n_tiles; t += kvd::THREADS) {
-      const bool fits = tile_fits(tile_info + 5 * t, T, B, width);
-      if (!fits) record_status(status, CX_ERR_BOUNDS);
-      const int from = fits ? t : valid;
-      for (int e = 0; e < 5; ++e)
-        tiles_out[5 * t + e] = from < n_tiles ? tile_info[5 * from + e] : e == 1;   // none fits: one row, one key
-    }
-  }
+  if (blockIdx.x == 0 && seq == 0) kv_prefill_plan(tile_info, n_tiles, T, B, width, Hq, out, status);
   __syncthreads();
-  if (tid == 0) tables_out[i] = (int)i;
+  if (tid == 0) out.tables[i] = (int)i;
   if (blockIdx.x >= (most + BS - 1) / BS) return;       // behind the end: never read
   const int id = tables[i];
   const bool in = id >= 0 && id < c.num_blocks;
@@ -1146,12 +1214,9 @@ __global__ void __launch_bounds__(kvd::THREADS)
 }
 
 void kv_dequant_blocks(const KvFp8& c, const int* tables, int B, int width, const int* tile_info, int n_tiles, int T,
-                       void* kout, void* vout, int* tables_out, int* tiles_out, int* status, cudaStream_t s) {
+                       int Hq, const KvChunks& o, int* status, cudaStream_t s) {
   if (B == 0 || width == 0) return;
-  kv_dequant_kernel<<<dim3(width, B), kvd::THREADS, 0, s>>>(c, tables, width, tile_info, n_tiles, T,
-                                                            reinterpret_cast<__nv_bfloat16*>(kout),
-                                                            reinterpret_cast<__nv_bfloat16*>(vout), tables_out,
-                                                            tiles_out, status);
+  kv_dequant_kernel<<<dim3(width, B), kvd::THREADS, 0, s>>>(c, tables, width, tile_info, n_tiles, T, Hq, o, status);
 }
 
 }  // namespace cx

@@ -43,11 +43,21 @@ void decode_attention_fp8(const void* q, int ldq, const KvFp8& c, const int* blo
 void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes, int num_blocks, int64_t block_bytes,
                     int Hkv, int sms, int* status, cudaStream_t s);
 
+// What kv_dequant_blocks leaves for the attention over its blocks.
+struct KvChunks {
+  void* k;          // bf16 [B * width, Hkv, 16, 128]
+  void* v;
+  int* tables;      // [B, width]: entry i is block i
+  int* tiles;       // [n_tiles, 5]: the tiles that fit, in their order
+  int2* cuts;       // [n_cta / team + 1], see AttnPlan
+  int* arrived;     // [2 n_cta], zero
+  int64_t* before;  // [n_tiles + 1] scratch
+  int n_cta, team;
+};
 // The e4m3 blocks that the tiles (tile_info [n_tiles, 5] of the paged prefill)
-// read through tables [B, width], as bf16 blocks of kout / vout [B * width,
-// Hkv, 16, 128]: entry i in block i; tables_out[i] = i.  tiles_out: the tiles,
-// those that do not fit T rows and the tables replaced.
+// read through tables [B, width], as bf16 blocks: entry i in block i.  Tiles
+// that do not fit T rows and the tables are left out.
 void kv_dequant_blocks(const KvFp8& c, const int* tables, int B, int width, const int* tile_info, int n_tiles, int T,
-                       void* kout, void* vout, int* tables_out, int* tiles_out, int* status, cudaStream_t s);
+                       int Hq, const KvChunks& o, int* status, cudaStream_t s);
 
 }  // namespace cx

@@ -29,15 +29,29 @@ void attention_exp_split(int n);
 // attention's per-CTA cycle counters (0: off).
 void attention_profile(int64_t ptr);
 
+// Work of the two-tile prefill attention in equal shares (built on the device,
+// see kv_prefill_plan).  Teams of `team` CTAs, a divisor of Hq / Hkv, take that
+// many query heads of one KV head side by side: team i the items (tile, heads)
+// from (cuts[i].x, key tile cuts[i].y) up to where cuts[i + 1] begins.  part:
+// SLOT floats for each of a CTA's two pieces of cut items; arrived: 2 n_cta
+// counters, zero.
+struct AttnPlan {
+  static constexpr int SLOT = 2 * 130 * 128;   // two tiles: O and the rows' maxima and sums
+  const int2* cuts;
+  float* part;
+  int* arrived;
+  int n_cta, team;
+};
+
 // The same over a paged cache (chunked prefill): q rows from QKV; K/V of the
 // whole context from the caches [blocks, Hkv, 16, 128] (cache_rows =
 // blocks * Hkv * 16) through block_tables [B, bt_stride]; tile_info: [n_tiles,
 // 5] int32 of (seq start row, new tokens, first query, context length,
-// sequence index).
+// sequence index).  With a plan the work is divided by it (tile_rows 256).
 void prefill_attention_paged_tc(const void* qkv, int ldq, int qkv_cols, int T, const void* kc, const void* vc,
                                 int64_t cache_rows, const int* block_tables, int bt_stride, void* out, int ldo,
                                 const int* tile_info, int n_tiles, int Hq, int Hkv, float scale, int* status,
-                                cudaStream_t s, int tile_rows);
+                                cudaStream_t s, int tile_rows, const AttnPlan* plan = nullptr);
 
 // Paged decode attention.  q: [B, *] rows (ld ldq, q heads first).
 // Caches [blocks, Hkv, BS, 128]; block_tables [B, max_blocks]; ctx_lens [B].

@@ -348,16 +348,22 @@ def prefill_attention_paged_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache:
     ``tile_info`` from ``prefill_tile_info(n_new, device, ctx)``.  The blocks
     that the chunks read are turned into bf16 first (exact: the scales are
     powers of two), in a workspace of the tables' size, so the tables should
-    be no wider than the longest sequence.  Entries behind a sequence's end
+    be no wider than the longest sequence.  The work is divided on the device
+    in equal shares of the keys, so few rows over a long context use every SM
+    (another 39 MB of workspace).  Entries behind a sequence's end
     are not read.  A block id out of range reads as zeros, and a tile that
     does not fit ``q``'s rows or the tables is left out; both are recorded in
     ``status``."""
     if out is None:
         out = torch.empty(q.shape[0], n_q_heads * 128, dtype=q.dtype, device=q.device)
-    k = torch.empty(block_tables.numel(), n_kv_heads, 16, 128, dtype=torch.bfloat16, device=q.device)
+    kv = torch.empty(2, block_tables.numel(), n_kv_heads, 16, 128, dtype=torch.bfloat16, device=q.device)
+    ints = part = None
+    if q.is_cuda:
+        n_ints, n_part = _C.prefill_fp8_words(q.device.index, block_tables.numel(), tile_info.shape[0])
+        ints = torch.empty(n_ints, dtype=torch.int32, device=q.device)
+        part = torch.empty(n_part, dtype=torch.float32, device=q.device)
     _C.prefill_attention_paged_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tables, out, tile_info, n_q_heads,
-                                   n_kv_heads, scale if scale is not None else 1.0 / math.sqrt(128), k,
-                                   torch.empty_like(k), torch.empty_like(block_tables), torch.empty_like(tile_info),
+                                   n_kv_heads, scale if scale is not None else 1.0 / math.sqrt(128), kv, ints, part,
                                    status)
     _n(2)
     return out

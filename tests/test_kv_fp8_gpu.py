@@ -117,10 +117,10 @@ def test_decode_attention(dev, heads, lens):
 
 
 PREFILL_ROWS = [[(0, 100)], [(64, 128)], [(1000, 300), (17, 5)], [(2000, 1), (130, 513)], [(5, 64), (0, 200), (3999, 129)],
-                [(2048, 600)], [(7, 9), (0, 1), (15, 1), (16, 1)], [(300, 0), (41, 30)]]
+                [(2048, 600)], [(7, 9), (0, 1), (15, 1), (16, 1)], [(300, 0), (41, 30)], [(12000, 33), (500, 257)]]
 
 
-@pytest.mark.parametrize("heads", [(8, 2), (3, 3), (7, 1), (16, 1)])
+@pytest.mark.parametrize("heads", [(8, 2), (3, 3), (7, 1), (16, 1), (6, 2)])
 @pytest.mark.parametrize("rows", PREFILL_ROWS, ids=lambda v: "_".join(f"{c}+{n}" for c, n in v))
 def test_prefill_attention(dev, heads, rows):
     from connex_b200 import ops
@@ -144,6 +144,31 @@ def test_prefill_attention(dev, heads, rows):
     tol = _attention_tolerance(ref, mag, q.view(T, hq, D), k, ks, table, ctx, new, U_BF16, float(vs.max()) * 448)
     err = (out.view(T, hq, D).double() - ref).abs()
     assert (err <= tol).all(), float((err / tol).max())
+
+
+def test_prefill_replayed(dev):
+    """A captured call divides the work from what the tiles hold at its replay, and gives an eager call's bits."""
+    from connex_b200 import ops
+    hq, hkv = 8, 2
+    table, nb = _table([5000, 700], dev, 9)
+    table = table.clamp(min=0)
+    k, ks = _cache(nb, hkv, dev, 10)
+    v, vs = _cache(nb, hkv, dev, 11)
+    q = torch.randn(300, hq * D, generator=_g(dev, 12), device=dev).to(torch.bfloat16)
+    tiles = [ops.prefill_tile_info([200, 100], dev, ctx=c) for c in ([4800, 600], [3, 0], [100, 333])]
+    ti = tiles[0].clone()
+    call = lambda: ops.prefill_attention_paged_fp8(q, k, v, ks, vs, table, ti, hq, hkv)  # noqa: E731
+    call()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+    for t in tiles + tiles[:1]:
+        assert t.shape == ti.shape
+        ti.copy_(t)
+        g.replay()
+        got = out.clone()
+        g.replay()
+        assert torch.equal(out, got) and torch.equal(call(), got)
 
 
 def _write_case(dev, rows, hq, hkv, seed, norm=False, spread=3.0):

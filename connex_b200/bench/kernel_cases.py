@@ -10,7 +10,7 @@ capture of the case runs.
 
 Cases: gemm (8192^3), gemm_qkv (T=8192 Llama-3-8B QKV), gemm_silu (T=8192
 gate/up + SiLU-mul), attn (8 x 2048-token causal prefill, 32/8 heads),
-attn_paged (the paged variant: 8 chunks of 2048 queries over 2048 cached tokens), decode_attn (64 x 4096-token paged decode), kv_push (one layer of a 64k-token
+attn_paged (the paged variant: 8 chunks of 2048 queries over 2048 cached tokens), decode_attn (64 x 4096-token paged decode), attn_paged_fp8 and decode_attn_fp8 (the same over the 8-bit cache), kv_push (one layer of a 64k-token
 KV push, local), kv_push_nvlink (the same layer pushed from GPU 0 into GPU 1's
 memory over NVLink, one process, peer access; ``--ctas`` sets the grid,
 ``--pull`` runs the kernel on GPU 1 reading GPU 0's memory instead, ``--ce``
@@ -132,6 +132,39 @@ def case_decode_attn(dev, B=64, ctx=4096, hq=32, hkv=8):
     ws = ops.decode_workspace(B, hq, ctx, dev)
     out = torch.empty(B, hq * 128, dtype=torch.bfloat16, device=dev)
     return (lambda: ops.decode_attention(q, k, v, bt, cl, hq, ctx, ws, out)), {"bytes": 2 * k.numel() * 2}
+
+
+def _fp8_cache(dev, nb, hkv):
+    """K or V of an 8-bit cache with its scales."""
+    return (torch.randn(nb, hkv, 16, 128, device=dev) * 100).to(torch.float8_e4m3fn), \
+        torch.full((nb, hkv), 2.0 ** -7, device=dev)
+
+
+def case_attn_paged_fp8(dev, n_seq=8, ctx=2048, L=2048, hq=32, hkv=8):
+    """:func:`case_attn_paged` over an 8-bit cache."""
+    T, per = n_seq * L, (ctx + L) // 16
+    nb = n_seq * per
+    (k, ks), (v, vs) = _fp8_cache(dev, nb, hkv), _fp8_cache(dev, nb, hkv)
+    bt = torch.randperm(nb, device=dev).to(torch.int32).view(n_seq, per).contiguous()
+    q = (torch.randn(T, hq * 128, device=dev) * 0.5).bfloat16()
+    ti = ops.prefill_tile_info([L] * n_seq, dev, ctx=[ctx] * n_seq)
+    out = torch.empty(T, hq * 128, dtype=torch.bfloat16, device=dev)
+    st = ops.new_status(dev)
+    return (lambda: ops.prefill_attention_paged_fp8(q, k, v, ks, vs, bt, ti, hq, hkv, out, status=st)), {
+        "flops": n_seq * hq * 4 * 128 * (L * ctx + L * L / 2), "check": _status_check(st, "8-bit paged prefill attention")}
+
+
+def case_decode_attn_fp8(dev, B=64, ctx=4096, hq=32, hkv=8):
+    nb = B * ctx // 16
+    (k, ks), (v, vs) = _fp8_cache(dev, nb, hkv), _fp8_cache(dev, nb, hkv)
+    bt = torch.randperm(nb, device=dev).to(torch.int32).view(B, ctx // 16).contiguous()
+    cl = torch.full((B,), ctx, dtype=torch.int32, device=dev)
+    q = torch.randn(B, hq * 128, device=dev).bfloat16()
+    ws = ops.decode_workspace_fp8(B, hq, hkv, dev)
+    out = torch.empty(B, hq * 128, dtype=torch.bfloat16, device=dev)
+    st = ops.new_status(dev)
+    return (lambda: ops.decode_attention_fp8(q, k, v, ks, vs, bt, cl, hq, ws, out, status=st)), {
+        "bytes": 2 * k.numel() + 8 * ks.numel(), "check": _status_check(st, "8-bit decode attention")}
 
 
 def case_kv_push(dev, tokens=65536, hkv=8):
@@ -270,7 +303,7 @@ def case_gemm_m(dev, M=1, N=28672, K=4096, silu=False):
     return (lambda: ops.gemm(a, b, out, silu_mul=silu)), {"bytes": N * K * 2 + M * K * 2 + M * N * 2}
 
 
-def case_decode_step(dev, B=1, ctx=1024, graphs=True):
+def case_decode_step(dev, B=1, ctx=1024, graphs=True, kv_dtype=torch.bfloat16):
     """One Llama-3-8B decode step for B sequences of ``ctx`` cached tokens,
     replayed from its CUDA graph (device time of the whole step; bytes =
     weights + the KV read)."""
@@ -279,7 +312,7 @@ def case_decode_step(dev, B=1, ctx=1024, graphs=True):
     from connex_b200.runtime.pp import StageRuntime
     cfg = LlamaConfig.llama3_8b()
     rt = StageRuntime(cfg, 0, cfg.layers, dev, num_blocks=B * (ctx + 64) // 16 + 64, max_tokens=max(B * ctx, 8192),
-                      max_batch=B, max_ctx=ctx + 64)
+                      max_batch=B, max_ctx=ctx + 64, kv_dtype=kv_dtype)
     if graphs:
         rt.enable_decode_graphs()
     rids = [f"r{i}" for i in range(B)]
@@ -294,7 +327,7 @@ def case_decode_step(dev, B=1, ctx=1024, graphs=True):
         fn = lambda: rt.compute(step, [])          # noqa: E731 - the same step again, launched eagerly
     weights = sum(t.numel() * 2 for lw in rt.weights.layers for t in (lw.wqkv, lw.wo, lw.w13, lw.w2)) \
         + rt.weights.lm_head.numel() * 2
-    kv = B * (ctx + 1) * cfg.kv_bytes_per_token
+    kv = B * (ctx + 1) * cfg.kv_bytes_per_token * rt.cache.kv.element_size() // 2
     return fn, {"bytes": weights + kv}
 
 
@@ -308,13 +341,15 @@ CASES = {"gemm": lambda d: case_gemm(d), "gemm_qkv": lambda d: case_gemm(d, 8192
          "attn_2x8192_t256": lambda d: case_attn(d, n_seq=2, L=8192, tile=256),
          "attn_cudnn_2x8192": lambda d: case_attn_library(d, "cudnn", n_seq=2, L=8192), "attn_cudnn": lambda d: case_attn_library(d, "cudnn"),
          "attn_torch_flash": lambda d: case_attn_library(d, "flash"),
-         "decode_attn": case_decode_attn, "kv_push": case_kv_push, "wsync": case_wsync, "ep_gemm": case_ep_gemm,
+         "decode_attn": case_decode_attn, "decode_attn_fp8": case_decode_attn_fp8,
+         "attn_paged_fp8": case_attn_paged_fp8, "kv_push": case_kv_push, "wsync": case_wsync, "ep_gemm": case_ep_gemm,
          "ep_t128": lambda d: case_ep_gemm(d, 128),
          "gemm_m1_qkv": lambda d: case_gemm_m(d, 1, 6144, 4096), "gemm_m1_o": lambda d: case_gemm_m(d, 1, 4096, 4096),
          "gemm_m1_gateup": lambda d: case_gemm_m(d, 1, 28672, 4096, silu=True),
          "gemm_m1_down": lambda d: case_gemm_m(d, 1, 4096, 14336),
          "gemm_m32_gateup": lambda d: case_gemm_m(d, 32, 28672, 4096, silu=True),
          "decode_step_b1": lambda d: case_decode_step(d, 1), "decode_step_b32": lambda d: case_decode_step(d, 32),
+         "decode_step_b32_fp8": lambda d: case_decode_step(d, 32, kv_dtype=torch.float8_e4m3fn),
          "decode_step_b1_eager": lambda d: case_decode_step(d, 1, graphs=False)}
 NEEDS_ARGS = {"kv_push_nvlink": case_kv_push_nvlink}
 

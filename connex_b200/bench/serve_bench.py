@@ -87,6 +87,7 @@ def main(argv=None) -> int:
     ap.add_argument("--warmup-requests", type=int, default=3)
     ap.add_argument("--max-batch", type=int, default=64)
     ap.add_argument("--num-blocks", type=int, default=0)
+    ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "fp8"])
     ap.add_argument("--rule", action="store_true", help="CPU stand-in model (wiring check)")
     ap.add_argument("--no-graphs", action="store_true", help="eager decode steps (no CUDA graphs)")
     a = ap.parse_args(argv)
@@ -98,7 +99,7 @@ def main(argv=None) -> int:
                             max_ctx=a.prompt_len + a.max_tokens + 64, max_step_tokens=max(8192, a.prompt_len + 64),
                             num_stages=1, stage_starts=None, directory=None, data="link", store=None,
                             store_master=False, replica=0, advertise_host="127.0.0.1", recv_timeout_s=30.0,
-                            no_graphs=a.no_graphs, tp=1)
+                            no_graphs=a.no_graphs, tp=1, kv_dtype=a.kv_dtype)
     stepper, _ = build_stepper(ns)
     engine = GenerationEngine(stepper).start()
     server = Server(engine, "bench")

@@ -107,7 +107,7 @@ def build_stepper(a):
     if a.num_stages == 1:
         n = kv_blocks(a, cfg, 0, cfg.layers)
         return ModelStepper(cfg, dev, n, a.max_batch, a.max_ctx, a.max_step_tokens, a.checkpoint, a.seed,
-                            graphs=not a.no_graphs, kv_dtype=a.kv_dtype), None
+                            graphs=not a.no_graphs, kv_dtype=getattr(a, "kv_dtype", "bf16")), None
     from connex_b200.serve import pipeline
     ranges = pipeline.split_layers(cfg.layers, a.num_stages, a.stage_starts)
     if not a.directory:
@@ -116,7 +116,7 @@ def build_stepper(a):
     ep, client = pipeline.join(a.model_name or "connex-b200", 0, a.num_stages, a.replica, dev, a.directory, a.data,
                                a.store, a.store_master, a.advertise_host, a.recv_timeout_s)
     st = PipelineStepper(cfg, ranges[0][1], dev, ep, n, a.max_batch, a.max_ctx, a.max_step_tokens, a.checkpoint,
-                         a.seed, a.recv_timeout_s, graphs=not a.no_graphs, kv_dtype=a.kv_dtype)
+                         a.seed, a.recv_timeout_s, graphs=not a.no_graphs, kv_dtype=getattr(a, "kv_dtype", "bf16"))
     ep.warm_stage(1)
     ep.auto_warm = True
     ep.watchdog = pipeline.watchdog(ep, st.link, client, step_timeout=a.step_timeout_s)
@@ -168,7 +168,7 @@ def _tp_stepper(a, cfg):
     t = torch.tensor([blocks], device=dev)
     dist.all_reduce(t, op=dist.ReduceOp.MIN)              # every rank sizes its KV cache alike
     inner = ModelStepper(cfg, dev, int(t.item()), a.max_batch, a.max_ctx, a.max_step_tokens, a.checkpoint,
-                         a.seed, graphs=False, tp=TPGroup(rank, world), kv_dtype=a.kv_dtype)
+                         a.seed, graphs=False, tp=TPGroup(rank, world), kv_dtype=getattr(a, "kv_dtype", "bf16"))
     if rank == 0:
         return TPStepper(inner, cpu), ("tp", cpu)
     log.info("TP rank %d of %d following rank 0", rank, world)

@@ -24,6 +24,10 @@ namespace {
 
 cudaStream_t cur_stream(const at::Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
+// A number of a message.  (Not left to the message's stream: this library may carry a C++ runtime of
+// its own beside the one torch uses, and writing a number to a stream of the other ends the process.)
+std::string num(int64_t x) { return std::to_string(x); }
+
 int* status_ptr(const c10::optional<at::Tensor>& st) {
   if (!st.has_value()) return nullptr;
   TORCH_CHECK(st->scalar_type() == at::kInt && st->is_cuda(), "status must be an int32 CUDA tensor");
@@ -322,7 +326,7 @@ void decode_attention_fp8(const at::Tensor& q, const at::Tensor& kc, const at::T
               "decode_attention_fp8: the query heads must be a multiple of the KV heads, 16 of them per KV head at most");
   TORCH_CHECK(q.size(1) >= Hq * 128 && out.size(0) == B && out.size(1) == Hq * 128,
               "decode_attention_fp8: q must hold Hq heads of 128 per row and out be [B, Hq * 128]");
-  TORCH_CHECK(B <= cx::DEC8_MAX_BATCH, "decode_attention_fp8: at most ", cx::DEC8_MAX_BATCH, " sequences per call");
+  TORCH_CHECK(B <= cx::DEC8_MAX_BATCH, "decode_attention_fp8: at most ", num(cx::DEC8_MAX_BATCH), " sequences per call");
   TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
                   block_tables.size(0) == B,
               "decode_attention_fp8: block_tables must be contiguous int32 [B, max_blocks]");
@@ -334,7 +338,7 @@ void decode_attention_fp8(const at::Tensor& q, const at::Tensor& kc, const at::T
   CHECK_CUDA(q);
   TORCH_CHECK(ws.scalar_type() == at::kFloat && ws.is_contiguous() && ws.dim() == 2 && ws.size(1) == G * cx::DEC8_ROW &&
                   ws.size(0) >= cx::decode_fp8_rows(sms_of(q), (int)B, c.Hkv, (int)G),
-              "decode_attention_fp8: the workspace must come from decode_workspace_fp8 for these heads and at least ", B,
+              "decode_attention_fp8: the workspace must come from decode_workspace_fp8 for these heads and at least ", num(B),
               " sequences");
   const c10::cuda::CUDAGuard g(q.device());
   cx::decode_attention_fp8(q.data_ptr(), ldq, c, block_tables.data_ptr<int>(), (int)block_tables.size(1),
@@ -400,18 +404,22 @@ void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, cons
                   tile_info.is_contiguous() && (tile_info.size(0) + 1) * Hq <= INT_MAX,
               "prefill_attention_paged_fp8: tile_info must be contiguous int32 [n, 5]");
   TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
-                  block_tables.numel() * Hkv * 16 <= INT_MAX && block_tables.size(0) <= 65535,
-              "prefill_attention_paged_fp8: block_tables must be contiguous int32 [B, max_blocks]");
+                  block_tables.numel() <= INT_MAX && block_tables.size(0) <= cx::KVQ_MAX_CHUNKS,
+              "prefill_attention_paged_fp8: block_tables must be contiguous int32 [B, max_blocks], B up to ",
+              num(cx::KVQ_MAX_CHUNKS));
+  TORCH_CHECK(kv.dim() == 5 && kv.size(0) == 2 && kv.size(2) == Hkv && kv.size(3) == 16 && kv.size(4) == 128 &&
+                  kv.is_contiguous() && kv.scalar_type() == at::kBFloat16 && kv.size(1) * Hkv * 16 <= INT_MAX,
+              "prefill_attention_paged_fp8: the blocks' workspace must be contiguous bf16 [2, n_blocks, Hkv, 16, 128]");
   CHECK_CUDA(q);
   const int64_t entries = block_tables.numel(), n_tiles = tile_info.size(0);
   const auto [n_ints, n_part] = prefill_fp8_words(q.device().index(), entries, n_tiles);
-  TORCH_CHECK(kv.numel() == 2 * entries * Hkv * 16 * 128 && kv.is_contiguous() && kv.scalar_type() == at::kBFloat16 &&
-                  ints.has_value() && ints->scalar_type() == at::kInt && ints->numel() == n_ints && ints->is_contiguous() &&
+  TORCH_CHECK(ints.has_value() && ints->scalar_type() == at::kInt && ints->numel() == n_ints && ints->is_contiguous() &&
                   part.has_value() && part->scalar_type() == at::kFloat && part->numel() == n_part && part->is_contiguous(),
               "prefill_attention_paged_fp8: workspaces of other sizes");
   check_same_device(q, {&*ints, &*part}, "prefill_attention_paged_fp8");
   const c10::cuda::CUDAGuard g(q.device());
-  TORCH_CHECK(T == 0 || n_tiles == 0 || entries > 0, "prefill_attention_paged_fp8: no block table for the tiles");
+  TORCH_CHECK(T == 0 || n_tiles == 0 || (entries > 0 && kv.size(1) > 0),
+              "prefill_attention_paged_fp8: no block table for the tiles");
   if (T == 0 || n_tiles == 0) return;
   cx::KvChunks o;
   o.k = kv.data_ptr();
@@ -423,6 +431,7 @@ void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, cons
   for (int t = 2; t <= 4; ++t)
     if (Hq / Hkv % t == 0) o.team = t;
   const int sms = sms_of(q);
+  o.blocks = (int)kv.size(1);
   o.n_cta = std::max(1, sms / o.team) * o.team;
   o.before = reinterpret_cast<int64_t*>(ints->data_ptr<int>());      // the 8-byte words first
   o.cuts = reinterpret_cast<int2*>(o.before + n_tiles + 1);
@@ -433,7 +442,7 @@ void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, cons
                         tile_info.data_ptr<int>(), (int)n_tiles, (int)T, (int)Hq, o, status_ptr(status), cur_stream(q));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   const cx::AttnPlan plan{o.cuts, part->data_ptr<float>(), o.arrived, o.n_cta, o.team};
-  cx::prefill_attention_paged_tc(q.data_ptr(), ldq, (int)(Hq * 128), (int)T, o.k, o.v, entries * Hkv * 16, o.tables,
+  cx::prefill_attention_paged_tc(q.data_ptr(), ldq, (int)(Hq * 128), (int)T, o.k, o.v, kv.size(1) * Hkv * 16, o.tables,
                                  (int)block_tables.size(1), out.data_ptr(), ldo, o.tiles, (int)n_tiles, (int)Hq,
                                  (int)Hkv, (float)scale, status_ptr(status), cur_stream(q), 256, &plan);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
@@ -470,7 +479,7 @@ int64_t wsync(const at::Tensor& jobs_dev, const at::Tensor& jobs_cpu, int64_t ds
               std::vector<int64_t> flags, int64_t mc_base, int64_t mc_flag, int64_t max_ctas, int64_t scatter_bytes) {
   TORCH_CHECK(jobs_dev.is_cuda() && jobs_dev.scalar_type() == at::kLong && jobs_dev.is_contiguous() &&
                   jobs_dev.dim() == 2 && jobs_dev.size(1) == cx::WS_JOB_COLS,
-              "jobs_dev must be contiguous int64 CUDA [n, ", cx::WS_JOB_COLS, "]");
+              "jobs_dev must be contiguous int64 CUDA [n, ", num(cx::WS_JOB_COLS), "]");
   TORCH_CHECK(!jobs_cpu.is_cuda() && jobs_cpu.scalar_type() == at::kLong && jobs_cpu.is_contiguous() &&
                   jobs_cpu.sizes() == jobs_dev.sizes(),
               "jobs_cpu must be the contiguous host copy of jobs_dev");

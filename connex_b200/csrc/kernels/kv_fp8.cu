@@ -1065,13 +1065,13 @@ void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes
 
 // --------------------------------------------------------- dequantised blocks
 // The blocks that the tiles of a chunked prefill read, as bf16 (exact: the
-// scales are powers of two), entry i of the tables in block i, and the tables
-// that find them there.  Bound by memory and short next to the attention that
+// scales are powers of two), sequence after sequence, and the tables that find
+// them there.  Bound by memory and short next to the attention that
 // follows: 12 of 211 us for 2048 rows at 6144.  (Converting inside the
 // attention kernel, by four more warps between the copies and the MMAs, took
 // 302 us where two launches took 225: the thread that issues the MMAs is busy
 // 83 % of its time, and a converter on its SM quarter slows it.)
-// One CTA per entry: all heads of K, then of V, 16 bytes of a lane each.  The
+// One CTA per block: all heads of K, then of V, 16 bytes of a lane each.  The
 // first CTA also hands on the tiles that fit the rows and the tables -- the
 // attention kernel takes them as they are -- and divides their work.
 //
@@ -1165,28 +1165,62 @@ __device__ __forceinline__ void kv_prefill_plan(const int* __restrict__ tile_inf
   }
 }
 __global__ void __launch_bounds__(kvd::THREADS)
-    kv_dequant_kernel(KvFp8 c, const int* __restrict__ tables, int width, const int* __restrict__ tile_info, int n_tiles,
-                      int T, int Hq, KvChunks out, int* status) {
+    kv_dequant_kernel(KvFp8 c, const int* __restrict__ tables, int B, int width, const int* __restrict__ tile_info,
+                      int n_tiles, int T, int Hq, KvChunks out, int* status) {
   using namespace kvq;
-  const int seq = blockIdx.y, tid = threadIdx.x, B = gridDim.y;
-  const int64_t i = (int64_t)seq * width + blockIdx.x;
-  __nv_bfloat16 *ko = reinterpret_cast<__nv_bfloat16*>(out.k), *vo = reinterpret_cast<__nv_bfloat16*>(out.v);
-  // tokens of the sequence: any of its tiles tells
+  extern __shared__ int from[];                         // [B + 1]: blocks of the sequences before b
+  __shared__ int wsum[kvd::WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int b = tid; b <= B; b += kvd::THREADS) from[b] = 0;
+  __syncthreads();
+  // blocks of a sequence: any of its tiles tells
+  for (int t = tid; t < n_tiles; t += kvd::THREADS) {
+    const int* ti = tile_info + 5 * (int64_t)t;
+    if (tile_fits(ti, T, B, width)) atomicMax(&from[1 + ti[4]], (ti[1] + ti[3] + BS - 1) / BS);
+  }
+  __syncthreads();
   int total = 0;
-  for (int t = tid; t < n_tiles; t += kvd::THREADS)
-    if (tile_info[5 * t + 4] == seq && tile_fits(tile_info + 5 * t, T, B, width))
-      total = max(total, tile_info[5 * t + 1] + tile_info[5 * t + 3]);
-  __shared__ int most;
-  if (tid == 0) most = 0;
-  __syncthreads();
-  if (total > 0) atomicMax(&most, total);
-  if (blockIdx.x == 0 && seq == 0) kv_prefill_plan(tile_info, n_tiles, T, B, width, Hq, out, status);
-  __syncthreads();
-  if (tid == 0) out.tables[i] = (int)i;
-  if (blockIdx.x >= (most + BS - 1) / BS) return;       // behind the end: never read
-  const int id = tables[i];
+  for (int b0 = 0; b0 < B; b0 += kvd::THREADS) {
+    const int b = b0 + tid;
+    int x = b < B ? from[1 + b] : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 31) wsum[warp] = x;
+    __syncthreads();
+    int add = total;
+#pragma unroll
+    for (int w = 0; w < kvd::WARPS; ++w) {
+      if (w < warp) add += wsum[w];
+      total += wsum[w];
+    }
+    if (b < B) from[1 + b] = add + x;
+    __syncthreads();
+  }
+  auto entry = [&](int i) {                             // of the tables: the i-th that is read
+    int lo = 0, hi = B;                                 // the sequence: the last one with from[lo] <= i
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (from[mid] <= i) lo = mid;
+      else hi = mid;
+    }
+    return (int64_t)lo * width + i - from[lo];
+  };
+  if (blockIdx.x == 0) {
+    kv_prefill_plan(tile_info, n_tiles, T, B, width, Hq, out, status);
+    if (total > out.blocks && tid == 0) record_status(status, CX_ERR_BOUNDS);
+    for (int i = out.blocks + tid; i < total; i += kvd::THREADS) out.tables[entry(i)] = 0;   // no room: any block
+  }
+  const int i = blockIdx.x;
+  if (i >= min(total, out.blocks)) return;
+  const int64_t at = entry(i);
+  if (tid == 0) out.tables[at] = i;
+  const int id = tables[at];
   const bool in = id >= 0 && id < c.num_blocks;
   if (!in && tid == 0) record_status(status, CX_ERR_BOUNDS);
+  __nv_bfloat16 *ko = reinterpret_cast<__nv_bfloat16*>(out.k), *vo = reinterpret_cast<__nv_bfloat16*>(out.v);
   const int per = c.Hkv * (BS * D / 16);                // 16-byte pieces of K, and of V
 #pragma unroll 4
   for (int v = tid; v < 2 * per; v += kvd::THREADS) {
@@ -1216,7 +1250,8 @@ __global__ void __launch_bounds__(kvd::THREADS)
 void kv_dequant_blocks(const KvFp8& c, const int* tables, int B, int width, const int* tile_info, int n_tiles, int T,
                        int Hq, const KvChunks& o, int* status, cudaStream_t s) {
   if (B == 0 || width == 0) return;
-  kv_dequant_kernel<<<dim3(width, B), kvd::THREADS, 0, s>>>(c, tables, width, tile_info, n_tiles, T, Hq, o, status);
+  kv_dequant_kernel<<<std::max(1, o.blocks), kvd::THREADS, (B + 1) * sizeof(int), s>>>(c, tables, B, width, tile_info,
+                                                                                       n_tiles, T, Hq, o, status);
 }
 
 }  // namespace cx

@@ -43,11 +43,14 @@ void decode_attention_fp8(const void* q, int ldq, const KvFp8& c, const int* blo
 void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes, int num_blocks, int64_t block_bytes,
                     int Hkv, int sms, int* status, cudaStream_t s);
 
+constexpr int KVQ_MAX_CHUNKS = 8192;
+
 // What kv_dequant_blocks leaves for the attention over its blocks.
 struct KvChunks {
-  void* k;          // bf16 [B * width, Hkv, 16, 128]
+  void* k;          // bf16 [blocks, Hkv, 16, 128]
   void* v;
-  int* tables;      // [B, width]: entry i is block i
+  int blocks;       // room for this many
+  int* tables;      // [B, width]
   int* tiles;       // [n_tiles, 5]: the tiles that fit, in their order
   int2* cuts;       // [n_cta / team + 1], see AttnPlan
   int* arrived;     // [2 n_cta], zero
@@ -55,8 +58,9 @@ struct KvChunks {
   int n_cta, team;
 };
 // The e4m3 blocks that the tiles (tile_info [n_tiles, 5] of the paged prefill)
-// read through tables [B, width], as bf16 blocks: entry i in block i.  Tiles
-// that do not fit T rows and the tables are left out.
+// read through tables [B, width] (B <= KVQ_MAX_CHUNKS), as bf16 blocks, those
+// of one sequence behind those of another.  Tiles that do not fit T rows and
+// the tables are left out; more blocks than there is room for are recorded.
 void kv_dequant_blocks(const KvFp8& c, const int* tables, int B, int width, const int* tile_info, int n_tiles, int T,
                        int Hq, const KvChunks& o, int* status, cudaStream_t s);
 

@@ -407,14 +407,14 @@ class LlamaModel:
                                      workspace, out=out, status=self.status)
 
     def _chunk_attention(self, i: int, q: torch.Tensor, block_tables: torch.Tensor, tile_info: torch.Tensor,
-                         out: torch.Tensor) -> None:
+                         out: torch.Tensor, n_blocks: Optional[int] = None) -> None:
         cfg, c = self.cfg, self.cache
         if c.scales is None:
             ops.prefill_attention_paged(q, c.k(i), c.v(i), block_tables, tile_info, cfg.heads, cfg.kv_heads, out=out,
                                         status=self.status)
         else:
             ops.prefill_attention_paged_fp8(q, c.k(i), c.v(i), c.k_scale(i), c.v_scale(i), block_tables, tile_info,
-                                            cfg.heads, cfg.kv_heads, out=out, status=self.status)
+                                            cfg.heads, cfg.kv_heads, out=out, status=self.status, n_blocks=n_blocks)
 
     def decode_workspace(self, max_batch: int, max_ctx: int) -> torch.Tensor:
         """The decode attention's workspace for this model's cache."""

@@ -341,22 +341,24 @@ def prefill_attention_paged_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache:
                                 k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
                                 tile_info: torch.Tensor, n_q_heads: int, n_kv_heads: int,
                                 out: Optional[torch.Tensor] = None, scale: Optional[float] = None,
-                                status: Optional[torch.Tensor] = None) -> torch.Tensor:
+                                status: Optional[torch.Tensor] = None, n_blocks: Optional[int] = None) -> torch.Tensor:
     """:func:`prefill_attention_paged` over an 8-bit cache: causal attention of
     prompt chunks, ``q`` [T, >= Hq * 128] rotated (q heads first), keys and
     values of the whole context -- this chunk's included -- from the cache.
     ``tile_info`` from ``prefill_tile_info(n_new, device, ctx)``.  The blocks
     that the chunks read are turned into bf16 first (exact: the scales are
-    powers of two), in a workspace of the tables' size, so the tables should
-    be no wider than the longest sequence.  The work is divided on the device
+    powers of two), in a workspace of ``n_blocks`` blocks: a bound on those
+    of all the sequences together, by default the tables' size.  The work is divided on the device
     in equal shares of the keys, so few rows over a long context use every SM
     (another 39 MB of workspace).  Entries behind a sequence's end
     are not read.  A block id out of range reads as zeros, and a tile that
     does not fit ``q``'s rows or the tables is left out; both are recorded in
-    ``status``."""
+    ``status``, and so are more blocks than ``n_blocks`` (rows that need them
+    are then wrong)."""
     if out is None:
         out = torch.empty(q.shape[0], n_q_heads * 128, dtype=q.dtype, device=q.device)
-    kv = torch.empty(2, block_tables.numel(), n_kv_heads, 16, 128, dtype=torch.bfloat16, device=q.device)
+    n_blocks = block_tables.numel() if n_blocks is None else max(0, min(n_blocks, block_tables.numel()))
+    kv = torch.empty(2, n_blocks, n_kv_heads, 16, 128, dtype=torch.bfloat16, device=q.device)
     ints = part = None
     if q.is_cuda:
         n_ints, n_part = _C.prefill_fp8_words(q.device.index, block_tables.numel(), tile_info.shape[0])

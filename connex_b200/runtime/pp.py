@@ -95,7 +95,8 @@ class StageModel(LlamaModel):
         ops.rmsnorm(self.x[:T], self.w.layers[0].attn_norm, self.cfg.eps, out=self.h[:T])
 
     def run(self, inp: torch.Tensor, positions, slots, *, prefill: bool, tile_info=None, block_tables=None,
-            ctx_lens=None, max_ctx: int = 0, workspace=None, rows=None, B: int = 0, n_dec: Optional[int] = None):
+            ctx_lens=None, max_ctx: int = 0, workspace=None, rows=None, B: int = 0, n_dec: Optional[int] = None,
+            n_blocks: Optional[int] = None):
         """Ids (first stage) or the residual stream in; the residual stream
         (``x[:T]``) or, on the last stage, the greedy next ids of ``rows`` out.
 
@@ -103,7 +104,8 @@ class StageModel(LlamaModel):
         rows (paged decode attention over ``block_tables[:n_dec]`` /
         ``ctx_lens``), the rest are prefill chunks that continue cached
         sequences (the paged prefill kernel over ``block_tables[n_dec:]`` and
-        ``tile_info`` of width 5); every GEMM runs once over all rows."""
+        ``tile_info`` of width 5; ``n_blocks``: cache blocks that they read,
+        for an 8-bit cache); every GEMM runs once over all rows."""
         cfg, T = self.cfg, inp.shape[0]
         assert T <= self.max_tokens
         self._enter(inp, T)
@@ -116,7 +118,8 @@ class StageModel(LlamaModel):
                     self._decode_attention(i, q[:n_dec], block_tables[:n_dec], ctx_lens, max_ctx, workspace,
                                            self.attn[:n_dec])
                 if T > n_dec:
-                    self._chunk_attention(i, q[n_dec:], block_tables[n_dec:], tile_info, self.attn[n_dec:T])
+                    self._chunk_attention(i, q[n_dec:], block_tables[n_dec:], tile_info, self.attn[n_dec:T],
+                                          n_blocks)
             elif prefill:
                 ops.prefill_attention(qkv, tile_info, cfg.heads, cfg.kv_heads, out=self.attn[:T])
             else:
@@ -369,7 +372,8 @@ class StageRuntime:
             for i, r in enumerate(rids):
                 t = self.tables[r]
                 bt[i, :len(t)] = torch.tensor(t[:mb], dtype=torch.int32)
-            kw.update(n_dec=n_dec, block_tables=bt.pin_memory().to(dev, non_blocking=True),
+            kw.update(n_dec=n_dec, n_blocks=sum(-(-x // self.bs) for x in lens[n_dec:]),
+                      block_tables=bt.pin_memory().to(dev, non_blocking=True),
                       tile_info=ops.prefill_tile_info(n_new[n_dec:], dev, ctx=ctx[n_dec:]),
                       rows=torch.tensor(last_rows, dtype=torch.int32).pin_memory().to(dev, non_blocking=True))
             if n_dec:

@@ -293,3 +293,34 @@ def test_cli_kv_dtype(monkeypatch):
         torch_kv_dtype("int8")
     with pytest.raises(SystemExit):
         ap.parse_args(["--kv-dtype", "int8"])
+
+
+@pytest.mark.parametrize("given", [None, "fp8"])
+def test_stepper_from_the_command_line(monkeypatch, given):
+    """``--kv-dtype`` reaches the runtime; callers with options of their own that do not name it get bf16."""
+    from connex_b200.serve import __main__ as m, engine
+    ap = argparse.ArgumentParser()
+    m.model_args(ap)
+    a = ap.parse_args([] if given is None else ["--kv-dtype", given])
+    if given is None:
+        del a.kv_dtype
+    for k, v in dict(num_stages=1, num_blocks=64, device="cpu", no_graphs=True).items():
+        setattr(a, k, v)
+    seen = {}
+    monkeypatch.setattr(torch.cuda, "set_device", lambda d: None)
+    monkeypatch.setattr(engine, "ModelStepper", lambda *x, **kw: seen.update(kw))
+    m.build_stepper(a)
+    assert seen["kv_dtype"] == (given or "bf16")
+
+
+def test_refusals_that_name_a_number():
+    """Messages with numbers in them are exceptions like the others."""
+    a = _args(B=5000)
+    with pytest.raises(RuntimeError, match="at most 4096 sequences"):
+        _decode(a)
+    a = _args(B=9000)
+    with pytest.raises(RuntimeError, match="B up to 8192"):
+        _prefill(a)
+    jobs = torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="jobs_dev must be contiguous"):
+        ops._C.wsync(jobs, jobs, 0, [], [], 0, 0, 0, 0)

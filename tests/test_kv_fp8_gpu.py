@@ -454,6 +454,15 @@ def test_prefill_bad_pages_and_tiles(dev):
         with pytest.raises(RuntimeError, match="bounds"):
             ops.check_status(st)
         assert torch.equal(out[:20], ref[:20]) and (out[20:] == 7.0).all()
+    # room for just the blocks read (3 of the first sequence, 2 of the second), and for one fewer
+    st = ops.new_status(dev)
+    out = ops.prefill_attention_paged_fp8(q, k, v, ks, vs, table, i32(good), hq, hkv, status=st, n_blocks=5)
+    ops.check_status(st)
+    assert torch.equal(out, ref)
+    out = ops.prefill_attention_paged_fp8(q, k, v, ks, vs, table, i32(good), hq, hkv, status=st, n_blocks=4)
+    with pytest.raises(RuntimeError, match="bounds"):
+        ops.check_status(st)
+    assert torch.equal(out[:20], ref[:20])
     for bad in (nb, -1, 2**31 - 1):
         st = ops.new_status(dev)
         t = table.clone()

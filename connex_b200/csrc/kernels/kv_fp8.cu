@@ -1078,9 +1078,10 @@ void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes
 // The work: an item is a tile and a team's query heads, its length its key
 // tiles and ITEM_COST for its fixed cost.  The items, laid end to end, are cut
 // into equal shares, one per team; a cut within CUT_SLACK of an item's start
-// or end moves there.  Against one item per CTA at a time: 16 rows at 131056
-// 540 us, 1810 without; 256 rows at 7936 60 us, 131; 2048 rows at 6144 211 us,
-// 225; eight prompts of 2048, whose items balance by themselves, 304 and 292.
+// or end moves there.  Against one item per CTA at a time, the conversion
+// not counted in the latter: 16 rows at 131056 534 and 1692 us, 256 rows at
+// 7936 61 and 121; 2048 rows at 6144 200 and 213; eight prompts of 2048, whose
+// items balance by themselves, 290 and 276.
 namespace kvd {
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int ROWS = 256, KEYS = 128;                   // of a tile of the attention

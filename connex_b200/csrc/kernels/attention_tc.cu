@@ -454,7 +454,10 @@ __global__ void __launch_bounds__(fatc::THREADS, 2)
 // done, its first scores are computed while the softmax warps still store
 // the previous item's O, and the next P.V (which overwrites O_X) waits for
 // P_X(0) -- which that warpgroup writes only after its epilogue read O_X.
-// SPLIT: the CTAs' work comes from a plan (AttnPlan): equal shares of the
+// SPLIT: a Q tile's 128 rows are the query heads of a KV head side by side (as
+// many as the power of two in their number) by 128 / that many tokens, so a
+// short chunk fills the rows and reads its keys once for all of them; and the
+// CTAs' work comes from a plan (AttnPlan): equal shares of the
 // items' key tiles laid end to end, so an item may be cut into pieces of
 // consecutive CTAs.  A piece leaves its unnormalised O, running maxima and
 // sums in the workspace; the warpgroup that arrives last for a tile adds them
@@ -585,7 +588,8 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int n_items = SPLIT ? n_tiles * (Hq / plan.team) : n_tiles * Hq;
+  const int n_items = SPLIT ? n_tiles * Hq / plan.team : n_tiles * Hq;
+  const int tokens = SPLIT ? BM >> plan.pack : BM;   // query positions of a Q tile
   // the CTA's k-th item (n_items: no more)
   int2 cut0 = make_int2(0, 0), cut1 = cut0;
   int team = 0, member = 0;
@@ -604,17 +608,30 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
     }
   };
   auto item = [&](int w, int k) -> Item {
-    Item it = item_of<PAGED>(SPLIT ? w * plan.team + member : w, tile_info, n_tiles, Hq, Hkv, block_tables, bt_stride);
     if constexpr (SPLIT) {
+      Item it;
+      const int each = (Hq >> plan.pack) / plan.team, tile = w / each;
+      const int* ti = tile_info + tile * 5;
+      it.h = ((w - tile * each) * plan.team + member) << plan.pack;      // the first of its heads
+      it.g = it.h / (Hq / Hkv);
+      it.seq_start = ti[0];
+      it.seq_len = ti[1];
+      it.q0 = ti[2];
+      it.ctx = ti[3];
+      it.total = it.ctx + it.seq_len;
+      it.bt = block_tables + (size_t)ti[4] * bt_stride;
       it.j0 = k == 0 ? cut0.y : 0;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        it.all[x] = it.nt[x];
-        it.nt[x] = max(0, (w == cut1.x ? min(it.nt[x], cut1.y) : it.nt[x]) - it.j0);
+        const int r0 = it.q0 + x * tokens;
+        it.all[x] = r0 < it.seq_len ? (min(it.total, it.ctx + r0 + tokens) + BN - 1) / BN : 0;
+        it.nt[x] = max(0, (w == cut1.x ? min(it.all[x], cut1.y) : it.all[x]) - it.j0);
       }
       it.nkv = max(it.nt[0], it.nt[1]);
+      return it;
+    } else {
+      return item_of<PAGED>(w, tile_info, n_tiles, Hq, Hkv, block_tables, bt_stride);
     }
-    return it;
   };
 
   if (warp < 4) {
@@ -641,9 +658,15 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
             if (!pwait(&q_empty[x], (n_it & 1) ^ 1)) { good = false; break; }
             ++nq[x];
             mbar_arrive_expect_tx(&q_full[x], TILE_Q);
-            tma_load_2d(smem + OFF_Q + x * TILE_Q, &tmq, &q_full[x], qcol, it.seq_start + it.q0 + x * BM);
-            tma_load_2d(smem + OFF_Q + x * TILE_Q + HALF_Q, &tmq, &q_full[x], qcol + 64,
-                        it.seq_start + it.q0 + x * BM);
+            if constexpr (SPLIT) {   // a token's heads in consecutive rows
+              tma_load_3d(smem + OFF_Q + x * TILE_Q, &tmq, &q_full[x], 0, it.h, it.seq_start + it.q0 + x * tokens);
+              tma_load_3d(smem + OFF_Q + x * TILE_Q + HALF_Q, &tmq, &q_full[x], 64, it.h,
+                          it.seq_start + it.q0 + x * tokens);
+            } else {
+              tma_load_2d(smem + OFF_Q + x * TILE_Q, &tmq, &q_full[x], qcol, it.seq_start + it.q0 + x * BM);
+              tma_load_2d(smem + OFF_Q + x * TILE_Q + HALF_Q, &tmq, &q_full[x], qcol + 64,
+                          it.seq_start + it.q0 + x * BM);
+            }
           }
           if (!good) break;
           // paged: cache rows of the eight 16-token blocks of a key tile (tile j's
@@ -811,8 +834,9 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
     long long t_s = 0, t_c = 0, t_e = 0, t_o = 0, t_mark = 0;
     for (int k = 0, w = item_no(0); w < n_items && ok; ++k, w = item_no(k)) {
       const Item it = item(w, k);
-      const int r0 = it.q0 + x * BM;      // first query of the tile
-      const int qpos = it.ctx + r0 + row; // position in the sequence
+      const int r0 = it.q0 + x * tokens;  // first query of the tile
+      const int rt = SPLIT ? row >> plan.pack : row;   // the row's query among them
+      const int qpos = it.ctx + r0 + rt;  // position in the sequence
       const int n = it.nt[x];
       const int zero_x = it.nt[0] == it.nkv ? 0 : 1;   // the tile whose P.V reads the last V tile first
       float m = -INFINITY, l = 0.f;
@@ -928,8 +952,9 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
         if (rec) t_o += clock64() - te0;
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        const bool valid = r0 + row < it.seq_len;
-        __nv_bfloat16* orow = out + (size_t)(it.seq_start + r0 + row) * ldo + (size_t)it.h * D;
+        const bool valid = r0 + rt < it.seq_len;
+        const int head = SPLIT ? it.h + (row & ((1 << plan.pack) - 1)) : it.h;
+        __nv_bfloat16* orow = out + (size_t)(it.seq_start + r0 + rt) * ldo + (size_t)head * D;
         if constexpr (SPLIT) {
           // the teams whose CTAs have a piece of this tile
           int c0 = team, c1 = team;
@@ -1171,6 +1196,8 @@ void prefill_attention_paged_tc(const void* qkv, int ldq, int qkv_cols, int T, c
   a.status = status;
   if (plan != nullptr) {
     a.plan = *plan;
+    const uint32_t heads = 1u << plan->pack;
+    a.tq = make_tmap_bf16_3d(qkv, 128, (uint64_t)Hq, (uint64_t)T, 256, (uint64_t)ldq * 2, 64, heads, 128 / heads);
     launch_attn<true, true, 0, false, true>(a, s);
   } else if (tile_rows == fap::ROWS)
     launch_attn_split<true, true>(a, s);

@@ -378,10 +378,17 @@ void kv_copy_blocks(at::Tensor& kv, const at::Tensor& pairs, const c10::optional
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
+// log2 of the query heads that a prefill tile holds side by side: the power of two in the group, up to 128
+int pack_log(int64_t group) {
+  int p = 0;
+  while (p < 7 && group > 0 && group % (2ll << p) == 0) ++p;
+  return p;
+}
+
 // Workspace of prefill_attention_paged_fp8 besides the blocks: int32 words and fp32 words.
-std::tuple<int64_t, int64_t> prefill_fp8_words(int64_t device, int64_t entries, int64_t n_tiles) {
-  const int64_t ctas = at::cuda::getDeviceProperties(device)->multiProcessorCount;
-  return {2 * (n_tiles + 1) + 2 * (ctas + 1) + 2 * ctas + entries + 5 * n_tiles, 2 * ctas * cx::AttnPlan::SLOT};
+std::tuple<int64_t, int64_t> prefill_fp8_words(int64_t device, int64_t entries, int64_t n_tiles, int64_t group) {
+  const int64_t ctas = at::cuda::getDeviceProperties(device)->multiProcessorCount, items = n_tiles << pack_log(group);
+  return {2 * items + 2 * (ctas + 1) + 2 * ctas + entries + 5 * items, 2 * ctas * cx::AttnPlan::SLOT};
 }
 
 // Two launches: the tables' blocks as bf16 into workspaces of the caller, the
@@ -401,10 +408,11 @@ void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, cons
   TORCH_CHECK(q.size(1) >= Hq * 128 && out.size(0) == T && out.size(1) == Hq * 128,
               "prefill_attention_paged_fp8: q must hold Hq heads of 128 per row and out be [T, Hq * 128]");
   TORCH_CHECK(tile_info.scalar_type() == at::kInt && tile_info.dim() == 2 && tile_info.size(1) == 5 &&
-                  tile_info.is_contiguous() && (tile_info.size(0) + 1) * Hq <= INT_MAX,
+                  tile_info.is_contiguous() && (tile_info.size(0) + 1) * Hq <= INT_MAX / 5,
               "prefill_attention_paged_fp8: tile_info must be contiguous int32 [n, 5]");
   TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
-                  block_tables.numel() <= INT_MAX && block_tables.size(0) <= cx::KVQ_MAX_CHUNKS,
+                  block_tables.numel() <= INT_MAX && block_tables.size(1) < (int64_t)1 << 26 &&
+                  block_tables.size(0) <= cx::KVQ_MAX_CHUNKS,
               "prefill_attention_paged_fp8: block_tables must be contiguous int32 [B, max_blocks], B up to ",
               num(cx::KVQ_MAX_CHUNKS));
   TORCH_CHECK(kv.dim() == 5 && kv.size(0) == 2 && kv.size(2) == Hkv && kv.size(3) == 16 && kv.size(4) == 128 &&
@@ -412,7 +420,11 @@ void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, cons
               "prefill_attention_paged_fp8: the blocks' workspace must be contiguous bf16 [2, n_blocks, Hkv, 16, 128]");
   CHECK_CUDA(q);
   const int64_t entries = block_tables.numel(), n_tiles = tile_info.size(0);
-  const auto [n_ints, n_part] = prefill_fp8_words(q.device().index(), entries, n_tiles);
+  // The query heads of a KV head share a tile's rows where tokens alone would leave a quarter of them empty
+  // (32/8 heads, 16 chunks at 4000: of 16 rows 141 us, 285 with tokens alone, of 128 rows 213 and 300; one
+  // chunk at 30000: of 16 rows 107 and 147, of 192 137 and 158, of 256 160 and 157; one of 128 at 500 25 and 23).
+  const int pack = T * 4 <= n_tiles * 256 * 3 ? pack_log(Hq / Hkv) : 0;
+  const auto [n_ints, n_part] = prefill_fp8_words(q.device().index(), entries, n_tiles, Hq / Hkv);   // room for either
   TORCH_CHECK(ints.has_value() && ints->scalar_type() == at::kInt && ints->numel() == n_ints && ints->is_contiguous() &&
                   part.has_value() && part->scalar_type() == at::kFloat && part->numel() == n_part && part->is_contiguous(),
               "prefill_attention_paged_fp8: workspaces of other sizes");
@@ -424,24 +436,25 @@ void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, cons
   cx::KvChunks o;
   o.k = kv.data_ptr();
   o.v = static_cast<char*>(kv.data_ptr()) + kv.nbytes() / 2;
-  // query heads of a KV head run side by side, so that its keys come from L2 for all but one
-  // (2 x 256 rows at 32256: 263 us, 272 one by one); four at most, or the last team leaves
-  // SMs without work (8 query heads of one KV head, 2048 rows at 6144: 71 us, 79 with eight)
+  o.pack = pack;
+  // else they run side by side, so that the keys come from L2 for all but one (2 x 256 rows at 32256: 263 us,
+  // 272 one by one); four at most, or the last team leaves SMs without work (8 query heads of one KV head,
+  // 2048 rows at 6144: 71 us, 79 with eight)
   o.team = 1;
-  for (int t = 2; t <= 4; ++t)
+  for (int t = 2; pack == 0 && t <= 4; ++t)
     if (Hq / Hkv % t == 0) o.team = t;
-  const int sms = sms_of(q);
   o.blocks = (int)kv.size(1);
+  const int sms = sms_of(q);
   o.n_cta = std::max(1, sms / o.team) * o.team;
   o.before = reinterpret_cast<int64_t*>(ints->data_ptr<int>());      // the 8-byte words first
-  o.cuts = reinterpret_cast<int2*>(o.before + n_tiles + 1);
+  o.cuts = reinterpret_cast<int2*>(o.before + (n_tiles << pack));
   o.arrived = reinterpret_cast<int*>(o.cuts + sms + 1);
   o.tables = o.arrived + 2 * sms;
   o.tiles = o.tables + entries;
   cx::kv_dequant_blocks(c, block_tables.data_ptr<int>(), (int)block_tables.size(0), (int)block_tables.size(1),
                         tile_info.data_ptr<int>(), (int)n_tiles, (int)T, (int)Hq, o, status_ptr(status), cur_stream(q));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  const cx::AttnPlan plan{o.cuts, part->data_ptr<float>(), o.arrived, o.n_cta, o.team};
+  const cx::AttnPlan plan{o.cuts, part->data_ptr<float>(), o.arrived, o.n_cta, o.pack, o.team};
   cx::prefill_attention_paged_tc(q.data_ptr(), ldq, (int)(Hq * 128), (int)T, o.k, o.v, kv.size(1) * Hkv * 16, o.tables,
                                  (int)block_tables.size(1), out.data_ptr(), ldo, o.tiles, (int)n_tiles, (int)Hq,
                                  (int)Hkv, (float)scale, status_ptr(status), cur_stream(q), 256, &plan);

@@ -378,6 +378,23 @@ CUtensorMap make_tmap_bf16_2d(const void* base, uint64_t inner, uint64_t outer, 
   return m;
 }
 
+CUtensorMap make_tmap_bf16_3d(const void* base, uint64_t inner, uint64_t mid, uint64_t outer, uint64_t mid_stride_bytes,
+                              uint64_t outer_stride_bytes, uint32_t box_inner, uint32_t box_mid, uint32_t box_outer) {
+  if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) throw std::runtime_error("cx: TMA base not 16-byte aligned");
+  if (((mid_stride_bytes | outer_stride_bytes) & 15) != 0)
+    throw std::runtime_error("cx: TMA row stride not a multiple of 16 bytes");
+  CUtensorMap m;
+  cuuint64_t dims[3] = {inner, mid, outer};
+  cuuint64_t strides[2] = {mid_stride_bytes, outer_stride_bytes};
+  cuuint32_t box[3] = {box_inner, box_mid, box_outer};
+  cuuint32_t es[3] = {1, 1, 1};
+  CUresult r = get_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+                               es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("cx: cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+  return m;
+}
+
 int num_sms() {
   static int n = 0;
   if (n == 0) {

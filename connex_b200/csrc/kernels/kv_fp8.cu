@@ -1075,13 +1075,13 @@ void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes
 // first CTA also hands on the tiles that fit the rows and the tables -- the
 // attention kernel takes them as they are -- and divides their work.
 //
-// The work: an item is a tile and a team's query heads, its length its key
-// tiles and ITEM_COST for its fixed cost.  The items, laid end to end, are cut
-// into equal shares, one per team; a cut within CUT_SLACK of an item's start
-// or end moves there.  Against one item per CTA at a time, the conversion
-// not counted in the latter: 16 rows at 131056 534 and 1692 us, 256 rows at
-// 7936 61 and 121; 2048 rows at 6144 200 and 213; eight prompts of 2048, whose
-// items balance by themselves, 290 and 276.
+// The work: an item is 256 rows (tokens of a tile by query heads) for each CTA
+// of a team, its length its key tiles and ITEM_COST for its fixed cost.  The
+// items, laid end to end, are cut into equal shares, one per team; a cut within
+// CUT_SLACK of an item's start or end moves there.  Against one item per CTA at a time, the conversion
+// not counted in the latter: 256 rows at 7936 60 and 121 us, 2 x 256 at 32256
+// 263 and 465, 2048 rows at 6144 201 and 211; eight prompts of 2048, whose items
+// balance by themselves, 294 and 279.
 namespace kvd {
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int ROWS = 256, KEYS = 128;                   // of a tile of the attention
@@ -1094,38 +1094,50 @@ __device__ __forceinline__ bool tile_fits(const int* ti, int T, int B, int width
   return seq >= 0 && seq < B && n > 0 && q0 >= 0 && q0 < n && ctx >= 0 && start >= 0 && (int64_t)start + n <= T &&
          (int64_t)ctx + n <= (int64_t)width * kvq::BS;
 }
-// key tiles of a tile that fits
-__device__ __forceinline__ int tile_keys(const int* ti) {
-  return (min(ti[3] + ti[1], ti[3] + ti[2] + kvd::ROWS) + kvd::KEYS - 1) / kvd::KEYS;
+// key tiles of `tokens` queries from q0
+__device__ __forceinline__ int tile_keys(const int* ti, int q0, int tokens) {
+  return (min(ti[3] + ti[1], ti[3] + q0 + tokens) + kvd::KEYS - 1) / kvd::KEYS;
 }
 __device__ __forceinline__ void kv_prefill_plan(const int* __restrict__ tile_info, int n_tiles, int T, int B, int width,
                                                 int Hq, const KvChunks& o, int* status) {
   using namespace kvd;
   __shared__ int64_t wlen[WARPS];
   __shared__ int wfit[WARPS];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t len = 0;                                      // of the tiles so far, for one head
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, tokens = ROWS >> o.pack;
+  int64_t len = 0;                                      // of the tiles so far, for one set of heads
   int kept = 0;
+  __shared__ int longest;
+  if (tid == 0) longest = 0;
+  __syncthreads();
   for (int t0 = 0; t0 < n_tiles; t0 += THREADS) {
     const int t = t0 + tid;
     const int* ti = tile_info + 5 * (int64_t)t;
     const bool fits = t < n_tiles && tile_fits(ti, T, B, width);
     if (t < n_tiles && !fits) record_status(status, CX_ERR_BOUNDS);
-    const int64_t n = fits ? tile_keys(ti) + ITEM_COST : 0;
+    int parts = 0;                                      // items of the tile for one set of heads
+    int64_t n = 0;                                      // their length
+    if (fits)
+      for (int q0 = ti[2], q1 = min(ti[1], ti[2] + ROWS); q0 < q1; q0 += tokens, ++parts)
+        n += tile_keys(ti, q0, tokens) + ITEM_COST;
+    if (fits) atomicMax(&longest, tile_keys(ti, ti[2], ROWS));
     int64_t x = n;
+    int y = parts;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
-      if (lane >= d) x += y;
+      const int64_t xu = __shfl_up_sync(0xffffffffu, x, d);
+      const int yu = __shfl_up_sync(0xffffffffu, y, d);
+      if (lane >= d) {
+        x += xu;
+        y += yu;
+      }
     }
-    const uint32_t fit = __ballot_sync(0xffffffffu, fits);
     if (lane == 31) {
       wlen[warp] = x;
-      wfit[warp] = __popc(fit);
+      wfit[warp] = y;
     }
     __syncthreads();
     int64_t at = len + x - n;
-    int to = kept + __popc(fit & ((1u << lane) - 1));
+    int to = kept + y - parts;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       if (w < warp) {
@@ -1135,15 +1147,18 @@ __device__ __forceinline__ void kv_prefill_plan(const int* __restrict__ tile_inf
       len += wlen[w];
       kept += wfit[w];
     }
-    if (fits) {
-      for (int e = 0; e < 5; ++e) o.tiles[5 * (int64_t)to + e] = ti[e];
+    for (int k = 0; k < parts; ++k, ++to) {
+      for (int e = 0; e < 5; ++e) o.tiles[5 * (int64_t)to + e] = ti[e] + (e == 2 ? k * tokens : 0);
       o.before[to] = at;
+      at += tile_keys(ti, ti[2] + k * tokens, tokens) + ITEM_COST;
     }
     __syncthreads();
   }
   for (int i = tid; i < 2 * o.n_cta; i += THREADS) o.arrived[i] = 0;
-  const int teams = o.n_cta / o.team, each = Hq / o.team;    // items of a tile
-  const int64_t total = len * each, per = max((int64_t)MIN_SHARE, (total + teams - 1) / teams);
+  const int teams = o.n_cta / o.team, each = (Hq >> o.pack) / o.team;     // items of a tile
+  // a piece costs its item's merge about what a key tile costs its CTA: shares of at least sqrt(length)
+  const int least = max(MIN_SHARE, (int)sqrtf((float)longest));
+  const int64_t total = len * each, per = max((int64_t)least, (total + teams - 1) / teams);
   for (int i = tid; i <= teams; i += THREADS) {
     const int64_t x = i * per;
     int2 cut = make_int2(kept * each, 0);
@@ -1154,7 +1169,7 @@ __device__ __forceinline__ void kv_prefill_plan(const int* __restrict__ tile_inf
         if (o.before[mid] * each <= x) lo = mid;
         else hi = mid;
       }
-      const int n = tile_keys(o.tiles + 5 * (int64_t)lo) + ITEM_COST;
+      const int n = tile_keys(o.tiles + 5 * (int64_t)lo, o.tiles[5 * (int64_t)lo + 2], tokens) + ITEM_COST;
       const int64_t in = x - o.before[lo] * each;
       const int h = (int)(in / n), p = (int)(in - (int64_t)h * n);
       const int slack = min((n - ITEM_COST) / 2, CUT_SLACK);

@@ -51,11 +51,11 @@ struct KvChunks {
   void* v;
   int blocks;       // room for this many
   int* tables;      // [B, width]
-  int* tiles;       // [n_tiles, 5]: the tiles that fit, in their order
+  int* tiles;       // [n_tiles << pack, 5]: the tiles that fit, in their order, in 256 >> pack tokens each
   int2* cuts;       // [n_cta / team + 1], see AttnPlan
   int* arrived;     // [2 n_cta], zero
-  int64_t* before;  // [n_tiles + 1] scratch
-  int n_cta, team;
+  int64_t* before;  // [n_tiles << pack] scratch
+  int n_cta, pack, team;
 };
 // The e4m3 blocks that the tiles (tile_info [n_tiles, 5] of the paged prefill)
 // read through tables [B, width] (B <= KVQ_MAX_CHUNKS), as bf16 blocks, those

@@ -30,24 +30,26 @@ void attention_exp_split(int n);
 void attention_profile(int64_t ptr);
 
 // Work of the two-tile prefill attention in equal shares (built on the device,
-// see kv_prefill_plan).  Teams of `team` CTAs, a divisor of Hq / Hkv, take that
-// many query heads of one KV head side by side: team i the items (tile, heads)
-// from (cuts[i].x, key tile cuts[i].y) up to where cuts[i + 1] begins.  part:
-// SLOT floats for each of a CTA's two pieces of cut items; arrived: 2 n_cta
+// see kv_prefill_plan).  A tile's 256 rows are 256 >> pack tokens of 1 << pack
+// query heads, which share a KV head.  Teams of `team` CTAs take that many sets
+// of heads of one KV head side by side: team i the items (tile, sets) from
+// (cuts[i].x, key tile cuts[i].y) up to where cuts[i + 1] begins.  part: SLOT
+// floats for each of a CTA's two pieces of cut items; arrived: 2 n_cta
 // counters, zero.
 struct AttnPlan {
   static constexpr int SLOT = 2 * 130 * 128;   // two tiles: O and the rows' maxima and sums
   const int2* cuts;
   float* part;
   int* arrived;
-  int n_cta, team;
+  int n_cta, pack, team;
 };
 
 // The same over a paged cache (chunked prefill): q rows from QKV; K/V of the
 // whole context from the caches [blocks, Hkv, 16, 128] (cache_rows =
 // blocks * Hkv * 16) through block_tables [B, bt_stride]; tile_info: [n_tiles,
 // 5] int32 of (seq start row, new tokens, first query, context length,
-// sequence index).  With a plan the work is divided by it (tile_rows 256).
+// sequence index).  With a plan the work is divided by it (tile_rows 256), and
+// the tiles are the plan's.
 void prefill_attention_paged_tc(const void* qkv, int ldq, int qkv_cols, int T, const void* kc, const void* vc,
                                 int64_t cache_rows, const int* block_tables, int bt_stride, void* out, int ldo,
                                 const int* tile_info, int n_tiles, int Hq, int Hkv, float scale, int* status,

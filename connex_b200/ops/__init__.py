@@ -361,7 +361,8 @@ def prefill_attention_paged_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache:
     kv = torch.empty(2, n_blocks, n_kv_heads, 16, 128, dtype=torch.bfloat16, device=q.device)
     ints = part = None
     if q.is_cuda:
-        n_ints, n_part = _C.prefill_fp8_words(q.device.index, block_tables.numel(), tile_info.shape[0])
+        n_ints, n_part = _C.prefill_fp8_words(q.device.index, block_tables.numel(), tile_info.shape[0],
+                                             n_q_heads // max(1, n_kv_heads))
         ints = torch.empty(n_ints, dtype=torch.int32, device=q.device)
         part = torch.empty(n_part, dtype=torch.float32, device=q.device)
     _C.prefill_attention_paged_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tables, out, tile_info, n_q_heads,

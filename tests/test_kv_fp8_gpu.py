@@ -146,6 +146,12 @@ def test_prefill_attention(dev, heads, rows):
     assert (err <= tol).all(), float((err / tol).max())
 
 
+@pytest.mark.parametrize("heads", [(128, 1), (12, 1), (40, 8)])
+def test_prefill_other_groups(dev, heads):
+    """Groups of which all, some or none of the heads share a tile's rows."""
+    test_prefill_attention(dev, heads, [(200, 9), (40, 130)])
+
+
 def test_prefill_replayed(dev):
     """A captured call divides the work from what the tiles hold at its replay, and gives an eager call's bits."""
     from connex_b200 import ops

@@ -108,11 +108,15 @@ struct alignas(16) f32x4 {        // two pairs of fp32
 // keeps the result independent of the rows' order (of two rows for one slot
 // the later wins).  Each of its warps takes K or V of one KV head on its own:
 // all rows' loads in flight together, K rotated, the largest magnitude, the
-// scale, the block's older rows requantised if the scale grew, the new rows.  A block whose row 0 is written
-// starts anew; otherwise its scale never shrinks.  Tokens are dealt to these
-// CTAs with an odd stride: the first rows of blocks, every 16th token of a
-// prompt, then spread over all of them, and so do the rows of decode steps.
-// Rotation CTAs take the q heads, eight of a token per warp at a time.
+// scale, the block's older rows requantised if the scale grew, the new rows.
+// A block whose row 0 is written starts anew; otherwise its scale never
+// shrinks.  Tokens are dealt to these CTAs with an odd stride: the first rows
+// of blocks, every 16th token of a prompt, then spread over all of them, and
+// so do the rows of decode steps.  Rotation CTAs take the q heads, eight of a
+// token per warp at a time.
+// 8192 rows of 32/8 heads take 43 us: rotating q alone 25 (134 MB at 5.3
+// TB/s), and on the same SMs the scans 6, the blocks' stores 3.5 and their
+// arithmetic 4.
 __device__ __forceinline__ void write_block(const __nv_bfloat16* qkv, int ldq, const int* pos, const float* cos_sin,
                                             const int64_t* slots, const KvFp8& c, int t, int blk, int group, int T,
                                             int Hq, int max_pos, const __nv_bfloat16* kn, float eps) {
@@ -446,14 +450,16 @@ void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_s
 // equal shares, one per CTA, from the lengths themselves -- the same launch (a
 // graph replay) is balanced for any lengths.  A pair that spans several CTAs
 // leaves partial results in the workspace, and the CTA that arrives last
-// merges them (a counter that wraps to zero by itself).  Where no pair is
+// merges them (a counter that wraps to zero by itself).  64 x 4096 tokens of
+// 32/8 heads take 100 us, 0.82 of the rate of a copy (the loads alone 95, a
+// fixed 10 of it before the first byte and after the last).  Where no pair is
 // longer than two shares, cuts move by up to SLACK blocks' worth to the pair's
 // start or end: a part more costs a CTA more than that (64 x 128 tokens 7.7 us,
 // 14.3 with the cuts where they fall; 64 x 500 15.2 and 19.5; with twice the
 // slack 100 x 2048 takes 84, not 80; ragged lengths gain nothing).
 namespace dec8 {
 constexpr int D = kvq::D, BS = kvq::BS, WARPS = 4, THREADS = 32 * WARPS, CTAS_PER_SM = 4;
-constexpr int MIN_UNITS = 2 * WARPS;    // a CTA takes at least this many blocks' worth (500 tokens alone: 6.6 us; 7.5 with twice as many)
+constexpr int MIN_UNITS = 2 * WARPS;    // blocks' worth of a CTA, at least (500 tokens alone: 6.6 us; 7.5 with 16)
 constexpr int PAIR_COST = 4 * WARPS;    // measured on ragged lengths: 41 us with 8, 34 with 16 and with 32
 constexpr int SLACK = 2 * PAIR_COST;    // see the work split above
 constexpr float RESCALE = 8.f;          // O is rescaled once mv has grown by this much: weights stay under 2^9

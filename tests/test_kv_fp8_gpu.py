@@ -485,6 +485,40 @@ def test_prefill_bad_pages_and_tiles(dev):
         assert (err <= U_BF16 * want.abs() + mag * 2.0 ** -6 + 1e-6).all()
 
 
+def test_empty_calls(dev):
+    """No rows, no sequences, no tiles, no table, no pairs: nothing is written and nothing fails."""
+    from connex_b200 import ops
+    hq, hkv, nb = 8, 2, 6
+    k, ks = _cache(nb, hkv, dev, 131)
+    v, vs = _cache(nb, hkv, dev, 132)
+    was = [t.view(torch.uint8).clone() for t in (k, v)]
+    i32 = lambda *n: torch.zeros(*n, dtype=torch.int32, device=dev)  # noqa: E731
+    st = ops.new_status(dev)
+    cs = ops.rope_cos_sin(64, D, 5e5, dev)
+    qkv = torch.zeros(0, (hq + 2 * hkv) * D, dtype=torch.bfloat16, device=dev)
+    out = ops.rope_cache_fp8(qkv, i32(0), cs, hq, hkv, torch.zeros(0, dtype=torch.int64, device=dev), k, v, ks, vs, status=st)
+    assert out.shape == (0, hq * D)
+    ws = ops.decode_workspace_fp8(3, hq, hkv, dev)
+    q = torch.ones(3, hq * D, dtype=torch.bfloat16, device=dev)
+    assert ops.decode_attention_fp8(q[:0], k, v, ks, vs, i32(0, 4), i32(0), hq, ws, status=st).shape == (0, hq * D)
+    assert (ops.decode_attention_fp8(q, k, v, ks, vs, i32(3, 0), i32(3), hq, ws, status=st) == 0).all()
+    tiles = torch.tensor([[0, 3, 0, 0, 0]], dtype=torch.int32, device=dev)
+    ops.prefill_attention_paged_fp8(q[:0], k, v, ks, vs, i32(1, 4), tiles, hq, hkv, status=st)
+    kept = torch.full((3, hq * D), 7.0, dtype=torch.bfloat16, device=dev)
+    ops.prefill_attention_paged_fp8(q, k, v, ks, vs, i32(1, 4), tiles[:0], hq, hkv, out=kept, status=st)
+    assert (kept == 7.0).all()
+    for table, n in ((i32(0, 4), None), (i32(1, 0), None), (i32(1, 4), 0)):
+        with pytest.raises(RuntimeError, match="no block table"):
+            ops.prefill_attention_paged_fp8(q, k, v, ks, vs, table, tiles, hq, hkv, status=st, n_blocks=n)
+    ops.kv_copy_blocks(torch.stack((k, v))[None], i32(0, 2), torch.stack((ks, vs))[None], status=st)
+    ops.check_status(st)
+    assert all(torch.equal(t.view(torch.uint8), w) for t, w in zip((k, v), was))
+    # a length but no table: cut, and recorded
+    assert (ops.decode_attention_fp8(q, k, v, ks, vs, i32(3, 0), i32(3) + 5, hq, ws, status=st) == 0).all()
+    with pytest.raises(RuntimeError, match="bounds"):
+        ops.check_status(st)
+
+
 def test_decode_nan_and_extreme_logits(dev):
     """A NaN key poisons its own head only; logits far apart and q's of any size stay exact enough."""
     from connex_b200 import ops

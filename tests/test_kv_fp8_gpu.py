@@ -485,6 +485,39 @@ def test_prefill_bad_pages_and_tiles(dev):
         assert (err <= U_BF16 * want.abs() + mag * 2.0 ** -6 + 1e-6).all()
 
 
+def test_offsets_past_32_bits(dev):
+    """Blocks that lie more than 4 GB into the cache give the bits of the same blocks at its start."""
+    from connex_b200 import ops
+    hq, hkv, far = 16, 8, 270000
+    assert far * hkv * BS * D > 2 ** 32
+    n, T = 40, 600
+    big = torch.empty(1, 2, far + n, hkv, BS, D, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+    sc = torch.ones(1, 2, far + n, hkv, device=dev)
+    qkv = torch.randn(T, (hq + 2 * hkv) * D, generator=_g(dev, 141), device=dev).to(torch.bfloat16)
+    cs = ops.rope_cos_sin(T, D, 5e5, dev)
+    pos = torch.arange(T, dtype=torch.int32, device=dev)
+    ws = ops.decode_workspace_fp8(1, hq, hkv, dev)
+    lens = torch.tensor([T], dtype=torch.int32, device=dev)
+    ti = ops.prefill_tile_info([T], dev, ctx=[0])
+    got = []
+    for at in (0, far):
+        k, v, ks, vs = big[0, 0], big[0, 1], sc[0, 0], sc[0, 1]
+        st = ops.new_status(dev)
+        q = ops.rope_cache_fp8(qkv, pos, cs, hq, hkv, torch.arange(T, device=dev) + at * BS, k, v, ks, vs, status=st)
+        table = torch.arange(at, at + n, dtype=torch.int32, device=dev)[None]
+        got.append((k[at:at + n].clone().view(torch.uint8).flatten()[:T * hkv * D], ks[at:at + n].clone(),
+                    ops.decode_attention_fp8(q[-1:], k, v, ks, vs, table, lens, hq, ws, status=st),
+                    ops.prefill_attention_paged_fp8(q, k, v, ks, vs, table, ti, hq, hkv, status=st)))
+        ops.check_status(st)
+    full = T // BS * hkv * BS * D
+    assert torch.equal(got[0][0][:full], got[1][0][:full])
+    assert all(torch.equal(a, b) for a, b in zip(got[0][1:], got[1][1:]))
+    pairs = torch.tensor([[far + i, i + 1] for i in range(30)], dtype=torch.int32, device=dev)
+    ops.kv_copy_blocks(big, pairs, sc)
+    assert torch.equal(big[:, :, 1:31].view(torch.uint8), big[:, :, far:far + 30].view(torch.uint8))
+    assert torch.equal(sc[:, :, 1:31], sc[:, :, far:far + 30])
+
+
 def test_empty_calls(dev):
     """No rows, no sequences, no tiles, no table, no pairs: nothing is written and nothing fails."""
     from connex_b200 import ops

@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <string>
 #include <vector>
 
@@ -405,6 +406,8 @@ void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, cons
   const int64_t T = q.size(0);
   TORCH_CHECK(Hkv == c.Hkv && Hq > 0 && Hq % Hkv == 0,
               "prefill_attention_paged_fp8: Hkv as in the cache, the query heads a multiple of it");
+  // the kernel takes the row's largest score before it is scaled
+  TORCH_CHECK(scale > 0 && std::isfinite(scale), "prefill_attention_paged_fp8: the scale must be positive");
   TORCH_CHECK(q.size(1) >= Hq * 128 && out.size(0) == T && out.size(1) == Hq * 128,
               "prefill_attention_paged_fp8: q must hold Hq heads of 128 per row and out be [T, Hq * 128]");
   TORCH_CHECK(tile_info.scalar_type() == at::kInt && tile_info.dim() == 2 && tile_info.size(1) == 5 &&

@@ -348,7 +348,8 @@ def prefill_attention_paged_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache:
     ``tile_info`` from ``prefill_tile_info(n_new, device, ctx)``.  The blocks
     that the chunks read are turned into bf16 first (exact: the scales are
     powers of two), in a workspace of ``n_blocks`` blocks: a bound on those
-    of all the sequences together, by default the tables' size.  The work is divided on the device
+    of all the sequences together, by default the tables' size.  ``scale``
+    must be positive.  The work is divided on the device
     in equal shares of the keys, so few rows over a long context use every SM
     (another 39 MB of workspace).  Entries behind a sequence's end
     are not read.  A block id out of range reads as zeros, and a tile that

@@ -3,6 +3,7 @@ append's plain statement against its definition, shared blocks (fork, free,
 compaction) of both cache types, and the refusals of the operators' entry
 points -- argument checks come before the device check, so they run here."""
 import argparse
+import math
 import random
 
 import pytest
@@ -311,6 +312,12 @@ def test_stepper_from_the_command_line(monkeypatch, given):
     monkeypatch.setattr(engine, "ModelStepper", lambda *x, **kw: seen.update(kw))
     m.build_stepper(a)
     assert seen["kv_dtype"] == (given or "bf16")
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, math.inf, math.nan])
+def test_prefill_scale(scale):
+    with pytest.raises(RuntimeError, match="scale must be positive"):
+        _prefill(_args(), scale=scale)
 
 
 def test_refusals_that_name_a_number():

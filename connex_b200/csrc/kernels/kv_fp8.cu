@@ -458,6 +458,8 @@ void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_s
 // 14.3 with the cuts where they fall; 64 x 500 15.2 and 19.5; with twice the
 // slack 100 x 2048 takes 84, not 80; ragged lengths gain nothing).
 namespace dec8 {
+// Two CTAs of eight warps took 99 us of 2 x 131072 (102 with four of four) and 32.5 of ragged lengths (34), but
+// 18.2 of 64 x 500 (15.2) and 9.5 of 64 x 16 (6.0): a pair's start and end wait for all the CTA's warps.
 constexpr int D = kvq::D, BS = kvq::BS, WARPS = 4, THREADS = 32 * WARPS, CTAS_PER_SM = 4;
 constexpr int MIN_UNITS = 2 * WARPS;    // blocks' worth of a CTA, at least (500 tokens alone: 6.6 us; 7.5 with 16)
 constexpr int PAIR_COST = 4 * WARPS;    // measured on ragged lengths: 41 us with 8, 34 with 16 and with 32

@@ -1006,7 +1006,7 @@ void decode_attention_fp8(const void* q, int ldq, const KvFp8& c, const int* blo
 // A CTA moves one pair's block in a run of planes.  A pair whose destination
 // is another pair's source, or the destination of another source, has no
 // defined result: it is left out and recorded.  The check is a scan of the
-// pairs while the first plane's bytes are in flight.
+// pairs while the first vectors are in flight.
 namespace kvc {
 constexpr int THREADS = 256;
 }
@@ -1021,15 +1021,6 @@ __global__ void __launch_bounds__(kvc::THREADS)
     return;
   }
   if (src == dst) return;
-  bool bad = false;
-  for (int k = tid; k < n; k += kvc::THREADS) {
-    const int s = pairs[2 * k], d = pairs[2 * k + 1];
-    bad |= (s == dst && d != dst) || (d == dst && s != src);
-  }
-  if (__syncthreads_or(bad)) {
-    if (tid == 0) record_status(status, CX_ERR_BOUNDS);
-    return;
-  }
   // the planes' vectors end to end, eight of a thread in flight
   const int nv = (int)(block_bytes >> 4);
   const int64_t plane = (int64_t)num_blocks * block_bytes;
@@ -1038,9 +1029,9 @@ __global__ void __launch_bounds__(kvc::THREADS)
   const int total = (p1 - p0) * nv;
   int v = tid;                    // the thread's next vector of plane `at`
   int64_t at = 0;
-  for (int i = tid; i < total; i += 8 * kvc::THREADS) {
-    u128 r[8];
-    int64_t off[8];
+  u128 r[8];
+  int64_t off[8];
+  auto load = [&](int i) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       while (v >= nv) {
@@ -1051,9 +1042,23 @@ __global__ void __launch_bounds__(kvc::THREADS)
       if (i + e * kvc::THREADS < total) r[e] = ld_nc_v4(a + off[e]);
       v += kvc::THREADS;
     }
+  };
+  load(tid);
+  bool bad = false;
+  for (int k = tid; k < n; k += kvc::THREADS) {
+    const int s = pairs[2 * k], d = pairs[2 * k + 1];
+    bad |= (s == dst && d != dst) || (d == dst && s != src);
+  }
+  if (__syncthreads_or(bad)) {
+    if (tid == 0) record_status(status, CX_ERR_BOUNDS);
+    return;
+  }
+  for (int i = tid; i < total;) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (i + e * kvc::THREADS < total) st_cs_v4(b + off[e], r[e]);
+    i += 8 * kvc::THREADS;
+    if (i < total) load(i);
   }
   if (scales != nullptr)
     for (int i = tid; i < (p1 - p0) * Hkv; i += kvc::THREADS) {

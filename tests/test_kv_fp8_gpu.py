@@ -485,6 +485,39 @@ def test_prefill_bad_pages_and_tiles(dev):
         assert (err <= U_BF16 * want.abs() + mag * 2.0 ** -6 + 1e-6).all()
 
 
+def test_two_streams_at_once(dev):
+    """Calls on two streams, each with a workspace of its own, give the bits of calls one after another."""
+    from connex_b200 import ops
+    hq, hkv = 16, 4
+    sides = []
+    for i, lens in enumerate(([3000, 17, 900], [64, 5000, 1, 333])):
+        table, nb = _table(lens, dev, 151 + i)
+        k, ks = _cache(nb, hkv, dev, 153 + i)
+        v, vs = _cache(nb, hkv, dev, 155 + i)
+        new = [min(n, 70) for n in lens]
+        q = torch.randn(sum(new), hq * D, generator=_g(dev, 157 + i), device=dev).to(torch.bfloat16)
+        cache = (k, v, ks, vs, table)
+        sides.append((cache, q, torch.tensor(lens, dtype=torch.int32, device=dev),
+                      ops.prefill_tile_info(new, dev, ctx=[n - m for n, m in zip(lens, new)]),
+                      ops.decode_workspace_fp8(len(lens), hq, hkv, dev)))
+
+    def both(side):
+        cache, q, lens, ti, ws = side
+        return (ops.decode_attention_fp8(q[:len(lens)], *cache, lens, hq, ws),
+                ops.prefill_attention_paged_fp8(q, *cache, ti, hq, hkv))
+    want = [both(side) for side in sides]
+    streams = [torch.cuda.Stream(dev) for _ in sides]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (side, stream) in enumerate(zip(sides, streams)):
+            with torch.cuda.stream(stream):
+                got[i].append(both(side))
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        assert all(torch.equal(x, y) for run in runs for x, y in zip(run, w))
+
+
 def test_offsets_past_32_bits(dev):
     """Blocks that lie more than 4 GB into the cache give the bits of the same blocks at its start."""
     from connex_b200 import ops

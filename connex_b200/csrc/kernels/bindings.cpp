@@ -357,8 +357,9 @@ void kv_copy_blocks(at::Tensor& kv, const at::Tensor& pairs, const c10::optional
   TORCH_CHECK(pairs.scalar_type() == at::kInt && pairs.dim() == 2 && pairs.size(1) == 2 && pairs.is_contiguous(),
               "kv_copy_blocks: pairs must be contiguous int32 [n, 2] (source, destination)");
   const int64_t n = pairs.size(0), block = kv.size(3) * kv.size(4) * kv.size(5) * kv.element_size();
-  TORCH_CHECK(block % 16 == 0 && (reinterpret_cast<uintptr_t>(kv.data_ptr()) & 15) == 0,
-              "kv_copy_blocks: blocks must be multiples of 16 bytes on 16-byte boundaries");
+  // (a block of no bytes is one of no vectors, and the kernel counts in whole ones)
+  TORCH_CHECK(block > 0 && block % 16 == 0 && (reinterpret_cast<uintptr_t>(kv.data_ptr()) & 15) == 0,
+              "kv_copy_blocks: blocks must be multiples of 16 bytes, not empty, on 16-byte boundaries");
   TORCH_CHECK(n <= INT_MAX && kv.size(0) * 2 <= 65535 && kv.size(2) <= INT_MAX && kv.size(0) * 2 * (block / 16) <= INT_MAX / 2,
               "kv_copy_blocks: too many blocks, or blocks too large");
   float* sp = nullptr;

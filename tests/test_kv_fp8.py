@@ -331,3 +331,13 @@ def test_refusals_that_name_a_number():
     jobs = torch.zeros(1, dtype=torch.int64)
     with pytest.raises(RuntimeError, match="jobs_dev must be contiguous"):
         ops._C.wsync(jobs, jobs, 0, [], [], 0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 4, 0, BS, D), (1, 2, 4, 2, 0, D), (1, 2, 4, 2, BS, 0)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_copy_of_blocks_without_bytes_is_refused(shape, dtype):
+    """A block without bytes has no vectors for the kernel to walk."""
+    kv = torch.empty(shape, dtype=dtype)
+    scales = torch.ones(shape[:4]) if dtype == torch.float8_e4m3fn else None
+    with pytest.raises(RuntimeError, match="multiples of 16 bytes"):
+        ops.kv_copy_blocks(kv, torch.tensor([[0, 1]], dtype=torch.int32), scales)

@@ -360,7 +360,9 @@ void kv_copy_blocks(at::Tensor& kv, const at::Tensor& pairs, const c10::optional
   // (a block of no bytes is one of no vectors, and the kernel counts in whole ones)
   TORCH_CHECK(block > 0 && block % 16 == 0 && (reinterpret_cast<uintptr_t>(kv.data_ptr()) & 15) == 0,
               "kv_copy_blocks: blocks must be multiples of 16 bytes, not empty, on 16-byte boundaries");
-  TORCH_CHECK(n <= INT_MAX && kv.size(0) * 2 <= 65535 && kv.size(2) <= INT_MAX && kv.size(0) * 2 * (block / 16) <= INT_MAX / 2,
+  // pair i lies at the 32-bit words 2 i and 2 i + 1
+  TORCH_CHECK(n <= INT_MAX / 2 && kv.size(0) * 2 <= 65535 && kv.size(2) <= INT_MAX &&
+                  kv.size(0) * 2 * (block / 16) <= INT_MAX / 2,
               "kv_copy_blocks: too many blocks, or blocks too large");
   float* sp = nullptr;
   if (scales.has_value()) {

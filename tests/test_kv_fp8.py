@@ -341,3 +341,13 @@ def test_copy_of_blocks_without_bytes_is_refused(shape, dtype):
     scales = torch.ones(shape[:4]) if dtype == torch.float8_e4m3fn else None
     with pytest.raises(RuntimeError, match="multiples of 16 bytes"):
         ops.kv_copy_blocks(kv, torch.tensor([[0, 1]], dtype=torch.int32), scales)
+
+
+def test_copy_of_more_pairs_than_an_index_counts_is_refused():
+    """The kernel finds pair i at words 2 i and 2 i + 1, counted in 32 bits."""
+    kv = torch.empty(1, 2, 4, 2, BS, D, dtype=torch.bfloat16, device="meta")
+    pairs = torch.empty(2 ** 30, 2, dtype=torch.int32, device="meta")
+    with pytest.raises(RuntimeError, match="too many"):
+        ops.kv_copy_blocks(kv, pairs)
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        ops.kv_copy_blocks(kv, pairs[:2 ** 30 - 1])

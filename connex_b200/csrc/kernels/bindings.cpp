@@ -106,6 +106,16 @@ void rope_cache(at::Tensor& qkv, const at::Tensor& pos, const at::Tensor& cos_si
                 const c10::optional<at::Tensor>& vc, int64_t Hq, int64_t Hkv, const c10::optional<at::Tensor>& status,
                 const c10::optional<at::Tensor>& q_norm, const c10::optional<at::Tensor>& k_norm, double eps) {
   CHECK_BF16(qkv);
+  if (slots.has_value()) {
+    TORCH_CHECK(kc.has_value() && vc.has_value(), "rope_cache: caches required with a slot mapping");
+    // the kernel addresses them by these sizes and stores two bytes per element
+    TORCH_CHECK(kc->scalar_type() == at::kBFloat16 && vc->scalar_type() == at::kBFloat16 && kc->dim() == 4 &&
+                    kc->size(1) == Hkv && kc->size(2) > 0 && kc->size(3) == 128 && kc->is_contiguous() &&
+                    vc->is_contiguous() && vc->sizes() == kc->sizes(),
+                "rope_cache: caches must be contiguous bf16 [blocks, Hkv, tokens, 128]; an 8-bit cache is written by "
+                "rope_cache_fp8");
+    TORCH_CHECK(kc->is_cuda() && vc->is_cuda(), "rope_cache: each cache must be a CUDA tensor");
+  }
   const void* qn = nullptr;
   const void* kn = nullptr;
   for (const auto* w : {&q_norm, &k_norm})
@@ -123,7 +133,6 @@ void rope_cache(at::Tensor& qkv, const at::Tensor& pos, const at::Tensor& cos_si
   int BS = 16, nb = 0;
   if (slots.has_value()) {
     TORCH_CHECK(slots->scalar_type() == at::kLong, "slot_mapping must be int64");
-    TORCH_CHECK(kc.has_value() && vc.has_value(), "rope_cache: caches required with a slot mapping");
     sp = slots->data_ptr<int64_t>();
     kp = kc->data_ptr();
     vp = vc->data_ptr();

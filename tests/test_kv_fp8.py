@@ -351,3 +351,29 @@ def test_copy_of_more_pairs_than_an_index_counts_is_refused():
         ops.kv_copy_blocks(kv, pairs)
     with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
         ops.kv_copy_blocks(kv, pairs[:2 ** 30 - 1])
+
+
+@pytest.mark.parametrize("k,v", [
+    (torch.float8_e4m3fn, torch.float8_e4m3fn), (torch.bfloat16, torch.float8_e4m3fn),
+    (torch.float8_e4m3fn, torch.bfloat16), (torch.uint8, torch.uint8)])
+def test_bf16_write_refuses_a_cache_of_another_type(k, v):
+    """It stores two bytes per element: past the end of an 8-bit cache."""
+    a = _args()
+    with pytest.raises(RuntimeError, match="rope_cache: caches must be"):
+        ops.rope_cache(a["qkv"], a["pos"], a["cs"], 4, 2, a["slots"], torch.zeros(5, 2, BS, D).to(k),
+                       torch.zeros(5, 2, BS, D).to(v))
+
+
+@pytest.mark.parametrize("k,v", [
+    ((5, 1, BS, D), (5, 1, BS, D)), ((5, 2, BS, D), (4, 2, BS, D)), ((5, 2, BS, 64), (5, 2, BS, 64)),
+    ((10, BS, D), (10, BS, D)), ((5, 2, 0, D), (5, 2, 0, D))])
+def test_bf16_write_refuses_a_cache_of_another_shape(k, v):
+    a = _args()
+    k, v = torch.zeros(k, dtype=torch.bfloat16), torch.zeros(v, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="rope_cache: caches must be"):
+        ops.rope_cache(a["qkv"], a["pos"], a["cs"], 4, 2, a["slots"], k, v)
+    whole = torch.zeros(5, 4, BS, D, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="rope_cache: caches must be"):
+        ops.rope_cache(a["qkv"], a["pos"], a["cs"], 4, 2, a["slots"], whole[:, ::2], whole[:, ::2])
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        ops.rope_cache(a["qkv"], a["pos"], a["cs"], 4, 4, a["slots"], whole, whole.clone())

@@ -210,6 +210,7 @@ void decode_attention(const at::Tensor& q, const at::Tensor& kc, const at::Tenso
                       at::Tensor& workspace) {
   CHECK_BF16(q);
   CHECK_BF16(kc);
+  CHECK_BF16(vc);
   TORCH_CHECK(block_tables.scalar_type() == at::kInt && ctx_lens.scalar_type() == at::kInt, "int32 tables");
   TORCH_CHECK(workspace.scalar_type() == at::kFloat, "workspace must be fp32");
   const c10::cuda::CUDAGuard g(q.device());

@@ -377,3 +377,11 @@ def test_bf16_write_refuses_a_cache_of_another_shape(k, v):
         ops.rope_cache(a["qkv"], a["pos"], a["cs"], 4, 2, a["slots"], whole[:, ::2], whole[:, ::2])
     with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
         ops.rope_cache(a["qkv"], a["pos"], a["cs"], 4, 4, a["slots"], whole, whole.clone())
+
+
+def test_bf16_decode_refuses_values_in_8_bits():
+    """Both caches are read at two bytes per element."""
+    a = _args()
+    k, ws = torch.zeros(5, 2, BS, D, dtype=torch.bfloat16), torch.zeros(1 << 16)
+    with pytest.raises(RuntimeError, match="vc must be bf16"):
+        ops.decode_attention(a["q"], k, a["v"], a["bt"], a["lens"], 4, 64, ws)

@@ -105,9 +105,14 @@ class StageModel(LlamaModel):
         ``ctx_lens``), the rest are prefill chunks that continue cached
         sequences (the paged prefill kernel over ``block_tables[n_dec:]`` and
         ``tile_info`` of width 5; ``n_blocks``: cache blocks that they read,
-        for an 8-bit cache); every GEMM runs once over all rows."""
+        for an 8-bit cache); every GEMM runs once over all rows.
+
+        ``prefill`` without ``n_dec`` attends to the step's own rows, which an
+        8-bit cache's write leaves with unrotated keys: refused over one."""
         cfg, T = self.cfg, inp.shape[0]
         assert T <= self.max_tokens
+        if prefill and n_dec is None and self.cache.scales is not None:
+            raise ValueError("prefill over an 8-bit cache reads the cache: run it as a mixed step (n_dec, block_tables)")
         self._enter(inp, T)
         for i, lw in enumerate(self.w.layers):
             qkv = self.qkv[:T]

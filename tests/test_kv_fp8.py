@@ -385,3 +385,19 @@ def test_bf16_decode_refuses_values_in_8_bits():
     k, ws = torch.zeros(5, 2, BS, D, dtype=torch.bfloat16), torch.zeros(1 << 16)
     with pytest.raises(RuntimeError, match="vc must be bf16"):
         ops.decode_attention(a["q"], k, a["v"], a["bt"], a["lens"], 4, 64, ws)
+
+
+def _runtime(monkeypatch, dtype, layers=(0, 2), blocks=32):
+    """A stage of the model on the CPU: its bookkeeping runs here, its kernels do not."""
+    from connex_b200.runtime.pp import StageRuntime
+    monkeypatch.setattr(ops, "decode_workspace_fp8", lambda *a: torch.zeros(1))       # sized by the GPU's SMs
+    return StageRuntime(LlamaConfig.tiny(layers=2), *layers, "cpu", num_blocks=blocks, max_tokens=64, max_batch=8,
+                        max_ctx=128, kv_dtype=dtype)
+
+
+def test_stage_refuses_a_prefill_that_does_not_read_the_8_bit_cache(monkeypatch):
+    """The 8-bit write leaves the fused rows' keys unrotated, so attention over those rows would be wrong."""
+    model = _runtime(monkeypatch, torch.float8_e4m3fn).model
+    ids = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="8-bit cache"):
+        model.run(ids, ids, ids.long(), prefill=True, tile_info=torch.tensor([[0, 3, 0]], dtype=torch.int32), B=1)

@@ -265,14 +265,23 @@ class StageRuntime:
         self.act = torch.empty(max_requests, self.max_ctx, self.cfg.hidden, dtype=torch.bfloat16,
                                device=self.device)
 
+    def _unlogged(self, rids) -> list:
+        """Those of ``rids`` that have no log slot yet; raises when the log has no room for them."""
+        new = [r for r in dict.fromkeys(rids) if r not in self.act_slot]
+        if len(self.act_slot) + len(new) > self.act.shape[0]:
+            raise MemoryError("activation log full")
+        return new
+
+    def _act_slots(self, rids) -> List[int]:
+        """Log slots of ``rids``.  A request keeps its slot, so those in use are
+        the numbers below ``len(act_slot)`` and the next request takes that one."""
+        for r in self._unlogged(rids):
+            self.act_slot[r] = len(self.act_slot)
+        return [self.act_slot[r] for r in rids]
+
     def _log(self, rids, ctx, n_new, out) -> None:
         slots, poss = [], []
-        for r, c, n in zip(rids, ctx, n_new):
-            sl = self.act_slot.get(r)
-            if sl is None:
-                sl = self.act_slot[r] = len(self.act_slot)
-                if sl >= self.act.shape[0]:
-                    raise MemoryError("activation log full")
+        for sl, c, n in zip(self._act_slots(rids), ctx, n_new):
             slots += [sl] * n
             poss += range(c, c + n)
         idx = (torch.tensor(slots, dtype=torch.int64).pin_memory().to(self.device, non_blocking=True),
@@ -310,16 +319,15 @@ class StageRuntime:
         if len(set(new_rids)) != len(new_rids) or any(r in self.tables for r in new_rids):
             raise ValueError("fork: the new requests must be new and distinct")
         n = self.held[rid]
-        slots = []
         if self.act is not None:
-            if len(self.act_slot) + len(new_rids) > self.act.shape[0]:
-                raise MemoryError("activation log full")
-            slots = range(len(self.act_slot), len(self.act_slot) + len(new_rids))
+            if rid not in self.act_slot:
+                raise ValueError(f"fork: {rid!r} is not in the activation log")
+            self._unlogged(new_rids)                 # room for them, before anything changes
         for r, t in zip(new_rids, self.cache.fork(self.tables[rid], n, len(new_rids))):
             self.tables[r], self.held[r] = t, n
-        for r, sl in zip(new_rids, slots):
-            self.act_slot[r] = sl
-            self.act[sl, :n] = self.act[self.act_slot[rid], :n]
+        if self.act is not None:
+            for sl in self._act_slots(new_rids):
+                self.act[sl, :n] = self.act[self.act_slot[rid], :n]
 
     def compact(self) -> int:
         """Move the live requests' KV blocks to the low end of the pool; returns the number moved."""

@@ -401,3 +401,54 @@ def test_stage_refuses_a_prefill_that_does_not_read_the_8_bit_cache(monkeypatch)
     ids = torch.zeros(3, dtype=torch.int32)
     with pytest.raises(ValueError, match="8-bit cache"):
         model.run(ids, ids, ids.long(), prefill=True, tile_info=torch.tensor([[0, 3, 0]], dtype=torch.int32), B=1)
+
+
+def _hold(rt, rid, n, value):
+    """What a step leaves behind: blocks, held tokens and, with the log on, the step's rows."""
+    rt._blocks_for(rid, n)
+    if rt.act is not None:
+        rt._log([rid], [0], [n], torch.full((n, rt.cfg.hidden), float(value), dtype=torch.bfloat16))
+    rt.held[rid] = n
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_fork_gives_every_request_a_log_of_its_own(monkeypatch, dtype):
+    """A request that was released and comes back by a fork, then a new one: each replays its own rows."""
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t: t)
+    rt = _runtime(monkeypatch, dtype, (0, 1))
+    rt.enable_activation_log(6)
+    _hold(rt, "a", 20, 1)
+    _hold(rt, "b", 5, 2)
+    rt.release(["b"])
+    rt.fork("a", ["b", "c"])
+    _hold(rt, "d", 7, 4)
+    rt.fork("d", ["e"])
+    assert len(set(rt.act_slot.values())) == len(rt.act_slot)
+    for rid, n, value in (("a", 20, 1), ("b", 20, 1), ("c", 20, 1), ("d", 7, 4), ("e", 7, 4)):
+        x, lens = rt.replay([rid])
+        assert lens == [n] and (x == value).all(), rid
+
+
+def test_fork_with_a_log_refuses_before_it_changes_anything(monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t: t)
+    rt = _runtime(monkeypatch, torch.bfloat16, (0, 1))
+    _hold(rt, "early", 20, 0)                        # before the log was kept
+    rt.enable_activation_log(3)
+    _hold(rt, "a", 20, 1)
+    _hold(rt, "gone", 4, 2)
+    rt.release(["gone"])
+
+    def state():
+        return (dict(rt.held), {r: list(t) for r, t in rt.tables.items()}, dict(rt.act_slot), dict(rt.cache._shared),
+                list(rt.cache._free))
+    before = state()
+    with pytest.raises(ValueError, match="activation log"):
+        rt.fork("early", ["x"])
+    with pytest.raises(MemoryError, match="activation log full"):
+        rt.fork("a", ["x", "y"])
+    assert state() == before
+    rt.fork("a", ["x", "gone"])                      # "gone" has its slot already
+    assert (rt.replay(["gone"])[0] == 1).all() and (rt.replay(["x"])[0] == 1).all()
+    with pytest.raises(MemoryError, match="activation log full"):
+        _hold(rt, "z", 3, 3)
+    assert "z" not in rt.act_slot

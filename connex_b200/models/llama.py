@@ -24,6 +24,7 @@ PD path launch the KV push of layer l while layers l+1.. still compute.
 from __future__ import annotations
 
 import math
+from collections import Counter
 from dataclasses import dataclass, field
 from typing import Callable, List, Optional, Sequence
 
@@ -312,12 +313,13 @@ class PagedKVCache:
     def compact(self, tables) -> int:
         """Move the blocks of ``tables`` (the block lists of the live
         sequences, changed in place) down so that the pool's used blocks are
-        its lowest ones; blocks in none of them stay where they are.  Returns
-        the number of blocks moved."""
-        tables = list(tables)
+        its lowest ones; blocks in none of them, and shared ones with an owner
+        beside them, stay where they are.  Returns the number of blocks moved."""
+        tables = list({id(t): t for t in tables}.values())
         used = self.num_blocks - len(self._free)
         holes = sorted(b for b in self._free if b < used)
-        high = sorted({b for t in tables for b in t if b >= used}, reverse=True)
+        owners = Counter(b for t in tables for b in set(t))
+        high = sorted((b for b, n in owners.items() if b >= used and n > self._shared.get(b, 0)), reverse=True)
         moves = dict(zip(high, holes))
         if not moves:
             return 0

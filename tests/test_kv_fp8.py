@@ -452,3 +452,26 @@ def test_fork_with_a_log_refuses_before_it_changes_anything(monkeypatch):
     with pytest.raises(MemoryError, match="activation log full"):
         _hold(rt, "z", 3, 3)
     assert "z" not in rt.act_slot
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_compact_leaves_blocks_of_owners_it_was_not_given(dtype):
+    """A shared block moves only when every table that names it is changed with it."""
+    c = _cache(dtype)
+    low = c.allocate(3)
+    parent = c.allocate(3)
+    child, = c.fork(parent, 2 * BS + 5)
+    c.free(low)
+    want = [_rows(c, t, 2 * BS + 5) for t in (parent, child)]
+    assert c.compact([child]) == 1                    # its own last block; the shared ones have another owner
+    assert child[:2] == parent[:2] == [3, 4] and child[2] < 3
+    for t, x in zip((parent, child), want):
+        assert torch.equal(_rows(c, t, 2 * BS + 5), x)
+    assert c.compact([child, child]) == 0             # one owner named twice is still one
+    assert c.compact([child, parent]) == 2
+    assert set(child) | set(parent) == set(range(4))
+    for t, x in zip((parent, child), want):
+        assert torch.equal(_rows(c, t, 2 * BS + 5), x)
+    c.free(parent)
+    c.free(child)
+    assert sorted(c._free) == list(range(24)) and not c._shared

@@ -212,8 +212,9 @@ class PagedKVCache:
 
     Blocks can be shared: :meth:`fork` gives sequences that continue another
     one tables on its full blocks, and :meth:`free` returns a block to the
-    pool with its last owner.  Shared blocks are only read (a sequence appends
-    behind its last full block)."""
+    pool with its last owner.  Shared blocks are only read: a sequence appends
+    behind its last full block, and :meth:`own` comes before a write to any
+    earlier one."""
 
     def __init__(self, cfg: LlamaConfig, num_blocks: int, device, dtype=torch.bfloat16,
                  storage: Optional[torch.Tensor] = None):
@@ -309,6 +310,21 @@ class PagedKVCache:
             for b in blocks[:full]:
                 self._shared[b] = self._shared.get(b, 0) + n
         return [list(blocks[:full]) + tails[i:i + 1] for i in range(n)]
+
+    def own(self, blocks: List[int], start: int, stop: int) -> None:
+        """Before the sequence with table ``blocks`` (changed in place) writes its
+        tokens [start, stop): shared blocks that they fall into give way to
+        blocks of its own, the first of which keeps the tokens before ``start``."""
+        if not self._shared:
+            return
+        bs = self.cfg.block_size
+        at = [i for i in range(start // bs, min(len(blocks), -(-stop // bs))) if blocks[i] in self._shared]
+        mine = self.allocate(len(at))
+        if at and start > at[0] * bs:
+            self.copy_blocks([(blocks[at[0]], mine[0])])
+        for i, b in zip(at, mine):
+            self.free([blocks[i]])
+            blocks[i] = b
 
     def compact(self, tables) -> int:
         """Move the blocks of ``tables`` (the block lists of the live

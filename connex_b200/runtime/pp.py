@@ -333,9 +333,12 @@ class StageRuntime:
         """Move the live requests' KV blocks to the low end of the pool; returns the number moved."""
         return self.cache.compact(self.tables.values())
 
-    def _blocks_for(self, rid, upto: int) -> List[int]:
+    def _blocks_for(self, rid, upto: int, start: Optional[int] = None) -> List[int]:
+        """The request's block table for ``upto`` tokens; those from ``start`` on may be written."""
         t = self.tables.setdefault(rid, [])
         need = -(-upto // self.bs)
+        if start is not None:
+            self.cache.own(t, start, upto)
         if len(t) < need:
             t += self.cache.allocate(need - len(t))
         return t
@@ -357,7 +360,7 @@ class StageRuntime:
         for r, c, n in zip(rids, ctx, n_new):
             if r in miss:
                 self.release([r])
-            t = self._blocks_for(r, c + n)
+            t = self._blocks_for(r, c + n, c)
             for p in range(c, c + n):
                 pos.append(p)
                 slots.append(t[p // self.bs] * self.bs + p % self.bs)

@@ -475,3 +475,39 @@ def test_compact_leaves_blocks_of_owners_it_was_not_given(dtype):
     c.free(parent)
     c.free(child)
     assert sorted(c._free) == list(range(24)) and not c._shared
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("start,stop", [(0, 1), (5, 6), (16, 17), (20, 40), (47, 50), (0, 64), (48, 49)])
+def test_a_step_behind_a_fork_writes_blocks_of_its_own(monkeypatch, dtype, start, stop):
+    """A request that goes on from before the end of its shared blocks leaves the other owners' rows alone."""
+    rt = _runtime(monkeypatch, dtype)
+    c = rt.cache
+    raw = torch.randint(0, 120, c.kv.shape, generator=torch.Generator().manual_seed(7), dtype=torch.uint8)
+    c.kv.copy_(raw.view(torch.float8_e4m3fn) if c.scales is not None else raw.float())
+    _hold(rt, "a", 50, 0)
+    before = _rows(c, rt.tables["a"], 50)
+    rt.fork("a", ["x", "y"])
+    t = rt._blocks_for("x", stop, start)
+    assert torch.equal(_rows(c, t, start).flatten(), before[:start].flatten())
+    for p in range(start, stop):                      # the step's writes
+        c.kv.view(torch.uint8 if c.scales is not None else torch.bfloat16)[:, :, t[p // BS], :, p % BS] = 1
+        if c.scales is not None:
+            c.scales[:, :, t[p // BS]] *= 4
+    for r in ("a", "y"):
+        assert torch.equal(_rows(c, rt.tables[r], 50), before)
+    rt.release(["a", "x", "y"])
+    assert sorted(c._free) == list(range(32)) and not c._shared
+
+
+def test_blocks_of_ones_own_need_room():
+    c = _cache(torch.bfloat16)
+    t = c.allocate(4)
+    x, = c.fork(t, 64)
+    c.allocate(19)
+    held = list(x), dict(c._shared)
+    with pytest.raises(MemoryError):
+        c.own(x, 20, 40)
+    assert (x, c._shared) == held and c.free_blocks == 1
+    c.own(x, 64, 70)                                  # behind the shared blocks: nothing to do
+    assert (x, c._shared) == held

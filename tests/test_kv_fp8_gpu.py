@@ -739,6 +739,32 @@ def test_decode_graphs_and_fork_8_bit(dev):
     assert outs[0] == outs[1]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_fork_that_goes_back_leaves_its_parent_alone(dev, dtype):
+    """A forked request continued from before its shared blocks' end, with other tokens: the parent's cached
+    rows keep their bytes, and the child's step equals one of a request that shares nothing."""
+    g = torch.Generator().manual_seed(6)
+    prompt = torch.randint(3, 1000, (50,), generator=g).tolist()
+    other = torch.randint(3, 1000, (9,), generator=g).tolist()
+    cfg, rt = _runtime(dev, dtype)
+    _compute(rt, "prefill", ["a", "z"], [0, 0], [50, 50], prompt * 2)
+    rt.fork("a", ["x"])
+    raw = torch.uint8 if rt.cache.scales is not None else torch.int16
+
+    def rows(rid):
+        ids = torch.tensor(rt.tables[rid][:3], device=dev)
+        parts = [rt.cache.kv[:, :, ids].view(raw)]
+        return parts + ([rt.cache.scales[:, :, ids]] if rt.cache.scales is not None else [])
+    before = rows("a")
+    got = _compute(rt, "mixed", ["x", "z"], [20, 20], [9, 9], other * 2, n_dec=0).tolist()
+    assert got[0] == got[1]
+    assert all(torch.equal(p, q) for p, q in zip(rows("a"), before))
+    assert rt.tables["x"][0] == rt.tables["a"][0] and rt.tables["x"][1] != rt.tables["a"][1]
+    assert int(rt.model.status) == 0
+    rt.release(["a", "x", "z"])
+    assert rt.cache.free_blocks == 128 and not rt.cache._shared
+
+
 def test_model_stepper_8_bit(dev):
     """The serving engine's stepper over an 8-bit cache: prefill, chunked prefill and decode agree."""
     from connex_b200.models.llama import LlamaConfig

@@ -78,7 +78,8 @@ def llama_config(a):
 def kv_blocks(a, cfg, l0: int, l1: int) -> int:
     """``--num-blocks``, or the blocks of layers [l0, l1) that fit in
     ``--kv-fraction`` of the device memory free after the weights (an
-    estimate of the weights' bytes is subtracted before they are loaded)."""
+    estimate of the weights' bytes is subtracted before they are loaded), and
+    over an 8-bit cache leave room for what a prompt step holds beside it."""
     if a.num_blocks:
         return a.num_blocks
     import torch
@@ -86,10 +87,16 @@ def kv_blocks(a, cfg, l0: int, l1: int) -> int:
     n_layers = l1 - l0
     per_layer = cfg.qkv_dim * cfg.hidden + cfg.hidden * cfg.heads * cfg.head_dim + 3 * cfg.ffn * cfg.hidden
     weights = 2 * (n_layers * per_layer + 2 * cfg.vocab_size * cfg.hidden)
-    head = cfg.block_size * cfg.head_dim + 4 if getattr(a, "kv_dtype", "bf16") == "fp8" else cfg.block_size * cfg.head_dim * 2
-    block = 2 * n_layers * cfg.kv_heads * head
     scratch = 2 << 30                       # activations, workspaces, allocator slack
-    return max(64, int((free - weights - scratch) * a.kv_fraction) // block)
+    room, bf16 = free - weights - scratch, cfg.block_size * cfg.head_dim * 2
+    fp8 = getattr(a, "kv_dtype", "bf16") == "fp8"
+    block = 2 * n_layers * cfg.kv_heads * (bf16 // 2 + 4 if fp8 else bf16)
+    n = int(room * a.kv_fraction) // block
+    if fp8:       # a prompt step holds the blocks that it reads as bf16, for one layer at a time
+        copy = 2 * cfg.kv_heads * bf16
+        most = min(a.max_batch, a.max_step_tokens) * -(-a.max_ctx // cfg.block_size)     # that one step reads
+        n = min(n, max(room // (block + copy), (room - most * copy) // block))
+    return max(64, n)
 
 
 def build_stepper(a):

@@ -511,3 +511,28 @@ def test_blocks_of_ones_own_need_room():
     assert (x, c._shared) == held and c.free_blocks == 1
     c.own(x, 64, 70)                                  # behind the shared blocks: nothing to do
     assert (x, c._shared) == held
+
+
+@pytest.mark.parametrize("fraction", [0.8, 0.95, 1.0])
+@pytest.mark.parametrize("layers", [1, 2, 8, 32])
+@pytest.mark.parametrize("batch,ctx,step", [(64, 4096, 8192), (8, 130000, 8192), (256, 8192, 16), (1, 128, 128)])
+def test_pool_leaves_room_for_a_prefill_steps_blocks(monkeypatch, fraction, layers, batch, ctx, step):
+    """A prompt step holds the blocks that it reads as bf16, a layer at a time, beside the pool."""
+    from connex_b200.serve.__main__ import kv_blocks, model_args
+    ap = argparse.ArgumentParser()
+    model_args(ap)
+    cfg, free = LlamaConfig(max_pos=131072), 60 << 30
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a: (free, 0))
+
+    def blocks(dtype):
+        return kv_blocks(ap.parse_args(["--kv-dtype", dtype, "--kv-fraction", str(fraction), "--max-batch", str(batch),
+                                        "--max-ctx", str(ctx), "--max-step-tokens", str(step)]), cfg, 0, layers)
+    weights = 2 * (layers * (6144 * 4096 + 4096 * 4096 + 3 * 14336 * 4096) + 2 * 128256 * 4096)
+    room = free - weights - (2 << 30)
+    n, block = blocks("fp8"), 2 * layers * 8 * (BS * D + 4)
+    read = min(n, min(batch, step) * -(-ctx // BS))                  # of a step, at most
+    copy = 2 * 8 * BS * D * 2
+    assert n * block + read * copy <= room
+    more = n + 1                                                     # one block more would not fit, or pass the share
+    assert more * block > room * fraction or more * block + min(more, min(batch, step) * -(-ctx // BS)) * copy > room
+    assert blocks("bf16") == int(room * fraction) // (2 * layers * 8 * BS * D * 2)

@@ -461,12 +461,14 @@ class LlamaModel:
     def prefill(self, ids: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                 seq_lens: Sequence[int], last_rows: torch.Tensor, tile_info: torch.Tensor,
                 layer_hook: Optional[LayerHook] = None, hook_after_attention: bool = False,
-                block_tables: Optional[torch.Tensor] = None) -> torch.Tensor:
+                block_tables: Optional[torch.Tensor] = None, n_blocks: Optional[int] = None) -> torch.Tensor:
         """Prefill a packed batch; returns the greedy next token of each sequence.
 
         With an 8-bit cache the attention reads it: ``block_tables`` [B,
         max_blocks] is then needed, and ``tile_info`` from
-        ``prefill_tile_info(seq_lens, device, ctx)``.
+        ``prefill_tile_info(seq_lens, device, ctx)``; ``n_blocks``, the blocks
+        that the sequences have together, bounds the workspace (by default the
+        tables' size, as much as the longest sequence takes for each of them).
 
         ``layer_hook(l)`` runs (on the host, in stream order) right after layer
         l's K/V are in the paged cache: the PD path launches its push there.
@@ -490,7 +492,7 @@ class LlamaModel:
             if self.cache.scales is None:
                 ops.prefill_attention(qkv, tile_info, cfg.heads, cfg.kv_heads, out=self.attn[:T])
             else:
-                self._chunk_attention(l, q, block_tables, tile_info, self.attn[:T])
+                self._chunk_attention(l, q, block_tables, tile_info, self.attn[:T], n_blocks)
             if layer_hook is not None and hook_after_attention:
                 layer_hook(l)
             self._layer_tail(l, T)

@@ -536,3 +536,23 @@ def test_pool_leaves_room_for_a_prefill_steps_blocks(monkeypatch, fraction, laye
     more = n + 1                                                     # one block more would not fit, or pass the share
     assert more * block > room * fraction or more * block + min(more, min(batch, step) * -(-ctx // BS)) * copy > room
     assert blocks("bf16") == int(room * fraction) // (2 * layers * 8 * BS * D * 2)
+
+
+@pytest.mark.parametrize("n_blocks", [None, 7])
+def test_model_prefill_hands_on_the_blocks_it_reads(monkeypatch, n_blocks):
+    """Without the number the workspace is the tables' whole rectangle."""
+    from connex_b200.models.llama import LlamaModel, LlamaWeights
+    cfg = LlamaConfig.tiny(layers=1)
+    model = LlamaModel(LlamaWeights.random(cfg, "cpu"), PagedKVCache(cfg, 24, "cpu", torch.float8_e4m3fn), 64, 4)
+    for name in ("embedding", "rmsnorm", "gemm"):
+        monkeypatch.setattr(ops, name, lambda *a, **kw: None)
+    for name in ("_layer_tail", "_head"):
+        monkeypatch.setattr(model, name, lambda *a: None)
+    monkeypatch.setattr(model, "_rotate_and_cache", lambda i, qkv, *a: qkv)
+    seen = []
+    monkeypatch.setattr(ops, "prefill_attention_paged_fp8", lambda *a, **kw: seen.append(kw["n_blocks"]))
+    ids = torch.zeros(40, dtype=torch.int32)
+    kw = {} if n_blocks is None else {"n_blocks": n_blocks}
+    model.prefill(ids, ids, ids.long(), [8, 32], ids[:2], torch.zeros(2, 5, dtype=torch.int32),
+                  block_tables=torch.zeros(2, 20, dtype=torch.int32), **kw)
+    assert seen == [n_blocks]

@@ -722,6 +722,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rope_cache_fp8", &rope_cache_fp8);
   m.def("decode_fp8_rows", &decode_fp8_rows);
   m.attr("DECODE_FP8_ROW") = cx::DEC8_ROW;
+  m.def("decode_fp8_resident", &cx::decode_fp8_resident);
   m.def("decode_attention_fp8", &decode_attention_fp8);
   m.def("kv_copy_blocks", &kv_copy_blocks);
   m.def("prefill_fp8_words", &prefill_fp8_words);

@@ -460,7 +460,9 @@ void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_s
 namespace dec8 {
 // Two CTAs of eight warps took 99 us of 2 x 131072 (102 with four of four) and 32.5 of ragged lengths (34), but
 // 18.2 of 64 x 500 (15.2) and 9.5 of 64 x 16 (6.0): a pair's start and end wait for all the CTA's warps.
-constexpr int D = kvq::D, BS = kvq::BS, WARPS = 4, THREADS = 32 * WARPS, CTAS_PER_SM = 4;
+constexpr int D = kvq::D, BS = kvq::BS, WARPS = 4, THREADS = 32 * WARPS;
+// CTAs that an SM holds at a time, by the registers of the variant for nt tiles of query heads
+constexpr int ctas_per_sm(int nt) { return nt == 1 ? 4 : 3; }
 constexpr int MIN_UNITS = 2 * WARPS;    // blocks' worth of a CTA, at least (500 tokens alone: 6.6 us; 7.5 with 16)
 constexpr int PAIR_COST = 4 * WARPS;    // measured on ragged lengths: 41 us with 8, 34 with 16 and with 32
 constexpr int SLACK = 2 * PAIR_COST;    // see the work split above
@@ -500,7 +502,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // NT: tiles of 8 query heads per KV head (1: groups up to 8, 2: up to 16).
 template <int NT>
-__global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
+__global__ void __launch_bounds__(dec8::THREADS, dec8::ctas_per_sm(NT))
     decode_attn_fp8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, KvFp8 c, const int* __restrict__ tables,
                            int max_blocks, const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, int ldo,
                            int B, int Hq, float scale_log2, float* __restrict__ part, uint32_t* __restrict__ counters,
@@ -969,7 +971,17 @@ __global__ void __launch_bounds__(dec8::THREADS, NT == 1 ? 4 : 3)
   }
 }
 
-int decode_fp8_ctas(int sms) { return sms * dec8::CTAS_PER_SM; }
+int decode_fp8_ctas(int sms) { return sms * dec8::ctas_per_sm(1); }
+// The shares are equal, so one more CTA than an SM holds would run a whole share after the others: the
+// grid counts what fits, by registers and beside the prefix sums (four up to about 1400 sequences, then
+// three).  64 x 4096 tokens of 128/8 heads take 103 us, 131 with four CTAs' shares on an SM; of 16/1 heads
+// 25 and 41; 2000 x 128 of 32/8 heads 163 and 205, 4096 x 64 of 8/2 heads 89 and 119.
+int decode_fp8_resident(int B, int G) {
+  const int nt = G > 8 ? 2 : 1;
+  const int smem = nt == 2 ? dec8::Smem<2>::bytes(B) : dec8::Smem<1>::bytes(B);
+  constexpr int PER_SM = 228 * 1024, OTHER = 1024 + 256;      // of a CTA: the system's, and the static variables
+  return std::min(dec8::ctas_per_sm(nt), PER_SM / (smem + OTHER));
+}
 long decode_fp8_rows(int sms, int B, int Hkv, int G) {
   const long row = (long)G * DEC8_ROW;
   return 2L * decode_fp8_ctas(sms) + ((long)B * Hkv + row - 1) / row;
@@ -981,11 +993,12 @@ void decode_attention_fp8(const void* q, int ldq, const KvFp8& c, const int* blo
   if (B == 0) return;
   const int G = Hq / c.Hkv;
   const int ctas = decode_fp8_ctas(sms);
-  // the partial results sit at the front, the counters behind them: neither moves with the batch
+  // the partial results (room for the largest grid) sit at the front, the counters behind them: neither
+  // moves with the batch
   uint32_t* counters = reinterpret_cast<uint32_t*>(ws + 2L * ctas * G * DEC8_ROW);
   const int nt = G > 8 ? 2 : 1;
   const long most = ((long)B * c.Hkv * (max_blocks + dec8::PAIR_COST) + dec8::MIN_UNITS - 1) / dec8::MIN_UNITS;
-  const int grid = (int)std::max(1L, std::min((long)ctas, most));
+  const int grid = (int)std::max(1L, std::min((long)sms * decode_fp8_resident(B, G), most));
   const int smem = nt == 2 ? dec8::Smem<2>::bytes(B) : dec8::Smem<1>::bytes(B);
   auto kern = nt == 2 ? decode_attn_fp8_kernel<2> : decode_attn_fp8_kernel<1>;
   static bool attr[64][2] = {};

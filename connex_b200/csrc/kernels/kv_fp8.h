@@ -32,7 +32,8 @@ constexpr int KVQ_MAX_ROWS = 8192;
 // (each call leaves its counters zero).
 constexpr int DEC8_ROW = 132;        // floats of one head's partial result
 constexpr int DEC8_MAX_BATCH = 4096;
-int decode_fp8_ctas(int sms);
+int decode_fp8_ctas(int sms);                // of a call, at most
+int decode_fp8_resident(int B, int G);       // that an SM holds at a time in a call of B sequences
 long decode_fp8_rows(int sms, int B, int Hkv, int G);
 void decode_attention_fp8(const void* q, int ldq, const KvFp8& c, const int* block_tables, int max_blocks,
                           const int* ctx_lens, void* out, int ldo, int B, int Hq, float scale, float* ws, long ws_rows,

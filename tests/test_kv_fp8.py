@@ -556,3 +556,11 @@ def test_model_prefill_hands_on_the_blocks_it_reads(monkeypatch, n_blocks):
     model.prefill(ids, ids, ids.long(), [8, 32], ids[:2], torch.zeros(2, 5, dtype=torch.int32),
                   block_tables=torch.zeros(2, 20, dtype=torch.int32), **kw)
     assert seen == [n_blocks]
+
+
+@pytest.mark.parametrize("heads,fit", [(1, 4), (4, 4), (8, 4), (9, 3), (10, 3), (16, 3)])
+def test_decode_plans_for_the_ctas_that_an_sm_holds(heads, fit):
+    """Query heads per KV head past 8 take three CTAs' registers, and the lengths of some 1400 sequences
+    the fourth one's shared memory (228 KB of an SM, one of them the system's for each CTA)."""
+    per_sm = [ops._C.decode_fp8_resident(B, heads) for B in (1, 64, 1300, 1500, 4096)]
+    assert per_sm == [fit, fit, fit, 3, 3]

@@ -116,6 +116,34 @@ def test_decode_attention(dev, heads, lens):
     assert torch.equal(again.view(torch.int16), out.view(torch.int16))
 
 
+@pytest.mark.parametrize("heads", [(4, 1), (20, 2)])
+def test_decode_of_many_sequences(dev, heads):
+    """Up to the most sequences of a call, next to calls of a few with the same workspace: the grid depends on
+    their number, the workspace's layout does not."""
+    from connex_b200 import ops
+    from connex_b200.ops import reference as R
+    hq, hkv = heads
+    ws = ops.decode_workspace_fp8(4096, hq, hkv, dev)
+    for seed, lens in enumerate(([i % 70 for i in range(4096)], [3000, 1, 900], [200 + i % 90 for i in range(1450)], [5000])):
+        table, nb = _table(lens, dev, 131 + seed)
+        k, ks = _cache(nb, hkv, dev, 141 + seed)
+        v, vs = _cache(nb, hkv, dev, 151 + seed)
+        q = (torch.randn(len(lens), hq * D, generator=_g(dev, 161 + seed), device=dev) * 1.5).to(torch.bfloat16)
+        lt = torch.tensor(lens, dtype=torch.int32, device=dev)
+        st = ops.new_status(dev)
+        out = ops.decode_attention_fp8(q, k, v, ks, vs, table, lt, hq, ws, status=st)
+        ops.check_status(st)
+        live = [b for b, n in enumerate(lens) if n]
+        assert not out[[b for b, n in enumerate(lens) if not n]].any()
+        ctx, ones = [lens[b] - 1 for b in live], [1] * len(live)
+        rows, tl = q[live].view(-1, hq, D), table[live]
+        ref, mag = R.paged_attention_fp8(rows, k, v, ks, vs, tl, ctx, ones)
+        tol = _attention_tolerance(ref, mag, rows, k, ks, tl, ctx, ones, U_F16, float(vs.max()) * 448)
+        assert ((out[live].view(-1, hq, D).double() - ref).abs() <= tol).all()
+        again = ops.decode_attention_fp8(q, k, v, ks, vs, table, lt, hq, ws)
+        assert torch.equal(again.view(torch.int16), out.view(torch.int16))
+
+
 PREFILL_ROWS = [[(0, 100)], [(64, 128)], [(1000, 300), (17, 5)], [(2000, 1), (130, 513)], [(5, 64), (0, 200), (3999, 129)],
                 [(2048, 600)], [(7, 9), (0, 1), (15, 1), (16, 1)], [(300, 0), (41, 30)], [(12000, 33), (500, 257)]]
 

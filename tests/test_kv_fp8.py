@@ -564,3 +564,32 @@ def test_decode_plans_for_the_ctas_that_an_sm_holds(heads, fit):
     the fourth one's shared memory (228 KB of an SM, one of them the system's for each CTA)."""
     per_sm = [ops._C.decode_fp8_resident(B, heads) for B in (1, 64, 1300, 1500, 4096)]
     assert per_sm == [fit, fit, fit, 3, 3]
+
+
+def test_every_stage_takes_the_cache_type_from_the_command_line(monkeypatch):
+    """``--kv-dtype`` of a later pipeline stage reaches its runtime and its pool's size."""
+    from connex_b200.models import hf  # noqa: F401
+    from connex_b200.runtime import pp
+    from connex_b200.serve import __main__ as m, stage
+    ap = argparse.ArgumentParser()
+    m.model_args(ap)
+    seen = {}
+
+    class Stop(Exception):
+        pass
+
+    def runtime(cfg, l0, l1, dev, **kw):
+        seen.update(kw, layers=(l0, l1))
+        raise Stop
+    monkeypatch.setattr(torch.cuda, "set_device", lambda d: None)
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a: (60 << 30, 0))
+    monkeypatch.setattr(pp, "StageRuntime", runtime)
+    blocks = {}
+    for given, dtype in (("bf16", torch.bfloat16), ("fp8", torch.float8_e4m3fn)):
+        a = ap.parse_args(["--num-stages", "2", "--kv-dtype", given])
+        a.stage, a.rule = 1, False
+        with pytest.raises(Stop):
+            stage.run_stage(a, None)
+        assert seen["kv_dtype"] == dtype and seen["layers"] == (16, 32)
+        blocks[given] = seen["num_blocks"]
+    assert 1.99 < blocks["fp8"] / blocks["bf16"] <= 2.0

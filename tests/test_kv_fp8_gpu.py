@@ -808,6 +808,60 @@ def test_model_stepper_8_bit(dev):
     st.release(["p", "q"])
 
 
+def test_qwen3_moe_rank_8_bit(dev):
+    """Decode steps with q/k norms: layer 0 holds the bf16 cache's rows to half an e4m3 step (its input does not
+    depend on the cache), and each step's attention is that of the cache it left."""
+    from connex_b200 import ops
+    from connex_b200.models.qwen3_moe import Qwen3MoeConfig, Qwen3MoeRank
+    from connex_b200.ops import reference as R
+
+    class NoExperts:
+        def forward(self, h, idx, w, l2p, cnt, out):
+            return out.zero_()
+    cfg, B, steps = Qwen3MoeConfig.tiny(), 3, 37
+    lens0 = [0, 5, 16]
+    width = 4
+    table = torch.randperm(B * width, generator=_g(dev, 171), device=dev).to(torch.int32).view(B, width)
+    ids = torch.randint(3, 1000, (steps, B), generator=_g(dev, 172), device=dev).to(torch.int32)
+    none = [(None, None)] * cfg.layers
+    models = {}
+    for dtype in (torch.bfloat16, torch.float8_e4m3fn):
+        m = models[dtype] = Qwen3MoeRank(cfg, 0, 1, [[-1]] * cfg.layers, dev, B * width, B, kv_dtype=dtype)
+        m.moe = NoExperts()
+        for a in m.attn:
+            a.q_norm.uniform_(0.5, 1.5, generator=_g(dev, 173))
+            a.k_norm.uniform_(0.5, 1.5, generator=_g(dev, 174))
+        # rows before the first step: zeros in both
+        m.cache.kv.view(torch.int16 if dtype == torch.bfloat16 else torch.uint8).zero_()
+        ws = (ops.decode_workspace(B, cfg.heads, width * BS, dev) if dtype == torch.bfloat16
+              else ops.decode_workspace_fp8(B, cfg.heads, cfg.kv_heads, dev))
+        for t in range(steps):
+            pos = torch.tensor([n + t for n in lens0], dtype=torch.int32, device=dev)
+            slots = table.gather(1, (pos.long() // BS)[:, None])[:, 0].long() * BS + pos.long() % BS
+            m.decode(ids[t], pos, slots, table, pos + 1, width * BS, ws, none, none, none)
+            if dtype == torch.float8_e4m3fn and t % 9 == 0:
+                c, l = m.cache, cfg.layers - 1
+                q = m.qkv[:, :cfg.heads * D].reshape(B, cfg.heads, D)
+                ctx = [n + t for n in lens0]
+                args = (c.k(l), c.v(l), c.k_scale(l), c.v_scale(l), table, ctx, [1] * B)
+                ref, mag = R.paged_attention_fp8(q, *args)
+                tol = _attention_tolerance(ref, mag, q, c.k(l), c.k_scale(l), table, ctx, [1] * B, U_F16,
+                                           float(c.v_scale(l).max()) * 448)
+                assert ((m.att.view(B, cfg.heads, D).double() - ref).abs() <= tol).all()
+        ops.check_status(m.status)
+    a, b = models[torch.bfloat16].cache, models[torch.float8_e4m3fn].cache
+    for x, y, s, turned in ((a.k(0), b.k(0), b.k_scale(0), True), (a.v(0), b.v(0), b.v_scale(0), False)):
+        x = x.double()
+        # K: both writes round the normed pair to bf16, each to 2^-8 of it, and the rotated elements again; the
+        # pair's two magnitudes add up to at most sqrt(2) of its length
+        pair = torch.hypot(x[..., :D // 2], x[..., D // 2:]).repeat(1, 1, 1, 2) * math.sqrt(2) * (1 + 2 * U_BF16)
+        d = 2 * U_BF16 * (x.abs() + pair) if turned else torch.zeros_like(x)
+        # a row is rounded when it arrives and once more for each later growth of its block's scale, each of
+        # which at least doubles it: halves of the smallest step, 2^-10 (1 + 1/2 + 1/4 + ..) of the last scale
+        bound = d + U_E4M3 * (x.abs() + d) + 2 * 2.0 ** -10 * s.double()[..., None, None]
+        assert ((R.fp8_values(y, s) - x).abs() <= bound).all()
+
+
 def test_push_moves_an_8_bit_cache_in_two_calls(dev):
     """kv_push_layer takes the values by head slices of 2 KB and the scales as one 16-byte unit per block."""
     from connex_b200 import ops

@@ -1049,6 +1049,7 @@ __global__ void __maxnreg__(fap::LAUNCH_REGS)
               }
             }
             tc_fence_before();                       // as below
+            if (rec) t_e += clock64() - te0;
             kv += it.nkv;
             continue;
           }
@@ -1137,18 +1138,18 @@ static void launch_attn(const AttnArgs& a, cudaStream_t s) {
       a.scale_log2, a.bt, a.bt_stride, a.status, PAIR ? g_attn_prof : nullptr, a.plan);
 }
 
-template <bool PAIR, bool PAGED>
+template <bool PAIR, bool PAGED, bool SPLIT = false>
 static void launch_attn_split(const AttnArgs& a, cudaStream_t s) {
   if (PAIR && g_attn_prof != nullptr)
-    launch_attn<PAIR, PAGED, 0, true>(a, s);
+    launch_attn<PAIR, PAGED, 0, true, SPLIT>(a, s);
   else if (g_exp_split == 1 && PAIR)
-    launch_attn<PAIR, PAGED, 1>(a, s);
+    launch_attn<PAIR, PAGED, 1, false, SPLIT>(a, s);
   else if (g_exp_split == 2)
-    launch_attn<PAIR, PAGED, 2>(a, s);
+    launch_attn<PAIR, PAGED, 2, false, SPLIT>(a, s);
   else if (g_exp_split == 4)
-    launch_attn<PAIR, PAGED, 4>(a, s);
+    launch_attn<PAIR, PAGED, 4, false, SPLIT>(a, s);
   else
-    launch_attn<PAIR, PAGED, 0>(a, s);
+    launch_attn<PAIR, PAGED, 0, false, SPLIT>(a, s);
 }
 
 void prefill_attention_tc(const void* qkv, int ldq, int qkv_cols, int T, void* out, int ldo, const int* tile_info,
@@ -1198,7 +1199,7 @@ void prefill_attention_paged_tc(const void* qkv, int ldq, int qkv_cols, int T, c
     a.plan = *plan;
     const uint32_t heads = 1u << plan->pack;
     a.tq = make_tmap_bf16_3d(qkv, 128, (uint64_t)Hq, (uint64_t)T, 256, (uint64_t)ldq * 2, 64, heads, 128 / heads);
-    launch_attn<true, true, 0, false, true>(a, s);
+    launch_attn_split<true, true, true>(a, s);
   } else if (tile_rows == fap::ROWS)
     launch_attn_split<true, true>(a, s);
   else

@@ -174,6 +174,68 @@ def test_prefill_attention(dev, heads, rows):
     assert (err <= tol).all(), float((err / tol).max())
 
 
+@pytest.mark.parametrize("mode", [1, 2, 4])
+@pytest.mark.parametrize("rows", [[(12000, 33), (500, 257)], [(2048, 600)]])
+def test_prefill_with_other_exponentials(dev, mode, rows):
+    """attention_exp_split holds for this attention, too: other bits, within the mode's own error."""
+    from connex_b200 import ops
+    from connex_b200.ops import reference as R
+    hq, hkv = 8, 2
+    ctx, new = [c for c, _ in rows], [n for _, n in rows]
+    table, nb = _table([c + n for c, n in rows], dev, 181)
+    k, ks = _cache(nb, hkv, dev, 182)
+    v, vs = _cache(nb, hkv, dev, 183, -10, -2)
+    q = (torch.randn(sum(new), hq * D, generator=_g(dev, 184), device=dev) * 0.25).to(torch.bfloat16)
+    ti = ops.prefill_tile_info(new, dev, ctx=ctx)
+    st = ops.new_status(dev)
+    plain = ops.prefill_attention_paged_fp8(q, k, v, ks, vs, table, ti, hq, hkv, status=st)
+    try:
+        ops._C.attention_exp_split(mode)
+        out = ops.prefill_attention_paged_fp8(q, k, v, ks, vs, table, ti, hq, hkv, status=st)
+        torch.cuda.synchronize()
+    finally:
+        ops._C.attention_exp_split(0)
+    ops.check_status(st)
+    assert not torch.equal(out.view(torch.int16), plain.view(torch.int16))
+    q3 = q.view(-1, hq, D)
+    ref, mag = R.paged_attention_fp8(q3, k, v, ks, vs, table, ctx, new)
+    # a weight's relative error: its rounding to bf16 and the cubic's 7.5e-5 (1e-4 with its own fp32 roundings); or
+    # 2^-7 of the packed instruction and an exponent rounded to bf16, 2^-8 of its size, which is at most twice the
+    # largest logit in base 2 and 8 for the late rescale
+    if mode == 1:
+        norms = (R.fp8_values(k.view(torch.uint8).view(k.dtype), ks).square().sum(-1).sqrt().max().item()
+                 * q3.double().square().sum(-1).sqrt().max().item())
+        u = 2.0 ** -7 + U_BF16 * math.log(2) * (2 * norms / math.sqrt(D) / math.log(2) + 8)
+    else:
+        u = U_BF16 + 1e-4
+    tol = _attention_tolerance(ref, mag, q3, k, ks, table, ctx, new, u, float(vs.max()) * 448)
+    assert ((out.view(-1, hq, D).double() - ref).abs() <= tol).all()
+
+
+def test_prefill_profile(dev):
+    """attention_profile's counters are filled by this attention, too, and its result is the same."""
+    from connex_b200 import ops
+    hq, hkv = 8, 2
+    table, nb = _table([2148], dev, 191)
+    k, ks = _cache(nb, hkv, dev, 192)
+    v, vs = _cache(nb, hkv, dev, 193)
+    q = torch.randn(300, hq * D, generator=_g(dev, 194), device=dev).to(torch.bfloat16)
+    ti = ops.prefill_tile_info([300], dev, ctx=[1848])
+    plain = ops.prefill_attention_paged_fp8(q, k, v, ks, vs, table, ti, hq, hkv)
+    sms = torch.cuda.get_device_properties(dev).multi_processor_count
+    buf = torch.zeros(sms, 16, dtype=torch.int64, device=dev)
+    ops._C.attention_profile(buf.data_ptr())
+    try:
+        out = ops.prefill_attention_paged_fp8(q, k, v, ks, vs, table, ti, hq, hkv)
+        torch.cuda.synchronize()
+    finally:
+        ops._C.attention_profile(0)
+    assert torch.equal(out.view(torch.int16), plain.view(torch.int16))
+    # CTAs with work: the MMA thread's total, both softmax warpgroups' waits, work and epilogues
+    busy = buf[buf[:, 5] > 0]
+    assert busy.shape[0] > 0 and (busy[:, 6:14].sum(0) > 0).all()
+
+
 @pytest.mark.parametrize("heads", [(128, 1), (12, 1), (40, 8)])
 def test_prefill_other_groups(dev, heads):
     """Groups of which all, some or none of the heads share a tile's rows."""

@@ -10,7 +10,9 @@ capture of the case runs.
 
 Cases: gemm (8192^3), gemm_qkv (T=8192 Llama-3-8B QKV), gemm_silu (T=8192
 gate/up + SiLU-mul), attn (8 x 2048-token causal prefill, 32/8 heads),
-attn_paged (the paged variant: 8 chunks of 2048 queries over 2048 cached tokens), decode_attn (64 x 4096-token paged decode), attn_paged_fp8 and decode_attn_fp8 (the same over the 8-bit cache), kv_push (one layer of a 64k-token
+attn_paged (the paged variant: 8 chunks of 2048 queries over 2048 cached tokens), decode_attn (64 x 4096-token paged decode), attn_paged_fp8 and decode_attn_fp8 (the same over the 8-bit cache), write_fp8 and write_fp8_rows
+(its quantising write: 4 x 2048 prompt rows, 64 rows of as many sequences), kv_copy_blocks (400 of its blocks in 32
+layers), kv_push (one layer of a 64k-token
 KV push, local), kv_push_nvlink (the same layer pushed from GPU 0 into GPU 1's
 memory over NVLink, one process, peer access; ``--ctas`` sets the grid,
 ``--pull`` runs the kernel on GPU 1 reading GPU 0's memory instead, ``--ce``
@@ -165,6 +167,30 @@ def case_decode_attn_fp8(dev, B=64, ctx=4096, hq=32, hkv=8):
     st = ops.new_status(dev)
     return (lambda: ops.decode_attention_fp8(q, k, v, ks, vs, bt, cl, hq, ws, out, status=st)), {
         "bytes": 2 * k.numel() + 8 * ks.numel(), "check": _status_check(st, "8-bit decode attention")}
+
+
+def case_write_fp8(dev, T=8192, per=2048, hq=32, hkv=8):
+    """RoPE and quantising write of T / per prompts' rows (``per`` 1: one row per sequence, inside a block)."""
+    nb = T if per == 1 else T // 16
+    (k, ks), (v, vs) = _fp8_cache(dev, nb, hkv), _fp8_cache(dev, nb, hkv)
+    qkv = torch.randn(T, (hq + 2 * hkv) * 128, device=dev).bfloat16()
+    pos = (torch.arange(T, device=dev) % per + (1000 if per == 1 else 0)).to(torch.int32)
+    slots = torch.randperm(nb, device=dev) * 16 + 8 if per == 1 else torch.arange(T, device=dev)
+    cs = ops.rope_cos_sin(4096, 128, 5e5, dev)
+    out = torch.empty(T, hq * 128, dtype=torch.bfloat16, device=dev)
+    st = ops.new_status(dev)
+    return (lambda: ops.rope_cache_fp8(qkv, pos, cs, hq, hkv, slots, k, v, ks, vs, out, st)), {
+        "bytes": T * ((2 * hq + 2 * hkv) * 256 + 2 * hkv * 128), "check": _status_check(st, "8-bit cache write")}
+
+
+def case_kv_copy_blocks(dev, n=400, layers=32, nb=1024, hkv=8):
+    """n blocks of every layer of an 8-bit cache, with their scales."""
+    kv = torch.randint(0, 120, (layers, 2, nb, hkv, 16, 128), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+    sc = torch.ones(layers, 2, nb, hkv, device=dev)
+    pairs = torch.randperm(nb, device=dev)[:2 * n].to(torch.int32).view(n, 2)
+    st = ops.new_status(dev)
+    return (lambda: ops.kv_copy_blocks(kv, pairs, sc, st)), {
+        "bytes": 2 * n * layers * 2 * hkv * (16 * 128 + 4), "check": _status_check(st, "block copies")}
 
 
 def case_kv_push(dev, tokens=65536, hkv=8):
@@ -342,7 +368,8 @@ CASES = {"gemm": lambda d: case_gemm(d), "gemm_qkv": lambda d: case_gemm(d, 8192
          "attn_cudnn_2x8192": lambda d: case_attn_library(d, "cudnn", n_seq=2, L=8192), "attn_cudnn": lambda d: case_attn_library(d, "cudnn"),
          "attn_torch_flash": lambda d: case_attn_library(d, "flash"),
          "decode_attn": case_decode_attn, "decode_attn_fp8": case_decode_attn_fp8,
-         "attn_paged_fp8": case_attn_paged_fp8, "kv_push": case_kv_push, "wsync": case_wsync, "ep_gemm": case_ep_gemm,
+         "attn_paged_fp8": case_attn_paged_fp8, "write_fp8": case_write_fp8,
+         "write_fp8_rows": lambda d: case_write_fp8(d, 64, 1), "kv_copy_blocks": case_kv_copy_blocks, "kv_push": case_kv_push, "wsync": case_wsync, "ep_gemm": case_ep_gemm,
          "ep_t128": lambda d: case_ep_gemm(d, 128),
          "gemm_m1_qkv": lambda d: case_gemm_m(d, 1, 6144, 4096), "gemm_m1_o": lambda d: case_gemm_m(d, 1, 4096, 4096),
          "gemm_m1_gateup": lambda d: case_gemm_m(d, 1, 28672, 4096, silu=True),

@@ -114,9 +114,11 @@ struct alignas(16) f32x4 {        // two pairs of fp32
 // of blocks, every 16th token of a prompt, then spread over all of them, and
 // so do the rows of decode steps.  Rotation CTAs take the q heads, eight of a
 // token per warp at a time.
-// 8192 rows of 32/8 heads take 43 us: rotating q alone 25 (134 MB at 5.3
+// 8192 rows of 32/8 heads take 42 us: rotating q alone 25 (134 MB at 5.3
 // TB/s), and on the same SMs the scans 6, the blocks' stores 3.5 and their
-// arithmetic 4.
+// arithmetic 4.  A bf16 cache's write takes 65.  One row each of many
+// sequences is a block CTA and a scan per row: 4.4, 6.3, 18.6 and 75 us for
+// 64, 256, 1024 and 4096 rows, where the bf16 write takes 2.4, 3.5, 8.3 and 27.
 __device__ __forceinline__ void write_block(const __nv_bfloat16* qkv, int ldq, const int* pos, const float* cos_sin,
                                             const int64_t* slots, const KvFp8& c, int t, int blk, int group, int T,
                                             int Hq, int max_pos, const __nv_bfloat16* kn, float eps) {
@@ -423,11 +425,10 @@ void rope_cache_fp8(const void* qkv, int ldq, const int* pos, const float* cos_s
 // S = q.K^T and O^T = V^T.W^T on mma.sync m16n8k16 (f16 in, fp32 out).  The
 // cached bytes are turned into f16 (exact) in registers, in the fragments'
 // layout as they come from the cache; the block scales stay out of the
-// operands.  (mma.sync takes e4m3 operands too, but on this GPU it converts
-// both of them at every instruction: 17 instructions and 30 cycles of an SM
-// quarter for one m16n8k32, where two f16 ones take 16 cycles and q needs no
-// conversion at all; 64 x 4096 took 103 us with them, 101 with f16, ragged
-// lengths 38 and 34.)
+// operands.  (mma.sync takes e4m3 operands too.  With them the kernel executed
+// 61 million warp instructions at 64 x 4096, with f16 ones 43 million, and q,
+// made f16 once, has to be converted no further: 103 us with e4m3, 101 with
+// f16, ragged lengths 38 and 34.)
 //   K: lane (g = lane / 4, c = lane % 4) takes bytes [16 c, 16 c + 16) of both
 //      64-byte halves of tokens g and g + 8.  The contraction may take the
 //      dims in any order as long as q uses the same one, so each word of a
@@ -1107,7 +1108,7 @@ void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes
 // CUT_SLACK of an item's start or end moves there.  Against one item per CTA at a time, the conversion
 // not counted in the latter: 256 rows at 7936 60 and 121 us, 2 x 256 at 32256
 // 263 and 465, 2048 rows at 6144 201 and 211; eight prompts of 2048, whose items
-// balance by themselves, 294 and 279.
+// balance by themselves, 295 and 271: there the cuts only cost.
 namespace kvd {
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int ROWS = 256, KEYS = 128;                   // of a tile of the attention

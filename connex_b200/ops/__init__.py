@@ -291,7 +291,9 @@ def rope_cache_fp8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Te
     NaN.  A row with slot < 0 is not cached; one with a position or slot out
     of range is not cached either and recorded in ``status`` (a position out
     of range also gives a q of zeros).  Of two rows for the same slot the
-    later wins.  More than 8192 rows run as successive calls of 8192.
+    later wins.  More than 8192 rows run as successive calls of 8192: a row 0
+    that comes in a later one starts its block anew, so give a block's rows
+    in rising order there.
     ``q_norm`` / ``k_norm`` as in :func:`rope_cache`."""
     if out is None:
         out = torch.empty(qkv.shape[0], n_q_heads * 128, dtype=qkv.dtype, device=qkv.device)
@@ -325,7 +327,9 @@ def decode_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     :func:`rope_cache_fp8`; scales must be powers of two), up to 16 query
     heads per KV head.  ``q`` [B, >= Hq * 128] (q heads first), ``ctx_lens``
     [B] tokens to attend to (0: a row of zeros), ``block_tables``
-    [B, max_blocks].  The work is divided on the device from ``ctx_lens``, so
+    [B, max_blocks].  The weights are held in f16 (2^-11 of each) next to
+    fp32 sums; of a scale of V that is no power of two only the power of two
+    below it counts.  The work is divided on the device from ``ctx_lens``, so
     a captured call stays balanced for any lengths.  A block id out of range
     is left out, and a length beyond the table cut, both recorded in
     ``status``."""
@@ -346,10 +350,13 @@ def prefill_attention_paged_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache:
     prompt chunks, ``q`` [T, >= Hq * 128] rotated (q heads first), keys and
     values of the whole context -- this chunk's included -- from the cache.
     ``tile_info`` from ``prefill_tile_info(n_new, device, ctx)``.  The blocks
-    that the chunks read are turned into bf16 first (exact: the scales are
-    powers of two), in a workspace of ``n_blocks`` blocks: a bound on those
-    of all the sequences together, by default the tables' size.  ``scale``
-    must be positive.  The work is divided on the device
+    that the chunks read are turned into bf16 first (exact where the scales
+    are powers of two, as :func:`rope_cache_fp8` leaves them), in a workspace
+    of ``n_blocks`` blocks: a bound on those of all the sequences together
+    (one that several sequences share counts for each), by default the tables'
+    size.  ``scale`` must be positive.  The softmax's weights are rounded to
+    bf16 for the product with V (2^-8 of each, as over a bf16 cache); sums and
+    maxima are fp32.  The work is divided on the device
     in equal shares of the keys, so few rows over a long context use every SM
     (another 39 MB of workspace).  Entries behind a sequence's end
     are not read.  A block id out of range reads as zeros, and a tile that

@@ -14,7 +14,9 @@
 
 #include "comm.h"
 #include "gemm.h"
+#include "gemm_fp8.h"
 #include "kv_fp8.h"
+#include "kv_int4.h"
 #include "layers.h"
 #include "moe.h"
 
@@ -274,49 +276,82 @@ cx::KvFp8 fp8_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& 
                    vs.data_ptr<float>(), (int)k.size(0), (int)k.size(1)};
 }
 
-void rope_cache_fp8(const at::Tensor& qkv, const at::Tensor& pos, const at::Tensor& cos_sin, const at::Tensor& slots,
-                    const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
-                    at::Tensor& out, int64_t Hq, int64_t Hkv, const c10::optional<at::Tensor>& status,
-                    const c10::optional<at::Tensor>& q_norm, const c10::optional<at::Tensor>& k_norm, double eps) {
-  check_same_device(qkv, {&pos, &cos_sin, &slots, &kc, &out}, "rope_cache_fp8");
-  check_status_device(qkv, status, "rope_cache_fp8");
-  const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "rope_cache_fp8");
-  const int ldq = row_ld16(qkv, "rope_cache_fp8: qkv"), ldo = row_ld16(out, "rope_cache_fp8: out");
+// What the quantising writes ask of their rows.
+struct RopeRows {
+  int ldq, ldo, max_pos;
+  const void *qn, *kn;
+};
+RopeRows rope_rows(const std::string& what, const at::Tensor& qkv, const at::Tensor& pos, const at::Tensor& cos_sin,
+                   const at::Tensor& slots, const at::Tensor& kc, const at::Tensor& out, int64_t Hq, int64_t Hkv,
+                   const c10::optional<at::Tensor>& q_norm, const c10::optional<at::Tensor>& k_norm) {
+  RopeRows r{};
+  r.ldq = row_ld16(qkv, (what + ": qkv").c_str());
+  r.ldo = row_ld16(out, (what + ": out").c_str());
   const int64_t T = qkv.size(0);
   TORCH_CHECK(Hq > 0 && Hkv == kc.size(1) && qkv.size(1) == (Hq + 2 * Hkv) * 128,
-              "rope_cache_fp8: qkv must hold exactly (Hq + 2 Hkv) heads of 128, Hkv as in the cache");
-  TORCH_CHECK(out.size(0) == T && out.size(1) == Hq * 128, "rope_cache_fp8: out must be [T, Hq * 128]");
-  TORCH_CHECK(T <= INT_MAX, "rope_cache_fp8: too many rows");
+              what, ": qkv must hold exactly (Hq + 2 Hkv) heads of 128, Hkv as in the cache");
+  TORCH_CHECK(out.size(0) == T && out.size(1) == Hq * 128, what, ": out must be [T, Hq * 128]");
+  TORCH_CHECK(T <= INT_MAX, what, ": too many rows");
   TORCH_CHECK(pos.scalar_type() == at::kInt && pos.is_contiguous() && pos.numel() == T,
-              "rope_cache_fp8: positions must be contiguous int32 [T]");
+              what, ": positions must be contiguous int32 [T]");
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.numel() == T,
-              "rope_cache_fp8: slot_mapping must be contiguous int64 [T]");
+              what, ": slot_mapping must be contiguous int64 [T]");
   TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.dim() == 2 && cos_sin.size(1) == 128 &&
                   cos_sin.is_contiguous() && (reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) & 15) == 0,
-              "rope_cache_fp8: cos_sin must be contiguous fp32 [positions, 128]");
-  const void *qn = nullptr, *kn = nullptr;
+              what, ": cos_sin must be contiguous fp32 [positions, 128]");
   for (const auto* w : {&q_norm, &k_norm})
     if (w->has_value())
       TORCH_CHECK((*w)->device() == qkv.device() && (*w)->scalar_type() == at::kBFloat16 && (*w)->numel() == 128 &&
                       (*w)->is_contiguous() && (reinterpret_cast<uintptr_t>((*w)->data_ptr()) & 15) == 0,
-                  "rope_cache_fp8: q/k norm weights must be contiguous bf16 CUDA [128]");
-  if (q_norm.has_value()) qn = q_norm->data_ptr();
-  if (k_norm.has_value()) kn = k_norm->data_ptr();
+                  what, ": q/k norm weights must be contiguous bf16 CUDA [128]");
+  if (q_norm.has_value()) r.qn = q_norm->data_ptr();
+  if (k_norm.has_value()) r.kn = k_norm->data_ptr();
   // q is rotated by the block that reads it: out may be qkv's own q columns, but no other part of it
   if (T > 0) {
     const char* a = static_cast<const char*>(qkv.data_ptr());
     const char* b = static_cast<const char*>(out.data_ptr());
-    const char* a1 = a + ((T - 1) * (int64_t)ldq + qkv.size(1)) * 2;
-    const char* b1 = b + ((T - 1) * (int64_t)ldo + out.size(1)) * 2;
-    TORCH_CHECK(b1 <= a || a1 <= b || (a == b && (ldq == ldo || T == 1)),
-                "rope_cache_fp8: out overlaps qkv other than as its q columns");
+    const char* a1 = a + ((T - 1) * (int64_t)r.ldq + qkv.size(1)) * 2;
+    const char* b1 = b + ((T - 1) * (int64_t)r.ldo + out.size(1)) * 2;
+    TORCH_CHECK(b1 <= a || a1 <= b || (a == b && (r.ldq == r.ldo || T == 1)),
+                what, ": out overlaps qkv other than as its q columns");
   }
+  r.max_pos = (int)std::min<int64_t>(cos_sin.size(0), INT_MAX);
+  return r;
+}
+
+void rope_cache_fp8(const at::Tensor& qkv, const at::Tensor& pos, const at::Tensor& cos_sin, const at::Tensor& slots,
+                    const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
+                    at::Tensor& out, int64_t Hq, int64_t Hkv, const c10::optional<at::Tensor>& status,
+                    const c10::optional<at::Tensor>& q_norm, const c10::optional<at::Tensor>& k_norm, double eps) {
+  const char* what = "rope_cache_fp8";
+  check_same_device(qkv, {&pos, &cos_sin, &slots, &kc, &out}, what);
+  check_status_device(qkv, status, what);
+  const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, what);
+  const RopeRows r = rope_rows(what, qkv, pos, cos_sin, slots, kc, out, Hq, Hkv, q_norm, k_norm);
   CHECK_CUDA(qkv);
   const c10::cuda::CUDAGuard g(qkv.device());
-  cx::rope_cache_fp8(qkv.data_ptr(), ldq, pos.data_ptr<int>(), cos_sin.data_ptr<float>(), slots.data_ptr<int64_t>(), c,
-                     out.data_ptr(), ldo, (int)T, (int)Hq, (int)std::min<int64_t>(cos_sin.size(0), INT_MAX), sms_of(qkv),
-                     status_ptr(status), cur_stream(qkv), qn, kn, (float)eps);
+  cx::rope_cache_fp8(qkv.data_ptr(), r.ldq, pos.data_ptr<int>(), cos_sin.data_ptr<float>(), slots.data_ptr<int64_t>(), c,
+                     out.data_ptr(), r.ldo, (int)qkv.size(0), (int)Hq, r.max_pos, sms_of(qkv), status_ptr(status),
+                     cur_stream(qkv), r.qn, r.kn, (float)eps);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// What decode attention over a quantised cache asks of its arguments, the workspace apart.
+void check_decode(const char* what, const at::Tensor& q, const at::Tensor& block_tables, const at::Tensor& ctx_lens,
+                  const at::Tensor& out, int64_t Hq, int64_t Hkv, int64_t max_batch) {
+  const int64_t B = q.size(0);
+  TORCH_CHECK(Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16, what,
+              ": the query heads must be a multiple of the KV heads, 16 of them per KV head at most");
+  TORCH_CHECK(q.size(1) >= Hq * 128 && out.size(0) == B && out.size(1) == Hq * 128, what,
+              ": q must hold Hq heads of 128 per row and out be [B, Hq * 128]");
+  TORCH_CHECK(B <= max_batch, what, ": at most ", num(max_batch), " sequences per call");
+  TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
+                  block_tables.size(0) == B,
+              what, ": block_tables must be contiguous int32 [B, max_blocks]");
+  TORCH_CHECK(ctx_lens.scalar_type() == at::kInt && ctx_lens.is_contiguous() && ctx_lens.numel() == B, what,
+              ": ctx_lens must be contiguous int32 [B]");
+  TORCH_CHECK(B * Hkv * (block_tables.size(1) + 16) < (int64_t)1 << 30 && block_tables.size(1) < (int64_t)1 << 26, what,
+              ": block tables too large");
 }
 
 int64_t decode_fp8_rows(int64_t device, int64_t B, int64_t Hkv, int64_t G) {
@@ -328,28 +363,17 @@ void decode_attention_fp8(const at::Tensor& q, const at::Tensor& kc, const at::T
                           const at::Tensor& vs, const at::Tensor& block_tables, const at::Tensor& ctx_lens,
                           at::Tensor& out, int64_t Hq, double scale, at::Tensor& ws,
                           const c10::optional<at::Tensor>& status) {
-  check_same_device(q, {&kc, &block_tables, &ctx_lens, &out, &ws}, "decode_attention_fp8");
-  check_status_device(q, status, "decode_attention_fp8");
-  const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "decode_attention_fp8");
+  const char* what = "decode_attention_fp8";
+  check_same_device(q, {&kc, &block_tables, &ctx_lens, &out, &ws}, what);
+  check_status_device(q, status, what);
+  const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, what);
   const int ldq = row_ld16(q, "decode_attention_fp8: q"), ldo = row_ld16(out, "decode_attention_fp8: out");
-  const int64_t B = q.size(0);
-  TORCH_CHECK(Hq > 0 && Hq % c.Hkv == 0 && Hq / c.Hkv <= 16,
-              "decode_attention_fp8: the query heads must be a multiple of the KV heads, 16 of them per KV head at most");
-  TORCH_CHECK(q.size(1) >= Hq * 128 && out.size(0) == B && out.size(1) == Hq * 128,
-              "decode_attention_fp8: q must hold Hq heads of 128 per row and out be [B, Hq * 128]");
-  TORCH_CHECK(B <= cx::DEC8_MAX_BATCH, "decode_attention_fp8: at most ", num(cx::DEC8_MAX_BATCH), " sequences per call");
-  TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
-                  block_tables.size(0) == B,
-              "decode_attention_fp8: block_tables must be contiguous int32 [B, max_blocks]");
-  TORCH_CHECK(ctx_lens.scalar_type() == at::kInt && ctx_lens.is_contiguous() && ctx_lens.numel() == B,
-              "decode_attention_fp8: ctx_lens must be contiguous int32 [B]");
-  TORCH_CHECK(B * c.Hkv * (block_tables.size(1) + 16) < (int64_t)1 << 30 && block_tables.size(1) < (int64_t)1 << 26,
-              "decode_attention_fp8: block tables too large");
-  const int64_t G = Hq / c.Hkv;
+  check_decode(what, q, block_tables, ctx_lens, out, Hq, c.Hkv, cx::DEC8_MAX_BATCH);
   CHECK_CUDA(q);
+  const int64_t B = q.size(0), G = Hq / c.Hkv;
   TORCH_CHECK(ws.scalar_type() == at::kFloat && ws.is_contiguous() && ws.dim() == 2 && ws.size(1) == G * cx::DEC8_ROW &&
                   ws.size(0) >= cx::decode_fp8_rows(sms_of(q), (int)B, c.Hkv, (int)G),
-              "decode_attention_fp8: the workspace must come from decode_workspace_fp8 for these heads and at least ", num(B),
+              what, ": the workspace must come from decode_workspace_fp8 for these heads and at least ", num(B),
               " sequences");
   const c10::cuda::CUDAGuard g(q.device());
   cx::decode_attention_fp8(q.data_ptr(), ldq, c, block_tables.data_ptr<int>(), (int)block_tables.size(1),
@@ -406,34 +430,31 @@ std::tuple<int64_t, int64_t> prefill_fp8_words(int64_t device, int64_t entries, 
 }
 
 // Two launches: the tables' blocks as bf16 into workspaces of the caller, the
-// paged prefill attention over them.
-void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
-                                 const at::Tensor& vs, const at::Tensor& block_tables, at::Tensor& out,
-                                 const at::Tensor& tile_info, int64_t Hq, int64_t Hkv, double scale, at::Tensor& kv,
-                                 const c10::optional<at::Tensor>& ints, const c10::optional<at::Tensor>& part,
-                                 const c10::optional<at::Tensor>& status) {
-  check_same_device(q, {&kc, &block_tables, &out, &tile_info, &kv}, "prefill_attention_paged_fp8");
-  check_status_device(q, status, "prefill_attention_paged_fp8");
-  const cx::KvFp8 c = fp8_cache(kc, vc, ks, vs, "prefill_attention_paged_fp8");
-  const int ldq = row_ld16(q, "prefill_attention_paged_fp8: q"), ldo = row_ld16(out, "prefill_attention_paged_fp8: out");
+// paged prefill attention over them.  c: the quantised cache; what: the call's name.
+template <class Cache>
+void prefill_attention_quantised(const std::string& what, const at::Tensor& q, const Cache& c,
+                                 const at::Tensor& block_tables, at::Tensor& out, const at::Tensor& tile_info, int64_t Hq,
+                                 int64_t Hkv, double scale, at::Tensor& kv, const c10::optional<at::Tensor>& ints,
+                                 const c10::optional<at::Tensor>& part, const c10::optional<at::Tensor>& status) {
+  const int ldq = row_ld16(q, (what + ": q").c_str()), ldo = row_ld16(out, (what + ": out").c_str());
   const int64_t T = q.size(0);
   TORCH_CHECK(Hkv == c.Hkv && Hq > 0 && Hq % Hkv == 0,
-              "prefill_attention_paged_fp8: Hkv as in the cache, the query heads a multiple of it");
+              what, ": Hkv as in the cache, the query heads a multiple of it");
   // the kernel takes the row's largest score before it is scaled
-  TORCH_CHECK(scale > 0 && std::isfinite(scale), "prefill_attention_paged_fp8: the scale must be positive");
+  TORCH_CHECK(scale > 0 && std::isfinite(scale), what, ": the scale must be positive");
   TORCH_CHECK(q.size(1) >= Hq * 128 && out.size(0) == T && out.size(1) == Hq * 128,
-              "prefill_attention_paged_fp8: q must hold Hq heads of 128 per row and out be [T, Hq * 128]");
+              what, ": q must hold Hq heads of 128 per row and out be [T, Hq * 128]");
   TORCH_CHECK(tile_info.scalar_type() == at::kInt && tile_info.dim() == 2 && tile_info.size(1) == 5 &&
                   tile_info.is_contiguous() && (tile_info.size(0) + 1) * Hq <= INT_MAX / 5,
-              "prefill_attention_paged_fp8: tile_info must be contiguous int32 [n, 5]");
+              what, ": tile_info must be contiguous int32 [n, 5]");
   TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
                   block_tables.numel() <= INT_MAX && block_tables.size(1) < (int64_t)1 << 26 &&
                   block_tables.size(0) <= cx::KVQ_MAX_CHUNKS,
-              "prefill_attention_paged_fp8: block_tables must be contiguous int32 [B, max_blocks], B up to ",
+              what, ": block_tables must be contiguous int32 [B, max_blocks], B up to ",
               num(cx::KVQ_MAX_CHUNKS));
   TORCH_CHECK(kv.dim() == 5 && kv.size(0) == 2 && kv.size(2) == Hkv && kv.size(3) == 16 && kv.size(4) == 128 &&
                   kv.is_contiguous() && kv.scalar_type() == at::kBFloat16 && kv.size(1) * Hkv * 16 <= INT_MAX,
-              "prefill_attention_paged_fp8: the blocks' workspace must be contiguous bf16 [2, n_blocks, Hkv, 16, 128]");
+              what, ": the blocks' workspace must be contiguous bf16 [2, n_blocks, Hkv, 16, 128]");
   CHECK_CUDA(q);
   const int64_t entries = block_tables.numel(), n_tiles = tile_info.size(0);
   // The query heads of a KV head share a tile's rows where tokens alone would leave a quarter of them empty
@@ -443,11 +464,11 @@ void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, cons
   const auto [n_ints, n_part] = prefill_fp8_words(q.device().index(), entries, n_tiles, Hq / Hkv);   // room for either
   TORCH_CHECK(ints.has_value() && ints->scalar_type() == at::kInt && ints->numel() == n_ints && ints->is_contiguous() &&
                   part.has_value() && part->scalar_type() == at::kFloat && part->numel() == n_part && part->is_contiguous(),
-              "prefill_attention_paged_fp8: workspaces of other sizes");
-  check_same_device(q, {&*ints, &*part}, "prefill_attention_paged_fp8");
+              what, ": workspaces of other sizes");
+  check_same_device(q, {&*ints, &*part}, what.c_str());
   const c10::cuda::CUDAGuard g(q.device());
   TORCH_CHECK(T == 0 || n_tiles == 0 || (entries > 0 && kv.size(1) > 0),
-              "prefill_attention_paged_fp8: no block table for the tiles");
+              what, ": no block table for the tiles");
   if (T == 0 || n_tiles == 0) return;
   cx::KvChunks o;
   o.k = kv.data_ptr();
@@ -474,6 +495,219 @@ void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, cons
   cx::prefill_attention_paged_tc(q.data_ptr(), ldq, (int)(Hq * 128), (int)T, o.k, o.v, kv.size(1) * Hkv * 16, o.tables,
                                  (int)block_tables.size(1), out.data_ptr(), ldo, o.tiles, (int)n_tiles, (int)Hq,
                                  (int)Hkv, (float)scale, status_ptr(status), cur_stream(q), 256, &plan);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+void prefill_attention_paged_fp8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
+                                 const at::Tensor& vs, const at::Tensor& block_tables, at::Tensor& out,
+                                 const at::Tensor& tile_info, int64_t Hq, int64_t Hkv, double scale, at::Tensor& kv,
+                                 const c10::optional<at::Tensor>& ints, const c10::optional<at::Tensor>& part,
+                                 const c10::optional<at::Tensor>& status) {
+  const char* what = "prefill_attention_paged_fp8";
+  check_same_device(q, {&kc, &block_tables, &out, &tile_info, &kv}, what);
+  check_status_device(q, status, what);
+  prefill_attention_quantised(what, q, fp8_cache(kc, vc, ks, vs, what), block_tables, out, tile_info, Hq, Hkv, scale, kv,
+                              ints, part, status);
+}
+
+// ---- 4-bit paged KV cache ----------------------------------------------------
+cx::KvInt4 int4_cache(const at::Tensor& k, const at::Tensor& v, const char* what) {
+  check_same_device(k, {&v}, what);
+  TORCH_CHECK(k.dim() == 4 && k.size(2) == 16 && k.size(3) == cx::KV4_ROW && k.size(1) > 0 && k.is_contiguous() &&
+                  v.is_contiguous() && v.sizes() == k.sizes() && k.scalar_type() == at::kByte && v.scalar_type() == at::kByte,
+              what, ": caches must be contiguous uint8 [blocks, Hkv, 16, 72]");
+  TORCH_CHECK(k.size(0) <= INT_MAX && k.size(1) <= INT_MAX && ((reinterpret_cast<uintptr_t>(k.data_ptr()) |
+                                        reinterpret_cast<uintptr_t>(v.data_ptr())) & 15) == 0,
+              what, ": caches must start on a 16-byte boundary");
+  return cx::KvInt4{static_cast<uint8_t*>(k.data_ptr()), static_cast<uint8_t*>(v.data_ptr()), (int)k.size(0),
+                    (int)k.size(1)};
+}
+
+void rope_cache_int4(const at::Tensor& qkv, const at::Tensor& pos, const at::Tensor& cos_sin, const at::Tensor& slots,
+                     const at::Tensor& kc, const at::Tensor& vc, at::Tensor& out, int64_t Hq,
+                     int64_t Hkv, const c10::optional<at::Tensor>& status, const c10::optional<at::Tensor>& q_norm,
+                     const c10::optional<at::Tensor>& k_norm, double eps) {
+  const char* what = "rope_cache_int4";
+  check_same_device(qkv, {&pos, &cos_sin, &slots, &kc, &out}, what);
+  check_status_device(qkv, status, what);
+  const cx::KvInt4 c = int4_cache(kc, vc, what);
+  const RopeRows r = rope_rows(what, qkv, pos, cos_sin, slots, kc, out, Hq, Hkv, q_norm, k_norm);
+  CHECK_CUDA(qkv);
+  const c10::cuda::CUDAGuard g(qkv.device());
+  cx::rope_cache_int4(qkv.data_ptr(), r.ldq, pos.data_ptr<int>(), cos_sin.data_ptr<float>(), slots.data_ptr<int64_t>(), c,
+                      out.data_ptr(), r.ldo, (int)qkv.size(0), (int)Hq, r.max_pos, status_ptr(status), cur_stream(qkv),
+                      r.qn, r.kn, (float)eps);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+void kv_values_int4(const at::Tensor& cache, at::Tensor& out) {
+  check_same_device(cache, {&out}, "kv_values_int4");
+  TORCH_CHECK(cache.scalar_type() == at::kByte && cache.dim() >= 1 && cache.size(-1) == cx::KV4_ROW &&
+                  cache.is_contiguous() && (reinterpret_cast<uintptr_t>(cache.data_ptr()) & 3) == 0,
+              "kv_values_int4: the cache must be contiguous uint8 [..., 72]");
+  auto shape = cache.sizes().vec();
+  shape.back() = 128;
+  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.sizes() == at::IntArrayRef(shape) &&
+                  (reinterpret_cast<uintptr_t>(out.data_ptr()) & 15) == 0,
+              "kv_values_int4: out must be contiguous bf16 [..., 128]");
+  CHECK_CUDA(cache);
+  const c10::cuda::CUDAGuard g(cache.device());
+  cx::kv_values_int4(cache.data_ptr(), out.data_ptr(), cache.numel() / cx::KV4_ROW, sms_of(cache), cur_stream(cache));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+int64_t decode_int4_rows(int64_t device, int64_t B, int64_t Hkv, int64_t G) {
+  TORCH_CHECK(B >= 0 && Hkv > 0 && G > 0, "decode_workspace_int4: bad sizes");
+  return cx::decode_int4_rows(at::cuda::getDeviceProperties(device)->multiProcessorCount, (int)B, (int)Hkv, (int)G);
+}
+
+void decode_attention_int4(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
+                           const at::Tensor& block_tables, const at::Tensor& ctx_lens, at::Tensor& out, int64_t Hq,
+                           double scale, at::Tensor& ws, const c10::optional<at::Tensor>& status) {
+  const char* what = "decode_attention_int4";
+  check_same_device(q, {&kc, &block_tables, &ctx_lens, &out, &ws}, what);
+  check_status_device(q, status, what);
+  const cx::KvInt4 c = int4_cache(kc, vc, what);
+  const int ldq = row_ld16(q, "decode_attention_int4: q"), ldo = row_ld16(out, "decode_attention_int4: out");
+  check_decode(what, q, block_tables, ctx_lens, out, Hq, c.Hkv, cx::DEC4_MAX_BATCH);
+  CHECK_CUDA(q);
+  const int64_t B = q.size(0), G = Hq / c.Hkv;
+  TORCH_CHECK(ws.scalar_type() == at::kFloat && ws.is_contiguous() && ws.dim() == 2 && ws.size(1) == G * cx::DEC4_ROW &&
+                  ws.size(0) >= cx::decode_int4_rows(sms_of(q), (int)B, c.Hkv, (int)G),
+              what, ": the workspace must come from decode_workspace_int4 for these heads and at least ", num(B),
+              " sequences");
+  const c10::cuda::CUDAGuard g(q.device());
+  cx::decode_attention_int4(q.data_ptr(), ldq, c, block_tables.data_ptr<int>(), (int)block_tables.size(1),
+                            ctx_lens.data_ptr<int>(), out.data_ptr(), ldo, (int)B, (int)Hq, (float)scale,
+                            ws.data_ptr<float>(), sms_of(q), status_ptr(status), cur_stream(q));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+void prefill_attention_paged_int4(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
+                                  const at::Tensor& block_tables, at::Tensor& out, const at::Tensor& tile_info, int64_t Hq,
+                                  int64_t Hkv, double scale, at::Tensor& kv, const c10::optional<at::Tensor>& ints,
+                                  const c10::optional<at::Tensor>& part, const c10::optional<at::Tensor>& status) {
+  const char* what = "prefill_attention_paged_int4";
+  check_same_device(q, {&kc, &block_tables, &out, &tile_info, &kv}, what);
+  check_status_device(q, status, what);
+  prefill_attention_quantised(what, q, int4_cache(kc, vc, what), block_tables, out, tile_info, Hq, Hkv, scale, kv, ints,
+                              part, status);
+}
+
+// ---- block-scaled fp8 ----------------------------------------------------------
+// e4m3 rows that a TMA can read: [rows, cols], contiguous rows on 16-byte boundaries
+int64_t fp8_ld(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(t.dim() == 2 && t.scalar_type() == at::kFloat8_e4m3fn && (t.size(1) <= 1 || t.stride(1) == 1), what,
+              " must be float8_e4m3fn [rows, columns] with contiguous rows");
+  const int64_t ld = t.size(0) > 1 ? t.stride(0) : t.size(1);
+  TORCH_CHECK(t.size(1) % 16 == 0 && ld >= t.size(1) && ld % 16 == 0 &&
+                  (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && t.size(0) <= INT_MAX / 2 &&
+                  t.size(1) <= INT_MAX / 2 && ld < (int64_t)1 << 39,
+              what, ": columns must be a multiple of 16 and rows start on 16-byte boundaries without overlap");
+  return ld;
+}
+// fp32 scales of `rows` rows (or blocks of them) and ceil(cols / 128) column blocks, any strides
+cx::Fp8Scales fp8_scales(const at::Tensor& s, int64_t rows, int64_t cols, const char* what) {
+  TORCH_CHECK(s.scalar_type() == at::kFloat && s.dim() == 2 && s.size(0) == rows && s.size(1) == (cols + 127) / 128, what,
+              " must be fp32 [", num(rows), ", ", num((cols + 127) / 128), "]");
+  return cx::Fp8Scales{s.data_ptr<float>(), s.stride(0), s.stride(1)};
+}
+// scales that a call writes: no two of them in one place
+cx::Fp8Scales fp8_scales_out(const at::Tensor& s, int64_t rows, int64_t cols, const char* what) {
+  const cx::Fp8Scales r = fp8_scales(s, rows, cols, what);
+  const int64_t kb = s.size(1);
+  TORCH_CHECK((rows <= 1 || r.row > 0) && (kb <= 1 || r.col > 0) &&
+                  (rows <= 1 || kb <= 1 || r.row >= kb * r.col || r.col >= rows * r.row),
+              what, " must not overlap itself");
+  return r;
+}
+
+void quantize_fp8(const at::Tensor& x, const c10::optional<at::Tensor>& norm, double eps, at::Tensor& q,
+                  at::Tensor& scale) {
+  check_same_device(x, {&q, &scale}, "quantize_fp8");
+  const int ldx = row_ld16(x, "quantize_fp8: x");
+  const int64_t T = x.size(0), K = x.size(1), ldq = fp8_ld(q, "quantize_fp8: out");
+  TORCH_CHECK(q.size(0) == T && q.size(1) == K, "quantize_fp8: out must have x's shape");
+  const cx::Fp8Scales s = fp8_scales_out(scale, T, K, "quantize_fp8: scale");
+  const void* w = nullptr;
+  if (norm.has_value()) {
+    check_same_device(x, {&*norm}, "quantize_fp8");
+    TORCH_CHECK(norm->scalar_type() == at::kBFloat16 && norm->dim() == 1 && norm->numel() == K && norm->is_contiguous() &&
+                    (reinterpret_cast<uintptr_t>(norm->data_ptr()) & 15) == 0,
+                "quantize_fp8: norm must be contiguous bf16 [columns of x]");
+    TORCH_CHECK(K <= cx::QUANT_NORM_MAX_K, "quantize_fp8: at most ", num(cx::QUANT_NORM_MAX_K), " columns with a norm");
+    w = norm->data_ptr();
+  }
+  CHECK_CUDA(x);
+  const c10::cuda::CUDAGuard g(x.device());
+  cx::quantize_fp8(x.data_ptr(), ldx, w, (float)eps, q.data_ptr(), ldq, s, (int)T, (int)K, cur_stream(x));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+void quantize_weight_fp8(const at::Tensor& w, at::Tensor& q, at::Tensor& scale) {
+  check_same_device(w, {&q, &scale}, "quantize_weight_fp8");
+  const int ldw = row_ld16(w, "quantize_weight_fp8: w");
+  const int64_t N = w.size(0), K = w.size(1), ldq = fp8_ld(q, "quantize_weight_fp8: out");
+  TORCH_CHECK(q.size(0) == N && q.size(1) == K, "quantize_weight_fp8: out must have w's shape");
+  const cx::Fp8Scales s = fp8_scales_out(scale, (N + 127) / 128, K, "quantize_weight_fp8: scale");
+  TORCH_CHECK((N + 127) / 128 <= 65535, "quantize_weight_fp8: too many rows");
+  CHECK_CUDA(w);
+  const c10::cuda::CUDAGuard g(w.device());
+  cx::quantize_weight_fp8(w.data_ptr(), ldw, q.data_ptr(), ldq, s, (int)N, (int)K, cur_stream(w));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// out: bf16, or e4m3 with out_scale (SiLU-mul alone)
+void gemm_fp8(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb, at::Tensor& out,
+              const c10::optional<at::Tensor>& out_scale, const c10::optional<at::Tensor>& residual, int64_t epi,
+              const c10::optional<at::Tensor>& status) {
+  check_same_device(a, {&sa, &b, &sb, &out}, "gemm_fp8");
+  check_status_device(a, status, "gemm_fp8");
+  cx::GemmFp8 g{};
+  g.lda = fp8_ld(a, "gemm_fp8: a");
+  g.ldb = fp8_ld(b, "gemm_fp8: b");
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(0);
+  TORCH_CHECK(b.size(1) == K && K > 0, "gemm_fp8: a and b must have the same columns, not none");
+  TORCH_CHECK(N % 8 == 0, "gemm_fp8: the rows of b must be a multiple of 8");
+  g.sa = fp8_scales(sa, M, K, "gemm_fp8: a's scales");
+  g.sb = fp8_scales(sb, (N + 127) / 128, K, "gemm_fp8: b's scales");
+  const bool silu = epi == cx::EPI_SILU_MUL;
+  TORCH_CHECK(epi == cx::EPI_STORE || epi == cx::EPI_ADD || silu, "gemm_fp8: unknown epilogue");
+  TORCH_CHECK(!silu || N % 256 == 0, "gemm_fp8: SiLU-mul needs the rows of b to be a multiple of 256");
+  const int64_t n_out = silu ? N / 2 : N;
+  TORCH_CHECK(out.dim() == 2 && out.size(0) == M && out.size(1) == n_out, "gemm_fp8: out must be [", num(M), ", ",
+              num(n_out), "]");
+  if (out.numel() == 0) return;
+  if (out_scale.has_value()) {
+    TORCH_CHECK(silu, "gemm_fp8: only the SiLU-mul output is quantised");
+    check_same_device(a, {&*out_scale}, "gemm_fp8");
+    g.ldd = fp8_ld(out, "gemm_fp8: out");
+    g.sd = fp8_scales_out(*out_scale, M, n_out, "gemm_fp8: out's scales");
+  } else {
+    g.ldd = row_ld16(out, "gemm_fp8: out");
+  }
+  TORCH_CHECK((epi == cx::EPI_ADD) == residual.has_value(), "gemm_fp8: the residual goes with its epilogue");
+  if (residual.has_value()) {
+    check_same_device(a, {&*residual}, "gemm_fp8");
+    g.ldr = row_ld16(*residual, "gemm_fp8: residual");
+    TORCH_CHECK(residual->sizes() == out.sizes(), "gemm_fp8: residual must have out's shape");
+    // read and written element by element by one thread each: the same place or another, but not shifted
+    const char *x0 = static_cast<const char*>(residual->data_ptr()), *y0 = static_cast<const char*>(out.data_ptr());
+    const char *x1 = x0 + (M > 0 ? ((M - 1) * g.ldr + N) * 2 : 0), *y1 = y0 + (M > 0 ? ((M - 1) * g.ldd + N) * 2 : 0);
+    TORCH_CHECK(x1 <= y0 || y1 <= x0 || (x0 == y0 && (g.ldr == g.ldd || M == 1)),
+                "gemm_fp8: out overlaps the residual other than as itself");
+    g.r = residual->data_ptr();
+  }
+  CHECK_CUDA(a);
+  const c10::cuda::CUDAGuard guard(a.device());
+  g.a = a.data_ptr();
+  g.b = b.data_ptr();
+  g.d = out.data_ptr();
+  g.M = (int)M;
+  g.N = (int)N;
+  g.K = (int)K;
+  g.epi = (int)epi;
+  cx::gemm_fp8(g, sms_of(a), status_ptr(status), cur_stream(a));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -727,6 +961,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_copy_blocks", &kv_copy_blocks);
   m.def("prefill_fp8_words", &prefill_fp8_words);
   m.def("prefill_attention_paged_fp8", &prefill_attention_paged_fp8);
+  m.def("rope_cache_int4", &rope_cache_int4);
+  m.def("kv_values_int4", &kv_values_int4);
+  m.def("decode_int4_rows", &decode_int4_rows);
+  m.attr("DECODE_INT4_ROW") = cx::DEC4_ROW;
+  m.attr("KV_INT4_ROW") = cx::KV4_ROW;
+  m.def("decode_attention_int4", &decode_attention_int4);
+  m.def("prefill_attention_paged_int4", &prefill_attention_paged_int4);
+  m.def("quantize_fp8", &quantize_fp8);
+  m.def("quantize_weight_fp8", &quantize_weight_fp8);
+  m.def("gemm_fp8", &gemm_fp8);
   m.def("kv_push_layer", &kv_push_layer);
   m.def("gemm_splits", &gemm_splits);
   m.def("gemm_raster_group", &cx::gemm_raster_group);

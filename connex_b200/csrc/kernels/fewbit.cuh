@@ -1,0 +1,103 @@
+// Device helpers of the kernels that hold values in few bits: conversions,
+// fp16 tensor-core steps on registers, asynchronous 16-byte copies.
+#pragma once
+
+#include "common.cuh"
+
+namespace cx {
+
+// 2^e for e of [-126, 127]
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// two fp32 -> two e4m3 bytes (lo in the low byte), nearest even, NaN kept
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// two e4m3 bytes -> f16x2, exact
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return r;
+}
+__device__ __forceinline__ float f16_lo(uint32_t v) {
+  float f;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.f32.f16 %0, l;\n\t}" : "=f"(f) : "r"(v));
+  return f;
+}
+__device__ __forceinline__ float f16_hi(uint32_t v) {
+  float f;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.f32.f16 %0, h;\n\t}" : "=f"(f) : "r"(v));
+  return f;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float finite_or_zero(float a) {   // |a| of a finite value, 0 of Inf and NaN
+  const uint32_t u = __float_as_uint(a) & 0x7fffffffu;
+  return u < 0x7f800000u ? __uint_as_float(u) : 0.f;
+}
+__device__ __forceinline__ uint64_t unpack_bf16x2(uint32_t w) { return f32x2(bf16_lo(w), bf16_hi(w)); }
+// a cos + b sin of a pair of dims, rounded to bf16
+__device__ __forceinline__ uint32_t turn_bf16x2(uint32_t a, uint32_t b, uint64_t co, uint64_t si) {
+  const uint64_t r = fma_f32x2(unpack_bf16x2(b), si, mul_f32x2(unpack_bf16x2(a), co));
+  return pack_bf16x2(lo_f32(r), hi_f32(r));
+}
+struct alignas(16) f32x4 {        // two pairs of fp32
+  uint64_t a, b;
+};
+
+// Eight 4-bit codes of a word, dim i in bits [4i, 4i + 4), and their scale |
+// minimum << 16 (bf16 each) -> minimum + code * scale, rounded to bf16.
+__device__ __forceinline__ u128 int4_values(uint32_t codes, uint32_t par) {
+  const float s = bf16_lo(par), m = bf16_hi(par);
+  u128 r;
+  uint32_t* p = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    p[i] = pack_bf16x2(fmaf((float)(codes >> (8 * i) & 15u), s, m), fmaf((float)(codes >> (8 * i + 4) & 15u), s, m));
+  return r;
+}
+
+// ------------------------------------------------------------ shared memory
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ u128 lds16(uint32_t a) {
+  u128 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ void sts16(uint32_t a, const u128& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// -------------------------------------------------------------------- fp16
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t word(const u128& v, int i) { return reinterpret_cast<const uint32_t*>(&v)[i]; }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace cx

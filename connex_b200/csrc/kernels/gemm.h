@@ -32,6 +32,9 @@ bool gemv_bf16_tn(const void* A, const void* B, void* D, const void* R, int M, i
 
 CUtensorMap make_tmap_bf16_2d(const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
                               uint32_t box_inner, uint32_t box_outer, bool swizzle128);
+// rows of bytes (an fp8 operand), 128-byte swizzle
+CUtensorMap make_tmap_u8_2d(const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
+                            uint32_t box_inner, uint32_t box_outer);
 // [outer][mid][inner] of bf16, 128-byte swizzle
 CUtensorMap make_tmap_bf16_3d(const void* base, uint64_t inner, uint64_t mid, uint64_t outer, uint64_t mid_stride_bytes,
                               uint64_t outer_stride_bytes, uint32_t box_inner, uint32_t box_mid, uint32_t box_outer);

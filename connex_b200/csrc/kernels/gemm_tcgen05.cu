@@ -20,6 +20,7 @@
 // code and the CTA drains its tensor-core work before freeing TMEM.
 #include "common.cuh"
 #include "gemm.h"
+#include "gemm_tile.cuh"
 
 #include <algorithm>
 #include <cstdio>
@@ -42,26 +43,12 @@ struct GemmCfg {
   static constexpr int SMEM = 1024 /*align slack*/ + STAGES * STAGE_BYTES + 256 /*barriers*/;
 };
 
-// Grouped raster: bands of `group` tile-rows, each band walked column by
-// column, so the CTAs of one wave share A rows and B columns through L2.
-__device__ __forceinline__ void tile_coords(int t, int num_m, int num_n, int group, int& tm, int& tn) {
-  const int per_group = group * num_n;
-  const int g = t / per_group;
-  const int first_m = g * group;
-  const int gm = min(num_m - first_m, group);
-  const int r = t - g * per_group;
-  tm = first_m + r % gm;
-  tn = r / gm;
-}
-
 __device__ __forceinline__ void tile_coords_split(int t, int num_m, int num_n, int splits, int group, int& tm,
                                                   int& tn, int& ks) {
   const int tt = t / splits;
   ks = t - tt * splits;
   tile_coords(tt, num_m, num_n, group, tm, tn);
 }
-
-__device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x)); }
 
 // Vector fp32 reduction into global memory (split-K partial sums).
 __device__ __forceinline__ void red_add_v4_f32(float* p, float a, float b, float c, float d) {
@@ -359,6 +346,22 @@ static EncodeTiledFn get_encode_fn() {
     fn = reinterpret_cast<EncodeTiledFn>(p);
   });
   return fn;
+}
+
+CUtensorMap make_tmap_u8_2d(const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
+                            uint32_t box_inner, uint32_t box_outer) {
+  if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) throw std::runtime_error("cx: TMA base not 16-byte aligned");
+  if ((row_stride_bytes & 15) != 0) throw std::runtime_error("cx: TMA row stride not a multiple of 16 bytes");
+  CUtensorMap m;
+  cuuint64_t dims[2] = {inner, outer};
+  cuuint64_t strides[1] = {row_stride_bytes};
+  cuuint32_t box[2] = {box_inner, box_outer};
+  cuuint32_t es[2] = {1, 1};
+  CUresult r = get_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("cx: cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+  return m;
 }
 
 CUtensorMap make_tmap_bf16_2d(const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,

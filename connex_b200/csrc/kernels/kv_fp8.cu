@@ -10,8 +10,9 @@
 #include <stdexcept>
 #include <type_traits>
 
-#include "common.cuh"
+#include "fewbit.cuh"
 #include "kv_fp8.h"
+#include "kv_int4.h"
 
 namespace cx {
 
@@ -22,8 +23,6 @@ constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int SMEM = BS * D * 4 + WARPS * BS * D * 2;   // cos / sin rows, each warp's rows
 }  // namespace kvq
 
-// 2^e for e of [-126, 127]
-__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 // The smallest e >= MIN_EXP with a <= 448 * 2^e = 1.75 * 2^(e + 8), for finite a >= 0.
 __device__ __forceinline__ int fp8_exp_for(float a) {
   const uint32_t u = __float_as_uint(a);
@@ -33,74 +32,17 @@ __device__ __forceinline__ int fp8_exp_for(float a) {
 __device__ __forceinline__ int fp8_exp_of(float scale) {
   return min(max((int)((__float_as_uint(scale) >> 23) & 255u) - 127, kvq::MIN_EXP), kvq::MAX_EXP);
 }
-// two fp32 -> two e4m3 bytes (lo in the low byte), nearest even, NaN kept
-__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// two e4m3 bytes -> f16x2, exact
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t v) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
-  return r;
-}
-__device__ __forceinline__ float f16_lo(uint32_t v) {
-  float f;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.f32.f16 %0, l;\n\t}" : "=f"(f) : "r"(v));
-  return f;
-}
-__device__ __forceinline__ float f16_hi(uint32_t v) {
-  float f;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.f32.f16 %0, h;\n\t}" : "=f"(f) : "r"(v));
-  return f;
-}
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float finite_or_zero(float a) {   // |a| of a finite value, 0 of Inf and NaN
-  const uint32_t u = __float_as_uint(a) & 0x7fffffffu;
-  return u < 0x7f800000u ? __uint_as_float(u) : 0.f;
-}
 // x * mul as e4m3 would hold it: e4m3 has no infinities, so Inf becomes NaN
 __device__ __forceinline__ float scaled_or_nan(float x, float mul) {
   return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fffffffu) : x * mul;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ u128 lds16(uint32_t a) {
-  u128 r;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
-  return r;
-}
-__device__ __forceinline__ void sts16(uint32_t a, const u128& v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-__device__ __forceinline__ uint64_t unpack_bf16x2(uint32_t w) { return f32x2(bf16_lo(w), bf16_hi(w)); }
 // larger magnitudes of two bf16 pairs, signs undefined; NaN only where both are
 __device__ __forceinline__ uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// a cos + b sin of a pair of dims, rounded to bf16
-__device__ __forceinline__ uint32_t turn_bf16x2(uint32_t a, uint32_t b, uint64_t co, uint64_t si) {
-  const uint64_t r = fma_f32x2(unpack_bf16x2(b), si, mul_f32x2(unpack_bf16x2(a), co));
-  return pack_bf16x2(lo_f32(r), hi_f32(r));
-}
-struct alignas(16) f32x4 {        // two pairs of fp32
-  uint64_t a, b;
-};
-
 // ------------------------------------------------- RoPE + quantising write
 // CTAs of two kinds.  Block CTAs write the cache.  A block's scale depends on
 // every row that the call puts there, so one CTA collects them: the one whose
@@ -482,25 +424,6 @@ struct Smem {                           // rings, later the warps' O | their (m,
 };
 }  // namespace dec8
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint2 lds8(uint32_t a) {
-  uint2 r;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
-  return r;
-}
-__device__ __forceinline__ uint32_t word(const u128& v, int i) { return reinterpret_cast<const uint32_t*>(&v)[i]; }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // NT: tiles of 8 query heads per KV head (1: groups up to 8, 2: up to 16).
 template <int NT>
 __global__ void __launch_bounds__(dec8::THREADS, dec8::ctas_per_sm(NT))
@@ -1091,9 +1014,10 @@ void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes
 }
 
 // --------------------------------------------------------- dequantised blocks
-// The blocks that the tiles of a chunked prefill read, as bf16 (exact: the
-// scales are powers of two), sequence after sequence, and the tables that find
-// them there.  Bound by memory and short next to the attention that
+// The blocks that the tiles of a chunked prefill read, as bf16, sequence after
+// sequence, and the tables that find them there.  From e4m3 that is exact (the
+// scales are powers of two), from 4 bits minimum + code * scale is rounded
+// (2^-9 of it, next to steps of a fifteenth of a half's range).  Bound by memory and short next to the attention that
 // follows: 12 of 211 us for 2048 rows at 6144.  (Converting inside the
 // attention kernel, by four more warps between the copies and the MMAs, took
 // 302 us where two launches took 225: the thread that issues the MMAs is busy
@@ -1209,8 +1133,48 @@ __device__ __forceinline__ void kv_prefill_plan(const int* __restrict__ tile_inf
     o.cuts[i] = cut;
   }
 }
+// Sixteen e4m3 values (dims [16 i, 16 i + 16) of the block's heads, end to end) as bf16; zeros without a block.
+struct Fp8Blocks {
+  static constexpr int DIMS = 16;
+  KvFp8 c;
+  __device__ __forceinline__ void load(bool is_v, int id, bool in, int i, u128 (&o)[2]) const {
+    using namespace kvq;
+    const int e = i * DIMS, h = e / (BS * D);
+    u128 raw{0, 0, 0, 0};
+    float f = 0.f;
+    if (in) {
+      raw = ld_nc_v4((is_v ? c.v : c.k) + (size_t)id * c.Hkv * (BS * D) + e);
+      f = (is_v ? c.vs : c.ks)[(size_t)id * c.Hkv + h];
+    }
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
+    uint32_t* po = reinterpret_cast<uint32_t*>(o);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t a = e4m3x2_to_f16x2((uint16_t)w[k]), b = e4m3x2_to_f16x2((uint16_t)(w[k] >> 16));
+      po[2 * k] = pack_bf16x2(f16_lo(a) * f, f16_hi(a) * f);
+      po[2 * k + 1] = pack_bf16x2(f16_lo(b) * f, f16_hi(b) * f);
+    }
+  }
+};
+// The same of 4-bit codes: two words of one half.
+struct Int4Blocks {
+  static constexpr int DIMS = 16;
+  KvInt4 c;
+  __device__ __forceinline__ void load(bool is_v, int id, bool in, int i, u128 (&o)[2]) const {
+    uint2 w = make_uint2(0, 0);
+    uint32_t par = 0;
+    if (in) {
+      const uint8_t* row = (is_v ? c.v : c.k) + ((size_t)id * c.Hkv * kvq::BS + (i >> 3)) * KV4_ROW;
+      w = __ldg(reinterpret_cast<const uint2*>(row + 8 * (i & 7)));
+      par = __ldg(reinterpret_cast<const uint32_t*>(row + 64 + (i & 4)));
+    }
+    o[0] = int4_values(w.x, par);
+    o[1] = int4_values(w.y, par);
+  }
+};
+template <class Blocks>
 __global__ void __launch_bounds__(kvd::THREADS)
-    kv_dequant_kernel(KvFp8 c, const int* __restrict__ tables, int B, int width, const int* __restrict__ tile_info,
+    kv_dequant_kernel(Blocks src, const int* __restrict__ tables, int B, int width, const int* __restrict__ tile_info,
                       int n_tiles, int T, int Hq, KvChunks out, int* status) {
   using namespace kvq;
   extern __shared__ int from[];                         // [B + 1]: blocks of the sequences before b
@@ -1263,40 +1227,36 @@ __global__ void __launch_bounds__(kvd::THREADS)
   const int64_t at = entry(i);
   if (tid == 0) out.tables[at] = i;
   const int id = tables[at];
-  const bool in = id >= 0 && id < c.num_blocks;
+  const bool in = id >= 0 && id < src.c.num_blocks;
   if (!in && tid == 0) record_status(status, CX_ERR_BOUNDS);
   __nv_bfloat16 *ko = reinterpret_cast<__nv_bfloat16*>(out.k), *vo = reinterpret_cast<__nv_bfloat16*>(out.v);
-  const int per = c.Hkv * (BS * D / 16);                // 16-byte pieces of K, and of V
+  const int per = src.c.Hkv * (BS * D / Blocks::DIMS);  // pieces of K, and of V
 #pragma unroll 4
   for (int v = tid; v < 2 * per; v += kvd::THREADS) {
     const bool is_v = v >= per;
-    const int e = (is_v ? v - per : v) * 16, h = e / (BS * D);
-    u128 raw{0, 0, 0, 0};                               // an id out of range reads as zeros
-    float f = 0.f;
-    if (in) {
-      raw = ld_nc_v4((is_v ? c.v : c.k) + (size_t)id * c.Hkv * (BS * D) + e);
-      f = (is_v ? c.vs : c.ks)[(size_t)id * c.Hkv + h];
-    }
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
+    const int e = is_v ? v - per : v;
     u128 o[2];
-    uint32_t* po = reinterpret_cast<uint32_t*>(o);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t a = e4m3x2_to_f16x2((uint16_t)w[k]), b = e4m3x2_to_f16x2((uint16_t)(w[k] >> 16));
-      po[2 * k] = pack_bf16x2(f16_lo(a) * f, f16_hi(a) * f);
-      po[2 * k + 1] = pack_bf16x2(f16_lo(b) * f, f16_hi(b) * f);
-    }
-    __nv_bfloat16* d = (is_v ? vo : ko) + (size_t)i * c.Hkv * (BS * D) + e;
+    src.load(is_v, id, in, e, o);
+    __nv_bfloat16* d = (is_v ? vo : ko) + (size_t)i * src.c.Hkv * (BS * D) + e * Blocks::DIMS;
     st_v4(d, o[0]);
     st_v4(d + 8, o[1]);
   }
 }
 
+template <class Blocks>
+static void dequant_blocks(const Blocks& src, const int* tables, int B, int width, const int* tile_info, int n_tiles,
+                           int T, int Hq, const KvChunks& o, int* status, cudaStream_t s) {
+  if (B == 0 || width == 0) return;
+  kv_dequant_kernel<<<std::max(1, o.blocks), kvd::THREADS, (B + 1) * sizeof(int), s>>>(src, tables, B, width, tile_info,
+                                                                                       n_tiles, T, Hq, o, status);
+}
 void kv_dequant_blocks(const KvFp8& c, const int* tables, int B, int width, const int* tile_info, int n_tiles, int T,
                        int Hq, const KvChunks& o, int* status, cudaStream_t s) {
-  if (B == 0 || width == 0) return;
-  kv_dequant_kernel<<<std::max(1, o.blocks), kvd::THREADS, (B + 1) * sizeof(int), s>>>(c, tables, B, width, tile_info,
-                                                                                       n_tiles, T, Hq, o, status);
+  dequant_blocks(Fp8Blocks{c}, tables, B, width, tile_info, n_tiles, T, Hq, o, status, s);
+}
+void kv_dequant_blocks(const KvInt4& c, const int* tables, int B, int width, const int* tile_info, int n_tiles, int T,
+                       int Hq, const KvChunks& o, int* status, cudaStream_t s) {
+  dequant_blocks(Int4Blocks{c}, tables, B, width, tile_info, n_tiles, T, Hq, o, status, s);
 }
 
 }  // namespace cx

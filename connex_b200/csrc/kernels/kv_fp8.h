@@ -58,10 +58,13 @@ struct KvChunks {
   int64_t* before;  // [n_tiles << pack] scratch
   int n_cta, pack, team;
 };
-// The e4m3 blocks that the tiles (tile_info [n_tiles, 5] of the paged prefill)
+// The blocks (e4m3, or 4 bits) that the tiles (tile_info [n_tiles, 5] of the paged prefill)
 // read through tables [B, width] (B <= KVQ_MAX_CHUNKS), as bf16 blocks, those
 // of one sequence behind those of another.  Tiles that do not fit T rows and
 // the tables are left out; more blocks than there is room for are recorded.
+struct KvInt4;
+void kv_dequant_blocks(const KvInt4& c, const int* tables, int B, int width, const int* tile_info, int n_tiles, int T,
+                       int Hq, const KvChunks& o, int* status, cudaStream_t s);
 void kv_dequant_blocks(const KvFp8& c, const int* tables, int B, int width, const int* tile_info, int n_tiles, int T,
                        int Hq, const KvChunks& o, int* status, cudaStream_t s);
 

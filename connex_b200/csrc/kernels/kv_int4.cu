@@ -1,0 +1,715 @@
+// The 4-bit paged KV cache: quantising write, its values, decode attention over
+// it.  (Chunked prefill turns the blocks into bf16, as for the 8-bit cache.)
+//
+//   minimum = min x,  scale = (max x - min x) / 15,  code = round((x - minimum) / scale)
+//
+// over the 64 dims of a half of a token's head: the halves that RoPE rotates
+// with one another.  With a minimum, all 16 levels lie between the extremes
+// also for keys whose channels have a mean.  Scale and minimum are bf16 and lie
+// in the token's own row: a token is written without reading its block, and a
+// block is copied, shared or moved as bytes.
+#include <algorithm>
+#include <stdexcept>
+
+#include "decode_split.cuh"
+#include "fewbit.cuh"
+#include "kv_int4.h"
+
+namespace cx {
+
+namespace kv4 {
+constexpr int D = 128, BS = 16, ROW = KV4_ROW;
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr uint32_t NAN_PAIR = 0x7fff7fffu;     // scale and minimum of a half without finite range
+}  // namespace kv4
+
+// --------------------------------------------------- RoPE + quantising write
+// Eight bf16 dims of a lane, eight lanes to a half: scale | minimum << 16, and
+// the lane's codes.
+__device__ __forceinline__ uint32_t quant4(const uint32_t (&w)[4], uint32_t& codes) {
+  float v[8], lo, hi;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = bf16_lo(w[i]);
+    v[2 * i + 1] = bf16_hi(w[i]);
+    odd |= (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
+  }
+  lo = hi = v[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    lo = fminf(lo, v[i]);
+    hi = fmaxf(hi, v[i]);
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.f));
+  const float s = __bfloat162float(sb);
+  odd |= !(s < INFINITY);                                // the range is no finite number
+  const uint32_t mates = 0xffu << (threadIdx.x & 24);
+  odd = (__ballot_sync(0xffffffffu, odd) & mates) != 0;
+  codes = 0;
+  if (odd) return kv4::NAN_PAIR;
+  const float inv = s > 0.f ? fminf(__fdiv_rn(1.f, s), 3.4028234e38f) : 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) codes |= min(__float2uint_rn((v[i] - lo) * inv), 15u) << (4 * i);
+  return (uint32_t)__bfloat16_as_ushort(sb) | (__float_as_uint(lo) & 0xffff0000u);   // lo is one of the bf16 values
+}
+
+// A warp: eight heads of a token, two at a time, eight dims of a lane.  q's
+// heads are rotated, k's rotated and quantised, v's quantised.
+__global__ void __launch_bounds__(kv4::THREADS)
+    rope_cache_int4_kernel(const __nv_bfloat16* qkv, int ldq, const int* __restrict__ pos,
+                           const float* __restrict__ cos_sin, const int64_t* __restrict__ slots, KvInt4 c,
+                           __nv_bfloat16* out, int ldo, int64_t units, int per_token, int Hq, int max_pos, int* status,
+                           const __nv_bfloat16* __restrict__ qn, const __nv_bfloat16* __restrict__ kn, float eps) {
+  using namespace kv4;
+  const int lane = threadIdx.x & 31, j = lane & 15;
+  const int64_t u = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (u >= units) return;
+  const int64_t t = u / per_token;
+  const int Hkv = c.Hkv, heads = Hq + 2 * Hkv, h0 = 8 * (int)(u - t * per_token) + (lane >> 4);
+  u128 raw[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    raw[k] = h0 + 2 * k < heads ? ld_v4(qkv + t * ldq + (int64_t)(h0 + 2 * k) * D + 8 * j) : u128{0, 0, 0, 0};
+  const int p = pos[t];
+  const int64_t slot = slots[t];
+  const bool pos_ok = p >= 0 && p < max_pos, cached = pos_ok && slot >= 0 && (slot >> 4) < c.num_blocks;
+  if (h0 == 0 && j == 0 && (!pos_ok || (slot >= 0 && !cached))) record_status(status, CX_ERR_BOUNDS);
+  float co[8], si[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) co[e] = si[e] = 0.f;
+  if (pos_ok) {
+    const float4* cs = reinterpret_cast<const float4*>(cos_sin + (int64_t)p * D + 8 * (j & 7));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      reinterpret_cast<float4*>(co)[e] = __ldg(cs + e);
+      reinterpret_cast<float4*>(si)[e] = __ldg(cs + D / 8 + e);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) si[e] = j < 8 ? -si[e] : si[e];      // a cos - b sin in the first half, a cos + b sin
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int h = h0 + 2 * k;
+    uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+    const bool turned = h < Hq + Hkv;
+    const __nv_bfloat16* nw = h < Hq ? qn : kn;
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ss += bf16_lo(w[e]) * bf16_lo(w[e]) + bf16_hi(w[e]) * bf16_hi(w[e]);
+    if (qn != nullptr || kn != nullptr) {
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (turned && nw != nullptr) {
+        // bf16 between the norm and the rotation, like a norm layer of its own
+        const float n = rsqrtf(ss * (1.0f / D) + eps);
+        const u128 g = ld_v4(nw + 8 * j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = pack_bf16x2(bf16_lo(w[e]) * n * bf16_lo(word(g, e)), bf16_hi(w[e]) * n * bf16_hi(word(g, e)));
+      }
+    }
+    uint32_t r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t b = __shfl_xor_sync(0xffffffffu, w[e], 8);      // the partner dims, 64 away
+      r[e] = pack_bf16x2(__fadd_rn(__fmul_rn(bf16_lo(w[e]), co[2 * e]), __fmul_rn(bf16_lo(b), si[2 * e])),
+                         __fadd_rn(__fmul_rn(bf16_hi(w[e]), co[2 * e + 1]), __fmul_rn(bf16_hi(b), si[2 * e + 1])));
+    }
+    if (h < Hq) {
+      st_v4(out + t * ldo + (int64_t)h * D + 8 * j, u128{r[0], r[1], r[2], r[3]});   // a position out of range: zeros
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = turned ? r[e] : w[e];         // what a bf16 cache would hold is quantised
+    if (!__any_sync(0xffffffffu, h >= Hq)) continue;
+    uint32_t codes;
+    const uint32_t par = quant4(w, codes);
+    if (!cached || h < Hq || h >= heads) continue;
+    const bool is_v = h >= Hq + Hkv;
+    uint8_t* row = (is_v ? c.v : c.k) +
+                   (((slot >> 4) * Hkv + (h - Hq - (is_v ? Hkv : 0))) * BS + (slot & 15)) * ROW;
+    *reinterpret_cast<uint32_t*>(row + 4 * j) = codes;
+    if ((j & 7) == 0) *reinterpret_cast<uint32_t*>(row + D / 2 + 4 * (j >> 3)) = par;
+  }
+}
+
+void rope_cache_int4(const void* qkv, int ldq, const int* pos, const float* cos_sin, const int64_t* slots,
+                     const KvInt4& c, void* out, int ldo, int T, int Hq, int max_pos, int* status, cudaStream_t s,
+                     const void* q_norm, const void* k_norm, float eps) {
+  if (T == 0) return;
+  const int per_token = (Hq + 2 * c.Hkv + 7) / 8;
+  const int64_t units = (int64_t)T * per_token, ctas = (units + kv4::WARPS - 1) / kv4::WARPS;
+  rope_cache_int4_kernel<<<(unsigned)ctas, kv4::THREADS, 0, s>>>(
+      reinterpret_cast<const __nv_bfloat16*>(qkv), ldq, pos, cos_sin, slots, c, reinterpret_cast<__nv_bfloat16*>(out), ldo,
+      units, per_token, Hq, max_pos, status, reinterpret_cast<const __nv_bfloat16*>(q_norm),
+      reinterpret_cast<const __nv_bfloat16*>(k_norm), eps);
+}
+
+// ------------------------------------------------------------------- values
+// Eight dims of a lane: one word of codes, 16 bytes out.
+__global__ void __launch_bounds__(kv4::THREADS)
+    kv_values_int4_kernel(const uint8_t* __restrict__ cache, __nv_bfloat16* __restrict__ out, int64_t words) {
+  using namespace kv4;
+  for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < words; i += (int64_t)gridDim.x * THREADS) {
+    const uint8_t* row = cache + (i >> 4) * ROW;
+    const int j = (int)(i & 15);
+    st_v4(out + i * 8, int4_values(*reinterpret_cast<const uint32_t*>(row + 4 * j),
+                                   *reinterpret_cast<const uint32_t*>(row + D / 2 + 4 * (j >> 3))));
+  }
+}
+
+void kv_values_int4(const void* cache, void* out, int64_t rows, int sms, cudaStream_t s) {
+  const int64_t words = rows * 16;
+  if (words == 0) return;
+  const int64_t ctas = std::min<int64_t>((words + kv4::THREADS - 1) / kv4::THREADS, (int64_t)sms * 8);
+  kv_values_int4_kernel<<<(unsigned)ctas, kv4::THREADS, 0, s>>>(reinterpret_cast<const uint8_t*>(cache),
+                                                                reinterpret_cast<__nv_bfloat16*>(out), words);
+}
+
+// ---------------------------------------------------------- decode attention
+// S = q.K^T and O^T = V^T.W^T on mma.sync m16n8k16 (f16 in, fp32 out), a query
+// row per sequence filling 4 or 8 of an MMA's columns: bytes decide, not tensor
+// work.  A code needs no conversion: four bits under a mask are an f16 number
+// already, the subnormal code * 2^-24 (the low half of a byte) or code * 2^-20
+// (the high half), exact in the product.  The factor 2^4 between the two kinds
+// is part of q for K, and of O's rows for V.
+//   K: lane (g = lane / 4, t = lane % 4) takes bytes [8 t, 8 t + 8) of a half of
+//      tokens g and g + 8: 16 dims, two words.  The contraction may take the
+//      dims in any order as long as q uses the same one.  S of each half comes
+//      out by itself; scale and minimum of a token are applied to it in fp32:
+//      x = sum_halves scale * S + minimum * sum(q).
+//   V: the lane takes word g of a half (8 dims) of tokens 2t, 2t + 1, 2t + 8,
+//      2t + 9 -- those whose weights S leaves in this lane -- and puts two
+//      tokens side by side.  Scale is part of the weight, weight * scale, held in f16 (2^-11 of each)
+//      relative to a running maximum of its own; the minimum's part, sum of
+//      weight * minimum, is one fp32 number per half.
+// q is scaled by a power of two per head into f16's range.
+//
+// Loads: a block of a head is 1152 contiguous bytes, one asynchronous bulk copy.
+// A warp has K and V of two pairs of blocks in a ring of four slots: one is read
+// while three are under way, without barriers between warps.
+namespace dec4 {
+struct Cfg {
+  static constexpr int WARPS = 4, THREADS = 32 * WARPS, BS = kv4::BS;
+  static constexpr int MIN_UNITS = 2 * WARPS, PAIR_COST = 4 * WARPS, SLACK = 2 * PAIR_COST;
+};
+constexpr int WARPS = Cfg::WARPS, THREADS = Cfg::THREADS, D = kv4::D, BS = kv4::BS, ROW = kv4::ROW;
+constexpr int ctas_per_sm(int nt) { return nt == 1 ? 4 : 3; }
+constexpr float RESCALE = 8.f;          // O is rescaled once mv has grown by this much: weights stay under 2^9
+constexpr int BLOCK = BS * ROW;         // of one head
+constexpr int SLOT = 2 * BLOCK;         // K (or V) of two blocks
+constexpr int SLOTS = 4;                // K, V, K, V
+constexpr int RING = WARPS * SLOTS * SLOT;
+constexpr int O_ROW = D + 4;            // floats of a head's row of O: eight lanes' stores fall on eight banks
+template <int NT>
+struct Smem {                           // rings, later the warps' O | their statistics | q fragments | barriers | sums
+  static constexpr int STATS = RING;
+  static_assert(WARPS * 8 * NT * O_ROW * 4 <= RING, "O fits in the drained rings");
+  static constexpr int Q = STATS + WARPS * 8 * NT * 32;
+  static constexpr int BAR = Q + NT * 4 * 32 * 16;
+  static constexpr int PRE = BAR + WARPS * SLOTS * 8;
+  static constexpr int bytes(int B) { return PRE + (B + 1) * 4; }
+};
+}  // namespace dec4
+
+// contiguous 16-byte multiples from global memory; completes `bytes` on `bar`
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ uint32_t lds4(uint32_t a) {
+  uint32_t r;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// NT: tiles of 8 query heads per KV head (1: groups up to 8, 2: up to 16).
+template <int NT>
+__global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
+    decode_attn_int4_kernel(const __nv_bfloat16* __restrict__ q, int ldq, KvInt4 c, const int* __restrict__ tables,
+                            int max_blocks, const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, int ldo,
+                            int B, int Hq, float scale_log2, float* __restrict__ part, uint32_t* __restrict__ counters,
+                            int* status) {
+  using namespace dec4;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* so = reinterpret_cast<float*>(smem);                           // [WARPS][8 NT][O_ROW], once the rings are drained
+  float* sm = reinterpret_cast<float*>(smem + Smem<NT>::STATS);         // [WARPS][8 NT][m, l, mv, -, z0, z1, -, -]
+  uint4* sq = reinterpret_cast<uint4*>(smem + Smem<NT>::Q);             // [NT][4 words][32 lanes]
+  int* pre = reinterpret_cast<int*>(smem + Smem<NT>::PRE);              // [B + 1] units of the pairs before sequence b
+  __shared__ uint32_t ticket;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int gq = lane >> 2, qd = lane & 3;
+  const int Hkv = c.Hkv, G = Hq / Hkv;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem<NT>::BAR) + warp * SLOTS;
+  if (lane == 0) {
+    for (int i = 0; i < SLOTS; ++i) mbar_init(&bars[i], 1);
+    fence_barrier_init();
+  }
+  const DecodeShare share = decode_share<Cfg>(ctx_lens, B, max_blocks, Hkv, pre, status);   // (its barriers order the init)
+  // rows without tokens: zeros
+  for (int b = blockIdx.x; b < B; b += gridDim.x)
+    if (pre[b + 1] == pre[b])
+      for (int i = tid; i < Hq * D / 8; i += THREADS) st_v4(out + (size_t)b * ldo + 8 * i, u128{0, 0, 0, 0});
+
+  const uint32_t ring = smem_u32(smem) + warp * (SLOTS * SLOT);
+  const uint32_t kget = gq * ROW + 8 * qd;             // + 32 for the second half, + 8 ROW for token g + 8
+  const uint32_t vget = 2 * qd * ROW + 4 * gq;
+  const uint32_t pget = 2 * qd * ROW + D / 2;          // scales and minima of the lane's tokens
+  uint32_t turn = 0;                                   // pairs of blocks that the warp has consumed
+  bool ok = true;                                      // false once a wait ran out
+
+  int b = share.b;
+  for (int u = share.u0; u < share.u1;) {
+    // ---- the blocks [j0, j1) of KV head h of sequence b
+    while (pre[b + 1] <= u) ++b;
+    const int units = (pre[b + 1] - pre[b]) / Hkv;
+    const int h = (u - pre[b]) / units;
+    const int pair0 = pre[b] + h * units;                      // first unit of the pair
+    const int j0 = max(0, u - pair0 - Cfg::PAIR_COST), j1 = min(units, share.u1 - pair0) - Cfg::PAIR_COST;
+    u = min(pair0 + units, share.u1);
+    if (j1 <= 0) continue;                                     // none but the pair's fixed cost
+    const int len = min(max(ctx_lens[b], 0), max_blocks * BS);
+
+    // ---- the warp's loads, two blocks at a time
+    int fj = j0 + 2 * warp, fcount = 0, ids = -1, id0 = -1, id1 = -1;
+    uint32_t given = 0;                                        // which of the two blocks there are, 2 bits for each turn's parity
+    auto next_ids = [&]() {
+      if ((fcount & 15) == 0) {                                // ids of the next 32 blocks, one per lane
+        const int mine = fj + (lane >> 1) * (2 * WARPS) + (lane & 1);
+        ids = -1;
+        if (mine < j1) {
+          ids = tables[(size_t)b * max_blocks + mine];
+          if (ids < 0 || ids >= c.num_blocks) {
+            record_status(status, CX_ERR_BOUNDS);
+            ids = -1;
+          }
+        }
+      }
+      id0 = __shfl_sync(0xffffffffu, ids, 2 * (fcount & 15));
+      id1 = __shfl_sync(0xffffffffu, ids, 2 * (fcount & 15) + 1);
+      fj += 2 * WARPS;
+      ++fcount;
+    };
+    auto fetch = [&](const uint8_t* cache, int slot) {
+      if (lane == 0) {
+        const uint32_t bytes = (id0 >= 0 ? BLOCK : 0) + (id1 >= 0 ? BLOCK : 0);
+        mbar_arrive_expect_tx(&bars[slot], bytes);
+        if (id0 >= 0) bulk_load(ring + slot * SLOT, cache + ((size_t)id0 * Hkv + h) * BLOCK, BLOCK, &bars[slot]);
+        if (id1 >= 0) bulk_load(ring + slot * SLOT + BLOCK, cache + ((size_t)id1 * Hkv + h) * BLOCK, BLOCK, &bars[slot]);
+      }
+    };
+    const int mine0 = j0 + 2 * warp;                           // the warp's first block
+    const int turns = mine0 < j1 ? (j1 - mine0 + 2 * WARPS - 1) / (2 * WARPS) : 0;
+    if (lane == 0) fence_proxy_async_smem();                   // O of the run before was written to the rings
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (i >= turns) continue;
+      const uint32_t par = (turn + i) & 1;
+      next_ids();
+      given = (given & ~(3u << 2 * par)) | ((id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u)) << 2 * par;
+      fetch(c.k, 2 * par);
+      fetch(c.v, 2 * par + 1);
+    }
+    // ---- q fragments: a word's dims 8w + {0, 4}, {2, 6}, {1, 5}, {3, 7}; warp i makes [.][i]
+    float qf[NT], qs[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const bool on = gq + 8 * nt < G;
+      u128 raw[4];                                             // [half][word]: dims half * 64 + qd * 16 + word * 8 ..
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        raw[i] = on ? ld_v4(q + (size_t)b * ldq + (size_t)(h * G + gq + 8 * nt) * D + (i >> 1) * 64 + qd * 16 + (i & 1) * 8)
+                    : u128{0, 0, 0, 0};
+      float am = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          am = fmaxf(am, fmaxf(finite_or_zero(bf16_lo(word(raw[i], e))), finite_or_zero(bf16_hi(word(raw[i], e)))));
+      am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+      am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
+      // am * 2^-eq in [2^14, 2^15)
+      const int eq = am > 0.f ? max((int)(__float_as_uint(am) >> 23) - 127 - 14, -126) : 0;
+      const float down = exp2_int(-eq);
+      qf[nt] = exp2_int(eq) * scale_log2;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a += (bf16_lo(word(raw[2 * half + i], e)) + bf16_hi(word(raw[2 * half + i], e))) * down;
+        a += __shfl_xor_sync(0xffffffffu, a, 1);
+        a += __shfl_xor_sync(0xffffffffu, a, 2);
+        qs[nt][half] = a * 5.9604645e-8f;                      // 2^-24
+      }
+      static_assert(WARPS == 4, "a warp per word");
+      const u128 w = warp == 0 ? raw[0] : warp == 1 ? raw[1] : warp == 2 ? raw[2] : raw[3];
+      const float d16 = down * 0.0625f;
+      sq[(nt * 4 + warp) * 32 + lane] =
+          make_uint4(pack_f16x2(bf16_lo(w.x) * down, bf16_lo(w.z) * down), pack_f16x2(bf16_lo(w.y) * down, bf16_lo(w.w) * down),
+                     pack_f16x2(bf16_hi(w.x) * d16, bf16_hi(w.z) * d16), pack_f16x2(bf16_hi(w.y) * d16, bf16_hi(w.w) * d16));
+    }
+    __syncthreads();
+
+    float o[NT][8][4], z[NT][2], m[NT], l[NT], mv[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt] = mv[nt] = -INFINITY;
+      l[nt] = z[nt][0] = z[nt][1] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][mt][e] = 0.f;
+    }
+    int i0 = 0;
+    for (; i0 < turns; ++i0, ++turn) {
+      const uint32_t par = turn & 1, phase = (turn >> 1) & 1;
+      const uint32_t sk = ring + 2 * par * SLOT, sv = sk + SLOT;
+      const int j = mine0 + i0 * 2 * WARPS;
+      const uint32_t here = given >> 2 * par & 3;
+      // what of the lane's tokens counts: bit 4 block + 2 (token + 8) + (token + 1)
+      const int tok0 = j * BS + 2 * qd;
+      uint32_t live = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if ((here >> (e >> 2) & 1) && tok0 + (e & 1) + (e >> 1 & 1) * 8 + (e >> 2) * BS < len) live |= 1u << e;
+      ok = ok && mbar_wait(&bars[2 * par], phase, status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      // ---- S of each half; x = sum of scale * S + minimum * sum(q)
+      float x[NT][8];
+      uint2 kp[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) kp[e] = lds8(sk + pget + (e >> 2) * BLOCK + ((e >> 1 & 1) * 8 + (e & 1)) * ROW);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float s[2][2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i][tt][e] = 0.f;
+        uint2 kw[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt) kw[i][tt] = lds8(sk + kget + half * 32 + i * BLOCK + tt * 8 * ROW);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          uint4 qa[NT];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) qa[nt] = sq[(nt * 4 + 2 * half + w) * 32 + lane];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+              const uint32_t a = w ? kw[i][tt].y : kw[i][tt].x, a8 = a >> 8;
+              mma_f16(s[i][tt], qa[0].x, NT == 2 ? qa[NT - 1].x : 0u, qa[0].y, NT == 2 ? qa[NT - 1].y : 0u,
+                      a & 0x000f000fu, a8 & 0x000f000fu);
+              mma_f16(s[i][tt], qa[0].z, NT == 2 ? qa[NT - 1].z : 0u, qa[0].w, NT == 2 ? qa[NT - 1].w : 0u,
+                      a & 0x00f000f0u, a8 & 0x00f000f0u);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t pr = half ? kp[e].y : kp[e].x;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float v = fmaf(bf16_lo(pr), s[e >> 2][e >> 1 & 1][2 * nt + (e & 1)], bf16_hi(pr) * qs[nt][half]);
+            x[nt][e] = half ? x[nt][e] + v : v;
+          }
+        }
+      }
+      __syncwarp();                                            // K has been read by all
+      const bool more = i0 + 2 < turns;
+      if (more) {
+        next_ids();
+        fetch(c.k, 2 * par);
+        given = (given & ~(3u << 2 * par)) | ((id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u)) << 2 * par;
+      }
+      ok = ok && mbar_wait(&bars[2 * par + 1], phase, status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      // ---- weights
+      float vs[2][8], vm[2][8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint2 pr = lds8(sv + pget + (e >> 2) * BLOCK + ((e >> 1 & 1) * 8 + (e & 1)) * ROW);
+        if (!(live >> e & 1)) pr = make_uint2(0, 0);           // rows never written may hold NaN
+        vs[0][e] = bf16_lo(pr.x);
+        vm[0][e] = bf16_hi(pr.x);
+        vs[1][e] = bf16_lo(pr.y);
+        vm[1][e] = bf16_hi(pr.y);
+      }
+      uint32_t wb[NT][2][4];                                   // B fragments of the second product, for each half
+      float alpha[NT];
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[nt][e] = live >> e & 1 ? x[nt][e] * 16777216.f * qf[nt] : -INFINITY;    // S counts in 2^-24
+          top = fmaxf(top, x[nt][e]);
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float m_new = fmaxf(m[nt], top), base = m_new == -INFINITY ? 0.f : m_new;
+        float p[8], big = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = ex2(x[nt][e] - base);
+          big = fmaxf(big, p[e] * fmaxf(vs[0][e], vs[1][e]));
+        }
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        const float keep = ex2(m[nt] - base);
+        l[nt] = l[nt] * keep + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
+        m[nt] = m_new;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float a = z[nt][half] * keep;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a = fmaf(p[e], vm[half][e], a);
+          z[nt][half] = a;
+        }
+        const float mt = base + lg2(big);                      // of x + log2 of V's scale
+        alpha[nt] = 1.f;
+        if (mt > mv[nt] + RESCALE || (mv[nt] == -INFINITY && mt > -INFINITY)) {
+          alpha[nt] = ex2(mv[nt] - mt);
+          mv[nt] = mt;
+          grow = true;
+        }
+        const float f = ex2(fminf(base - mv[nt], 126.f));      // no scale above 0 so far: 0 times a finite number
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            wb[nt][half][i] = pack_f16x2(p[2 * i] * f * vs[half][2 * i], p[2 * i + 1] * f * vs[half][2 * i + 1]);
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {                      // O^T's columns are heads 2 qd, 2 qd + 1
+          const float a0 = __shfl_sync(0xffffffffu, alpha[nt], 8 * qd), a1 = __shfl_sync(0xffffffffu, alpha[nt], 8 * qd + 4);
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) {
+            o[nt][mt][0] *= a0;
+            o[nt][mt][1] *= a1;
+            o[nt][mt][2] *= a0;
+            o[nt][mt][3] *= a1;
+          }
+        }
+      }
+      // ---- O^T
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {                          // blocks
+          uint32_t vw[4];                                      // tokens 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vw[e] = lds4(sv + vget + half * 32 + i * BLOCK + ((e >> 1) * 8 + (e & 1)) * ROW);
+#pragma unroll
+          for (int hw = 0; hw < 2; ++hw) {                     // dims 4 hw .. of the word, two tokens side by side
+            const uint32_t y = __byte_perm(vw[0], vw[1], hw ? 0x7632 : 0x5410), y8 = y >> 8;
+            const uint32_t w = __byte_perm(vw[2], vw[3], hw ? 0x7632 : 0x5410), w8 = w >> 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_f16(o[nt][4 * half + 2 * hw], y & 0x000f000fu, y8 & 0x000f000fu, w & 0x000f000fu, w8 & 0x000f000fu,
+                      wb[nt][half][2 * i], wb[nt][half][2 * i + 1]);
+              mma_f16(o[nt][4 * half + 2 * hw + 1], y & 0x00f000f0u, y8 & 0x00f000f0u, w & 0x00f000f0u, w8 & 0x00f000f0u,
+                      wb[nt][half][2 * i], wb[nt][half][2 * i + 1]);
+            }
+          }
+        }
+      __syncwarp();                                            // V has been read by all
+      if (more) fetch(c.v, 2 * par + 1);
+    }
+    if (!ok)   // a wait ran out (recorded): the copies under way get a bounded time to land before the CTA ends
+      for (uint32_t i = 0; i < 2 && i0 + (int)i < turns; ++i)
+        for (uint32_t kv = 0; kv < 2; ++kv)
+          mbar_wait(&bars[2 * ((turn + i) & 1) + kv], (turn + i) >> 1 & 1, nullptr, 100000000ull);
+    if (__syncthreads_or(!ok)) return;                         // every warp has drained its ring
+
+    // ---- the warps' results of this run
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], d);
+        z[nt][0] += __shfl_xor_sync(0xffffffffu, z[nt][0], d);
+        z[nt][1] += __shfl_xor_sync(0xffffffffu, z[nt][1], d);
+      }
+      if (qd == 0) {
+        float4* st = reinterpret_cast<float4*>(sm + (warp * 8 * NT + nt * 8 + gq) * 8);
+        st[0] = make_float4(m[nt], l[nt], mv[nt], 0.f);
+        st[1] = make_float4(z[nt][0], z[nt][1], 0.f, 0.f);
+      }
+      // dim half * 64 + 8 g + n in column (half * 8 + n) * 8 + g
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = (mt >> 1 & 1) * 4 + (mt & 1) + 2 * (e >> 1);
+          so[(warp * 8 * NT + nt * 8 + 2 * qd + (e & 1)) * O_ROW + ((mt >> 2) * 8 + n) * 8 + gq] =
+              o[nt][mt][e] * (mt & 1 ? 1048576.f : 16777216.f);
+        }
+    }
+    __syncthreads();
+    // the CTAs that share the pair: those of the cuts left inside it, and the one before
+    const int slack = decode_slack<Cfg>(units, share.most);
+    const int c0 = (pair0 + Cfg::PAIR_COST + slack) / share.per, c1 = (pair0 + units - slack - 1) / share.per;
+    // two heads at a time, a thread for two dims of one
+    for (int hh = tid >> 6; hh < G; hh += 2) {
+      const int d8 = tid & 7, d2 = tid >> 3 & 7, half = d2 >> 2, dim = half * 64 + 8 * d8 + 2 * (d2 & 3);
+      float M = -INFINITY, MV = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        M = fmaxf(M, sm[(w * 8 * NT + hh) * 8]);
+        MV = fmaxf(MV, sm[(w * 8 * NT + hh) * 8 + 2]);
+      }
+      const float mb = M == -INFINITY ? 0.f : M, vb = MV == -INFINITY ? 0.f : MV;
+      float2 num = make_float2(0.f, 0.f), zz = make_float2(0.f, 0.f);
+      float den = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float* p = so + (w * 8 * NT + hh) * O_ROW + 16 * d2 + d8;
+        const float* st = sm + (w * 8 * NT + hh) * 8;
+        const float f = ex2(st[2] - vb), fm = ex2(st[0] - mb);
+        num.x += p[0] * f;
+        num.y += p[8] * f;
+        den += st[1] * fm;
+        zz.x += st[4] * fm;
+        zz.y += st[5] * fm;
+      }
+      if (c0 >= c1) {
+        const float inv = den == 0.f ? 0.f : 1.f / den, f = ex2(vb - mb), zh = half ? zz.y : zz.x;
+        *reinterpret_cast<uint32_t*>(out + (size_t)b * ldo + (size_t)(h * G + hh) * D + dim) =
+            pack_bf16x2(fmaf(num.x, f, zh) * inv, fmaf(num.y, f, zh) * inv);
+      } else {   // slot 1 for the pair that goes on in the next CTA, 0 for one that began before
+        float* p = part + ((size_t)(blockIdx.x * 2 + ((int)blockIdx.x == c0)) * G + hh) * DEC4_ROW;
+        *reinterpret_cast<float2*>(p + dim) = num;
+        if ((tid & 63) == 0) {
+          *reinterpret_cast<float4*>(p + D) = make_float4(M, den, MV, 0.f);
+          *reinterpret_cast<float4*>(p + D + 4) = make_float4(zz.x, zz.y, 0.f, 0.f);
+        }
+      }
+    }
+    if (c0 < c1) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) ticket = atomicInc(&counters[b * Hkv + h], (uint32_t)(c1 - c0));
+      __syncthreads();
+      if (ticket == (uint32_t)(c1 - c0)) {
+        __threadfence();
+        // a warp per head: lanes over the CTAs for the statistics, over the dims for the sums
+        for (int hh = warp; hh < G; hh += WARPS) {
+          auto slot = [&](int cc) {
+            return part + ((size_t)(cc * 2 + (cc == c0)) * G + hh) * DEC4_ROW;
+          };
+          float m_all = -INFINITY, mv_all = -INFINITY, den = 0.f, z0 = 0.f, z1 = 0.f;
+          float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int cb = c0; cb <= c1; cb += 32) {              // 32 CTAs at a time, rescaled as the maxima grow
+            const int n = min(32, c1 - cb + 1);
+            float4 st = make_float4(-INFINITY, 0.f, -INFINITY, 0.f), zs = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (lane < n) {
+              st = __ldcg(reinterpret_cast<const float4*>(slot(cb + lane) + D));
+              zs = __ldcg(reinterpret_cast<const float4*>(slot(cb + lane) + D + 4));
+            }
+            const float m_new = fmaxf(m_all, warp_max(st.x)), mv_new = fmaxf(mv_all, warp_max(st.z));
+            const float mb = m_new == -INFINITY ? 0.f : m_new, vb = mv_new == -INFINITY ? 0.f : mv_new;
+            const float fv = ex2(mv_all - vb), fm = ex2(m_all - mb), mine = ex2(st.x - mb);
+            den = den * fm + st.y * mine;
+            z0 = z0 * fm + zs.x * mine;
+            z1 = z1 * fm + zs.y * mine;
+            num.x *= fv;
+            num.y *= fv;
+            num.z *= fv;
+            num.w *= fv;
+            m_all = m_new;
+            mv_all = mv_new;
+            const float f = ex2(st.z - vb);
+            for (int i = 0; i < n; i += 8) {
+              float4 y[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                y[k] = i + k < n ? __ldcg(reinterpret_cast<const float4*>(slot(cb + i + k)) + lane)
+                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float g = __shfl_sync(0xffffffffu, f, (i + k) & 31);
+                if (i + k < n) {
+                  num.x += y[k].x * g;
+                  num.y += y[k].y * g;
+                  num.z += y[k].z * g;
+                  num.w += y[k].w * g;
+                }
+              }
+            }
+          }
+          const float mb = m_all == -INFINITY ? 0.f : m_all, vb = mv_all == -INFINITY ? 0.f : mv_all;
+          den = warp_sum(den);
+          z0 = warp_sum(z0);
+          z1 = warp_sum(z1);
+          const float inv = den == 0.f ? 0.f : 1.f / den, f = ex2(vb - mb), zh = lane < 16 ? z0 : z1;
+          uint2 w;
+          w.x = pack_bf16x2(fmaf(num.x, f, zh) * inv, fmaf(num.y, f, zh) * inv);
+          w.y = pack_bf16x2(fmaf(num.z, f, zh) * inv, fmaf(num.w, f, zh) * inv);
+          *reinterpret_cast<uint2*>(out + (size_t)b * ldo + (size_t)(h * G + hh) * D + 4 * lane) = w;
+        }
+      }
+    }
+    fence_proxy_async_smem();                                  // the rings are copied into again
+    __syncthreads();                                           // O and the statistics have been read
+  }
+}
+
+static int decode_int4_resident(int B, int nt) {
+  const int smem = nt == 2 ? dec4::Smem<2>::bytes(B) : dec4::Smem<1>::bytes(B);
+  constexpr int PER_SM = 228 * 1024, OTHER = 1024 + 256;      // of a CTA: the system's, and the static variables
+  return std::min(dec4::ctas_per_sm(nt), PER_SM / (smem + OTHER));
+}
+long decode_int4_rows(int sms, int B, int Hkv, int G) {
+  const long row = (long)G * DEC4_ROW;
+  return 2L * sms * dec4::ctas_per_sm(1) + ((long)B * Hkv + row - 1) / row;
+}
+
+void decode_attention_int4(const void* q, int ldq, const KvInt4& c, const int* block_tables, int max_blocks,
+                           const int* ctx_lens, void* out, int ldo, int B, int Hq, float scale, float* ws, int sms,
+                           int* status, cudaStream_t s) {
+  if (B == 0) return;
+  const int G = Hq / c.Hkv, nt = G > 8 ? 2 : 1;
+  // the partial results (room for the largest grid) sit at the front, the counters behind them: neither
+  // moves with the batch
+  uint32_t* counters = reinterpret_cast<uint32_t*>(ws + 2L * sms * dec4::ctas_per_sm(1) * G * DEC4_ROW);
+  const long most = ((long)B * c.Hkv * (max_blocks + dec4::Cfg::PAIR_COST) + dec4::Cfg::MIN_UNITS - 1) / dec4::Cfg::MIN_UNITS;
+  const int grid = (int)std::max(1L, std::min((long)sms * decode_int4_resident(B, nt), most));
+  const int smem = nt == 2 ? dec4::Smem<2>::bytes(B) : dec4::Smem<1>::bytes(B);
+  auto kern = nt == 2 ? decode_attn_int4_kernel<2> : decode_attn_int4_kernel<1>;
+  static bool attr[64][2] = {};
+  int dev;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63][nt - 1]) {
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         nt == 2 ? dec4::Smem<2>::bytes(DEC4_MAX_BATCH) : dec4::Smem<1>::bytes(DEC4_MAX_BATCH));
+    cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    attr[dev & 63][nt - 1] = true;
+  }
+  kern<<<grid, dec4::THREADS, smem, s>>>(reinterpret_cast<const __nv_bfloat16*>(q), ldq, c, block_tables, max_blocks,
+                                         ctx_lens, reinterpret_cast<__nv_bfloat16*>(out), ldo, B, Hq,
+                                         scale * 1.4426950408889634f, ws, counters, status);
+}
+
+}  // namespace cx

@@ -118,6 +118,79 @@ def deinterleave_gate_up(w: torch.Tensor, tile: int = GATE_UP_TILE):
     return x[:, 0].reshape(-1, K), x[:, 1].reshape(-1, K)
 
 
+# --------------------------------------------------- block-scaled fp8
+FP8_BLOCK = 128         # columns (and, of a weight, rows) that share a scale
+
+
+def quantize_fp8(x: torch.Tensor, norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None):
+    """Rows ``x`` [T, K] (bf16) -> (e4m3 [T, K], fp32 scales [T, ceil(K / 128)]).
+
+    An element stands for value * scale, scale = largest magnitude of the
+    row's 128 columns / 448 (a largest magnitude under 2^-100 counts as
+    2^-100).  ``norm`` [K]: RMSNorm with these weights first, its result
+    quantised from fp32; up to 16384 columns.  Infinities and NaN become NaN and do
+    not count for the scale.  K must be a multiple of 16.  The scales of a
+    column block lie side by side (``scale`` may have any strides)."""
+    T, K = x.shape
+    if out is None:
+        out = torch.empty(T, K, dtype=torch.float8_e4m3fn, device=x.device)
+    if scale is None:
+        scale = torch.empty(-(-K // FP8_BLOCK), T, dtype=torch.float32, device=x.device).t()
+    _C.quantize_fp8(x, norm, eps, out, scale)
+    _n()
+    return out, scale
+
+
+def quantize_weight_fp8(w: torch.Tensor, out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None):
+    """A weight [N, K] (bf16) -> (e4m3 [N, K], fp32 scales [ceil(N / 128),
+    ceil(K / 128)]), one scale per block of 128 x 128, as in
+    :func:`quantize_fp8`."""
+    N, K = w.shape
+    if out is None:
+        out = torch.empty(N, K, dtype=torch.float8_e4m3fn, device=w.device)
+    if scale is None:
+        scale = torch.empty(-(-N // FP8_BLOCK), -(-K // FP8_BLOCK), dtype=torch.float32, device=w.device)
+    _C.quantize_weight_fp8(w, out, scale)
+    _n()
+    return out, scale
+
+
+def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+             out: Optional[torch.Tensor] = None, out_scale: Optional[torch.Tensor] = None, *,
+             residual: Optional[torch.Tensor] = None, silu_mul: bool = False,
+             status: Optional[torch.Tensor] = None):
+    """``a[M,K] @ b[N,K]^T`` of e4m3 operands with a scale for each block of 128.
+
+    ``a_scale`` fp32 [M, ceil(K / 128)] (:func:`quantize_fp8`), ``b_scale``
+    fp32 [ceil(N / 128), ceil(K / 128)] (:func:`quantize_weight_fp8`, or a
+    checkpoint's), any strides; both scales are arbitrary numbers.  Sums are
+    fp32, the scales are applied to the sum of each block of 128 columns.  K
+    must be a multiple of 16 and N of 8.
+
+    Returns bf16 [M, N]; ``residual`` (bf16, may be ``out``) is added to it.
+    ``silu_mul``: ``b`` holds gate and up rows in turns of 128
+    (:func:`interleave_gate_up`, N a multiple of 256), and the result is
+    SiLU(gate) * up of width N / 2, quantised from fp32 for the next product:
+    (e4m3 [M, N / 2], scales [M, N / 256]).  With a bf16 ``out`` it is stored as
+    bf16 instead, and ``out`` alone returned."""
+    M, N = a.shape[0], b.shape[0]
+    if out is None:
+        out = torch.empty(M, N // 2 if silu_mul else N, dtype=torch.float8_e4m3fn if silu_mul else torch.bfloat16,
+                          device=a.device)
+    quantised = out.dtype == torch.float8_e4m3fn
+    if quantised and out_scale is None:
+        out_scale = torch.empty(-(-out.shape[1] // FP8_BLOCK), M, dtype=torch.float32, device=a.device).t()
+    if not quantised and out_scale is not None:
+        raise ValueError("gemm_fp8: scales go with a float8_e4m3fn out")
+    if silu_mul and residual is not None:
+        raise ValueError("gemm_fp8: no residual with silu_mul")
+    epi = EPI_SILU_MUL if silu_mul else (EPI_ADD if residual is not None else EPI_STORE)
+    _C.gemm_fp8(a, a_scale, b, b_scale, out, out_scale, residual, epi, status)
+    _n()
+    return (out, out_scale) if quantised else out
+
+
 # ------------------------------------------------------------- layers
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[torch.Tensor] = None,
             residual: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -341,6 +414,19 @@ def decode_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     return out
 
 
+def _prefill_workspaces(q, block_tables, tile_info, n_q_heads, n_kv_heads, n_blocks):
+    """The bf16 blocks, the plan's words and the partial results of a chunked prefill over a quantised cache."""
+    n_blocks = block_tables.numel() if n_blocks is None else max(0, min(n_blocks, block_tables.numel()))
+    kv = torch.empty(2, n_blocks, n_kv_heads, 16, 128, dtype=torch.bfloat16, device=q.device)
+    ints = part = None
+    if q.is_cuda:
+        n_ints, n_part = _C.prefill_fp8_words(q.device.index, block_tables.numel(), tile_info.shape[0],
+                                             n_q_heads // max(1, n_kv_heads))
+        ints = torch.empty(n_ints, dtype=torch.int32, device=q.device)
+        part = torch.empty(n_part, dtype=torch.float32, device=q.device)
+    return kv, ints, part
+
+
 def prefill_attention_paged_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                                 k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
                                 tile_info: torch.Tensor, n_q_heads: int, n_kv_heads: int,
@@ -365,17 +451,106 @@ def prefill_attention_paged_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache:
     are then wrong)."""
     if out is None:
         out = torch.empty(q.shape[0], n_q_heads * 128, dtype=q.dtype, device=q.device)
-    n_blocks = block_tables.numel() if n_blocks is None else max(0, min(n_blocks, block_tables.numel()))
-    kv = torch.empty(2, n_blocks, n_kv_heads, 16, 128, dtype=torch.bfloat16, device=q.device)
-    ints = part = None
-    if q.is_cuda:
-        n_ints, n_part = _C.prefill_fp8_words(q.device.index, block_tables.numel(), tile_info.shape[0],
-                                             n_q_heads // max(1, n_kv_heads))
-        ints = torch.empty(n_ints, dtype=torch.int32, device=q.device)
-        part = torch.empty(n_part, dtype=torch.float32, device=q.device)
+    kv, ints, part = _prefill_workspaces(q, block_tables, tile_info, n_q_heads, n_kv_heads, n_blocks)
     _C.prefill_attention_paged_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tables, out, tile_info, n_q_heads,
                                    n_kv_heads, scale if scale is not None else 1.0 / math.sqrt(128), kv, ints, part,
                                    status)
+    _n(2)
+    return out
+
+
+# ------------------------------------------------------ 4-bit KV cache
+# Bytes of a cached token's head: 64 of 4-bit codes (dims 2i and 2i + 1 in the
+# low and the high half of byte i), then scale and minimum, bf16 each, of dims
+# 0..63 and of dims 64..127.
+KV_INT4_ROW = _C.KV_INT4_ROW
+
+
+def rope_cache_int4(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, n_q_heads: int,
+                    n_kv_heads: int, slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None,
+                    q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
+                    eps: float = 1e-6) -> torch.Tensor:
+    """Rotate q and k of the fused QKV rows and quantise k and v into a 4-bit
+    paged cache; returns the rotated q [T, Hq * 128] (``out``; may be
+    ``qkv[:, :Hq * 128]``).  ``qkv``'s k and v columns stay as they are.
+
+    ``k_cache`` / ``v_cache``: uint8 [blocks, Hkv, 16, 72] (``KV_INT4_ROW``).
+    A code stands for minimum + code * scale, with the minimum of a half (64
+    dims) of the token's head and scale = (maximum - minimum) / 15, rounded to
+    bf16.  k is rounded to bf16 before, as a bf16 cache would hold it.  A half
+    with an infinity or NaN, or whose range is no finite fp32 number, reads as
+    NaN throughout.  A row with slot < 0 is not cached; one with a position or
+    slot out of range is not cached either and recorded in ``status`` (a
+    position out of range also gives a q of zeros).  Give a slot once per
+    call: of two rows for one, parts of each may be left.
+    ``q_norm`` / ``k_norm`` as in :func:`rope_cache`."""
+    if out is None:
+        out = torch.empty(qkv.shape[0], n_q_heads * 128, dtype=qkv.dtype, device=qkv.device)
+    _C.rope_cache_int4(qkv, positions, cos_sin, slot_mapping, k_cache, v_cache, out, n_q_heads, n_kv_heads, status,
+                       q_norm, k_norm, eps)
+    _n()
+    return out
+
+
+def kv_values_int4(cache: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """What a 4-bit cache (or any rows of one) [..., 72] stands for, rounded to
+    bf16: [..., 128]."""
+    if out is None:
+        out = torch.empty(*cache.shape[:-1], 128, dtype=torch.bfloat16, device=cache.device)
+    _C.kv_values_int4(cache, out)
+    _n()
+    return out
+
+
+def decode_workspace_int4(batch: int, n_q_heads: int, n_kv_heads: int, device) -> torch.Tensor:
+    """Workspace of :func:`decode_attention_int4` for up to ``batch`` sequences:
+    zero before its first use, and left ready for the next call.  Calls that
+    may run at the same time (on different streams, or graphs replayed side
+    by side) each need their own."""
+    if n_kv_heads <= 0 or n_q_heads <= 0 or n_q_heads % n_kv_heads:
+        raise ValueError("decode_workspace_int4: the query heads must be a multiple of the KV heads")
+    g = n_q_heads // n_kv_heads
+    if g > 16:
+        raise ValueError("decode_workspace_int4: at most 16 query heads per KV head")
+    device = torch.device(device)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return torch.zeros(_C.decode_int4_rows(index, batch, n_kv_heads, g), g * _C.DECODE_INT4_ROW, dtype=torch.float32,
+                       device=device)
+
+
+def decode_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                          ctx_lens: torch.Tensor, n_q_heads: int, workspace: torch.Tensor,
+                          out: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                          status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One query row per sequence over its 4-bit paged cache (see
+    :func:`rope_cache_int4`), up to 16 query heads per KV head.  ``q``
+    [B, >= Hq * 128] (q heads first), ``ctx_lens`` [B] tokens to attend to (0: a
+    row of zeros), ``block_tables`` [B, max_blocks].  The weights, V's scales
+    in them, are held in f16 (2^-11 of each) next to fp32 sums.  The work is
+    divided on the device from ``ctx_lens``, so a captured call stays balanced
+    for any lengths.  A block id out of range is left out, and a length beyond
+    the table cut, both recorded in ``status``."""
+    if out is None:
+        out = torch.empty(q.shape[0], n_q_heads * 128, dtype=q.dtype, device=q.device)
+    _C.decode_attention_int4(q, k_cache, v_cache, block_tables, ctx_lens, out, n_q_heads,
+                             scale if scale is not None else 1.0 / math.sqrt(128), workspace, status)
+    _n()
+    return out
+
+
+def prefill_attention_paged_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                 block_tables: torch.Tensor, tile_info: torch.Tensor, n_q_heads: int,
+                                 n_kv_heads: int, out: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                                 status: Optional[torch.Tensor] = None, n_blocks: Optional[int] = None) -> torch.Tensor:
+    """:func:`prefill_attention_paged_fp8` over a 4-bit cache: the same
+    arguments but for the scales, the same workspaces and bounds.  The blocks
+    are turned into bf16 for the product (2^-9 of each value)."""
+    if out is None:
+        out = torch.empty(q.shape[0], n_q_heads * 128, dtype=q.dtype, device=q.device)
+    kv, ints, part = _prefill_workspaces(q, block_tables, tile_info, n_q_heads, n_kv_heads, n_blocks)
+    _C.prefill_attention_paged_int4(q, k_cache, v_cache, block_tables, out, tile_info, n_q_heads, n_kv_heads,
+                                    scale if scale is not None else 1.0 / math.sqrt(128), kv, ints, part, status)
     _n(2)
     return out
 

@@ -169,6 +169,87 @@ def paged_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx
     return out, mag
 
 
+# ---- block-scaled fp8 (64-bit arithmetic)
+def fp8_block_values(q, scale):
+    """What e4m3 [R, K] with scales [R or ceil(R / 128), ceil(K / 128)] stands for."""
+    R, K = q.shape
+    if scale.shape[0] != R:
+        scale = scale.repeat_interleave(128, 0)[:R]
+    return q.double() * scale.double().repeat_interleave(128, 1)[:, :K]
+
+
+def fp8_block_scale(x, rows=1):
+    """Scales of ``x`` [R, K] in blocks of ``rows`` x 128: largest finite magnitude / 448, of at least 2^-100."""
+    R, K = x.shape
+    f = torch.zeros(-(-R // rows) * rows, -(-K // 128) * 128, dtype=torch.float64, device=x.device)
+    f[:R, :K] = torch.where(torch.isfinite(x), x.double().abs(), torch.zeros_like(x, dtype=torch.float64))
+    return f.view(f.shape[0] // rows, rows, -1, 128).amax((1, 3)).clamp(min=2.0 ** -100) / 448
+
+
+def gemm_fp8(a, a_scale, b, b_scale, residual=None):
+    y = fp8_block_values(a, a_scale) @ fp8_block_values(b, b_scale).t()
+    return y if residual is None else y + residual.double()
+
+
+def silu_mul_columns(y, tile=256):
+    """SiLU(gate) * up of columns [.., N] that alternate in blocks of tile / 2."""
+    g, u = (t.flatten(-2) for t in y.unflatten(-1, (-1, 2, tile // 2)).unbind(-2))
+    return g * torch.sigmoid(g) * u
+
+
+# ---- 4-bit KV cache (64-bit arithmetic)
+def int4_values(rows):
+    """uint8 [..., 72] -> fp64 [..., 128]."""
+    code = torch.stack([rows[..., :64] & 15, rows[..., :64] >> 4], -1).flatten(-2).double().unflatten(-1, (2, 64))
+    par = rows[..., 64:].contiguous().view(torch.bfloat16).double()
+    return (code * par[..., 0::2, None] + par[..., 1::2, None]).flatten(-2)
+
+
+def int4_rows(x):
+    """bf16 [..., 128] -> uint8 [..., 72]."""
+    h = x.double().unflatten(-1, (2, 64))
+    lo, hi = h.amin(-1), h.amax(-1)
+    scale = ((hi - lo) / 15).to(torch.bfloat16)
+    s = scale.double()[..., None]
+    code = torch.where(s > 0, (h - lo[..., None]) / s.clamp(min=1e-300), torch.zeros_like(h)).round().clamp(0, 15)
+    code = code.nan_to_num(0.0).to(torch.uint8).flatten(-2)
+    bad = ~torch.isfinite(scale.float()) | ~torch.isfinite(h).all(-1)
+    par = torch.stack([scale, lo.to(torch.bfloat16)], -1)
+    par = torch.where(bad[..., None], torch.full_like(par, math.nan), par)
+    code = torch.where(bad.repeat_interleave(64, -1), torch.zeros_like(code), code)
+    return torch.cat([code[..., 0::2] | code[..., 1::2] << 4, par.flatten(-2).contiguous().view(torch.uint8)], -1)
+
+
+def int4_append(cache, rows, slots):
+    """In place: ``rows`` [T, Hkv, 128] (bf16) into their slots of [blocks, Hkv, 16, 72]; slots < 0 are skipped."""
+    keep = slots >= 0
+    s = slots[keep]
+    cache[s // 16, :, s % 16] = int4_rows(rows[keep])
+
+
+def paged_attention_int4(q, k_cache, v_cache, block_tables, ctx, n_new, scale=None):
+    """:func:`paged_attention_fp8` over a 4-bit cache: outputs and the same sums over |v|, fp64."""
+    T, Hq, D = q.shape
+    Hkv = k_cache.shape[1]
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    out = torch.zeros(T, Hq, D, dtype=torch.float64, device=q.device)
+    mag = torch.zeros_like(out)
+    s = 0
+    for b, (c, n) in enumerate(zip(ctx, n_new)):
+        tot = c + n
+        if tot > 0 and n > 0:
+            ids = block_tables[b, :(tot + 15) // 16].long()
+            k, v = (int4_values(x[ids]).transpose(0, 1).reshape(Hkv, -1, D)[:, :tot].repeat_interleave(Hq // Hkv, 0)
+                    for x in (k_cache, v_cache))
+            a = (q[s:s + n].double().transpose(0, 1) @ k.transpose(1, 2)) * scale
+            late = torch.arange(tot, device=q.device) > (c + torch.arange(n, device=q.device))[:, None]
+            p = a.masked_fill(late, float("-inf")).softmax(-1)
+            out[s:s + n] = (p @ v).transpose(0, 1)
+            mag[s:s + n] = (p @ v.abs()).transpose(0, 1)
+        s += n
+    return out, mag
+
+
 def kv_copy_blocks(kv, pairs, scales=None):
     """In-place reference of kv_copy_blocks on plain tensors."""
     src, dst = pairs[:, 0].long(), pairs[:, 1].long()

@@ -172,27 +172,31 @@ void kv_values_int4(const void* cache, void* out, int64_t rows, int sms, cudaStr
 }
 
 // ---------------------------------------------------------- decode attention
-// S = q.K^T and O^T = V^T.W^T on mma.sync m16n8k16 (f16 in, fp32 out), a query
-// row per sequence filling 4 or 8 of an MMA's columns: bytes decide, not tensor
-// work.  A code needs no conversion: four bits under a mask are an f16 number
-// already, the subnormal code * 2^-24 (the low half of a byte) or code * 2^-20
-// (the high half), exact in the product.  The factor 2^4 between the two kinds
-// is part of q for K, and of O's rows for V.
+// S^T = K.q^T and O^T = V^T.W^T on mma.sync m16n8k16 (f16 in, fp32 out), the
+// query heads of a KV head being an MMA's eight columns: bytes decide, and the
+// instructions that take them apart, not tensor work.  A code needs no
+// conversion: four bits under a mask are an f16 number already, the subnormal
+// code * 2^-24 (the low half of a byte) or code * 2^-20 (the high half), exact in
+// the product.  The factor 2^4 between the two kinds is part of q for K, and of
+// O's rows for V.
 //   K: lane (g = lane / 4, t = lane % 4) takes bytes [8 t, 8 t + 8) of a half of
 //      tokens g and g + 8: 16 dims, two words.  The contraction may take the
 //      dims in any order as long as q uses the same one.  S of each half comes
-//      out by itself; scale and minimum of a token are applied to it in fp32:
-//      x = sum_halves scale * S + minimum * sum(q).
-//   V: the lane takes word g of a half (8 dims) of tokens 2t, 2t + 1, 2t + 8,
-//      2t + 9 -- those whose weights S leaves in this lane -- and puts two
-//      tokens side by side.  Scale is part of the weight, weight * scale, held in f16 (2^-11 of each)
-//      relative to a running maximum of its own; the minimum's part, sum of
-//      weight * minimum, is one fp32 number per half.
-// q is scaled by a power of two per head into f16's range.
+//      out by itself, heads 2t and 2t + 1 of the lane's two tokens; scale and
+//      minimum are applied to it in fp32: x = sum_halves scale * S + minimum *
+//      sum(q).
+//   V: the weights, scale included (weight * scale, held in f16, 2^-11 of each, relative
+//      to a running maximum of their own), are turned round by movmatrix: the
+//      lane then holds head g of tokens 2t, 2t + 1, 2t + 8, 2t + 9, of which it
+//      takes word g of a half (8 dims), two tokens side by side.  The minimum's
+//      part, sum of weight * minimum, is one fp32 number per half.
+// q is scaled by a power of two per head into f16's range.  Both running maxima
+// move only once a weight has outgrown them by 2^8 and more, and the warp votes
+// on that: the steps in between have no shuffles and no rescaling.
 //
 // Loads: a block of a head is 1152 contiguous bytes, one asynchronous bulk copy.
-// A warp has K and V of two pairs of blocks in a ring of four slots: one is read
-// while three are under way, without barriers between warps.
+// A warp has K and V of two blocks in each of two stages, one read while the
+// other is under way, without barriers between warps.
 namespace dec4 {
 struct Cfg {
   static constexpr int WARPS = 4, THREADS = 32 * WARPS, BS = kv4::BS;
@@ -200,11 +204,12 @@ struct Cfg {
 };
 constexpr int WARPS = Cfg::WARPS, THREADS = Cfg::THREADS, D = kv4::D, BS = kv4::BS, ROW = kv4::ROW;
 constexpr int ctas_per_sm(int nt) { return nt == 1 ? 4 : 3; }
-constexpr float RESCALE = 8.f;          // O is rescaled once mv has grown by this much: weights stay under 2^9
+constexpr float LATE = 8.f;             // a logit may be this far above the running maximum: weights stay under 2^8
+constexpr uint32_t MOST_W = 0x70007000u;  // f16 pair of 2^13: beyond it the weights' own maximum moves
 constexpr int BLOCK = BS * ROW;         // of one head
-constexpr int SLOT = 2 * BLOCK;         // K (or V) of two blocks
-constexpr int SLOTS = 4;                // K, V, K, V
-constexpr int RING = WARPS * SLOTS * SLOT;
+constexpr int STAGE = 4 * BLOCK;        // K of two blocks, V of two blocks
+constexpr int STAGES = 2;
+constexpr int RING = WARPS * STAGES * STAGE;
 constexpr int O_ROW = D + 4;            // floats of a head's row of O: eight lanes' stores fall on eight banks
 template <int NT>
 struct Smem {                           // rings, later the warps' O | their statistics | q fragments | barriers | sums
@@ -212,7 +217,7 @@ struct Smem {                           // rings, later the warps' O | their sta
   static_assert(WARPS * 8 * NT * O_ROW * 4 <= RING, "O fits in the drained rings");
   static constexpr int Q = STATS + WARPS * 8 * NT * 32;
   static constexpr int BAR = Q + NT * 4 * 32 * 16;
-  static constexpr int PRE = BAR + WARPS * SLOTS * 8;
+  static constexpr int PRE = BAR + WARPS * STAGES * 8;
   static constexpr int bytes(int B) { return PRE + (B + 1) * 4; }
 };
 }  // namespace dec4
@@ -233,6 +238,38 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// the 8 x 8 matrix of 16-bit elements that a warp holds in rows, transposed
+__device__ __forceinline__ uint32_t turned8x8(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ bool any_above_f16x2(uint32_t a, uint32_t b) {     // in either half
+  uint32_t r;
+  asm("set.gt.u32.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r != 0;
+}
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// the largest over the lanes of the same t: tokens
+__device__ __forceinline__ float tokens_max(float a) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+  return a;
+}
+__device__ __forceinline__ float tokens_sum(float a) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  return a;
+}
 
 // NT: tiles of 8 query heads per KV head (1: groups up to 8, 2: up to 16).
 template <int NT>
@@ -248,12 +285,13 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
   uint4* sq = reinterpret_cast<uint4*>(smem + Smem<NT>::Q);             // [NT][4 words][32 lanes]
   int* pre = reinterpret_cast<int*>(smem + Smem<NT>::PRE);              // [B + 1] units of the pairs before sequence b
   __shared__ uint32_t ticket;
+  __shared__ __align__(16) float sqf[8 * NT][4];                        // of a head: factor of the logits, sums of q
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gq = lane >> 2, qd = lane & 3;
   const int Hkv = c.Hkv, G = Hq / Hkv;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem<NT>::BAR) + warp * SLOTS;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem<NT>::BAR) + warp * STAGES;
   if (lane == 0) {
-    for (int i = 0; i < SLOTS; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < STAGES; ++i) mbar_init(&bars[i], 1);
     fence_barrier_init();
   }
   const DecodeShare share = decode_share<Cfg>(ctx_lens, B, max_blocks, Hkv, pre, status);   // (its barriers order the init)
@@ -262,10 +300,10 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
     if (pre[b + 1] == pre[b])
       for (int i = tid; i < Hq * D / 8; i += THREADS) st_v4(out + (size_t)b * ldo + 8 * i, u128{0, 0, 0, 0});
 
-  const uint32_t ring = smem_u32(smem) + warp * (SLOTS * SLOT);
+  const uint32_t ring = smem_u32(smem) + warp * (STAGES * STAGE);
   const uint32_t kget = gq * ROW + 8 * qd;             // + 32 for the second half, + 8 ROW for token g + 8
   const uint32_t vget = 2 * qd * ROW + 4 * gq;
-  const uint32_t pget = 2 * qd * ROW + D / 2;          // scales and minima of the lane's tokens
+  const uint32_t pget = gq * ROW + D / 2;              // scales and minima of token g
   uint32_t turn = 0;                                   // pairs of blocks that the warp has consumed
   bool ok = true;                                      // false once a wait ran out
 
@@ -282,11 +320,14 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
     const int len = min(max(ctx_lens[b], 0), max_blocks * BS);
 
     // ---- the warp's loads, two blocks at a time
-    int fj = j0 + 2 * warp, fcount = 0, ids = -1, id0 = -1, id1 = -1;
-    uint32_t given = 0;                                        // which of the two blocks there are, 2 bits for each turn's parity
-    auto next_ids = [&]() {
+    const int mine0 = j0 + 2 * warp;                           // the warp's first block
+    const int turns = mine0 < j1 ? (j1 - mine0 + 2 * WARPS - 1) / (2 * WARPS) : 0;
+    int fcount = 0, ids = -1;
+    uint32_t valid = 0, given = 0;          // blocks of `ids` that there are; of the stages' two blocks, 2 bits a stage
+    const uint8_t* mycache = (lane & 2 ? c.v : c.k) + (size_t)h * BLOCK;      // lanes 0..3: K, K, V, V
+    auto fetch = [&](uint32_t stage) {
       if ((fcount & 15) == 0) {                                // ids of the next 32 blocks, one per lane
-        const int mine = fj + (lane >> 1) * (2 * WARPS) + (lane & 1);
+        const int mine = mine0 + (fcount + (lane >> 1)) * (2 * WARPS) + (lane & 1);
         ids = -1;
         if (mine < j1) {
           ids = tables[(size_t)b * max_blocks + mine];
@@ -295,34 +336,23 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
             ids = -1;
           }
         }
+        valid = __ballot_sync(0xffffffffu, ids >= 0);
       }
-      id0 = __shfl_sync(0xffffffffu, ids, 2 * (fcount & 15));
-      id1 = __shfl_sync(0xffffffffu, ids, 2 * (fcount & 15) + 1);
-      fj += 2 * WARPS;
+      const int at = 2 * (fcount & 15);
+      const int id = __shfl_sync(0xffffffffu, ids, at + (lane & 1));
+      const uint32_t two = valid >> at & 3;
+      given = (given & ~(3u << 2 * stage)) | two << 2 * stage;
+      if (lane == 0) mbar_arrive_expect_tx(&bars[stage], __popc(two) * 2 * BLOCK);
+      __syncwarp();
+      if (lane < 4 && id >= 0)
+        bulk_load(ring + stage * STAGE + lane * BLOCK, mycache + (size_t)id * Hkv * BLOCK, BLOCK, &bars[stage]);
       ++fcount;
     };
-    auto fetch = [&](const uint8_t* cache, int slot) {
-      if (lane == 0) {
-        const uint32_t bytes = (id0 >= 0 ? BLOCK : 0) + (id1 >= 0 ? BLOCK : 0);
-        mbar_arrive_expect_tx(&bars[slot], bytes);
-        if (id0 >= 0) bulk_load(ring + slot * SLOT, cache + ((size_t)id0 * Hkv + h) * BLOCK, BLOCK, &bars[slot]);
-        if (id1 >= 0) bulk_load(ring + slot * SLOT + BLOCK, cache + ((size_t)id1 * Hkv + h) * BLOCK, BLOCK, &bars[slot]);
-      }
-    };
-    const int mine0 = j0 + 2 * warp;                           // the warp's first block
-    const int turns = mine0 < j1 ? (j1 - mine0 + 2 * WARPS - 1) / (2 * WARPS) : 0;
-    if (lane == 0) fence_proxy_async_smem();                   // O of the run before was written to the rings
+    fence_proxy_async_smem();                                  // O of the run before was written to the rings
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (i >= turns) continue;
-      const uint32_t par = (turn + i) & 1;
-      next_ids();
-      given = (given & ~(3u << 2 * par)) | ((id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u)) << 2 * par;
-      fetch(c.k, 2 * par);
-      fetch(c.v, 2 * par + 1);
-    }
+    for (uint32_t i = 0; i < STAGES; ++i)
+      if ((int)i < turns) fetch((turn + i) & 1);
     // ---- q fragments: a word's dims 8w + {0, 4}, {2, 6}, {1, 5}, {3, 7}; warp i makes [.][i]
-    float qf[NT], qs[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const bool on = gq + 8 * nt < G;
@@ -342,17 +372,20 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
       // am * 2^-eq in [2^14, 2^15)
       const int eq = am > 0.f ? max((int)(__float_as_uint(am) >> 23) - 127 - 14, -126) : 0;
       const float down = exp2_int(-eq);
-      qf[nt] = exp2_int(eq) * scale_log2;
+      if (warp == 0) {
+        float qs[2];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float a = 0.f;
+        for (int half = 0; half < 2; ++half) {
+          float a = 0.f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) a += (bf16_lo(word(raw[2 * half + i], e)) + bf16_hi(word(raw[2 * half + i], e))) * down;
-        a += __shfl_xor_sync(0xffffffffu, a, 1);
-        a += __shfl_xor_sync(0xffffffffu, a, 2);
-        qs[nt][half] = a * 5.9604645e-8f;                      // 2^-24
+            for (int e = 0; e < 4; ++e) a += (bf16_lo(word(raw[2 * half + i], e)) + bf16_hi(word(raw[2 * half + i], e))) * down;
+          a += __shfl_xor_sync(0xffffffffu, a, 1);
+          a += __shfl_xor_sync(0xffffffffu, a, 2);
+          qs[half] = a * 5.9604645e-8f;                        // S counts in 2^-24
+        }
+        if (qd == 0) *reinterpret_cast<float4*>(sqf[8 * nt + gq]) = make_float4(exp2_int(eq) * scale_log2, qs[0], qs[1], 0.f);
       }
       static_assert(WARPS == 4, "a warp per word");
       const u128 w = warp == 0 ? raw[0] : warp == 1 ? raw[1] : warp == 2 ? raw[2] : raw[3];
@@ -363,156 +396,211 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
     }
     __syncthreads();
 
-    float o[NT][8][4], z[NT][2], m[NT], l[NT], mv[NT];
+    // of heads 8 nt + 2 qd + {0, 1}: the logits' factor, sums of q, running maximum m of the logits, sum l, sums z of
+    // weight * minimum, running maximum mv of the weights times scales, f = 2^(m - mv)
+    float o[NT][8][4], z[NT][2][2], m[NT][2], l[NT][2], mv[NT][2], f[NT][2], qf[NT][2], qs[NT][2][2];
+    bool far = false;                                          // q beyond 2^100: 2^24 is not folded into its factor
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt] = mv[nt] = -INFINITY;
-      l[nt] = z[nt][0] = z[nt][1] = 0.f;
+#pragma unroll
+      for (int cc = 0; cc < 2; ++cc) {
+        const float4 t = *reinterpret_cast<const float4*>(sqf[8 * nt + 2 * qd + cc]);
+        qf[nt][cc] = t.x;
+        qs[nt][cc][0] = t.y;
+        qs[nt][cc][1] = t.z;
+        far |= fabsf(t.x) > 1e30f;
+        m[nt][cc] = mv[nt][cc] = -INFINITY;
+        f[nt][cc] = l[nt][cc] = z[nt][cc][0] = z[nt][cc][1] = 0.f;
+      }
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][mt][e] = 0.f;
     }
+    far = __any_sync(0xffffffffu, far);
+    if (!far)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        qf[nt][0] *= 16777216.f;
+        qf[nt][1] *= 16777216.f;
+      }
     int i0 = 0;
     for (; i0 < turns; ++i0, ++turn) {
-      const uint32_t par = turn & 1, phase = (turn >> 1) & 1;
-      const uint32_t sk = ring + 2 * par * SLOT, sv = sk + SLOT;
+      const uint32_t stage = turn & 1;
+      const uint32_t sk = ring + stage * STAGE, sv = sk + 2 * BLOCK;
       const int j = mine0 + i0 * 2 * WARPS;
-      const uint32_t here = given >> 2 * par & 3;
-      // what of the lane's tokens counts: bit 4 block + 2 (token + 8) + (token + 1)
-      const int tok0 = j * BS + 2 * qd;
-      uint32_t live = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if ((here >> (e >> 2) & 1) && tok0 + (e & 1) + (e >> 1 & 1) * 8 + (e >> 2) * BS < len) live |= 1u << e;
-      ok = ok && mbar_wait(&bars[2 * par], phase, status);
-      ok = __all_sync(0xffffffffu, ok);
+      const uint32_t here = given >> 2 * stage & 3;
+      const bool full = here == 3 && (j + 2) * BS <= len;      // the same for the whole warp
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars[stage], turn >> 1 & 1, status));
       if (!ok) break;
-      // ---- S of each half; x = sum of scale * S + minimum * sum(q)
-      float x[NT][8];
-      uint2 kp[8];
+      // ---- logits of tokens g and g + 8 of both blocks: x[nt][block][token][head]
+      float x[NT][2][2][2];
+      uint2 kp[2][2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) kp[e] = lds8(sk + pget + (e >> 2) * BLOCK + ((e >> 1 & 1) * 8 + (e & 1)) * ROW);
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) kp[i][tt] = lds8(sk + pget + i * BLOCK + tt * 8 * ROW);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        float s[2][2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][tt][e] = 0.f;
+        float s[NT][2][4];
         uint2 kw[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt) kw[i][tt] = lds8(sk + kget + half * 32 + i * BLOCK + tt * 8 * ROW);
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          uint4 qa[NT];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) qa[nt] = sq[(nt * 4 + 2 * half + w) * 32 + lane];
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt) {
-              const uint32_t a = w ? kw[i][tt].y : kw[i][tt].x, a8 = a >> 8;
-              mma_f16(s[i][tt], qa[0].x, NT == 2 ? qa[NT - 1].x : 0u, qa[0].y, NT == 2 ? qa[NT - 1].y : 0u,
-                      a & 0x000f000fu, a8 & 0x000f000fu);
-              mma_f16(s[i][tt], qa[0].z, NT == 2 ? qa[NT - 1].z : 0u, qa[0].w, NT == 2 ? qa[NT - 1].w : 0u,
-                      a & 0x00f000f0u, a8 & 0x00f000f0u);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t pr = half ? kp[e].y : kp[e].x;
+        for (int w = 0; w < 2; ++w)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const float v = fmaf(bf16_lo(pr), s[e >> 2][e >> 1 & 1][2 * nt + (e & 1)], bf16_hi(pr) * qs[nt][half]);
-            x[nt][e] = half ? x[nt][e] + v : v;
-          }
-        }
-      }
-      __syncwarp();                                            // K has been read by all
-      const bool more = i0 + 2 < turns;
-      if (more) {
-        next_ids();
-        fetch(c.k, 2 * par);
-        given = (given & ~(3u << 2 * par)) | ((id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u)) << 2 * par;
-      }
-      ok = ok && mbar_wait(&bars[2 * par + 1], phase, status);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      // ---- weights
-      float vs[2][8], vm[2][8];
+            const uint4 qa = sq[(nt * 4 + 2 * half + w) * 32 + lane];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        uint2 pr = lds8(sv + pget + (e >> 2) * BLOCK + ((e >> 1 & 1) * 8 + (e & 1)) * ROW);
-        if (!(live >> e & 1)) pr = make_uint2(0, 0);           // rows never written may hold NaN
-        vs[0][e] = bf16_lo(pr.x);
-        vm[0][e] = bf16_hi(pr.x);
-        vs[1][e] = bf16_lo(pr.y);
-        vm[1][e] = bf16_hi(pr.y);
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t a = w ? kw[i][0].y : kw[i][0].x, a8 = a >> 8, e = w ? kw[i][1].y : kw[i][1].x, e8 = e >> 8;
+              if (w == 0)
+                mma_f16_first(s[nt][i], a & 0x000f000fu, e & 0x000f000fu, a8 & 0x000f000fu, e8 & 0x000f000fu, qa.x, qa.y);
+              else
+                mma_f16(s[nt][i], a & 0x000f000fu, e & 0x000f000fu, a8 & 0x000f000fu, e8 & 0x000f000fu, qa.x, qa.y);
+              mma_f16(s[nt][i], a & 0x00f000f0u, e & 0x00f000f0u, a8 & 0x00f000f0u, e8 & 0x00f000f0u, qa.z, qa.w);
+            }
+          }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt) {
+            const uint32_t pr = half ? kp[i][tt].y : kp[i][tt].x;
+            const float ps = bf16_lo(pr), pm = bf16_hi(pr);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int cc = 0; cc < 2; ++cc)
+                x[nt][i][tt][cc] = fmaf(ps, s[nt][i][2 * tt + cc],
+                                        half ? fmaf(pm, qs[nt][cc][1], x[nt][i][tt][cc]) : pm * qs[nt][cc][0]);
+          }
       }
-      uint32_t wb[NT][2][4];                                   // B fragments of the second product, for each half
-      float alpha[NT];
-      bool grow = false;
+      float vs[2][2][2], vm[2][2][2];                          // [half][block][token]
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+          const uint2 pr = lds8(sv + pget + i * BLOCK + tt * 8 * ROW);
+          vs[0][i][tt] = bf16_lo(pr.x);
+          vm[0][i][tt] = bf16_hi(pr.x);
+          vs[1][i][tt] = bf16_lo(pr.y);
+          vm[1][i][tt] = bf16_hi(pr.y);
+        }
+      if (far)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[nt][e >> 2][e >> 1 & 1][e & 1] *= 16777216.f;
+      // ---- weights: y = logit - m
+      float y[NT][2][2][2], top = -INFINITY;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          y[nt][e >> 2][e >> 1 & 1][e & 1] = fmaf(x[nt][e >> 2][e >> 1 & 1][e & 1], qf[nt][e & 1], -m[nt][e & 1]);
+      if (!full) {
+        // tokens behind the end, blocks that are not there: no weight, and what their rows hold does not count
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+            if (!(here >> i & 1) || (j + i) * BS + tt * 8 + gq >= len) {
+              vs[0][i][tt] = vs[1][i][tt] = vm[0][i][tt] = vm[1][i][tt] = 0.f;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                y[nt][i][tt][0] = y[nt][i][tt][1] = -INFINITY;
+            }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, y[nt][e >> 2][e >> 1 & 1][e & 1]);
+      if (__any_sync(0xffffffffu, top > LATE)) {               // m moves (from -inf: y is infinite, or not a number)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (y[nt][e >> 1][e & 1][cc] != -INFINITY) most = fmaxf(most, x[nt][e >> 1][e & 1][cc] * qf[nt][cc]);
+            const float now = fmaxf(m[nt][cc], tokens_max(most)), base = now == -INFINITY ? 0.f : now;
+            const float keep = ex2(m[nt][cc] - base);
+            l[nt][cc] *= keep;
+            z[nt][cc][0] *= keep;
+            z[nt][cc][1] *= keep;
+            m[nt][cc] = now;
+            f[nt][cc] = mv[nt][cc] == -INFINITY ? 0.f : ex2(fminf(base - mv[nt][cc], 126.f));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (y[nt][e >> 1][e & 1][cc] != -INFINITY)       // (the product is rounded in `now` and not here)
+                y[nt][e >> 1][e & 1][cc] = min_or_nan(fmaf(x[nt][e >> 1][e & 1][cc], qf[nt][cc], -base), 0.f);
+          }
+      }
+      uint32_t wb[NT][2][2][2];                                // [half][block][token]: heads 2 qd, 2 qd + 1
+      uint32_t big = 0;
+      bool fresh = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[nt][e] = live >> e & 1 ? x[nt][e] * 16777216.f * qf[nt] : -INFINITY;    // S counts in 2^-24
-          top = fmaxf(top, x[nt][e]);
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float m_new = fmaxf(m[nt], top), base = m_new == -INFINITY ? 0.f : m_new;
-        float p[8], big = 0.f;
+        for (int e = 0; e < 8; ++e) y[nt][e >> 2][e >> 1 & 1][e & 1] = ex2(y[nt][e >> 2][e >> 1 & 1][e & 1]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = ex2(x[nt][e] - base);
-          big = fmaxf(big, p[e] * fmaxf(vs[0][e], vs[1][e]));
-        }
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        const float keep = ex2(m[nt] - base);
-        l[nt] = l[nt] * keep + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
-        m[nt] = m_new;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float a = z[nt][half] * keep;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) a = fmaf(p[e], vm[half][e], a);
-          z[nt][half] = a;
-        }
-        const float mt = base + lg2(big);                      // of x + log2 of V's scale
-        alpha[nt] = 1.f;
-        if (mt > mv[nt] + RESCALE || (mv[nt] == -INFINITY && mt > -INFINITY)) {
-          alpha[nt] = ex2(mv[nt] - mt);
-          mv[nt] = mt;
-          grow = true;
-        }
-        const float f = ex2(fminf(base - mv[nt], 126.f));      // no scale above 0 so far: 0 times a finite number
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int cc = 0; cc < 2; ++cc) {
+          l[nt][cc] += (y[nt][0][0][cc] + y[nt][0][1][cc]) + (y[nt][1][0][cc] + y[nt][1][1][cc]);
 #pragma unroll
           for (int half = 0; half < 2; ++half)
-            wb[nt][half][i] = pack_f16x2(p[2 * i] * f * vs[half][2 * i], p[2 * i + 1] * f * vs[half][2 * i + 1]);
-      }
-      if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {                      // O^T's columns are heads 2 qd, 2 qd + 1
-          const float a0 = __shfl_sync(0xffffffffu, alpha[nt], 8 * qd), a1 = __shfl_sync(0xffffffffu, alpha[nt], 8 * qd + 4);
+            for (int e = 0; e < 4; ++e) z[nt][cc][half] = fmaf(y[nt][e >> 1][e & 1][cc], vm[half][e >> 1][e & 1], z[nt][cc][half]);
+          fresh |= f[nt][cc] == 0.f;
+        }
 #pragma unroll
-          for (int mt = 0; mt < 8; ++mt) {
-            o[nt][mt][0] *= a0;
-            o[nt][mt][1] *= a1;
-            o[nt][mt][2] *= a0;
-            o[nt][mt][3] *= a1;
+        for (int e = 0; e < 4; ++e) {
+          const float w0 = y[nt][e >> 1][e & 1][0] * f[nt][0], w1 = y[nt][e >> 1][e & 1][1] * f[nt][1];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            wb[nt][half][e >> 1][e & 1] = pack_f16x2(w0 * vs[half][e >> 1][e & 1], w1 * vs[half][e >> 1][e & 1]);
+            big = max_f16x2(big, wb[nt][half][e >> 1][e & 1]);
           }
         }
       }
+      if (__any_sync(0xffffffffu, fresh || any_above_f16x2(big, MOST_W))) {     // mv moves
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            float most = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              most = fmaxf(most, y[nt][e >> 1][e & 1][cc] * fmaxf(vs[0][e >> 1][e & 1], vs[1][e >> 1][e & 1]));
+            const float base = m[nt][cc] == -INFINITY ? 0.f : m[nt][cc];
+            const float mt = base + lg2(tokens_max(most));
+            if (mt > mv[nt][cc]) {
+              const float keep = ex2(mv[nt][cc] - mt);
+              mv[nt][cc] = mt;
+              f[nt][cc] = ex2(fminf(base - mt, 126.f));
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                o[nt][k][cc] *= keep;
+                o[nt][k][2 + cc] *= keep;
+              }
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+              wb[nt][half][e >> 1][e & 1] = pack_f16x2(y[nt][e >> 1][e & 1][0] * f[nt][0] * vs[half][e >> 1][e & 1],
+                                                       y[nt][e >> 1][e & 1][1] * f[nt][1] * vs[half][e >> 1][e & 1]);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) wb[nt][half][e >> 1][e & 1] = turned8x8(wb[nt][half][e >> 1][e & 1]);
       // ---- O^T
 #pragma unroll
       for (int half = 0; half < 2; ++half)
@@ -528,35 +616,34 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               mma_f16(o[nt][4 * half + 2 * hw], y & 0x000f000fu, y8 & 0x000f000fu, w & 0x000f000fu, w8 & 0x000f000fu,
-                      wb[nt][half][2 * i], wb[nt][half][2 * i + 1]);
+                      wb[nt][half][i][0], wb[nt][half][i][1]);
               mma_f16(o[nt][4 * half + 2 * hw + 1], y & 0x00f000f0u, y8 & 0x00f000f0u, w & 0x00f000f0u, w8 & 0x00f000f0u,
-                      wb[nt][half][2 * i], wb[nt][half][2 * i + 1]);
+                      wb[nt][half][i][0], wb[nt][half][i][1]);
             }
           }
         }
-      __syncwarp();                                            // V has been read by all
-      if (more) fetch(c.v, 2 * par + 1);
+      __syncwarp();                                            // the stage has been read by all
+      if (i0 + STAGES < turns) fetch(stage);
     }
     if (!ok)   // a wait ran out (recorded): the copies under way get a bounded time to land before the CTA ends
-      for (uint32_t i = 0; i < 2 && i0 + (int)i < turns; ++i)
-        for (uint32_t kv = 0; kv < 2; ++kv)
-          mbar_wait(&bars[2 * ((turn + i) & 1) + kv], (turn + i) >> 1 & 1, nullptr, 100000000ull);
+      for (uint32_t i = 0; i < STAGES && i0 + (int)i < turns; ++i)
+        mbar_wait(&bars[(turn + i) & 1], (turn + i) >> 1 & 1, nullptr, 100000000ull);
     if (__syncthreads_or(!ok)) return;                         // every warp has drained its ring
 
     // ---- the warps' results of this run
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], d);
-        z[nt][0] += __shfl_xor_sync(0xffffffffu, z[nt][0], d);
-        z[nt][1] += __shfl_xor_sync(0xffffffffu, z[nt][1], d);
+      for (int cc = 0; cc < 2; ++cc) {
+        const float ls = tokens_sum(l[nt][cc]), z0 = tokens_sum(z[nt][cc][0]), z1 = tokens_sum(z[nt][cc][1]);
+        if (gq == 0) {
+          float4* st = reinterpret_cast<float4*>(sm + (warp * 8 * NT + nt * 8 + 2 * qd + cc) * 8);
+          st[0] = make_float4(m[nt][cc], ls, mv[nt][cc], 0.f);
+          st[1] = make_float4(z0, z1, 0.f, 0.f);
+        }
       }
-      if (qd == 0) {
-        float4* st = reinterpret_cast<float4*>(sm + (warp * 8 * NT + nt * 8 + gq) * 8);
-        st[0] = make_float4(m[nt], l[nt], mv[nt], 0.f);
-        st[1] = make_float4(z[nt][0], z[nt][1], 0.f, 0.f);
-      }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
       // dim half * 64 + 8 g + n in column (half * 8 + n) * 8 + g
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt)
@@ -566,7 +653,6 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
           so[(warp * 8 * NT + nt * 8 + 2 * qd + (e & 1)) * O_ROW + ((mt >> 2) * 8 + n) * 8 + gq] =
               o[nt][mt][e] * (mt & 1 ? 1048576.f : 16777216.f);
         }
-    }
     __syncthreads();
     // the CTAs that share the pair: those of the cuts left inside it, and the one before
     const int slack = decode_slack<Cfg>(units, share.most);

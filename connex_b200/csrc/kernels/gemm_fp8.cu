@@ -203,9 +203,18 @@ void quantize_weight_fp8(const void* w, int64_t ldw, void* q, int64_t ldq, const
 //   warp 0      TMA: 128 x 128 bytes of A and 256 x 128 of B per stage, 128-byte swizzle
 //   warp 1      tcgen05.mma, M = 128, N = 256, K = 32 e4m3, four per stage: one block of 128 columns, into one of
 //               two accumulators in TMEM
+//   warp 3      the scales of the CTA's rows and of the tile's two blocks of B, up to sixteen blocks of 128 columns ahead (each
+//               is a line of its own: fetched one block ahead by the warps that use them they took longer than the MMAs)
 //   warps 4-11  promotion: two warpgroups; a thread takes a row, and columns [64 g, 64 g + 64) of both halves of
 //               the tile, reads the block's sums from TMEM, multiplies by the scales and adds in registers.  One
 //               accumulator is read while the MMAs fill the other.
+// What bounds it is the way round: an accumulator's MMAs (513 cycles), the word that it is complete (some 260), its
+// promotion by two warps on each SM quarter (350 to 600), the word that it is free (90).  Two accumulators of 256
+// columns are all of TMEM, so a block takes 700 cycles at least (an SM by itself, operands in place), 1000 here.
+// Measured on 8192 x 28672 x 4096 with SiLU(gate) * up, as variants of this kernel: pairs of CTAs on one tile of 256 x
+// 256 (cta_group::2) 1060 us, their way round being longer by two signals between SMs; four warpgroups of half the
+// columns 1190; four accumulators of 128 columns 1280 (the issuing thread falls behind); barriers waited for in
+// mbarrier.try_wait, which suspends, where single threads poll here, 1150.
 // A warpgroup holds gate and up of the same outputs, so SiLU(gate) * up needs no exchange; a row's largest value
 // over the tile's 128 outputs, for quantised output, passes through shared memory.
 namespace g8 {
@@ -213,14 +222,21 @@ constexpr int BM = 128, BN = 256, BK = 128;
 constexpr int STAGES = 4;
 constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
-// 128 fp32 sums of a thread and the block's next 32 need more than an equal share of the registers.  The
+// 128 fp32 sums of a thread and the block's next 64 need more than an equal share of the registers.  The
 // warpgroups' shares add up to no more than the block's at launch, 168 each.
 constexpr int REGS_AUX = 64, REGS_EPI = 216;
-static_assert(128 * REGS_AUX + 32 * EPI_WARPS * REGS_EPI <= THREADS * 168, "register shares");
+constexpr int REGS_ALL = 128 * REGS_AUX + 32 * EPI_WARPS * REGS_EPI;
+static_assert(REGS_ALL <= THREADS * 168, "register shares");
 constexpr int TMEM_COLS = 2 * BN;
-constexpr int SMEM = 1024 /* alignment */ + STAGES * STAGE_BYTES + 2 * 2 * BM * 4 /* row maxima */ + 256 /* barriers */;
-constexpr int GROUP = 16;            // tile-rows per raster band
+// scales of four blocks of columns at a time (one wait for all of them): the rows', then B's two of each
+constexpr int SC_SLOTS = 4, SC_KB = 4, SC_ROW = SC_KB * BM + 2 * SC_KB;
+constexpr int SMEM = 1024 /* alignment */ + STAGES * STAGE_BYTES + SC_SLOTS * SC_ROW * 4 + 2 * 2 * BM * 4 /* row maxima */ +
+                     512 /* barriers */;
+constexpr int GROUP = 16;             // tile-rows per raster band
 }  // namespace g8
+
+// x / (1 + e^-x) with the approximate quotient (2 ulp; beyond 2^126 it is 0, and so is the value nearly)
+__device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.0f + ex2(x * -1.4426950408889634f)); }
 
 template <int N>
 __device__ __forceinline__ void regs_dec() {
@@ -243,17 +259,21 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * A_BYTES;
-  float* tops = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);      // [tile parity][warpgroup][row]
+  float* scales = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);    // [slot][SC_ROW]
+  float* tops = scales + SC_SLOTS * SC_ROW;                                 // [tile parity][warpgroup][row]
   uint64_t* full = reinterpret_cast<uint64_t*>(tops + 2 * 2 * BM);
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;
   uint64_t* tempty = tfull + 2;
-  uint64_t* drain = tempty + 2;
+  uint64_t* sfull = tempty + 2;
+  uint64_t* sempty = sfull + SC_SLOTS;
+  uint64_t* drain = sempty + SC_SLOTS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
 
   const int warp = warp_id(), lane = lane_id();
   const int M = g.M, N = g.N, num_m = (M + BM - 1) / BM, num_n = (N + BN - 1) / BN;
   const int total = num_m * num_n, nk = (g.K + BK - 1) / BK;
+  const int first = blockIdx.x, step = gridDim.x;
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -263,6 +283,10 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
       mbar_init(&tempty[a], EPI_WARPS);
+    }
+    for (int i = 0; i < SC_SLOTS; ++i) {
+      mbar_init(&sfull[i], 32);
+      mbar_init(&sempty[i], EPI_WARPS);
     }
     mbar_init(drain, 1);
     fence_barrier_init();
@@ -283,11 +307,11 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
     regs_dec<REGS_AUX>();
     if (warp == 0 && lane == 0) {
       uint32_t stage = 0, phase = 0;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      for (int t = first; t < total && ok; t += step) {
         int tm, tn;
         tile_coords(t, num_m, num_n, GROUP, tm, tn);
         for (int kb = 0; kb < nk; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, status)) {
+          if (!mbar_wait_poll(&empty[stage], phase ^ 1, status)) {
             ok = false;
             break;
           }
@@ -306,9 +330,9 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
       constexpr uint32_t IDESC = umma_idesc_e4m3(BM, BN);
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
       bool issued = false;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      for (int t = first; t < total && ok; t += step) {
         for (int kb = 0; kb < nk; ++kb) {
-          if (!mbar_wait(&tempty[acc], acc_phase ^ 1, status) || !mbar_wait(&full[stage], phase, status)) {
+          if (!mbar_wait_poll(&tempty[acc], acc_phase ^ 1, status) || !mbar_wait_poll(&full[stage], phase, status)) {
             ok = false;
             break;
           }
@@ -318,8 +342,8 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
           for (int k = 0; k < BK / 32; ++k)
             umma_e4m3(tmem_base + acc * BN, umma_desc_sw128(a0 + k * 32), umma_desc_sw128(b0 + k * 32), IDESC, k != 0);
           issued = true;
-          umma_commit(&empty[stage]);
           umma_commit(&tfull[acc]);
+          umma_commit(&empty[stage]);
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
@@ -332,54 +356,85 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
         umma_commit(drain);
         mbar_wait(drain, 0, nullptr, 100000000ull);
       }
+    } else if (warp == 3) {
+      uint32_t slot = 0, phase = 0;
+      for (int t = first; t < total && ok; t += step) {
+        int tm, tn;
+        tile_coords(t, num_m, num_n, GROUP, tm, tn);
+        const int row0 = tm * BM + lane;
+        const float* src = lane < 2 ? g.sb.p + (int64_t)min(2 * tn + lane, (N - 1) / BK) * g.sb.row : nullptr;
+        for (int kb = 0; kb < nk; kb += SC_KB) {
+          ok = mbar_wait_warp(&sempty[slot], phase ^ 1, status);
+          if (!ok) break;
+          const uint32_t dst = smem_u32(scales + slot * SC_ROW);
+          for (int k = 0; k < min(SC_KB, nk - kb); ++k) {
+#pragma unroll
+            for (int i = 0; i < BM / 32; ++i) {
+              const int row = row0 + 32 * i;
+              cp_async4(dst + 4 * (k * BM + 32 * i + lane), g.sa.p + (row < M ? row * g.sa.row + (kb + k) * g.sa.col : 0),
+                        row < M);
+            }
+            if (lane < 2) cp_async4(dst + 4 * (SC_KB * BM + 2 * k + lane), src + (kb + k) * g.sb.col, true);
+          }
+          cp_async_arrive(&sfull[slot]);
+          if (++slot == SC_SLOTS) {
+            slot = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
     }
-    __syncwarp();
   } else {
     regs_inc<REGS_EPI>();
     // A warp reads the TMEM lanes of its number modulo four.  One whose wait ran out takes part in the barriers
     // all the same, so that the others reach their end, and stores nothing.
     const int quad = warp & 3, wg = (warp - 4) >> 2;
-    uint32_t acc = 0, acc_phase = 0;
+    uint32_t acc = 0, acc_phase = 0, slot = 0, sc_phase = 0;
     int parity = 0;
-    for (int t = blockIdx.x; t < total; t += gridDim.x, parity ^= 1) {
+    for (int t = first; t < total; t += step, parity ^= 1) {
       int tm, tn;
       tile_coords(t, num_m, num_n, GROUP, tm, tn);
       const int row_in = quad * 32 + lane, row = tm * BM + row_in;
       const bool in = row < M;
-      const float* sa = g.sa.p + (in ? row : 0) * g.sa.row;
-      const int nb_last = (N - 1) / BK;
-      const float* sb0 = g.sb.p + (int64_t)min(2 * tn, nb_last) * g.sb.row;
-      const float* sb1 = g.sb.p + (int64_t)min(2 * tn + 1, nb_last) * g.sb.row;
-      uint64_t sum[64];                       // columns 2i, 2i + 1 of [64 wg, 64 wg + 64), then 128 further on
+      float sum[128];                         // columns [64 wg, 64 wg + 64) of the tile, then those 128 further on
 #pragma unroll
-      for (int i = 0; i < 64; ++i) sum[i] = 0ull;
-      float na = __ldg(sa), n0 = __ldg(sb0), n1 = __ldg(sb1);
+      for (int i = 0; i < 128; ++i) sum[i] = 0.f;
       for (int kb = 0; kb < nk; ++kb) {
-        const float f0 = na * n0, f1 = na * n1;
-        if (kb + 1 < nk) {                    // the next block's, while this one's sums are awaited
-          na = __ldg(sa + (kb + 1) * g.sa.col);
-          n0 = __ldg(sb0 + (kb + 1) * g.sb.col);
-          n1 = __ldg(sb1 + (kb + 1) * g.sb.col);
-        }
-        ok = ok && mbar_wait(&tfull[acc], acc_phase, status);
-        ok = __all_sync(0xffffffffu, ok);
+        const int k = kb & (SC_KB - 1);
+        if (k == 0) ok = ok && mbar_wait_warp(&sfull[slot], sc_phase, status);
+        const float* sc = scales + slot * SC_ROW;
+        const float sa = sc[k * BM + row_in];
+        const float2 sb = *reinterpret_cast<const float2*>(sc + SC_KB * BM + 2 * k);
+        const float f0 = sa * sb.x, f1 = sa * sb.y;
+        ok = ok && mbar_wait_warp(&tfull[acc], acc_phase, status);
         if (ok) {
           tc_fence_after();
           const uint32_t tb = tmem_base + acc * BN + wg * 64 + ((uint32_t)(quad * 32) << 16);
+          // 32 columns are multiplied while the next 32 come
+          uint32_t r[2][32];
+          tmem_ld32(tb, r[0]);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t r[32];
-            tmem_ld32(tb + (c >> 1) * 128 + (c & 1) * 32, r);
-            tmem_ld_wait();
-            if (c == 3) {
+            tmem_ld_wait_for(r[c & 1]);
+            if (c < 3) {
+              tmem_ld32(tb + ((c + 1) >> 1) * 128 + ((c + 1) & 1) * 32, r[(c + 1) & 1]);
+            } else {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&tempty[acc]);
             }
-            const uint64_t f = c < 2 ? f32x2(f0, f0) : f32x2(f1, f1);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              sum[c * 16 + i] = fma_f32x2(f32x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), f, sum[c * 16 + i]);
+            for (int i = 0; i < 32; ++i) sum[c * 32 + i] = fmaf(__uint_as_float(r[c & 1][i]), c < 2 ? f0 : f1, sum[c * 32 + i]);
+          }
+        }
+        if (k == SC_KB - 1 || kb == nk - 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sempty[slot]);
+          if (++slot == SC_SLOTS) {
+            slot = 0;
+            sc_phase ^= 1;
           }
         }
         acc ^= 1;
@@ -389,15 +444,20 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
       if constexpr (EPI == EPI_SILU_MUL) {
         float h[64];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          h[2 * i] = silu(lo_f32(sum[i])) * lo_f32(sum[32 + i]);
-          h[2 * i + 1] = silu(hi_f32(sum[i])) * hi_f32(sum[32 + i]);
-        }
+        for (int i = 0; i < 64; ++i) h[i] = silu_fast(sum[i]) * sum[64 + i];
         const int col = tn * 128 + wg * 64;
         if constexpr (QUANT) {
           float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < 64; ++i) top = fmaxf(top, finite_or_zero(h[i]));
+          for (int i = 0; i < 64; ++i) top = fmaxf(top, fabsf(h[i]));     // (passes over NaN)
+          if (!(top < INFINITY)) {              // infinities become NaN and do not count
+            top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) {
+              top = fmaxf(top, finite_or_zero(h[i]));
+              if (fabsf(h[i]) == INFINITY) h[i] = __uint_as_float(0x7fffffffu);
+            }
+          }
           float* mine = tops + parity * 2 * BM;
           mine[wg * BM + row_in] = top;
           bar_sync(1, 32 * EPI_WARPS);         // once per tile: the other parity's maxima have been read by then
@@ -411,8 +471,8 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
               uint32_t* po = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                po[e] = quant_pair(h[16 * v + 4 * e], h[16 * v + 4 * e + 1], mul) |
-                        quant_pair(h[16 * v + 4 * e + 2], h[16 * v + 4 * e + 3], mul) << 16;
+                po[e] = to_e4m3x2(h[16 * v + 4 * e] * mul, h[16 * v + 4 * e + 1] * mul) |
+                        to_e4m3x2(h[16 * v + 4 * e + 2] * mul, h[16 * v + 4 * e + 3] * mul) << 16;
               st_v4(d + 16 * v, o);
             }
             if (wg == 0) g.sd.p[row * g.sd.row + tn * g.sd.col] = top / q8::TOP;
@@ -435,10 +495,10 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
             const u128 rv = ld_v4(reinterpret_cast<const __nv_bfloat16*>(g.r) + (int64_t)row * g.ldr + col);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              po[e] = pack_bf16x2(lo_f32(sum[4 * v + e]) + bf16_lo(word(rv, e)), hi_f32(sum[4 * v + e]) + bf16_hi(word(rv, e)));
+              po[e] = pack_bf16x2(sum[8 * v + 2 * e] + bf16_lo(word(rv, e)), sum[8 * v + 2 * e + 1] + bf16_hi(word(rv, e)));
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) po[e] = pack_bf16x2(lo_f32(sum[4 * v + e]), hi_f32(sum[4 * v + e]));
+            for (int e = 0; e < 4; ++e) po[e] = pack_bf16x2(sum[8 * v + 2 * e], sum[8 * v + 2 * e + 1]);
           }
           st_v4(reinterpret_cast<__nv_bfloat16*>(g.d) + (int64_t)row * g.ldd + col, o);
         }
@@ -461,6 +521,9 @@ static void launch_gemm_fp8(const GemmFp8& g, int sms, int* status, cudaStream_t
   int dev;
   cudaGetDevice(&dev);
   if (!attr[dev & 63]) {
+    cudaFuncAttributes a;
+    if (cudaFuncGetAttributes(&a, kern) != cudaSuccess || a.numRegs * THREADS < REGS_ALL)
+      throw std::runtime_error("cx gemm_fp8: built with fewer registers than its warpgroups take");   // they would wait
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     attr[dev & 63] = true;
   }

@@ -971,6 +971,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("quantize_fp8", &quantize_fp8);
   m.def("quantize_weight_fp8", &quantize_weight_fp8);
   m.def("gemm_fp8", &gemm_fp8);
+  // (activations per tile or 0, CTAs per tile) of a call
+  m.def("gemm_fp8_plan", [](int64_t M, int64_t N, int64_t K, int64_t epi, int64_t sms) {
+    const cx::GemmFp8Plan p = cx::gemm_fp8_plan((int)M, (int)N, (int)K, (int)epi, (int)sms);
+    return std::make_tuple(p.nt, p.splits);
+  });
   m.def("kv_push_layer", &kv_push_layer);
   m.def("gemm_splits", &gemm_splits);
   m.def("gemm_raster_group", &cx::gemm_raster_group);

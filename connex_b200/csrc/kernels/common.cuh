@@ -253,12 +253,15 @@ __device__ __forceinline__ bool mbar_wait_poll(uint64_t* bar, uint32_t parity, i
 }
 
 // mbar_wait of a whole warp, for waits that come once in a few hundred cycles: the first tries are one loop of two
-// instructions, which the lanes leave together.  (A try suspends the thread for a time limit of the hardware's.  A
-// vote on the result took the block-scaled GEMM from 1010 us to 1170: it stands between the barrier and the loads.)
+// instructions, which the lanes leave together.  (A try suspends the thread for a time limit of the hardware's, and
+// takes twice the time of a test where the phase is complete already.  A vote on the result took the block-scaled GEMM
+// from 1010 us to 1170: it stands between the barrier and the loads.)
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra WARP_DONE;\n\t"
       "mov.u32 n, 0;\n\t"
       "WARP_TRY:\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
@@ -319,11 +322,6 @@ __device__ __forceinline__ void tc_fence_after() {
 }
 
 // ------------------------------------------------------------------ clusters
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
 // every thread of every CTA of the cluster; orders their shared-memory accesses
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -333,11 +331,6 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t local, uint32_t rank) 
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
   return r;
-}
-// Arrival on a barrier of another CTA.  It orders no other memory accesses of this thread (.release.cluster would, by
-// a memory barrier of some 1000 cycles): for what the asynchronous units read or wrote.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 
 // Shared-memory matrix descriptor for a K-major operand tile stored with the
@@ -460,6 +453,18 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// One thread of a converged warp, the same one each time.
+__device__ __forceinline__ bool elect_sync() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// umma_desc_sw128 in two words: the upper one is constant, and 32 bytes further on the lower one is 2 more.
+__device__ __forceinline__ uint32_t umma_desc_sw128_lo(uint32_t smem_addr) { return ((smem_addr >> 4) & 0x3FFFu) | 1u << 16; }
+__device__ __forceinline__ uint64_t umma_desc_sw128_of(uint32_t lo) {
+  constexpr uint32_t HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+  return (uint64_t)HI << 32 | lo;
+}
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 31; }
 __device__ __forceinline__ int warp_id() { return threadIdx.x >> 5; }
 __device__ __forceinline__ bool elect_one() { return lane_id() == 0; }

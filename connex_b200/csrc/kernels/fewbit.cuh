@@ -40,6 +40,12 @@ __device__ __forceinline__ float finite_or_zero(float a) {   // |a| of a finite 
   return u < 0x7f800000u ? __uint_as_float(u) : 0.f;
 }
 __device__ __forceinline__ uint64_t unpack_bf16x2(uint32_t w) { return f32x2(bf16_lo(w), bf16_hi(w)); }
+// larger magnitudes of two bf16 pairs, signs undefined; NaN only where both are
+__device__ __forceinline__ uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 // a cos + b sin of a pair of dims, rounded to bf16
 __device__ __forceinline__ uint32_t turn_bf16x2(uint32_t a, uint32_t b, uint64_t co, uint64_t si) {
   const uint64_t r = fma_f32x2(unpack_bf16x2(b), si, mul_f32x2(unpack_bf16x2(a), co));

@@ -56,33 +56,51 @@ __device__ __forceinline__ void unpack8(const u128& r, float (&v)[8]) {
   }
 }
 
-// A half-warp per block, eight columns of a lane, UNROLL blocks in flight.
-template <int UNROLL>
+// A half-warp per block, eight columns of a lane; a CTA takes 2^lc column blocks of 16 / 2^lc rows at a time, four such
+// groups of rows in flight.  (With a running block number, divided by the row's blocks in 64 bits, 8192 x 4096 took 35
+// us.)
 __global__ void __launch_bounds__(q8::THREADS)
     quantize_fp8_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq,
-                        Fp8Scales s, int64_t blocks, int kb, int K) {
+                        Fp8Scales s, int T, int K, int lc) {
   using namespace q8;
-  const int lane = threadIdx.x & 31, j = lane & 15;
-  const int64_t per = (int64_t)gridDim.x * (THREADS / 16);
-  const int64_t first = (int64_t)blockIdx.x * (THREADS / 16) + (threadIdx.x >> 4);
-  for (int64_t u0 = first - (lane >> 4); u0 < blocks; u0 += UNROLL * per) {   // the same for the whole warp
+  constexpr int UNROLL = 4;
+  const int hw = threadIdx.x >> 4, j = threadIdx.x & 15;
+  const int b = (blockIdx.x << lc) + (hw & ((1 << lc) - 1)), c = b * Q + 8 * j;
+  const int64_t step = (int64_t)gridDim.y << (4 - lc), row0 = ((int64_t)blockIdx.y << (4 - lc)) + (hw >> lc);
+  for (int64_t r0 = (int64_t)blockIdx.y << (4 - lc); r0 < T; r0 += UNROLL * step) {        // the same for the whole CTA
+    const int64_t first = row0 + (r0 - ((int64_t)blockIdx.y << (4 - lc)));
     u128 raw[UNROLL];
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
-      const int64_t u = u0 + (lane >> 4) + i * per, row = u / kb;
-      const int c = (int)(u - row * kb) * Q + 8 * j;
-      raw[i] = u < blocks && c < K ? ld_nc_v4(x + row * ldx + c) : u128{0, 0, 0, 0};
+      const int64_t row = first + i * step;
+      raw[i] = row < T && c < K ? ld_nc_v4(x + row * ldx + c) : u128{0, 0, 0, 0};
     }
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
-      const int64_t u = u0 + (lane >> 4) + i * per, row = u / kb;
-      const int b = (int)(u - row * kb), c = b * Q + 8 * j;
-      float v[8];
-      unpack8(raw[i], v);
-      const float top = fmaxf(half_warp_max(top8(v)), TINY);
-      if (u >= blocks) continue;
-      if (c < K) *reinterpret_cast<uint2*>(q + row * ldq + c) = quant8(v, TOP / top);
-      if (j == 0) s.p[row * s.row + b * s.col] = top / TOP;
+      const int64_t row = first + i * step;
+      // magnitudes as pairs of bf16 (NaN is passed over)
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
+      const uint32_t m = max_abs_bf16x2(max_abs_bf16x2(w[0], w[1]), max_abs_bf16x2(w[2], w[3])) & 0x7fff7fffu;
+      float top = fmaxf(bf16_lo(m), bf16_hi(m));
+      const bool odd = !(top < INFINITY);
+      if (odd) {
+        float v[8];
+        unpack8(raw[i], v);
+        top = top8(v);
+      }
+      top = fmaxf(half_warp_max(top), TINY);
+      const float mul = TOP / top;
+      if (row < T && c < K) {
+        uint32_t o[4];
+        const uint64_t mul2 = f32x2(mul, mul);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint64_t r = mul_f32x2(unpack_bf16x2(w[e]), mul2);
+          o[e] = odd ? quant_pair(bf16_lo(w[e]), bf16_hi(w[e]), mul) : to_e4m3x2(lo_f32(r), hi_f32(r));
+        }
+        *reinterpret_cast<uint2*>(q + row * ldq + c) = make_uint2(o[0] | o[1] << 16, o[2] | o[3] << 16);
+        if (j == 0) s.p[row * s.row + b * s.col] = top / TOP;
+      }
     }
   }
 }
@@ -176,9 +194,12 @@ void quantize_fp8(const void* x, int64_t ldx, const void* w, float eps, void* q,
   auto O = reinterpret_cast<uint8_t*>(q);
   const int kb = (K + Q - 1) / Q;
   if (w == nullptr) {
-    const int64_t blocks = (int64_t)T * kb;
-    const int64_t ctas = std::min<int64_t>((blocks + THREADS / 16 - 1) / (THREADS / 16), 148 * 8);
-    quantize_fp8_kernel<4><<<(int)ctas, THREADS, 0, stream>>>(X, ldx, O, ldq, s, blocks, kb, K);
+    int lc = 0;
+    while (lc < 4 && 1 << lc < kb) ++lc;
+    const int gx = (kb + (1 << lc) - 1) >> lc;
+    const int64_t groups = ((int64_t)T + (16 >> lc) - 1) >> (4 - lc);          // of rows
+    const int gy = (int)std::max<int64_t>(1, std::min<int64_t>(groups, std::max(1, 148 * 8 / gx)));
+    quantize_fp8_kernel<<<dim3(gx, gy), THREADS, 0, stream>>>(X, ldx, O, ldq, s, T, K, lc);
     return;
   }
   const int vpt = (K / 8 + THREADS - 1) / THREADS;
@@ -305,19 +326,22 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
 
   if (warp < 4) {
     regs_dec<REGS_AUX>();
-    if (warp == 0 && lane == 0) {
+    // (Whole warps walk through the loops and one thread acts: what the instructions take in uniform registers then
+    // lies there.  Left to one thread's branch, an MMA took 75 cycles to issue.)
+    if (warp == 0) {
       uint32_t stage = 0, phase = 0;
       for (int t = first; t < total && ok; t += step) {
         int tm, tn;
         tile_coords(t, num_m, num_n, GROUP, tm, tn);
         for (int kb = 0; kb < nk; ++kb) {
-          if (!mbar_wait_poll(&empty[stage], phase ^ 1, status)) {
-            ok = false;
-            break;
+          ok = mbar_wait_poll(&empty[stage], phase ^ 1, status);
+          if (!ok) break;
+          if (elect_sync()) {
+            mbar_arrive_expect_tx(&full[stage], STAGE_BYTES);
+            tma_load_2d(sA + stage * A_BYTES, &tmA, &full[stage], kb * BK, tm * BM);
+            tma_load_2d(sB + stage * B_BYTES, &tmB, &full[stage], kb * BK, tn * BN);
           }
-          mbar_arrive_expect_tx(&full[stage], STAGE_BYTES);
-          tma_load_2d(sA + stage * A_BYTES, &tmA, &full[stage], kb * BK, tm * BM);
-          tma_load_2d(sB + stage * B_BYTES, &tmB, &full[stage], kb * BK, tn * BN);
+          __syncwarp();
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
@@ -326,24 +350,26 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
       }
       if (!ok)   // let loads already in flight land before the CTA can exit
         for (int s = 0; s < STAGES; ++s) mbar_wait(&full[s], 0, nullptr, 100000000ull);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       constexpr uint32_t IDESC = umma_idesc_e4m3(BM, BN);
+      const uint32_t a_lo = umma_desc_sw128_lo(smem_u32(sA)), b_lo = umma_desc_sw128_lo(smem_u32(sB));
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
       bool issued = false;
       for (int t = first; t < total && ok; t += step) {
         for (int kb = 0; kb < nk; ++kb) {
-          if (!mbar_wait_poll(&tempty[acc], acc_phase ^ 1, status) || !mbar_wait_poll(&full[stage], phase, status)) {
-            ok = false;
-            break;
-          }
+          ok = mbar_wait_poll(&tempty[acc], acc_phase ^ 1, status) && mbar_wait_poll(&full[stage], phase, status);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t a0 = smem_u32(sA + stage * A_BYTES), b0 = smem_u32(sB + stage * B_BYTES);
+          if (elect_sync()) {
+            const uint32_t al = a_lo + stage * (A_BYTES / 16), bl = b_lo + stage * (B_BYTES / 16);
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)
-            umma_e4m3(tmem_base + acc * BN, umma_desc_sw128(a0 + k * 32), umma_desc_sw128(b0 + k * 32), IDESC, k != 0);
+            for (int k = 0; k < BK / 32; ++k)
+              umma_e4m3(tmem_base + acc * BN, umma_desc_sw128_of(al + 2 * k), umma_desc_sw128_of(bl + 2 * k), IDESC, k != 0);
+            umma_commit(&tfull[acc]);
+            umma_commit(&empty[stage]);
+          }
+          __syncwarp();
           issued = true;
-          umma_commit(&tfull[acc]);
-          umma_commit(&empty[stage]);
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
@@ -353,7 +379,8 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
         }
       }
       if (!ok && issued) {   // wait (bounded) for every issued MMA before TMEM is freed
-        umma_commit(drain);
+        if (elect_sync()) umma_commit(drain);
+        __syncwarp();
         mbar_wait(drain, 0, nullptr, 100000000ull);
       }
     } else if (warp == 3) {
@@ -533,10 +560,408 @@ static void launch_gemm_fp8(const GemmFp8& g, int sms, int* status, cudaStream_t
   kern<<<(int)std::min<int64_t>(tiles, sms), THREADS, SMEM, stream>>>(ta, tb, g, status);
 }
 
+// ------------------------------------------------------- few rows: split K
+// Where the 128 x 256 tiles would leave SMs idle: the weight's rows are the MMA's 128 rows and NT activations its
+// columns, and the CTAs of a cluster share a tile's blocks of 128 columns among them.  Each adds up its part in
+// registers as above (a thread per weight row; the scales of a block lie in shared memory, a's times b's), leaves it
+// in shared memory, and the CTAs then add the parts of a slice of the activations each, in the order of their ranks,
+// over the cluster's shared memory: no workspace, no atomics, the same bits from run to run.  A warp writes a row of
+// 128 outputs.  SiLU-mul takes R = 2 blocks of weight rows, gate and up.
+// What bounds it: a block of 128 columns takes a CTA 500 to 600 cycles (the issuing thread's two waits and four MMAs,
+// up to 64 activations; the promotion beyond), and 5 to 6 us pass around that (launch, first loads, the cluster's
+// sums): 64 x 4096 x 14336 takes 17.4 us where reading the operands takes 9.4, one row 14.8.
+namespace g8s {
+constexpr int BK = 128, Q = 128;
+constexpr int SC_SLOTS = 2;
+template <int NT, int R>
+struct Cfg {
+  // two CTAs on an SM where their stages and registers fit: one computes while the other waits
+  static constexpr int PER_SM = R * NT <= 32 ? 2 : 1;
+  static constexpr int A_BYTES = R * Q * BK, B_BYTES = NT * BK, STAGE = A_BYTES + B_BYTES;
+  static constexpr int SC_KB = R == 1 && NT <= 64 ? 8 : 4;  // blocks of columns whose scales come together
+  static constexpr int SCALES = SC_SLOTS * SC_KB * R * NT * 4;
+  static constexpr int PARTS = NT * R * Q * 4;    // in the stages, once they are empty
+  static constexpr int ROOM = (PER_SM == 2 ? 113 * 1024 : 200 * 1024) - SCALES - 1024 - 512;
+  static constexpr int STAGES = ROOM / STAGE;
+  static_assert(STAGES >= 3 && PARTS <= STAGES * STAGE, "stages");
+  static constexpr int SMEM = 1024 + STAGES * STAGE + SCALES + 512;
+  // Accumulators in TMEM, up to eight: a block's sums are read some 1000 cycles after its MMAs have begun.
+  static constexpr int ACCS = 512 / PER_SM / (R * NT) < 8 ? 512 / PER_SM / (R * NT) : 8;
+  static constexpr int COLS = ACCS * R * NT;
+  static constexpr int GROUPS = R * NT > 128 ? 2 : 1, THREADS = 128 + 128 * GROUPS;
+  static constexpr int MINE = NT / GROUPS;        // activations of a thread
+  static constexpr int CH = GROUPS == 1 && MINE >= 32 ? 32 : 16;                 // of them, read from TMEM at a time
+};
+}  // namespace g8s
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int NT, int R>
+__global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER_SM)
+    gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, GemmFp8 g,
+                          int splits, int* status) {
+  using namespace g8s;
+  using C = Cfg<NT, R>;
+  constexpr int STAGES = C::STAGES, SC_KB = C::SC_KB;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* parts = reinterpret_cast<float*>(smem);                                 // [NT][R * 128]
+  float* scales = reinterpret_cast<float*>(smem + STAGES * C::STAGE);            // [slot][SC_KB][R][NT]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE + C::SCALES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + C::ACCS;
+  uint64_t* sfull = tempty + C::ACCS;
+  uint64_t* sempty = sfull + SC_SLOTS;
+  uint64_t* drain = sempty + SC_SLOTS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+
+  const int warp = warp_id(), lane = lane_id();
+  const int rank = blockIdx.x % splits, tile = blockIdx.x / splits, m0 = blockIdx.y * NT;
+  const int nk = (g.K + BK - 1) / BK;
+  const int k0 = (int)((int64_t)nk * rank / splits), k1 = (int)((int64_t)nk * (rank + 1) / splits);
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < C::ACCS; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 4 * C::GROUPS);
+    }
+    for (int i = 0; i < SC_SLOTS; ++i) {
+      mbar_init(&sfull[i], 32);
+      mbar_init(&sempty[i], 4 * C::GROUPS);
+    }
+    mbar_init(drain, 1);
+    fence_barrier_init();
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::COLS);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  bool ok = true;
+
+  if (warp == 0) {
+    uint32_t stage = 0, phase = 0;
+    for (int kb = k0; kb < k1; ++kb) {
+      ok = mbar_wait_poll(&empty[stage], phase ^ 1, status);
+      if (!ok) break;
+      if (elect_sync()) {
+        uint8_t* at = smem + stage * C::STAGE;
+        mbar_arrive_expect_tx(&full[stage], C::STAGE);
+        tma_load_2d(at, &tmB, &full[stage], kb * BK, tile * R * Q);              // the weight
+        tma_load_2d(at + C::A_BYTES, &tmA, &full[stage], kb * BK, m0);
+      }
+      __syncwarp();
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    if (!ok)
+      for (int s = 0; s < STAGES; ++s) mbar_wait(&full[s], 0, nullptr, 100000000ull);
+  } else if (warp == 1) {
+    constexpr uint32_t IDESC = umma_idesc_e4m3(Q, NT);
+    const uint32_t w_lo = umma_desc_sw128_lo(smem_u32(smem));
+    uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+    bool issued = false;
+    for (int kb = k0; kb < k1; ++kb) {
+      ok = mbar_wait_poll(&tempty[acc], acc_phase ^ 1, status) && mbar_wait_poll(&full[stage], phase, status);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_sync()) {
+        const uint32_t wl = w_lo + stage * (C::STAGE / 16), xl = wl + C::A_BYTES / 16;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            umma_e4m3(tmem_base + (acc * R + r) * NT, umma_desc_sw128_of(wl + r * (Q * BK / 16) + 2 * k),
+                      umma_desc_sw128_of(xl + 2 * k), IDESC, k != 0);
+        umma_commit(&tfull[acc]);
+        umma_commit(&empty[stage]);
+      }
+      __syncwarp();
+      issued = true;
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+      if (++acc == C::ACCS) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+    if (!ok && issued) {
+      if (elect_sync()) umma_commit(drain);
+      __syncwarp();
+      mbar_wait(drain, 0, nullptr, 100000000ull);
+    }
+  } else if (warp == 3) {
+    // A batch's scales are on their way while the one before is written: the loads take a microsecond and more, as
+    // long as several blocks' MMAs.
+    constexpr int PER = (NT + 31) / 32;
+    uint32_t slot = 0, phase = 0;
+    const int last = (g.N - 1) / Q;
+    float v[SC_KB][PER], b[SC_KB][R];
+    auto load = [&](int kb) {
+#pragma unroll
+      for (int k = 0; k < SC_KB; ++k) {
+        const bool there = kb + k < k1;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int m = m0 + 32 * i + lane;
+          v[k][i] = there && m < g.M ? __ldg(g.sa.p + m * g.sa.row + (kb + k) * g.sa.col) : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          b[k][r] = there ? __ldg(g.sb.p + min(tile * R + r, last) * g.sb.row + (kb + k) * g.sb.col) : 0.f;
+      }
+    };
+    load(k0);
+    for (int kb = k0; kb < k1 && ok; kb += SC_KB) {
+      float f[SC_KB][R][PER];
+#pragma unroll
+      for (int k = 0; k < SC_KB; ++k)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < PER; ++i) f[k][r][i] = v[k][i] * b[k][r];
+      load(kb + SC_KB);
+      ok = mbar_wait_warp(&sempty[slot], phase ^ 1, status);
+      if (!ok) break;
+#pragma unroll
+      for (int k = 0; k < SC_KB; ++k)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            if (32 * i + lane < NT) scales[((slot * SC_KB + k) * R + r) * NT + 32 * i + lane] = f[k][r][i];
+      mbar_arrive(&sfull[slot]);
+      if (++slot == SC_SLOTS) {
+        slot = 0;
+        phase ^= 1;
+      }
+    }
+  } else if (warp >= 4) {
+    const int quad = warp & 3, wg = (warp - 4) >> 2;
+    uint32_t acc = 0, acc_phase = 0, slot = 0, sc_phase = 0;
+    float sum[R][C::MINE];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < C::MINE; ++i) sum[r][i] = 0.f;
+    for (int kb = k0; kb < k1; ++kb) {
+      const int k = (kb - k0) & (SC_KB - 1);
+      if (k == 0) ok = ok && mbar_wait_warp(&sfull[slot], sc_phase, status);
+      ok = ok && mbar_wait_warp(&tfull[acc], acc_phase, status);
+      if (ok) {
+        tc_fence_after();
+        const uint32_t tb = tmem_base + acc * R * NT + wg * C::MINE + ((uint32_t)(quad * 32) << 16);
+        const float* sc = scales + (slot * SC_KB + k) * R * NT + wg * C::MINE;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int c = 0; c < C::MINE / C::CH; ++c) {
+            uint32_t t[C::CH];
+            if constexpr (C::CH == 32) tmem_ld32(tb + r * NT + c * C::CH, t);
+            else tmem_ld16(tb + r * NT + c * C::CH, t);
+            float4 f[C::CH / 4];
+#pragma unroll
+            for (int i = 0; i < C::CH / 4; ++i) f[i] = *reinterpret_cast<const float4*>(sc + r * NT + c * C::CH + 4 * i);
+            tmem_ld_wait_for(t);
+            if (r == R - 1 && c == C::MINE / C::CH - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&tempty[acc]);
+            }
+#pragma unroll
+            for (int i = 0; i < C::CH; ++i)
+              sum[r][c * C::CH + i] =
+                  fmaf(__uint_as_float(t[i]), reinterpret_cast<const float*>(f)[i], sum[r][c * C::CH + i]);
+          }
+      }
+      if (k == SC_KB - 1 || kb == k1 - 1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sempty[slot]);
+        if (++slot == SC_SLOTS) {
+          slot = 0;
+          sc_phase ^= 1;
+        }
+      }
+      if (++acc == C::ACCS) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+    // every MMA is complete and every stage read, for the last accumulator is
+    if (ok)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < C::MINE; ++i) parts[(wg * C::MINE + i) * (R * Q) + r * Q + quad * 32 + lane] = sum[r][i];
+  }
+  __syncwarp();
+  const bool failed = __syncthreads_or(!ok);
+  if (splits > 1) cluster_sync();
+
+  // ---- a warp per row of outputs: the parts of all ranks in their order
+  const int rows = min(NT, g.M - m0);
+  const uint32_t base = smem_u32(parts);
+  for (int i = rank + splits * warp; i < rows && !failed; i += splits * (C::THREADS / 32)) {
+    float4 v[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < splits; ++s)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint32_t at = base + (i * (R * Q) + r * Q + 4 * lane) * 4;
+        const float4 x = splits > 1 ? ld_cluster_f32x4(cluster_addr(at, s)) : *reinterpret_cast<const float4*>(
+                                                                                  parts + i * (R * Q) + r * Q + 4 * lane);
+        v[r].x += x.x;
+        v[r].y += x.y;
+        v[r].z += x.z;
+        v[r].w += x.w;
+      }
+    const int64_t m = m0 + i;
+    const int col = tile * Q + 4 * lane;
+    if constexpr (R == 2) {
+      float h[4] = {silu_fast(v[0].x) * v[1].x, silu_fast(v[0].y) * v[1].y, silu_fast(v[0].z) * v[1].z,
+                    silu_fast(v[0].w) * v[1].w};
+      if (g.sd.p != nullptr) {
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, finite_or_zero(h[e]));
+        top = fmaxf(warp_max(top), q8::TINY);
+        const float mul = q8::TOP / top;
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(g.d) + m * g.ldd + col) =
+            quant_pair(h[0], h[1], mul) | quant_pair(h[2], h[3], mul) << 16;
+        if (lane == 0) g.sd.p[m * g.sd.row + tile * g.sd.col] = top / q8::TOP;
+      } else {
+        *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(g.d) + m * g.ldd + col) =
+            make_uint2(pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3]));
+      }
+    } else if (col < g.N) {
+      if (g.epi == EPI_ADD) {
+        const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(g.r) + m * g.ldr + col);
+        v[0].x += bf16_lo(x.x);
+        v[0].y += bf16_hi(x.x);
+        v[0].z += bf16_lo(x.y);
+        v[0].w += bf16_hi(x.y);
+      }
+      *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(g.d) + m * g.ldd + col) =
+          make_uint2(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[0].z, v[0].w));
+    }
+  }
+  __syncwarp();
+  if (splits > 1) cluster_sync();          // no CTA ends while another may still read its parts
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::COLS);
+  }
+}
+
+template <int NT, int R>
+static void launch_gemm_fp8_split(const GemmFp8& g, int splits, int* status, cudaStream_t stream) {
+  using C = g8s::Cfg<NT, R>;
+  auto kern = gemm_fp8_split_kernel<NT, R>;
+  static bool attr[64] = {};
+  int dev;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63]) {
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    attr[dev & 63] = true;
+  }
+  const CUtensorMap ta = make_tmap_u8_2d(g.a, (uint64_t)g.K, (uint64_t)g.M, (uint64_t)g.lda, g8s::BK, NT);
+  const CUtensorMap tb = make_tmap_u8_2d(g.b, (uint64_t)g.K, (uint64_t)g.N, (uint64_t)g.ldb, g8s::BK, R * g8s::Q);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((g.N + R * g8s::Q - 1) / (R * g8s::Q) * splits, (g.M + NT - 1) / NT);
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = splits;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kern, ta, tb, g, splits, status);
+}
+
+// Which way a call goes: the least of the estimated times, in us.  A CTA takes `per` for a block of 128 columns and a
+// fixed start and end; clusters of four and eight do not fill every SM (132 and 120 of 148 are reached); reading the
+// operands takes its time whatever the CTAs.  The constants are fits to measured calls: 4096 weight rows with K = 4096
+// and 14336, one CTA per tile, and for the tiles of 128 x 256.  Estimated and measured: 1 x 6144 x 4096 8.3 and 9.2 (16
+// activations, four CTAs; one CTA 12.1, 128 x 256 tiles 21), 64 x 4096 x 14336 15.6 and 17.4 (64, four; 65), 613 x 2048
+// x 4096 23.3 and 26.6 (256, two; 30), 64 x 28672 x 4096 with SiLU-mul 25.6 and 25.6 (128 x 256 tiles; 64 activations
+// by one CTA 28.5), 512 x 4096 x 14336 60 and 63 (256, two; 71).
+GemmFp8Plan gemm_fp8_plan(int M, int N, int K, int epi, int sms) {
+  const int r = epi == EPI_SILU_MUL ? 2 : 1, nk = (K + 127) / 128;
+  const double read = ((double)M + N) * K / 5.5e6 + 4.0;
+  const int64_t tiles = (int64_t)((M + 127) / 128) * ((N + 255) / 256);
+  GemmFp8Plan best{0, 1};
+  double cost = std::max(read, (double)((tiles + sms - 1) / sms) * (nk * 0.55 + 8.0));
+  constexpr double per[2][5] = {{0.26, 0.29, 0.32, 0.58, 0.92}, {0.35, 0.45, 0.75, 1.15, 0}};
+  for (int i = 0; i < (r == 2 ? 4 : 5); ++i) {
+    const int nt = 16 << i;
+    const int64_t base = (int64_t)((M + nt - 1) / nt) * ((N + 128 * r - 1) / (128 * r));
+    if (base > (int64_t)1 << 24 || (M + nt - 1) / nt > 65535) continue;
+    for (int s = 1; s <= 8 && s <= nk; s *= 2) {
+      const int64_t room = (int64_t)((r * nt <= 32 ? 2 : 1) * sms * (s == 8 ? 0.81 : s == 4 ? 0.89 : 1.0));
+      const int64_t waves = (base * s + room - 1) / room;
+      // two CTAs on an SM take 1.6 times as long
+      const double crowd = 0.4 + 0.6 * std::min(std::max(base * s * (r * nt <= 32 ? 2.0 : 1.0) / room, 1.0), 2.0);
+      const double c = std::max(read, waves * ((nk + s - 1) / s * per[r - 1][i] * (r * nt <= 32 ? crowd : 1.0) + 4.5 + (s > 1 ? 1.5 : 0.0) + 0.01 * r * nt));
+      if (c < cost) {
+        cost = c;
+        best = {nt, s};
+      }
+    }
+  }
+  return best;
+}
+
 void gemm_fp8(const GemmFp8& g, int sms, int* status, cudaStream_t stream) {
   if (g.M == 0 || g.N == 0) return;
-  if (g.epi == EPI_SILU_MUL && g.sd.p != nullptr) launch_gemm_fp8<EPI_SILU_MUL, true>(g, sms, status, stream);
-  else if (g.epi == EPI_SILU_MUL) launch_gemm_fp8<EPI_SILU_MUL, false>(g, sms, status, stream);
+  const GemmFp8Plan p = gemm_fp8_plan(g.M, g.N, g.K, g.epi, sms);
+  const bool two = g.epi == EPI_SILU_MUL;
+  switch (p.nt) {
+    case 16: return two ? launch_gemm_fp8_split<16, 2>(g, p.splits, status, stream) : launch_gemm_fp8_split<16, 1>(g, p.splits, status, stream);
+    case 32: return two ? launch_gemm_fp8_split<32, 2>(g, p.splits, status, stream) : launch_gemm_fp8_split<32, 1>(g, p.splits, status, stream);
+    case 64: return two ? launch_gemm_fp8_split<64, 2>(g, p.splits, status, stream) : launch_gemm_fp8_split<64, 1>(g, p.splits, status, stream);
+    case 128: return two ? launch_gemm_fp8_split<128, 2>(g, p.splits, status, stream) : launch_gemm_fp8_split<128, 1>(g, p.splits, status, stream);
+    case 256: return launch_gemm_fp8_split<256, 1>(g, p.splits, status, stream);
+    default: break;
+  }
+  if (two && g.sd.p != nullptr) launch_gemm_fp8<EPI_SILU_MUL, true>(g, sms, status, stream);
+  else if (two) launch_gemm_fp8<EPI_SILU_MUL, false>(g, sms, status, stream);
   else if (g.epi == EPI_ADD) launch_gemm_fp8<EPI_ADD, false>(g, sms, status, stream);
   else launch_gemm_fp8<EPI_STORE, false>(g, sms, status, stream);
 }

@@ -34,6 +34,12 @@ struct GemmFp8 {
   int64_t ldr;
   Fp8Scales sd;               // p == nullptr: bf16 output
 };
+// How a call runs: nt = 0: tiles of 128 x 256; else tiles of 128 weight rows (SiLU-mul: 256) by nt activations,
+// each shared by `splits` CTAs.
+struct GemmFp8Plan {
+  int nt, splits;
+};
+GemmFp8Plan gemm_fp8_plan(int M, int N, int K, int epi, int sms);
 void gemm_fp8(const GemmFp8& g, int sms, int* status, cudaStream_t stream);
 
 }  // namespace cx

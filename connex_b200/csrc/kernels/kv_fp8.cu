@@ -37,12 +37,6 @@ __device__ __forceinline__ float scaled_or_nan(float x, float mul) {
   return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fffffffu) : x * mul;
 }
 
-// larger magnitudes of two bf16 pairs, signs undefined; NaN only where both are
-__device__ __forceinline__ uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 // ------------------------------------------------- RoPE + quantising write
 // CTAs of two kinds.  Block CTAs write the cache.  A block's scale depends on
 // every row that the call puts there, so one CTA collects them: the one whose

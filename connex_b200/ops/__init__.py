@@ -136,7 +136,7 @@ def quantize_fp8(x: torch.Tensor, norm: Optional[torch.Tensor] = None, eps: floa
     if out is None:
         out = torch.empty(T, K, dtype=torch.float8_e4m3fn, device=x.device)
     if scale is None:
-        scale = torch.empty(-(-K // FP8_BLOCK), T, dtype=torch.float32, device=x.device).t()
+        scale = torch.empty_strided((T, -(-K // FP8_BLOCK)), (1, max(T, 1)), dtype=torch.float32, device=x.device)
     _C.quantize_fp8(x, norm, eps, out, scale)
     _n()
     return out, scale
@@ -180,7 +180,8 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
                           device=a.device)
     quantised = out.dtype == torch.float8_e4m3fn
     if quantised and out_scale is None:
-        out_scale = torch.empty(-(-out.shape[1] // FP8_BLOCK), M, dtype=torch.float32, device=a.device).t()
+        out_scale = torch.empty_strided((M, -(-out.shape[1] // FP8_BLOCK)), (1, max(M, 1)), dtype=torch.float32,
+                                        device=a.device)
     if not quantised and out_scale is not None:
         raise ValueError("gemm_fp8: scales go with a float8_e4m3fn out")
     if silu_mul and residual is not None:

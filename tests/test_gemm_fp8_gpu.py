@@ -104,7 +104,8 @@ def _product_tolerance(a, sa, b, sb):
 
 
 GEMMS = [(1, 8, 16), (1, 6144, 1024), (2, 128, 128), (17, 264, 144), (64, 1000, 112), (128, 256, 256), (129, 72, 1040),
-         (300, 520, 2048), (513, 1288, 272), (640, 2304, 4096), (16, 4096, 14336), (200, 384, 7168)]
+         (300, 520, 2048), (513, 1288, 272), (640, 2304, 4096), (16, 4096, 14336), (200, 384, 7168),
+         (2300, 4872, 400), (8200, 1096, 1024), (130, 20000, 64), (33, 40, 14336), (1, 128256, 256)]
 
 
 @pytest.mark.parametrize("residual", [False, True])
@@ -130,7 +131,8 @@ def test_gemm(dev, shape, residual):
     assert torch.equal(again.view(torch.int16), out.view(torch.int16))
 
 
-@pytest.mark.parametrize("shape", [(1, 256, 128), (5, 512, 400), (64, 2048, 1024), (129, 768, 2064), (700, 2560, 512), (256, 1024, 4096)],
+@pytest.mark.parametrize("shape", [(1, 256, 128), (5, 512, 400), (64, 2048, 1024), (129, 768, 2064), (700, 2560, 512), (256, 1024, 4096),
+                                   (17, 256, 8192), (2200, 5120, 272), (40, 28672, 256)],
                          ids=lambda v: "x".join(map(str, v)))
 def test_gemm_silu_mul(dev, shape):
     from connex_b200 import ops

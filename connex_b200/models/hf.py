@@ -11,7 +11,10 @@ the device once:
   RoPE convention the kernels use);
 * ``gate_proj``, ``up_proj`` -> ``w13``, rows interleaved in blocks of half
   the SiLU-mul GEMM tile (:func:`connex_b200.ops.interleave_gate_up`);
-* ``lm_head`` = ``embed_tokens`` when ``tie_word_embeddings``.
+* ``lm_head`` = ``embed_tokens`` when ``tie_word_embeddings``;
+* projections stored in e4m3 with a scale per 128 x 128 block (``quant_method``
+  ``fp8``: ``<name>_scale_inv`` beside each weight) stay so
+  (:class:`~connex_b200.models.llama.Fp8Weight`), rows and scales fused alike.
 
 Only layers ``[l0, l1)`` are read for a pipeline stage, plus the embedding
 on the first stage and the final norm and LM head on the last.  The
@@ -28,7 +31,7 @@ from typing import Dict, Iterable, Optional, Tuple
 import torch
 
 from connex_b200 import ops
-from connex_b200.models.llama import LayerWeights, LlamaConfig, LlamaWeights
+from connex_b200.models.llama import Fp8Weight, LayerWeights, LlamaConfig, LlamaWeights
 
 HEAD_DIM = 128          # the attention kernels' head size
 
@@ -101,12 +104,18 @@ class _Shards:
 
 
 def load_llama(path: str, device, dtype=torch.bfloat16, layers: Optional[Tuple[int, int]] = None,
-               cfg: Optional[LlamaConfig] = None, tp: Optional[Tuple[int, int]] = None) -> LlamaWeights:
+               cfg: Optional[LlamaConfig] = None, tp: Optional[Tuple[int, int]] = None,
+               fp8: bool = False) -> LlamaWeights:
     """Weights of layers ``[l0, l1)`` (all by default) of the checkpoint in
     ``path``, in the kernels' layouts, on ``device``.  Tensors the stage
     does not own (embedding off the first stage, head off the last) are
     ``None``.  ``tp = (rank, world)`` keeps only that tensor-parallel rank's
-    shard of every layer (cut on the host, so the device never holds more)."""
+    shard of every layer (cut on the host, so the device never holds more).
+
+    ``fp8``: the projections in e4m3 with a scale per 128 x 128 block, quantised
+    on ``device`` layer by layer.  A checkpoint's own fp8 projections are taken
+    as they are, with or without it; under ``tp`` they are cut as their bf16
+    values (``fp8`` then quantises the shards anew)."""
     cfg = cfg or config_from_hf(path)
     l0, l1 = layers or (0, cfg.layers)
     if not 0 <= l0 < l1 <= cfg.layers:
@@ -114,31 +123,61 @@ def load_llama(path: str, device, dtype=torch.bfloat16, layers: Optional[Tuple[i
     sh = _Shards(path)
     dev = torch.device(device)
 
+    def stored(name):
+        """A checkpoint's weight: a tensor, or an Fp8Weight."""
+        t = sh.get(name)
+        if t.dtype != torch.float8_e4m3fn:
+            return t.to(dtype)
+        if not sh.has(name + "_scale_inv"):
+            raise ValueError(f"{name} is e4m3 without {name}_scale_inv (a scale per 128 x 128 block)")
+        s = sh.get(name + "_scale_inv").float()
+        if s.shape != tuple(-(-n // ops.FP8_BLOCK) for n in t.shape):
+            raise ValueError(f"{name}: scales {tuple(s.shape)} are not one per 128 x 128 block of {tuple(t.shape)}")
+        return Fp8Weight(t, s)
+
     def get(name):
-        return sh.get(name).to(dtype)
+        t = stored(name)
+        return t.float().to(dtype) if isinstance(t, Fp8Weight) else t
+
+    def fused(parts, fuse, block):
+        """Weights fused by ``fuse(rows of each, rows per block)``; e4m3 ones with their scales."""
+        if tp_shards or not all(isinstance(t, Fp8Weight) for t in parts):
+            return fuse([t.float().to(dtype) if isinstance(t, Fp8Weight) else t for t in parts], block)
+        q = fuse([t.q.view(torch.uint8) for t in parts], block).view(torch.float8_e4m3fn)
+        return Fp8Weight(q, fuse([t.scale for t in parts], max(1, block // ops.FP8_BLOCK)))
+
+    def stack(parts, _):
+        return torch.cat(parts, 0)
+
+    def interleave(parts, block):
+        return ops.interleave_gate_up(parts[0], parts[1], 2 * block)
 
     def put(t):
+        if isinstance(t, Fp8Weight):
+            return Fp8Weight(t.q.contiguous().to(dev), t.scale.contiguous().to(dev))
         return t.contiguous().to(dev)
 
-    shard = None
-    if tp is not None and tp[1] > 1:
+    shard, tp_shards = None, tp is not None and tp[1] > 1
+    if tp_shards:
         from connex_b200.parallel.tp import shard_layer, tp_config
         shard = (lambda lw: shard_layer(lw, cfg, tp[0], tp[1]))
     out_layers = []
     for i in range(l0, l1):
         p = f"model.layers.{i}."
-        q, k, v = get(p + "self_attn.q_proj.weight"), get(p + "self_attn.k_proj.weight"), \
-            get(p + "self_attn.v_proj.weight")
+        q, k, v = (stored(p + f"self_attn.{n}_proj.weight") for n in "qkv")
         if q.shape != (cfg.heads * HEAD_DIM, cfg.hidden) or k.shape != (cfg.kv_heads * HEAD_DIM, cfg.hidden):
             raise ValueError(f"layer {i}: q/k shapes {tuple(q.shape)} / {tuple(k.shape)} do not match the config")
         lw = LayerWeights(
-            attn_norm=get(p + "input_layernorm.weight"), wqkv=torch.cat([q, k, v], 0),
-            wo=get(p + "self_attn.o_proj.weight"), mlp_norm=get(p + "post_attention_layernorm.weight"),
-            w13=ops.interleave_gate_up(get(p + "mlp.gate_proj.weight"), get(p + "mlp.up_proj.weight")),
-            w2=get(p + "mlp.down_proj.weight"))
+            attn_norm=get(p + "input_layernorm.weight"), wqkv=fused([q, k, v], stack, ops.FP8_BLOCK),
+            wo=fused([stored(p + "self_attn.o_proj.weight")], stack, ops.FP8_BLOCK),
+            mlp_norm=get(p + "post_attention_layernorm.weight"),
+            w13=fused([stored(p + "mlp.gate_proj.weight"), stored(p + "mlp.up_proj.weight")], interleave,
+                      ops.GATE_UP_TILE // 2),
+            w2=fused([stored(p + "mlp.down_proj.weight")], stack, ops.FP8_BLOCK))
         if shard is not None:           # cut on the host: the device only ever holds this rank's part
             lw = shard(lw)
-        out_layers.append(LayerWeights(**{name: put(t) for name, t in lw.__dict__.items()}))
+        lw = LayerWeights(**{name: put(t) for name, t in lw.__dict__.items()})
+        out_layers.append(lw.to_fp8() if fp8 else lw)
     first, last = l0 == 0, l1 == cfg.layers
     embed = put(get("model.embed_tokens.weight")) if first else None
     head = None
@@ -168,6 +207,8 @@ def hf_config(cfg: LlamaConfig, tie: bool = False) -> dict:
 def hf_tensors(w: LlamaWeights) -> Iterable[Tuple[str, torch.Tensor]]:
     """(name, tensor) of ``w`` unfused into checkpoint names (host copies)."""
     cfg = w.cfg
+    if any(isinstance(t, Fp8Weight) for lw in w.layers for t in lw.__dict__.values()):
+        raise ValueError("checkpoints are written from bf16 weights, not from quantised ones")
     yield "model.embed_tokens.weight", w.embed
     for i, lw in enumerate(w.layers):
         p = f"model.layers.{i}."

@@ -13,9 +13,13 @@ Storage layout, chosen for the kernels rather than for checkpoint parity:
 * paged KV cache [L, 2, blocks, Hkv, 16, 128]: one head of one block is a
   contiguous 4 KB slice, the unit the PD push kernel moves.  With
   ``dtype=torch.float8_e4m3fn`` it holds 8-bit values and one power-of-two
-  scale per (block, KV head); attention then reads K and V from the cache in
-  prefill steps too, so a prompt split at block boundaries attends to the same
-  keys and values as a whole one.
+  scale per (block, KV head), with ``dtype=torch.uint8`` 4-bit codes with a scale
+  and a minimum per half of a token's head ([.., 16, 72] bytes); attention then
+  reads K and V from the cache in prefill steps too, so a prompt split at block
+  boundaries attends to the same keys and values as a whole one.
+* projections may be :class:`Fp8Weight` (e4m3 with a scale per 128 x 128 block):
+  their inputs are then quantised per row and 128 columns, by the norm before
+  them or by the SiLU-mul product itself
 
 The forward passes launch only this package's kernels (tcgen05 GEMM,
 RMSNorm, RoPE + cache write, attention, argmax); a per-layer hook lets the
@@ -79,13 +83,50 @@ class LlamaConfig:
 
 
 @dataclass
+class Fp8Weight:
+    """A projection [N, K] in e4m3, ``q``, with fp32 ``scale`` [ceil(N / 128),
+    ceil(K / 128)]: an element stands for value * its block's scale."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+    @classmethod
+    def of(cls, w: torch.Tensor) -> "Fp8Weight":
+        """A bf16 weight, quantised on its GPU."""
+        return cls(*ops.quantize_weight_fp8(w))
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.q.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.q.device
+
+    def float(self) -> torch.Tensor:
+        """fp32 [N, K] of the values."""
+        s = self.scale.repeat_interleave(128, 0)[:self.q.shape[0]].repeat_interleave(128, 1)[:, :self.q.shape[1]]
+        return self.q.float() * s
+
+    def to(self, device) -> "Fp8Weight":
+        return Fp8Weight(self.q.to(device), self.scale.to(device))
+
+
+PROJECTIONS = ("wqkv", "wo", "w13", "w2")
+
+
+@dataclass
 class LayerWeights:
     attn_norm: torch.Tensor
-    wqkv: torch.Tensor
+    wqkv: torch.Tensor              # the projections: bf16 tensors or Fp8Weight
     wo: torch.Tensor
     mlp_norm: torch.Tensor
     w13: torch.Tensor
     w2: torch.Tensor
+
+    def to_fp8(self) -> "LayerWeights":
+        """The same layer with its projections in e4m3 (those that are already stay as they are)."""
+        return LayerWeights(**{n: Fp8Weight.of(t) if n in PROJECTIONS and not isinstance(t, Fp8Weight) else t
+                               for n, t in self.__dict__.items()})
 
 
 @dataclass
@@ -124,6 +165,13 @@ class LlamaWeights:
         return cls(cfg=cfg, embed=rnd(cfg.vocab_size, cfg.hidden), layers=layers,
                    final_norm=ones(cfg.hidden), lm_head=rnd(cfg.vocab_size, cfg.hidden))
 
+    def to_fp8(self) -> "LlamaWeights":
+        """Quantises the layers' projections, one layer at a time in place:
+        embedding, norms and head stay bf16."""
+        for i, lw in enumerate(self.layers):
+            self.layers[i] = lw.to_fp8()
+        return self
+
     @staticmethod
     def layout(cfg: LlamaConfig):
         """``(name, shape)`` of every engine tensor, in :meth:`named_tensors` order."""
@@ -156,16 +204,23 @@ class LlamaWeights:
                    lm_head=t["lm_head.weight"])
 
     def named_tensors(self):
-        """(name, tensor) in HF-style naming with fused qkv / gate_up tensors."""
+        """(name, tensor) in HF-style naming with fused qkv / gate_up tensors; the
+        scales of an :class:`Fp8Weight` follow it as ``<name>_scale_inv``."""
+        def both(name, w):
+            if isinstance(w, Fp8Weight):
+                yield name, w.q
+                yield name + "_scale_inv", w.scale
+            else:
+                yield name, w
         yield "model.embed_tokens.weight", self.embed
         for i, lw in enumerate(self.layers):
             p = f"model.layers.{i}."
             yield p + "input_layernorm.weight", lw.attn_norm
-            yield p + "self_attn.qkv_proj.weight", lw.wqkv
-            yield p + "self_attn.o_proj.weight", lw.wo
+            yield from both(p + "self_attn.qkv_proj.weight", lw.wqkv)
+            yield from both(p + "self_attn.o_proj.weight", lw.wo)
             yield p + "post_attention_layernorm.weight", lw.mlp_norm
-            yield p + "mlp.gate_up_proj.weight", lw.w13
-            yield p + "mlp.down_proj.weight", lw.w2
+            yield from both(p + "mlp.gate_up_proj.weight", lw.w13)
+            yield from both(p + "mlp.down_proj.weight", lw.w2)
         yield "model.norm.weight", self.final_norm
         yield "lm_head.weight", self.lm_head
 
@@ -208,7 +263,9 @@ class PagedKVCache:
 
     ``dtype=torch.float8_e4m3fn``: an 8-bit cache; ``scales`` [L, 2, blocks,
     Hkv] fp32 then belong to it (see :func:`connex_b200.ops.rope_cache_fp8`),
-    otherwise ``scales`` is None.
+    otherwise ``scales`` is None.  ``dtype=torch.uint8``: a 4-bit cache [L, 2,
+    blocks, Hkv, BS, 72], whose rows hold their scales and minima themselves
+    (see :func:`connex_b200.ops.rope_cache_int4`).
 
     Blocks can be shared: :meth:`fork` gives sequences that continue another
     one tables on its full blocks, and :meth:`free` returns a block to the
@@ -220,13 +277,19 @@ class PagedKVCache:
                  storage: Optional[torch.Tensor] = None):
         self.cfg = cfg
         self.num_blocks = num_blocks
-        shape = (cfg.layers, 2, num_blocks, cfg.kv_heads, cfg.block_size, cfg.head_dim)
+        four = (storage.dtype if storage is not None else dtype) == torch.uint8
+        shape = (cfg.layers, 2, num_blocks, cfg.kv_heads, cfg.block_size, ops.KV_INT4_ROW if four else cfg.head_dim)
         self.kv = storage.view(shape) if storage is not None else torch.empty(shape, dtype=dtype, device=device)
         self.scales = None
         if self.kv.dtype == torch.float8_e4m3fn:
             self.scales = torch.ones(shape[:4], dtype=torch.float32, device=self.kv.device)
         self._free = list(range(num_blocks - 1, -1, -1))
         self._shared = {}              # block -> owners beyond the first
+
+    @property
+    def kind(self) -> str:
+        """``bf16``, ``fp8`` or ``int4``."""
+        return {torch.float8_e4m3fn: "fp8", torch.uint8: "int4"}.get(self.kv.dtype, "bf16")
 
     def k(self, layer: int) -> torch.Tensor:
         return self.kv[layer, 0]
@@ -240,9 +303,24 @@ class PagedKVCache:
     def v_scale(self, layer: int) -> torch.Tensor:
         return self.scales[layer, 1]
 
+    def values(self, layer: int, blocks: Sequence[int]):
+        """What K and V of ``blocks`` stand for, bf16 [n, Hkv, BS, D] each (of
+        any kind of cache; 4-bit values are rounded to bf16)."""
+        at = torch.tensor(list(blocks), dtype=torch.long, device=self.kv.device)
+        out = []
+        for i in range(2):
+            if self.kind == "fp8":
+                x = self.kv[layer, i].view(torch.uint8)[at].view(self.kv.dtype)
+                out.append((x.float() * self.scales[layer, i][at][..., None, None]).to(torch.bfloat16))
+            elif self.kind == "int4":
+                out.append(ops.kv_values_int4(self.kv[layer, i][at]))
+            else:
+                out.append(self.kv[layer, i][at])
+        return tuple(out)
+
     @property
     def head_slice_bytes(self) -> int:
-        return self.cfg.block_size * self.cfg.head_dim * self.kv.element_size()
+        return self.kv.shape[-2] * self.kv.shape[-1] * self.kv.element_size()
 
     @property
     def layer_stride_bytes(self) -> int:
@@ -389,28 +467,80 @@ class LlamaModel:
         self.logits = torch.empty(max_batch, cfg.vocab_size, **bf)
         self.next_ids = torch.empty(max_batch, dtype=torch.int32, device=dev)
         self.max_batch = max_batch
+        # e4m3 inputs of Fp8Weight projections, with their scales: the normed rows, the attention's, the MLP's
+        self.q8 = {}
+        if any(isinstance(getattr(lw, n), Fp8Weight) for lw in weights.layers for n in PROJECTIONS):
+            for name, width in (("h", cfg.hidden), ("attn", cfg.heads * cfg.head_dim), ("mid", cfg.ffn)):
+                self.q8[name] = (torch.empty(max_tokens, width, dtype=torch.float8_e4m3fn, device=dev),
+                                 torch.empty(max_tokens * -(-width // ops.FP8_BLOCK), dtype=torch.float32, device=dev))
 
     # ------------------------------------------------------------ layers
-    def _residual_gemm(self, a: torch.Tensor, w: torch.Tensor, x: torch.Tensor) -> None:
+    def _q8(self, name: str, T: int):
+        """The first ``T`` rows of an e4m3 buffer and of its scales."""
+        q, s = self.q8[name]
+        return q[:T], s[:T * -(-q.shape[1] // ops.FP8_BLOCK)].view(-1, T).t()
+
+    def _norm(self, x: torch.Tensor, norm: torch.Tensor, w, T: int) -> None:
+        """RMSNorm of ``x`` as the input of the projection ``w`` (None: the head's)."""
+        if isinstance(w, Fp8Weight):
+            q, s = self._q8("h", T)
+            ops.quantize_fp8(x, norm=norm, eps=self.cfg.eps, out=q, scale=s)
+        else:
+            ops.rmsnorm(x, norm, self.cfg.eps, out=self.h[:T])
+
+    def _qkv(self, lw: LayerWeights, T: int) -> torch.Tensor:
+        """The fused projection of the rows that :meth:`_norm` left."""
+        qkv = self.qkv[:T]
+        if isinstance(lw.wqkv, Fp8Weight):
+            ops.gemm_fp8(*self._q8("h", T), lw.wqkv.q, lw.wqkv.scale, out=qkv, status=self.status)
+        else:
+            ops.gemm(self.h[:T], lw.wqkv, qkv, status=self.status)
+        return qkv
+
+    def _mlp(self, lw: LayerWeights, T: int, x: torch.Tensor) -> None:
+        """x += down(SiLU(gate) * up) of the rows that :meth:`_norm` left."""
+        q13, q2 = isinstance(lw.w13, Fp8Weight), isinstance(lw.w2, Fp8Weight)
+        mid = self.mid[:T]
+        if q13:
+            q, s = self._q8("mid", T)
+            out, scale = (q, s) if q2 else (mid, None)
+            ops.gemm_fp8(*self._q8("h", T), lw.w13.q, lw.w13.scale, out=out, out_scale=scale, silu_mul=True,
+                         status=self.status)
+        else:
+            ops.gemm(self.h[:T], lw.w13, mid, silu_mul=True, status=self.status)
+        self._residual_gemm(mid, lw.w2, x, "mid", quantised=q13 and q2)
+
+    def _residual_gemm(self, a: torch.Tensor, w, x: torch.Tensor, name: str = "attn", quantised: bool = False) -> None:
         """x += a @ w^T; under tensor parallelism summed over the group: rank 0
         adds its partial to x in the epilogue, the others store theirs into
-        x, and an all-reduce of x adds them up."""
+        x, and an all-reduce of x adds them up.  ``name``: the buffer that
+        ``a`` is quantised into for an Fp8Weight; it holds it already if
+        ``quantised``."""
         tp = self.tp
-        if tp is None or tp.world == 1:
-            ops.gemm(a, w, x, residual=x, status=self.status)
-            return
-        ops.gemm(a, w, x, residual=x if tp.rank == 0 else None, status=self.status)
-        tp.all_reduce(x)
+        alone = tp is None or tp.world == 1
+        residual = x if alone or tp.rank == 0 else None
+        if isinstance(w, Fp8Weight):
+            q, s = self._q8(name, x.shape[0])
+            if not quantised:
+                ops.quantize_fp8(a, out=q, scale=s)
+            ops.gemm_fp8(q, s, w.q, w.scale, out=x, residual=residual, status=self.status)
+        else:
+            ops.gemm(a, w, x, residual=residual, status=self.status)
+        if not alone:
+            tp.all_reduce(x)
 
     def _rotate_and_cache(self, i: int, qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                           **norms) -> torch.Tensor:
         """Rotate q (in place) and write the rows' K and V to layer ``i`` of the
         cache; returns what the attention reads its queries from."""
         cfg, c = self.cfg, self.cache
-        if c.scales is None:
+        if c.kind == "bf16":
             ops.rope_cache(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots, c.k(i), c.v(i),
                            status=self.status, **norms)
             return qkv
+        if c.kind == "int4":
+            return ops.rope_cache_int4(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots, c.k(i), c.v(i),
+                                       out=qkv[:, :cfg.heads * cfg.head_dim], status=self.status, **norms)
         return ops.rope_cache_fp8(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots, c.k(i), c.v(i),
                                   c.k_scale(i), c.v_scale(i), out=qkv[:, :cfg.heads * cfg.head_dim],
                                   status=self.status, **norms)
@@ -418,7 +548,10 @@ class LlamaModel:
     def _decode_attention(self, i: int, q: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
                           max_ctx: int, workspace: torch.Tensor, out: torch.Tensor) -> None:
         cfg, c = self.cfg, self.cache
-        if c.scales is None:
+        if c.kind == "int4":
+            ops.decode_attention_int4(q, c.k(i), c.v(i), block_tables, ctx_lens, cfg.heads, workspace, out=out,
+                                      status=self.status)
+        elif c.kind == "bf16":
             ops.decode_attention(q, c.k(i), c.v(i), block_tables, ctx_lens, cfg.heads, max_ctx, workspace, out=out)
         else:
             ops.decode_attention_fp8(q, c.k(i), c.v(i), c.k_scale(i), c.v_scale(i), block_tables, ctx_lens, cfg.heads,
@@ -427,7 +560,10 @@ class LlamaModel:
     def _chunk_attention(self, i: int, q: torch.Tensor, block_tables: torch.Tensor, tile_info: torch.Tensor,
                          out: torch.Tensor, n_blocks: Optional[int] = None) -> None:
         cfg, c = self.cfg, self.cache
-        if c.scales is None:
+        if c.kind == "int4":
+            ops.prefill_attention_paged_int4(q, c.k(i), c.v(i), block_tables, tile_info, cfg.heads, cfg.kv_heads, out=out,
+                                             status=self.status, n_blocks=n_blocks)
+        elif c.kind == "bf16":
             ops.prefill_attention_paged(q, c.k(i), c.v(i), block_tables, tile_info, cfg.heads, cfg.kv_heads, out=out,
                                         status=self.status)
         else:
@@ -437,19 +573,21 @@ class LlamaModel:
     def decode_workspace(self, max_batch: int, max_ctx: int) -> torch.Tensor:
         """The decode attention's workspace for this model's cache."""
         cfg = self.cfg
-        if self.cache.scales is None:
+        if self.cache.kind == "bf16":
             return ops.decode_workspace(max_batch, cfg.heads, max_ctx, self.device)
+        if self.cache.kind == "int4":
+            return ops.decode_workspace_int4(max_batch, cfg.heads, cfg.kv_heads, self.device)
         return ops.decode_workspace_fp8(max_batch, cfg.heads, cfg.kv_heads, self.device)
 
     def _layer_tail(self, l: int, T: int):
-        cfg, lw = self.cfg, self.w.layers[l]
-        x, h = self.x[:T], self.h[:T]
+        layers, lw, x = self.w.layers, self.w.layers[l], self.x[:T]
         self._residual_gemm(self.attn[:T], lw.wo, x)
-        ops.rmsnorm(x, lw.mlp_norm, cfg.eps, out=h)
-        ops.gemm(h, lw.w13, self.mid[:T], silu_mul=True, status=self.status)
-        self._residual_gemm(self.mid[:T], lw.w2, x)
-        nw = self.w.layers[l + 1].attn_norm if l + 1 < cfg.layers else self.w.final_norm
-        ops.rmsnorm(x, nw, cfg.eps, out=h)
+        self._norm(x, lw.mlp_norm, lw.w13, T)
+        self._mlp(lw, T, x)
+        if l + 1 < len(layers):
+            self._norm(x, layers[l + 1].attn_norm, layers[l + 1].wqkv, T)
+        else:
+            self._norm(x, self.w.final_norm, None, T)
 
     def _head(self, rows: torch.Tensor, B: int) -> torch.Tensor:
         last = self.last[:B]
@@ -464,7 +602,7 @@ class LlamaModel:
                 block_tables: Optional[torch.Tensor] = None, n_blocks: Optional[int] = None) -> torch.Tensor:
         """Prefill a packed batch; returns the greedy next token of each sequence.
 
-        With an 8-bit cache the attention reads it: ``block_tables`` [B,
+        With an 8-bit or a 4-bit cache the attention reads it: ``block_tables`` [B,
         max_blocks] is then needed, and ``tile_info`` from
         ``prefill_tile_info(seq_lens, device, ctx)``; ``n_blocks``, the blocks
         that the sequences have together, bounds the workspace (by default the
@@ -477,19 +615,18 @@ class LlamaModel:
         than its attention kernel)."""
         cfg, T = self.cfg, ids.numel()
         assert T <= self.max_tokens
-        if self.cache.scales is not None and block_tables is None:
-            raise ValueError("prefill over an 8-bit cache needs block_tables")
+        if self.cache.kind != "bf16" and block_tables is None:
+            raise ValueError("prefill over an 8-bit cache, or one of 4 bits, needs block_tables")
         nvtx.push(f"prefill T={T}")
         ops.embedding(ids, self.w.embed, self.x[:T], status=self.status)
-        ops.rmsnorm(self.x[:T], self.w.layers[0].attn_norm, cfg.eps, out=self.h[:T])
+        self._norm(self.x[:T], self.w.layers[0].attn_norm, self.w.layers[0].wqkv, T)
         for l, lw in enumerate(self.w.layers):
             nvtx.push(f"layer {l}")
-            qkv = self.qkv[:T]
-            ops.gemm(self.h[:T], lw.wqkv, qkv, status=self.status)
+            qkv = self._qkv(lw, T)
             q = self._rotate_and_cache(l, qkv, positions, slots)
             if layer_hook is not None and not hook_after_attention:
                 layer_hook(l)
-            if self.cache.scales is None:
+            if self.cache.kind == "bf16":
                 ops.prefill_attention(qkv, tile_info, cfg.heads, cfg.kv_heads, out=self.attn[:T])
             else:
                 self._chunk_attention(l, q, block_tables, tile_info, self.attn[:T], n_blocks)
@@ -509,10 +646,9 @@ class LlamaModel:
         cfg, B = self.cfg, ids.numel()
         nvtx.push(f"decode B={B}")
         ops.embedding(ids, self.w.embed, self.x[:B], status=self.status)
-        ops.rmsnorm(self.x[:B], self.w.layers[0].attn_norm, cfg.eps, out=self.h[:B])
+        self._norm(self.x[:B], self.w.layers[0].attn_norm, self.w.layers[0].wqkv, B)
         for l, lw in enumerate(self.w.layers):
-            qkv = self.qkv[:B]
-            ops.gemm(self.h[:B], lw.wqkv, qkv, status=self.status)
+            qkv = self._qkv(lw, B)
             q = self._rotate_and_cache(l, qkv, positions, slots)
             self._decode_attention(l, q, block_tables, ctx_lens, max_ctx, workspace, self.attn[:B])
             self._layer_tail(l, B)
@@ -525,6 +661,9 @@ class LlamaModel:
 def reference_forward(weights: LlamaWeights, seqs: Sequence[Sequence[int]]) -> List[torch.Tensor]:
     """fp32 PyTorch forward (no cache) returning last-position logits per sequence."""
     from connex_b200.ops import reference as R
+
+    def plain(w):
+        return w.float() if isinstance(w, Fp8Weight) else w
     cfg = weights.cfg
     cos_sin = ops.rope_cos_sin(cfg.max_pos, cfg.head_dim, cfg.rope_theta, weights.embed.device,
                                cfg.rope_scaling)
@@ -544,7 +683,7 @@ def reference_forward(weights: LlamaWeights, seqs: Sequence[Sequence[int]]) -> L
             a = R.causal_attention(q, k, v, [n]).reshape(n, -1)
             x = x + a @ lw.wo.float().t()
             h = R.rmsnorm(x, lw.mlp_norm, cfg.eps)
-            x = x + R.silu_mul_gemm(h, lw.w13) @ lw.w2.float().t()
+            x = x + R.silu_mul_gemm(h, plain(lw.w13)) @ lw.w2.float().t()
         h = R.rmsnorm(x[-1:], weights.final_norm, cfg.eps)
         outs.append((h @ weights.lm_head.float().t())[0])
     return outs

@@ -150,7 +150,8 @@ class Qwen3MoeRank:
 
     def decode(self, ids, positions, slots, block_tables, ctx_lens, max_ctx, workspace, routing, l2p, l2p_cnt):
         """One decode step of this rank's batch; ``routing[l] = (topk_idx, topk_w)``;
-        ``workspace`` from ``ops.decode_workspace`` (8-bit cache: ``ops.decode_workspace_fp8``)."""
+        ``workspace`` from ``ops.decode_workspace`` (8-bit cache: ``ops.decode_workspace_fp8``, 4-bit:
+        ``ops.decode_workspace_int4``)."""
         cfg, T = self.cfg, ids.numel()
         x, h = self.x[:T], self.h[:T]
         ops.embedding(ids, self.embed, x, status=self.status)
@@ -159,7 +160,13 @@ class Qwen3MoeRank:
             qkv = self.qkv[:T]
             ops.gemm(h, a.wqkv, qkv, status=self.status)
             c = self.cache
-            if c.scales is None:
+            if c.kind == "int4":
+                q = ops.rope_cache_int4(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots, c.k(l), c.v(l),
+                                        out=qkv[:, :cfg.heads * cfg.head_dim], status=self.status, q_norm=a.q_norm,
+                                        k_norm=a.k_norm, eps=cfg.eps)
+                ops.decode_attention_int4(q, c.k(l), c.v(l), block_tables, ctx_lens, cfg.heads, workspace,
+                                          out=self.att[:T], status=self.status)
+            elif c.kind == "bf16":
                 ops.rope_cache(qkv, positions, self.cos_sin, cfg.heads, cfg.kv_heads, slots, c.k(l), c.v(l),
                                status=self.status, q_norm=a.q_norm, k_norm=a.k_norm, eps=cfg.eps)
                 ops.decode_attention(qkv, c.k(l), c.v(l), block_tables, ctx_lens, cfg.heads, max_ctx, workspace,

@@ -32,7 +32,7 @@ from typing import Optional
 import torch
 
 from connex_b200 import ops
-from connex_b200.models.llama import LayerWeights, LlamaConfig, LlamaWeights
+from connex_b200.models.llama import Fp8Weight, LayerWeights, LlamaConfig, LlamaWeights
 
 HEAD_DIM = 128
 
@@ -62,6 +62,8 @@ def tp_config(cfg: LlamaConfig, world: int) -> LlamaConfig:
 
 
 def shard_layer(lw: LayerWeights, cfg: LlamaConfig, rank: int, world: int) -> LayerWeights:
+    if any(isinstance(t, Fp8Weight) for t in lw.__dict__.values()):
+        raise ValueError("layers are cut into shards as bf16; quantise the shards (LlamaWeights.to_fp8)")
     hq, hkv = cfg.heads // world, cfg.kv_heads // world
     q0 = cfg.heads * HEAD_DIM
     qs = lw.wqkv[rank * hq * HEAD_DIM:(rank + 1) * hq * HEAD_DIM]

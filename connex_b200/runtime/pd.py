@@ -42,7 +42,9 @@ from connex_b200.models.llama import LlamaModel, PagedKVCache, slot_mapping
 
 def _bf16_only(cache: PagedKVCache) -> None:
     """The layerwise transfer moves a cache's values alone: an 8-bit cache's
-    scales would be left behind."""
+    scales would be left behind, and its prefill does not read a 4-bit one."""
+    if getattr(cache, "kind", "bf16") == "int4":
+        raise ValueError("the layerwise KV transfer moves bf16 caches, not 4-bit ones")
     if getattr(cache, "scales", None) is not None:
         raise ValueError("the layerwise KV transfer moves bf16 caches; an 8-bit cache's scales do not travel with it")
 

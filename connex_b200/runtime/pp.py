@@ -77,22 +77,20 @@ class StageModel(LlamaModel):
         return self.w.final_norm if self.is_last else None
 
     def _tail(self, i: int, T: int) -> None:
-        cfg, lw = self.cfg, self.w.layers[i]
-        x, h = self.x[:T], self.h[:T]
+        layers, lw, x = self.w.layers, self.w.layers[i], self.x[:T]
         self._residual_gemm(self.attn[:T], lw.wo, x)
-        ops.rmsnorm(x, lw.mlp_norm, cfg.eps, out=h)
-        ops.gemm(h, lw.w13, self.mid[:T], silu_mul=True, status=self.status)
-        self._residual_gemm(self.mid[:T], lw.w2, x)
+        self._norm(x, lw.mlp_norm, lw.w13, T)
+        self._mlp(lw, T, x)
         nw = self._next_norm(i)
         if nw is not None:
-            ops.rmsnorm(x, nw, self.cfg.eps, out=h)
+            self._norm(x, nw, layers[i + 1].wqkv if i + 1 < len(layers) else None, T)
 
     def _enter(self, inp: torch.Tensor, T: int) -> None:
         if self.is_first:
             ops.embedding(inp, self.w.embed, self.x[:T], status=self.status)
         else:
             self.x[:T].copy_(inp)
-        ops.rmsnorm(self.x[:T], self.w.layers[0].attn_norm, self.cfg.eps, out=self.h[:T])
+        self._norm(self.x[:T], self.w.layers[0].attn_norm, self.w.layers[0].wqkv, T)
 
     def run(self, inp: torch.Tensor, positions, slots, *, prefill: bool, tile_info=None, block_tables=None,
             ctx_lens=None, max_ctx: int = 0, workspace=None, rows=None, B: int = 0, n_dec: Optional[int] = None,
@@ -107,16 +105,17 @@ class StageModel(LlamaModel):
         ``tile_info`` of width 5; ``n_blocks``: cache blocks that they read,
         for an 8-bit cache); every GEMM runs once over all rows.
 
-        ``prefill`` without ``n_dec`` attends to the step's own rows, which an
-        8-bit cache's write leaves with unrotated keys: refused over one."""
+        ``prefill`` without ``n_dec`` attends to the step's own rows, which the
+        write of an 8-bit or a 4-bit cache leaves with unrotated keys: refused
+        over one."""
         cfg, T = self.cfg, inp.shape[0]
         assert T <= self.max_tokens
-        if prefill and n_dec is None and self.cache.scales is not None:
-            raise ValueError("prefill over an 8-bit cache reads the cache: run it as a mixed step (n_dec, block_tables)")
+        if prefill and n_dec is None and self.cache.kind != "bf16":
+            raise ValueError("prefill over an 8-bit cache, or one of 4 bits, reads the cache: run it as a mixed step "
+                             "(n_dec, block_tables)")
         self._enter(inp, T)
         for i, lw in enumerate(self.w.layers):
-            qkv = self.qkv[:T]
-            ops.gemm(self.h[:T], lw.wqkv, qkv, status=self.status)
+            qkv = self._qkv(lw, T)
             q = self._rotate_and_cache(i, qkv, positions, slots)
             if n_dec is not None:
                 if n_dec:
@@ -143,7 +142,8 @@ class StageRuntime:
                  tp=None, kv_dtype: torch.dtype = torch.bfloat16):
         """``weights``: layers ``[l0, l1)`` already on ``device`` (e.g. from
         :func:`connex_b200.models.hf.load_llama`); random from ``seed`` if absent.
-        ``kv_dtype``: ``torch.float8_e4m3fn`` for an 8-bit KV cache."""
+        ``kv_dtype``: ``torch.float8_e4m3fn`` for an 8-bit KV cache, ``torch.uint8``
+        for one of 4 bits."""
         self.cfg = cfg
         self.device = torch.device(device)
         if weights is not None and len(weights.layers) != l1 - l0:
@@ -350,8 +350,8 @@ class StageRuntime:
         ctx = list(td[CX_CTX])
         n_new = list(td["n_new"])
         kind = td["kind"]
-        # chunks that continue cached sequences; an 8-bit cache is read for whole prompts, too
-        if kind == "prefill" and (any(ctx) or self.cache.scales is not None):
+        # chunks that continue cached sequences; a quantised cache is read for whole prompts, too
+        if kind == "prefill" and (any(ctx) or self.cache.kind != "bf16"):
             kind = "mixed"
         n_dec = int(td.get("n_dec", 0)) if kind == "mixed" else None
         prefill = kind == "prefill"

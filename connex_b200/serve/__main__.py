@@ -38,8 +38,12 @@ def model_args(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--device", default="cuda:0")
     ap.add_argument("--num-blocks", type=int, default=0, help="KV blocks (0: from --kv-fraction of free memory)")
     ap.add_argument("--kv-fraction", type=float, default=0.8)
-    ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "fp8"],
-                    help="KV cache: bf16, or fp8 (e4m3 with a scale per block and head: twice the blocks)")
+    ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "fp8", "int4"],
+                    help="KV cache: bf16, fp8 (e4m3 with a scale per block and head: twice the blocks) or int4 (4-bit "
+                    "codes, a scale and a minimum per half of a token's head: 3.5 times the blocks)")
+    ap.add_argument("--weight-dtype", default="bf16", choices=["bf16", "fp8"],
+                    help="the layers' projections: bf16, or fp8 (e4m3 with a scale per 128 x 128 block; an fp8 "
+                    "checkpoint's are taken as they are either way)")
     ap.add_argument("--max-batch", type=int, default=64)
     ap.add_argument("--max-ctx", type=int, default=4096)
     ap.add_argument("--max-step-tokens", type=int, default=8192)
@@ -86,13 +90,15 @@ def kv_blocks(a, cfg, l0: int, l1: int) -> int:
     free, _ = torch.cuda.mem_get_info(torch.device(a.device))
     n_layers = l1 - l0
     per_layer = cfg.qkv_dim * cfg.hidden + cfg.hidden * cfg.heads * cfg.head_dim + 3 * cfg.ffn * cfg.hidden
-    weights = 2 * (n_layers * per_layer + 2 * cfg.vocab_size * cfg.hidden)
+    per_weight = 1 if getattr(a, "weight_dtype", "bf16") == "fp8" else 2
+    weights = per_weight * n_layers * per_layer + 2 * 2 * cfg.vocab_size * cfg.hidden
     scratch = 2 << 30                       # activations, workspaces, allocator slack
     room, bf16 = free - weights - scratch, cfg.block_size * cfg.head_dim * 2
-    fp8 = getattr(a, "kv_dtype", "bf16") == "fp8"
-    block = 2 * n_layers * cfg.kv_heads * (bf16 // 2 + 4 if fp8 else bf16)
+    kind = getattr(a, "kv_dtype", "bf16")
+    head = {"fp8": bf16 // 2 + 4, "int4": cfg.block_size * 72}.get(kind, bf16)
+    block = 2 * n_layers * cfg.kv_heads * head
     n = int(room * a.kv_fraction) // block
-    if fp8:       # a prompt step holds the blocks that it reads as bf16, for one layer at a time
+    if kind != "bf16":       # a prompt step holds the blocks that it reads as bf16, for one layer at a time
         copy = 2 * cfg.kv_heads * bf16
         most = min(a.max_batch, a.max_step_tokens) * -(-a.max_ctx // cfg.block_size)     # that one step reads
         n = min(n, max(room // (block + copy), (room - most * copy) // block))
@@ -114,7 +120,8 @@ def build_stepper(a):
     if a.num_stages == 1:
         n = kv_blocks(a, cfg, 0, cfg.layers)
         return ModelStepper(cfg, dev, n, a.max_batch, a.max_ctx, a.max_step_tokens, a.checkpoint, a.seed,
-                            graphs=not a.no_graphs, kv_dtype=getattr(a, "kv_dtype", "bf16")), None
+                            graphs=not a.no_graphs, kv_dtype=getattr(a, "kv_dtype", "bf16"),
+                         weight_dtype=getattr(a, "weight_dtype", "bf16")), None
     from connex_b200.serve import pipeline
     ranges = pipeline.split_layers(cfg.layers, a.num_stages, a.stage_starts)
     if not a.directory:
@@ -123,7 +130,8 @@ def build_stepper(a):
     ep, client = pipeline.join(a.model_name or "connex-b200", 0, a.num_stages, a.replica, dev, a.directory, a.data,
                                a.store, a.store_master, a.advertise_host, a.recv_timeout_s)
     st = PipelineStepper(cfg, ranges[0][1], dev, ep, n, a.max_batch, a.max_ctx, a.max_step_tokens, a.checkpoint,
-                         a.seed, a.recv_timeout_s, graphs=not a.no_graphs, kv_dtype=getattr(a, "kv_dtype", "bf16"))
+                         a.seed, a.recv_timeout_s, graphs=not a.no_graphs, kv_dtype=getattr(a, "kv_dtype", "bf16"),
+                         weight_dtype=getattr(a, "weight_dtype", "bf16"))
     ep.warm_stage(1)
     ep.auto_warm = True
     ep.watchdog = pipeline.watchdog(ep, st.link, client, step_timeout=a.step_timeout_s)
@@ -175,7 +183,8 @@ def _tp_stepper(a, cfg):
     t = torch.tensor([blocks], device=dev)
     dist.all_reduce(t, op=dist.ReduceOp.MIN)              # every rank sizes its KV cache alike
     inner = ModelStepper(cfg, dev, int(t.item()), a.max_batch, a.max_ctx, a.max_step_tokens, a.checkpoint,
-                         a.seed, graphs=False, tp=TPGroup(rank, world), kv_dtype=getattr(a, "kv_dtype", "bf16"))
+                         a.seed, graphs=False, tp=TPGroup(rank, world), kv_dtype=getattr(a, "kv_dtype", "bf16"),
+                         weight_dtype=getattr(a, "weight_dtype", "bf16"))
     if rank == 0:
         return TPStepper(inner, cpu), ("tp", cpu)
     log.info("TP rank %d of %d following rank 0", rank, world)

@@ -32,14 +32,17 @@ def run_stage(a, stop: threading.Event) -> dict:
                                    a.directory, "inline", None, False, a.advertise_host, a.recv_timeout_s)
         return _serve_loop(ep, client, StageWorker(ep, rt, rt.compute), stop, a, (a.stage, a.stage + 1))
     from connex_b200.models.hf import load_llama
-    from connex_b200.runtime.pp import StageRuntime
+    from connex_b200.runtime.pp import StageRuntime, stage_weights
     from connex_b200.serve import pipeline
     from connex_b200.serve.engine import torch_kv_dtype
     cfg = llama_config(a)
     dev = torch.device(a.device)
     torch.cuda.set_device(dev)
     l0, l1 = pipeline.split_layers(cfg.layers, a.num_stages, a.stage_starts)[a.stage]
-    weights = load_llama(a.checkpoint, dev, layers=(l0, l1), cfg=cfg) if a.checkpoint else None
+    fp8 = getattr(a, "weight_dtype", "bf16") == "fp8"
+    weights = load_llama(a.checkpoint, dev, layers=(l0, l1), cfg=cfg, fp8=fp8) if a.checkpoint else None
+    if fp8 and weights is None:
+        weights = stage_weights(cfg, l0, l1, dev, a.seed).to_fp8()
     rt = StageRuntime(cfg, l0, l1, dev, num_blocks=kv_blocks(a, cfg, l0, l1), max_tokens=a.max_step_tokens,
                       max_batch=a.max_batch, max_ctx=a.max_ctx, seed=a.seed, weights=weights,
                       kv_dtype=torch_kv_dtype(getattr(a, "kv_dtype", "bf16")))

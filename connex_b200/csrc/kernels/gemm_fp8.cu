@@ -562,14 +562,17 @@ static void launch_gemm_fp8(const GemmFp8& g, int sms, int* status, cudaStream_t
 
 // ------------------------------------------------------- few rows: split K
 // Where the 128 x 256 tiles would leave SMs idle: the weight's rows are the MMA's 128 rows and NT activations its
-// columns, and the CTAs of a cluster share a tile's blocks of 128 columns among them.  Each adds up its part in
-// registers as above (a thread per weight row; the scales of a block lie in shared memory, a's times b's), leaves it
-// in shared memory, and the CTAs then add the parts of a slice of the activations each, in the order of their ranks,
-// over the cluster's shared memory: no workspace, no atomics, the same bits from run to run.  A warp writes a row of
-// 128 outputs.  SiLU-mul takes R = 2 blocks of weight rows, gate and up.
-// What bounds it: a block of 128 columns takes a CTA 500 to 600 cycles (the issuing thread's two waits and four MMAs,
-// up to 64 activations; the promotion beyond), and 5 to 6 us pass around that (launch, first loads, the cluster's
-// sums): 64 x 4096 x 14336 takes 17.4 us where reading the operands takes 9.4, one row 14.8.
+// columns (or 128 activations its rows and 128 weight rows its columns), and the CTAs of a cluster share a tile's blocks
+// of 128 columns among them.  Each adds up its part in registers as above (a thread per MMA row; the scales of a block
+// lie in shared memory, a's times b's), leaves it in shared memory, and the CTAs then add the parts of a slice of the
+// activations each, in the order of their ranks, over the cluster's shared memory: no workspace, no atomics, the same
+// bits from run to run.  A warp writes a row of 128 outputs.  SiLU-mul takes R = 2 blocks of weight rows, gate and up.
+// What bounds it: a block of 128 columns takes a CTA 500 to 700 cycles, as long with two warpgroups that add up the
+// blocks in turn or with half the waits of the issuing thread: 40 to 50 bytes a cycle come to an SM.  5 to 6 us pass
+// around that (launch, first loads, the cluster's sums): 64 x 4096 x 14336 takes 17.4 us where reading the operands
+// takes 9.4, one row 14.8.  With activations as columns a thread needs another scale for each of its sums, and shared
+// memory brings 32 of them a cycle: 1024 cycles for 256 activations.  So 128 of them are rows, a scale a thread: 613 x
+// 2048 x 4096 takes 18.2 us (256 activations as columns 26.2), 512 x 4096 x 14336 48 (63).
 namespace g8s {
 constexpr int BK = 128, Q = 128;
 constexpr int SC_SLOTS = 2;
@@ -577,20 +580,27 @@ template <int NT, int R>
 struct Cfg {
   // two CTAs on an SM where their stages and registers fit: one computes while the other waits
   static constexpr int PER_SM = R * NT <= 32 ? 2 : 1;
-  static constexpr int A_BYTES = R * Q * BK, B_BYTES = NT * BK, STAGE = A_BYTES + B_BYTES;
+  static constexpr bool TALL = NT == Q;           // the activations are the MMA's rows
+  // Blocks of columns of a stage, its waits and commits.  (512 x 4096 x 14336 52.0 us with one; with two, 64 x 4096 x
+  // 14336 17.9 us, with one 17.4: fewer loads are on their way at the start.)
+  static constexpr int KS = TALL ? 2 : 1;
+  static constexpr int A_BYTES = R * Q * BK, B_BYTES = NT * BK, BLOCK = A_BYTES + B_BYTES, STAGE = KS * BLOCK;
   static constexpr int SC_KB = R == 1 && NT <= 64 ? 8 : 4;  // blocks of columns whose scales come together
   static constexpr int SCALES = SC_SLOTS * SC_KB * R * NT * 4;
-  static constexpr int PARTS = NT * R * Q * 4;    // in the stages, once they are empty
+  // In the stages, once they are empty.  (Eight lanes that store four columns of a row each: rows 16 bytes apart in the
+  // banks.)
+  static constexpr int PITCH = R * Q + (TALL ? 4 : 0), PARTS = NT * PITCH * 4;
   static constexpr int ROOM = (PER_SM == 2 ? 113 * 1024 : 200 * 1024) - SCALES - 1024 - 512;
   static constexpr int STAGES = ROOM / STAGE;
-  static_assert(STAGES >= 3 && PARTS <= STAGES * STAGE, "stages");
+  static_assert(STAGES >= 2 && PARTS <= STAGES * STAGE, "stages");
   static constexpr int SMEM = 1024 + STAGES * STAGE + SCALES + 512;
   // Accumulators in TMEM, up to eight: a block's sums are read some 1000 cycles after its MMAs have begun.
-  static constexpr int ACCS = 512 / PER_SM / (R * NT) < 8 ? 512 / PER_SM / (R * NT) : 8;
-  static constexpr int COLS = ACCS * R * NT;
-  static constexpr int GROUPS = R * NT > 128 ? 2 : 1, THREADS = 128 + 128 * GROUPS;
-  static constexpr int MINE = NT / GROUPS;        // activations of a thread
-  static constexpr int CH = GROUPS == 1 && MINE >= 32 ? 32 : 16;                 // of them, read from TMEM at a time
+  static constexpr int ACCS = (512 / PER_SM / (R * NT) < 8 ? 512 / PER_SM / (R * NT) : 8) / KS;    // groups of KS
+  static constexpr int COLS = ACCS * KS * R * NT;
+  static constexpr int GROUPS = R * NT >= 128 ? 2 : 1, THREADS = 128 + 128 * GROUPS;
+  static constexpr int MINE = NT / GROUPS;        // sums of a thread, of each r
+  static constexpr int CH = MINE >= 32 ? 32 : 16; // of them, read from TMEM at a time
+  static_assert(!TALL || R == 1, "one block of weight rows");
 };
 }  // namespace g8s
 
@@ -621,7 +631,7 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
                           int splits, int* status) {
   using namespace g8s;
   using C = Cfg<NT, R>;
-  constexpr int STAGES = C::STAGES, SC_KB = C::SC_KB;
+  constexpr int STAGES = C::STAGES, SC_KB = C::SC_KB, KS = C::KS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* parts = reinterpret_cast<float*>(smem);                                 // [NT][R * 128]
@@ -670,14 +680,18 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
 
   if (warp == 0) {
     uint32_t stage = 0, phase = 0;
-    for (int kb = k0; kb < k1; ++kb) {
+    for (int kb = k0; kb < k1; kb += KS) {
       ok = mbar_wait_poll(&empty[stage], phase ^ 1, status);
       if (!ok) break;
       if (elect_sync()) {
         uint8_t* at = smem + stage * C::STAGE;
-        mbar_arrive_expect_tx(&full[stage], C::STAGE);
-        tma_load_2d(at, &tmB, &full[stage], kb * BK, tile * R * Q);              // the weight
-        tma_load_2d(at + C::A_BYTES, &tmA, &full[stage], kb * BK, m0);
+        mbar_arrive_expect_tx(&full[stage], min(KS, k1 - kb) * C::BLOCK);
+#pragma unroll
+        for (int j = 0; j < KS; ++j, at += C::BLOCK)
+          if (kb + j < k1) {
+            tma_load_2d(at, &tmB, &full[stage], (kb + j) * BK, tile * R * Q);    // the weight
+            tma_load_2d(at + C::A_BYTES, &tmA, &full[stage], (kb + j) * BK, m0);
+          }
       }
       __syncwarp();
       if (++stage == STAGES) {
@@ -692,18 +706,24 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
     const uint32_t w_lo = umma_desc_sw128_lo(smem_u32(smem));
     uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
     bool issued = false;
-    for (int kb = k0; kb < k1; ++kb) {
+    for (int kb = k0; kb < k1; kb += KS) {
       ok = mbar_wait_poll(&tempty[acc], acc_phase ^ 1, status) && mbar_wait_poll(&full[stage], phase, status);
       if (!ok) break;
       tc_fence_after();
       if (elect_sync()) {
-        const uint32_t wl = w_lo + stage * (C::STAGE / 16), xl = wl + C::A_BYTES / 16;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int j = 0; j < KS; ++j) {
+          // (the two operands' tiles have the same size where they change places)
+          const uint32_t at = w_lo + (stage * C::STAGE + j * C::BLOCK) / 16, other = at + C::A_BYTES / 16;
+          const uint32_t wl = C::TALL ? other : at, xl = C::TALL ? at : other;
+          if (kb + j < k1)
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)
-            umma_e4m3(tmem_base + (acc * R + r) * NT, umma_desc_sw128_of(wl + r * (Q * BK / 16) + 2 * k),
-                      umma_desc_sw128_of(xl + 2 * k), IDESC, k != 0);
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+              for (int k = 0; k < BK / 32; ++k)
+                umma_e4m3(tmem_base + ((acc * KS + j) * R + r) * NT, umma_desc_sw128_of(wl + r * (Q * BK / 16) + 2 * k),
+                          umma_desc_sw128_of(xl + 2 * k), IDESC, k != 0);
+        }
         umma_commit(&tfull[acc]);
         umma_commit(&empty[stage]);
       }
@@ -778,34 +798,52 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
 #pragma unroll
       for (int i = 0; i < C::MINE; ++i) sum[r][i] = 0.f;
     for (int kb = k0; kb < k1; ++kb) {
-      const int k = (kb - k0) & (SC_KB - 1);
+      const int k = (kb - k0) & (SC_KB - 1), j = k & (KS - 1);
+      const bool last = j == KS - 1 || kb == k1 - 1;           // of its group
       if (k == 0) ok = ok && mbar_wait_warp(&sfull[slot], sc_phase, status);
-      ok = ok && mbar_wait_warp(&tfull[acc], acc_phase, status);
+      if (j == 0) ok = ok && mbar_wait_warp(&tfull[acc], acc_phase, status);
       if (ok) {
         tc_fence_after();
-        const uint32_t tb = tmem_base + acc * R * NT + wg * C::MINE + ((uint32_t)(quad * 32) << 16);
-        const float* sc = scales + (slot * SC_KB + k) * R * NT + wg * C::MINE;
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int c = 0; c < C::MINE / C::CH; ++c) {
-            uint32_t t[C::CH];
-            if constexpr (C::CH == 32) tmem_ld32(tb + r * NT + c * C::CH, t);
-            else tmem_ld16(tb + r * NT + c * C::CH, t);
-            float4 f[C::CH / 4];
-#pragma unroll
-            for (int i = 0; i < C::CH / 4; ++i) f[i] = *reinterpret_cast<const float4*>(sc + r * NT + c * C::CH + 4 * i);
-            tmem_ld_wait_for(t);
-            if (r == R - 1 && c == C::MINE / C::CH - 1) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&tempty[acc]);
-            }
-#pragma unroll
-            for (int i = 0; i < C::CH; ++i)
-              sum[r][c * C::CH + i] =
-                  fmaf(__uint_as_float(t[i]), reinterpret_cast<const float*>(f)[i], sum[r][c * C::CH + i]);
+        const uint32_t tb = tmem_base + (acc * KS + j) * R * NT + wg * C::MINE + ((uint32_t)(quad * 32) << 16);
+        const float* sc = scales + (slot * SC_KB + k) * R * NT + (C::TALL ? quad * 32 + lane : wg * C::MINE);
+        if constexpr (C::TALL) {
+          static_assert(C::MINE == 64, "two reads of 32");
+          uint32_t t[2][32];
+          tmem_ld32(tb, t[0]);
+          tmem_ld32(tb + 32, t[1]);
+          const float f = *sc;
+          tmem_ld_wait_for(t[0]);
+          tmem_ld_wait_for(t[1]);
+          if (last) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[acc]);
           }
+#pragma unroll
+          for (int i = 0; i < 64; ++i) sum[0][i] = fmaf(__uint_as_float(t[i >> 5][i & 31]), f, sum[0][i]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int c = 0; c < C::MINE / C::CH; ++c) {
+              uint32_t t[C::CH];
+              if constexpr (C::CH == 32) tmem_ld32(tb + r * NT + c * C::CH, t);
+              else tmem_ld16(tb + r * NT + c * C::CH, t);
+              float4 f[C::CH / 4];
+#pragma unroll
+              for (int i = 0; i < C::CH / 4; ++i) f[i] = *reinterpret_cast<const float4*>(sc + r * NT + c * C::CH + 4 * i);
+              tmem_ld_wait_for(t);
+              if (r == R - 1 && c == C::MINE / C::CH - 1 && last) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&tempty[acc]);
+              }
+#pragma unroll
+              for (int i = 0; i < C::CH; ++i)
+                sum[r][c * C::CH + i] =
+                    fmaf(__uint_as_float(t[i]), reinterpret_cast<const float*>(f)[i], sum[r][c * C::CH + i]);
+            }
+        }
       }
       if (k == SC_KB - 1 || kb == k1 - 1) {
         __syncwarp();
@@ -815,7 +853,7 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
           sc_phase ^= 1;
         }
       }
-      if (++acc == C::ACCS) {
+      if (last && ++acc == C::ACCS) {
         acc = 0;
         acc_phase ^= 1;
       }
@@ -825,7 +863,15 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 0; i < C::MINE; ++i) parts[(wg * C::MINE + i) * (R * Q) + r * Q + quad * 32 + lane] = sum[r][i];
+        for (int i = 0; i < C::MINE; ++i) {
+          if constexpr (C::TALL) {
+            if (i % 4 == 0)
+              *reinterpret_cast<float4*>(parts + (quad * 32 + lane) * C::PITCH + wg * C::MINE + i) =
+                  make_float4(sum[r][i], sum[r][i + 1], sum[r][i + 2], sum[r][i + 3]);
+          } else {
+            parts[(wg * C::MINE + i) * C::PITCH + r * Q + quad * 32 + lane] = sum[r][i];
+          }
+        }
   }
   __syncwarp();
   const bool failed = __syncthreads_or(!ok);
@@ -841,9 +887,9 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
     for (int s = 0; s < splits; ++s)
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const uint32_t at = base + (i * (R * Q) + r * Q + 4 * lane) * 4;
+        const uint32_t at = base + (i * C::PITCH + r * Q + 4 * lane) * 4;
         const float4 x = splits > 1 ? ld_cluster_f32x4(cluster_addr(at, s)) : *reinterpret_cast<const float4*>(
-                                                                                  parts + i * (R * Q) + r * Q + 4 * lane);
+                                                                                  parts + i * C::PITCH + r * Q + 4 * lane);
         v[r].x += x.x;
         v[r].y += x.y;
         v[r].z += x.z;
@@ -918,18 +964,18 @@ static void launch_gemm_fp8_split(const GemmFp8& g, int splits, int* status, cud
 // Which way a call goes: the least of the estimated times, in us.  A CTA takes `per` for a block of 128 columns and a
 // fixed start and end; clusters of four and eight do not fill every SM (132 and 120 of 148 are reached); reading the
 // operands takes its time whatever the CTAs.  The constants are fits to measured calls: 4096 weight rows with K = 4096
-// and 14336, one CTA per tile, and for the tiles of 128 x 256.  Estimated and measured: 1 x 6144 x 4096 8.3 and 9.2 (16
-// activations, four CTAs; one CTA 12.1, 128 x 256 tiles 21), 64 x 4096 x 14336 15.6 and 17.4 (64, four; 65), 613 x 2048
-// x 4096 23.3 and 26.6 (256, two; 30), 64 x 28672 x 4096 with SiLU-mul 25.6 and 25.6 (128 x 256 tiles; 64 activations
-// by one CTA 28.5), 512 x 4096 x 14336 60 and 63 (256, two; 71).
+// and 14336, one CTA per tile, and for the tiles of 128 x 256.  Estimated and measured: 1 x 6144 x 4096 8.3 and 9.5 (16
+// activations, four CTAs; one CTA 12.6, 128 x 256 tiles 21), 64 x 4096 x 14336 15.6 and 17.4 (64, four; 65), 613 x 2048
+// x 4096 17.8 and 18.2 (128, one; 29), 64 x 28672 x 4096 with SiLU-mul 25.6 and 26.0 (128 x 256 tiles; 64 activations
+// by one CTA 28), 512 x 4096 x 14336 48 and 48 (128, one; 71).
 GemmFp8Plan gemm_fp8_plan(int M, int N, int K, int epi, int sms) {
   const int r = epi == EPI_SILU_MUL ? 2 : 1, nk = (K + 127) / 128;
   const double read = ((double)M + N) * K / 5.5e6 + 4.0;
   const int64_t tiles = (int64_t)((M + 127) / 128) * ((N + 255) / 256);
   GemmFp8Plan best{0, 1};
   double cost = std::max(read, (double)((tiles + sms - 1) / sms) * (nk * 0.55 + 8.0));
-  constexpr double per[2][5] = {{0.26, 0.29, 0.32, 0.58, 0.92}, {0.35, 0.45, 0.75, 1.15, 0}};
-  for (int i = 0; i < (r == 2 ? 4 : 5); ++i) {
+  constexpr double per[2][4] = {{0.26, 0.29, 0.32, 0.375}, {0.35, 0.45, 0.70, 0}};
+  for (int i = 0; i < (r == 2 ? 3 : 4); ++i) {
     const int nt = 16 << i;
     const int64_t base = (int64_t)((M + nt - 1) / nt) * ((N + 128 * r - 1) / (128 * r));
     if (base > (int64_t)1 << 24 || (M + nt - 1) / nt > 65535) continue;
@@ -956,8 +1002,7 @@ void gemm_fp8(const GemmFp8& g, int sms, int* status, cudaStream_t stream) {
     case 16: return two ? launch_gemm_fp8_split<16, 2>(g, p.splits, status, stream) : launch_gemm_fp8_split<16, 1>(g, p.splits, status, stream);
     case 32: return two ? launch_gemm_fp8_split<32, 2>(g, p.splits, status, stream) : launch_gemm_fp8_split<32, 1>(g, p.splits, status, stream);
     case 64: return two ? launch_gemm_fp8_split<64, 2>(g, p.splits, status, stream) : launch_gemm_fp8_split<64, 1>(g, p.splits, status, stream);
-    case 128: return two ? launch_gemm_fp8_split<128, 2>(g, p.splits, status, stream) : launch_gemm_fp8_split<128, 1>(g, p.splits, status, stream);
-    case 256: return launch_gemm_fp8_split<256, 1>(g, p.splits, status, stream);
+    case 128: return launch_gemm_fp8_split<128, 1>(g, p.splits, status, stream);
     default: break;
   }
   if (two && g.sd.p != nullptr) launch_gemm_fp8<EPI_SILU_MUL, true>(g, sms, status, stream);

@@ -12,7 +12,9 @@ Cases: gemm (8192^3), gemm_qkv (T=8192 Llama-3-8B QKV), gemm_silu (T=8192
 gate/up + SiLU-mul), attn (8 x 2048-token causal prefill, 32/8 heads),
 attn_paged (the paged variant: 8 chunks of 2048 queries over 2048 cached tokens), decode_attn (64 x 4096-token paged decode), attn_paged_fp8 and decode_attn_fp8 (the same over the 8-bit cache), write_fp8 and write_fp8_rows
 (its quantising write: 4 x 2048 prompt rows, 64 rows of as many sequences), kv_copy_blocks (400 of its blocks in 32
-layers), kv_push (one layer of a 64k-token
+layers), quant_fp8 and gemm_fp8 (block-scaled fp8: 8192 rows of 4096; 8192 x 28672 x 4096 + SiLU-mul; gemm_fp8_m1
+and _m64: the few rows of a decode step), decode_attn_int4, attn_paged_int4, write_int4 (4-bit cache, as the 8-bit
+cases), kv_push (one layer of a 64k-token
 KV push, local), kv_push_nvlink (the same layer pushed from GPU 0 into GPU 1's
 memory over NVLink, one process, peer access; ``--ctas`` sets the grid,
 ``--pull`` runs the kernel on GPU 1 reading GPU 0's memory instead, ``--ce``
@@ -183,6 +185,75 @@ def case_write_fp8(dev, T=8192, per=2048, hq=32, hkv=8):
         "bytes": T * ((2 * hq + 2 * hkv) * 256 + 2 * hkv * 128), "check": _status_check(st, "8-bit cache write")}
 
 
+def _int4_cache(dev, nb, hkv):
+    """K or V of a 4-bit cache: any codes, scales 1 and minima -8."""
+    c = torch.randint(0, 256, (nb, hkv, 16, ops.KV_INT4_ROW), dtype=torch.uint8, device=dev)
+    c[..., 64:] = torch.tensor([1.0, -8.0, 1.0, -8.0], dtype=torch.bfloat16, device=dev).view(torch.uint8)
+    return c
+
+
+def case_attn_paged_int4(dev, n_seq=8, ctx=2048, L=2048, hq=32, hkv=8):
+    """:func:`case_attn_paged` over a 4-bit cache."""
+    T, per = n_seq * L, (ctx + L) // 16
+    nb = n_seq * per
+    k, v = _int4_cache(dev, nb, hkv), _int4_cache(dev, nb, hkv)
+    bt = torch.randperm(nb, device=dev).to(torch.int32).view(n_seq, per).contiguous()
+    q = (torch.randn(T, hq * 128, device=dev) * 0.1).bfloat16()
+    ti = ops.prefill_tile_info([L] * n_seq, dev, ctx=[ctx] * n_seq)
+    out = torch.empty(T, hq * 128, dtype=torch.bfloat16, device=dev)
+    st = ops.new_status(dev)
+    return (lambda: ops.prefill_attention_paged_int4(q, k, v, bt, ti, hq, hkv, out, status=st)), {
+        "flops": n_seq * hq * 4 * 128 * (L * ctx + L * L / 2), "check": _status_check(st, "4-bit paged prefill attention")}
+
+
+def case_decode_attn_int4(dev, B=64, ctx=4096, hq=32, hkv=8):
+    nb = B * ctx // 16
+    k, v = _int4_cache(dev, nb, hkv), _int4_cache(dev, nb, hkv)
+    bt = torch.randperm(nb, device=dev).to(torch.int32).view(B, ctx // 16).contiguous()
+    cl = torch.full((B,), ctx, dtype=torch.int32, device=dev)
+    q = (torch.randn(B, hq * 128, device=dev) * 0.1).bfloat16()
+    ws = ops.decode_workspace_int4(B, hq, hkv, dev)
+    out = torch.empty(B, hq * 128, dtype=torch.bfloat16, device=dev)
+    st = ops.new_status(dev)
+    return (lambda: ops.decode_attention_int4(q, k, v, bt, cl, hq, ws, out, status=st)), {
+        "bytes": 2 * k.numel(), "check": _status_check(st, "4-bit decode attention")}
+
+
+def case_write_int4(dev, T=8192, hq=32, hkv=8):
+    """RoPE and quantising write of T rows of prompts of 2048."""
+    k, v = _int4_cache(dev, T // 16, hkv), _int4_cache(dev, T // 16, hkv)
+    qkv = torch.randn(T, (hq + 2 * hkv) * 128, device=dev).bfloat16()
+    pos = (torch.arange(T, device=dev) % 2048).to(torch.int32)
+    slots = torch.arange(T, device=dev)
+    cs = ops.rope_cos_sin(4096, 128, 5e5, dev)
+    out = torch.empty(T, hq * 128, dtype=torch.bfloat16, device=dev)
+    st = ops.new_status(dev)
+    return (lambda: ops.rope_cache_int4(qkv, pos, cs, hq, hkv, slots, k, v, out, st)), {
+        "bytes": T * ((2 * hq + 2 * hkv) * 256 + 2 * hkv * ops.KV_INT4_ROW), "check": _status_check(st, "4-bit cache write")}
+
+
+def case_quant_fp8(dev, T=8192, K=4096, norm=False):
+    x = torch.randn(T, K, device=dev).bfloat16()
+    w = torch.ones(K, dtype=torch.bfloat16, device=dev) if norm else None
+    out, scale = ops.quantize_fp8(x, norm=w)
+    return (lambda: ops.quantize_fp8(x, norm=w, out=out, scale=scale)), {"bytes": T * K * 3 + scale.numel() * 4}
+
+
+def case_gemm_fp8(dev, M=8192, N=28672, K=4096, silu=True):
+    """The block-scaled product; few rows read other weights from call to call, more than the L2 holds."""
+    a, sa = ops.quantize_fp8(torch.randn(M, K, device=dev).bfloat16())
+    ws = [ops.quantize_weight_fp8(torch.randn(N, K, device=dev).bfloat16()) for _ in range(1 if silu else 2 + 2 ** 28 // (N * K))]
+    st, turn = ops.new_status(dev), [0]
+
+    def call():
+        turn[0] = (turn[0] + 1) % len(ws)
+        return ops.gemm_fp8(a, sa, *ws[turn[0]], silu_mul=silu, status=st)
+    work = {"flops": 2 * M * N * K, "check": _status_check(st, "block-scaled fp8 product")}
+    if M < 1024:
+        work["bytes"] = N * K + M * K + M * N * 2
+    return call, work
+
+
 def case_kv_copy_blocks(dev, n=400, layers=32, nb=1024, hkv=8):
     """n blocks of every layer of an 8-bit cache, with their scales."""
     kv = torch.randint(0, 120, (layers, 2, nb, hkv, 16, 128), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
@@ -329,16 +400,18 @@ def case_gemm_m(dev, M=1, N=28672, K=4096, silu=False):
     return (lambda: ops.gemm(a, b, out, silu_mul=silu)), {"bytes": N * K * 2 + M * K * 2 + M * N * 2}
 
 
-def case_decode_step(dev, B=1, ctx=1024, graphs=True, kv_dtype=torch.bfloat16):
+def case_decode_step(dev, B=1, ctx=1024, graphs=True, kv_dtype=torch.bfloat16, fp8=False):
     """One Llama-3-8B decode step for B sequences of ``ctx`` cached tokens,
     replayed from its CUDA graph (device time of the whole step; bytes =
-    weights + the KV read)."""
+    weights + the KV read); ``fp8``: block-scaled e4m3 projections.  A uint8
+    cache is the 4-bit one."""
     from connex.pp.handover import CX_CTX, REQUEST_IDS
     from connex_b200.models.llama import LlamaConfig
-    from connex_b200.runtime.pp import StageRuntime
+    from connex_b200.runtime.pp import StageRuntime, stage_weights
     cfg = LlamaConfig.llama3_8b()
+    sw = stage_weights(cfg, 0, cfg.layers, dev, 0)
     rt = StageRuntime(cfg, 0, cfg.layers, dev, num_blocks=B * (ctx + 64) // 16 + 64, max_tokens=max(B * ctx, 8192),
-                      max_batch=B, max_ctx=ctx + 64, kv_dtype=kv_dtype)
+                      max_batch=B, max_ctx=ctx + 64, kv_dtype=kv_dtype, weights=sw.to_fp8() if fp8 else sw)
     if graphs:
         rt.enable_decode_graphs()
     rids = [f"r{i}" for i in range(B)]
@@ -351,9 +424,9 @@ def case_decode_step(dev, B=1, ctx=1024, graphs=True, kv_dtype=torch.bfloat16):
         fn = rt.graphs[next(b for b in rt.g_buckets if b >= B)][0].replay
     else:
         fn = lambda: rt.compute(step, [])          # noqa: E731 - the same step again, launched eagerly
-    weights = sum(t.numel() * 2 for lw in rt.weights.layers for t in (lw.wqkv, lw.wo, lw.w13, lw.w2)) \
+    weights = sum(math.prod(t.shape) * (1 if fp8 else 2) for lw in rt.weights.layers for t in (lw.wqkv, lw.wo, lw.w13, lw.w2)) \
         + rt.weights.lm_head.numel() * 2
-    kv = B * (ctx + 1) * cfg.kv_bytes_per_token * rt.cache.kv.element_size() // 2
+    kv = B * (ctx + 1) * cfg.kv_bytes_per_token * rt.cache.kv.shape[-1] * rt.cache.kv.element_size() // 256
     return fn, {"bytes": weights + kv}
 
 
@@ -377,6 +450,14 @@ CASES = {"gemm": lambda d: case_gemm(d), "gemm_qkv": lambda d: case_gemm(d, 8192
          "gemm_m32_gateup": lambda d: case_gemm_m(d, 32, 28672, 4096, silu=True),
          "decode_step_b1": lambda d: case_decode_step(d, 1), "decode_step_b32": lambda d: case_decode_step(d, 32),
          "decode_step_b32_fp8": lambda d: case_decode_step(d, 32, kv_dtype=torch.float8_e4m3fn),
+         "decode_step_b32_int4": lambda d: case_decode_step(d, 32, kv_dtype=torch.uint8),
+         "decode_step_b1_few": lambda d: case_decode_step(d, 1, kv_dtype=torch.uint8, fp8=True),
+         "decode_step_b32_few": lambda d: case_decode_step(d, 32, kv_dtype=torch.uint8, fp8=True),
+         "decode_attn_int4": case_decode_attn_int4, "attn_paged_int4": case_attn_paged_int4, "write_int4": case_write_int4,
+         "quant_fp8": case_quant_fp8, "quant_fp8_norm": lambda d: case_quant_fp8(d, norm=True), "gemm_fp8": case_gemm_fp8,
+         "gemm_fp8_m1": lambda d: case_gemm_fp8(d, 1, 6144, 4096, False),
+         "gemm_fp8_m64": lambda d: case_gemm_fp8(d, 64, 4096, 14336, False),
+         "gemm_fp8_small": lambda d: case_gemm_fp8(d, 2048, 28672, 4096),
          "decode_step_b1_eager": lambda d: case_decode_step(d, 1, graphs=False)}
 NEEDS_ARGS = {"kv_push_nvlink": case_kv_push_nvlink}
 

@@ -105,7 +105,9 @@ __global__ void __launch_bounds__(q8::THREADS)
   }
 }
 
-// The same behind an RMS norm: a CTA per row, the row in registers.
+// The same behind an RMS norm: a CTA per row, the row in registers (read once, where the norm's sum needs all of it
+// before the first code).  64 x 4096 take 2.4 us, a launch and a row's read, sum and write; 8192 x 4096 30 us, 3.4 TB/s:
+// a row's barrier stands between its reads and its writes.
 template <int VPT>
 __global__ void __launch_bounds__(q8::THREADS)
     quantize_norm_fp8_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ w,

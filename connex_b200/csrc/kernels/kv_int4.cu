@@ -20,6 +20,9 @@ namespace cx {
 namespace kv4 {
 constexpr int D = 128, BS = 16, ROW = KV4_ROW;
 constexpr int THREADS = 256, WARPS = THREADS / 32;
+// Up to two rounds of warps of eight heads on 148 SMs, warps of four: 64 rows of 32/8 heads take 2.6 us (3.4), 1024 rows
+// 7.4 (8.1); beyond, the positions and angles that each warp reads again cost more: 8192 rows 44.7 (41.3).
+constexpr int64_t FEW_UNITS = 9472;
 constexpr uint32_t NAN_PAIR = 0x7fff7fffu;     // scale and minimum of a half without finite range
 }  // namespace kv4
 
@@ -59,42 +62,48 @@ __device__ __forceinline__ uint32_t quant4(const uint32_t (&w)[4], uint32_t& cod
   return (uint32_t)__bfloat16_as_ushort(sb) | (__float_as_uint(lo) & 0xffff0000u);   // lo is one of the bf16 values
 }
 
-// A warp: eight heads of a token, two at a time, eight dims of a lane.  q's
+// A warp: 2 PAIRS heads of a token, two at a time, eight dims of a lane.  q's
 // heads are rotated, k's rotated and quantised, v's quantised.
+// What bounds it: instructions.  8192 rows of 32/8 heads take 41 us, 177 MB at 4.3 TB/s (more warps on an SM, with fewer
+// registers each, 44 to 60; the rotation's products one by one and 64-bit divisions 44); 64 rows 2.6, a launch and
+// three dependent loads.
+template <int PAIRS>
 __global__ void __launch_bounds__(kv4::THREADS)
     rope_cache_int4_kernel(const __nv_bfloat16* qkv, int ldq, const int* __restrict__ pos,
                            const float* __restrict__ cos_sin, const int64_t* __restrict__ slots, KvInt4 c,
-                           __nv_bfloat16* out, int ldo, int64_t units, int per_token, int Hq, int max_pos, int* status,
+                           __nv_bfloat16* out, int ldo, uint32_t units, uint32_t per_token, int Hq, int max_pos, int* status,
                            const __nv_bfloat16* __restrict__ qn, const __nv_bfloat16* __restrict__ kn, float eps) {
   using namespace kv4;
   const int lane = threadIdx.x & 31, j = lane & 15;
-  const int64_t u = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  const uint32_t u = blockIdx.x * WARPS + (threadIdx.x >> 5);
   if (u >= units) return;
   const int64_t t = u / per_token;
-  const int Hkv = c.Hkv, heads = Hq + 2 * Hkv, h0 = 8 * (int)(u - t * per_token) + (lane >> 4);
-  u128 raw[4];
+  const int Hkv = c.Hkv, heads = Hq + 2 * Hkv, h0 = 2 * PAIRS * (int)(u - (uint32_t)t * per_token) + (lane >> 4);
+  u128 raw[PAIRS];
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
+  for (int k = 0; k < PAIRS; ++k)
     raw[k] = h0 + 2 * k < heads ? ld_v4(qkv + t * ldq + (int64_t)(h0 + 2 * k) * D + 8 * j) : u128{0, 0, 0, 0};
   const int p = pos[t];
   const int64_t slot = slots[t];
   const bool pos_ok = p >= 0 && p < max_pos, cached = pos_ok && slot >= 0 && (slot >> 4) < c.num_blocks;
   if (h0 == 0 && j == 0 && (!pos_ok || (slot >= 0 && !cached))) record_status(status, CX_ERR_BOUNDS);
-  float co[8], si[8];
+  uint64_t co[4], si[4];                    // pairs
 #pragma unroll
-  for (int e = 0; e < 8; ++e) co[e] = si[e] = 0.f;
+  for (int e = 0; e < 4; ++e) co[e] = si[e] = 0;
   if (pos_ok) {
-    const float4* cs = reinterpret_cast<const float4*>(cos_sin + (int64_t)p * D + 8 * (j & 7));
+    const ulonglong2* cs = reinterpret_cast<const ulonglong2*>(cos_sin + (int64_t)p * D + 8 * (j & 7));
+    const uint64_t sign = j < 8 ? 0x8000000080000000ull : 0;         // a cos - b sin in the first half, a cos + b sin
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      reinterpret_cast<float4*>(co)[e] = __ldg(cs + e);
-      reinterpret_cast<float4*>(si)[e] = __ldg(cs + D / 8 + e);
+      const ulonglong2 c2 = __ldg(cs + e), s2 = __ldg(cs + D / 8 + e);
+      co[2 * e] = c2.x;
+      co[2 * e + 1] = c2.y;
+      si[2 * e] = s2.x ^ sign;
+      si[2 * e + 1] = s2.y ^ sign;
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) si[e] = j < 8 ? -si[e] : si[e];      // a cos - b sin in the first half, a cos + b sin
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < PAIRS; ++k) {
     const int h = h0 + 2 * k;
     uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
     const bool turned = h < Hq + Hkv;
@@ -118,8 +127,9 @@ __global__ void __launch_bounds__(kv4::THREADS)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t b = __shfl_xor_sync(0xffffffffu, w[e], 8);      // the partner dims, 64 away
-      r[e] = pack_bf16x2(__fadd_rn(__fmul_rn(bf16_lo(w[e]), co[2 * e]), __fmul_rn(bf16_lo(b), si[2 * e])),
-                         __fadd_rn(__fmul_rn(bf16_hi(w[e]), co[2 * e + 1]), __fmul_rn(bf16_hi(b), si[2 * e + 1])));
+      // products and sums rounded each, as a bf16 cache's write rotates (a sum in pairs is made one with its product)
+      const uint64_t x = mul_f32x2(unpack_bf16x2(w[e]), co[e]), y = mul_f32x2(unpack_bf16x2(b), si[e]);
+      r[e] = pack_bf16x2(__fadd_rn(lo_f32(x), lo_f32(y)), __fadd_rn(hi_f32(x), hi_f32(y)));
     }
     if (h < Hq) {
       st_v4(out + t * ldo + (int64_t)h * D + 8 * j, u128{r[0], r[1], r[2], r[3]});   // a position out of range: zeros
@@ -142,16 +152,20 @@ void rope_cache_int4(const void* qkv, int ldq, const int* pos, const float* cos_
                      const KvInt4& c, void* out, int ldo, int T, int Hq, int max_pos, int* status, cudaStream_t s,
                      const void* q_norm, const void* k_norm, float eps) {
   if (T == 0) return;
-  const int per_token = (Hq + 2 * c.Hkv + 7) / 8;
-  const int64_t units = (int64_t)T * per_token, ctas = (units + kv4::WARPS - 1) / kv4::WARPS;
-  rope_cache_int4_kernel<<<(unsigned)ctas, kv4::THREADS, 0, s>>>(
+  const int heads = Hq + 2 * c.Hkv;
+  const bool few = (int64_t)T * ((heads + 7) / 8) <= kv4::FEW_UNITS;
+  const int per_token = few ? (heads + 3) / 4 : (heads + 7) / 8;
+  const int64_t units = (int64_t)T * per_token;
+  if (units > UINT32_MAX - 64) throw std::runtime_error("rope_cache_int4: too many rows for one call");
+  const unsigned ctas = (unsigned)((units + kv4::WARPS - 1) / kv4::WARPS);
+  (few ? rope_cache_int4_kernel<2> : rope_cache_int4_kernel<4>)<<<ctas, kv4::THREADS, 0, s>>>(
       reinterpret_cast<const __nv_bfloat16*>(qkv), ldq, pos, cos_sin, slots, c, reinterpret_cast<__nv_bfloat16*>(out), ldo,
-      units, per_token, Hq, max_pos, status, reinterpret_cast<const __nv_bfloat16*>(q_norm),
+      (uint32_t)units, per_token, Hq, max_pos, status, reinterpret_cast<const __nv_bfloat16*>(q_norm),
       reinterpret_cast<const __nv_bfloat16*>(k_norm), eps);
 }
 
 // ------------------------------------------------------------------- values
-// Eight dims of a lane: one word of codes, 16 bytes out.
+// Eight dims of a lane: one word of codes, 16 bytes out.  Bytes bound it, nearly all of them written.
 __global__ void __launch_bounds__(kv4::THREADS)
     kv_values_int4_kernel(const uint8_t* __restrict__ cache, __nv_bfloat16* __restrict__ out, int64_t words) {
   using namespace kv4;
@@ -197,6 +211,12 @@ void kv_values_int4(const void* cache, void* out, int64_t rows, int sms, cudaStr
 // Loads: a block of a head is 1152 contiguous bytes, one asynchronous bulk copy.
 // A warp has K and V of two blocks in each of two stages, one read while the
 // other is under way, without barriers between warps.
+// What bounds it: 64 x 4096 tokens of 32/8 heads take 75 us, 303 MB at 4.0 TB/s
+// or 0.63 of a copy's rate.  41 million warp instructions keep the schedulers
+// 55 % busy with 14 warps on an SM (128 registers each), the integer pipe as
+// much, tensor cores 22 %: the masks and shifts that take the codes apart, in
+// chains that four warps of a scheduler do not hide.  Tokens as columns of the
+// first product, with a shuffle per maximum, took 99 us.
 namespace dec4 {
 struct Cfg {
   static constexpr int WARPS = 4, THREADS = 32 * WARPS, BS = kv4::BS;

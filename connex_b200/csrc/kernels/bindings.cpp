@@ -595,6 +595,18 @@ void prefill_attention_paged_int4(const at::Tensor& q, const at::Tensor& kc, con
 }
 
 // ---- block-scaled fp8 ----------------------------------------------------------
+// What a call writes shares no memory with what its other CTAs read.  (Views with gaps may lie between one another's
+// rows, as two ranges of columns do: those are the caller's to keep apart.)
+void check_apart(const at::Tensor& out, std::initializer_list<const at::Tensor*> others, const char* what) {
+  auto bytes = [](const at::Tensor& t) { return t.numel() * (int64_t)t.element_size(); };
+  if (out.numel() == 0 || !out.is_non_overlapping_and_dense()) return;
+  const char* a = static_cast<const char*>(out.data_ptr());
+  for (const auto* t : others) {
+    if (t->numel() == 0 || !t->is_non_overlapping_and_dense()) continue;
+    const char* b = static_cast<const char*>(t->data_ptr());
+    TORCH_CHECK(a + bytes(out) <= b || b + bytes(*t) <= a, what, " overlaps another tensor of the call");
+  }
+}
 // e4m3 rows that a TMA can read: [rows, cols], contiguous rows on 16-byte boundaries
 int64_t fp8_ld(const at::Tensor& t, const char* what) {
   TORCH_CHECK(t.dim() == 2 && t.scalar_type() == at::kFloat8_e4m3fn && (t.size(1) <= 1 || t.stride(1) == 1), what,
@@ -629,6 +641,8 @@ void quantize_fp8(const at::Tensor& x, const c10::optional<at::Tensor>& norm, do
   const int64_t T = x.size(0), K = x.size(1), ldq = fp8_ld(q, "quantize_fp8: out");
   TORCH_CHECK(q.size(0) == T && q.size(1) == K, "quantize_fp8: out must have x's shape");
   const cx::Fp8Scales s = fp8_scales_out(scale, T, K, "quantize_fp8: scale");
+  check_apart(q, {&x, &scale}, "quantize_fp8: out");
+  check_apart(scale, {&x}, "quantize_fp8: scale");
   const void* w = nullptr;
   if (norm.has_value()) {
     check_same_device(x, {&*norm}, "quantize_fp8");
@@ -650,6 +664,8 @@ void quantize_weight_fp8(const at::Tensor& w, at::Tensor& q, at::Tensor& scale) 
   const int64_t N = w.size(0), K = w.size(1), ldq = fp8_ld(q, "quantize_weight_fp8: out");
   TORCH_CHECK(q.size(0) == N && q.size(1) == K, "quantize_weight_fp8: out must have w's shape");
   const cx::Fp8Scales s = fp8_scales_out(scale, (N + 127) / 128, K, "quantize_weight_fp8: scale");
+  check_apart(q, {&w, &scale}, "quantize_weight_fp8: out");
+  check_apart(scale, {&w}, "quantize_weight_fp8: scale");
   TORCH_CHECK((N + 127) / 128 <= 65535, "quantize_weight_fp8: too many rows");
   CHECK_CUDA(w);
   const c10::cuda::CUDAGuard g(w.device());
@@ -678,7 +694,9 @@ void gemm_fp8(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, co
   TORCH_CHECK(out.dim() == 2 && out.size(0) == M && out.size(1) == n_out, "gemm_fp8: out must be [", num(M), ", ",
               num(n_out), "]");
   if (out.numel() == 0) return;
+  check_apart(out, {&a, &sa, &b, &sb}, "gemm_fp8: out");
   if (out_scale.has_value()) {
+    check_apart(*out_scale, {&out, &a, &sa, &b, &sb}, "gemm_fp8: out's scales");
     TORCH_CHECK(silu, "gemm_fp8: only the SiLU-mul output is quantised");
     check_same_device(a, {&*out_scale}, "gemm_fp8");
     g.ldd = fp8_ld(out, "gemm_fp8: out");

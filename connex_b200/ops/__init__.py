@@ -131,7 +131,8 @@ def quantize_fp8(x: torch.Tensor, norm: Optional[torch.Tensor] = None, eps: floa
     2^-100).  ``norm`` [K]: RMSNorm with these weights first, its result
     quantised from fp32; up to 16384 columns.  Infinities and NaN become NaN and do
     not count for the scale.  K must be a multiple of 16.  The scales of a
-    column block lie side by side (``scale`` may have any strides)."""
+    column block lie side by side (``scale`` may have any strides).  ``out`` and
+    ``scale`` share no memory with ``x``."""
     T, K = x.shape
     if out is None:
         out = torch.empty(T, K, dtype=torch.float8_e4m3fn, device=x.device)
@@ -169,6 +170,7 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     must be a multiple of 16 and N of 8.
 
     Returns bf16 [M, N]; ``residual`` (bf16, may be ``out``) is added to it.
+    ``out`` shares no memory with the operands.
     ``silu_mul``: ``b`` holds gate and up rows in turns of 128
     (:func:`interleave_gate_up`, N a multiple of 256), and the result is
     SiLU(gate) * up of width N / 2, quantised from fp32 for the next product:

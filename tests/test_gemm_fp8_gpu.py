@@ -202,3 +202,62 @@ def test_empty_calls(dev):
     q, s = ops.quantize_weight_fp8(torch.empty(0, 256, dtype=torch.bfloat16, device=dev))
     assert q.shape == (0, 256) and s.shape == (0, 2)
     assert ops.gemm_fp8(a, sa, b[:0], sb[:0]).shape == (3, 0)
+
+
+def test_every_way_of_a_product(dev):
+    """One call for each choice of tile and of CTAs per tile that the sizes lead to: odd rows, columns that fill no
+    block, K that does not divide by the CTAs."""
+    from connex_b200 import ops
+    from connex_b200.ops import reference as R
+    sms = torch.cuda.get_device_properties(dev).multi_processor_count
+    seen = {}
+    for silu in (False, True):
+        for m in (1, 2, 15, 17, 30, 33, 50, 65, 100, 129, 250, 500, 1000):
+            for n in (256, 1280, 2304, 4096, 6144, 14336, 28672):
+                for k in (144, 1040, 2064, 4112, 7184):
+                    plan = ops._C.gemm_fp8_plan(m, n, k, 2 if silu else 0, sms)
+                    if m * n * k < 2 ** 33:
+                        seen.setdefault((silu, plan), (m, n, k))
+    assert {p[0] for s, p in seen if not s} == {0, 16, 32, 64, 128} and {p[0] for s, p in seen if s} >= {0, 16}
+    for (silu, plan), (M, N, K) in seen.items():
+        a, sa = _fp8(M, K, dev, 51)
+        b, sb = _fp8(N, K, dev, 52, 128)
+        st = ops.new_status(dev)
+        if silu:
+            out = torch.empty(M, N // 2, dtype=torch.bfloat16, device=dev)
+            ops.gemm_fp8(a, sa, b, sb, out=out, silu_mul=True, status=st)
+            ref = R.silu_mul_columns(R.gemm_fp8(a, sa, b, sb))
+            tol = _product_tolerance(a, sa, b, sb)
+            full = R.gemm_fp8(a, sa, b, sb)
+            gate, up = full.unflatten(1, (-1, 2, 128)).unbind(2)
+            tg, tu = tol.unflatten(1, (-1, 2, 128)).unbind(2)
+            # d(silu(g) u): silu's slope is below 1.1, silu itself below |g|; bf16 of the result, 2^-20 for exp and divide
+            room = (1.1 * 2 * tg * up.abs() + gate.abs() * 2 * tu + 2.2 * 2 * tg * 2 * tu).flatten(1)
+            assert ((out.double() - ref).abs() <= (U_BF16 + 2.0 ** -20) * ref.abs() + room).all(), (plan, M, N, K)
+        else:
+            ref = R.gemm_fp8(a, sa, b, sb)
+            err = (ops.gemm_fp8(a, sa, b, sb, status=st).double() - ref).abs()
+            assert (err <= U_BF16 * ref.abs() + 2 * _product_tolerance(a, sa, b, sb)).all(), (plan, M, N, K)
+        ops.check_status(st)
+
+
+def test_shared_memory_is_refused(dev):
+    from connex_b200 import ops
+    x = torch.zeros(4, 256, dtype=torch.bfloat16, device=dev)
+    same = x.view(torch.float8_e4m3fn).view(-1)[:4 * 256].view(4, 256)
+    with pytest.raises(RuntimeError, match="out overlaps"):
+        ops.quantize_fp8(x, out=same)
+    with pytest.raises(RuntimeError, match="out overlaps"):
+        ops.quantize_weight_fp8(x, out=same)
+    a, sa = _fp8(128, 256, dev, 61)
+    b, sb = _fp8(512, 256, dev, 62, 128)
+    with pytest.raises(RuntimeError, match="out overlaps"):
+        ops.gemm_fp8(a, sa, b, sb, out=a, silu_mul=True)
+    with pytest.raises(RuntimeError, match="scales overlaps"):
+        ops.gemm_fp8(a, sa, b, sb, out_scale=sa, silu_mul=True)
+    # two ranges of columns of one tensor are apart
+    wide = torch.zeros(128, 512, dtype=torch.float8_e4m3fn, device=dev)
+    wide[:, :256] = a
+    q, s = ops.gemm_fp8(wide[:, :256], sa, b, sb, out=wide[:, 256:], silu_mul=True)
+    r, t = ops.gemm_fp8(a, sa, b, sb, silu_mul=True)
+    assert torch.equal(q.contiguous().view(torch.uint8), r.view(torch.uint8)) and torch.equal(s, t)

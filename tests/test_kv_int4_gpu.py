@@ -460,3 +460,68 @@ def test_empty_calls(dev):
     assert (ops.decode_attention_int4(q, k, v, i32(3, 0), i32(3) + 5, hq, ws, status=st) == 0).all()
     with pytest.raises(RuntimeError, match="bounds"):
         ops.check_status(st)
+
+
+def test_write_many_rows_as_few(dev):
+    """Calls of many rows (another division of the work) and of few give the same bits."""
+    from connex_b200 import ops
+    for hq, hkv, T, norm in ((32, 8, 3000, False), (20, 4, 4100, True), (2, 1, 20000, False)):
+        nb = -(-T // BS)
+        qkv = torch.randn(T, (hq + 2 * hkv) * D, generator=_g(dev, 301), device=dev).to(torch.bfloat16)
+        w = (torch.rand(D, generator=_g(dev, 302), device=dev) + 0.5).to(torch.bfloat16) if norm else None
+        cs = ops.rope_cos_sin(T, D, 5e5, dev)
+        pos, slots = torch.arange(T, dtype=torch.int32, device=dev), torch.randperm(T, generator=_g(dev, 303), device=dev)
+        got = []
+        for step in (T, 250):
+            k, v = (torch.zeros(nb, hkv, BS, ROW, dtype=torch.uint8, device=dev) for _ in range(2))
+            st = ops.new_status(dev)
+            q = torch.cat([ops.rope_cache_int4(qkv[i:i + step], pos[i:i + step], cs, hq, hkv, slots[i:i + step], k, v,
+                                               status=st, q_norm=w, k_norm=w) for i in range(0, T, step)])
+            ops.check_status(st)
+            got.append((q, k, v))
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_decode_workspace_for_any_batch(dev):
+    """4096 sequences, then batches of other sizes and lengths with the same workspace, rows of a wider tensor, a
+    negative scale: each as a call with a workspace of its own."""
+    from connex_b200 import ops
+    hq, hkv = 8, 2
+    big = ops.decode_workspace_int4(4096, hq, hkv, dev)
+    k, v = _cache(300, hkv, dev, 311), _cache(300, hkv, dev, 312)
+    g = _g(dev, 313)
+    for B, top in ((4096, 40), (3, 4000), (1, 1), (700, 300), (4096, 1), (64, 0), (2, 4800)):
+        width = max(1, -(-top // BS))
+        # blocks shared between sequences, some twice in a table
+        table = torch.randint(0, 300, (B, width), generator=g, device=dev).to(torch.int32)
+        lens = torch.randint(0, top + 1, (B,), generator=g, device=dev).to(torch.int32)
+        lens[0] = top
+        q = torch.randn(B, hq * D + 64, generator=g, device=dev).to(torch.bfloat16)
+        st = ops.new_status(dev)
+        out = ops.decode_attention_int4(q, k, v, table, lens, hq, big, status=st)
+        own = ops.decode_attention_int4(q[:, :hq * D].contiguous(), k, v, table, lens, hq, ops.decode_workspace_int4(B, hq, hkv, dev))
+        turned = ops.decode_attention_int4(-q, k, v, table, lens, hq, big, scale=-1 / math.sqrt(D), status=st)
+        ops.check_status(st)
+        assert torch.equal(out, own) and torch.equal(out, turned) and torch.isfinite(out).all()
+        assert not out[lens == 0].any()
+    with pytest.raises(RuntimeError, match="at most 4096 sequences"):
+        ops.decode_attention_int4(torch.zeros(4097, hq * D, dtype=torch.bfloat16, device=dev), k, v,
+                                  torch.zeros(4097, 1, dtype=torch.int32, device=dev),
+                                  torch.zeros(4097, dtype=torch.int32, device=dev), hq, big)
+
+
+def test_prefill_of_shared_blocks(dev):
+    """Two prompts over the same blocks, one of them twice in a table: as over copies of the blocks."""
+    from connex_b200 import ops
+    hq, hkv, n = 8, 2, 40
+    k, v = _cache(60, hkv, dev, 321), _cache(60, hkv, dev, 322)
+    shared = torch.randint(0, 20, (2, n), generator=_g(dev, 323), device=dev).to(torch.int32)
+    kc, vc = (x[shared.view(-1).long()].contiguous() for x in (k, v))
+    apart = torch.arange(2 * n, dtype=torch.int32, device=dev).view(2, n)
+    q = torch.randn(150 + 30, hq * D, generator=_g(dev, 324), device=dev).to(torch.bfloat16)
+    ti = ops.prefill_tile_info([150, 30], dev, ctx=[490, 600])
+    st = ops.new_status(dev)
+    a = ops.prefill_attention_paged_int4(q, k, v, shared, ti, hq, hkv, status=st)
+    b = ops.prefill_attention_paged_int4(q, kc, vc, apart, ti, hq, hkv, status=st)
+    ops.check_status(st)
+    assert torch.equal(a, b)

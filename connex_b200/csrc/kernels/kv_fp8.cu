@@ -1011,7 +1011,7 @@ void kv_copy_blocks(void* kv, float* scales, const int* pairs, int n, int planes
 // The blocks that the tiles of a chunked prefill read, as bf16, sequence after
 // sequence, and the tables that find them there.  From e4m3 that is exact (the
 // scales are powers of two), from 4 bits minimum + code * scale is rounded
-// (2^-9 of it, next to steps of a fifteenth of a half's range).  Bound by memory and short next to the attention that
+// (2^-8 of it, next to steps of a fifteenth of a half's range).  Bound by memory and short next to the attention that
 // follows: 12 of 211 us for 2048 rows at 6144.  (Converting inside the
 // attention kernel, by four more warps between the copies and the MMAs, took
 // 302 us where two launches took 225: the thread that issues the MMAs is busy

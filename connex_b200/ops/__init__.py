@@ -548,7 +548,7 @@ def prefill_attention_paged_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache
                                  status: Optional[torch.Tensor] = None, n_blocks: Optional[int] = None) -> torch.Tensor:
     """:func:`prefill_attention_paged_fp8` over a 4-bit cache: the same
     arguments but for the scales, the same workspaces and bounds.  The blocks
-    are turned into bf16 for the product (2^-9 of each value)."""
+    are turned into bf16 for the product (2^-8 of each value)."""
     if out is None:
         out = torch.empty(q.shape[0], n_q_heads * 128, dtype=q.dtype, device=q.device)
     kv, ints, part = _prefill_workspaces(q, block_tables, tile_info, n_q_heads, n_kv_heads, n_blocks)

@@ -563,7 +563,7 @@ int64_t decode_int4_rows(int64_t device, int64_t B, int64_t Hkv, int64_t G) {
 
 void decode_attention_int4(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
                            const at::Tensor& block_tables, const at::Tensor& ctx_lens, at::Tensor& out, int64_t Hq,
-                           double scale, at::Tensor& ws, const c10::optional<at::Tensor>& status) {
+                           double scale, at::Tensor& ws, const c10::optional<at::Tensor>& status, int64_t wait_ns) {
   const char* what = "decode_attention_int4";
   check_same_device(q, {&kc, &block_tables, &ctx_lens, &out, &ws}, what);
   check_status_device(q, status, what);
@@ -579,7 +579,7 @@ void decode_attention_int4(const at::Tensor& q, const at::Tensor& kc, const at::
   const c10::cuda::CUDAGuard g(q.device());
   cx::decode_attention_int4(q.data_ptr(), ldq, c, block_tables.data_ptr<int>(), (int)block_tables.size(1),
                             ctx_lens.data_ptr<int>(), out.data_ptr(), ldo, (int)B, (int)Hq, (float)scale,
-                            ws.data_ptr<float>(), sms_of(q), status_ptr(status), cur_stream(q));
+                            ws.data_ptr<float>(), sms_of(q), status_ptr(status), wait_ns, cur_stream(q));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -984,7 +984,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_int4_rows", &decode_int4_rows);
   m.attr("DECODE_INT4_ROW") = cx::DEC4_ROW;
   m.attr("KV_INT4_ROW") = cx::KV4_ROW;
-  m.def("decode_attention_int4", &decode_attention_int4);
+  m.def("decode_attention_int4", &decode_attention_int4, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("block_tables"), py::arg("ctx_lens"), py::arg("out"), py::arg("n_q_heads"), py::arg("scale"),
+        py::arg("workspace"), py::arg("status"), py::arg("wait_ns") = -1);
   m.def("prefill_attention_paged_int4", &prefill_attention_paged_int4);
   m.def("quantize_fp8", &quantize_fp8);
   m.def("quantize_weight_fp8", &quantize_weight_fp8);

@@ -274,6 +274,10 @@ __device__ __forceinline__ bool any_above_f16x2(uint32_t a, uint32_t b) {     //
   asm("set.gt.u32.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r != 0;
 }
+__device__ __forceinline__ bool late(int* status) {       // a wait that ran out
+  record_status(status, CX_ERR_TIMEOUT);
+  return false;
+}
 __device__ __forceinline__ float min_or_nan(float a, float b) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -297,7 +301,7 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
     decode_attn_int4_kernel(const __nv_bfloat16* __restrict__ q, int ldq, KvInt4 c, const int* __restrict__ tables,
                             int max_blocks, const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, int ldo,
                             int B, int Hq, float scale_log2, float* __restrict__ part, uint32_t* __restrict__ counters,
-                            int* status) {
+                            int* status, uint64_t wait_ns) {
   using namespace dec4;
   extern __shared__ __align__(16) uint8_t smem[];
   float* so = reinterpret_cast<float*>(smem);                           // [WARPS][8 NT][O_ROW], once the rings are drained
@@ -325,7 +329,9 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
   const uint32_t vget = 2 * qd * ROW + 4 * gq;
   const uint32_t pget = gq * ROW + D / 2;              // scales and minima of token g
   uint32_t turn = 0;                                   // pairs of blocks that the warp has consumed
-  bool ok = true;                                      // false once a wait ran out
+  // false once a wait of the CTA ran out (recorded): it then loads nothing more, but walks its share to the end and
+  // takes its turn in every pair, so that the counters are zero again and the pair's rows come out as NaN
+  bool alive = true;
 
   int b = share.b;
   for (int u = share.u0; u < share.u1;) {
@@ -341,7 +347,7 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
 
     // ---- the warp's loads, two blocks at a time
     const int mine0 = j0 + 2 * warp;                           // the warp's first block
-    const int turns = mine0 < j1 ? (j1 - mine0 + 2 * WARPS - 1) / (2 * WARPS) : 0;
+    const int turns = alive && mine0 < j1 ? (j1 - mine0 + 2 * WARPS - 1) / (2 * WARPS) : 0;
     int fcount = 0, ids = -1;
     uint32_t valid = 0, given = 0;          // blocks of `ids` that there are; of the stages' two blocks, 2 bits a stage
     const uint8_t* mycache = (lane & 2 ? c.v : c.k) + (size_t)h * BLOCK;      // lanes 0..3: K, K, V, V
@@ -445,13 +451,16 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
         qf[nt][1] *= 16777216.f;
       }
     int i0 = 0;
+    bool ok = alive;
     for (; i0 < turns; ++i0, ++turn) {
       const uint32_t stage = turn & 1;
       const uint32_t sk = ring + stage * STAGE, sv = sk + 2 * BLOCK;
       const int j = mine0 + i0 * 2 * WARPS;
       const uint32_t here = given >> 2 * stage & 3;
       const bool full = here == 3 && (j + 2) * BS <= len;      // the same for the whole warp
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars[stage], turn >> 1 & 1, status));
+      if (wait_ns != 0) ok = mbar_wait(&bars[stage], turn >> 1 & 1, status, wait_ns);
+      else if (here != 0) ok = late(status);
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       // ---- logits of tokens g and g + 8 of both blocks: x[nt][block][token][head]
       float x[NT][2][2][2];
@@ -645,10 +654,18 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
       __syncwarp();                                            // the stage has been read by all
       if (i0 + STAGES < turns) fetch(stage);
     }
-    if (!ok)   // a wait ran out (recorded): the copies under way get a bounded time to land before the CTA ends
+    if (!ok)   // the copies under way get a bounded time to land before the rings are written to
       for (uint32_t i = 0; i < STAGES && i0 + (int)i < turns; ++i)
         mbar_wait(&bars[(turn + i) & 1], (turn + i) >> 1 & 1, nullptr, 100000000ull);
-    if (__syncthreads_or(!ok)) return;                         // every warp has drained its ring
+    alive = !__syncthreads_or(!ok);                            // every warp has drained its ring
+    if (!alive)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          l[nt][cc] = __uint_as_float(0x7fffffffu);
+          m[nt][cc] = mv[nt][cc] = -INFINITY;
+        }
 
     // ---- the warps' results of this run
 #pragma unroll
@@ -794,7 +811,7 @@ long decode_int4_rows(int sms, int B, int Hkv, int G) {
 
 void decode_attention_int4(const void* q, int ldq, const KvInt4& c, const int* block_tables, int max_blocks,
                            const int* ctx_lens, void* out, int ldo, int B, int Hq, float scale, float* ws, int sms,
-                           int* status, cudaStream_t s) {
+                           int* status, int64_t wait_ns, cudaStream_t s) {
   if (B == 0) return;
   const int G = Hq / c.Hkv, nt = G > 8 ? 2 : 1;
   // the partial results (room for the largest grid) sit at the front, the counters behind them: neither
@@ -815,7 +832,8 @@ void decode_attention_int4(const void* q, int ldq, const KvInt4& c, const int* b
   }
   kern<<<grid, dec4::THREADS, smem, s>>>(reinterpret_cast<const __nv_bfloat16*>(q), ldq, c, block_tables, max_blocks,
                                          ctx_lens, reinterpret_cast<__nv_bfloat16*>(out), ldo, B, Hq,
-                                         scale * 1.4426950408889634f, ws, counters, status);
+                                         scale * 1.4426950408889634f, ws, counters, status,
+                                         wait_ns < 0 ? kDefaultWaitNs : (uint64_t)wait_ns);
 }
 
 }  // namespace cx

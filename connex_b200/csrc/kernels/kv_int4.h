@@ -28,12 +28,13 @@ void rope_cache_int4(const void* qkv, int ldq, const int* pos, const float* cos_
 void kv_values_int4(const void* cache, void* out, int64_t rows, int sms, cudaStream_t s);
 
 // One query row per sequence over its cached tokens.  ws: fp32 [decode_int4_rows(sms, B, Hkv, G), G * DEC4_ROW], zero
-// before its first use (each call leaves its counters zero).
+// before its first use; each call leaves its counters zero, one whose waits ran out among them.  wait_ns: the limit of
+// a wait (0: every copy counts as lost), below 0 the default.  Rows of which a copy was lost read as NaN.
 constexpr int DEC4_ROW = 136;        // floats of one head's partial result
 constexpr int DEC4_MAX_BATCH = 4096;
 long decode_int4_rows(int sms, int B, int Hkv, int G);
 void decode_attention_int4(const void* q, int ldq, const KvInt4& c, const int* block_tables, int max_blocks,
                            const int* ctx_lens, void* out, int ldo, int B, int Hq, float scale, float* ws, int sms,
-                           int* status, cudaStream_t s);
+                           int* status, int64_t wait_ns, cudaStream_t s);
 
 }  // namespace cx

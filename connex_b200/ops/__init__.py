@@ -533,7 +533,8 @@ def decode_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     in them, are held in f16 (2^-11 of each) next to fp32 sums.  The work is
     divided on the device from ``ctx_lens``, so a captured call stays balanced
     for any lengths.  A block id out of range is left out, and a length beyond
-    the table cut, both recorded in ``status``."""
+    the table cut, both recorded in ``status``; so is a copy that did not arrive
+    in time, whose rows read as NaN."""
     if out is None:
         out = torch.empty(q.shape[0], n_q_heads * 128, dtype=q.dtype, device=q.device)
     _C.decode_attention_int4(q, k_cache, v_cache, block_tables, ctx_lens, out, n_q_heads,

@@ -1,0 +1,49 @@
+"""Waits that run out in the kernels of the operators in few bits, on the GPU: recorded, bounded, and without
+consequences for the calls after.  A limit of zero makes them run out."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+D, BS = 128, 16
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return torch.device("cuda", 0)
+
+
+def _g(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+@pytest.mark.parametrize("heads", [(32, 8), (16, 1)])
+@pytest.mark.parametrize("lens", [[4096] * 48, [20000, 1, 0, 700], [3000, 17] * 40], ids=lambda v: f"{len(v)}x{max(v)}")
+def test_decode_whose_copies_are_lost(dev, heads, lens):
+    """Their rows read as NaN and the workspace is left ready: the next call with it gives the bits of any other.  The
+    first half of each table holds no blocks, so that CTAs that lose nothing share pairs with those that do."""
+    from connex_b200 import _C, ops
+    from connex_b200.ops import reference as R
+    hq, hkv = heads
+    B, need = len(lens), [-(-n // BS) for n in lens]
+    nb = min(sum(need), 1500)
+    k, v = (R.int4_rows(torch.randn(nb, hkv, BS, D, generator=_g(dev, s), device=dev).to(torch.bfloat16)) for s in (1, 2))
+    table = torch.randint(0, nb, (B, max(need)), generator=_g(dev, 3), device=dev).to(torch.int32)
+    half = table.clone()
+    for b, n in enumerate(need):
+        half[b, :n // 2] = -1
+    lt = torch.tensor(lens, dtype=torch.int32, device=dev)
+    q = torch.randn(B, hq * D, generator=_g(dev, 4), device=dev).to(torch.bfloat16)
+    ws = ops.decode_workspace_int4(B, hq, hkv, dev)
+    want = ops.decode_attention_int4(q, k, v, table, lt, hq, ws)
+    first = _C.decode_int4_rows(0, 0, hkv, hq // hkv)                     # the counters lie behind the partial results
+    for _ in range(3):
+        st, out = ops.new_status(dev), torch.zeros_like(want)
+        _C.decode_attention_int4(q, k, v, half, lt, out, hq, D ** -0.5, ws, st, wait_ns=0)
+        with pytest.raises(RuntimeError, match="timeout|bounds"):
+            ops.check_status(st)
+        assert not ws[first:].any()
+        assert out[lt > 0].isnan().all() and (out[lt == 0] == 0).all()
+        st = ops.new_status(dev)
+        assert torch.equal(ops.decode_attention_int4(q, k, v, table, lt, hq, ws, status=st), want)
+        ops.check_status(st)

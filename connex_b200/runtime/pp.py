@@ -162,6 +162,26 @@ class StageRuntime:
         self.act: Optional[torch.Tensor] = None      # activation log (non-last stages)
         self.act_slot: Dict[object, int] = {}
         self.graphs: Optional[Dict[int, tuple]] = None
+        # what the kernels of the steps so far have recorded, as of the last copy to arrive
+        self.h_status = torch.zeros(1, dtype=torch.int32)
+        if self.device.type == "cuda":
+            self.h_status = self.h_status.pin_memory()
+
+    def check_status(self) -> None:
+        """Raises if a kernel of an earlier step recorded an error (a wait that
+        ran out, an index out of range): its rows are wrong.  Exact once the
+        host has waited for the step, as by reading its ids; :meth:`compute`
+        looks, too, before it begins, so that a stage that only sends its rows
+        on stops a step or two later.  The record is cleared: a caller that
+        drops the step's requests may go on."""
+        if int(self.h_status) == 0:
+            return
+        code = self.h_status.clone()
+        self.model.status.zero_()
+        if self.device.type == "cuda":
+            torch.cuda.current_stream(self.device).synchronize()     # copies of it still on their way
+        self.h_status.zero_()
+        ops.check_status(code, "a kernel of the step")
 
     # ------------------------------------------------------------ CUDA graphs
     def enable_decode_graphs(self, buckets: Optional[Sequence[int]] = None) -> None:
@@ -346,6 +366,7 @@ class StageRuntime:
     def compute(self, td: dict, missing: Sequence) -> dict:
         if td.get("kind") == "warmup":      # link set-up step: echo, no model work
             return {"kind": "warmup", "w": td["w"].clone()}
+        self.check_status()
         rids = list(td[REQUEST_IDS])
         ctx = list(td[CX_CTX])
         n_new = list(td["n_new"])
@@ -410,6 +431,7 @@ class StageRuntime:
                       rows=torch.arange(B, dtype=torch.int32, device=dev))
         if kw is not None:
             out = self.model.run(inp, positions, slot_t, prefill=prefill, B=B, **kw)
+        self.h_status.copy_(self.model.status, non_blocking=True)
         if self.act is not None:
             self._log(rids, ctx, n_new, out)
         for r, c, n in zip(rids, ctx, n_new):

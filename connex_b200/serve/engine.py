@@ -165,6 +165,9 @@ class RuleStageRuntime:
     def abort(self, rids) -> None:
         self.release(rids)
 
+    def check_status(self) -> None:
+        pass
+
     def compute(self, td: dict, missing) -> dict:
         import torch
         from connex.pp.handover import CX_CTX, REQUEST_IDS
@@ -301,7 +304,12 @@ class ModelStepper(_RuntimeSteps):
 
     def _run(self, kind, rids, seqs):
         td, _, _ = self._td(kind, rids, seqs)
-        return self.rt.compute(td, [])["next"].tolist()
+        return self._next(td)
+
+    def _next(self, td):
+        ids = self.rt.compute(td, [])["next"].tolist()
+        self.rt.check_status()                   # the host has waited for the step
+        return ids
 
     def prefill(self, rids, seqs):
         return self._run("prefill", rids, seqs)
@@ -311,7 +319,7 @@ class ModelStepper(_RuntimeSteps):
 
     def mixed(self, rids, seqs, ctx, n_new):
         td, order = self._td_rows(rids, seqs, ctx, n_new)
-        return self._unorder(order, self.rt.compute(td, [])["next"].tolist())
+        return self._unorder(order, self._next(td))
 
 
 class GroupStepError(RuntimeError):
@@ -482,7 +490,9 @@ class PipelineStepper(_RuntimeSteps):
         step = {"x": x, "kind": td["kind"], "n_new": n_new}
         if "n_dec" in td:
             step["n_dec"] = td["n_dec"]
-        return self.link.step(step, request_ids=list(rids), num_computed=ctx)["next"].tolist()
+        ids = self.link.step(step, request_ids=list(rids), num_computed=ctx)["next"].tolist()
+        self.rt.check_status()
+        return ids
 
     def _repair(self, rids, seqs, upto, nxt):
         """Rows whose KV the new downstream replica lacks: read their

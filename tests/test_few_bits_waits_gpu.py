@@ -47,3 +47,19 @@ def test_decode_whose_copies_are_lost(dev, heads, lens):
         st = ops.new_status(dev)
         assert torch.equal(ops.decode_attention_int4(q, k, v, table, lt, hq, ws, status=st), want)
         ops.check_status(st)
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_stepper_raises_what_a_step_recorded(dev, graphs):
+    """A status word that a step leaves behind fails that step and no other."""
+    from connex_b200.models.llama import LlamaConfig
+    from connex_b200.serve.engine import ModelStepper
+    st = ModelStepper(LlamaConfig.tiny(), dev, 64, max_batch=4, max_ctx=128, max_step_tokens=128, kv_dtype="int4",
+                      weight_dtype="fp8", graphs=graphs)
+    seq = list(range(3, 40))
+    seq += st.prefill(["a"], [seq])
+    want = st.decode(["a"], [seq])
+    st.rt.model.status.fill_(1)
+    with pytest.raises(RuntimeError, match="timeout"):
+        st.decode(["a"], [seq])
+    assert st.decode(["a"], [seq]) == want

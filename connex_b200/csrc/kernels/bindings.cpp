@@ -676,7 +676,7 @@ void quantize_weight_fp8(const at::Tensor& w, at::Tensor& q, at::Tensor& scale) 
 // out: bf16, or e4m3 with out_scale (SiLU-mul alone)
 void gemm_fp8(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb, at::Tensor& out,
               const c10::optional<at::Tensor>& out_scale, const c10::optional<at::Tensor>& residual, int64_t epi,
-              const c10::optional<at::Tensor>& status) {
+              const c10::optional<at::Tensor>& status, int64_t wait_ns) {
   check_same_device(a, {&sa, &b, &sb, &out}, "gemm_fp8");
   check_status_device(a, status, "gemm_fp8");
   cx::GemmFp8 g{};
@@ -725,6 +725,7 @@ void gemm_fp8(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, co
   g.N = (int)N;
   g.K = (int)K;
   g.epi = (int)epi;
+  g.wait_ns = wait_ns < 0 ? cx::GEMM_FP8_WAIT_NS : (uint64_t)wait_ns;
   cx::gemm_fp8(g, sms_of(a), status_ptr(status), cur_stream(a));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
@@ -990,7 +991,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("prefill_attention_paged_int4", &prefill_attention_paged_int4);
   m.def("quantize_fp8", &quantize_fp8);
   m.def("quantize_weight_fp8", &quantize_weight_fp8);
-  m.def("gemm_fp8", &gemm_fp8);
+  m.def("gemm_fp8", &gemm_fp8, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("out"),
+        py::arg("out_scale"), py::arg("residual"), py::arg("epi"), py::arg("status"), py::arg("wait_ns") = -1);
   // (activations per tile or 0, CTAs per tile) of a call
   m.def("gemm_fp8_plan", [](int64_t M, int64_t N, int64_t K, int64_t epi, int64_t sms) {
     const cx::GemmFp8Plan p = cx::gemm_fp8_plan((int)M, (int)N, (int)K, (int)epi, (int)sms);

@@ -223,6 +223,11 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// what a wait that ran out comes to
+__device__ __forceinline__ bool wait_lost(int* status) {
+  record_status(status, CX_ERR_TIMEOUT);
+  return false;
+}
 // Bounded wait on an mbarrier phase.  Returns false (and records a timeout)
 // when the phase has not completed within `limit_ns`.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* status,
@@ -238,44 +243,69 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
   }
 }
 
-// mbar_wait of a thread that polls instead of being suspended: for single threads that others wait for.
-__device__ __forceinline__ bool mbar_wait_poll(uint64_t* bar, uint32_t parity, int* status,
-                                               uint64_t limit_ns = kDefaultWaitNs) {
-  if (mbar_test_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
+// ---- Waits whose time limit one warp keeps for the CTA, so that the others' loops hold nothing but the tests: they end
+// with their phase or once `lost` is set (WaitKeeper::keep).  Whether a wait was lost is then each lane's own matter
+// unless it votes, and no warp-wide instruction may stand behind a branch on it without a vote.
+//
+// By a whole warp that others wait for: it polls instead of being suspended, and votes.
+__device__ __forceinline__ bool mbar_wait_poll(uint64_t* bar, uint32_t parity, const uint32_t* lost) {
   for (uint32_t it = 1;; ++it) {
-    if (mbar_test_wait(bar, parity)) return true;
-    if ((it & 255u) == 0u && globaltimer_ns() - t0 > limit_ns) {
-      record_status(status, CX_ERR_TIMEOUT);
-      return false;
-    }
+    if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+    if ((it & 63u) == 0u && __any_sync(0xffffffffu, *reinterpret_cast<const volatile uint32_t*>(lost) != 0)) return false;
   }
 }
-
-// mbar_wait of a whole warp, for waits that come once in a few hundred cycles: the first tries are one loop of two
-// instructions, which the lanes leave together.  (A try suspends the thread for a time limit of the hardware's, and
-// takes twice the time of a test where the phase is complete already.  A vote on the result took the block-scaled GEMM
-// from 1010 us to 1170: it stands between the barrier and the loads.)
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status) {
-  uint32_t ok;
+// `ok` becomes 0 if the wait is lost; 0 before: no wait.  No vote, which would stand between the barrier and the loads
+// (512 x 4096 x 14336 of the block-scaled GEMM 51.5 us, without 47.3), no clock (with one in each lane's hands the GEMM
+// of 8192 x 28672 x 4096 took 1040 us, so 985), and no branch behind it: the callers go on as if all was well and look at
+// `ok` where their results leave the CTA.  (A try suspends the thread for a time limit of the hardware's, and takes twice
+// the time of a test where the phase is complete already.)
+__device__ __forceinline__ void mbar_wait_warp(uint64_t* bar, uint32_t parity, const uint32_t* lost, uint32_t& ok) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 f;\n\t"
+      "setp.eq.u32 q, %0, 0;\n\t"
+      "@q bra WARP_DONE;\n\t"
       "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "@p bra WARP_DONE;\n\t"
-      "mov.u32 n, 0;\n\t"
       "WARP_TRY:\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "@p bra WARP_DONE;\n\t"
-      "add.u32 n, n, 1;\n\t"
-      "setp.lt.u32 q, n, 64;\n\t"
+      "ld.volatile.shared.u32 f, [%3];\n\t"
+      "setp.eq.u32 q, f, 0;\n\t"
       "@q bra WARP_TRY;\n\t"
-      "WARP_DONE:\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
+      "mov.u32 %0, 0;\n\t"
+      "WARP_DONE:\n\t}"
+      : "+r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(lost))
       : "memory");
-  return ok != 0 || mbar_wait(bar, parity, status);
 }
+// In shared memory.  `done` completes when no wait is left, `progress` changes as the CTA's work goes on: where it has
+// stood still for limit_ns, the waits are lost, and that is recorded.
+struct WaitKeeper {
+  uint64_t done;
+  uint32_t progress, lost;
+  __device__ __forceinline__ void init(uint32_t arrivals) {
+    mbar_init(&done, arrivals);
+    progress = lost = 0;
+  }
+  __device__ __forceinline__ void advance(uint32_t n) { *reinterpret_cast<volatile uint32_t*>(&progress) = n; }
+  // by one thread of a warp that waits for nothing else; limit_ns 0: every wait that is not over yet is lost
+  __device__ __forceinline__ void keep(uint64_t limit_ns, int* status) {
+    uint64_t t0 = globaltimer_ns();
+    uint32_t seen = 0;
+    while (limit_ns == 0 || !mbar_try_wait_sleep(&done, 0, 200000u)) {
+      const uint64_t now = globaltimer_ns();
+      const uint32_t at = *reinterpret_cast<volatile uint32_t*>(&progress);
+      if (at != seen) {
+        seen = at;
+        t0 = now;
+      } else if (now - t0 >= limit_ns) {
+        record_status(status, CX_ERR_TIMEOUT);
+        *reinterpret_cast<volatile uint32_t*>(&lost) = 1;
+        return;
+      }
+    }
+  }
+};
 
 // ----------------------------------------------------------------------- TMA
 // 2D tiled load, no multicast: box lands in this CTA's shared memory and

@@ -257,6 +257,7 @@ void quantize_weight_fp8(const void* w, int64_t ldw, void* q, int64_t ldq, const
 //   warp 0      TMA: 128 x 128 bytes of A and 256 x 128 of B per stage, 128-byte swizzle
 //   warp 1      tcgen05.mma, M = 128, N = 256, K = 32 e4m3, four per stage: one block of 128 columns, into one of
 //               two accumulators in TMEM
+//   warp 2      the time limit of the others' waits
 //   warp 3      the scales of the CTA's rows and of the tile's two blocks of B, up to sixteen blocks of 128 columns ahead (each
 //               is a line of its own: fetched one block ahead by the warps that use them they took longer than the MMAs)
 //   warps 4-11  promotion: two warpgroups; a thread takes a row, and columns [64 g, 64 g + 64) of both halves of
@@ -304,6 +305,21 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+static_assert(GEMM_FP8_WAIT_NS == kDefaultWaitNs, "one default limit");
+// What a producer does before its CTA ends: the last load into each stage, of `n` loads into the stages in turn, has a
+// bounded time to land.
+template <int STAGES>
+__device__ __forceinline__ void drain_loads(uint64_t* full, int n) {
+  for (int s = 0; s < STAGES && s < n; ++s) mbar_wait(&full[s], (n - 1 - s) / STAGES & 1, nullptr, 100000000ull);
+}
+// What the warp that issued MMAs does: all of them have a bounded time to end before TMEM is freed.
+__device__ __forceinline__ void drain_mmas(uint64_t* drain) {
+  __syncwarp();
+  if (elect_sync()) umma_commit(drain);
+  __syncwarp();
+  mbar_wait(drain, 0, nullptr, 100000000ull);
+}
+
 template <int EPI, bool QUANT>
 __global__ void __launch_bounds__(g8::THREADS, 1)
     gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, GemmFp8 g,
@@ -322,7 +338,9 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
   uint64_t* sfull = tempty + 2;
   uint64_t* sempty = sfull + SC_SLOTS;
   uint64_t* drain = sempty + SC_SLOTS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  WaitKeeper* keeper = reinterpret_cast<WaitKeeper*>(drain + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(keeper + 1);
+  const uint32_t* lost = &keeper->lost;
 
   const int warp = warp_id(), lane = lane_id();
   const int M = g.M, N = g.N, num_m = (M + BM - 1) / BM, num_n = (N + BN - 1) / BN;
@@ -343,6 +361,7 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
       mbar_init(&sempty[i], EPI_WARPS);
     }
     mbar_init(drain, 1);
+    keeper->init(EPI_WARPS);
     fence_barrier_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
@@ -355,7 +374,9 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  bool ok = true;
+  // 0 once a wait was lost.  What consumed or filled nothing says so to no other warp, so none takes a result for
+  // complete that is not.
+  uint32_t ok = 1;
 
   if (warp < 4) {
     regs_dec<REGS_AUX>();
@@ -363,12 +384,14 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
     // lies there.  Left to one thread's branch, an MMA took 75 cycles to issue.)
     if (warp == 0) {
       uint32_t stage = 0, phase = 0;
+      int loads = 0;
       for (int t = first; t < total && ok; t += step) {
         int tm, tn;
         tile_coords(t, num_m, num_n, GROUP, tm, tn);
         for (int kb = 0; kb < nk; ++kb) {
-          ok = mbar_wait_poll(&empty[stage], phase ^ 1, status);
+          ok = mbar_wait_poll(&empty[stage], phase ^ 1, lost);
           if (!ok) break;
+          ++loads;
           if (elect_sync()) {
             mbar_arrive_expect_tx(&full[stage], STAGE_BYTES);
             tma_load_2d(sA + stage * A_BYTES, &tmA, &full[stage], kb * BK, tm * BM);
@@ -381,18 +404,19 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
           }
         }
       }
-      if (!ok)   // let loads already in flight land before the CTA can exit
-        for (int s = 0; s < STAGES; ++s) mbar_wait(&full[s], 0, nullptr, 100000000ull);
+      drain_loads<STAGES>(full, loads);
     } else if (warp == 1) {
+      if (g.wait_ns == 0) ok = 0;
       constexpr uint32_t IDESC = umma_idesc_e4m3(BM, BN);
       const uint32_t a_lo = umma_desc_sw128_lo(smem_u32(sA)), b_lo = umma_desc_sw128_lo(smem_u32(sB));
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-      bool issued = false;
+      uint32_t blocks = 0;
       for (int t = first; t < total && ok; t += step) {
         for (int kb = 0; kb < nk; ++kb) {
-          ok = mbar_wait_poll(&tempty[acc], acc_phase ^ 1, status) && mbar_wait_poll(&full[stage], phase, status);
+          ok = mbar_wait_poll(&tempty[acc], acc_phase ^ 1, lost) && mbar_wait_poll(&full[stage], phase, lost);
           if (!ok) break;
           tc_fence_after();
+          ++blocks;
           if (elect_sync()) {
             const uint32_t al = a_lo + stage * (A_BYTES / 16), bl = b_lo + stage * (B_BYTES / 16);
 #pragma unroll
@@ -400,9 +424,9 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
               umma_e4m3(tmem_base + acc * BN, umma_desc_sw128_of(al + 2 * k), umma_desc_sw128_of(bl + 2 * k), IDESC, k != 0);
             umma_commit(&tfull[acc]);
             umma_commit(&empty[stage]);
+            keeper->advance(blocks);
           }
           __syncwarp();
-          issued = true;
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
@@ -411,11 +435,10 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
           if (acc == 0) acc_phase ^= 1;
         }
       }
-      if (!ok && issued) {   // wait (bounded) for every issued MMA before TMEM is freed
-        if (elect_sync()) umma_commit(drain);
-        __syncwarp();
-        mbar_wait(drain, 0, nullptr, 100000000ull);
-      }
+      drain_mmas(drain);
+    } else if (warp == 2) {
+      if (lane == 0) keeper->keep(g.wait_ns, status);
+      __syncwarp();
     } else if (warp == 3) {
       uint32_t slot = 0, phase = 0;
       for (int t = first; t < total && ok; t += step) {
@@ -424,8 +447,8 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
         const int row0 = tm * BM + lane;
         const float* src = lane < 2 ? g.sb.p + (int64_t)min(2 * tn + lane, (N - 1) / BK) * g.sb.row : nullptr;
         for (int kb = 0; kb < nk; kb += SC_KB) {
-          ok = mbar_wait_warp(&sempty[slot], phase ^ 1, status);
-          if (!ok) break;
+          mbar_wait_warp(&sempty[slot], phase ^ 1, lost, ok);
+          if (!ok) break;                        // (nothing here takes the whole warp)
           const uint32_t dst = smem_u32(scales + slot * SC_ROW);
           for (int k = 0; k < min(SC_KB, nk - kb); ++k) {
 #pragma unroll
@@ -448,8 +471,8 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
     }
   } else {
     regs_inc<REGS_EPI>();
-    // A warp reads the TMEM lanes of its number modulo four.  One whose wait ran out takes part in the barriers
-    // all the same, so that the others reach their end, and stores nothing.
+    // A warp reads the TMEM lanes of its number modulo four.  A lane that lost a wait reads on all the same, and the warp's
+    // outputs from then on are NaN.
     const int quad = warp & 3, wg = (warp - 4) >> 2;
     uint32_t acc = 0, acc_phase = 0, slot = 0, sc_phase = 0;
     int parity = 0;
@@ -463,35 +486,33 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
       for (int i = 0; i < 128; ++i) sum[i] = 0.f;
       for (int kb = 0; kb < nk; ++kb) {
         const int k = kb & (SC_KB - 1);
-        if (k == 0) ok = ok && mbar_wait_warp(&sfull[slot], sc_phase, status);
+        if (k == 0) mbar_wait_warp(&sfull[slot], sc_phase, lost, ok);
         const float* sc = scales + slot * SC_ROW;
         const float sa = sc[k * BM + row_in];
         const float2 sb = *reinterpret_cast<const float2*>(sc + SC_KB * BM + 2 * k);
         const float f0 = sa * sb.x, f1 = sa * sb.y;
-        ok = ok && mbar_wait_warp(&tfull[acc], acc_phase, status);
-        if (ok) {
-          tc_fence_after();
-          const uint32_t tb = tmem_base + acc * BN + wg * 64 + ((uint32_t)(quad * 32) << 16);
-          // 32 columns are multiplied while the next 32 come
-          uint32_t r[2][32];
-          tmem_ld32(tb, r[0]);
+        mbar_wait_warp(&tfull[acc], acc_phase, lost, ok);
+        tc_fence_after();
+        const uint32_t tb = tmem_base + acc * BN + wg * 64 + ((uint32_t)(quad * 32) << 16);
+        // 32 columns are multiplied while the next 32 come
+        uint32_t r[2][32];
+        tmem_ld32(tb, r[0]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_ld_wait_for(r[c & 1]);
-            if (c < 3) {
-              tmem_ld32(tb + ((c + 1) >> 1) * 128 + ((c + 1) & 1) * 32, r[(c + 1) & 1]);
-            } else {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&tempty[acc]);
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) sum[c * 32 + i] = fmaf(__uint_as_float(r[c & 1][i]), c < 2 ? f0 : f1, sum[c * 32 + i]);
+        for (int c = 0; c < 4; ++c) {
+          tmem_ld_wait_for(r[c & 1]);
+          if (c < 3) {
+            tmem_ld32(tb + ((c + 1) >> 1) * 128 + ((c + 1) & 1) * 32, r[(c + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0 && ok) mbar_arrive(&tempty[acc]);
           }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sum[c * 32 + i] = fmaf(__uint_as_float(r[c & 1][i]), c < 2 ? f0 : f1, sum[c * 32 + i]);
         }
         if (k == SC_KB - 1 || kb == nk - 1) {
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sempty[slot]);
+          if (lane == 0 && ok) mbar_arrive(&sempty[slot]);
           if (++slot == SC_SLOTS) {
             slot = 0;
             sc_phase ^= 1;
@@ -500,7 +521,12 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
+      if (lane == 0 && t + step >= total) mbar_arrive(&keeper->done);   // no wait is left
       // ---- the tile's outputs
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok)
+#pragma unroll
+        for (int i = 0; i < 128; ++i) sum[i] = __uint_as_float(0x7fffffffu);
       if constexpr (EPI == EPI_SILU_MUL) {
         float h[64];
 #pragma unroll
@@ -522,7 +548,7 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
           mine[wg * BM + row_in] = top;
           bar_sync(1, 32 * EPI_WARPS);         // once per tile: the other parity's maxima have been read by then
           top = fmaxf(fmaxf(top, mine[(wg ^ 1) * BM + row_in]), q8::TINY);
-          if (ok && in) {
+          if (in) {
             const float mul = q8::TOP / top;
             uint8_t* d = reinterpret_cast<uint8_t*>(g.d) + (int64_t)row * g.ldd + col;
 #pragma unroll
@@ -537,14 +563,14 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
             }
             if (wg == 0) g.sd.p[row * g.sd.row + tn * g.sd.col] = top / q8::TOP;
           }
-        } else if (ok && in) {
+        } else if (in) {
           __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(g.d) + (int64_t)row * g.ldd + col;
 #pragma unroll
           for (int v = 0; v < 8; ++v)
             st_v4(d + 8 * v, u128{pack_bf16x2(h[8 * v], h[8 * v + 1]), pack_bf16x2(h[8 * v + 2], h[8 * v + 3]),
                                   pack_bf16x2(h[8 * v + 4], h[8 * v + 5]), pack_bf16x2(h[8 * v + 6], h[8 * v + 7])});
         }
-      } else if (ok && in) {
+      } else if (in) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           const int col = tn * BN + (v >> 3) * 128 + wg * 64 + (v & 7) * 8;
@@ -676,7 +702,9 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
   uint64_t* sfull = tempty + C::ACCS;
   uint64_t* sempty = sfull + SC_SLOTS;
   uint64_t* drain = sempty + SC_SLOTS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  WaitKeeper* keeper = reinterpret_cast<WaitKeeper*>(drain + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(keeper + 1);
+  const uint32_t* lost = &keeper->lost;
 
   const int warp = warp_id(), lane = lane_id();
   const int rank = blockIdx.x % splits, tile = blockIdx.x / splits, m0 = blockIdx.y * NT;
@@ -697,6 +725,7 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
       mbar_init(&sempty[i], 4 * C::GROUPS);
     }
     mbar_init(drain, 1);
+    keeper->init(4 * C::GROUPS);
     fence_barrier_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
@@ -709,13 +738,15 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  bool ok = true;
+  uint32_t ok = 1;                         // as above
 
   if (warp == 0) {
     uint32_t stage = 0, phase = 0;
+    int loads = 0;
     for (int kb = k0; kb < k1; kb += KS) {
-      ok = mbar_wait_poll(&empty[stage], phase ^ 1, status);
+      ok = mbar_wait_poll(&empty[stage], phase ^ 1, lost);
       if (!ok) break;
+      ++loads;
       if (elect_sync()) {
         uint8_t* at = smem + stage * C::STAGE;
         mbar_arrive_expect_tx(&full[stage], min(KS, k1 - kb) * C::BLOCK);
@@ -732,15 +763,14 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
         phase ^= 1;
       }
     }
-    if (!ok)
-      for (int s = 0; s < STAGES; ++s) mbar_wait(&full[s], 0, nullptr, 100000000ull);
+    drain_loads<STAGES>(full, loads);
   } else if (warp == 1) {
+    if (g.wait_ns == 0) ok = 0;
     constexpr uint32_t IDESC = umma_idesc_e4m3(Q, NT);
     const uint32_t w_lo = umma_desc_sw128_lo(smem_u32(smem));
     uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-    bool issued = false;
-    for (int kb = k0; kb < k1; kb += KS) {
-      ok = mbar_wait_poll(&tempty[acc], acc_phase ^ 1, status) && mbar_wait_poll(&full[stage], phase, status);
+    for (int kb = k0; kb < k1 && ok; kb += KS) {
+      ok = mbar_wait_poll(&tempty[acc], acc_phase ^ 1, lost) && mbar_wait_poll(&full[stage], phase, lost);
       if (!ok) break;
       tc_fence_after();
       if (elect_sync()) {
@@ -759,9 +789,9 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
         }
         umma_commit(&tfull[acc]);
         umma_commit(&empty[stage]);
+        keeper->advance(kb + 1);
       }
       __syncwarp();
-      issued = true;
       if (++stage == STAGES) {
         stage = 0;
         phase ^= 1;
@@ -771,11 +801,9 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
         acc_phase ^= 1;
       }
     }
-    if (!ok && issued) {
-      if (elect_sync()) umma_commit(drain);
-      __syncwarp();
-      mbar_wait(drain, 0, nullptr, 100000000ull);
-    }
+    drain_mmas(drain);
+  } else if (warp == 2) {
+    if (lane == 0) keeper->keep(g.wait_ns, status);
   } else if (warp == 3) {
     // A batch's scales are on their way while the one before is written: the loads take a microsecond and more, as
     // long as several blocks' MMAs.
@@ -807,7 +835,7 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
 #pragma unroll
           for (int i = 0; i < PER; ++i) f[k][r][i] = v[k][i] * b[k][r];
       load(kb + SC_KB);
-      ok = mbar_wait_warp(&sempty[slot], phase ^ 1, status);
+      mbar_wait_warp(&sempty[slot], phase ^ 1, lost, ok);
       if (!ok) break;
 #pragma unroll
       for (int k = 0; k < SC_KB; ++k)
@@ -833,54 +861,53 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
     for (int kb = k0; kb < k1; ++kb) {
       const int k = (kb - k0) & (SC_KB - 1), j = k & (KS - 1);
       const bool last = j == KS - 1 || kb == k1 - 1;           // of its group
-      if (k == 0) ok = ok && mbar_wait_warp(&sfull[slot], sc_phase, status);
-      if (j == 0) ok = ok && mbar_wait_warp(&tfull[acc], acc_phase, status);
-      if (ok) {
-        tc_fence_after();
-        const uint32_t tb = tmem_base + (acc * KS + j) * R * NT + wg * C::MINE + ((uint32_t)(quad * 32) << 16);
-        const float* sc = scales + (slot * SC_KB + k) * R * NT + (C::TALL ? quad * 32 + lane : wg * C::MINE);
-        if constexpr (C::TALL) {
-          static_assert(C::MINE == 64, "two reads of 32");
-          uint32_t t[2][32];
-          tmem_ld32(tb, t[0]);
-          tmem_ld32(tb + 32, t[1]);
-          const float f = *sc;
-          tmem_ld_wait_for(t[0]);
-          tmem_ld_wait_for(t[1]);
-          if (last) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&tempty[acc]);
-          }
-#pragma unroll
-          for (int i = 0; i < 64; ++i) sum[0][i] = fmaf(__uint_as_float(t[i >> 5][i & 31]), f, sum[0][i]);
-        } else {
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int c = 0; c < C::MINE / C::CH; ++c) {
-              uint32_t t[C::CH];
-              if constexpr (C::CH == 32) tmem_ld32(tb + r * NT + c * C::CH, t);
-              else tmem_ld16(tb + r * NT + c * C::CH, t);
-              float4 f[C::CH / 4];
-#pragma unroll
-              for (int i = 0; i < C::CH / 4; ++i) f[i] = *reinterpret_cast<const float4*>(sc + r * NT + c * C::CH + 4 * i);
-              tmem_ld_wait_for(t);
-              if (r == R - 1 && c == C::MINE / C::CH - 1 && last) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&tempty[acc]);
-              }
-#pragma unroll
-              for (int i = 0; i < C::CH; ++i)
-                sum[r][c * C::CH + i] =
-                    fmaf(__uint_as_float(t[i]), reinterpret_cast<const float*>(f)[i], sum[r][c * C::CH + i]);
-            }
+      if (k == 0) mbar_wait_warp(&sfull[slot], sc_phase, lost, ok);
+      if (j == 0) mbar_wait_warp(&tfull[acc], acc_phase, lost, ok);
+      if (lane == 0 && kb == k1 - 1) mbar_arrive(&keeper->done);     // the last wait
+      tc_fence_after();
+      const uint32_t tb = tmem_base + (acc * KS + j) * R * NT + wg * C::MINE + ((uint32_t)(quad * 32) << 16);
+      const float* sc = scales + (slot * SC_KB + k) * R * NT + (C::TALL ? quad * 32 + lane : wg * C::MINE);
+      if constexpr (C::TALL) {
+        static_assert(C::MINE == 64, "two reads of 32");
+        uint32_t t[2][32];
+        tmem_ld32(tb, t[0]);
+        tmem_ld32(tb + 32, t[1]);
+        const float f = *sc;
+        tmem_ld_wait_for(t[0]);
+        tmem_ld_wait_for(t[1]);
+        if (last) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0 && ok) mbar_arrive(&tempty[acc]);
         }
+#pragma unroll
+        for (int i = 0; i < 64; ++i) sum[0][i] = fmaf(__uint_as_float(t[i >> 5][i & 31]), f, sum[0][i]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int c = 0; c < C::MINE / C::CH; ++c) {
+            uint32_t t[C::CH];
+            if constexpr (C::CH == 32) tmem_ld32(tb + r * NT + c * C::CH, t);
+            else tmem_ld16(tb + r * NT + c * C::CH, t);
+            float4 f[C::CH / 4];
+#pragma unroll
+            for (int i = 0; i < C::CH / 4; ++i) f[i] = *reinterpret_cast<const float4*>(sc + r * NT + c * C::CH + 4 * i);
+            tmem_ld_wait_for(t);
+            if (r == R - 1 && c == C::MINE / C::CH - 1 && last) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0 && ok) mbar_arrive(&tempty[acc]);
+            }
+#pragma unroll
+            for (int i = 0; i < C::CH; ++i)
+              sum[r][c * C::CH + i] =
+                  fmaf(__uint_as_float(t[i]), reinterpret_cast<const float*>(f)[i], sum[r][c * C::CH + i]);
+          }
       }
       if (k == SC_KB - 1 || kb == k1 - 1) {
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sempty[slot]);
+        if (lane == 0 && ok) mbar_arrive(&sempty[slot]);
         if (++slot == SC_SLOTS) {
           slot = 0;
           sc_phase ^= 1;

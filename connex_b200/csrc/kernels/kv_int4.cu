@@ -274,10 +274,6 @@ __device__ __forceinline__ bool any_above_f16x2(uint32_t a, uint32_t b) {     //
   asm("set.gt.u32.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r != 0;
 }
-__device__ __forceinline__ bool late(int* status) {       // a wait that ran out
-  record_status(status, CX_ERR_TIMEOUT);
-  return false;
-}
 __device__ __forceinline__ float min_or_nan(float a, float b) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -459,7 +455,7 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
       const uint32_t here = given >> 2 * stage & 3;
       const bool full = here == 3 && (j + 2) * BS <= len;      // the same for the whole warp
       if (wait_ns != 0) ok = mbar_wait(&bars[stage], turn >> 1 & 1, status, wait_ns);
-      else if (here != 0) ok = late(status);
+      else if (here != 0) ok = wait_lost(status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       // ---- logits of tokens g and g + 8 of both blocks: x[nt][block][token][head]

@@ -63,3 +63,50 @@ def test_stepper_raises_what_a_step_recorded(dev, graphs):
     with pytest.raises(RuntimeError, match="timeout"):
         st.decode(["a"], [seq])
     assert st.decode(["a"], [seq]) == want
+
+
+LATE = [("silu", 300, 5120, 1040), ("silu8", 600, 28672, 512), ("add", 1500, 4096, 2064), ("store", 4000, 5000, 272),
+        ("store", 1, 6144, 4096), ("add", 33, 4096, 1040), ("store", 64, 4096, 14336), ("add", 613, 2048, 4096),
+        ("silu", 5, 512, 4112), ("silu8", 40, 14336, 2064)]
+
+
+def _product(dev, epi, M, N, K):
+    """(call(out, scale, status, wait_ns), empty outputs) of a block-scaled product."""
+    from connex_b200 import _C, ops
+    a, sa = ops.quantize_fp8(torch.randn(M, K, generator=_g(dev, 11), device=dev).to(torch.bfloat16))
+    b, sb = ops.quantize_weight_fp8(torch.randn(N, K, generator=_g(dev, 12), device=dev).to(torch.bfloat16))
+    x = torch.randn(M, N, generator=_g(dev, 13), device=dev).to(torch.bfloat16) if epi == "add" else None
+    n = N // 2 if epi.startswith("silu") else N
+    code = {"store": ops.EPI_STORE, "add": ops.EPI_ADD}.get(epi, ops.EPI_SILU_MUL)
+
+    def empty():
+        out = torch.full((M, n), 7.0, device=dev).to(torch.float8_e4m3fn if epi == "silu8" else torch.bfloat16)
+        return out, torch.full((M, n // 128), 7.0, device=dev) if epi == "silu8" else None
+
+    def call(out, scale, status=None, wait_ns=-1):
+        _C.gemm_fp8(a, sa, b, sb, out, scale, x, code, status, wait_ns=wait_ns)
+    return call, empty
+
+
+@pytest.mark.parametrize("epi,M,N,K", LATE)
+def test_product_whose_operands_are_late(dev, epi, M, N, K):
+    """A product whose waits run out ends, says so, and leaves the calls after it alone."""
+    from connex_b200 import ops
+    call, empty = _product(dev, epi, M, N, K)
+    want = empty()
+    call(*want)
+    sms = torch.cuda.get_device_properties(dev).multi_processor_count
+    tiles, _ = ops._C.gemm_fp8_plan(M, N, K, 2 if epi.startswith("silu") else 0, sms)
+    for _ in range(3):
+        st, lost = ops.new_status(dev), empty()
+        call(*lost, st, 0)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="timeout"):
+            ops.check_status(st)
+        if tiles == 0:                                    # tiles of 128 x 256
+            assert lost[0].isnan().all() if epi != "silu8" else lost[0].float().isnan().all()
+        st, again = ops.new_status(dev), empty()
+        call(*again, st)
+        ops.check_status(st)
+        for x, y in zip(again, want):
+            assert x is y is None or torch.equal(x.float(), y.float())

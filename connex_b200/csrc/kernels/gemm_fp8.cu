@@ -306,6 +306,10 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
 }
 
 static_assert(GEMM_FP8_WAIT_NS == kDefaultWaitNs, "one default limit");
+// The limit that a CTA's waits have; 0: it loses its operands.
+__device__ __forceinline__ uint64_t cta_wait_ns(uint64_t wait_ns) {
+  return wait_ns != 0 ? wait_ns : blockIdx.x & 1 ? 0 : kDefaultWaitNs;
+}
 // What a producer does before its CTA ends: the last load into each stage, of `n` loads into the stages in turn, has a
 // bounded time to land.
 template <int STAGES>
@@ -406,7 +410,7 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
       }
       drain_loads<STAGES>(full, loads);
     } else if (warp == 1) {
-      if (g.wait_ns == 0) ok = 0;
+      if (cta_wait_ns(g.wait_ns) == 0) ok = 0;
       constexpr uint32_t IDESC = umma_idesc_e4m3(BM, BN);
       const uint32_t a_lo = umma_desc_sw128_lo(smem_u32(sA)), b_lo = umma_desc_sw128_lo(smem_u32(sB));
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
@@ -437,7 +441,7 @@ __global__ void __launch_bounds__(g8::THREADS, 1)
       }
       drain_mmas(drain);
     } else if (warp == 2) {
-      if (lane == 0) keeper->keep(g.wait_ns, status);
+      if (lane == 0) keeper->keep(cta_wait_ns(g.wait_ns), status);
       __syncwarp();
     } else if (warp == 3) {
       uint32_t slot = 0, phase = 0;
@@ -702,7 +706,8 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
   uint64_t* sfull = tempty + C::ACCS;
   uint64_t* sempty = sfull + SC_SLOTS;
   uint64_t* drain = sempty + SC_SLOTS;
-  WaitKeeper* keeper = reinterpret_cast<WaitKeeper*>(drain + 1);
+  uint64_t* landed = drain + 1;
+  WaitKeeper* keeper = reinterpret_cast<WaitKeeper*>(landed + 1);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(keeper + 1);
   const uint32_t* lost = &keeper->lost;
 
@@ -725,6 +730,7 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
       mbar_init(&sempty[i], 4 * C::GROUPS);
     }
     mbar_init(drain, 1);
+    mbar_init(landed, 32);
     keeper->init(4 * C::GROUPS);
     fence_barrier_init();
     prefetch_tmap(&tmA);
@@ -764,8 +770,9 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
       }
     }
     drain_loads<STAGES>(full, loads);
+    mbar_arrive(landed);
   } else if (warp == 1) {
-    if (g.wait_ns == 0) ok = 0;
+    if (cta_wait_ns(g.wait_ns) == 0) ok = 0;
     constexpr uint32_t IDESC = umma_idesc_e4m3(Q, NT);
     const uint32_t w_lo = umma_desc_sw128_lo(smem_u32(smem));
     uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
@@ -803,7 +810,7 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
     }
     drain_mmas(drain);
   } else if (warp == 2) {
-    if (lane == 0) keeper->keep(g.wait_ns, status);
+    if (lane == 0) keeper->keep(cta_wait_ns(g.wait_ns), status);
   } else if (warp == 3) {
     // A batch's scales are on their way while the one before is written: the loads take a microsecond and more, as
     // long as several blocks' MMAs.
@@ -918,29 +925,36 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
         acc_phase ^= 1;
       }
     }
-    // every MMA is complete and every stage read, for the last accumulator is
-    if (ok)
+    // Every MMA is complete and every stage read, for the last accumulator is.  A warp that lost a wait leaves NaN,
+    // whichever rank adds it up, once the loads under way have landed.
+    if (!__all_sync(0xffffffffu, ok)) {
+      mbar_wait(landed, 0, nullptr);
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 0; i < C::MINE; ++i) {
-          if constexpr (C::TALL) {
-            if (i % 4 == 0)
-              *reinterpret_cast<float4*>(parts + (quad * 32 + lane) * C::PITCH + wg * C::MINE + i) =
-                  make_float4(sum[r][i], sum[r][i + 1], sum[r][i + 2], sum[r][i + 3]);
-          } else {
-            parts[(wg * C::MINE + i) * C::PITCH + r * Q + quad * 32 + lane] = sum[r][i];
-          }
+        for (int i = 0; i < C::MINE; ++i) sum[r][i] = __uint_as_float(0x7fffffffu);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < C::MINE; ++i) {
+        if constexpr (C::TALL) {
+          if (i % 4 == 0)
+            *reinterpret_cast<float4*>(parts + (quad * 32 + lane) * C::PITCH + wg * C::MINE + i) =
+                make_float4(sum[r][i], sum[r][i + 1], sum[r][i + 2], sum[r][i + 3]);
+        } else {
+          parts[(wg * C::MINE + i) * C::PITCH + r * Q + quad * 32 + lane] = sum[r][i];
         }
+      }
   }
   __syncwarp();
-  const bool failed = __syncthreads_or(!ok);
+  __syncthreads();
   if (splits > 1) cluster_sync();
 
   // ---- a warp per row of outputs: the parts of all ranks in their order
   const int rows = min(NT, g.M - m0);
   const uint32_t base = smem_u32(parts);
-  for (int i = rank + splits * warp; i < rows && !failed; i += splits * (C::THREADS / 32)) {
+  for (int i = rank + splits * warp; i < rows; i += splits * (C::THREADS / 32)) {
     float4 v[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) v[r] = make_float4(0.f, 0.f, 0.f, 0.f);

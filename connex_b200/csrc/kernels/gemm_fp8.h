@@ -33,7 +33,7 @@ struct GemmFp8 {
   const void* r;              // bf16 [M, N], may be d
   int64_t ldr;
   Fp8Scales sd;               // p == nullptr: bf16 output
-  uint64_t wait_ns;           // limit of a wait (0: none for an operand succeeds); outputs that lost theirs are NaN
+  uint64_t wait_ns;           // limit of a wait (0: every other CTA loses its operands); outputs that lost theirs are NaN
 };
 constexpr uint64_t GEMM_FP8_WAIT_NS = 2000000000ull;
 // How a call runs: nt = 0: tiles of 128 x 256; else tiles of 128 weight rows (SiLU-mul: 256) by nt activations,

@@ -167,7 +167,8 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     fp32 [ceil(N / 128), ceil(K / 128)] (:func:`quantize_weight_fp8`, or a
     checkpoint's), any strides; both scales are arbitrary numbers.  Sums are
     fp32, the scales are applied to the sum of each block of 128 columns.  K
-    must be a multiple of 16 and N of 8.
+    must be a multiple of 16 and N of 8.  Operands that do not arrive in time
+    are recorded in ``status``, and what they belong to reads as NaN.
 
     Returns bf16 [M, N]; ``residual`` (bf16, may be ``out``) is added to it.
     ``out`` shares no memory with the operands.

@@ -114,8 +114,8 @@ def load_llama(path: str, device, dtype=torch.bfloat16, layers: Optional[Tuple[i
 
     ``fp8``: the projections in e4m3 with a scale per 128 x 128 block, quantised
     on ``device`` layer by layer.  A checkpoint's own fp8 projections are taken
-    as they are, with or without it; under ``tp`` they are cut as their bf16
-    values (``fp8`` then quantises the shards anew)."""
+    as they are, with or without it, and under ``tp`` with it (codes and scales
+    are cut); without it a shard holds their bf16 values."""
     cfg = cfg or config_from_hf(path)
     l0, l1 = layers or (0, cfg.layers)
     if not 0 <= l0 < l1 <= cfg.layers:
@@ -141,7 +141,7 @@ def load_llama(path: str, device, dtype=torch.bfloat16, layers: Optional[Tuple[i
 
     def fused(parts, fuse, block):
         """Weights fused by ``fuse(rows of each, rows per block)``; e4m3 ones with their scales."""
-        if tp_shards or not all(isinstance(t, Fp8Weight) for t in parts):
+        if tp_shards and not fp8 or not all(isinstance(t, Fp8Weight) for t in parts):
             return fuse([t.float().to(dtype) if isinstance(t, Fp8Weight) else t for t in parts], block)
         q = fuse([t.q.view(torch.uint8) for t in parts], block).view(torch.float8_e4m3fn)
         return Fp8Weight(q, fuse([t.scale for t in parts], max(1, block // ops.FP8_BLOCK)))
@@ -160,7 +160,7 @@ def load_llama(path: str, device, dtype=torch.bfloat16, layers: Optional[Tuple[i
     shard, tp_shards = None, tp is not None and tp[1] > 1
     if tp_shards:
         from connex_b200.parallel.tp import shard_layer, tp_config
-        shard = (lambda lw: shard_layer(lw, cfg, tp[0], tp[1]))
+        shard = (lambda lw: shard_layer(lw, cfg, tp[0], tp[1], codes=fp8))
     out_layers = []
     for i in range(l0, l1):
         p = f"model.layers.{i}."

@@ -61,24 +61,37 @@ def tp_config(cfg: LlamaConfig, world: int) -> LlamaConfig:
                           "ffn": cfg.ffn // world})
 
 
-def shard_layer(lw: LayerWeights, cfg: LlamaConfig, rank: int, world: int) -> LayerWeights:
-    if any(isinstance(t, Fp8Weight) for t in lw.__dict__.values()):
+def _cut(w, parts):
+    """``w`` cut by ``parts(tensor, unit)``, ``unit`` rows and columns to an
+    element of the tensor.  Of an Fp8Weight codes and scales are cut alike: the
+    edges of a shard lie between blocks of 128, for heads are 128 wide and the
+    FFN width is split in such blocks (:func:`tp_config`)."""
+    if not isinstance(w, Fp8Weight):
+        return parts(w, 1).contiguous()
+    codes = parts(w.q.view(torch.uint8), 1).contiguous().view(w.q.dtype)
+    return Fp8Weight(codes, parts(w.scale, ops.FP8_BLOCK).contiguous())
+
+
+def shard_layer(lw: LayerWeights, cfg: LlamaConfig, rank: int, world: int, codes: bool = False) -> LayerWeights:
+    """Rank ``rank``'s part of a layer.  ``codes``: projections in e4m3 keep
+    their codes and scales; otherwise they are refused."""
+    if not codes and any(isinstance(t, Fp8Weight) for t in lw.__dict__.values()):
         raise ValueError("layers are cut into shards as bf16; quantise the shards (LlamaWeights.to_fp8)")
-    hq, hkv = cfg.heads // world, cfg.kv_heads // world
-    q0 = cfg.heads * HEAD_DIM
-    qs = lw.wqkv[rank * hq * HEAD_DIM:(rank + 1) * hq * HEAD_DIM]
-    ks = lw.wqkv[q0 + rank * hkv * HEAD_DIM:q0 + (rank + 1) * hkv * HEAD_DIM]
-    v0 = q0 + cfg.kv_heads * HEAD_DIM
-    vs = lw.wqkv[v0 + rank * hkv * HEAD_DIM:v0 + (rank + 1) * hkv * HEAD_DIM]
-    f = cfg.ffn // world
-    gate, up = ops.deinterleave_gate_up(lw.w13)
+    hq, hkv, f = (n // world for n in (cfg.heads * HEAD_DIM, cfg.kv_heads * HEAD_DIM, cfg.ffn))
+
+    def mine(n, unit):
+        return slice(rank * n // unit, (rank + 1) * n // unit)
+
+    def qkv(w, u):
+        q, k, v = w.split([n // u for n in (world * hq, world * hkv, world * hkv)])
+        return torch.cat([q[mine(hq, u)], k[mine(hkv, u)], v[mine(hkv, u)]], 0)
+
+    def gate_up(w, u):
+        gate, up = ops.deinterleave_gate_up(w, ops.GATE_UP_TILE // u)
+        return ops.interleave_gate_up(gate[mine(f, u)], up[mine(f, u)], ops.GATE_UP_TILE // u)
     return LayerWeights(
-        attn_norm=lw.attn_norm,
-        wqkv=torch.cat([qs, ks, vs], 0).contiguous(),
-        wo=lw.wo[:, rank * hq * HEAD_DIM:(rank + 1) * hq * HEAD_DIM].contiguous(),
-        mlp_norm=lw.mlp_norm,
-        w13=ops.interleave_gate_up(gate[rank * f:(rank + 1) * f], up[rank * f:(rank + 1) * f]),
-        w2=lw.w2[:, rank * f:(rank + 1) * f].contiguous())
+        attn_norm=lw.attn_norm, wqkv=_cut(lw.wqkv, qkv), wo=_cut(lw.wo, lambda w, u: w[:, mine(hq, u)]),
+        mlp_norm=lw.mlp_norm, w13=_cut(lw.w13, gate_up), w2=_cut(lw.w2, lambda w, u: w[:, mine(f, u)]))
 
 
 def shard_llama(w: LlamaWeights, rank: int, world: int) -> LlamaWeights:

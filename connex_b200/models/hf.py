@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import glob
 import json
+import math
 import os
 from typing import Dict, Iterable, Optional, Tuple
 
@@ -101,6 +102,26 @@ class _Shards:
 
     def has(self, name: str) -> bool:
         return name in self.where
+
+    def fp8(self, name: str) -> bool:
+        return self.has(name) and self.where[name].get_slice(name).get_dtype() == "F8_E4M3"
+
+
+# the projections that are fused (and so loaded in one type) in a layer
+FUSED = tuple(tuple(f"{m}_proj.weight" for m in names) for names in (
+    ("self_attn.q", "self_attn.k", "self_attn.v"), ("self_attn.o",), ("mlp.gate", "mlp.up"), ("mlp.down",)))
+
+
+def fp8_elements(path: str, layers: Tuple[int, int]) -> int:
+    """How many elements of the layers' projections :func:`load_llama` leaves
+    in e4m3 because the checkpoint in ``path`` holds them so."""
+    sh, n = _Shards(path), 0
+    for i in range(*layers):
+        for names in FUSED:
+            names = [f"model.layers.{i}.{m}" for m in names]
+            if all(sh.fp8(m) for m in names):
+                n += sum(math.prod(sh.where[m].get_slice(m).get_shape()) for m in names)
+    return n
 
 
 def load_llama(path: str, device, dtype=torch.bfloat16, layers: Optional[Tuple[int, int]] = None,

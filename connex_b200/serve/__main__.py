@@ -90,8 +90,12 @@ def kv_blocks(a, cfg, l0: int, l1: int) -> int:
     free, _ = torch.cuda.mem_get_info(torch.device(a.device))
     n_layers = l1 - l0
     per_layer = cfg.qkv_dim * cfg.hidden + cfg.hidden * cfg.heads * cfg.head_dim + 3 * cfg.ffn * cfg.hidden
-    per_weight = 1 if getattr(a, "weight_dtype", "bf16") == "fp8" else 2
-    weights = per_weight * n_layers * per_layer + 2 * 2 * cfg.vocab_size * cfg.hidden
+    weights = 2 * (n_layers * per_layer + 2 * cfg.vocab_size * cfg.hidden)
+    if getattr(a, "weight_dtype", "bf16") == "fp8":
+        weights -= n_layers * per_layer
+    elif getattr(a, "checkpoint", None) and getattr(a, "tp", 1) == 1:
+        from connex_b200.models.hf import fp8_elements
+        weights -= fp8_elements(a.checkpoint, (l0, l1))
     scratch = 2 << 30                       # activations, workspaces, allocator slack
     room, bf16 = free - weights - scratch, cfg.block_size * cfg.head_dim * 2
     kind = getattr(a, "kv_dtype", "bf16")

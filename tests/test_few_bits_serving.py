@@ -1,5 +1,7 @@
-"""What serving makes of the operators in few bits, on the CPU: errors that their kernels record and shards of
-e4m3 projections."""
+"""What serving makes of the operators in few bits, on the CPU: errors that their kernels record, shards of e4m3
+projections, the room that they leave to the cache."""
+import argparse
+
 import pytest
 import torch
 
@@ -129,3 +131,26 @@ def test_shards_of_a_quantised_layer():
         a, b = shard_layer(lw, cfg, rank, 4, codes=True), shard_layer(plain, cfg, rank, 4)
         for name in ("wqkv", "wo", "w13", "w2"):
             assert torch.equal(getattr(a, name).float(), getattr(b, name))
+
+
+def test_room_beside_an_fp8_checkpoint(tmp_path, monkeypatch):
+    """The pool is sized by the bytes that the weights will take, whichever of them the checkpoint holds in e4m3."""
+    from connex_b200.serve.__main__ import kv_blocks, model_args
+    cfg = LlamaConfig.tiny(layers=2)
+    path, plain = _fp8_checkpoint(tmp_path, cfg, keep=lambda n: "layers.1.mlp.down" in n or "layers.0.self_attn.v" in n)
+    ap = argparse.ArgumentParser()
+    model_args(ap)
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a: ((2 << 30) + (64 << 20), 0))
+
+    def blocks(*a):
+        return kv_blocks(ap.parse_args(["--kv-fraction", "1.0", "--max-ctx", "64", *a]), cfg, 0, 2)
+    weights = hf.load_llama(path, "cpu")
+    freed = sum(t.q.numel() for lw in weights.layers for t in lw.__dict__.values() if isinstance(t, Fp8Weight))
+    assert 0 < freed == hf.fp8_elements(path, (0, 2)) < sum(x.numel() for x in plain.values())
+    assert hf.fp8_elements(str(tmp_path / "bf16"), (0, 2)) == 0
+    block = 2 * 2 * cfg.kv_heads * cfg.block_size * cfg.head_dim * 2
+    none = blocks("--checkpoint", str(tmp_path / "bf16"))
+    assert none == blocks() and abs(blocks("--checkpoint", path) - none - freed / block) <= 1
+    # the flag makes e4m3 of all of them; a tensor-parallel rank without it holds bf16
+    assert blocks("--checkpoint", path, "--weight-dtype", "fp8") > blocks("--checkpoint", path)
+    assert blocks("--checkpoint", path, "--tp", "2") == none

@@ -199,12 +199,12 @@ void kv_values_int4(const void* cache, void* out, int64_t rows, int sms, cudaStr
 //      out by itself, heads 2t and 2t + 1 of the lane's two tokens; scale and
 //      minimum are applied to it in fp32: x = sum_halves scale * S + minimum *
 //      sum(q).
-//   V: the weights, scale included (weight * scale, held in f16, 2^-11 of each, relative
-//      to a running maximum of their own), are turned round by movmatrix: the
+//   V: the weights, scale included (weight * scale, held in f16 relative to a running maximum of their own for each
+//      half: see TOP_W), are turned round by movmatrix: the
 //      lane then holds head g of tokens 2t, 2t + 1, 2t + 8, 2t + 9, of which it
 //      takes word g of a half (8 dims), two tokens side by side.  The minimum's
 //      part, sum of weight * minimum, is one fp32 number per half.
-// q is scaled by a power of two per head into f16's range.  Both running maxima
+// q is scaled by a power of two per head into f16's range.  The running maxima
 // move only once a weight has outgrown them by 2^8 and more, and the warp votes
 // on that: the steps in between have no shuffles and no rescaling.
 //
@@ -225,7 +225,12 @@ struct Cfg {
 constexpr int WARPS = Cfg::WARPS, THREADS = Cfg::THREADS, D = kv4::D, BS = kv4::BS, ROW = kv4::ROW;
 constexpr int ctas_per_sm(int nt) { return nt == 1 ? 4 : 3; }
 constexpr float LATE = 8.f;             // a logit may be this far above the running maximum: weights stay under 2^8
-constexpr uint32_t MOST_W = 0x70007000u;  // f16 pair of 2^13: beyond it the weights' own maximum moves
+// The products weight * scale of a half are held in f16, times a power of two that makes the largest so far 2^TOP_W at
+// least and lets it grow to MOST_W (a pair of 2^15) before it is chosen anew: each to 2^-11 of itself from 2^-22 of the
+// largest up, and to 2^-33 of the largest below.  The power is at most 2^START: a weight (2^LATE at most) times that is
+// finite.
+constexpr int TOP_W = 8, START = 119;
+constexpr uint32_t MOST_W = 0x78007800u;
 constexpr int BLOCK = BS * ROW;         // of one head
 constexpr int STAGE = 4 * BLOCK;        // K of two blocks, V of two blocks
 constexpr int STAGES = 2;
@@ -301,7 +306,7 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
   using namespace dec4;
   extern __shared__ __align__(16) uint8_t smem[];
   float* so = reinterpret_cast<float*>(smem);                           // [WARPS][8 NT][O_ROW], once the rings are drained
-  float* sm = reinterpret_cast<float*>(smem + Smem<NT>::STATS);         // [WARPS][8 NT][m, l, mv, -, z0, z1, -, -]
+  float* sm = reinterpret_cast<float*>(smem + Smem<NT>::STATS);         // [WARPS][8 NT][m, l, mv0, mv1, z0, z1, -, -]
   uint4* sq = reinterpret_cast<uint4*>(smem + Smem<NT>::Q);             // [NT][4 words][32 lanes]
   int* pre = reinterpret_cast<int*>(smem + Smem<NT>::PRE);              // [B + 1] units of the pairs before sequence b
   __shared__ uint32_t ticket;
@@ -418,9 +423,17 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
     }
     __syncthreads();
 
-    // of heads 8 nt + 2 qd + {0, 1}: the logits' factor, sums of q, running maximum m of the logits, sum l, sums z of
-    // weight * minimum, running maximum mv of the weights times scales, f = 2^(m - mv)
-    float o[NT][8][4], z[NT][2][2], m[NT][2], l[NT][2], mv[NT][2], f[NT][2], qf[NT][2], qs[NT][2][2];
+    // of heads 8 nt + 2 qd + {0, 1}: the logits' factor, sums of q, running maximum m of the logits, sum l; of their
+    // halves: sums z of weight * minimum, the power of two f of the weights times scales
+    float o[NT][8][4], z[NT][2][2], m[NT][2], l[NT][2], f[NT][2][2], qf[NT][2], qs[NT][2][2];
+    auto power = [&](int nt, int cc, int half) { return (int)(__float_as_uint(f[nt][cc][half]) >> 23) - 127; };
+    auto scale_o = [&](int nt, int cc, int half, float by) {
+#pragma unroll
+      for (int k = 4 * half; k < 4 * half + 4; ++k) {
+        o[nt][k][cc] *= by;
+        o[nt][k][2 + cc] *= by;
+      }
+    };
     bool far = false;                                          // q beyond 2^100: 2^24 is not folded into its factor
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -431,8 +444,9 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
         qs[nt][cc][0] = t.y;
         qs[nt][cc][1] = t.z;
         far |= fabsf(t.x) > 1e30f;
-        m[nt][cc] = mv[nt][cc] = -INFINITY;
-        f[nt][cc] = l[nt][cc] = z[nt][cc][0] = z[nt][cc][1] = 0.f;
+        m[nt][cc] = -INFINITY;
+        f[nt][cc][0] = f[nt][cc][1] = exp2_int(START);
+        l[nt][cc] = z[nt][cc][0] = z[nt][cc][1] = 0.f;
       }
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt)
@@ -556,8 +570,15 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
             l[nt][cc] *= keep;
             z[nt][cc][0] *= keep;
             z[nt][cc][1] *= keep;
+            // O counts in 2^(m - power): the products so far are smaller next to the new maximum, and so the power may rise
+            const float rise = fminf(base - m[nt][cc], 1000.f);           // 1000: from no maximum at all
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int p = power(nt, cc, half), up = min((int)ceilf(rise), START - p);
+              f[nt][cc][half] = exp2_int(p + up);
+              scale_o(nt, cc, half, ex2((float)up - rise));
+            }
             m[nt][cc] = now;
-            f[nt][cc] = mv[nt][cc] == -INFINITY ? 0.f : ex2(fminf(base - mv[nt][cc], 126.f));
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (y[nt][e >> 1][e & 1][cc] != -INFINITY)       // (the product is rounded in `now` and not here)
@@ -566,7 +587,10 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
       }
       uint32_t wb[NT][2][2][2];                                // [half][block][token]: heads 2 qd, 2 qd + 1
       uint32_t big = 0;
-      bool fresh = false;
+      auto weights = [&](int nt, int half, int e) {
+        const float s = vs[half][e >> 1][e & 1];
+        return pack_f16x2(y[nt][e >> 1][e & 1][0] * f[nt][0][half] * s, y[nt][e >> 1][e & 1][1] * f[nt][1][half] * s);
+      };
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -578,47 +602,33 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
           for (int half = 0; half < 2; ++half)
 #pragma unroll
             for (int e = 0; e < 4; ++e) z[nt][cc][half] = fmaf(y[nt][e >> 1][e & 1][cc], vm[half][e >> 1][e & 1], z[nt][cc][half]);
-          fresh |= f[nt][cc] == 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float w0 = y[nt][e >> 1][e & 1][0] * f[nt][0], w1 = y[nt][e >> 1][e & 1][1] * f[nt][1];
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            wb[nt][half][e >> 1][e & 1] = pack_f16x2(w0 * vs[half][e >> 1][e & 1], w1 * vs[half][e >> 1][e & 1]);
+            wb[nt][half][e >> 1][e & 1] = weights(nt, half, e);
             big = max_f16x2(big, wb[nt][half][e >> 1][e & 1]);
           }
-        }
       }
-      if (__any_sync(0xffffffffu, fresh || any_above_f16x2(big, MOST_W))) {     // mv moves
+      if (__any_sync(0xffffffffu, any_above_f16x2(big, MOST_W))) {              // the powers sink
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int cc = 0; cc < 2; ++cc) {
-            float most = 0.f;
+          for (int half = 0; half < 2; ++half) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              most = fmaxf(most, y[nt][e >> 1][e & 1][cc] * fmaxf(vs[0][e >> 1][e & 1], vs[1][e >> 1][e & 1]));
-            const float base = m[nt][cc] == -INFINITY ? 0.f : m[nt][cc];
-            const float mt = base + lg2(tokens_max(most));
-            if (mt > mv[nt][cc]) {
-              const float keep = ex2(mv[nt][cc] - mt);
-              mv[nt][cc] = mt;
-              f[nt][cc] = ex2(fminf(base - mt, 126.f));
+            for (int cc = 0; cc < 2; ++cc) {
+              float most = 0.f;                                // (2^-16 of it: the product may be beyond fp32)
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                o[nt][k][cc] *= keep;
-                o[nt][k][2 + cc] *= keep;
-              }
+              for (int e = 0; e < 4; ++e)
+                most = fmaxf(most, y[nt][e >> 1][e & 1][cc] * (vs[half][e >> 1][e & 1] * 1.52587890625e-5f));
+              const int p = power(nt, cc, half), to = min(p, (int)ceilf(TOP_W - 16.f - lg2(fmaxf(tokens_max(most), 1e-37f))));
+              f[nt][cc][half] = exp2_int(to);
+              scale_o(nt, cc, half, ex2((float)(to - p)));
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) wb[nt][half][e >> 1][e & 1] = weights(nt, half, e);
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-              wb[nt][half][e >> 1][e & 1] = pack_f16x2(y[nt][e >> 1][e & 1][0] * f[nt][0] * vs[half][e >> 1][e & 1],
-                                                       y[nt][e >> 1][e & 1][1] * f[nt][1] * vs[half][e >> 1][e & 1]);
-        }
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -660,7 +670,7 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
           l[nt][cc] = __uint_as_float(0x7fffffffu);
-          m[nt][cc] = mv[nt][cc] = -INFINITY;
+          m[nt][cc] = -INFINITY;
         }
 
     // ---- the warps' results of this run
@@ -671,7 +681,7 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
         const float ls = tokens_sum(l[nt][cc]), z0 = tokens_sum(z[nt][cc][0]), z1 = tokens_sum(z[nt][cc][1]);
         if (gq == 0) {
           float4* st = reinterpret_cast<float4*>(sm + (warp * 8 * NT + nt * 8 + 2 * qd + cc) * 8);
-          st[0] = make_float4(m[nt][cc], ls, mv[nt][cc], 0.f);
+          st[0] = make_float4(m[nt][cc], ls, m[nt][cc] - power(nt, cc, 0), m[nt][cc] - power(nt, cc, 1));
           st[1] = make_float4(z0, z1, 0.f, 0.f);
         }
       }
@@ -693,20 +703,21 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
     // two heads at a time, a thread for two dims of one
     for (int hh = tid >> 6; hh < G; hh += 2) {
       const int d8 = tid & 7, d2 = tid >> 3 & 7, half = d2 >> 2, dim = half * 64 + 8 * d8 + 2 * (d2 & 3);
-      float M = -INFINITY, MV = -INFINITY;
+      float M = -INFINITY, MV0 = -INFINITY, MV1 = -INFINITY;   // (the units are infinite where the maximum is)
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
         M = fmaxf(M, sm[(w * 8 * NT + hh) * 8]);
-        MV = fmaxf(MV, sm[(w * 8 * NT + hh) * 8 + 2]);
+        MV0 = fmaxf(MV0, sm[(w * 8 * NT + hh) * 8 + 2]);
+        MV1 = fmaxf(MV1, sm[(w * 8 * NT + hh) * 8 + 3]);
       }
-      const float mb = M == -INFINITY ? 0.f : M, vb = MV == -INFINITY ? 0.f : MV;
+      const float mb = M == -INFINITY ? 0.f : M, vb = M == -INFINITY ? 0.f : half ? MV1 : MV0;
       float2 num = make_float2(0.f, 0.f), zz = make_float2(0.f, 0.f);
       float den = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
         const float* p = so + (w * 8 * NT + hh) * O_ROW + 16 * d2 + d8;
         const float* st = sm + (w * 8 * NT + hh) * 8;
-        const float f = ex2(st[2] - vb), fm = ex2(st[0] - mb);
+        const float f = ex2(st[2 + half] - vb), fm = ex2(st[0] - mb);
         num.x += p[0] * f;
         num.y += p[8] * f;
         den += st[1] * fm;
@@ -721,7 +732,7 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
         float* p = part + ((size_t)(blockIdx.x * 2 + ((int)blockIdx.x == c0)) * G + hh) * DEC4_ROW;
         *reinterpret_cast<float2*>(p + dim) = num;
         if ((tid & 63) == 0) {
-          *reinterpret_cast<float4*>(p + D) = make_float4(M, den, MV, 0.f);
+          *reinterpret_cast<float4*>(p + D) = make_float4(M, den, MV0, MV1);
           *reinterpret_cast<float4*>(p + D + 4) = make_float4(zz.x, zz.y, 0.f, 0.f);
         }
       }
@@ -738,28 +749,40 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
           auto slot = [&](int cc) {
             return part + ((size_t)(cc * 2 + (cc == c0)) * G + hh) * DEC4_ROW;
           };
-          float m_all = -INFINITY, mv_all = -INFINITY, den = 0.f, z0 = 0.f, z1 = 0.f;
+          const int of = lane & 16, at = lane & 15;            // a half-warp for each half of the dims
+          float m_all = -INFINITY, mv_all = -INFINITY, den = 0.f, zh = 0.f;
           float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int cb = c0; cb <= c1; cb += 32) {              // 32 CTAs at a time, rescaled as the maxima grow
-            const int n = min(32, c1 - cb + 1);
-            float4 st = make_float4(-INFINITY, 0.f, -INFINITY, 0.f), zs = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (lane < n) {
-              st = __ldcg(reinterpret_cast<const float4*>(slot(cb + lane) + D));
-              zs = __ldcg(reinterpret_cast<const float4*>(slot(cb + lane) + D + 4));
+          auto largest = [](float a) {
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+            return a;
+          };
+          auto total = [](float a) {
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+            return a;
+          };
+          for (int cb = c0; cb <= c1; cb += 16) {              // 16 CTAs at a time, rescaled as the maxima grow
+            const int n = min(16, c1 - cb + 1);
+            float4 st = make_float4(-INFINITY, 0.f, -INFINITY, -INFINITY);
+            float2 zs = make_float2(0.f, 0.f);
+            if (at < n) {
+              st = __ldcg(reinterpret_cast<const float4*>(slot(cb + at) + D));
+              zs = __ldcg(reinterpret_cast<const float2*>(slot(cb + at) + D + 4));
             }
-            const float m_new = fmaxf(m_all, warp_max(st.x)), mv_new = fmaxf(mv_all, warp_max(st.z));
-            const float mb = m_new == -INFINITY ? 0.f : m_new, vb = mv_new == -INFINITY ? 0.f : mv_new;
+            const float mv = of ? st.w : st.z;
+            const float m_new = fmaxf(m_all, largest(st.x)), mb = m_new == -INFINITY ? 0.f : m_new;
+            const float mv_new = fmaxf(mv_all, largest(mv)), vb = m_new == -INFINITY ? 0.f : mv_new;
             const float fv = ex2(mv_all - vb), fm = ex2(m_all - mb), mine = ex2(st.x - mb);
             den = den * fm + st.y * mine;
-            z0 = z0 * fm + zs.x * mine;
-            z1 = z1 * fm + zs.y * mine;
+            zh = zh * fm + (of ? zs.y : zs.x) * mine;
             num.x *= fv;
             num.y *= fv;
             num.z *= fv;
             num.w *= fv;
             m_all = m_new;
             mv_all = mv_new;
-            const float f = ex2(st.z - vb);
+            const float f = ex2(mv - vb);
             for (int i = 0; i < n; i += 8) {
               float4 y[8];
 #pragma unroll
@@ -768,7 +791,7 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
                                  : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
-                const float g = __shfl_sync(0xffffffffu, f, (i + k) & 31);
+                const float g = __shfl_sync(0xffffffffu, f, of + (i + k & 15));
                 if (i + k < n) {
                   num.x += y[k].x * g;
                   num.y += y[k].y * g;
@@ -778,11 +801,10 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
               }
             }
           }
-          const float mb = m_all == -INFINITY ? 0.f : m_all, vb = mv_all == -INFINITY ? 0.f : mv_all;
-          den = warp_sum(den);
-          z0 = warp_sum(z0);
-          z1 = warp_sum(z1);
-          const float inv = den == 0.f ? 0.f : 1.f / den, f = ex2(vb - mb), zh = lane < 16 ? z0 : z1;
+          const float mb = m_all == -INFINITY ? 0.f : m_all, vb = m_all == -INFINITY ? 0.f : mv_all;
+          den = total(den);
+          zh = total(zh);
+          const float inv = den == 0.f ? 0.f : 1.f / den, f = ex2(vb - mb);
           uint2 w;
           w.x = pack_bf16x2(fmaf(num.x, f, zh) * inv, fmaf(num.y, f, zh) * inv);
           w.y = pack_bf16x2(fmaf(num.z, f, zh) * inv, fmaf(num.w, f, zh) * inv);

@@ -531,7 +531,8 @@ def decode_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     :func:`rope_cache_int4`), up to 16 query heads per KV head.  ``q``
     [B, >= Hq * 128] (q heads first), ``ctx_lens`` [B] tokens to attend to (0: a
     row of zeros), ``block_tables`` [B, max_blocks].  The weights, V's scales
-    in them, are held in f16 (2^-11 of each) next to fp32 sums.  The work is
+    in them, are held in f16 next to fp32 sums: to 2^-11 of each, and to 2^-33 of
+    the largest of a query head and a half.  The work is
     divided on the device from ``ctx_lens``, so a captured call stays balanced
     for any lengths.  A block id out of range is left out, and a length beyond
     the table cut, both recorded in ``status``; so is a copy that did not arrive

@@ -259,6 +259,8 @@ def _make_runtime(cfg, l0, l1, device, num_blocks, max_batch, max_ctx, max_step_
     checkpoint holds them so."""
     from connex_b200.runtime.pp import StageRuntime, stage_weights
     weights, rcfg, kv = None, cfg, torch_kv_dtype(kv_dtype)
+    if weight_dtype not in ("bf16", "fp8"):
+        raise ValueError(f"weight type {weight_dtype!r}: bf16 or fp8")
     if checkpoint:
         from connex_b200.models.hf import load_llama
         weights = load_llama(checkpoint, device, layers=(l0, l1), cfg=cfg,

@@ -154,3 +154,13 @@ def test_room_beside_an_fp8_checkpoint(tmp_path, monkeypatch):
     # the flag makes e4m3 of all of them; a tensor-parallel rank without it holds bf16
     assert blocks("--checkpoint", path, "--weight-dtype", "fp8") > blocks("--checkpoint", path)
     assert blocks("--checkpoint", path, "--tp", "2") == none
+
+
+def test_unknown_types_are_refused():
+    """A type that is none is an error, and not bf16."""
+    from connex_b200.serve.engine import _make_runtime
+    args = (LlamaConfig.tiny(), 0, 1, "cpu", 8, 2, 64, 64, None, 0, None)
+    for kv, weight, match in (("int4", "e4m3", "weight type 'e4m3'"), ("bf16", "fp4", "weight type 'fp4'"),
+                              ("int8", "bf16", "KV cache type")):
+        with pytest.raises(ValueError, match=match):
+            _make_runtime(*args, kv, weight)

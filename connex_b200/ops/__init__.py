@@ -165,8 +165,10 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
 
     ``a_scale`` fp32 [M, ceil(K / 128)] (:func:`quantize_fp8`), ``b_scale``
     fp32 [ceil(N / 128), ceil(K / 128)] (:func:`quantize_weight_fp8`, or a
-    checkpoint's), any strides; both scales are arbitrary numbers.  Sums are
-    fp32, the scales are applied to the sum of each block of 128 columns.  K
+    checkpoint's), any strides; both scales are arbitrary numbers, but for
+    their product, which is formed in fp32 and should be a normal number there (a
+    smaller one counts as what it rounds to).  Sums are fp32, the scales are
+    applied to the sum of each block of 128 columns.  K
     must be a multiple of 16 and N of 8.  Operands that do not arrive in time
     are recorded in ``status``, and what they belong to reads as NaN.
 

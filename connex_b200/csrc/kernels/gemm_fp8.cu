@@ -750,7 +750,8 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
     uint32_t stage = 0, phase = 0;
     int loads = 0;
     for (int kb = k0; kb < k1; kb += KS) {
-      ok = mbar_wait_poll(&empty[stage], phase ^ 1, lost);
+      // (no wait for what is empty at first, nor for the accumulators below: 1 x 6144 x 4096 8.7 us, 8.95 with them)
+      ok = loads < STAGES || mbar_wait_poll(&empty[stage], phase ^ 1, lost);
       if (!ok) break;
       ++loads;
       if (elect_sync()) {
@@ -777,7 +778,8 @@ __global__ void __launch_bounds__(g8s::Cfg<NT, R>::THREADS, g8s::Cfg<NT, R>::PER
     const uint32_t w_lo = umma_desc_sw128_lo(smem_u32(smem));
     uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
     for (int kb = k0; kb < k1 && ok; kb += KS) {
-      ok = mbar_wait_poll(&tempty[acc], acc_phase ^ 1, lost) && mbar_wait_poll(&full[stage], phase, lost);
+      ok = (kb - k0 < C::ACCS * KS || mbar_wait_poll(&tempty[acc], acc_phase ^ 1, lost)) &&
+           mbar_wait_poll(&full[stage], phase, lost);
       if (!ok) break;
       tc_fence_after();
       if (elect_sync()) {

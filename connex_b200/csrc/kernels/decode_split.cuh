@@ -1,5 +1,6 @@
-// How decode attention over a quantised cache is divided among CTAs, on the
-// device, from the sequences' lengths.
+// How decode attention over the 4-bit cache is divided among CTAs, on the
+// device, from the sequences' lengths.  (The kernel over the 8-bit cache holds
+// the same division itself: what is mended here has to be mended there.)
 //
 // A pair is a (sequence, KV head).  The blocks of all pairs, laid end to end
 // with PAIR_COST blocks' worth for the fixed cost of a pair, are cut into equal

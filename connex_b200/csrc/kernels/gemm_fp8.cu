@@ -57,8 +57,9 @@ __device__ __forceinline__ void unpack8(const u128& r, float (&v)[8]) {
 }
 
 // A half-warp per block, eight columns of a lane; a CTA takes 2^lc column blocks of 16 / 2^lc rows at a time, four such
-// groups of rows in flight.  (With a running block number, divided by the row's blocks in 64 bits, 8192 x 4096 took 35
-// us.)
+// groups of rows in flight.  8192 x 4096 take 22.2 us, 0.72 of a copy's rate.  The grid is at most 1184 CTAs; at 46
+// registers an SM holds five of them, 740 on 148, so that many rows run as 1.6 rounds of CTAs: that, and not DRAM, is
+// what is left there.  (With a running block number, divided by the row's blocks in 64 bits, 35 us.)
 __global__ void __launch_bounds__(q8::THREADS)
     quantize_fp8_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq,
                         Fp8Scales s, int T, int K, int lc) {
@@ -106,9 +107,9 @@ __global__ void __launch_bounds__(q8::THREADS)
 }
 
 // The same behind an RMS norm: a CTA per row, the row in registers (read once, where the norm's sum needs all of it
-// before the first code).  64 x 4096 take 2.2 us, a launch and a row's read, sum and write; 8192 x 4096 28 us, 3.7 TB/s:
-// a row's barrier stands between its reads and its writes.  (Weights read behind the barrier, infinities looked for in
-// every element: 2.5 and 30.7.)
+// before the first code).  64 x 4096 take 2.2 us, a launch and a row's read, sum and write; 8192 x 4096 28 to 30 us, 3.5
+// TB/s: a row's barrier stands between its reads and its writes, and nothing of a CTA's next row is under way there.
+// (Weights read behind the barrier, infinities looked for in every element: 2.5 and 2.7 more than 28.)
 template <int VPT>
 __global__ void __launch_bounds__(q8::THREADS)
     quantize_norm_fp8_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ w,
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(q8::THREADS)
   }
 }
 
-// A CTA per 128 x 128 block of a weight.
+// A CTA per 128 x 128 block of a weight: 28672 x 4096 take 76 us, 4.6 TB/s (once, as weights are loaded).
 __global__ void __launch_bounds__(q8::THREADS)
     quantize_weight_fp8_kernel(const __nv_bfloat16* __restrict__ w, int64_t ldw, uint8_t* __restrict__ q, int64_t ldq,
                                Fp8Scales s, int N, int K) {
@@ -263,13 +264,16 @@ void quantize_weight_fp8(const void* w, int64_t ldw, void* q, int64_t ldq, const
 //   warps 4-11  promotion: two warpgroups; a thread takes a row, and columns [64 g, 64 g + 64) of both halves of
 //               the tile, reads the block's sums from TMEM, multiplies by the scales and adds in registers.  One
 //               accumulator is read while the MMAs fill the other.
-// What bounds it is the way round: an accumulator's MMAs (513 cycles), the word that it is complete (some 260), its
-// promotion by two warps on each SM quarter (350 to 600), the word that it is free (90).  Two accumulators of 256
-// columns are all of TMEM, so a block takes 700 cycles at least (an SM by itself, operands in place), 1000 here.
-// Measured on 8192 x 28672 x 4096 with SiLU(gate) * up, as variants of this kernel: pairs of CTAs on one tile of 256 x
-// 256 (cta_group::2) 1060 us, their way round being longer by two signals between SMs; four warpgroups of half the
-// columns 1190; four accumulators of 128 columns 1280 (the issuing thread falls behind); barriers waited for in
-// mbarrier.try_wait, which suspends, where single threads poll here, 1150.
+// 8192 x 28672 x 4096 with SiLU(gate) * up takes 965 us at full clock (up to 1130 after seconds of load), 6144 columns
+// without it 224; the MMAs are half of the time (513 of 1040 cycles of a block, outputs included).  The other half is
+// owned in part: the way round of an accumulator is its MMAs, the word that it is complete (some 260), its promotion by
+// two warps on each SM quarter (350 to 600), the word that it is free (90), and two accumulators of 256 columns are all
+// of TMEM, so a block takes 700 cycles at least (an SM by itself, operands in place).  What takes the rest is not known;
+// a block's operands are 48 KB, 47 bytes a cycle, about what comes to an SM in the kernel for few rows, too.
+// Variants, timed when the waits had their clocks in each lane and an MMA took 75 cycles to issue, this form then 1020
+// us: pairs of CTAs on one tile of 256 x 256 (cta_group::2) 1060; four warpgroups of half the columns 1190; four
+// accumulators of 128 columns 1280; barriers waited for in mbarrier.try_wait, which suspends, 1150.  They have not been
+// timed since.
 // A warpgroup holds gate and up of the same outputs, so SiLU(gate) * up needs no exchange; a row's largest value
 // over the tile's 128 outputs, for quantised output, passes through shared memory.
 namespace g8 {
@@ -632,10 +636,10 @@ static void launch_gemm_fp8(const GemmFp8& g, int sms, int* status, cudaStream_t
 // bits from run to run.  A warp writes a row of 128 outputs.  SiLU-mul takes R = 2 blocks of weight rows, gate and up.
 // What bounds it: a block of 128 columns takes a CTA 500 to 700 cycles, as long with two warpgroups that add up the
 // blocks in turn or with half the waits of the issuing thread: 40 to 50 bytes a cycle come to an SM.  5 to 6 us pass
-// around that (launch, first loads, the cluster's sums): 64 x 4096 x 14336 takes 17.4 us where reading the operands
-// takes 9.4, one row 14.8.  With activations as columns a thread needs another scale for each of its sums, and shared
+// around that (launch, first loads, the cluster's sums).  Times are with other weights each call, none of them in the L2:
+// 64 x 4096 x 14336 takes 16.8 us where reading the operands takes 9.4.  With activations as columns a thread needs another scale for each of its sums, and shared
 // memory brings 32 of them a cycle: 1024 cycles for 256 activations.  So 128 of them are rows, a scale a thread: 613 x
-// 2048 x 4096 takes 18.2 us (256 activations as columns 26.2), 512 x 4096 x 14336 48 (63).
+// 2048 x 4096 takes 18.2 us (256 activations as columns 26.2), 512 x 4096 x 14336 47.3 (63).
 namespace g8s {
 constexpr int BK = 128, Q = 128;
 constexpr int SC_SLOTS = 2;
@@ -1040,10 +1044,10 @@ static void launch_gemm_fp8_split(const GemmFp8& g, int splits, int* status, cud
 // Which way a call goes: the least of the estimated times, in us.  A CTA takes `per` for a block of 128 columns and a
 // fixed start and end; clusters of four and eight do not fill every SM (132 and 120 of 148 are reached); reading the
 // operands takes its time whatever the CTAs.  The constants are fits to measured calls: 4096 weight rows with K = 4096
-// and 14336, one CTA per tile, and for the tiles of 128 x 256.  Estimated and measured: 1 x 6144 x 4096 8.3 and 9.5 (16
-// activations, four CTAs; one CTA 12.6, 128 x 256 tiles 21), 64 x 4096 x 14336 15.6 and 17.4 (64, four; 65), 613 x 2048
-// x 4096 17.8 and 18.2 (128, one; 29), 64 x 28672 x 4096 with SiLU-mul 25.6 and 26.0 (128 x 256 tiles; 64 activations
-// by one CTA 28), 512 x 4096 x 14336 48 and 48 (128, one; 71).
+// and 14336, one CTA per tile, and for the tiles of 128 x 256.  Estimated and measured (other weights each call): 1 x 6144 x
+// 4096 8.3 and 8.7 (16 activations, four CTAs; one CTA 12.6, 128 x 256 tiles 21), 64 x 4096 x 14336 15.6 and 16.8 (64,
+// four; 65), 613 x 2048 x 4096 17.8 and 18.2 (128, one; 29), 64 x 28672 x 4096 with SiLU-mul 25.6 and 25.1 (128 x 256
+// tiles; 64 activations by one CTA 28), 512 x 4096 x 14336 48 and 47.3 (128, one; 71).
 GemmFp8Plan gemm_fp8_plan(int M, int N, int K, int epi, int sms) {
   const int r = epi == EPI_SILU_MUL ? 2 : 1, nk = (K + 127) / 128;
   const double read = ((double)M + N) * K / 5.5e6 + 4.0;

@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(dec8::THREADS, dec8::ctas_per_sm(NT))
   const int Hkv = c.Hkv, G = Hq / Hkv;
 
   auto len_of = [&](int b) { return min(max(ctx_lens[b], 0), max_blocks * BS); };
-  // ---- prefix sums of the pairs' units
+  // ---- prefix sums of the pairs' units (the division of decode_split.cuh)
   if (tid == 0) pre[0] = 0;
   int run = 0, top = 0;                                         // all units; the longest sequence's
   for (int b0 = 0; b0 < B; b0 += THREADS) {

@@ -165,7 +165,8 @@ void rope_cache_int4(const void* qkv, int ldq, const int* pos, const float* cos_
 }
 
 // ------------------------------------------------------------------- values
-// Eight dims of a lane: one word of codes, 16 bytes out.  Bytes bound it, nearly all of them written.
+// Eight dims of a lane: one word of codes, 16 bytes out.  Bytes bound it, nearly all of them written: 4096 blocks of 8
+// heads take 32.6 us, 5.3 TB/s.
 __global__ void __launch_bounds__(kv4::THREADS)
     kv_values_int4_kernel(const uint8_t* __restrict__ cache, __nv_bfloat16* __restrict__ out, int64_t words) {
   using namespace kv4;
@@ -211,12 +212,14 @@ void kv_values_int4(const void* cache, void* out, int64_t rows, int sms, cudaStr
 // Loads: a block of a head is 1152 contiguous bytes, one asynchronous bulk copy.
 // A warp has K and V of two blocks in each of two stages, one read while the
 // other is under way, without barriers between warps.
-// What bounds it: 64 x 4096 tokens of 32/8 heads take 75 us, 303 MB at 4.0 TB/s
-// or 0.63 of a copy's rate.  41 million warp instructions keep the schedulers
-// 55 % busy with 14 warps on an SM (128 registers each), the integer pipe as
-// much, tensor cores 22 %: the masks and shifts that take the codes apart, in
-// chains that four warps of a scheduler do not hide.  Tokens as columns of the
-// first product, with a shuffle per maximum, took 99 us.
+// What bounds it: 64 x 4096 tokens of 32/8 heads take 74.6 us, 302 MB at 4.05
+// TB/s or 0.63 of a copy's rate.  42.6 million warp instructions keep the
+// schedulers 57 % busy with 14 warps on an SM (128 registers each), the integer
+// pipe 56 %, tensor cores 22 %: the masks and shifts that take the codes apart,
+// in chains that four warps of a scheduler do not hide.  Tokens as columns of
+// the first product, with a shuffle per maximum, took 99 us.  16 query heads of
+// one KV head take 29.0 us for 64 x 4096, of four 69.3 (2.2 TB/s: twice the
+// products for the bytes, three CTAs on an SM).
 namespace dec4 {
 struct Cfg {
   static constexpr int WARPS = 4, THREADS = 32 * WARPS, BS = kv4::BS;

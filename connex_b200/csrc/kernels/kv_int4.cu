@@ -625,7 +625,8 @@ __global__ void __launch_bounds__(dec4::THREADS, dec4::ctas_per_sm(NT))
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 most = fmaxf(most, y[nt][e >> 1][e & 1][cc] * (vs[half][e >> 1][e & 1] * 1.52587890625e-5f));
-              const int p = power(nt, cc, half), to = min(p, (int)ceilf(TOP_W - 16.f - lg2(fmaxf(tokens_max(most), 1e-37f))));
+              const float room = TOP_W - 16.f - lg2(fmaxf(tokens_max(most), 1e-37f));
+              const int p = power(nt, cc, half), to = min(p, (int)fmaxf(ceilf(room), -126.f));
               f[nt][cc][half] = exp2_int(to);
               scale_o(nt, cc, half, ex2((float)(to - p)));
             }

@@ -132,3 +132,39 @@ def test_logits_far_from_zero(dev, logit, step, constant):
                                     ops.decode_workspace_int4(1, hq, hkv, dev))
     _check(out, q, k, v, table, [n], hkv)
     assert ((out.view(hq, D)[:, :64].float() + 2.5).abs() <= 2.5 * U_BF16).all()
+
+
+@pytest.mark.parametrize("bits", [0x7F80, 0x7F7F, 0x7F00])
+@pytest.mark.parametrize("step", [0.0, 5.0])
+def test_scales_that_no_write_leaves(dev, bits, step):
+    """An infinite scale of V, the largest number and 2^127 in one half of one token: that half of its heads is not finite
+    or the sum of what fp32 holds, everything else as without it."""
+    from connex_b200 import ops
+    hq, hkv, n = 8, 2, 300
+    kr = torch.zeros(n, hkv, D, device=dev)
+    kr[..., 0] = step * (torch.arange(n, device=dev) // 32)[:, None]
+    k, table = _paged([kr.to(torch.bfloat16)], dev, 9)
+    v, _ = _paged([torch.randn(n, hkv, D, generator=_g(dev, 10), device=dev).to(torch.bfloat16)], dev, 9)
+    q = torch.zeros(1, hq, D, dtype=torch.bfloat16, device=dev)
+    q[..., 0] = math.sqrt(D)
+    lens = torch.tensor([n], dtype=torch.int32, device=dev)
+
+    def call():
+        return ops.decode_attention_int4(q.view(1, -1), k, v, table, lens, hq,
+                                         ops.decode_workspace_int4(1, hq, hkv, dev)).view(hq, D)
+    want = call()
+    at = v[int(table[0, 250 // BS]), 1, 250 % BS]
+    at[68], at[69] = bits & 0xFF, bits >> 8                      # the second half's scale of KV head 1
+    at[32:64] = 0xF1                                             # codes 1 and 15
+    got = call()
+    assert torch.equal(got[:4], want[:4]) and torch.equal(got[4:, :64], want[4:, :64])
+    # codes of 15 leave fp32's range; those of 1 hold weight * 2^127 where that is the scale
+    from connex_b200.ops import reference as R
+    logits = R.int4_values(k[table[0].long(), 1]).view(-1, D)[:n, 0]       # of the keys as they are cached: 15 * bf16(x / 15)
+    weight = torch.softmax(logits, 0)[250]
+    assert not torch.isfinite(got[4:, 65::2]).any() or weight * 15 * 2.0 ** 127 < 3e38
+    if bits == 0x7F00:
+        high = got[4:, 64::2].double()
+        assert (torch.isnan(high) | ((high - weight * 2.0 ** 127).abs() <= 2.0 ** -6 * weight * 2.0 ** 127)).all()
+    else:
+        assert bits != 0x7F80 or not torch.isfinite(got[4:, 64:]).any()
